@@ -208,8 +208,9 @@ def _plain_checkpoint(s):
     blocks = _blocks(x32)
     most, exponent = torch.frexp(blocks.abs().amax(dim=2, keepdim=True))   # most in [0.5, 1): 448 = 0.875 * 2^9
     exponent = (exponent - 9 + (most > E4M3_MAX / 512).to(exponent.dtype)).clamp(min=-126)
-    held = torch.ldexp(blocks, -exponent).to(torch.float8_e4m3fn)
-    kept = torch.ldexp(held.float(), exponent).reshape(x.shape[0], -1)[:, :x.shape[1]]
+    power = ((exponent + 127) << 23).view(torch.float32)    # 2^exponent, exactly
+    held = (blocks / power).to(torch.float8_e4m3fn)
+    kept = (held.float() * power).reshape(x.shape[0], -1)[:, :x.shape[1]]
     return {"y": y.to(x.dtype), "grad": (g.float() * _plain_act_grad(kept, case["act"])).to(x.dtype),
             "mid": _plain_act(kept, case["act"]).to(x.dtype)}
 
