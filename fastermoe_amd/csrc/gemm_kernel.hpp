@@ -2,6 +2,7 @@
 // gemm_inst.hip (one translation unit per element type and product, so that the
 // variants build in parallel) and by grouped_gemm.hip (host dispatch).
 #pragma once
+#include "gelu_terms.hpp"
 #include "grouped_gemm.hpp"
 #include "profile.hpp"
 
@@ -149,23 +150,6 @@ __device__ __forceinline__ void mma_part(int product, f32x16 &acc, const Split8 
     const u32x4 a = product == 0 ? p.lo : product == 2 || product == 3 ? p.mid : p.hi;
     const u32x4 b = product == 1 ? q.lo : product == 2 || product == 4 ? q.mid : q.hi;
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-}
-
-// erf by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7): a reciprocal, an exponential and
-// five multiply-adds instead of the library routine's branches.  The same exponential,
-// exp(-x^2/2), is the Gaussian of GELU's derivative.
-struct GeluTerms {
-    float cdf;  // Phi(x) = 0.5 (1 + erf(x / sqrt 2))
-    float pdf;  // phi(x) = exp(-x^2 / 2) / sqrt(2 pi)
-};
-__device__ __forceinline__ GeluTerms gelu_terms(float x) {
-    const float z = fabsf(x) * 0.70710678118654752440f;
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * z);
-    const float e = __expf(-z * z);
-    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float erf_abs = 1.f - poly * e;
-    const float half_erf = 0.5f * (x < 0.f ? -erf_abs : erf_abs);
-    return GeluTerms{0.5f + half_erf, 0.39894228040143267794f * e};
 }
 
 // Phi(x) - 1/2 for results that are rounded to 16 bits: an odd polynomial of degree 17 in x

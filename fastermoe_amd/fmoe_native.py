@@ -794,6 +794,227 @@ def linear_wgrad_dev(grad_y, x, weight, table, rows_cap, with_bias):
     return grad_w, grad_b
 
 
+# ---- activations kept in 8 bits -------------------------------------------------------
+
+SCALE_ELEMS = 32   # elements along a row that share a scale
+
+
+def _activation_of(activation):
+    if activation not in (_lib.ACT_NONE, _lib.ACT_RELU, _lib.ACT_GELU):
+        raise ValueError(f"unknown activation code {activation}")
+    return activation
+
+
+def _live_rows(table, rows, device):
+    """A segment table whose counts say how many of ``rows`` rows there are, or ``None``."""
+    if table is not None:
+        _near("segment_table", _dev("segment_table", table, torch.int32), device)
+        if table.numel() < 8:
+            raise ValueError("segment_table is no segment table")
+    return _ptr(table)
+
+
+def act_checkpoint_supported(dtype):
+    """Whether rows of this type are kept in 8 bits."""
+    return dtype in (torch.float32, torch.bfloat16, torch.float16)
+
+
+def act_checkpoint_forward(x, activation, with_act=True, table=None):
+    """``(act(x) or None, held, scale)``: ``x [rows, features]`` in 8 bits (``held``, ``float8_e4m3fn``), 32 elements along a row under
+    one power of two (``scale [rows, ceil(features / 32)]``, ``float8_e8m0fnu``), for :func:`act_checkpoint_backward`.  ``table``: a
+    segment table; only the rows that its counts add up to are read and written."""
+    dt = _rows("x", x)
+    if not act_checkpoint_supported(x.dtype):
+        raise TypeError(f"act_checkpoint_forward does not take {x.dtype}")
+    activation = _activation_of(activation)
+    n, d = x.shape
+    held = torch.empty(n, d, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(n, -(-d // SCALE_ELEMS), dtype=torch.float8_e8m0fnu, device=x.device)
+    y = torch.empty_like(x) if with_act else None
+    with _on(x.device):
+        check(_lib.load().fmoe_act_checkpoint_forward(_ptr(x), _ptr(y), _ptr(held), _ptr(scale), _live_rows(table, n, x.device), n, d, dt,
+                                                      activation, _stream(x)))
+    return y, held, scale
+
+
+def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=None, in_place=False):
+    """``(grad * act'(v), act(v) or None)`` with ``v`` the values that ``held`` and ``scale`` stand for.  ``in_place``: the first result
+    is written over ``grad``."""
+    dt = _rows("grad", grad)
+    if not act_checkpoint_supported(grad.dtype):
+        raise TypeError(f"act_checkpoint_backward does not take {grad.dtype}")
+    activation = _activation_of(activation)
+    n, d = grad.shape
+    _near("held", _dev("held", held, torch.float8_e4m3fn), grad.device)
+    _near("scale", _dev("scale", scale, torch.float8_e8m0fnu), grad.device)
+    if tuple(held.shape) != (n, d) or tuple(scale.shape) != (n, -(-d // SCALE_ELEMS)):
+        raise ValueError(f"held must be [{n}, {d}] and scale [{n}, {-(-d // SCALE_ELEMS)}]")
+    grad_x = grad if in_place else torch.empty_like(grad)
+    mid = torch.empty_like(grad) if with_mid else None
+    with _on(grad.device):
+        check(_lib.load().fmoe_act_checkpoint_backward(_ptr(grad), _ptr(held), _ptr(scale), _ptr(grad_x), _ptr(mid),
+                                                       _live_rows(table, n, grad.device), n, d, dt, activation, _stream(grad)))
+    return grad_x, mid
+
+
+# ---- layer norm of token rows -----------------------------------------------------------
+
+def _near(name, t, device):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t
+
+
+def _strided_rows(name, t, like=None):
+    """``(t, elements between its rows)`` for rows of adjacent elements that may lie apart, be the same one or overlap."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA (HIP) tensor, got device {t.device}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D [rows, features], got shape {tuple(t.shape)}")
+    if like is not None:
+        _near(name, t, like.device)
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must have dtype {like.dtype}, got {t.dtype}")
+        if t.shape != like.shape:
+            raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _norm_params(x, weight, bias):
+    """Code of the parameters' type."""
+    dtype = x.dtype
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        _near(name, _dev(name, p), x.device)
+        if p.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{name} must have dtype {x.dtype} or torch.float32, got {p.dtype}")
+        if tuple(p.shape) != (x.shape[1],):
+            raise ValueError(f"{name} must be [{x.shape[1]}], got {tuple(p.shape)}")
+        dtype = p.dtype
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}")
+    return _DTYPES[dtype]
+
+
+def layer_norm_supported(dtype):
+    """Whether rows of this type are normalised."""
+    return dtype in (torch.float32, torch.bfloat16, torch.float16)
+
+
+def layer_norm_forward(x, residual, weight, bias, eps, keep=True):
+    """``(y, sum, mean, rstd)`` of the rows ``x [rows, features]`` plus ``residual`` (or ``None``: ``sum`` is ``None`` too).  ``keep``:
+    the rows' means and reciprocal deviations (float32) are wanted for :func:`layer_norm_backward`."""
+    x, x_stride = _strided_rows("x", x)
+    if not layer_norm_supported(x.dtype):
+        raise TypeError(f"layer_norm_forward does not take {x.dtype}")
+    n, d = x.shape
+    if d == 0:
+        raise ValueError("rows without features have no norm")
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"eps must be a number that is not negative, got {eps}")
+    r_stride = 0
+    if residual is not None:
+        residual, r_stride = _strided_rows("residual", residual, x)
+    pt = _norm_params(x, weight, bias)
+    y = torch.empty(n, d, dtype=x.dtype, device=x.device)
+    total = torch.empty_like(y) if residual is not None else None
+    mean, rstd = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
+    with _on(x.device):
+        check(_lib.load().fmoe_layer_norm_forward(_ptr(x), x_stride, _ptr(residual), r_stride, _ptr(weight), _ptr(bias), _ptr(total),
+                                                  _ptr(y), _ptr(mean), _ptr(rstd), n, d, float(eps), _DTYPES[x.dtype], pt, _stream(x)))
+    return y, total, mean, rstd
+
+
+def layer_norm_backward(grad_y, grad_sum, x, mean, rstd, weight, bias, want_x=True, want_weight=True, want_bias=True):
+    """``(grad_x, grad_weight, grad_bias)``, ``None`` where not wanted; ``x`` are the rows that were normalised, ``grad_sum`` the
+    gradient that they have besides (or ``None``)."""
+    x, x_stride = _strided_rows("x", x)
+    if not layer_norm_supported(x.dtype):
+        raise TypeError(f"layer_norm_backward does not take {x.dtype}")
+    grad_y, gy_stride = _strided_rows("grad_y", grad_y, x)
+    gs_stride = 0
+    if grad_sum is not None:
+        grad_sum, gs_stride = _strided_rows("grad_sum", grad_sum, x)
+    n, d = x.shape
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _near(name, _dev(name, t, torch.float32), x.device)
+        if t.numel() != n:
+            raise ValueError(f"{name} must have one entry per row")
+    pt = _norm_params(x, weight, bias)
+    param = lambda p, wanted: torch.empty_like(p) if wanted and p is not None else None
+    grad_x = torch.empty(n, d, dtype=x.dtype, device=x.device) if want_x else None
+    grad_w, grad_b = param(weight, want_weight), param(bias, want_bias)
+    lib = _lib.load()
+    with _on(x.device):
+        ws = _workspace(lib.fmoe_layer_norm_backward_workspace_bytes(n, d), x.device) if grad_w is not None or grad_b is not None else None
+        check(lib.fmoe_layer_norm_backward(_ptr(grad_y), gy_stride, _ptr(grad_sum), gs_stride, _ptr(x), x_stride, _ptr(mean), _ptr(rstd),
+                                           _ptr(weight), _ptr(grad_x), _ptr(grad_w), _ptr(grad_b), n, d, _DTYPES[x.dtype], pt, _ptr(ws),
+                                           0 if ws is None else ws.numel(), _stream(x)))
+    return grad_x, grad_w, grad_b
+
+
+# ---- balance loss of a gate -----------------------------------------------------------
+
+def balance_loss_supported(n_expert, dtype):
+    """Whether :func:`balance_loss_forward` takes this gate."""
+    return 1 <= n_expert <= 8192 and dtype in (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _balance_args(logits, mask):
+    dt = _rows("logits", logits)
+    n, e = logits.shape
+    if not balance_loss_supported(e, logits.dtype):
+        raise ValueError(f"balance_loss does not take n_expert={e}, dtype={logits.dtype}")
+    if mask is not None:
+        _near("mask", _dev("mask", mask, torch.bool), logits.device)
+        if mask.numel() != n:
+            raise ValueError(f"mask has {mask.numel()} entries, expected one for each of {n} tokens")
+    return dt, n, e
+
+
+def balance_loss_forward(logits, topk_idx, mask, per_slot):
+    """``(loss, expert_count int64 [E], prob float32 [E], slope)`` of ``logits [N, E]`` and the indices that a gate made of them;
+    ``mask`` (bool, one entry per token, or ``None``): true for tokens that do not count.  ``slope`` is for
+    :func:`balance_loss_backward`."""
+    dt, n, e = _balance_args(logits, mask)
+    _near("topk_idx", _dev("topk_idx", topk_idx, torch.int64), logits.device)
+    if topk_idx.numel() % max(n, 1) or (n and not topk_idx.numel()):
+        raise ValueError(f"topk_idx has {topk_idx.numel()} entries, expected as many for each of {n} tokens")
+    k = topk_idx.numel() // n if n else 1
+    lib = _lib.load()
+    dev = logits.device
+    with _on(dev):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        count = torch.empty(e, dtype=torch.int64, device=dev)
+        prob = torch.empty(e, dtype=torch.float32, device=dev)
+        slope = torch.empty(e + 1, dtype=torch.float32, device=dev)
+        ws = _workspace(lib.fmoe_balance_loss_workspace_bytes(n, e), dev)
+        check(lib.fmoe_balance_loss_forward(_ptr(logits), _ptr(topk_idx), _ptr(mask), n, e, k, dt, int(bool(per_slot)), _ptr(loss),
+                                            _ptr(count), _ptr(prob), _ptr(slope), _ptr(ws), ws.numel(), _stream(logits)))
+    return loss, count, prob, slope
+
+
+def balance_loss_backward(logits, mask, slope, grad_loss, grad_prob):
+    """Gradient of the logits from those of the loss and of ``prob`` (each float32, or ``None``)."""
+    dt, n, e = _balance_args(logits, mask)
+    for name, t, size in (("slope", slope, e + 1), ("grad_loss", grad_loss, 1), ("grad_prob", grad_prob, e)):
+        if t is None and name != "slope":
+            continue
+        _near(name, _dev(name, t, torch.float32), logits.device)
+        if t.numel() != size:
+            raise ValueError(f"{name} must have {size} entries, got {t.numel()}")
+    grad = torch.empty_like(logits)
+    with _on(logits.device):
+        check(_lib.load().fmoe_balance_loss_backward(_ptr(logits), _ptr(mask), _ptr(slope), _ptr(grad_loss), _ptr(grad_prob), _ptr(grad),
+                                                     n, e, dt, _stream(logits)))
+    return grad
+
+
 # ---- a whole layer pass in one call ----------------------------------------------------
 
 def layer_infer(inp, gate_w, gate_b, score, routing, w1, b1, w2, b2, top_k, activation, gate):

@@ -7,6 +7,7 @@ outside this package and raises ``NotImplementedError``.
 """
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 from torch.utils._device import DeviceContext
 
 from . import _lib, fmoe_native
@@ -175,6 +176,51 @@ class NoisyTopK(Function):
         g_clean, g_raw = fmoe_native.noisy_gate_backward(clean, raw, noise, top_k, eps, idx, gates, thr_val, thr_idx,
                                                          grad_gates.contiguous(), grad_load.float().contiguous())
         return g_clean, g_raw, None, None, None
+
+
+class BalanceLoss(Function):
+    r"""Balance loss of a gate with the experts' counts and mean probabilities (see :func:`balance_loss`)."""
+
+    @staticmethod
+    def forward(ctx, logits, topk_idx, mask, per_slot):
+        ctx.set_materialize_grads(False)
+        logits = logits.contiguous()
+        loss, count, prob, slope = fmoe_native.balance_loss_forward(logits, topk_idx, mask, per_slot)
+        ctx.save_for_backward(logits, mask, slope)
+        ctx.mark_non_differentiable(count)
+        return loss, count, prob
+
+    @staticmethod
+    def backward(ctx, grad_loss, _grad_count, grad_prob):
+        logits, mask, slope = ctx.saved_tensors
+        if grad_loss is None and grad_prob is None:
+            return None, None, None, None
+        if torch.is_grad_enabled():   # (a backward that is to be differentiated again needs torch operators)
+            u = 0 if grad_loss is None else grad_loss * slope[:-1]
+            u = u if grad_prob is None else u + grad_prob * slope[-1]
+            empty = (logits == -float("inf")).all(dim=1)
+            left_out = (empty if mask is None else empty | mask).unsqueeze(1)
+            p = torch.softmax(logits.float().masked_fill(left_out, 0), dim=1).masked_fill(left_out, 0)
+            return (p * (u - (p * u).sum(dim=1, keepdim=True))).to(logits.dtype), None, None, None
+        contiguous = lambda t: None if t is None else t.contiguous()
+        return fmoe_native.balance_loss_backward(logits, mask, slope, contiguous(grad_loss), contiguous(grad_prob)), None, None, None
+
+
+def balance_loss(logits, topk_idx, per="token", mask=None):
+    r"""``(loss, expert_count, prob)`` of a gate's ``logits [N, E]`` (float32, bfloat16 or float16; at most 8192 experts) and its choice ``topk_idx`` (int64, one or
+    more entries per token, -1 for dropped slots): with ``c`` the slots that name each expert and ``P`` the summed softmax
+    probabilities, ``loss = E sum_e c_e P_e / D^2``, ``D`` the number of tokens (``per="token"``, the loss of
+    fmoe/gates/gshard_gate.py:23-34) or of slots that name an expert (``per="slot"``, fmoe/gates/switch_gate.py:46-58);
+    ``expert_count`` is ``c`` (int64), ``prob`` is ``P`` over the number of tokens.  Float32 in the sums whatever the logits are.
+    ``loss`` and ``prob`` are differentiable with respect to the logits.  ``mask``: one entry per token, as ``FMoE``'s; tokens whose entry is not 0 (padding) do not
+    count.  Tokens whose logits are all ``-inf`` count but add no probability; nothing to divide by gives 0.  Nothing is read on
+    the host."""
+    if per not in ("token", "slot"):
+        raise ValueError(f'per must be "token" or "slot", got {per!r}')
+    if mask is not None:
+        mask = mask.reshape(-1)
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    return BalanceLoss.apply(logits, topk_idx.contiguous(), mask, per == "slot")
 
 
 def gate_topk(logits, top_k, score_mode=0):
@@ -370,6 +416,44 @@ class MOELinear(Function):
         grad_in, grad_w, grad_b = fmoe_native.linear_backward(
             grad_out.contiguous(), input_buf, fwd_expert_count, weight, bias)
         return grad_in, None, grad_w, grad_b
+
+
+class ActCheckpoint(Function):
+    r"""An activation whose argument is kept in 8 bits for the backward (see :func:`act_checkpoint`)."""
+
+    @staticmethod
+    def forward(ctx, inp, activation):
+        out, held, scale = fmoe_native.act_checkpoint_forward(inp.contiguous(), activation)
+        ctx.save_for_backward(held, scale)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        held, scale = ctx.saved_tensors
+        return fmoe_native.act_checkpoint_backward(grad_out.contiguous(), held, scale, ctx.activation, with_mid=False)[0], None
+
+
+def _as_rows(inp):
+    """``inp`` as rows of its last dimension."""
+    if inp.dim() == 0:
+        raise ValueError("a tensor without dimensions has no rows")
+    return inp.reshape(-1, inp.shape[-1]) if inp.dim() != 2 else inp
+
+
+def act_checkpoint(inp, activation):
+    r"""``activation(inp)`` (an ``ACT_*`` code, ``torch.nn.GELU()`` or ``torch.nn.ReLU()``; exact GELU, ReLU or none) over rows ``[rows, features]`` or of any
+    leading shape, from ``inp`` as it is; for the backward ``inp`` is kept as e4m3 numbers with a power of two for every 32
+    elements along a row, 1.03 bytes an element, and the derivative is taken where those are (off by at most 2^-4 of an element,
+    or 2^-10 of the block's scale where it is small against the block).  Float32, bfloat16 and float16."""
+    code = activation if type(activation) is int else _activation_code(activation)
+    return ActCheckpoint.apply(_as_rows(inp), code).view(inp.shape)
+
+
+def _activation_code(activation):
+    from .fused_functions import _activation_code as code
+    return code(activation)
 
 
 class MOEExpertMLP(Function):
@@ -682,6 +766,49 @@ class MaskRestore(Function):
             grad_fill = torch.zeros(fill.shape, dtype=torch.float32, device=fill.device).index_add_(
                 0, fill_row.clamp(min=0), contrib).to(fill.dtype)
         return grad_kept, None, None, grad_scale, grad_fill, None
+
+
+class LayerNorm(Function):
+    r"""Layer norm over rows, of a sum with a residual where there is one (see :func:`layer_norm`, :func:`add_layer_norm`)."""
+
+    @staticmethod
+    def forward(ctx, inp, residual, weight, bias, eps):
+        keep = any(ctx.needs_input_grad)
+        ctx.set_materialize_grads(False)
+        out, total, mean, rstd = fmoe_native.layer_norm_forward(inp, residual, weight, bias, eps, keep)
+        if keep:
+            ctx.save_for_backward(inp if total is None else total, mean, rstd, weight, bias)
+        return out if total is None else (out, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_total=None):
+        rows, mean, rstd, weight, bias = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if grad_out is None:
+            if grad_total is None:
+                return None, None, None, None, None
+            zeros = lambda p, wanted: torch.zeros_like(p) if wanted and p is not None else None
+            return grad_total, grad_total if need[1] else None, zeros(weight, need[2]), zeros(bias, need[3]), None
+        grad, grad_w, grad_b = fmoe_native.layer_norm_backward(grad_out, grad_total, rows, mean, rstd, weight, bias,
+                                                               need[0] or need[1], need[2], need[3])
+        return grad if need[0] else None, grad if need[1] else None, grad_w, grad_b, None
+
+
+def layer_norm(inp, weight=None, bias=None, eps=1e-5):
+    r"""``torch.nn.functional.layer_norm`` over the last dimension of ``inp`` (float32, bfloat16 or float16, any leading shape) in one
+    pass: what comes before, or after, the layer in a transformer block (examples/transformer-xl/mem_transformer.py:379-409).
+    ``weight`` and ``bias`` ``[features]``, or ``None``, may be float32 beside 16-bit rows; statistics are float32."""
+    return LayerNorm.apply(_as_rows(inp), None, weight, bias, eps).view(inp.shape)
+
+
+def add_layer_norm(inp, residual, weight=None, bias=None, eps=1e-5):
+    r"""``(layer_norm(s), s)`` of ``s = inp + residual`` (same shape and type, ``s`` rounded to it) in one pass; gradients through both
+    results come back in one pass too."""
+    if inp.shape != residual.shape:
+        raise ValueError(f"inp is {tuple(inp.shape)} and residual {tuple(residual.shape)}")
+    out, total = LayerNorm.apply(_as_rows(inp), _as_rows(residual), weight, bias, eps)
+    return out.view(inp.shape), total.view(inp.shape)
 
 
 class AllGather(Function):

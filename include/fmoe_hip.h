@@ -640,6 +640,94 @@ int fmoe_fused_mlp_backward(const fmoe_mlp_params *p, const void *grad_out,
                             void *grad_w2, void *grad_b2, int n_chunks,
                             void *stream);
 
+/* ---- layer norm of token rows -------------------------------------------- */
+
+/* s = x + residual, rounded to the rows' type (s = x without a residual), and
+ *   y = (s - mean(s)) / sqrt(mean((s - mean(s))^2) + eps) * weight + bias
+ * along every row.  FMOE_F32 / FMOE_BF16 / FMOE_F16; weight and bias [row_elems],
+ * each NULL (1 and 0) or of param_dtype, which is the rows' type or FMOE_F32.
+ *   x, residual  rows that begin x_stride, residual_stride elements apart (0:
+ *                every row the same), at any address; residual may be NULL
+ *   sum          [rows, row_elems], s; NULL only without a residual
+ *   mean, rstd   [rows] float32 for the backward, or both NULL
+ * The norm before or after the layer, examples/transformer-xl/mem_transformer.py:379-409. */
+int fmoe_layer_norm_forward(const void *x, int64_t x_stride,
+                            const void *residual, int64_t residual_stride,
+                            const void *weight, const void *bias, void *sum,
+                            void *y, float *mean, float *rstd, int64_t rows,
+                            int64_t row_elems, double eps, int dtype,
+                            int param_dtype, void *stream);
+
+/* Its backward.  x: the rows that were normalised (sum, where the forward had a
+ * residual); grad_sum: the gradient of sum, or NULL.  grad_x [rows, row_elems] is
+ * the gradient of x and of the residual alike; grad_weight, grad_bias [row_elems]
+ * of param_dtype; each of the three may be NULL.  The sums over the rows are made
+ * in a fixed order.  workspace: fmoe_layer_norm_backward_workspace_bytes, needed
+ * for the parameters' gradients only. */
+int64_t fmoe_layer_norm_backward_workspace_bytes(int64_t rows,
+                                                 int64_t row_elems);
+int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_stride,
+                             const void *grad_sum, int64_t grad_sum_stride,
+                             const void *x, int64_t x_stride, const float *mean,
+                             const float *rstd, const void *weight,
+                             void *grad_x, void *grad_weight, void *grad_bias,
+                             int64_t rows, int64_t row_elems, int dtype,
+                             int param_dtype, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
+/* ---- balance loss of a gate ----------------------------------------------- */
+
+/* Over the tokens whose token_mask byte is 0 (NULL: all), T of them:
+ *   expert_count [n_expert] int64  slots of topk_idx [n_tokens, top_k] that name
+ *                the expert (entries outside [0, n_expert) are skipped), S in all
+ *   prob [n_expert]  mean of softmax(logits)
+ *   loss [1]         n_expert * sum_e expert_count[e] * T * prob[e] / D^2, with
+ *                D = T (per_slot 0, fmoe/gates/gshard_gate.py:23-34) or D = S
+ *                (per_slot 1, fmoe/gates/switch_gate.py:46-58)
+ *   slope [n_expert + 1]  for the backward
+ * Nothing to divide by gives 0.  A token whose logits are all minus infinity is
+ * counted and adds no probability.  FMOE_F32 / FMOE_BF16 / FMOE_F16 logits
+ * [n_tokens, n_expert] in, float32 out; at most 8192 experts.  Sums are made in a
+ * fixed order. */
+int64_t fmoe_balance_loss_workspace_bytes(int64_t n_tokens, int64_t n_expert);
+int fmoe_balance_loss_forward(const void *logits, const int64_t *topk_idx,
+                              const void *token_mask, int64_t n_tokens,
+                              int64_t n_expert, int64_t top_k, int dtype,
+                              int per_slot, float *loss, int64_t *expert_count,
+                              float *prob, float *slope, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
+/* grad_logits [n_tokens, n_expert] from the gradients of loss [1] and prob
+ * [n_expert], each NULL for none; zeros for masked tokens. */
+int fmoe_balance_loss_backward(const void *logits, const void *token_mask,
+                               const float *slope, const float *grad_loss,
+                               const float *grad_prob, void *grad_logits,
+                               int64_t n_tokens, int64_t n_expert, int dtype,
+                               void *stream);
+
+/* ---- activations kept in 8 bits -------------------------------------------- */
+
+/* held [rows, row_elems] (e4m3) and scale [rows, ceil(row_elems / 32)]: 32
+ * elements along a row share the scale 2^(byte - 127), the smallest with
+ * max|x| <= 448 * scale over the finite ones (byte >= 1); held is x / scale
+ * rounded to nearest, infinities and NaN as NaN; what would round past the
+ * largest number of the type is held as the largest that it does.
+ * y [rows, row_elems]: act(x) from x itself; NULL: not wanted; may be x.
+ * segment_table (optional, of fmoe_segment_table_build): only the rows that its
+ * counts add up to are read and written.  FMOE_F32 / FMOE_BF16 / FMOE_F16. */
+int fmoe_act_checkpoint_forward(const void *x, void *y, void *held, void *scale,
+                                const void *segment_table, int64_t rows,
+                                int64_t row_elems, int dtype, int activation,
+                                void *stream);
+
+/* With v = held * scale: grad_x = grad * act'(v) (may be grad; both NULL: not
+ * wanted) and mid = act(v) (NULL: not wanted), [rows, row_elems] of dtype. */
+int fmoe_act_checkpoint_backward(const void *grad, const void *held,
+                                 const void *scale, void *grad_x, void *mid,
+                                 const void *segment_table, int64_t rows,
+                                 int64_t row_elems, int dtype, int activation,
+                                 void *stream);
+
 /* ---- a whole layer pass in one call ------------------------------------- */
 
 /* Where a layer pass takes its routing from: the gate's linear layer over x

@@ -1,0 +1,290 @@
+"""Layer norm of token rows, of their sum with a residual, and the gradients against the definition in float64.
+
+A result may be off by half a step of its type and by what float32 does on the way: every value passes through sums of ``d`` terms,
+of which a lane adds ``d / 64`` one after the other before some sixteen more steps, so each is off by at most
+``c = (16 + d / 64) 2^-24`` of the magnitudes that it was made of."""
+import pytest
+import torch
+
+from fastermoe_amd import functions
+
+pytestmark = pytest.mark.gpu
+ULP32 = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _half_step(ref, dtype):
+    info = torch.finfo(dtype)
+    return ref.abs().clamp(min=info.smallest_normal) * (info.eps / 2)
+
+
+def _check(got, ref, slack, what):
+    assert got.shape == ref.shape, what
+    d = (got.double() - ref).abs()
+    limit = _half_step(ref, got.dtype) + slack
+    bad = ~(d <= limit)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} are off, by {float((d / limit).nan_to_num(float('inf')).max()):.2f} times what they may"
+
+
+def _reference(s, w, b, eps):
+    """What the gradients and the bounds need, in float64."""
+    d = s.shape[1]
+    mean = s.mean(1, keepdim=True)
+    rstd = ((s - mean).square().mean(1, keepdim=True) + eps).rsqrt()
+    h = (s - mean) * rstd
+    reach = s.abs().amax(1, keepdim=True) * rstd    # what is rounded where the mean is taken off
+    c = (16 + d / 64) * ULP32
+    one = torch.ones(d, dtype=torch.float64, device=s.device)
+    w = one if w is None else w.detach().double()
+    b = 0 * one if b is None else b.detach().double()
+    return mean, rstd, h, reach, c, w, b
+
+
+def _check_forward(y, s, w, b, eps, what=""):
+    mean, rstd, h, reach, c, w, b = _reference(s, w, b, eps)
+    _check(y, h * w + b, c * ((h.abs() + reach) * w.abs() + b.abs()), what + "y")
+
+
+def _check_backward(grads, s, w, b, eps, dy, ds, what=""):
+    mean, rstd, h, reach, c, w64, _ = _reference(s, w, b, eps)
+    a = dy * w64
+    gx = rstd * (a - a.mean(1, keepdim=True) - h * (a * h).mean(1, keepdim=True)) + ds
+    hr = h.abs() + reach
+    slack = 2 * c * (rstd * (a.abs() + a.abs().mean(1, keepdim=True) + hr * (a.abs() * hr).mean(1, keepdim=True)) + ds.abs())
+    _check(grads[0], gx, slack, what + "grad_x")
+    n = s.shape[0]
+    chain = (160 + n / 64) * ULP32      # the sums over the rows
+    if w is not None:
+        _check(grads[1], (dy * h).sum(0), c * (dy.abs() * hr).sum(0) + chain * (dy * h).abs().sum(0), what + "grad_w")
+    if b is not None:
+        _check(grads[2], dy.sum(0), chain * dy.abs().sum(0), what + "grad_b")
+
+
+def _run(n, d, dtype, residual, params, eps=1e-5, gap=0, seed=0, offset=0.0, device="cuda"):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    normal = lambda *shape: torch.randn(shape, device=device, generator=gen)
+    dtype = TYPES[dtype]
+    x = (normal(n, d + gap) * torch.exp(normal(n, 1)) + offset).to(dtype)[:, :d].detach().requires_grad_(True)
+    r = normal(n, d).to(dtype).requires_grad_(True) if residual else None
+    w = b = None
+    if params != "none":
+        ptype = torch.float32 if params == "f32" else dtype
+        w = (1 + 0.3 * normal(d)).to(ptype).requires_grad_(True)
+        b = (0.2 * normal(d)).to(ptype).requires_grad_(True)
+    dy, ds = normal(n, d).to(dtype), normal(n, d).to(dtype)
+    leaves = [t for t in (x, r, w, b) if t is not None]
+    if residual:
+        y, s = functions.add_layer_norm(x, r, w, b, eps)
+        want = (x.detach().float() + r.detach().float()).to(dtype)
+        assert torch.equal(s, want)
+        grads = dict(zip([id(t) for t in leaves], torch.autograd.grad([y, s], leaves, [dy, ds])))
+        assert torch.equal(grads[id(x)], grads[id(r)])
+        total, ds = s.detach().double(), ds.double()
+    else:
+        y = functions.layer_norm(x, w, b, eps)
+        grads = dict(zip([id(t) for t in leaves], torch.autograd.grad(y, leaves, dy)))
+        total, ds = x.detach().double(), torch.zeros(n, d, dtype=torch.float64, device=device)
+    assert y.dtype == dtype and y.is_contiguous()
+    _check_forward(y.detach(), total, w, b, eps)
+    _check_backward([grads[id(x)], grads.get(id(w)), grads.get(id(b))], total, w, b, eps, dy.double(), ds)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 2), (1, 1024), (7, 37), (64, 64), (509, 500), (65, 1302), (33, 4096), (5, 8192), (3, 16400),
+                                 (2, 40001), (1030, 512), (4099, 96)])
+def test_sizes(n, d, residual, dtype, device):
+    _run(n, d, dtype, residual, "same")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("params", ["none", "f32"])
+def test_parameters(params, dtype, device):
+    _run(130, 515, dtype, True, params)
+    _run(130, 1024, dtype, False, params)
+
+
+@pytest.mark.parametrize("gap", [1, 8, 10])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_of_a_wider_tensor(gap, dtype, device):
+    _run(77, 1024, dtype, True, "same", gap=gap)
+    _run(77, 51, dtype, False, "same", gap=gap)
+
+
+def test_rows_far_from_zero(device):
+    _run(40, 2048, "f32", False, "same", offset=300.0)
+    _run(40, 2048, "bf16", True, "same", offset=50.0)
+
+
+def test_one_parameter_alone_and_gradients_that_are_not_wanted(device):
+    x = torch.randn(20, 72, device=device)
+    dy = torch.randn(20, 72, device=device)
+    for has in ("weight", "bias"):
+        p = torch.randn(72, device=device, requires_grad=True)
+        w, b = (p, None) if has == "weight" else (None, p)
+        y = functions.layer_norm(x, w, b)
+        _check_forward(y.detach(), x.double(), w, b, 1e-5, has + " ")
+        g, = torch.autograd.grad(y, p, dy)
+        h = _reference(x.double(), None, None, 1e-5)[2]
+        assert torch.allclose(g.double(), (dy.double() * h).sum(0) if has == "weight" else dy.double().sum(0), rtol=1e-4, atol=1e-5)
+    x.requires_grad_(True)
+    w = torch.randn(72, device=device)   # (not differentiated)
+    g, = torch.autograd.grad(functions.layer_norm(x, w), x, dy)
+    _check_backward([g, None, None], x.detach().double(), None, None, 1e-5, (dy * w).double(), torch.zeros_like(x).double())
+
+
+def test_gradients_against_differences(device):
+    """Directional derivatives in float64 of the definition, by central differences, against the kernels' gradients."""
+    torch.manual_seed(5)
+    x, r, w, b, dy, ds = (torch.randn(*s, device=device, dtype=torch.float64) for s in ((6, 40), (6, 40), (40,), (40,), (6, 40), (6, 40)))
+
+    def value(x, r, w, b):
+        s = x + r
+        h = (s - s.mean(1, keepdim=True)) * (s.var(1, correction=0, keepdim=True) + 1e-5).rsqrt()
+        return ((h * w + b) * dy).sum() + (s * ds).sum()
+
+    leaves = [t.float().requires_grad_(True) for t in (x, r, w, b)]
+    y, s = functions.add_layer_norm(*leaves)
+    grads = torch.autograd.grad([y, s], leaves, [dy.float(), ds.float()])
+    at = [t.detach().double() for t in leaves]
+    for i, g in enumerate(grads):
+        v = torch.randn_like(at[i])
+        step = 1e-5
+        up, down = (value(*[t + (k * step * v if j == i else 0) for j, t in enumerate(at)]) for k in (1, -1))
+        want = float((up - down) / (2 * step))
+        got = float((g.double() * v).sum())
+        assert abs(got - want) <= 1e-4 * float((g.double() * v).abs().sum()), i
+
+
+def test_constant_and_zero_rows(device):
+    """Nothing to normalise: the deviation is 0, the rows become the bias, and eps alone scales the gradient."""
+    w, b = torch.randn(96, device=device), torch.randn(96, device=device)
+    for value in (0.0, 2.5):
+        x = torch.full((4, 96), value, device=device, requires_grad=True)
+        y = functions.layer_norm(x, w, b, 1e-5)
+        assert torch.equal(y.detach(), b.expand(4, 96))
+        dy = torch.randn(4, 96, device=device)
+        g, = torch.autograd.grad(y, x, dy)
+        a = (dy * w).double()
+        _check(g, (a - a.mean(1, keepdim=True)) * 1e-5 ** -0.5, 20 * ULP32 * 1e-5 ** -0.5 * (a.abs() + a.abs().mean(1, keepdim=True)), "grad")
+
+
+def test_nan_and_infinity_stay_in_their_rows(device):
+    x = torch.randn(5, 300, device=device, dtype=torch.bfloat16)
+    clean = functions.layer_norm(x)
+    x[1, 7], x[3, 299] = float("nan"), float("inf")
+    y = functions.layer_norm(x)
+    assert bool(y[[1, 3]].isnan().any(1).all()) and torch.equal(y[[0, 2, 4]], clean[[0, 2, 4]])
+
+
+def test_no_rows_and_leading_shapes(device):
+    w = torch.ones(24, device=device, requires_grad=True)
+    x = torch.empty(0, 24, device=device, requires_grad=True)
+    y = functions.layer_norm(x, w)
+    gx, gw = torch.autograd.grad(y, [x, w], torch.empty(0, 24, device=device))
+    assert y.shape == (0, 24) and gx.shape == (0, 24) and torch.equal(gw, torch.zeros_like(w))
+    x = torch.randn(3, 5, 24, device=device)
+    assert torch.equal(functions.layer_norm(x, w), functions.layer_norm(x.view(15, 24), w).view(3, 5, 24))
+    assert torch.equal(functions.layer_norm(x[0, 0], w), functions.layer_norm(x.view(15, 24), w)[0])
+    t = x.transpose(0, 1)      # rows in another order
+    assert torch.equal(functions.layer_norm(t, w), functions.layer_norm(t.contiguous(), w))
+    wide = torch.randn(24, 15, device=device).t()   # adjacent rows, elements apart
+    assert torch.equal(functions.layer_norm(wide, w), functions.layer_norm(wide.contiguous(), w))
+
+
+def test_expanded_rows_and_gradients(device):
+    """A residual that is one row for all tokens, and a gradient that is one number for all elements."""
+    x = torch.randn(50, 128, device=device, requires_grad=True)
+    one = torch.randn(1, 128, device=device, requires_grad=True)
+    y, s = functions.add_layer_norm(x, one.expand(50, 128))
+    gx, g1 = torch.autograd.grad([y, s], [x, one], [torch.ones((), device=device).expand(50, 128), torch.randn(1, 128, device=device).expand(50, 128)])
+    copy = one.detach().expand(50, 128).contiguous()
+    y2, s2 = functions.add_layer_norm(x.detach(), copy)
+    assert torch.equal(y.detach(), y2) and torch.equal(s.detach(), s2)
+    assert torch.allclose(g1, gx.sum(0, keepdim=True), rtol=1e-4, atol=1e-5)
+
+
+def test_gradients_through_one_result_only(device):
+    x, r = (torch.randn(9, 64, device=device, requires_grad=True) for _ in range(2))
+    w = torch.randn(64, device=device, requires_grad=True)
+    y, s = functions.add_layer_norm(x, r, w)
+    g = torch.randn(9, 64, device=device)
+    gx, gr, gw = torch.autograd.grad(s, [x, r, w], g, retain_graph=True)
+    assert torch.equal(gx, g) and torch.equal(gr, g) and torch.equal(gw, torch.zeros_like(w))
+    gx, gw = torch.autograd.grad(y, [x, w], g)
+    _check_backward([gx, gw, None], s.detach().double(), w, None, 1e-5, g.double(), torch.zeros_like(g).double())
+
+
+def test_same_bits_every_time_and_by_row(device):
+    """A row's results do not depend on the other rows, and the sums over the rows are made in one order."""
+    x = torch.randn(3000, 768, device=device, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(768, device=device, dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.randn(3000, 768, device=device, dtype=torch.bfloat16)
+    run = lambda: (lambda y: (y,) + torch.autograd.grad(y, [x, w], dy))(functions.layer_norm(x, w))
+    first = run()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+    assert torch.equal(functions.layer_norm(x[17:18], w), first[0][17:18])
+
+
+def test_offsets_beyond_32_bits(device):
+    """Rows of a tensor of more than 2^31 elements, far apart."""
+    d, n = 64, 40
+    stride = (1 << 31) // (n // 2)
+    buf = torch.empty((n - 1) * stride + d, dtype=torch.bfloat16, device=device)
+    x = buf.as_strided((n, d), (stride, 1))
+    x.copy_(torch.randn(n, d, device=device))
+    copy = x.contiguous()
+    x.requires_grad_(True)
+    y = functions.layer_norm(x)
+    assert torch.equal(y.detach(), functions.layer_norm(copy))
+    dy = torch.randn(n, d, device=device, dtype=torch.bfloat16)
+    g, = torch.autograd.grad(y, x, dy)
+    copy.requires_grad_(True)
+    assert torch.equal(g, torch.autograd.grad(functions.layer_norm(copy), copy, dy)[0])
+
+
+def test_another_stream_and_a_graph(device):
+    """Captured, replayed with other rows between eager work, and every replay against the eager result."""
+    n, d = 300, 640
+    x, r, dy = (torch.randn(n, d, device=device, dtype=torch.bfloat16) for _ in range(3))
+    w, b = (torch.randn(d, device=device, dtype=torch.float32) for _ in range(2))
+
+    def step(x, r, dy, w, b):
+        leaves = [t.detach().requires_grad_(True) for t in (x, r, w, b)]
+        y, s = functions.add_layer_norm(*leaves)
+        return (y.detach(), s.detach()) + torch.autograd.grad([y, s], leaves, [dy, dy])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = step(x, r, dy, w, b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b_) for a, b_ in zip(warm, step(x, r, dy, w, b)))
+    del warm
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(x, r, dy, w, b)
+    for k in range(4):
+        for t in (x, r, dy):
+            t.copy_(torch.randn(n, d, device=device))
+        w.copy_(torch.randn(d, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(held, step(x, r, dy, w, b)):
+            assert torch.equal(a, e), k
+
+
+def test_checkpointed_and_module_parameters(device):
+    """Inside an activation checkpoint, with an nn.LayerNorm's parameters, against the module in float64."""
+    from torch.utils.checkpoint import checkpoint
+    norm = torch.nn.LayerNorm(256).to(device)
+    x = torch.randn(31, 256, device=device, requires_grad=True)
+    dy = torch.randn(31, 256, device=device)
+    y = checkpoint(lambda t: functions.layer_norm(t, norm.weight, norm.bias, norm.eps), x, use_reentrant=False)
+    got = torch.autograd.grad(y, [x, norm.weight, norm.bias], dy)
+    ref = torch.nn.LayerNorm(256).to(device).double()
+    x64 = x.detach().double().requires_grad_(True)
+    want = torch.autograd.grad(ref(x64), [x64, ref.weight, ref.bias], dy.double())
+    for g, e in zip(got, want):
+        assert torch.allclose(g.double(), e, rtol=1e-5, atol=1e-5)
