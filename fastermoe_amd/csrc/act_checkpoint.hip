@@ -7,9 +7,14 @@
 // block that can); infinities and NaN are held as NaN, so that a forward that overflowed still shows in the gradients.
 //
 //   forward   y = act(x), q, b          backward  x~ = q 2^b   mid = act(x~)   grad_x = grad act'(x~)
+//
+// A lane takes eight elements of a row, four lanes a block: one 16-byte load of a 16-bit type, a maximum over the lanes of a quad, eight
+// bytes out; P such pieces of a workgroup's run are in flight per lane.  Rows of whole blocks are one run of pieces (FLAT); others, of any length, are cut into
+// pieces row by row, and a row's last one is read and written element by element where it is not whole.
 #include "common.hpp"
 #include "gelu_terms.hpp"
 #include "grouped_gemm.hpp"
+#include "wave_piece.hpp"
 
 #include <type_traits>
 
@@ -17,20 +22,63 @@ namespace fmoe {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kScaleElems = 32;
+constexpr int kScaleElems = 32, kLaneElems = 8, kLanes = kScaleElems / kLaneElems;   // lanes that share a scale
+constexpr int kPieces = 4;                                                             // pieces in flight per lane
 
-__device__ __forceinline__ float act_value(float x, int act) {
-    if (act == FMOE_ACT_RELU) return x < 0.f ? 0.f : x;   // (NaN stays)
-    if (act == FMOE_ACT_GELU) return x * gemm::gelu_terms(x).cdf;
+template <int ACT> __device__ __forceinline__ float act_value(float x) {
+    if (ACT == FMOE_ACT_RELU) return x < 0.f ? 0.f : x;   // (NaN stays)
+    if (ACT == FMOE_ACT_GELU) return x * gemm::gelu_terms(x).cdf;
     return x;
 }
-__device__ __forceinline__ float act_slope(float x, int act) {
-    if (act == FMOE_ACT_RELU) return x > 0.f ? 1.f : x == x ? 0.f : x;
-    if (act == FMOE_ACT_GELU) {
+// act(x) and act'(x)
+template <int ACT> __device__ __forceinline__ void act_both(float x, float &value, float &slope) {
+    if (ACT == FMOE_ACT_RELU) {
+        value = x < 0.f ? 0.f : x;
+        slope = x > 0.f ? 1.f : x == x ? 0.f : x;
+    } else if (ACT == FMOE_ACT_GELU) {
         const gemm::GeluTerms g = gemm::gelu_terms(x);
-        return g.cdf + x * g.pdf;
+        value = x * g.cdf;
+        slope = g.cdf + x * g.pdf;
+    } else {
+        value = x;
+        slope = x == x ? 1.f : x;
     }
-    return x == x ? 1.f : x;
+}
+
+// Eight elements at p, wherever it lies, or the first n of them and zeros; WHOLE: eight or none.
+template <bool WHOLE, typename T> __device__ __forceinline__ void load8(const T *p, int n, T (&e)[kLaneElems]) {
+    if (WHOLE ? n > 0 : n >= kLaneElems) {
+        __builtin_memcpy(e, p, sizeof(e));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) e[j] = !WHOLE && j < n ? p[j] : T{};
+    }
+}
+template <bool WHOLE, typename T> __device__ __forceinline__ void store8(T *p, int n, const T (&e)[kLaneElems]) {
+    if (WHOLE ? n > 0 : n >= kLaneElems) {
+        __builtin_memcpy(p, e, sizeof(e));
+    } else if (!WHOLE) {
+#pragma unroll
+        for (int j = 0; j < kLaneElems - 1; ++j)
+            if (j < n) p[j] = e[j];
+    }
+}
+
+struct Bytes8 { uint8_t byte[kLaneElems]; };
+
+// Where a lane's piece lies: its elements begin at `at` and are n (0: past the row's or the rows' end), its block's scale is number `block`.
+struct Piece { int64_t at, block; int n; };
+// The pieces of the calling workgroup begin at `first`; the lane takes number `mine` of them.
+template <bool FLAT> __device__ __forceinline__ Piece piece_at(int64_t first, uint32_t mine, int64_t rows, int d, uint32_t per_row) {
+    if (FLAT) {
+        const int64_t i = first + mine;
+        return Piece{i * kLaneElems, i / kLanes, i < rows * per_row ? kLaneElems : 0};
+    }
+    const int64_t row0 = div_small(first, per_row);
+    const uint32_t from = (uint32_t)(first - row0 * per_row) + mine, down = from / per_row, c = from - down * per_row;
+    const int64_t row = row0 + down;
+    const int left = d - (int)c * kLaneElems;
+    return Piece{row * d + c * kLaneElems, row * (per_row / kLanes) + c / kLanes, row < rows ? left < kLaneElems ? left : kLaneElems : 0};
 }
 
 // The scale's byte for a block whose largest finite magnitude is `most`
@@ -53,43 +101,97 @@ __device__ __forceinline__ int64_t live_rows(const int32_t *table, int64_t rows)
     return n < rows ? n : rows;
 }
 
-template <typename T>
+// The largest of the values of the lanes that share a scale
+__device__ __forceinline__ float lanes_max(float v) {
+    static_assert(kLanes == 4, "a quad of lanes");
+    v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0xb1, 0xf, 0xf, true)));          // quad_perm 1 0 3 2
+    return fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x4e, 0xf, 0xf, true)));       // quad_perm 2 3 0 1
+}
+
+template <typename T, int ACT, bool FLAT>
 __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint8_t *__restrict__ held, uint8_t *__restrict__ scale,
-                                                          const int32_t *__restrict__ table, int64_t rows, int64_t d, int act) {
-    const int64_t per_row = (d + kScaleElems - 1) / kScaleElems;
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x, row = i / per_row, c0 = (i - row * per_row) * kScaleElems;
-    if (row >= live_rows(table, rows)) return;
-    const int n = (int)(d - c0 < kScaleElems ? d - c0 : kScaleElems);
-    const int64_t at = row * d + c0;
-    float most = 0.f;
-    for (int j = 0; j < n; ++j) most = fmaxf(most, finite_magnitude((float)x[at + j]));
-    const int b = scale_byte(most);
-    const float inv = __uint_as_float((uint32_t)(254 - b) << 23), limit = b == top_byte<T>() ? 240.f : 448.f;
-    scale[i] = (uint8_t)b;
-    for (int j = 0; j < n; ++j) {
-        const float v = (float)x[at + j];
-        const float q = fmaf(v, 0.f, __builtin_amdgcn_fmed3f(v * inv, -limit, limit));
-        held[at + j] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
-        if (y) y[at + j] = (T)act_value(v, act);
+                                                          const int32_t *__restrict__ table, int64_t rows, int d, int per_row) {
+    rows = live_rows(table, rows);
+    const int64_t first = (int64_t)blockIdx.x * (kBlock * kPieces);
+    if (first >= rows * per_row) return;
+    T e[kPieces][kLaneElems];
+    Piece at[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        at[p] = piece_at<FLAT>(first, p * kBlock + threadIdx.x, rows, d, per_row);
+        load8<FLAT>(x + at[p].at, at[p].n, e[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        float f[kLaneElems], most = 0.f;
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) {
+            f[j] = (float)e[p][j];
+            most = fmaxf(most, finite_magnitude(f[j]));
+        }
+        const int b = scale_byte(lanes_max(most));
+        if (at[p].n <= 0) continue;
+        const float inv = __uint_as_float((uint32_t)(254 - b) << 23), limit = b == top_byte<T>() ? 240.f : 448.f;
+        if (threadIdx.x % kLanes == 0) scale[at[p].block] = (uint8_t)b;
+        uint32_t q[2] = {0, 0};
+        float v[kLaneElems];
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) v[j] = fmaf(f[j], 0.f, __builtin_amdgcn_fmed3f(f[j] * inv, -limit, limit));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
+            q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], q[h], true);
+        }
+        store8<FLAT>(held + at[p].at, at[p].n, __builtin_bit_cast(Bytes8, q).byte);
+        if (y) {
+#pragma unroll
+            for (int j = 0; j < kLaneElems; ++j) e[p][j] = (T)act_value<ACT>(f[j]);
+            store8<FLAT>(y + at[p].at, at[p].n, e[p]);
+        }
     }
 }
 
-template <typename T>
+template <typename T, int ACT, bool FLAT>
 __global__ __launch_bounds__(kBlock) void ckpt_bwd_kernel(const T *grad, const uint8_t *__restrict__ held,
                                                           const uint8_t *__restrict__ scale, T *grad_x, T *__restrict__ mid,
-                                                          const int32_t *__restrict__ table, int64_t rows, int64_t d, int act) {
-    const int64_t per_row = (d + kScaleElems - 1) / kScaleElems;
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x, row = i / per_row, c0 = (i - row * per_row) * kScaleElems;
-    if (row >= live_rows(table, rows)) return;
-    const int n = (int)(d - c0 < kScaleElems ? d - c0 : kScaleElems);
-    const int64_t at = row * d + c0;
-    const float s = __uint_as_float((uint32_t)scale[i] << 23);
-    for (int j = 0; j < n; ++j) {
-        const float v = __builtin_amdgcn_cvt_f32_fp8((int)held[at + j], 0) * s;
-        if (grad_x) grad_x[at + j] = (T)((float)grad[at + j] * act_slope(v, act));
-        if (mid) mid[at + j] = (T)act_value(v, act);
+                                                          const int32_t *__restrict__ table, int64_t rows, int d, int per_row) {
+    rows = live_rows(table, rows);
+    const int64_t first = (int64_t)blockIdx.x * (kBlock * kPieces);
+    if (first >= rows * per_row) return;
+    T g[kPieces][kLaneElems];
+    uint8_t q[kPieces][kLaneElems];
+    uint32_t b[kPieces];
+    Piece at[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        at[p] = piece_at<FLAT>(first, p * kBlock + threadIdx.x, rows, d, per_row);
+        load8<FLAT>(held + at[p].at, at[p].n, q[p]);
+        b[p] = at[p].n > 0 ? scale[at[p].block] : 0;
+        if (grad) load8<FLAT>(grad + at[p].at, at[p].n, g[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+        const float s = __uint_as_float(b[p] << 23);
+        const uint2 w = __builtin_bit_cast(uint2, q[p]);
+        T m[kLaneElems];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const auto two = (h & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)(h < 2 ? w.x : w.y), true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)(h < 2 ? w.x : w.y), false);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float value, slope;
+                act_both<ACT>(two[i] * s, value, slope);
+                m[2 * h + i] = (T)value;
+                if (grad) g[p][2 * h + i] = (T)((float)g[p][2 * h + i] * slope);
+            }
+        }
+        if (grad) store8<FLAT>(grad_x + at[p].at, at[p].n, g[p]);
+        if (mid) store8<FLAT>(mid + at[p].at, at[p].n, m);
     }
 }
+
+int per_row(int64_t d) { return (int)(ceil_div(d, kScaleElems) * kLanes); }   // pieces
+int64_t n_blocks(int64_t rows, int64_t d) { return ceil_div(rows * per_row(d), kBlock * kPieces); }
 
 int check(const char *who, int64_t rows, int64_t d, int dtype, int activation) {
     FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who,
@@ -97,15 +199,26 @@ int check(const char *who, int64_t rows, int64_t d, int dtype, int activation) {
     FMOE_REQUIRE(activation == FMOE_ACT_NONE || activation == FMOE_ACT_RELU || activation == FMOE_ACT_GELU, "%s: unknown activation %d",
                  who, activation);
     FMOE_REQUIRE(rows >= 0 && d >= 0, "%s: bad sizes", who);
-    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 28) || ceil_div(rows * ceil_div(d, kScaleElems), kBlock) > INT32_MAX)
+    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 28) || n_blocks(rows, d) > INT32_MAX)
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     return FMOE_OK;
 }
 
-template <typename F> void with_type(int dtype, F &&f) {
-    if (dtype == FMOE_F32) f(float{});
-    else if (dtype == FMOE_BF16) f(__bf16{});
-    else f(_Float16{});
+// launch(kernel's type, activation, whether the rows are whole blocks)
+template <typename T, typename F> void with_activation(int activation, bool flat, F &&f) {
+    auto go = [&](auto act) {
+        if (flat) f(T{}, act, std::true_type{});
+        else f(T{}, act, std::false_type{});
+    };
+    if (activation == FMOE_ACT_RELU) go(std::integral_constant<int, FMOE_ACT_RELU>{});
+    else if (activation == FMOE_ACT_GELU) go(std::integral_constant<int, FMOE_ACT_GELU>{});
+    else go(std::integral_constant<int, FMOE_ACT_NONE>{});
+}
+template <typename F> void with_kernel(int dtype, int activation, int64_t d, F &&f) {
+    const bool flat = d % kScaleElems == 0;
+    if (dtype == FMOE_F32) with_activation<float>(activation, flat, f);
+    else if (dtype == FMOE_BF16) with_activation<__bf16>(activation, flat, f);
+    else with_activation<_Float16>(activation, flat, f);
 }
 
 }  // namespace
@@ -119,11 +232,10 @@ extern "C" int fmoe_act_checkpoint_forward(const void *x, void *y, void *held, v
     if (int rc = check(who, rows, row_elems, dtype, activation)) return rc;
     if (rows == 0 || row_elems == 0) return FMOE_OK;
     FMOE_REQUIRE(x && held && scale, "%s: NULL pointer", who);
-    const int blocks = (int)ceil_div(rows * ceil_div(row_elems, kScaleElems), kBlock);
-    with_type(dtype, [&](auto t) {
+    with_kernel(dtype, activation, row_elems, [&](auto t, auto act, auto flat) {
         using T = decltype(t);
-        ckpt_fwd_kernel<T><<<blocks, kBlock, 0, (hipStream_t)stream>>>((const T *)x, (T *)y, (uint8_t *)held, (uint8_t *)scale,
-                                                                       (const int32_t *)segment_table, rows, row_elems, activation);
+        ckpt_fwd_kernel<T, act.value, flat.value><<<(int)n_blocks(rows, row_elems), kBlock, 0, (hipStream_t)stream>>>(
+            (const T *)x, (T *)y, (uint8_t *)held, (uint8_t *)scale, (const int32_t *)segment_table, rows, (int)row_elems, per_row(row_elems));
     });
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
@@ -136,12 +248,11 @@ extern "C" int fmoe_act_checkpoint_backward(const void *grad, const void *held, 
     if (int rc = check(who, rows, row_elems, dtype, activation)) return rc;
     if (rows == 0 || row_elems == 0) return FMOE_OK;
     FMOE_REQUIRE(held && scale && !grad == !grad_x && (grad_x || mid), "%s: NULL pointer", who);
-    const int blocks = (int)ceil_div(rows * ceil_div(row_elems, kScaleElems), kBlock);
-    with_type(dtype, [&](auto t) {
+    with_kernel(dtype, activation, row_elems, [&](auto t, auto act, auto flat) {
         using T = decltype(t);
-        ckpt_bwd_kernel<T><<<blocks, kBlock, 0, (hipStream_t)stream>>>((const T *)grad, (const uint8_t *)held, (const uint8_t *)scale,
-                                                                       (T *)grad_x, (T *)mid, (const int32_t *)segment_table, rows,
-                                                                       row_elems, activation);
+        ckpt_bwd_kernel<T, act.value, flat.value><<<(int)n_blocks(rows, row_elems), kBlock, 0, (hipStream_t)stream>>>(
+            (const T *)grad, (const uint8_t *)held, (const uint8_t *)scale, (T *)grad_x, (T *)mid, (const int32_t *)segment_table, rows,
+            (int)row_elems, per_row(row_elems));
     });
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
