@@ -9,8 +9,11 @@
 //   forward   y = act(x), q, b          backward  x~ = q 2^b   mid = act(x~)   grad_x = grad act'(x~)
 //
 // A lane takes eight elements of a row, four lanes a block: one 16-byte load of a 16-bit type, a maximum over the lanes of a quad, eight
-// bytes out; P such pieces of a workgroup's run are in flight per lane.  Rows of whole blocks are one run of pieces (FLAT); others, of any length, are cut into
-// pieces row by row, and a row's last one is read and written element by element where it is not whole.
+// bytes out.  Rows of whole blocks are one run of such pieces (FLAT); others, of any length, are cut into pieces row by row, and a row's last one is
+// stored in parts.  Bound by memory: 32768 rows of 14336 in bfloat16 with GELU forward 381 us, without y 230, backward 543 (6.1 to 6.2 TB/s;
+// a large copy on the same card 5.0); 32768 of 4096 in float32 207 and 300 (5.8); 32768 of 1302 in bfloat16, whose rows begin anywhere, 44 and 58 (4.8
+// and 5.2).  One piece to a lane: two or four in flight, on a half or a quarter of the workgroups, took 383 and 572 or 413 and 586 us of the first,
+// and 4.8 and 7.0 of the 4.5 and 5.6 that 1554 rows of 1302 take.  A block to a thread, one element after the other, took 21600 for the first.
 #include "common.hpp"
 #include "gelu_terms.hpp"
 #include "grouped_gemm.hpp"
@@ -23,7 +26,6 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kScaleElems = 32, kLaneElems = 8, kLanes = kScaleElems / kLaneElems;   // lanes that share a scale
-constexpr int kPieces = 4;                                                             // pieces in flight per lane
 
 template <int ACT> __device__ __forceinline__ float act_value(float x) {
     if (ACT == FMOE_ACT_RELU) return x < 0.f ? 0.f : x;   // (NaN stays)
@@ -45,40 +47,58 @@ template <int ACT> __device__ __forceinline__ void act_both(float x, float &valu
     }
 }
 
-// Eight elements at p, wherever it lies, or the first n of them and zeros; WHOLE: eight or none.
-template <bool WHOLE, typename T> __device__ __forceinline__ void load8(const T *p, int n, T (&e)[kLaneElems]) {
-    if (WHOLE ? n > 0 : n >= kLaneElems) {
+// Eight elements at p, wherever it lies; WHOLE: or none.  Otherwise n may be less than eight: what is behind them (`inside`: the memory
+// there still is the tensor's) is read and made zeros.
+template <bool WHOLE, typename T> __device__ __forceinline__ void load8(const T *p, int n, bool inside, T (&e)[kLaneElems]) {
+    if (WHOLE ? n > 0 : n >= kLaneElems || (n > 0 && inside)) {
         __builtin_memcpy(e, p, sizeof(e));
+        if (!WHOLE) {
+#pragma unroll
+            for (int j = 1; j < kLaneElems; ++j) e[j] = j < n ? e[j] : T{};
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < kLaneElems; ++j) e[j] = !WHOLE && j < n ? p[j] : T{};
     }
 }
+// The first n of them: four, two and one at a time, out of registers (arrays of elements chosen by n would go through LDS)
+template <int WORDS> struct Words { uint32_t w[WORDS]; };
 template <bool WHOLE, typename T> __device__ __forceinline__ void store8(T *p, int n, const T (&e)[kLaneElems]) {
     if (WHOLE ? n > 0 : n >= kLaneElems) {
         __builtin_memcpy(p, e, sizeof(e));
-    } else if (!WHOLE) {
+    } else if (!WHOLE && n > 0) {
+        constexpr int kHalf = (int)sizeof(T);          // words of four elements
+        Words<2 * kHalf> all;
+        __builtin_memcpy(&all, e, sizeof(e));
+        Words<kHalf> four;
+        const uint32_t past4 = n & 4 ? ~0u : 0u, past2 = n & 2 ? ~0u : 0u;
+        if (n & 4) __builtin_memcpy(p, &all, 4 * sizeof(T));
 #pragma unroll
-        for (int j = 0; j < kLaneElems - 1; ++j)
-            if (j < n) p[j] = e[j];
+        for (int j = 0; j < kHalf; ++j) four.w[j] = (all.w[kHalf + j] & past4) | (all.w[j] & ~past4);
+        p += n & 4;
+        if (n & 2) __builtin_memcpy(p, &four, 2 * sizeof(T));
+        const uint32_t one = ((kHalf == 1 ? four.w[0] >> 16 : four.w[kHalf / 2]) & past2) | (four.w[0] & ~past2);
+        if (n & 1) __builtin_memcpy(p + (n & 2), &one, sizeof(T));
     }
 }
 
 struct Bytes8 { uint8_t byte[kLaneElems]; };
 
-// Where a lane's piece lies: its elements begin at `at` and are n (0: past the row's or the rows' end), its block's scale is number `block`.
-struct Piece { int64_t at, block; int n; };
-// The pieces of the calling workgroup begin at `first`; the lane takes number `mine` of them.
-template <bool FLAT> __device__ __forceinline__ Piece piece_at(int64_t first, uint32_t mine, int64_t rows, int d, uint32_t per_row) {
+// Where a lane's piece lies: its elements begin at `at` and are n (0 or less: past the row's or the rows' end), its block's scale is number
+// `block`; `inside`: eight elements there are the tensor's.
+struct Piece { int64_t at, block; int n; bool inside; };
+// The calling lane's; a workgroup's pieces begin at `first`.
+template <bool FLAT> __device__ __forceinline__ Piece piece_at(int64_t first, int64_t rows, int d, uint32_t per_row) {
+    const uint32_t mine = threadIdx.x;
     if (FLAT) {
         const int64_t i = first + mine;
-        return Piece{i * kLaneElems, i / kLanes, i < rows * per_row ? kLaneElems : 0};
+        return Piece{i * kLaneElems, i / kLanes, i < rows * per_row ? kLaneElems : 0, true};
     }
     const int64_t row0 = div_small(first, per_row);
     const uint32_t from = (uint32_t)(first - row0 * per_row) + mine, down = from / per_row, c = from - down * per_row;
-    const int64_t row = row0 + down;
+    const int64_t row = row0 + down, at = row * d + c * kLaneElems;
     const int left = d - (int)c * kLaneElems;
-    return Piece{row * d + c * kLaneElems, row * (per_row / kLanes) + c / kLanes, row < rows ? left < kLaneElems ? left : kLaneElems : 0};
+    return Piece{at, row * (per_row / kLanes) + c / kLanes, row < rows ? left < kLaneElems ? left : kLaneElems : 0, at + kLaneElems <= rows * d};
 }
 
 // The scale's byte for a block whose largest finite magnitude is `most`
@@ -112,42 +132,35 @@ template <typename T, int ACT, bool FLAT>
 __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint8_t *__restrict__ held, uint8_t *__restrict__ scale,
                                                           const int32_t *__restrict__ table, int64_t rows, int d, int per_row) {
     rows = live_rows(table, rows);
-    const int64_t first = (int64_t)blockIdx.x * (kBlock * kPieces);
+    const int64_t first = (int64_t)blockIdx.x * kBlock;
     if (first >= rows * per_row) return;
-    T e[kPieces][kLaneElems];
-    Piece at[kPieces];
+    const Piece at = piece_at<FLAT>(first, rows, d, per_row);
+    T e[kLaneElems];
+    load8<FLAT>(x + at.at, at.n, at.inside, e);
+    float f[kLaneElems], most = 0.f;
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-        at[p] = piece_at<FLAT>(first, p * kBlock + threadIdx.x, rows, d, per_row);
-        load8<FLAT>(x + at[p].at, at[p].n, e[p]);
+    for (int j = 0; j < kLaneElems; ++j) {
+        f[j] = (float)e[j];
+        most = fmaxf(most, finite_magnitude(f[j]));
     }
+    const int b = scale_byte(lanes_max(most));
+    if (at.n <= 0) return;
+    const float inv = __uint_as_float((uint32_t)(254 - b) << 23), limit = b == top_byte<T>() ? 240.f : 448.f;
+    if (threadIdx.x % kLanes == 0) scale[at.block] = (uint8_t)b;
+    float v[kLaneElems];
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-        float f[kLaneElems], most = 0.f;
+    for (int j = 0; j < kLaneElems; ++j) v[j] = fmaf(f[j], 0.f, __builtin_amdgcn_fmed3f(f[j] * inv, -limit, limit));
+    uint32_t q[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) {
-            f[j] = (float)e[p][j];
-            most = fmaxf(most, finite_magnitude(f[j]));
-        }
-        const int b = scale_byte(lanes_max(most));
-        if (at[p].n <= 0) continue;
-        const float inv = __uint_as_float((uint32_t)(254 - b) << 23), limit = b == top_byte<T>() ? 240.f : 448.f;
-        if (threadIdx.x % kLanes == 0) scale[at[p].block] = (uint8_t)b;
-        uint32_t q[2] = {0, 0};
-        float v[kLaneElems];
+    for (int h = 0; h < 2; ++h) {
+        q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
+        q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], q[h], true);
+    }
+    store8<FLAT>(held + at.at, at.n, __builtin_bit_cast(Bytes8, q).byte);
+    if (y) {
 #pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) v[j] = fmaf(f[j], 0.f, __builtin_amdgcn_fmed3f(f[j] * inv, -limit, limit));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
-            q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], q[h], true);
-        }
-        store8<FLAT>(held + at[p].at, at[p].n, __builtin_bit_cast(Bytes8, q).byte);
-        if (y) {
-#pragma unroll
-            for (int j = 0; j < kLaneElems; ++j) e[p][j] = (T)act_value<ACT>(f[j]);
-            store8<FLAT>(y + at[p].at, at[p].n, e[p]);
-        }
+        for (int j = 0; j < kLaneElems; ++j) e[j] = (T)act_value<ACT>(f[j]);
+        store8<FLAT>(y + at.at, at.n, e);
     }
 }
 
@@ -156,42 +169,32 @@ __global__ __launch_bounds__(kBlock) void ckpt_bwd_kernel(const T *grad, const u
                                                           const uint8_t *__restrict__ scale, T *grad_x, T *__restrict__ mid,
                                                           const int32_t *__restrict__ table, int64_t rows, int d, int per_row) {
     rows = live_rows(table, rows);
-    const int64_t first = (int64_t)blockIdx.x * (kBlock * kPieces);
+    const int64_t first = (int64_t)blockIdx.x * kBlock;
     if (first >= rows * per_row) return;
-    T g[kPieces][kLaneElems];
-    uint8_t q[kPieces][kLaneElems];
-    uint32_t b[kPieces];
-    Piece at[kPieces];
+    const Piece at = piece_at<FLAT>(first, rows, d, per_row);
+    T g[kLaneElems], m[kLaneElems];
+    uint8_t q[kLaneElems];
+    load8<FLAT>(held + at.at, at.n, at.inside, q);
+    const float s = __uint_as_float((uint32_t)(at.n > 0 ? scale[at.block] : 0) << 23);
+    if (grad) load8<FLAT>(grad + at.at, at.n, at.inside, g);
+    const uint2 w = __builtin_bit_cast(uint2, q);
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-        at[p] = piece_at<FLAT>(first, p * kBlock + threadIdx.x, rows, d, per_row);
-        load8<FLAT>(held + at[p].at, at[p].n, q[p]);
-        b[p] = at[p].n > 0 ? scale[at[p].block] : 0;
-        if (grad) load8<FLAT>(grad + at[p].at, at[p].n, g[p]);
-    }
+    for (int h = 0; h < 2; ++h) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(h ? w.y : w.x), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(h ? w.y : w.x), true);
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-        const float s = __uint_as_float(b[p] << 23);
-        const uint2 w = __builtin_bit_cast(uint2, q[p]);
-        T m[kLaneElems];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const auto two = (h & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)(h < 2 ? w.x : w.y), true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)(h < 2 ? w.x : w.y), false);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float value, slope;
-                act_both<ACT>(two[i] * s, value, slope);
-                m[2 * h + i] = (T)value;
-                if (grad) g[p][2 * h + i] = (T)((float)g[p][2 * h + i] * slope);
-            }
+        for (int i = 0; i < 4; ++i) {
+            float value, slope;
+            act_both<ACT>((i < 2 ? lo[i & 1] : hi[i & 1]) * s, value, slope);
+            m[4 * h + i] = (T)value;
+            if (grad) g[4 * h + i] = (T)((float)g[4 * h + i] * slope);
         }
-        if (grad) store8<FLAT>(grad_x + at[p].at, at[p].n, g[p]);
-        if (mid) store8<FLAT>(mid + at[p].at, at[p].n, m);
     }
+    if (grad) store8<FLAT>(grad_x + at.at, at.n, g);
+    if (mid) store8<FLAT>(mid + at.at, at.n, m);
 }
 
 int per_row(int64_t d) { return (int)(ceil_div(d, kScaleElems) * kLanes); }   // pieces
-int64_t n_blocks(int64_t rows, int64_t d) { return ceil_div(rows * per_row(d), kBlock * kPieces); }
+int64_t n_blocks(int64_t rows, int64_t d) { return ceil_div(rows * per_row(d), kBlock); }
 
 int check(const char *who, int64_t rows, int64_t d, int dtype, int activation) {
     FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who,
