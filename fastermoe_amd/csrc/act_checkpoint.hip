@@ -17,6 +17,7 @@
 #include "common.hpp"
 #include "gelu_terms.hpp"
 #include "grouped_gemm.hpp"
+#include "lane_elems.hpp"
 #include "wave_piece.hpp"
 
 #include <type_traits>
@@ -44,41 +45,6 @@ template <int ACT> __device__ __forceinline__ void act_both(float x, float &valu
     } else {
         value = x;
         slope = x == x ? 1.f : x;
-    }
-}
-
-// Eight elements at p, wherever it lies; WHOLE: or none.  Otherwise n may be less than eight: what is behind them (`inside`: the memory
-// there still is the tensor's) is read and made zeros.
-template <bool WHOLE, typename T> __device__ __forceinline__ void load8(const T *p, int n, bool inside, T (&e)[kLaneElems]) {
-    if (WHOLE ? n > 0 : n >= kLaneElems || (n > 0 && inside)) {
-        __builtin_memcpy(e, p, sizeof(e));
-        if (!WHOLE) {
-#pragma unroll
-            for (int j = 1; j < kLaneElems; ++j) e[j] = j < n ? e[j] : T{};
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) e[j] = !WHOLE && j < n ? p[j] : T{};
-    }
-}
-// The first n of them: four, two and one at a time, out of registers (arrays of elements chosen by n would go through LDS)
-template <int WORDS> struct Words { uint32_t w[WORDS]; };
-template <bool WHOLE, typename T> __device__ __forceinline__ void store8(T *p, int n, const T (&e)[kLaneElems]) {
-    if (WHOLE ? n > 0 : n >= kLaneElems) {
-        __builtin_memcpy(p, e, sizeof(e));
-    } else if (!WHOLE && n > 0) {
-        constexpr int kHalf = (int)sizeof(T);          // words of four elements
-        Words<2 * kHalf> all;
-        __builtin_memcpy(&all, e, sizeof(e));
-        Words<kHalf> four;
-        const uint32_t past4 = n & 4 ? ~0u : 0u, past2 = n & 2 ? ~0u : 0u;
-        if (n & 4) __builtin_memcpy(p, &all, 4 * sizeof(T));
-#pragma unroll
-        for (int j = 0; j < kHalf; ++j) four.w[j] = (all.w[kHalf + j] & past4) | (all.w[j] & ~past4);
-        p += n & 4;
-        if (n & 2) __builtin_memcpy(p, &four, 2 * sizeof(T));
-        const uint32_t one = ((kHalf == 1 ? four.w[0] >> 16 : four.w[kHalf / 2]) & past2) | (four.w[0] & ~past2);
-        if (n & 1) __builtin_memcpy(p + (n & 2), &one, sizeof(T));
     }
 }
 
@@ -136,7 +102,7 @@ __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint
     if (first >= rows * per_row) return;
     const Piece at = piece_at<FLAT>(first, rows, d, per_row);
     T e[kLaneElems];
-    load8<FLAT>(x + at.at, at.n, at.inside, e);
+    load_elems<FLAT>(x + at.at, at.n, at.inside, e);
     float f[kLaneElems], most = 0.f;
 #pragma unroll
     for (int j = 0; j < kLaneElems; ++j) {
@@ -156,11 +122,11 @@ __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint
         q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
         q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], q[h], true);
     }
-    store8<FLAT>(held + at.at, at.n, __builtin_bit_cast(Bytes8, q).byte);
+    store_elems<FLAT>(held + at.at, at.n, __builtin_bit_cast(Bytes8, q).byte);
     if (y) {
 #pragma unroll
         for (int j = 0; j < kLaneElems; ++j) e[j] = (T)act_value<ACT>(f[j]);
-        store8<FLAT>(y + at.at, at.n, e);
+        store_elems<FLAT>(y + at.at, at.n, e);
     }
 }
 
@@ -174,9 +140,9 @@ __global__ __launch_bounds__(kBlock) void ckpt_bwd_kernel(const T *grad, const u
     const Piece at = piece_at<FLAT>(first, rows, d, per_row);
     T g[kLaneElems], m[kLaneElems];
     uint8_t q[kLaneElems];
-    load8<FLAT>(held + at.at, at.n, at.inside, q);
+    load_elems<FLAT>(held + at.at, at.n, at.inside, q);
     const float s = __uint_as_float((uint32_t)(at.n > 0 ? scale[at.block] : 0) << 23);
-    if (grad) load8<FLAT>(grad + at.at, at.n, at.inside, g);
+    if (grad) load_elems<FLAT>(grad + at.at, at.n, at.inside, g);
     const uint2 w = __builtin_bit_cast(uint2, q);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -189,8 +155,8 @@ __global__ __launch_bounds__(kBlock) void ckpt_bwd_kernel(const T *grad, const u
             if (grad) g[4 * h + i] = (T)((float)g[4 * h + i] * slope);
         }
     }
-    if (grad) store8<FLAT>(grad_x + at.at, at.n, g);
-    if (mid) store8<FLAT>(mid + at.at, at.n, m);
+    if (grad) store_elems<FLAT>(grad_x + at.at, at.n, g);
+    if (mid) store_elems<FLAT>(mid + at.at, at.n, m);
 }
 
 int per_row(int64_t d) { return (int)(ceil_div(d, kScaleElems) * kLanes); }   // pieces
