@@ -51,12 +51,14 @@ template <bool WHOLE, int N, typename T> __device__ __forceinline__ void store_e
     }
 }
 
-// The same for 16 bytes as they lie in memory (elements of a 16-bit type in a register each would take twice the registers)
-template <typename T> __device__ __forceinline__ u32x4 load_vec(const T *p, int n, bool inside) {
+typedef uint32_t AnyVec __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes wherever they begin
+// The same for 16 bytes as they lie in memory (elements of a 16-bit type in a register each would take twice the registers); ONCE: not to
+// be kept in the caches
+template <bool ONCE, typename T> __device__ __forceinline__ u32x4 load_vec(const T *p, int n, bool inside) {
     constexpr int N = Vec<T>::N;
     u32x4 v = {0, 0, 0, 0};
     if (n >= N || (n > 0 && inside)) {
-        __builtin_memcpy(&v, p, 16);
+        v = ONCE ? __builtin_nontemporal_load((const AnyVec *)p) : *(const AnyVec *)p;
         if (n < N) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -72,7 +74,11 @@ template <typename T> __device__ __forceinline__ u32x4 load_vec(const T *p, int 
     }
     return v;
 }
-template <typename T> __device__ __forceinline__ void store_vec(T *p, int n, const u32x4 &v) {
+template <bool ONCE, typename T> __device__ __forceinline__ void store_vec(T *p, int n, const u32x4 &v) {
+    if (ONCE && n >= Vec<T>::N) {
+        __builtin_nontemporal_store(v, (AnyVec *)p);
+        return;
+    }
     T e[Vec<T>::N];
     __builtin_memcpy(e, &v, 16);
     store_elems<false>(p, n, e);

@@ -7,7 +7,17 @@
 // Statistics, sums and everything between the loads and the one rounding at a store are float32.
 //
 // A row lies in the registers of G lanes, V vectors of 16 bytes to each, between its one load and its one store: G x V is the smallest that
-// holds it (held_forward, held_backward).  Longer rows than any holds are read again for every sum (long_* kernels).
+// holds it (held_forward, held_backward).  Rows longer than any holds are read again for every sum (long_* kernels: 1000 bfloat16 rows of 40000 take
+// 208 us and 317).  Bound by memory (TB/s of what has to move; a large copy on the same card 5.0):
+//   rows x features             forward          backward            of it without the parameters' gradients
+//   16384 x 4096 bf16, residual   94 us  5.7        91 us  5.9         84 us  6.4
+//   32768 x 4096 bf16            101     5.3       143     5.6        136     5.9
+//   16384 x 2048 f32, residual    91     5.9        89     6.0         85     6.3
+//   32768 x 1024 bf16             27     4.9        41     4.9         36     5.6
+//   32768 x 500 bf16, any start   18     3.7        27     3.6         22     4.5
+//   509 x 4096 f16, residual      6.1               13                5.2
+//   64 x 4096 bf16, residual      3.8               8.8               4.0
+// (The first with a row read again for every sum and the parameters' gradients in a pass of their own: 358 and 431 us.)
 #include "common.hpp"
 #include "lane_elems.hpp"
 
@@ -20,6 +30,9 @@ constexpr int kBlock = 256;
 constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kBwdBlock = 1024;      // of the backward over rows in registers
 constexpr int kBwdMostBlocks = 256;  // and its workgroups at most, each of which leaves sums over its rows
+constexpr int64_t kPartBytes = 4 << 20;
+constexpr int64_t kCacheBytes = 256 << 20;   // of the memory-side cache
+constexpr int kFewRows = 2048;
 
 // ---- sums over the G lanes of a row, the same in all of them ------------------------------
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -38,7 +51,7 @@ template <int G> __device__ __forceinline__ float lanes_sum(float v) {   // G <=
     }
     return v;
 }
-// NS sums; rows of more than one wave meet in scratch [waves of the workgroup][NS], which the next call must not be handed
+// NS sums; rows of more than one wave meet in scratch [waves of the workgroup][NS], which the next call must not be handed again
 template <int G, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS], float (*scratch)[NS]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) v[i] = lanes_sum<(G < kWave ? G : kWave)>(v[i]);
@@ -60,37 +73,72 @@ template <int G, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS]
     }
 }
 
-// N parameters from column c on; `none` where there are no parameters
-template <typename P, int N> __device__ __forceinline__ void load_params(const P *p, int c, int d, float none, float (&f)[N]) {
+// weight or bias: of the rows' type T or float32 (kind: what the pointer is to; none where it is null)
+struct Param { const void *p; bool f32; };
+// N of them from column c on; `none` where there are none.  WHOLE: d is whole vectors.
+template <typename T, int N, bool WHOLE> __device__ __forceinline__ void load_params(const Param &p, int c, int d, float none, float (&f)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = none;
-    if (!p) return;
+    if (!p.p || (WHOLE && c >= d)) return;
+    auto vec = [&](auto *at, int n) { return WHOLE ? (u32x4) * (const AnyVec *)at : load_vec<false>(at, n, false); };
+    float t[8];
+    if (sizeof(T) == 2 && !p.f32) {
+        Vec<T>::unpack(vec((const T *)p.p + c, d - c), t);
 #pragma unroll
-    for (int k = 0; k < N; k += Vec<P>::N) {
-        float t[8];
-        Vec<P>::unpack(load_vec(p + c + k, d - c - k, false), t);
+        for (int i = 0; i < N; ++i) f[i] = t[i];
+    } else {
 #pragma unroll
-        for (int i = 0; i < Vec<P>::N && k + i < N; ++i) f[k + i] = t[i];
+        for (int k = 0; k < N; k += 4) {
+            Vec<float>::unpack(vec((const float *)p.p + c + k, d - c - k), t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[k + i] = t[i];
+        }
+    }
+}
+
+// The lane's vector of row `row` of rows that begin `stride` elements apart, zeros where it has none.  WHOLE: a row is whole vectors.
+template <typename T, bool WHOLE, bool ONCE>
+__device__ __forceinline__ u32x4 load_row(const T *p, int64_t stride, int64_t row, int64_t rows, int c, int d) {
+    constexpr int N = Vec<T>::N;
+    const bool live = row < rows;
+    if constexpr (WHOLE) {
+        u32x4 v = {0, 0, 0, 0};
+        if (live && c < d) {
+            const AnyVec *at = (const AnyVec *)(p + row * stride + c);
+            v = ONCE ? __builtin_nontemporal_load(at) : *at;
+        }
+        return v;
+    } else {
+        return load_vec<ONCE>(p + row * stride + c, live ? d - c : 0, (row - rows + 1) * stride + c + N <= d);
+    }
+}
+template <typename T, bool WHOLE, bool ONCE> __device__ __forceinline__ void store_row(T *p, int c, int d, const u32x4 &v) {
+    if constexpr (WHOLE) {
+        if (c < d) {
+            if (ONCE) __builtin_nontemporal_store(v, (AnyVec *)(p + c));
+            else *(AnyVec *)(p + c) = v;
+        }
+    } else {
+        store_vec<ONCE>(p + c, d - c, v);
     }
 }
 
 // ---- forward over rows in registers ------------------------------------------------------
-template <typename T, typename P, int G, int V>
+template <typename T, int G, int V, bool WHOLE>
 __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const T *__restrict__ x, int64_t x_stride, const T *__restrict__ r,
-                                                                           int64_t r_stride, const P *__restrict__ w, const P *__restrict__ b,
-                                                                           T *__restrict__ sum, T *__restrict__ y, float *__restrict__ mean,
+                                                                           int64_t r_stride, Param w, Param b, T *__restrict__ sum,
+                                                                           T *__restrict__ y, float *__restrict__ mean,
                                                                            float *__restrict__ rstd, int64_t rows, int d, float eps) {
     constexpr int N = Vec<T>::N, kRows = (G > kBlock ? G : kBlock) / G;
     __shared__ float scratch[2][kRows * G / kWave][1];
     const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
     const int lane = threadIdx.x % G;
-    const bool live = row < rows;
     u32x4 e[V], re[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * G + lane) * N, n = live ? d - c : 0;
-        e[v] = load_vec(x + row * x_stride + c, n, (row - rows + 1) * x_stride + c + N <= d);
-        if (r) re[v] = load_vec(r + row * r_stride + c, n, (row - rows + 1) * r_stride + c + N <= d);
+        const int c = (v * G + lane) * N;
+        e[v] = load_row<T, WHOLE, false>(x, x_stride, row, rows, c, d);
+        if (r) re[v] = load_row<T, WHOLE, false>(r, r_stride, row, rows, c, d);
     }
     float f[V][8], s[1] = {0.f};
 #pragma unroll
@@ -119,17 +167,17 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
         }
     row_sums<G>(s, scratch[1]);
     const float rs = 1.f / sqrtf(s[0] / (float)d + eps);
-    if (!live) return;
+    if (row >= rows) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * G + lane) * N, n = d - c;
+        const int c = (v * G + lane) * N;
         float wf[N], bf[N], out[8];
-        load_params(w, c, d, 1.f, wf);
-        load_params(b, c, d, 0.f, bf);
+        load_params<T, N, WHOLE>(w, c, d, 1.f, wf);
+        load_params<T, N, WHOLE>(b, c, d, 0.f, bf);
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = f[v][i] * rs * wf[i] + bf[i];
-        store_vec(y + row * d + c, n, Vec<T>::pack(out));
-        if (sum) store_vec(sum + row * d + c, n, e[v]);
+        store_row<T, WHOLE, false>(y + row * d, c, d, Vec<T>::pack(out));
+        if (sum) store_row<T, WHOLE, false>(sum + row * d, c, d, e[v]);
     }
     if (mean && lane == 0) {
         mean[row] = m;
@@ -137,56 +185,75 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
     }
 }
 
+// The lane's vector of a row to come.  WHOLE: loaded whatever it is, with neither a branch around the load nor a look at what it brought, either of
+// which would have the sums of the row before wait for it; the row is one that there is, and lanes behind its end take its beginning.
+template <typename T, bool WHOLE, bool ONCE>
+__device__ __forceinline__ u32x4 load_ahead(const T *p, int64_t stride, int64_t row, int64_t rows, int c, int d) {
+    if constexpr (WHOLE) {
+        const AnyVec *at = (const AnyVec *)(p + row * stride + (c < d ? c : 0));
+        return ONCE ? (u32x4)__builtin_nontemporal_load(at) : (u32x4)*at;
+    } else {
+        return load_row<T, WHOLE, ONCE>(p, stride, row, rows, c, d);
+    }
+}
+
 // ---- backward over rows in registers -----------------------------------------------------
-// A workgroup takes kRows rows at a time and every gridDim-th such set, with the next set's loads on their way.  The lanes keep the sums of
-// grad_y h and grad_y of their columns over all of them; at the end the sets' lanes meet in LDS and part[workgroup] gets 2 d sums.
+// A workgroup takes kRows rows at a time and every gridDim-th such set, with the next set's loads on their way (16384 x 4096: 104 us where a branch
+// or a select made the sums wait for them).  The lanes keep the sums of grad_y h and grad_y of their columns over all of them; at the end the
+// lanes of one column meet in LDS and part[workgroup] gets 2 d sums.  One workgroup of 1024 to a compute unit: two of 512 leave twice the parts (4096 x 8192:
+// 59 us against 68).  One vector to a lane: with two the next set's registers no longer fit beside this one's.
 template <int V> struct RowData {
     u32x4 g[V], x[V], gs[V];
     float mean, rstd;
 };
-template <typename T, typename P, int G, int V>
+template <typename T, int G, int V, bool WHOLE, bool ONCE, bool SUM>
 __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict__ gy, int64_t gy_stride, const T *__restrict__ gs,
                                                              int64_t gs_stride, const T *__restrict__ x, int64_t x_stride,
-                                                             const float *__restrict__ mean, const float *__restrict__ rstd,
-                                                             const P *__restrict__ w, T *__restrict__ gx, float *__restrict__ part,
-                                                             int64_t rows, int d) {
+                                                             const float *__restrict__ mean, const float *__restrict__ rstd, Param w,
+                                                             T *__restrict__ gx, float *__restrict__ part, int64_t rows, int d) {
     constexpr int N = Vec<T>::N, kRows = kBwdBlock / G;
     constexpr bool kAhead = V == 1 || V * N <= 8;
     __shared__ float scratch[2][kBwdBlock / kWave][2];
     __shared__ float sums[kRows > 1 ? kBwdBlock * V * N : 1];
     const int lane = threadIdx.x % G, mine = threadIdx.x / G;
+    const bool has_sum = WHOLE ? SUM : gs != nullptr;
     auto load = [&](int64_t row, RowData<V> &a) {
-        const bool live = row < rows;
-        const int64_t back = row - rows + 1;
+        if constexpr (WHOLE) row = row < rows ? row : rows - 1;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * G + lane) * N, n = live ? d - c : 0;
-            a.g[v] = load_vec(gy + row * gy_stride + c, n, back * gy_stride + c + N <= d);
-            a.x[v] = load_vec(x + row * x_stride + c, n, back * x_stride + c + N <= d);
-            if (gs) a.gs[v] = load_vec(gs + row * gs_stride + c, n, back * gs_stride + c + N <= d);
+            const int c = (v * G + lane) * N;
+            if (has_sum) a.gs[v] = load_ahead<T, WHOLE, ONCE>(gs, gs_stride, row, rows, c, d);
+            a.g[v] = load_ahead<T, WHOLE, ONCE>(gy, gy_stride, row, rows, c, d);
+            a.x[v] = load_ahead<T, WHOLE, ONCE>(x, x_stride, row, rows, c, d);
         }
-        a.mean = live ? mean[row] : 0.f;
-        a.rstd = live ? rstd[row] : 0.f;
+        const int64_t at = row < rows ? row : rows - 1;
+        a.mean = mean[at];
+        a.rstd = rstd[at];
+    };
+    // zeros for what load_ahead was not to load
+    auto have = [&](int64_t row, RowData<V> &a) {
+        if constexpr (!WHOLE) return;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const bool in = row < rows && (v * G + lane) * N < d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a.g[v][j] = in ? a.g[v][j] : 0;
+                a.x[v][j] = in ? a.x[v][j] : 0;
+            }
+        }
     };
     float wf[V][N], sw[V][N], sb[V][N];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * G + lane) * N;
-        load_params(w, c, d, 1.f, wf[v]);
+        load_params<T, N, WHOLE>(w, (v * G + lane) * N, d, 1.f, wf[v]);
 #pragma unroll
         for (int i = 0; i < N; ++i) sw[v][i] = sb[v][i] = 0.f;
     }
-    const int64_t step = (int64_t)gridDim.x * kRows;
-    RowData<V> a, next;
-    int64_t row = (int64_t)blockIdx.x * kRows + mine;
-    if (kAhead) load(row, a);
     int turn = 0;
-    for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step, turn ^= 1) {
-        if (kAhead) {
-            if (first + step < rows) load(row + step, next);
-        } else {
-            load(row, a);
-        }
+    // one set's rows: sums, the gradient of the rows, and what they add to the parameters'
+    auto use = [&](int64_t row, RowData<V> &a) {
+        have(row, a);
         float c12[2] = {0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -204,6 +271,7 @@ __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict
             }
         }
         row_sums<G>(c12, scratch[turn]);
+        turn ^= 1;
         if (gx && row < rows) {
             const float c1 = c12[0] / (float)d, c2 = c12[1] / (float)d;
 #pragma unroll
@@ -212,17 +280,39 @@ __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict
                 float g[8], h[8], t[8];
                 Vec<T>::unpack(a.g[v], g);
                 Vec<T>::unpack(a.x[v], h);
-                if (gs) Vec<T>::unpack(a.gs[v], t);
+                    if (has_sum) Vec<T>::unpack(a.gs[v], t);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     h[i] = (h[i] - a.mean) * a.rstd;
                     g[i] = a.rstd * (g[i] * wf[v][i] - c1 - h[i] * c2);
-                    if (gs) g[i] += t[i];
+                    if (has_sum) g[i] += t[i];
                 }
-                store_vec(gx + row * d + c, d - c, Vec<T>::pack(g));
+                store_row<T, WHOLE, ONCE>(gx + row * d, c, d, Vec<T>::pack(g));
             }
         }
-        if (kAhead) a = next;
+    };
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t first = (int64_t)blockIdx.x * kRows;
+    RowData<V> a;
+    if constexpr (kAhead) {
+        // (two sets' registers that change places, not one copied over the other, which would wait for its loads)
+        RowData<V> b;
+        load(first + mine, a);
+        while (true) {
+            load(first + step + mine, b);
+            use(first + mine, a);
+            first += step;
+            if (first >= rows) break;
+            load(first + step + mine, a);
+            use(first + mine, b);
+            first += step;
+            if (first >= rows) break;
+        }
+    } else {
+        for (; first < rows; first += step) {
+            load(first + mine, a);
+            use(first + mine, a);
+        }
     }
     if (!part) return;
     float *out = part + (int64_t)blockIdx.x * 2 * d;
@@ -333,10 +423,10 @@ __global__ __launch_bounds__(kBlock) void long_param_kernel(const T *__restrict_
     part[(int64_t)blockIdx.y * 2 * d + d + c] = sb;
 }
 
-// grad_w and grad_b out of the parts, in their order: 32 columns to a workgroup, eight ranges of parts side by side
-constexpr int kSumCols = 32, kSumRanges = kBlock / kSumCols;
+// grad_w and grad_b out of the parts, in their order: 32 columns to a workgroup, 16 ranges of parts side by side
+constexpr int kSumCols = 32, kSumRanges = 16, kSumBlock = kSumCols * kSumRanges;
 template <typename P>
-__global__ __launch_bounds__(kBlock) void norm_param_sum_kernel(const float *__restrict__ part, int n_parts, P *__restrict__ gw,
+__global__ __launch_bounds__(kSumBlock) void norm_param_sum_kernel(const float *__restrict__ part, int n_parts, P *__restrict__ gw,
                                                                 P *__restrict__ gb, int64_t d) {
     __shared__ float sums[kSumRanges][kSumCols];
     const int col = threadIdx.x % kSumCols, range = threadIdx.x / kSumCols;
@@ -362,9 +452,14 @@ template <int N, int G, int V, typename F> bool held_by(int64_t d, F &&f) {
     f(std::integral_constant<int, G>{}, std::integral_constant<int, V>{});
     return true;
 }
-template <int N, typename F> bool held_forward(int64_t d, F &&f) {
-    return held_by<N, 8, 1>(d, f) || held_by<N, 32, 1>(d, f) || held_by<N, 64, 1>(d, f) || held_by<N, 64, 2>(d, f) || held_by<N, 256, 1>(d, f) ||
-           held_by<N, 256, 2>(d, f) || held_by<N, 1024, 1>(d, f) || held_by<N, 1024, 2>(d, f) || held_by<N, 1024, 4>(d, f);
+// one_each: one vector to a lane where two would do too, for rows with a residual (two loads in flight already: 16384 x 4096 bfloat16 93 us against 99) and
+// launches of fewer than kFewRows rows (64 x 4096: 4.0 against 4.4); else two (32768 x 4096: 102 us against 122; 32768 x 1024: 27 against 31).
+template <int N, typename F> bool held_forward(int64_t d, bool one_each, F &&f) {
+    if (held_by<N, 8, 1>(d, f) || held_by<N, 32, 1>(d, f) || held_by<N, 64, 1>(d, f)) return true;
+    if (one_each ? held_by<N, 128, 1>(d, f) || held_by<N, 256, 1>(d, f) || held_by<N, 512, 1>(d, f)
+                 : held_by<N, 64, 2>(d, f) || held_by<N, 128, 2>(d, f) || held_by<N, 256, 2>(d, f))
+        return true;
+    return held_by<N, 512, 2>(d, f) || held_by<N, 1024, 2>(d, f) || held_by<N, 1024, 4>(d, f);
 }
 template <int N, typename F> bool held_backward(int64_t d, F &&f) {
     if (held_by<N, 8, 1>(d, f) || held_by<N, 32, 1>(d, f) || held_by<N, 64, 1>(d, f) || held_by<N, 128, 1>(d, f) || held_by<N, 256, 1>(d, f) ||
@@ -411,11 +506,13 @@ extern "C" int fmoe_layer_norm_forward(const void *x, int64_t x_stride, const vo
     with_types(dtype, param_dtype, [&](auto t, auto p) {
         using T = decltype(t);
         using P = decltype(p);
-        const bool held = held_forward<Vec<T>::N>(row_elems, [&](auto g, auto v) {
+        const bool whole = row_elems % Vec<T>::N == 0, param_f32 = std::is_same<P, float>::value;
+        const bool held = held_forward<Vec<T>::N>(row_elems, residual || rows < kFewRows, [&](auto g, auto v) {
             constexpr int kThreads = g.value > kBlock ? g.value : kBlock;
-            norm_fwd_kernel<T, P, g.value, v.value><<<(int)ceil_div(rows, kThreads / g.value), kThreads, 0, st>>>(
-                (const T *)x, x_stride, (const T *)residual, residual_stride, (const P *)weight, (const P *)bias, (T *)sum, (T *)y, mean, rstd,
-                rows, (int)row_elems, (float)eps);
+            (whole ? norm_fwd_kernel<T, g.value, v.value, true> : norm_fwd_kernel<T, g.value, v.value, false>)<<<
+                (int)ceil_div(rows, kThreads / g.value), kThreads, 0, st>>>(
+                (const T *)x, x_stride, (const T *)residual, residual_stride, Param{weight, param_f32}, Param{bias, param_f32}, (T *)sum, (T *)y,
+                mean, rstd, rows, (int)row_elems, (float)eps);
         });
         if (!held)
             long_fwd_kernel<T, P><<<(int)rows, kBlock, 0, st>>>((const T *)x, x_stride, (const T *)residual, residual_stride,
@@ -448,17 +545,26 @@ extern "C" int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_strid
     with_types(dtype, param_dtype, [&](auto t, auto p) {
         using T = decltype(t);
         using P = decltype(p);
+        // (rows that the memory-side cache could not hold go past the caches: nobody reads them again, 16384 x 4096 103 us through them, 95 past;
+        // smaller launches lose by it: 4096 x 8192 53 and 55; 65536 x 512 50 and 54.  Without rows there is nothing to load from, and the parameters' gradients are sums of no parts)
         int parts = 0;
-        const bool held = held_backward<Vec<T>::N>(row_elems, [&](auto g, auto v) {
-            const int64_t sets = ceil_div(rows < 1 ? 1 : rows, kBwdBlock / g.value);
-            parts = (int)(sets < kBwdMostBlocks ? sets : kBwdMostBlocks);
-            norm_bwd_kernel<T, P, g.value, v.value><<<parts, kBwdBlock, 0, st>>>(
-                (const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride, (const T *)x, x_stride, mean, rstd, (const P *)weight,
-                (T *)grad_x, params ? (float *)workspace : nullptr, rows, (int)row_elems);
+        const bool held = rows == 0 || held_backward<Vec<T>::N>(row_elems, [&](auto g, auto v) {
+            // (one set to a workgroup, unless the workgroups' sums would be more than kPartBytes, then two: 509 x 4096 float16 16.4 us with
+            // 255 workgroups, 13 with 128; 777 x 1302, whose 195 leave 2 MB, 12.1 and 14)
+            const int64_t sets = ceil_div(rows, kBwdBlock / g.value);
+            const int64_t blocks = params && sets * 8 * row_elems > kPartBytes ? ceil_div(sets, 2) : sets;
+            parts = (int)(blocks < kBwdMostBlocks ? blocks : kBwdMostBlocks);
+            const bool whole = row_elems % Vec<T>::N == 0, once = rows * row_elems * (int64_t)sizeof(T) * (grad_sum ? 4 : 3) > kCacheBytes;
+            auto kernel = !whole ? norm_bwd_kernel<T, g.value, v.value, false, false, false>
+                          : once ? (grad_sum ? norm_bwd_kernel<T, g.value, v.value, true, true, true> : norm_bwd_kernel<T, g.value, v.value, true, true, false>)
+                                 : (grad_sum ? norm_bwd_kernel<T, g.value, v.value, true, false, true> : norm_bwd_kernel<T, g.value, v.value, true, false, false>);
+            kernel<<<parts, kBwdBlock, 0, st>>>((const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride, (const T *)x, x_stride, mean,
+                                           rstd, Param{weight, std::is_same<P, float>::value}, (T *)grad_x,
+                                           params ? (float *)workspace : nullptr, rows, (int)row_elems);
         });
         if (!held) {
             parts = n_parts(rows) < kLongParts ? n_parts(rows) : kLongParts;
-            if (grad_x && rows > 0)
+            if (grad_x)
                 long_bwd_kernel<T, P><<<(int)rows, kBlock, 0, st>>>((const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride,
                                                                     (const T *)x, x_stride, mean, rstd, (const P *)weight, (T *)grad_x,
                                                                     row_elems);
@@ -467,7 +573,7 @@ extern "C" int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_strid
                     (const T *)grad_y, grad_y_stride, (const T *)x, x_stride, mean, rstd, (float *)workspace, rows, row_elems);
         }
         if (params)
-            norm_param_sum_kernel<P><<<(int)ceil_div(2 * row_elems, kSumCols), kBlock, 0, st>>>((const float *)workspace, parts, (P *)grad_weight,
+            norm_param_sum_kernel<P><<<(int)ceil_div(2 * row_elems, kSumCols), kSumBlock, 0, st>>>((const float *)workspace, parts, (P *)grad_weight,
                                                                                                (P *)grad_bias, row_elems);
     });
     FMOE_LAUNCH_CHECK();
