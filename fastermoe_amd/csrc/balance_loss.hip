@@ -6,151 +6,321 @@
 //
 // (The gradient does not feel a constant added to u, as the probabilities of a token add up to one: with the counts less
 // their mean, taken before anything is rounded, no two nearly equal numbers are subtracted where the experts are nearly balanced.)
+//
+// L lanes hold a token's logits, V vectors of 16 bytes to each (as many lanes and vectors as the experts need: held_logits), a wave 64 / L tokens; probabilities stay
+// in registers between the one load and the sums over the tokens, which each lane keeps for its experts over all the tokens of its workgroup's range.
 #include "common.hpp"
+#include "lane_elems.hpp"
+
+#include <type_traits>
 
 namespace fmoe {
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kWavesPerBlock = kBlock / kWave;
 constexpr int kMostExperts = 8192;
-constexpr int kMostParts = 256;
+constexpr int kMostParts = 256;      // workgroups of the forward, each of which leaves sums over its tokens
+constexpr int kBwdBlock = 256;
+constexpr int kOneRound = 4;
+constexpr int kSumCols = 32, kSumRanges = 16, kSumBlock = kSumCols * kSumRanges;
+constexpr int waves_of(int v) { return v <= 2 ? 16 : 4; }                // of a workgroup of the forward
+constexpr int ahead_of(int v) { return v == 1 ? 4 : v == 2 ? 2 : 1; }    // tokens in flight per lane
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// op over L adjacent lanes, the same in all of them
+template <int L, typename F> __device__ __forceinline__ float over_lanes(float v, F &&op) {
+    if (L > 1) v = op(v, dpp<0xb1>(v));      // quad_perm 1 0 3 2
+    if (L > 2) v = op(v, dpp<0x4e>(v));      // quad_perm 2 3 0 1
+    if (L > 4) v = op(v, dpp<0x141>(v));     // row_half_mirror
+    if (L > 8) v = op(v, dpp<0x140>(v));     // row_mirror
+    if (L == 32) v = op(v, __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401f)));   // the lane 16 away
+    if (L == 64) {
+        auto lane = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
+        v = op(op(lane(0), lane(16)), op(lane(32), lane(48)));
+    }
     return v;
 }
-__device__ __forceinline__ float wave_sum(float v) {
+
+// A token's logits as its lanes hold them.
+template <typename T, int L, int V, bool WHOLE> struct Logits {
+    static constexpr int N = Vec<T>::N;
+    u32x4 raw[V];
+    // token t of n (WHOLE, experts in whole vectors: of the last one where there is none, and nothing looks at what comes, so that loads run ahead)
+    __device__ __forceinline__ void load(const T *logits, int64_t t, int64_t n, int n_expert) {
+        const int lane = threadIdx.x % L;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int c = (v * L + lane) * N;
+            if constexpr (WHOLE) raw[v] = *(const AnyVec *)(logits + (t < n ? t : n - 1) * n_expert + (c < n_expert ? c : 0));
+            else raw[v] = load_vec<false>(logits + t * n_expert + c, t < n ? n_expert - c : 0, t * n_expert + c + N <= n * n_expert);
+        }
+    }
+    // p <- exp(logit - largest), 0 behind the experts; returns the reciprocal of their sum, 0 for a token that is not `counted` or whose logits are all
+    // minus infinity (it has no probabilities)
+    __device__ __forceinline__ float softmax(float (&p)[V][N], bool counted, int n_expert) const {
+        const int lane = threadIdx.x % L;
+        float most = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float f[8];
+            Vec<T>::unpack(raw[v], f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                p[v][i] = counted && (v * L + lane) * N + i < n_expert ? f[i] : -INFINITY;
+                most = fmaxf(most, p[v][i]);
+            }
+        }
+        most = over_lanes<L>(most, [](float a, float b) { return fmaxf(a, b); });
+        if (most == -INFINITY) most = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                p[v][i] = __expf(p[v][i] - most);
+                sum += p[v][i];
+            }
+        sum = over_lanes<L>(sum, [](float a, float b) { return a + b; });
+        return sum == 0.f ? 0.f : 1.f / sum;
+    }
+};
+
+// What the forward leaves behind its sums over ranges of tokens, and what becomes of them
+struct Sums {
+    double *loss;       // [columns' workgroups]
+    unsigned *done;     // workgroups of the columns that are through
+    float *prob;        // [parts][experts]
+    int *count;         // [parts][experts]
+    int2 *total;        // [parts]: tokens, slots
+};
+struct Results { int64_t *count; float *prob, *slope, *loss; int per_slot; };
+
+// expert e's results from its sums; returns its part of the loss, before the factor
+__device__ __forceinline__ double finish_expert(const Results &r, int e, int n_expert, double p, long long c, long long tokens, long long slots) {
+    const long long per = r.per_slot ? slots : tokens;
+    const double k = per ? (double)n_expert / ((double)per * (double)per) : 0.0;
+    r.count[e] = c;
+    r.prob[e] = tokens ? (float)(p / (double)tokens) : 0.f;
+    r.slope[e] = (float)(k * ((double)c - (double)slots / n_expert));
+    if (e == 0) r.slope[n_expert] = tokens ? (float)(1.0 / (double)tokens) : 0.f;
+    return k * p * (double)c;
+}
+__device__ __forceinline__ double lane_sum(double v) {
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
     return v;
 }
 
-// The row's largest logit and the reciprocal of the sum of exp(logit - largest), by one wave.  A row of minus infinities has no
-// probabilities: the reciprocal is 0, so that they come out as zeros.
-struct RowTerms { float most, inv; };
-template <typename T> __device__ __forceinline__ RowTerms row_terms(const T *row, int n_expert) {
-    const int lane = threadIdx.x % kWave;
-    float m = -INFINITY, s = 0.f;
-    for (int e = lane; e < n_expert; e += kWave) m = fmaxf(m, (float)row[e]);
-    m = wave_max(m);
-    if (m == -INFINITY) m = 0.f;
-    for (int e = lane; e < n_expert; e += kWave) s += expf((float)row[e] - m);
-    s = wave_sum(s);
-    return RowTerms{m, s == 0.f ? 0.f : 1.f / s};
-}
-
-template <typename T>
-__global__ __launch_bounds__(kBlock) void balance_rows_kernel(const T *__restrict__ logits, const uint8_t *__restrict__ mask,
-                                                              float2 *__restrict__ terms, int64_t n_tokens, int n_expert) {
-    const int64_t t = (int64_t)blockIdx.x * kWavesPerBlock + threadIdx.x / kWave;
-    if (t >= n_tokens) return;
-    RowTerms r{0.f, 0.f};
-    if (!mask || mask[t] == 0) r = row_terms(logits + t * n_expert, n_expert);
-    if (threadIdx.x % kWave == 0) terms[t] = make_float2(r.most, r.inv);
-}
-
-// A range of tokens and 256 experts per workgroup, an expert to each thread
-template <typename T>
-__global__ __launch_bounds__(kBlock) void balance_sum_kernel(const T *__restrict__ logits, const int64_t *__restrict__ idx,
-                                                             const uint8_t *__restrict__ mask, const float2 *__restrict__ terms,
-                                                             float *__restrict__ part_p, int *__restrict__ part_c,
-                                                             int *__restrict__ part_t, int64_t n_tokens, int n_expert, int top_k) {
-    __shared__ int count[kBlock];
-    const int e0 = blockIdx.x * kBlock, e = e0 + threadIdx.x;
-    const int64_t per = (n_tokens + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per, hi = lo + per < n_tokens ? lo + per : n_tokens;
-    count[threadIdx.x] = 0;
+// A range of tokens to each workgroup: the experts' counts from the slots, then the sums of the probabilities.  A launch of one workgroup goes on
+// to the results; otherwise balance_finish_kernel makes them.
+template <typename T, int L, int V, bool WHOLE>
+__global__ __launch_bounds__(waves_of(V) * kWave) void balance_sum_kernel(const T *__restrict__ logits, const int64_t *__restrict__ idx,
+                                                                           const uint8_t *__restrict__ mask, Sums sums, Results results,
+                                                                           int64_t n_tokens, int n_expert, int top_k) {
+    constexpr int N = Vec<T>::N, kWaves = waves_of(V), kThreads = kWaves * kWave, kTokens = kWave / L, kAhead = ahead_of(V);
+    __shared__ union {
+        int count[L * V * N];
+        float prob[kWaves][L * V * N];
+    } lds;
+    __shared__ int total[2];
+    __shared__ double loss[kWaves];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t per = (n_tokens + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < n_tokens ? lo + per : n_tokens;
+    for (int e = threadIdx.x; e < n_expert; e += kThreads) lds.count[e] = 0;
+    if (threadIdx.x < 2) total[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *sums.done = 0;
     __syncthreads();
-    for (int64_t s = lo * top_k + threadIdx.x; s < hi * top_k; s += kBlock) {
-        const int64_t named = idx[s] - e0;
-        if (idx[s] >= 0 && idx[s] < n_expert && named >= 0 && named < kBlock && (!mask || mask[s / top_k] == 0))
-            atomicAdd(&count[named], 1);
-    }
-    float p = 0.f;
-    int tokens = 0;
-    for (int64_t t = lo; t < hi; ++t) {
-        if (mask && mask[t]) continue;
-        ++tokens;
-        const float2 r = terms[t];
-        if (e < n_expert && r.y != 0.f) p += expf((float)logits[t * n_expert + e] - r.x) * r.y;
-    }
-    __syncthreads();
-    if (e < n_expert) {
-        part_p[(int64_t)blockIdx.y * n_expert + e] = p;
-        part_c[(int64_t)blockIdx.y * n_expert + e] = count[threadIdx.x];
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) part_t[blockIdx.y] = tokens;
-}
-
-// One workgroup: the sums over the ranges, what the gradient needs of them (slope [n_expert + 1]) and the loss
-__global__ __launch_bounds__(kBlock) void balance_finish_kernel(const float *__restrict__ part_p, const int *__restrict__ part_c,
-                                                                const int *__restrict__ part_t, int n_parts, int n_expert, int per_slot,
-                                                                int64_t *__restrict__ count, float *__restrict__ prob,
-                                                                float *__restrict__ slope, float *__restrict__ loss) {
-    __shared__ double scratch[kBlock];
-    __shared__ long long slots_lds;
-    if (threadIdx.x == 0) slots_lds = 0;
-    __syncthreads();
-    long long tokens = 0, slots = 0;
-    for (int g = 0; g < n_parts; ++g) tokens += part_t[g];
-    double sum = 0;
-    for (int e = threadIdx.x; e < n_expert; e += kBlock) {
-        long long c = 0;
-        double p = 0;
-        for (int g = 0; g < n_parts; ++g) {
-            c += part_c[(int64_t)g * n_expert + e];
-            p += part_p[(int64_t)g * n_expert + e];
+    int slots = 0, tokens = 0;
+    for (int64_t s = lo * top_k + threadIdx.x; s < hi * top_k; s += kThreads) {
+        const int64_t e = idx[s];
+        if (e >= 0 && e < n_expert && (!mask || mask[(uint32_t)s / (uint32_t)top_k] == 0)) {
+            atomicAdd(&lds.count[e], 1);
+            ++slots;
         }
-        count[e] = c;
-        slots += c;
-        sum += p * (double)c;
-        prob[e] = tokens ? (float)(p / (double)tokens) : 0.f;
     }
-    scratch[threadIdx.x] = sum;
-    atomicAdd((unsigned long long *)&slots_lds, (unsigned long long)slots);
     __syncthreads();
-    slots = slots_lds;
-    const long long per = per_slot ? slots : tokens;
-    const double k = per ? (double)n_expert / ((double)per * (double)per) : 0.0;
-    for (int e = threadIdx.x; e < n_expert; e += kBlock)
-        slope[e] = (float)(k * ((double)count[e] - (double)slots / n_expert));
-    if (threadIdx.x == 0) {
-        double total = 0;
-        for (int i = 0; i < kBlock; ++i) total += scratch[i];
-        *loss = (float)(k * total);
-        slope[n_expert] = tokens ? (float)(1.0 / (double)tokens) : 0.f;
+    int *part_count = sums.count + (int64_t)blockIdx.x * n_expert;
+    for (int e = threadIdx.x; e < n_expert; e += kThreads) part_count[e] = lds.count[e];
+    float acc[V][N] = {};
+    for (int64_t t0 = lo + wave * kTokens; t0 < hi; t0 += kWaves * kTokens * kAhead) {
+        Logits<T, L, V, WHOLE> a[kAhead];
+        bool counted[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t t = t0 + u * kWaves * kTokens + lane / L;
+            a[u].load(logits, t, hi, n_expert);
+            counted[u] = t < hi && (!mask || mask[t] == 0);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float p[V][N];
+            const float inv = a[u].softmax(p, counted[u], n_expert);
+            tokens += counted[u] && lane % L == 0 ? 1 : 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[v][i] += p[v][i] * inv;
+        }
     }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kBlock) void balance_bwd_kernel(const T *__restrict__ logits, const uint8_t *__restrict__ mask,
-                                                             const float *__restrict__ slope, const float *__restrict__ grad_loss,
-                                                             const float *__restrict__ grad_prob, T *__restrict__ grad,
-                                                             int64_t n_tokens, int n_expert) {
-    const int64_t t = (int64_t)blockIdx.x * kWavesPerBlock + threadIdx.x / kWave;
-    if (t >= n_tokens) return;
-    const int lane = threadIdx.x % kWave;
-    const T *row = logits + t * n_expert;
-    T *out = grad + t * n_expert;
-    RowTerms r{0.f, 0.f};
-    if (!mask || mask[t] == 0) r = row_terms(row, n_expert);
-    if (r.inv == 0.f) {
-        for (int e = lane; e < n_expert; e += kWave) out[e] = (T)0.f;
+    if (slots) atomicAdd(&total[1], slots);
+    if (tokens) atomicAdd(&total[0], tokens);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int off = L; off < kWave; off <<= 1) acc[v][i] += __shfl_xor(acc[v][i], off, kWave);
+    __syncthreads();
+    if (lane < L) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds.prob[wave][(v * L + lane) * N + i] = acc[v][i];
+    }
+    __syncthreads();
+    double sum = 0;
+    for (int e = threadIdx.x; e < n_expert; e += kThreads) {
+        float p = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) p += lds.prob[w][e];
+        if (gridDim.x > 1) sums.prob[(int64_t)blockIdx.x * n_expert + e] = p;
+        else sum += finish_expert(results, e, n_expert, p, part_count[e], total[0], total[1]);
+    }
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) sums.total[blockIdx.x] = make_int2(total[0], total[1]);
         return;
     }
-    const float gl = grad_loss ? *grad_loss : 0.f, per = slope[n_expert];
-    auto u = [&](int e) { return gl * slope[e] + (grad_prob ? grad_prob[e] * per : 0.f); };
-    float dot = 0.f;
-    for (int e = lane; e < n_expert; e += kWave) dot += expf((float)row[e] - r.most) * r.inv * u(e);
-    dot = wave_sum(dot);
-    for (int e = lane; e < n_expert; e += kWave) out[e] = (T)(expf((float)row[e] - r.most) * r.inv * (u(e) - dot));
+    sum = lane_sum(sum);
+    if (lane == 0) loss[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kWaves; ++w) sum += loss[w];
+        *results.loss = (float)sum;
+    }
 }
 
-int n_parts(int64_t n_tokens) {
-    const int64_t p = ceil_div(n_tokens < 1 ? 1 : n_tokens, 64);
-    return (int)(p < kMostParts ? p : kMostParts);
+// The results from the parts, kSumCols experts to a workgroup and kSumRanges ranges of parts side by side; the last workgroup that is through adds up
+// the loss, in the order of the experts.
+__global__ __launch_bounds__(kSumBlock) void balance_finish_kernel(Sums sums, Results results, int n_parts, int n_expert) {
+    __shared__ double prob[kSumRanges][kSumCols];
+    __shared__ int count[kSumRanges][kSumCols];
+    __shared__ long long total[2][kSumBlock / kWave];
+    __shared__ unsigned before;
+    const int col = threadIdx.x % kSumCols, range = threadIdx.x / kSumCols, e = blockIdx.x * kSumCols + col;
+    const int per = (n_parts + kSumRanges - 1) / kSumRanges, lo = range * per, hi = lo + per < n_parts ? lo + per : n_parts;
+    float p = 0.f;
+    int c = 0;
+    if (e < n_expert) {
+#pragma unroll 8
+        for (int g = lo; g < hi; ++g) {
+            p += sums.prob[(int64_t)g * n_expert + e];
+            c += sums.count[(int64_t)g * n_expert + e];
+        }
+    }
+    static_assert(kMostParts <= kSumBlock, "a part's totals to a thread");
+    const int2 mine = threadIdx.x < n_parts ? sums.total[threadIdx.x] : make_int2(0, 0);
+    long long tokens = mine.x, slots = mine.y;
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) {
+        tokens += __shfl_xor(tokens, off, kWave);
+        slots += __shfl_xor(slots, off, kWave);
+    }
+    if (threadIdx.x % kWave == 0) {
+        total[0][threadIdx.x / kWave] = tokens;
+        total[1][threadIdx.x / kWave] = slots;
+    }
+    prob[range][col] = p;
+    count[range][col] = c;
+    __syncthreads();
+    if (threadIdx.x >= kWave) return;
+    double sum = 0;
+    if (range == 0 && e < n_expert) {
+        tokens = slots = 0;
+        for (int w = 0; w < kSumBlock / kWave; ++w) {
+            tokens += total[0][w];
+            slots += total[1][w];
+        }
+        double all = 0;
+        long long named = 0;
+        for (int u = 0; u < kSumRanges; ++u) {
+            all += prob[u][col];
+            named += count[u][col];
+        }
+        sum = finish_expert(results, e, n_expert, all, named, tokens, slots);
+    }
+    sum = lane_sum(sum);
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(&sums.loss[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        before = __hip_atomic_fetch_add(sums.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == gridDim.x - 1) {
+            sum = 0;
+            for (unsigned i = 0; i < gridDim.x; ++i) sum += __hip_atomic_load(&sums.loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *results.loss = (float)sum;
+        }
+    }
 }
+
+template <typename T, int L, int V, bool WHOLE>
+__global__ __launch_bounds__(kBwdBlock) void balance_bwd_kernel(const T *__restrict__ logits, const uint8_t *__restrict__ mask,
+                                                                const float *__restrict__ slope, const float *__restrict__ grad_loss,
+                                                                const float *__restrict__ grad_prob, T *__restrict__ grad, int64_t n_tokens,
+                                                                int n_expert) {
+    constexpr int N = Vec<T>::N, kTokens = kBwdBlock / L;
+    const int lane = threadIdx.x % L;
+    const int64_t t = (int64_t)blockIdx.x * kTokens + threadIdx.x / L;
+    Logits<T, L, V, WHOLE> a;
+    a.load(logits, t, n_tokens, n_expert);
+    const bool counted = t < n_tokens && (!mask || mask[t] == 0);
+    const float gl = grad_loss ? *grad_loss : 0.f, per = slope[n_expert];
+    float p[V][N], u[V][N], dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = (v * L + lane) * N + i, at = e < n_expert ? e : 0;
+            u[v][i] = gl * slope[at] + (grad_prob ? grad_prob[at] * per : 0.f);
+        }
+    const float inv = a.softmax(p, counted, n_expert);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            p[v][i] *= inv;
+            dot += p[v][i] * u[v][i];
+        }
+    dot = over_lanes<L>(dot, [](float x, float y) { return x + y; });
+    if (t >= n_tokens) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int c = (v * L + lane) * N;
+        float out[8];
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = inv == 0.f ? 0.f : p[v][i] * (u[v][i] - dot);
+        if constexpr (WHOLE) {
+            if (c < n_expert) *(AnyVec *)(grad + t * n_expert + c) = Vec<T>::pack(out);
+        } else {
+            store_vec<false>(grad + t * n_expert + c, n_expert - c, Vec<T>::pack(out));
+        }
+    }
+}
+
+// How a token's logits are held: f(lanes, vectors to each, whether the experts are whole vectors), integral constants
+template <int N, typename F> void held_logits(int n_expert, F &&f) {
+    auto is = [&](auto l, auto v) {
+        if (n_expert > l.value * v.value * N) return false;
+        if (n_expert % N == 0) f(l, v, std::true_type{});
+        else f(l, v, std::false_type{});
+        return true;
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one{};
+    const integral_constant<int, 64> wave{};
+    (void)(is(one, one) || is(integral_constant<int, 2>{}, one) || is(integral_constant<int, 4>{}, one) || is(integral_constant<int, 8>{}, one) ||
+           is(integral_constant<int, 16>{}, one) || is(integral_constant<int, 32>{}, one) || is(wave, one) || is(wave, integral_constant<int, 2>{}) ||
+           is(wave, integral_constant<int, 4>{}) || is(wave, integral_constant<int, 8>{}) || is(wave, integral_constant<int, kMostExperts / kWave / N>{}));
+}
+
+int most_parts(int64_t n_tokens) { return (int)(n_tokens < 1 ? 1 : n_tokens < kMostParts ? n_tokens : kMostParts); }
 
 int check(const char *who, int64_t n_tokens, int64_t n_expert, int dtype) {
     FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who,
@@ -174,7 +344,7 @@ using namespace fmoe;
 
 extern "C" int64_t fmoe_balance_loss_workspace_bytes(int64_t n_tokens, int64_t n_expert) {
     if (n_tokens < 0 || n_expert < 1) return 0;
-    return 8 * n_tokens + (int64_t)n_parts(n_tokens) * (8 * n_expert + 4);
+    return 8 * ceil_div(n_expert, kSumCols) + 16 + (int64_t)most_parts(n_tokens) * (8 * n_expert + 8);
 }
 
 extern "C" int fmoe_balance_loss_forward(const void *logits, const int64_t *topk_idx, const void *token_mask, int64_t n_tokens,
@@ -189,20 +359,28 @@ extern "C" int fmoe_balance_loss_forward(const void *logits, const int64_t *topk
     if (!workspace || workspace_bytes < fmoe_balance_loss_workspace_bytes(n_tokens, n_expert))
         return fail(FMOE_EWORKSPACE, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                     (long long)fmoe_balance_loss_workspace_bytes(n_tokens, n_expert));
+    FMOE_REQUIRE(aligned16(workspace), "%s: workspace not on 16 bytes", who);
     hipStream_t st = (hipStream_t)stream;
-    const int parts = n_parts(n_tokens);
-    float2 *terms = (float2 *)workspace;
-    float *part_p = (float *)(terms + n_tokens);
-    int *part_c = (int *)(part_p + parts * n_expert), *part_t = part_c + parts * n_expert;
-    with_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (n_tokens > 0)
-            balance_rows_kernel<T><<<(int)ceil_div(n_tokens, kWavesPerBlock), kBlock, 0, st>>>((const T *)logits, (const uint8_t *)token_mask,
-                                                                                              terms, n_tokens, (int)n_expert);
-        balance_sum_kernel<T><<<dim3((int)ceil_div(n_expert, kBlock), parts), kBlock, 0, st>>>(
-            (const T *)logits, topk_idx, (const uint8_t *)token_mask, terms, part_p, part_c, part_t, n_tokens, (int)n_expert, (int)top_k);
+    const int columns = (int)ceil_div(n_expert, kSumCols), most = most_parts(n_tokens);
+    Sums sums;
+    sums.loss = (double *)workspace;
+    sums.done = (unsigned *)(sums.loss + columns);
+    sums.total = (int2 *)(sums.done + 2);
+    sums.prob = (float *)(sums.total + most);
+    sums.count = (int *)(sums.prob + most * n_expert);
+    const Results results{expert_count, prob, slope, loss, per_slot};
+    with_type(dtype, [&](auto type) {
+        using T = decltype(type);
+        held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
+            constexpr int kTokens = waves_of(v.value) * (kWave / l.value);
+            // (what one workgroup goes through in kOneRound rounds is not worth a second launch)
+            const int64_t rounds = ceil_div(n_tokens, kTokens);
+            const int parts = (int)(rounds <= kOneRound ? 1 : rounds < most ? rounds : most);
+            balance_sum_kernel<T, l.value, v.value, whole.value><<<parts, waves_of(v.value) * kWave, 0, st>>>(
+                (const T *)logits, topk_idx, (const uint8_t *)token_mask, sums, results, n_tokens, (int)n_expert, (int)top_k);
+            if (parts > 1) balance_finish_kernel<<<columns, kSumBlock, 0, st>>>(sums, results, parts, (int)n_expert);
+        });
     });
-    balance_finish_kernel<<<1, kBlock, 0, st>>>(part_p, part_c, part_t, parts, (int)n_expert, per_slot, expert_count, prob, slope, loss);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
 }
@@ -214,10 +392,12 @@ extern "C" int fmoe_balance_loss_backward(const void *logits, const void *token_
     if (int rc = check(who, n_tokens, n_expert, dtype)) return rc;
     if (n_tokens == 0) return FMOE_OK;
     FMOE_REQUIRE(logits && slope && grad_logits, "%s: NULL pointer", who);
-    with_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        balance_bwd_kernel<T><<<(int)ceil_div(n_tokens, kWavesPerBlock), kBlock, 0, (hipStream_t)stream>>>(
-            (const T *)logits, (const uint8_t *)token_mask, slope, grad_loss, grad_prob, (T *)grad_logits, n_tokens, (int)n_expert);
+    with_type(dtype, [&](auto type) {
+        using T = decltype(type);
+        held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
+            balance_bwd_kernel<T, l.value, v.value, whole.value><<<(int)ceil_div(n_tokens, kBwdBlock / l.value), kBwdBlock, 0, (hipStream_t)stream>>>(
+                (const T *)logits, (const uint8_t *)token_mask, slope, grad_loss, grad_prob, (T *)grad_logits, n_tokens, (int)n_expert);
+        });
     });
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
