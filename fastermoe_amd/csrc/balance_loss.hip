@@ -19,10 +19,10 @@ namespace {
 
 constexpr int kMostExperts = 8192;
 constexpr int kMostParts = 256;      // workgroups of the forward, each of which leaves sums over its tokens
-constexpr int kBwdBlock = 256;
+constexpr int kBwdBlock = 256, kBwdBlocks = 512;
 constexpr int kOneRound = 4;
-constexpr int kSumCols = 32, kSumRanges = 16, kSumBlock = kSumCols * kSumRanges;
-constexpr int waves_of(int v) { return v <= 2 ? 16 : 4; }                // of a workgroup of the forward
+constexpr int kSumCols = 16, kSumRanges = 64, kSumBlock = kSumCols * kSumRanges;
+constexpr int waves_of(int v) { return v <= 2 ? 16 : v <= 8 ? 8 : 3; }   // of a workgroup of the forward
 constexpr int ahead_of(int v) { return v == 1 ? 4 : v == 2 ? 2 : 1; }    // tokens in flight per lane
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -118,15 +118,13 @@ __global__ __launch_bounds__(waves_of(V) * kWave) void balance_sum_kernel(const 
                                                                            const uint8_t *__restrict__ mask, Sums sums, Results results,
                                                                            int64_t n_tokens, int n_expert, int top_k) {
     constexpr int N = Vec<T>::N, kWaves = waves_of(V), kThreads = kWaves * kWave, kTokens = kWave / L, kAhead = ahead_of(V);
-    __shared__ union {
-        int count[L * V * N];
-        float prob[kWaves][L * V * N];
-    } lds;
+    __shared__ int counts[L * V * N];
+    __shared__ float probs[kWaves][L * V * N];
     __shared__ int total[2];
     __shared__ double loss[kWaves];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int64_t per = (n_tokens + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per, hi = lo + per < n_tokens ? lo + per : n_tokens;
-    for (int e = threadIdx.x; e < n_expert; e += kThreads) lds.count[e] = 0;
+    for (int e = threadIdx.x; e < n_expert; e += kThreads) counts[e] = 0;
     if (threadIdx.x < 2) total[threadIdx.x] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *sums.done = 0;
     __syncthreads();
@@ -134,13 +132,10 @@ __global__ __launch_bounds__(waves_of(V) * kWave) void balance_sum_kernel(const 
     for (int64_t s = lo * top_k + threadIdx.x; s < hi * top_k; s += kThreads) {
         const int64_t e = idx[s];
         if (e >= 0 && e < n_expert && (!mask || mask[(uint32_t)s / (uint32_t)top_k] == 0)) {
-            atomicAdd(&lds.count[e], 1);
+            atomicAdd(&counts[e], 1);
             ++slots;
         }
     }
-    __syncthreads();
-    int *part_count = sums.count + (int64_t)blockIdx.x * n_expert;
-    for (int e = threadIdx.x; e < n_expert; e += kThreads) part_count[e] = lds.count[e];
     float acc[V][N] = {};
     for (int64_t t0 = lo + wave * kTokens; t0 < hi; t0 += kWaves * kTokens * kAhead) {
         Logits<T, L, V, WHOLE> a[kAhead];
@@ -153,38 +148,47 @@ __global__ __launch_bounds__(waves_of(V) * kWave) void balance_sum_kernel(const 
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
+            if (t0 + u * kWaves * kTokens >= hi) break;
             float p[V][N];
             const float inv = a[u].softmax(p, counted[u], n_expert);
-            tokens += counted[u] && lane % L == 0 ? 1 : 0;
+            tokens += __popcll(__ballot(counted[u] && lane % L == 0));
 #pragma unroll
             for (int v = 0; v < V; ++v)
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[v][i] += p[v][i] * inv;
         }
     }
-    if (slots) atomicAdd(&total[1], slots);
-    if (tokens) atomicAdd(&total[0], tokens);
+    // (a sum over the wave first: lanes that add to one address take turns, 1024 of them some 3 us)
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) slots += __shfl_xor(slots, off, kWave);
+    if (lane == 0) {
+        atomicAdd(&total[1], slots);
+        atomicAdd(&total[0], tokens);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int off = L; off < kWave; off <<= 1) acc[v][i] += __shfl_xor(acc[v][i], off, kWave);
-    __syncthreads();
     if (lane < L) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < N; ++i) lds.prob[wave][(v * L + lane) * N + i] = acc[v][i];
+            for (int i = 0; i < N; ++i) probs[wave][(v * L + lane) * N + i] = acc[v][i];
     }
     __syncthreads();
     double sum = 0;
     for (int e = threadIdx.x; e < n_expert; e += kThreads) {
         float p = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) p += lds.prob[w][e];
-        if (gridDim.x > 1) sums.prob[(int64_t)blockIdx.x * n_expert + e] = p;
-        else sum += finish_expert(results, e, n_expert, p, part_count[e], total[0], total[1]);
+        for (int w = 0; w < kWaves; ++w) p += probs[w][e];
+        if (gridDim.x > 1) {
+            sums.prob[(int64_t)blockIdx.x * n_expert + e] = p;
+            sums.count[(int64_t)blockIdx.x * n_expert + e] = counts[e];
+        } else {
+            sum += finish_expert(results, e, n_expert, p, counts[e], total[0], total[1]);
+        }
     }
     if (gridDim.x > 1) {
         if (threadIdx.x == 0) sums.total[blockIdx.x] = make_int2(total[0], total[1]);
@@ -199,107 +203,126 @@ __global__ __launch_bounds__(waves_of(V) * kWave) void balance_sum_kernel(const 
     }
 }
 
-// The results from the parts, kSumCols experts to a workgroup and kSumRanges ranges of parts side by side; the last workgroup that is through adds up
-// the loss, in the order of the experts.
+// The results from the parts, kSumCols experts to a workgroup and the parts in kSumRanges ranges side by side; the last workgroup that is through adds
+// up the loss, in the order of the experts.  (256 parts of 64 experts 6.1 us, of 16, where nobody has to be waited for, 3.6, of 256 7.2; one workgroup for
+// 64 experts takes 8.2 and for 256, whose 512 KiB come from the other XCDs' writes, 25.)
 __global__ __launch_bounds__(kSumBlock) void balance_finish_kernel(Sums sums, Results results, int n_parts, int n_expert) {
-    __shared__ double prob[kSumRanges][kSumCols];
-    __shared__ int count[kSumRanges][kSumCols];
-    __shared__ long long total[2][kSumBlock / kWave];
-    __shared__ unsigned before;
-    const int col = threadIdx.x % kSumCols, range = threadIdx.x / kSumCols, e = blockIdx.x * kSumCols + col;
-    const int per = (n_parts + kSumRanges - 1) / kSumRanges, lo = range * per, hi = lo + per < n_parts ? lo + per : n_parts;
-    float p = 0.f;
+    constexpr int kWaves = kSumBlock / kWave;
+    static_assert(kMostParts <= kSumBlock && kMostParts % kSumRanges == 0 && kSumCols < kWave, "a part's totals to a thread");
+    __shared__ double prob[kWaves][kSumCols];
+    __shared__ int count[kWaves][kSumCols];
+    __shared__ long long total[2][kWaves];
+    const int col = threadIdx.x % kSumCols, range = threadIdx.x / kSumCols, e = blockIdx.x * kSumCols + col, wave = threadIdx.x / kWave;
+    const int2 mine = (int)threadIdx.x < n_parts ? sums.total[threadIdx.x] : make_int2(0, 0);
+    double p = 0;
     int c = 0;
-    if (e < n_expert) {
-#pragma unroll 8
-        for (int g = lo; g < hi; ++g) {
-            p += sums.prob[(int64_t)g * n_expert + e];
-            c += sums.count[(int64_t)g * n_expert + e];
-        }
+#pragma unroll
+    for (int i = 0; i < kMostParts / kSumRanges; ++i) {
+        const int g = range + i * kSumRanges;
+        const bool in = g < n_parts && e < n_expert;
+        p += in ? sums.prob[(int64_t)g * n_expert + e] : 0.f;
+        c += in ? sums.count[(int64_t)g * n_expert + e] : 0;
     }
-    static_assert(kMostParts <= kSumBlock, "a part's totals to a thread");
-    const int2 mine = threadIdx.x < n_parts ? sums.total[threadIdx.x] : make_int2(0, 0);
     long long tokens = mine.x, slots = mine.y;
+#pragma unroll
+    for (int off = kSumCols; off < kWave; off <<= 1) {
+        p += __shfl_xor(p, off, kWave);
+        c += __shfl_xor(c, off, kWave);
+    }
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) {
         tokens += __shfl_xor(tokens, off, kWave);
         slots += __shfl_xor(slots, off, kWave);
     }
-    if (threadIdx.x % kWave == 0) {
-        total[0][threadIdx.x / kWave] = tokens;
-        total[1][threadIdx.x / kWave] = slots;
+    if (threadIdx.x % kWave < kSumCols) {
+        prob[wave][col] = p;
+        count[wave][col] = c;
     }
-    prob[range][col] = p;
-    count[range][col] = c;
+    if (threadIdx.x % kWave == 0) {
+        total[0][wave] = tokens;
+        total[1][wave] = slots;
+    }
     __syncthreads();
-    if (threadIdx.x >= kWave) return;
+    if (wave != 0) return;
     double sum = 0;
     if (range == 0 && e < n_expert) {
+#pragma unroll
+        for (int r = 1; r < kWaves; ++r) {
+            p += prob[r][col];
+            c += count[r][col];
+        }
         tokens = slots = 0;
-        for (int w = 0; w < kSumBlock / kWave; ++w) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
             tokens += total[0][w];
             slots += total[1][w];
         }
-        double all = 0;
-        long long named = 0;
-        for (int u = 0; u < kSumRanges; ++u) {
-            all += prob[u][col];
-            named += count[u][col];
-        }
-        sum = finish_expert(results, e, n_expert, all, named, tokens, slots);
+        sum = finish_expert(results, e, n_expert, p, c, tokens, slots);
     }
     sum = lane_sum(sum);
-    if (threadIdx.x == 0) {
-        __hip_atomic_store(&sums.loss[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        before = __hip_atomic_fetch_add(sums.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        if (before == gridDim.x - 1) {
-            sum = 0;
-            for (unsigned i = 0; i < gridDim.x; ++i) sum += __hip_atomic_load(&sums.loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            *results.loss = (float)sum;
+    if (gridDim.x > 1) {
+        unsigned before = 0;
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(&sums.loss[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            before = __hip_atomic_fetch_add(sums.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         }
+        if (__builtin_amdgcn_readfirstlane(before) != gridDim.x - 1) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        sum = 0;
+        for (unsigned i = threadIdx.x; i < gridDim.x; i += kWave) sum += __hip_atomic_load(&sums.loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sum = lane_sum(sum);
     }
+    if (threadIdx.x == 0) *results.loss = (float)sum;
 }
 
-template <typename T, int L, int V, bool WHOLE>
+template <typename T, int L, int V, bool WHOLE, int AHEAD>
 __global__ __launch_bounds__(kBwdBlock) void balance_bwd_kernel(const T *__restrict__ logits, const uint8_t *__restrict__ mask,
                                                                 const float *__restrict__ slope, const float *__restrict__ grad_loss,
                                                                 const float *__restrict__ grad_prob, T *__restrict__ grad, int64_t n_tokens,
                                                                 int n_expert) {
     constexpr int N = Vec<T>::N, kTokens = kBwdBlock / L;
     const int lane = threadIdx.x % L;
-    const int64_t t = (int64_t)blockIdx.x * kTokens + threadIdx.x / L;
-    Logits<T, L, V, WHOLE> a;
-    a.load(logits, t, n_tokens, n_expert);
-    const bool counted = t < n_tokens && (!mask || mask[t] == 0);
+    const int64_t t0 = (int64_t)blockIdx.x * (kTokens * AHEAD) + threadIdx.x / L;
+    Logits<T, L, V, WHOLE> a[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) a[k].load(logits, t0 + k * kTokens, n_tokens, n_expert);
     const float gl = grad_loss ? *grad_loss : 0.f, per = slope[n_expert];
-    float p[V][N], u[V][N], dot = 0.f;
+    float u[V][N];
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = (v * L + lane) * N + i, at = e < n_expert ? e : 0;
-            u[v][i] = gl * slope[at] + (grad_prob ? grad_prob[at] * per : 0.f);
+        for (int i = 0; i < N; i += 4) {
+            const int c = (v * L + lane) * N + i;
+            const u32x4 s = load_vec<false>(slope + c, n_expert - c, false);
+            const u32x4 g = grad_prob ? load_vec<false>(grad_prob + c, n_expert - c, false) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[v][i + j] = gl * __uint_as_float(s[j]) + __uint_as_float(g[j]) * per;
         }
-    const float inv = a.softmax(p, counted, n_expert);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int k = 0; k < AHEAD; ++k) {
+        const int64_t t = t0 + k * kTokens;
+        float p[V][N], dot = 0.f;
+        const float inv = a[k].softmax(p, t < n_tokens && (!mask || mask[t] == 0), n_expert);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            p[v][i] *= inv;
-            dot += p[v][i] * u[v][i];
-        }
-    dot = over_lanes<L>(dot, [](float x, float y) { return x + y; });
-    if (t >= n_tokens) return;
+        for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int c = (v * L + lane) * N;
-        float out[8];
+            for (int i = 0; i < N; ++i) {
+                p[v][i] *= inv;
+                dot += p[v][i] * u[v][i];
+            }
+        dot = over_lanes<L>(dot, [](float x, float y) { return x + y; });
+        if (t >= n_tokens) continue;
 #pragma unroll
-        for (int i = 0; i < N; ++i) out[i] = inv == 0.f ? 0.f : p[v][i] * (u[v][i] - dot);
-        if constexpr (WHOLE) {
-            if (c < n_expert) *(AnyVec *)(grad + t * n_expert + c) = Vec<T>::pack(out);
-        } else {
-            store_vec<false>(grad + t * n_expert + c, n_expert - c, Vec<T>::pack(out));
+        for (int v = 0; v < V; ++v) {
+            const int c = (v * L + lane) * N;
+            float out[8];
+#pragma unroll
+            for (int i = 0; i < N; ++i) out[i] = inv == 0.f ? 0.f : p[v][i] * (u[v][i] - dot);
+            if constexpr (WHOLE) {
+                if (c < n_expert) *(AnyVec *)(grad + t * n_expert + c) = Vec<T>::pack(out);
+            } else {
+                store_vec<false>(grad + t * n_expert + c, n_expert - c, Vec<T>::pack(out));
+            }
         }
     }
 }
@@ -395,7 +418,11 @@ extern "C" int fmoe_balance_loss_backward(const void *logits, const void *token_
     with_type(dtype, [&](auto type) {
         using T = decltype(type);
         held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
-            balance_bwd_kernel<T, l.value, v.value, whole.value><<<(int)ceil_div(n_tokens, kBwdBlock / l.value), kBwdBlock, 0, (hipStream_t)stream>>>(
+            // (one token in flight per lane where more would leave compute units without a workgroup)
+            constexpr int kTokens = kBwdBlock / l.value, kAhead = ahead_of(v.value);
+            const bool ahead = n_tokens >= kBwdBlocks * kTokens * kAhead;
+            (ahead ? balance_bwd_kernel<T, l.value, v.value, whole.value, kAhead> : balance_bwd_kernel<T, l.value, v.value, whole.value, 1>)<<<
+                (int)ceil_div(n_tokens, kTokens * (ahead ? kAhead : 1)), kBwdBlock, 0, (hipStream_t)stream>>>(
                 (const T *)logits, (const uint8_t *)token_mask, slope, grad_loss, grad_prob, (T *)grad_logits, n_tokens, (int)n_expert);
         });
     });
