@@ -164,7 +164,11 @@ def load_layer_call():
             warnings.warn(f"inference calls the layer from Python, some 10 us slower: {why} (run `python -m fastermoe_amd.build`)", RuntimeWarning)
             return None
         lib = load()
-        module.bind(*(ctypes.cast(fn, _vp).value for fn in (lib.fmoe_layer_sizes, lib.fmoe_layer_forward)))
+        address = lambda name: ctypes.cast(getattr(lib, name), _vp).value
+        module.bind(address("fmoe_layer_sizes"), address("fmoe_layer_forward"))
+        module.bind_block(*map(address, ("fmoe_last_error", "fmoe_layer_norm_forward", "fmoe_layer_norm_backward",
+                                         "fmoe_layer_norm_backward_workspace_bytes", "fmoe_balance_loss_forward", "fmoe_balance_loss_backward",
+                                         "fmoe_balance_loss_workspace_bytes")))
         _layer_call = module
     return _layer_call
 

@@ -18,7 +18,8 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "lib", "libfmoe_hip.so")
 LAYER_CALL = os.path.join(HERE, "lib", "_layer_call.so")   # host code over torch's tensors
 
-HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+ROCM = "/opt/rocm"
+HIPCC = os.environ.get("HIPCC", f"{ROCM}/bin/hipcc")
 ARCH = "gfx950"
 # -packed-fp32-ops is switched off on purpose: the packed fp32 VALU forms are not
 # to be generated for this target.
@@ -58,13 +59,14 @@ def _compile(unit):
 
 
 def _build_layer_call():
-    """The extension module of csrc/layer_call.cpp."""
+    """The extension module of csrc/layer_call.cpp and csrc/block_call.cpp."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     built_for = f"{torch.__version__} {sys.implementation.cache_tag}"   # what _lib.load_layer_call() compares
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DFMOE_BUILT_FOR="{built_for}"', f"-I{sysconfig.get_path('include')}", *(f"-I{p}" for p in include_paths()), os.path.join(CSRC, "layer_call.cpp"), "-o", LAYER_CALL,
-           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+           f'-DFMOE_BUILT_FOR="{built_for}"', f"-I{sysconfig.get_path('include')}", *(f"-I{p}" for p in include_paths()), "-D__HIP_PLATFORM_AMD__",
+           f"-I{ROCM}/include", *(os.path.join(CSRC, f) for f in ("layer_call.cpp", "block_call.cpp")), "-o", LAYER_CALL,
+           *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     return proc.returncode, "_layer_call.so", proc.stdout
 

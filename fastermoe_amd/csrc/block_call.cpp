@@ -1,0 +1,266 @@
+// Layer norm and the gate's balance loss as autograd nodes, from Python's tensors to the enqueued kernels (host code).
+//
+// Their kernels take 3 to 20 us on a small training step's tensors.  As Python nodes, a forward and a backward took 138 and 90 us to enqueue,
+// most of it in the backward's thread; a product and its gradient in torch itself take 46.  What a call takes is decided here; None sends it the
+// Python node's way, which says what is wrong with its tensors.
+#include "block_call.hpp"
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <array>
+#include <cmath>
+#include <cstdint>
+#include <optional>
+
+#include "../../include/fmoe_hip.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// the library's entry points, which Python has loaded (bind)
+struct Entries {
+    decltype(&fmoe_last_error) last_error;
+    decltype(&fmoe_layer_norm_forward) norm_forward;
+    decltype(&fmoe_layer_norm_backward) norm_backward;
+    decltype(&fmoe_layer_norm_backward_workspace_bytes) norm_bytes;
+    decltype(&fmoe_balance_loss_forward) balance_forward;
+    decltype(&fmoe_balance_loss_backward) balance_backward;
+    decltype(&fmoe_balance_loss_workspace_bytes) balance_bytes;
+} entry = {};
+
+int dtype_code(const at::Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return FMOE_F32;
+        case at::kBFloat16: return FMOE_BF16;
+        case at::kHalf: return FMOE_F16;
+        default: return -1;
+    }
+}
+void *pointer(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+float *floats(const at::Tensor &t) { return (float *)pointer(t); }
+void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+void ok(int rc) { TORCH_CHECK(rc == FMOE_OK, "libfmoe_hip error ", rc, ": ", entry.last_error()); }
+at::Tensor same(const at::Tensor &t) { return at::empty(t.sizes(), t.options()); }
+// rows of adjacent elements, as the kernels read them
+at::Tensor as_rows(const at::Tensor &t) { return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t; }
+
+using Maybe = std::optional<at::Tensor>;   // (what a node takes where there may be no tensor)
+Maybe maybe(const at::Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &given, const Maybe &of_residual, const Maybe &of_weight,
+                                 const Maybe &of_bias, double eps, bool keep) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const at::Tensor residual = of_residual.value_or(at::Tensor()), weight = of_weight.value_or(at::Tensor()), bias = of_bias.value_or(at::Tensor());
+        const c10::OptionalDeviceGuard guard(given.device());
+        const at::Tensor inp = as_rows(given), other = residual.defined() ? as_rows(residual) : residual;
+        const int64_t n = inp.size(0), d = inp.size(1);
+        const at::Tensor out = at::empty({n, d}, inp.options()), total = other.defined() ? same(out) : at::Tensor();
+        at::Tensor stats;   // the rows' means, then their reciprocal deviations
+        if (keep) stats = at::empty({2, n}, inp.options().dtype(at::kFloat));
+        const at::Tensor &param = weight.defined() ? weight : bias;
+        ok(entry.norm_forward(pointer(inp), inp.stride(0), pointer(other), other.defined() ? other.stride(0) : 0, pointer(weight), pointer(bias),
+                              pointer(total), pointer(out), floats(stats), keep ? floats(stats) + n : nullptr, n, d, eps, dtype_code(inp),
+                              param.defined() ? dtype_code(param) : dtype_code(inp), stream_of(inp)));
+        if (keep) {
+            ctx->save_for_backward({total.defined() ? total : inp, stats, weight, bias});
+            ctx->saved_data["eps"] = eps;
+            ctx->set_materialize_grads(false);
+        }
+        return total.defined() ? variable_list{out, total} : variable_list{out};
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &rows = saved[0], &stats = saved[1], &weight = saved[2], &bias = saved[3];
+        const at::Tensor total = grads.size() > 1 ? grads[1] : at::Tensor();
+        // (asked by the tensors that there were)
+        const size_t has_r = grads.size() > 1, has_w = weight.defined();
+        const bool need_x = ctx->needs_input_grad(0), need_r = has_r && ctx->needs_input_grad(1);
+        const bool need_w = has_w && ctx->needs_input_grad(1 + has_r), need_b = bias.defined() && ctx->needs_input_grad(1 + has_r + has_w);
+        at::Tensor x, w, b;
+        if (!grads[0].defined()) {
+            if (total.defined()) {
+                x = total;
+                if (need_w) w = at::zeros_like(weight);
+                if (need_b) b = at::zeros_like(bias);
+            }
+        } else if (at::GradMode::is_enabled()) {   // (a backward that is to be differentiated again needs torch's operators)
+            const at::Tensor t = rows.to(at::kFloat), g = grads[0].to(at::kFloat);
+            const at::Tensor centred = t - t.mean(1, true), rstd = (centred * centred).mean(1, true).add(ctx->saved_data["eps"].toDouble()).rsqrt();
+            const at::Tensor hat = centred * rstd, a = weight.defined() ? g * weight.to(at::kFloat) : g;
+            x = rstd * (a - a.mean(1, true) - hat * (a * hat).mean(1, true));
+            if (total.defined()) x = x + total.to(at::kFloat);
+            x = x.to(rows.scalar_type());
+            if (need_w) w = (g * hat).sum(0).to(weight.scalar_type());
+            if (need_b) b = g.sum(0).to(bias.scalar_type());
+        } else {
+            const c10::OptionalDeviceGuard guard(rows.device());
+            const at::Tensor gy = as_rows(grads[0]), gs = total.defined() ? as_rows(total) : total, at_rows = as_rows(rows);
+            const int64_t n = rows.size(0), d = rows.size(1);
+            const at::Tensor held = stats.contiguous();
+            if (need_x || need_r) x = at::empty({n, d}, rows.options());
+            if (need_w) w = same(weight);
+            if (need_b) b = same(bias);
+            const int64_t bytes = need_w || need_b ? entry.norm_bytes(n, d) : 0;
+            const at::Tensor space = bytes ? at::empty({bytes}, rows.options().dtype(at::kByte)) : at::Tensor();
+            const at::Tensor &param = weight.defined() ? weight : bias;
+            ok(entry.norm_backward(pointer(gy), gy.stride(0), pointer(gs), gs.defined() ? gs.stride(0) : 0, pointer(at_rows), at_rows.stride(0),
+                                   floats(held), floats(held) + n, pointer(weight), pointer(x), pointer(w), pointer(b), n, d, dtype_code(rows),
+                                   param.defined() ? dtype_code(param) : dtype_code(rows), pointer(space), bytes, stream_of(rows)));
+        }
+        const at::Tensor none;
+        return {need_x ? x : none, need_r ? x : none, need_w ? w : none, need_b ? b : none, none, none};
+    }
+};
+
+struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &given, const at::Tensor &index, const Maybe &of_mask, int64_t per_slot) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const at::Tensor mask = of_mask.value_or(at::Tensor());
+        const c10::OptionalDeviceGuard guard(given.device());
+        const at::Tensor logits = given.contiguous(), idx = index.contiguous();
+        const int64_t n = logits.size(0), e = logits.size(1), bytes = entry.balance_bytes(n, e);
+        const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
+        const at::Tensor loss = at::empty({}, f32), count = at::empty({e}, f32.dtype(at::kLong)), prob = at::empty({e}, f32);
+        const at::Tensor slope = at::empty({e + 1}, f32), space = at::empty({bytes}, f32.dtype(at::kByte));
+        ok(entry.balance_forward(pointer(logits), (int64_t *)pointer(idx), pointer(mask), n, e, n ? idx.numel() / n : 1, dtype_code(logits),
+                                 (int)per_slot, floats(loss), (int64_t *)pointer(count), floats(prob), floats(slope), pointer(space), bytes,
+                                 stream_of(logits)));
+        ctx->save_for_backward({logits, mask, slope});
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({count});
+        return {loss, count, prob};
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &mask = saved[1], &slope = saved[2], &of_loss = grads[0], &of_prob = grads[2];
+        at::Tensor grad;
+        if (of_loss.defined() || of_prob.defined()) {
+            if (at::GradMode::is_enabled()) {   // (as above)
+                const int64_t e = logits.size(1);
+                at::Tensor u;
+                if (of_loss.defined()) u = of_loss * slope.narrow(0, 0, e);
+                if (of_prob.defined()) u = u.defined() ? u + of_prob * slope.select(0, e) : of_prob * slope.select(0, e);
+                at::Tensor left_out = logits.eq(-INFINITY).all(1);
+                if (mask.defined()) left_out = left_out.logical_or(mask);
+                left_out = left_out.unsqueeze(1);
+                const at::Tensor p = at::softmax(logits.to(at::kFloat).masked_fill(left_out, 0), 1).masked_fill(left_out, 0);
+                grad = (p * (u - (p * u).sum(1, true))).to(logits.scalar_type());
+            } else {
+                const c10::OptionalDeviceGuard guard(logits.device());
+                auto dense = [](const at::Tensor &t) { return t.defined() ? t.contiguous() : t; };
+                const at::Tensor gl = dense(of_loss), gp = dense(of_prob), held = logits.contiguous(), by = slope.contiguous(), out = dense(mask);
+                grad = same(held);
+                ok(entry.balance_backward(pointer(held), pointer(out), floats(by), floats(gl), floats(gp), pointer(grad), logits.size(0),
+                                          logits.size(1), dtype_code(logits), stream_of(logits)));
+            }
+        }
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// The interpreter's lock, given back while this lives: an allocation may wait for the device, a launch for a full queue
+struct WithoutLock {
+    PyThreadState *state = PyEval_SaveThread();
+    ~WithoutLock() { PyEval_RestoreThread(state); }
+};
+
+// The first N arguments as tensors (undefined for None); false, with an exception set, where one is neither
+template <size_t N> bool tensors(PyObject *const *args, std::array<at::Tensor, N> &t) {
+    for (size_t i = 0; i < N; ++i) {
+        if (args[i] == Py_None) continue;
+        if (!THPVariable_Check(args[i])) {
+            PyErr_SetString(PyExc_TypeError, "tensors or None");
+            return false;
+        }
+        t[i] = THPVariable_Unpack(args[i]);
+    }
+    return true;
+}
+bool on_gpu(const at::Tensor &t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(); }
+
+}  // namespace
+
+PyObject *fmoe_block_bind(PyObject *, PyObject *args) {
+    unsigned long long a[7];
+    if (!PyArg_ParseTuple(args, "KKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6])) return nullptr;
+    auto set = [&](auto &fn, int i) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(static_cast<uintptr_t>(a[i])); };
+    set(entry.last_error, 0);
+    set(entry.norm_forward, 1);
+    set(entry.norm_backward, 2);
+    set(entry.norm_bytes, 3);
+    set(entry.balance_forward, 4);
+    set(entry.balance_backward, 5);
+    set(entry.balance_bytes, 6);
+    Py_RETURN_NONE;
+}
+
+// layer_norm(inp, residual, weight, bias, eps): the result of the rows' norm, with the sum behind it where there is a residual; None where the call does
+// not take these tensors
+PyObject *fmoe_block_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 5 || entry.norm_forward == nullptr) {
+        PyErr_SetString(PyExc_TypeError, "layer_norm: 5 arguments, after bind_block");
+        return nullptr;
+    }
+    std::array<at::Tensor, 4> t;
+    if (!tensors(args, t)) return nullptr;
+    const auto &[inp, residual, weight, bias] = t;
+    const double eps = PyFloat_AsDouble(args[4]);
+    if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+    if (!on_gpu(inp) || inp.dim() != 2 || inp.size(1) == 0 || dtype_code(inp) < 0 || !(eps >= 0) || std::isinf(eps)) Py_RETURN_NONE;
+    if (residual.defined() && (!on_gpu(residual) || residual.device() != inp.device() || residual.scalar_type() != inp.scalar_type() ||
+                               residual.sizes() != inp.sizes()))
+        Py_RETURN_NONE;
+    for (const at::Tensor *p : {&weight, &bias})
+        if (p->defined() && (!on_gpu(*p) || p->device() != inp.device() || !p->is_contiguous() || p->sizes() != at::IntArrayRef({inp.size(1)}) ||
+                             (p->scalar_type() != inp.scalar_type() && p->scalar_type() != at::kFloat)))
+            Py_RETURN_NONE;
+    if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) Py_RETURN_NONE;
+    variable_list out;
+    {
+        const WithoutLock no_lock;
+        bool keep = false;
+        for (const at::Tensor &p : t) keep |= p.defined() && p.requires_grad();
+        out = LayerNorm::apply(inp, maybe(residual), maybe(weight), maybe(bias), eps, keep && at::GradMode::is_enabled());
+    }
+    if (out.size() == 1) return THPVariable_Wrap(std::move(out[0]));
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])));
+    END_HANDLE_TH_ERRORS
+}
+
+// balance_loss(logits, topk_idx, mask, per_slot): (loss, counts, prob); None where the call does not take these tensors
+PyObject *fmoe_block_balance_loss(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 4 || entry.balance_forward == nullptr) {
+        PyErr_SetString(PyExc_TypeError, "balance_loss: 4 arguments, after bind_block");
+        return nullptr;
+    }
+    std::array<at::Tensor, 3> t;
+    if (!tensors(args, t)) return nullptr;
+    const auto &[logits, idx, mask] = t;
+    const long per_slot = PyLong_AsLong(args[3]);
+    if (per_slot == -1 && PyErr_Occurred()) return nullptr;
+    if (!on_gpu(logits) || !on_gpu(idx) || logits.dim() != 2 || dtype_code(logits) < 0 || idx.device() != logits.device() || idx.scalar_type() != at::kLong)
+        Py_RETURN_NONE;
+    const int64_t n = logits.size(0), e = logits.size(1);
+    if (e < 1 || e > 8192 || n > INT32_MAX / 8 || idx.numel() > INT32_MAX || idx.numel() % (n ? n : 1) != 0 || (n && !idx.numel())) Py_RETURN_NONE;
+    if (mask.defined() && (!on_gpu(mask) || mask.device() != logits.device() || mask.scalar_type() != at::kBool || mask.numel() != n || !mask.is_contiguous()))
+        Py_RETURN_NONE;
+    variable_list out;
+    {
+        const WithoutLock no_lock;
+        out = BalanceLoss::apply(logits, idx, maybe(mask), (int64_t)(per_slot != 0));
+    }
+    return Py_BuildValue("NNN", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])), THPVariable_Wrap(std::move(out[2])));
+    END_HANDLE_TH_ERRORS
+}

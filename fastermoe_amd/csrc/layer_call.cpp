@@ -16,6 +16,7 @@
 #include <cstdint>
 
 #include "../../include/fmoe_hip.h"
+#include "block_call.hpp"
 
 namespace {
 
@@ -111,6 +112,9 @@ PyObject *infer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "The addresses of fmoe_layer_sizes and fmoe_layer_forward."},
     {"infer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(infer)), METH_FASTCALL, "A layer's output where nothing is differentiated."},
+    {"bind_block", fmoe_block_bind, METH_VARARGS, "The addresses of the library's entry points that the next two call."},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fmoe_block_layer_norm)), METH_FASTCALL, "Layer norm of rows."},
+    {"balance_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fmoe_block_balance_loss)), METH_FASTCALL, "A gate's balance loss."},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_layer_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -179,7 +179,8 @@ class NoisyTopK(Function):
 
 
 class BalanceLoss(Function):
-    r"""Balance loss of a gate with the experts' counts and mean probabilities (see :func:`balance_loss`)."""
+    r"""Balance loss of a gate with the experts' counts and mean probabilities (see :func:`balance_loss`): what csrc/block_call.cpp does in native
+    code."""
 
     @staticmethod
     def forward(ctx, logits, topk_idx, mask, per_slot):
@@ -203,7 +204,7 @@ class BalanceLoss(Function):
             p = torch.softmax(logits.float().masked_fill(left_out, 0), dim=1).masked_fill(left_out, 0)
             return (p * (u - (p * u).sum(dim=1, keepdim=True))).to(logits.dtype), None, None, None
         contiguous = lambda t: None if t is None else t.contiguous()
-        return fmoe_native.balance_loss_backward(logits, mask, slope, contiguous(grad_loss), contiguous(grad_prob)), None, None, None
+        return fmoe_native.balance_loss_backward(*map(contiguous, (logits, mask, slope, grad_loss, grad_prob))), None, None, None
 
 
 def balance_loss(logits, topk_idx, per="token", mask=None):
@@ -220,6 +221,11 @@ def balance_loss(logits, topk_idx, per="token", mask=None):
     if mask is not None:
         mask = mask.reshape(-1)
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    module = _lib.load_layer_call()
+    if module is not None and nothing_watches(logits, topk_idx):
+        out = module.balance_loss(logits, topk_idx, mask, per == "slot")
+        if out is not None:
+            return out
     return BalanceLoss.apply(logits, topk_idx.contiguous(), mask, per == "slot")
 
 
@@ -448,7 +454,8 @@ def act_checkpoint(inp, activation):
     elements along a row, 1.03 bytes an element, and the derivative is taken where those are (off by at most 2^-4 of an element,
     or 2^-10 of the block's scale where it is small against the block).  Float32, bfloat16 and float16."""
     code = activation if type(activation) is int else _activation_code(activation)
-    return ActCheckpoint.apply(_as_rows(inp), code).view(inp.shape)
+    out = ActCheckpoint.apply(_as_rows(inp), code)
+    return out if inp.dim() == 2 else out.view(inp.shape)
 
 
 def _activation_code(activation):
@@ -769,7 +776,8 @@ class MaskRestore(Function):
 
 
 class LayerNorm(Function):
-    r"""Layer norm over rows, of a sum with a residual where there is one (see :func:`layer_norm`, :func:`add_layer_norm`)."""
+    r"""Layer norm over rows, of a sum with a residual where there is one (see :func:`layer_norm`, :func:`add_layer_norm`): what csrc/block_call.cpp
+    does in native code."""
 
     @staticmethod
     def forward(ctx, inp, residual, weight, bias, eps):
@@ -778,28 +786,48 @@ class LayerNorm(Function):
         out, total, mean, rstd = fmoe_native.layer_norm_forward(inp, residual, weight, bias, eps, keep)
         if keep:
             ctx.save_for_backward(inp if total is None else total, mean, rstd, weight, bias)
+            ctx.eps = eps
         return out if total is None else (out, total)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out, grad_total=None):
         rows, mean, rstd, weight, bias = ctx.saved_tensors
         need = ctx.needs_input_grad
+        need_w, need_b = weight is not None and need[2], bias is not None and need[3]
         if grad_out is None:
-            if grad_total is None:
-                return None, None, None, None, None
-            zeros = lambda p, wanted: torch.zeros_like(p) if wanted and p is not None else None
-            return grad_total, grad_total if need[1] else None, zeros(weight, need[2]), zeros(bias, need[3]), None
-        grad, grad_w, grad_b = fmoe_native.layer_norm_backward(grad_out, grad_total, rows, mean, rstd, weight, bias,
-                                                               need[0] or need[1], need[2], need[3])
+            grad = grad_total
+            grad_w, grad_b = (torch.zeros_like(p) if wanted and grad is not None else None for p, wanted in ((weight, need_w), (bias, need_b)))
+        elif torch.is_grad_enabled():   # (a backward that is to be differentiated again needs torch operators)
+            t, g = rows.float(), grad_out.float()
+            centred = t - t.mean(1, keepdim=True)
+            rstd = ((centred * centred).mean(1, keepdim=True) + ctx.eps).rsqrt()
+            hat, a = centred * rstd, g if weight is None else g * weight.float()
+            grad = rstd * (a - a.mean(1, keepdim=True) - hat * (a * hat).mean(1, keepdim=True))
+            grad = (grad if grad_total is None else grad + grad_total.float()).to(rows.dtype)
+            grad_w = (g * hat).sum(0).to(weight.dtype) if need_w else None
+            grad_b = g.sum(0).to(bias.dtype) if need_b else None
+        else:
+            grad, grad_w, grad_b = fmoe_native.layer_norm_backward(grad_out, grad_total, rows, mean.contiguous(), rstd.contiguous(), weight, bias,
+                                                                   need[0] or need[1], need_w, need_b)
         return grad if need[0] else None, grad if need[1] else None, grad_w, grad_b, None
+
+
+def _norm_rows(inp, residual, weight, bias, eps):
+    """:class:`LayerNorm` of rows; its node in native code where that takes the tensors and nothing has to see a Python one."""
+    module = _lib.load_layer_call()
+    if module is not None and nothing_watches(*(t for t in (inp, residual, weight, bias) if t is not None)):
+        out = module.layer_norm(inp, residual, weight, bias, eps)
+        if out is not None:
+            return out
+    return LayerNorm.apply(inp, residual, weight, bias, eps)
 
 
 def layer_norm(inp, weight=None, bias=None, eps=1e-5):
     r"""``torch.nn.functional.layer_norm`` over the last dimension of ``inp`` (float32, bfloat16 or float16, any leading shape) in one
     pass: what comes before, or after, the layer in a transformer block (examples/transformer-xl/mem_transformer.py:379-409).
     ``weight`` and ``bias`` ``[features]``, or ``None``, may be float32 beside 16-bit rows; statistics are float32."""
-    return LayerNorm.apply(_as_rows(inp), None, weight, bias, eps).view(inp.shape)
+    out = _norm_rows(_as_rows(inp), None, weight, bias, eps)
+    return out if inp.dim() == 2 else out.view(inp.shape)
 
 
 def add_layer_norm(inp, residual, weight=None, bias=None, eps=1e-5):
@@ -807,8 +835,8 @@ def add_layer_norm(inp, residual, weight=None, bias=None, eps=1e-5):
     results come back in one pass too."""
     if inp.shape != residual.shape:
         raise ValueError(f"inp is {tuple(inp.shape)} and residual {tuple(residual.shape)}")
-    out, total = LayerNorm.apply(_as_rows(inp), _as_rows(residual), weight, bias, eps)
-    return out.view(inp.shape), total.view(inp.shape)
+    out, total = _norm_rows(_as_rows(inp), _as_rows(residual), weight, bias, eps)
+    return (out, total) if inp.dim() == 2 else (out.view(inp.shape), total.view(inp.shape))
 
 
 class AllGather(Function):

@@ -6,7 +6,7 @@ all positive, are off by ``(16 + N / 64) 2^-24`` more."""
 import pytest
 import torch
 
-from fastermoe_amd import functions
+from fastermoe_amd import _lib, functions
 from fastermoe_amd.gates import GShardGate, SwitchGate
 
 pytestmark = pytest.mark.gpu
@@ -208,7 +208,10 @@ def test_gradients_against_differences(device):
     assert abs(float((g.double() * v).sum()) - want) <= 1e-5 * float((g.double() * v).abs().sum()) + 1e-9
 
 
-def test_second_derivatives_and_one_gradient_alone(device):
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives_and_one_gradient_alone(native, device, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_lib, "_layer_call", None)
     logits, idx = _inputs(40, 6, 2, "f32")
     logits.requires_grad_(True)
     loss, counts, prob = functions.balance_loss(logits, idx)
@@ -259,3 +262,31 @@ def test_another_stream_and_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step())), k
+
+
+def test_both_nodes_give_the_same_bits(device, monkeypatch):
+    """The node in native code and the Python one."""
+    logits, idx = _inputs(500, 30, 2, "bf16", drop=0.1)
+    mask = torch.rand(500, device=device) < 0.1
+    g = torch.randn(30, device=device)
+
+    def run():
+        leaf = logits.detach().requires_grad_(True)
+        loss, counts, prob = functions.balance_loss(leaf, idx, "slot", mask)
+        return loss.detach(), counts, prob.detach(), torch.autograd.grad([loss, prob], leaf, [torch.tensor(2.0, device=device), g])[0]
+
+    native = run()
+    assert type(functions.balance_loss(logits.requires_grad_(True), idx)[0].grad_fn).__name__ != "BalanceLossBackward"
+    monkeypatch.setattr(_lib, "_layer_call", None)
+    assert type(functions.balance_loss(logits, idx)[0].grad_fn).__name__ == "BalanceLossBackward"
+    assert all(torch.equal(a, b) for a, b in zip(native, run()))
+
+
+def test_saved_tensors_may_come_back_otherwise(device):
+    logits, idx = _inputs(60, 9, 2, "f32")
+    logits.requires_grad_(True)
+    want, = torch.autograd.grad(functions.balance_loss(logits, idx)[0], logits)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(device).t().contiguous().t()):
+        loss = functions.balance_loss(logits, idx)[0]
+    got, = torch.autograd.grad(loss, logits)
+    assert torch.equal(got, want)

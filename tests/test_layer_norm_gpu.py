@@ -6,7 +6,7 @@ of which a lane adds ``d / 64`` one after the other before some sixteen more ste
 import pytest
 import torch
 
-from fastermoe_amd import functions
+from fastermoe_amd import _lib, functions
 
 pytestmark = pytest.mark.gpu
 ULP32 = 2.0 ** -24
@@ -288,3 +288,62 @@ def test_checkpointed_and_module_parameters(device):
     want = torch.autograd.grad(ref(x64), [x64, ref.weight, ref.bias], dy.double())
     for g, e in zip(got, want):
         assert torch.allclose(g.double(), e, rtol=1e-5, atol=1e-5)
+
+
+def _twice(function, leaves, weights):
+    """Gradients of a sum of squares of the gradients."""
+    outs = function(*leaves)
+    outs = outs if isinstance(outs, tuple) else (outs,)
+    first = torch.autograd.grad(outs, leaves, weights[:len(outs)], create_graph=True)
+    return torch.autograd.grad(sum(g.double().square().sum() for g in first), leaves, materialize_grads=True)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives(native, device, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_lib, "_layer_call", None)
+    torch.manual_seed(1)
+    leaves = [torch.randn(*s, device=device) for s in ((5, 24), (5, 24), (24,), (24,))]
+    dy, ds = torch.randn(5, 24, device=device), torch.randn(5, 24, device=device)
+    got = _twice(functions.add_layer_norm, [t.clone().requires_grad_(True) for t in leaves], [dy, ds])
+
+    def plain(x, r, w, b):
+        s = x + r
+        return (s - s.mean(1, keepdim=True)) * (s.var(1, correction=0, keepdim=True) + 1e-5).rsqrt() * w + b, s
+
+    want = _twice(plain, [t.double().requires_grad_(True) for t in leaves], [dy.double(), ds.double()])
+    for g, e in zip(got, want):
+        assert torch.allclose(g.double(), e, rtol=1e-3, atol=1e-3 * float(e.abs().max()) + 1e-12)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_both_nodes_give_the_same_bits(dtype, device, monkeypatch):
+    """The node in native code and the Python one."""
+    t = TYPES[dtype]
+    x, r, dy, ds = (torch.randn(70, 200, device=device).to(t) for _ in range(4))
+    w, b = torch.randn(200, device=device), torch.randn(200, device=device)
+
+    def run():
+        leaves = [v.detach().requires_grad_(True) for v in (x, r, w, b)]
+        y, s = functions.add_layer_norm(*leaves)
+        z = functions.layer_norm(leaves[0], None, leaves[3] if dtype == "f32" else None)
+        return (y.detach(), s.detach(), z.detach()) + torch.autograd.grad([y, s, z], leaves, [dy, ds, dy])
+
+    native = run()
+    assert type(functions.layer_norm(x.requires_grad_(True)).grad_fn).__name__ != "LayerNormBackward"
+    monkeypatch.setattr(_lib, "_layer_call", None)
+    assert type(functions.layer_norm(x).grad_fn).__name__ == "LayerNormBackward"
+    assert all(torch.equal(a, e) for a, e in zip(native, run()))
+
+
+def test_saved_tensors_may_come_back_otherwise(device):
+    """Saved-tensor hooks hand back equal tensors that lie elsewhere, and in another order."""
+    x = torch.randn(33, 48, device=device, requires_grad=True)
+    w = torch.randn(48, device=device, requires_grad=True)
+    dy = torch.randn(33, 48, device=device)
+    want = torch.autograd.grad(functions.layer_norm(x, w), [x, w], dy)
+    back = lambda t: t.t().contiguous().t() if t.dim() == 2 else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: back(t.to(device))):
+        y = functions.layer_norm(x, w)
+    got = torch.autograd.grad(y, [x, w], dy)
+    assert all(torch.equal(a, e) for a, e in zip(want, got))
