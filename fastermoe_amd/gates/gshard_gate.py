@@ -3,7 +3,8 @@ r"""GShard top-2 gate: balance loss, per-expert capacity, random drop of the sec
 import torch
 
 from .naive_gate import NaiveGate
-from .utils import capacity_of, limit_by_capacity
+from .utils import balance_loss_kernel_applies, capacity_of, limit_by_capacity
+from ..functions import balance_loss
 
 
 class GShardGate(NaiveGate):
@@ -21,6 +22,9 @@ class GShardGate(NaiveGate):
         # [n_tokens, 2] index tensor, so its "top-1" list is the flattened list of BOTH choices of
         # every token (gshard_gate.py:23-31): c_e is the number of (token, choice) slots that name
         # expert e over the number of tokens, m_e the mean softmax probability of expert e.
+        if logits.dtype == torch.float32 and balance_loss_kernel_applies(logits):
+            return balance_loss(logits, topk_idx)[0]
+        # (16-bit logits: their mean probabilities are of 16 bits, which the kernel's are not)
         n_tokens = logits.shape[0]
         c_e = torch.bincount(topk_idx.reshape(-1), minlength=self.tot_expert).to(torch.float) / n_tokens
         m_e = torch.softmax(logits, dim=1).mean(dim=0)

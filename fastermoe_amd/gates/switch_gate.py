@@ -3,7 +3,8 @@ balance loss over the surviving tokens (behaviour of fmoe/gates/switch_gate.py:1
 import torch
 
 from .naive_gate import NaiveGate
-from .utils import capacity_of, limit_by_capacity
+from .utils import balance_loss_kernel_applies, capacity_of, limit_by_capacity
+from ..functions import balance_loss
 
 
 class SwitchGate(NaiveGate):
@@ -21,7 +22,8 @@ class SwitchGate(NaiveGate):
             # uniform in [1-eps, 1+eps], ADDED to the logits as in switch_gate.py:30-34
             eps = self.switch_eps
             logits = logits + (1.0 - eps + 2 * eps * torch.rand_like(logits))
-        prob = torch.softmax(logits.float(), dim=-1)   # the loss needs every expert's probability
+        logits = logits.float()
+        prob = torch.softmax(logits, dim=-1)   # the loss needs every expert's probability
         top1_score, top1_idx = prob.max(dim=-1, keepdim=True)
         top1_score = top1_score.to(inp.dtype)
 
@@ -30,6 +32,9 @@ class SwitchGate(NaiveGate):
 
         # fraction of the surviving tokens per expert x summed probability per expert, both over
         # the number of survivors (switch_gate.py:46-58)
+        if balance_loss_kernel_applies(logits):
+            self.set_loss(balance_loss(logits, top1_idx, per="slot")[0])
+            return top1_idx, top1_score
         kept = top1_idx[top1_idx >= 0]
         fraction = torch.bincount(kept, minlength=self.tot_expert).to(torch.float) / kept.numel()
         prob_sum = prob.sum(dim=0) / kept.numel()

@@ -1,10 +1,11 @@
-r"""Capacity helpers of the gates (fmoe/gates/utils.py:9-26)."""
+r"""Capacity helpers of the gates (fmoe/gates/utils.py:9-26), and when their balance loss is the kernel's."""
 import math
+import os
 
 import torch
 
 from .. import fmoe_native
-from ..functions import _attach_route, _route_launch, count_by_gate
+from ..functions import _attach_route, _route_launch, count_by_gate, nothing_watches
 
 
 def limit_by_capacity(topk_idx, num_expert, world_size, capacity):
@@ -38,3 +39,10 @@ def capacity_of(rates, training, n_tokens):
     r"""Slots an expert may take: ``rates = (train, eval)`` factors of the token count, rounded up
     (fmoe/gates/gshard_gate.py:36-37, switch_gate.py:40-41)."""
     return math.ceil(rates[0 if training else 1] * n_tokens)
+
+
+def balance_loss_kernel_applies(logits):
+    r"""Whether a gate's balance loss over ``logits`` is :func:`~fastermoe_amd.functions.balance_loss`, which reads nothing on the host (boolean
+    indexing and ``torch.bincount`` do): GPU tensors that it takes, unless ``FMOE_BALANCE_LOSS_KERNEL=0`` keeps the torch operators or something has to see them."""
+    return (logits.is_cuda and logits.dim() == 2 and logits.shape[0] > 0 and fmoe_native.balance_loss_supported(logits.shape[1], logits.dtype)
+            and os.environ.get("FMOE_BALANCE_LOSS_KERNEL", "1") != "0" and nothing_watches(logits))
