@@ -492,6 +492,35 @@ class MOEExpertMLP(Function):
         return g_inp, None, gw1, gb1, gw2, gb2, None
 
 
+class MOEExpertMLPCheckpointed(Function):
+    r""":class:`MOEExpertMLP` with what the backward needs of the activation kept in 8 bits, as :class:`MOERoutedMLPCheckpointed` does."""
+
+    @staticmethod
+    def forward(ctx, inp, fwd_expert_count, w1, b1, w2, b2, activation):
+        inp = inp.contiguous()
+        keep_pre = activation == _lib.ACT_GELU
+        mid, pre = fmoe_native.linear_act_forward(inp, fwd_expert_count, w1, b1, activation, keep_pre)
+        n = int(fmoe_native._host_counts("fwd_expert_count", fwd_expert_count).sum())   # (the rows behind the counted ones are nobody's)
+        _, held, scale = fmoe_native.act_checkpoint_forward((pre if keep_pre else mid)[:n], activation, with_act=False)
+        del pre
+        out = fmoe_native.linear_forward(mid, fwd_expert_count, w2, b2)
+        ctx.save_for_backward(inp, fwd_expert_count, w1, b1, w2, b2, held, scale)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        inp, fwd_expert_count, w1, b1, w2, b2, held, scale = ctx.saved_tensors
+        n = held.shape[0]
+        grad_out = grad_out.contiguous()
+        g_mid = fmoe_native.linear_dact_backward(grad_out, fwd_expert_count, w2, None, _lib.ACT_NONE)
+        _, mid = fmoe_native.act_checkpoint_backward(g_mid[:n], held, scale, ctx.activation, in_place=True)
+        gw2, gb2 = fmoe_native.linear_weight_backward(grad_out[:n], mid, fwd_expert_count, w2, b2)
+        g_inp, gw1, gb1 = fmoe_native.linear_backward(g_mid, inp, fwd_expert_count, w1, b1)
+        return g_inp, None, gw1, gb1, gw2, gb2, None
+
+
 class MOERoutedMLP(Function):
     r"""``MOEScatter`` -> ``Linear -> activation -> Linear`` (fmoe/functions.py:196-248,
     fmoe/transformer.py:22-30) over the rows as the routing kernels left them, with nothing read
@@ -539,6 +568,52 @@ class MOERoutedMLP(Function):
         rows = fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)
         gw1, gb1 = fmoe_native.linear_wgrad_dev(g_pre, rows, w1, table, n_slots, b1 is not None)
         return g_inp, gw1, gb1, gw2, gb2, None, None, None, None, None, None
+
+
+class MOERoutedMLPCheckpointed(Function):
+    r""":class:`MOERoutedMLP` with what the backward needs of the activation kept in 8 bits (``fmoe_native.act_checkpoint_forward``): the
+    pre-activations, or for ReLU and none the activations, whose sign says as much, instead of both in the rows' type: 1.03 bytes an element of ``[rows, d_hidden]``
+    instead of 4 for a 16-bit GELU layer.  The output is the same; the derivative is taken, and the second linear's weight gradient
+    made, where the numbers kept are."""
+
+    @staticmethod
+    def forward(ctx, inp, w1, b1, w2, b2, pos_buf, slot_to_row, table, top_k, activation):
+        inp = inp.contiguous()
+        n_slots = pos_buf.numel()
+        keep_pre = activation == _lib.ACT_GELU
+        n_expert, d_hidden, d_model = w1.shape
+        in_loader = (inp.numel() * inp.element_size() < (1 << 31)
+                     and not fmoe_native.linear_dev_reads_rows(n_slots, n_expert, d_model, d_hidden, inp.dtype, activation, keep_pre))
+        src = inp if in_loader else fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)
+        mid, pre = fmoe_native.linear_forward_dev(src, w1, b1, table, n_slots, activation, keep_pre,
+                                                  row_index=pos_buf if in_loader else None, index_div=top_k)
+        del src   # (its memory serves the output, which is as large)
+        _, held, scale = fmoe_native.act_checkpoint_forward(pre if keep_pre else mid, activation, with_act=False, table=table)
+        del pre
+        out, _ = fmoe_native.linear_forward_dev(mid, w2, b2, table, n_slots)
+        ctx.save_for_backward(inp, w1, b1, w2, b2, pos_buf, slot_to_row, table, held, scale)
+        ctx.moe_args = top_k, activation
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        inp, w1, b1, w2, b2, pos_buf, slot_to_row, table, held, scale = map(_as_chunks, ctx.saved_tensors)
+        top_k, activation = ctx.moe_args
+        n_slots = pos_buf.numel()
+        grad_out = grad_out.contiguous()
+        g_pre, mid = fmoe_native.act_checkpoint_backward(fmoe_native.linear_dgrad_dev(grad_out, w2, table, n_slots), held, scale, activation,
+                                                         table=table, in_place=True)
+        gw2, gb2 = fmoe_native.linear_wgrad_dev(grad_out, mid, w2, table, n_slots, b2 is not None)
+        del mid
+        g_inp = None
+        if ctx.needs_input_grad[0]:
+            g_rows = fmoe_native.linear_dgrad_dev(g_pre, w1, table, n_slots)
+            g_inp = fmoe_native.reduce_slots(g_rows, slot_to_row, inp.shape[0], top_k)
+            del g_rows
+        rows = fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)
+        gw1, gb1 = fmoe_native.linear_wgrad_dev(g_pre, rows, w1, table, n_slots, b1 is not None)
+        return g_inp, gw1, gb1, gw2, gb2, None, None, None, None, None
 
 
 class MOELayer(Function):

@@ -82,6 +82,8 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     # rows and CPU counts it can read (fmoe/layers.py:117-140).
     own = (inp.is_cuda and gate.is_cuda and inp.dim() == 2 and inp.shape[0] > 0
            and gate.numel() == inp.shape[0] * topk and fused and _own_expert_path(expert_fn, experts))
+    # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way)
+    enable_fuse = enable_fuse and not (getattr(experts, "act_checkpoint", False) and experts._checkpoints(inp))
     if own:
         _single_worker(world_size, "count_by_gate")
         enable_fuse = enable_fuse and not experts.unchunked_is_faster(inp, gate.numel())

@@ -5,25 +5,49 @@ import torch
 import torch.nn as nn
 
 from . import _lib, fmoe_native
-from .functions import MOEExpertMLP, MOERoutedMLP, layer_call, nothing_watches
+from .functions import (MOEExpertMLP, MOEExpertMLPCheckpointed, MOERoutedMLP, MOERoutedMLPCheckpointed, _no_hooks, add_layer_norm,
+                        layer_call, layer_norm, nothing_watches)
 from .gates import NaiveGate
 from .layers import FMoE, FMoELinear
 
 
 class _Expert(nn.Module):
     r"""All experts of a worker as two grouped linears around an activation
-    (fmoe/transformer.py:10-30)."""
+    (fmoe/transformer.py:10-30).  ``act_checkpoint`` (or ``FMOE_ACT_CHECKPOINT=1``): a training step keeps what its backward needs of
+    the activation in 8 bits."""
+
+    act_checkpoint = False
 
     def __init__(self, num_expert, d_model, d_hidden, activation, rank=0, bias=True):
         super().__init__()
         self.htoh4 = FMoELinear(num_expert, d_model, d_hidden, bias=bias, rank=rank)
         self.h4toh = FMoELinear(num_expert, d_hidden, d_model, bias=bias, rank=rank)
         self.activation = activation
+        if os.environ.get("FMOE_ACT_CHECKPOINT", "0") == "1":
+            self.act_checkpoint = True
+
+    def _saves(self, inp):
+        """Whether a backward through these experts may come."""
+        return torch.is_grad_enabled() and (inp.requires_grad or any(
+            p is not None and p.requires_grad for p in (self.htoh4.weight, self.htoh4.bias, self.h4toh.weight, self.h4toh.bias)))
+
+    def _checkpoints(self, inp):
+        r"""Whether this step keeps its activations in 8 bits; an error where it is to and cannot."""
+        if not self.act_checkpoint or not inp.is_cuda or not self._saves(inp):
+            return False
+        if self._epilogue_activation() is None:
+            raise NotImplementedError(f"act_checkpoint takes GELU, ReLU or no activation, got {self.activation!r}")
+        if not fmoe_native.act_checkpoint_supported(inp.dtype):
+            raise NotImplementedError(f"act_checkpoint does not take {inp.dtype}")
+        return True
 
     def forward(self, inp, fwd_expert_count):
         # GELU (exact), ReLU or no activation: one autograd node with the activation in the GEMM
         # epilogues (FMOE_EXPERT_EPILOGUE=0 keeps the three modules apart, as the reference runs them)
         code = self._epilogue_activation()
+        if self._checkpoints(inp):
+            return MOEExpertMLPCheckpointed.apply(inp, fwd_expert_count, self.htoh4.weight, self.htoh4.bias,
+                                                  self.h4toh.weight, self.h4toh.bias, code)
         # (float64 keeps torch's activation: the epilogue's GELU is evaluated in single precision)
         if (code is not None and inp.is_cuda and inp.dtype in (torch.float32, torch.bfloat16, torch.float16)
                 and os.environ.get("FMOE_EXPERT_EPILOGUE", "1") != "0"):
@@ -45,20 +69,23 @@ class _Expert(nn.Module):
         if table is None:
             table = fmoe_native.segment_table(counts_dev, pos_buf.numel())
         params = (self.htoh4.weight, self.htoh4.bias, self.h4toh.weight, self.h4toh.bias)
-        save = torch.is_grad_enabled() and (inp.requires_grad or any(p is not None and p.requires_grad for p in params))
-        return MOERoutedMLP.apply(inp, *params, pos_buf, slot_to_row, table, top_k, code, save)
+        if self._checkpoints(inp):
+            return MOERoutedMLPCheckpointed.apply(inp, *params, pos_buf, slot_to_row, table, top_k, code)
+        return MOERoutedMLP.apply(inp, *params, pos_buf, slot_to_row, table, top_k, code, self._saves(inp))
 
     def routed_layer(self, inp, gate_w, gate_b, score, routing, top_k):
         r"""The layer's output from its input as one call: with the gate's linear layer ``gate_w``, ``gate_b`` inside it, or
         over the ``score`` and ``routing`` (``pos_buf``, ``slot_to_row`` and the segment table) of a gate outside.  ``None``
         where that call does not apply: a subclass, replaced linears, another activation, tensors or sizes that it does not
-        take, or somebody who watches the operators."""
+        take, activations that are kept in 8 bits, or somebody who watches the operators."""
         first, second = self._modules.get("htoh4"), self._modules.get("h4toh")
         if type(self) is not _Expert or type(first) is not FMoELinear or type(second) is not FMoELinear:
             return None
         try:
             params = [linear._parameters[name] for linear in (first, second) for name in ("weight", "bias")]
         except KeyError:   # (parametrised, or a view that a sharding wrapper put there)
+            return None
+        if self.act_checkpoint and self._checkpoints(inp):
             return None
         code = self._epilogue_activation()
         if code is None or params[0] is None or params[2] is None or not nothing_watches(inp, *(t for t in (gate_w, gate_b, score, *params) if t is not None)):
@@ -135,3 +162,47 @@ class FMoETransformerMLP(FMoE):
         inp = inp.reshape(-1, self.d_model)
         output = super().forward(inp)
         return output.reshape(original_shape)
+
+    @property
+    def act_checkpoint(self):
+        r"""Whether a training step keeps what its backward needs of the experts' activations in 8 bits (off; ``FMOE_ACT_CHECKPOINT=1``
+        turns it on): the same output, a quarter of the memory, gradients made where the numbers kept are.  The fused pipeline
+        (``enable_fuse``) stands back for it."""
+        return getattr(self.experts, "act_checkpoint", False)
+
+    @act_checkpoint.setter
+    def act_checkpoint(self, on):
+        if not isinstance(self.experts, _Expert):
+            raise AttributeError("act_checkpoint is a matter of this package's own experts")
+        self.experts.act_checkpoint = bool(on)
+
+
+class FMoEPositionwiseFF(FMoETransformerMLP):
+    r"""The layer in a transformer block, with the layer norm and the residual around it (``CustomizedMoEPositionwiseFF``,
+    examples/transformer-xl/mem_transformer.py:379-409): ``x + layer(norm(x))`` with ``pre_lnorm``, else ``norm(x + layer(x))``, with dropout on
+    the layer's output.  Further arguments are those of :class:`FMoETransformerMLP`."""
+
+    def __init__(self, *args, pre_lnorm=False, dropout=0.0, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.layer_norm = nn.LayerNorm(self.d_model)
+        self.pre_lnorm = pre_lnorm
+        self.dropout = nn.Dropout(dropout)
+
+    def _norm_kernel_applies(self, *tensors):
+        """Whether calling ``layer_norm`` is the kernel on its parameters and nothing else."""
+        norm, first = self.layer_norm, tensors[0]
+        return (type(norm) is nn.LayerNorm and _no_hooks(norm) and norm.normalized_shape == (self.d_model,) and first.is_cuda
+                and fmoe_native.layer_norm_supported(first.dtype) and not torch.is_autocast_enabled()
+                and all(t.dtype == first.dtype and t.device == first.device and t.shape == first.shape for t in tensors)
+                and all(p is None or (p.device == first.device and p.dtype in (first.dtype, torch.float32)) for p in (norm.weight, norm.bias))
+                and (norm.weight is None or norm.bias is None or norm.weight.dtype == norm.bias.dtype))
+
+    def forward(self, inp):
+        norm = self.layer_norm
+        if self.pre_lnorm:
+            x = layer_norm(inp, norm.weight, norm.bias, norm.eps) if self._norm_kernel_applies(inp) else norm(inp)
+            return inp + self.dropout(super().forward(x))
+        out = self.dropout(super().forward(inp))
+        if self._norm_kernel_applies(out, inp):
+            return add_layer_norm(out, inp, norm.weight, norm.bias, norm.eps)[0]
+        return norm(inp + out)

@@ -11,7 +11,7 @@ import importlib
 import sys
 
 import fastermoe_amd as _impl
-from fastermoe_amd import DistributedGroupedDataParallel, FMoE, FMoELinear, FMoETransformerMLP
+from fastermoe_amd import DistributedGroupedDataParallel, FMoE, FMoELinear, FMoEPositionwiseFF, FMoETransformerMLP
 
 _MODULES = ("layers", "transformer", "functions", "fused_functions", "distributed", "gates", "gates.base_gate",
             "gates.naive_gate", "gates.gshard_gate", "gates.switch_gate", "gates.zero_gate", "gates.noisy_gate",
@@ -23,4 +23,4 @@ for _name in _MODULES:
         globals()[_name] = _mod
 del _name, _mod
 
-__all__ = ["FMoE", "FMoELinear", "FMoETransformerMLP", "DistributedGroupedDataParallel"]
+__all__ = ["FMoE", "FMoELinear", "FMoETransformerMLP", "FMoEPositionwiseFF", "DistributedGroupedDataParallel"]
