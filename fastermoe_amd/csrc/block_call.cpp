@@ -253,7 +253,7 @@ PyObject *fmoe_block_balance_loss(PyObject *, PyObject *const *args, Py_ssize_t 
     if (!on_gpu(logits) || !on_gpu(idx) || logits.dim() != 2 || dtype_code(logits) < 0 || idx.device() != logits.device() || idx.scalar_type() != at::kLong)
         Py_RETURN_NONE;
     const int64_t n = logits.size(0), e = logits.size(1);
-    if (e < 1 || e > 8192 || n > INT32_MAX / 8 || idx.numel() > INT32_MAX || idx.numel() % (n ? n : 1) != 0 || (n && !idx.numel())) Py_RETURN_NONE;
+    if (e < 1 || e > 8192 || n > INT32_MAX / 8 || idx.numel() > INT32_MAX || idx.numel() % (n ? n : 1) != 0 || (n == 0) != (idx.numel() == 0)) Py_RETURN_NONE;
     if (mask.defined() && (!on_gpu(mask) || mask.device() != logits.device() || mask.scalar_type() != at::kBool || mask.numel() != n || !mask.is_contiguous()))
         Py_RETURN_NONE;
     variable_list out;

@@ -983,7 +983,7 @@ def balance_loss_forward(logits, topk_idx, mask, per_slot):
     :func:`balance_loss_backward`."""
     dt, n, e = _balance_args(logits, mask)
     _near("topk_idx", _dev("topk_idx", topk_idx, torch.int64), logits.device)
-    if topk_idx.numel() % max(n, 1) or (n and not topk_idx.numel()):
+    if topk_idx.numel() % max(n, 1) or (n == 0) != (topk_idx.numel() == 0):
         raise ValueError(f"topk_idx has {topk_idx.numel()} entries, expected as many for each of {n} tokens")
     k = topk_idx.numel() // n if n else 1
     lib = _lib.load()

@@ -95,7 +95,7 @@ def test_refusals_on_the_gpu(device):
         (ValueError, lambda: functions.layer_norm(x, eps=float("nan"))), (ValueError, lambda: functions.layer_norm(x[:, :0])),
         (TypeError, lambda: functions.add_layer_norm(x, x.half())), (ValueError, lambda: functions.add_layer_norm(x, x.cpu())),
         (ValueError, lambda: functions.balance_loss(x.double(), idx)), (TypeError, lambda: functions.balance_loss(x, idx.int())),
-        (ValueError, lambda: functions.balance_loss(x, idx[:3])), (ValueError, lambda: functions.balance_loss(x, idx[:0])),
+        (ValueError, lambda: functions.balance_loss(x[:0], idx)), (ValueError, lambda: functions.balance_loss(x, idx[:3])), (ValueError, lambda: functions.balance_loss(x, idx[:0])),
         (ValueError, lambda: functions.balance_loss(x, idx.cpu())), (ValueError, lambda: functions.balance_loss(x, idx, mask=idx[:3])),
         (ValueError, lambda: functions.balance_loss(x[0], idx)), (ValueError, lambda: functions.balance_loss(torch.zeros(1, 8193, device=device), idx[:1])),
         (TypeError, lambda: functions.act_checkpoint(x.double(), None)), (ValueError, lambda: functions.act_checkpoint(x, 5)),
@@ -111,3 +111,46 @@ def test_refusals_on_the_gpu(device):
             fmoe_native.act_checkpoint_backward(x, *bad, 0)
     with pytest.raises(ValueError):
         fmoe_native.act_checkpoint_forward(x, 0, table=torch.zeros(3, dtype=torch.int32, device=device))
+
+
+@pytest.mark.gpu
+def test_under_inference_mode(device):
+    x, r = torch.randn(30, 64, device=device), torch.randn(30, 64, device=device)
+    w = torch.randn(64, device=device, requires_grad=True)
+    idx = x.topk(2, dim=1).indices
+
+    def run():
+        return (functions.layer_norm(x, w), *functions.add_layer_norm(x, r, w, w), *functions.balance_loss(x, idx), functions.act_checkpoint(x, torch.nn.GELU()))
+
+    want = run()
+    with torch.inference_mode():
+        got = run()
+        inner = functions.layer_norm(x + 0, w)      # (of a tensor made here)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0].requires_grad and torch.equal(inner, got[0])
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(device):
+    """Each call's workspace is its own: forward and backward passes that overlap give what they give alone."""
+    gen = torch.Generator(device=device).manual_seed(4)
+    jobs = [torch.randn(n, 512, device=device, generator=gen) for n in (4000, 3000)]
+
+    def run(x):
+        leaf, w = x.detach().requires_grad_(True), torch.ones(512, device=device, requires_grad=True)
+        y = functions.layer_norm(leaf, w)
+        loss, counts, prob = functions.balance_loss(leaf, idx[x.shape[0]])
+        z = functions.act_checkpoint(leaf, torch.nn.GELU())
+        return (y.detach(), loss.detach(), counts, z.detach()) + torch.autograd.grad([y, loss, z], [leaf, w], [x, torch.ones((), device=device), x])
+
+    idx = {x.shape[0]: x.topk(2, dim=1).indices for x in jobs}
+    want = [run(x) for x in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [None] * len(jobs)
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = run(jobs[i])
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
