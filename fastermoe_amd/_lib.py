@@ -168,7 +168,7 @@ def load_layer_call():
         module.bind(address("fmoe_layer_sizes"), address("fmoe_layer_forward"))
         module.bind_block(*map(address, ("fmoe_last_error", "fmoe_layer_norm_forward", "fmoe_layer_norm_backward",
                                          "fmoe_layer_norm_backward_workspace_bytes", "fmoe_balance_loss_forward", "fmoe_balance_loss_backward",
-                                         "fmoe_balance_loss_workspace_bytes")))
+                                         "fmoe_balance_loss_workspace_bytes", "fmoe_act_checkpoint_forward", "fmoe_act_checkpoint_backward")))
         _layer_call = module
     return _layer_call
 

@@ -1,8 +1,8 @@
-// Layer norm and the gate's balance loss as autograd nodes, from Python's tensors to the enqueued kernels (host code).
+// Layer norm and the gate's balance loss as autograd nodes, and rows kept in 8 bits, from Python's tensors to the enqueued kernels (host code).
 //
 // Their kernels take 3 to 20 us on a small training step's tensors.  As Python nodes, a forward and a backward took 138 and 90 us to enqueue,
-// most of it in the backward's thread; a product and its gradient in torch itself take 46.  What a call takes is decided here; None sends it the
-// Python node's way, which says what is wrong with its tensors.
+// most of it in the backward's thread; a product and its gradient in torch itself take 46.  The calls for rows in 8 bits took 9 us each from
+// Python, the kernels of a small batch 5.  What a call takes is decided here; None sends it the way through Python, which says what is wrong with its tensors.
 #include "block_call.hpp"
 
 #include <ATen/ATen.h>
@@ -33,6 +33,8 @@ struct Entries {
     decltype(&fmoe_balance_loss_forward) balance_forward;
     decltype(&fmoe_balance_loss_backward) balance_backward;
     decltype(&fmoe_balance_loss_workspace_bytes) balance_bytes;
+    decltype(&fmoe_act_checkpoint_forward) checkpoint_forward;
+    decltype(&fmoe_act_checkpoint_backward) checkpoint_backward;
 } entry = {};
 
 int dtype_code(const at::Tensor &t) {
@@ -186,13 +188,18 @@ template <size_t N> bool tensors(PyObject *const *args, std::array<at::Tensor, N
     }
     return true;
 }
+// The number behind them; false, with an exception set, where it is none
+bool number(PyObject *arg, long &n) {
+    n = PyLong_AsLong(arg);
+    return n != -1 || !PyErr_Occurred();
+}
 bool on_gpu(const at::Tensor &t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(); }
 
 }  // namespace
 
 PyObject *fmoe_block_bind(PyObject *, PyObject *args) {
-    unsigned long long a[7];
-    if (!PyArg_ParseTuple(args, "KKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6])) return nullptr;
+    unsigned long long a[9];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8])) return nullptr;
     auto set = [&](auto &fn, int i) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(static_cast<uintptr_t>(a[i])); };
     set(entry.last_error, 0);
     set(entry.norm_forward, 1);
@@ -201,6 +208,8 @@ PyObject *fmoe_block_bind(PyObject *, PyObject *args) {
     set(entry.balance_forward, 4);
     set(entry.balance_backward, 5);
     set(entry.balance_bytes, 6);
+    set(entry.checkpoint_forward, 7);
+    set(entry.checkpoint_backward, 8);
     Py_RETURN_NONE;
 }
 
@@ -262,5 +271,82 @@ PyObject *fmoe_block_balance_loss(PyObject *, PyObject *const *args, Py_ssize_t 
         out = BalanceLoss::apply(logits, idx, maybe(mask), (int64_t)(per_slot != 0));
     }
     return Py_BuildValue("NNN", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])), THPVariable_Wrap(std::move(out[2])));
+    END_HANDLE_TH_ERRORS
+}
+
+namespace {
+
+constexpr int64_t kScaleElems = 32;
+// rows that are kept in 8 bits
+bool keeps(const at::Tensor &x, long activation) {
+    return on_gpu(x) && x.dim() == 2 && x.is_contiguous() && dtype_code(x) >= 0 && activation >= FMOE_ACT_NONE && activation <= FMOE_ACT_GELU;
+}
+bool no_or_table(const at::Tensor &t, const at::Tensor &x) {
+    return !t.defined() || (on_gpu(t) && t.device() == x.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= 8);
+}
+PyObject *wrap_or_none(at::Tensor t) {
+    if (t.defined()) return THPVariable_Wrap(std::move(t));
+    Py_RETURN_NONE;
+}
+
+}  // namespace
+
+// act_checkpoint_forward(x, table, activation, with_act): (y or None, held, scale); None where the call does not take these tensors
+PyObject *fmoe_block_checkpoint_forward(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 4 || entry.checkpoint_forward == nullptr) {
+        PyErr_SetString(PyExc_TypeError, "act_checkpoint_forward: 4 arguments, after bind_block");
+        return nullptr;
+    }
+    std::array<at::Tensor, 2> t;
+    long activation, with_act;
+    if (!tensors(args, t) || !number(args[2], activation) || !number(args[3], with_act)) return nullptr;
+    const auto &[x, table] = t;
+    if (!keeps(x, activation) || !no_or_table(table, x)) Py_RETURN_NONE;
+    at::Tensor y, held, scale;
+    {
+        const WithoutLock no_lock;
+        const at::NoGradGuard no_grad;
+        const c10::OptionalDeviceGuard guard(x.device());
+        const int64_t n = x.size(0), d = x.size(1);
+        held = at::empty({n, d}, x.options().dtype(at::kFloat8_e4m3fn));
+        scale = at::empty({n, (d + kScaleElems - 1) / kScaleElems}, x.options().dtype(at::kFloat8_e8m0fnu));
+        if (with_act) y = at::empty({n, d}, x.options());
+        ok(entry.checkpoint_forward(pointer(x), pointer(y), pointer(held), pointer(scale), pointer(table), n, d, dtype_code(x), (int)activation,
+                                    stream_of(x)));
+    }
+    return Py_BuildValue("NNN", wrap_or_none(std::move(y)), THPVariable_Wrap(std::move(held)), THPVariable_Wrap(std::move(scale)));
+    END_HANDLE_TH_ERRORS
+}
+
+// act_checkpoint_backward(grad, held, scale, table, activation, with_mid, in_place): (grad_x, mid or None); None where the call does not take these tensors
+PyObject *fmoe_block_checkpoint_backward(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 7 || entry.checkpoint_backward == nullptr) {
+        PyErr_SetString(PyExc_TypeError, "act_checkpoint_backward: 7 arguments, after bind_block");
+        return nullptr;
+    }
+    std::array<at::Tensor, 4> t;
+    long activation, with_mid, in_place;
+    if (!tensors(args, t) || !number(args[4], activation) || !number(args[5], with_mid) || !number(args[6], in_place)) return nullptr;
+    const auto &[grad, held, scale, table] = t;
+    if (!keeps(grad, activation) || !no_or_table(table, grad)) Py_RETURN_NONE;
+    const int64_t n = grad.size(0), d = grad.size(1);
+    auto is = [&](const at::Tensor &kept, at::ScalarType type, int64_t columns) {
+        return on_gpu(kept) && kept.device() == grad.device() && kept.scalar_type() == type && kept.is_contiguous() &&
+               kept.sizes() == at::IntArrayRef({n, columns});
+    };
+    if (!is(held, at::kFloat8_e4m3fn, d) || !is(scale, at::kFloat8_e8m0fnu, (d + kScaleElems - 1) / kScaleElems)) Py_RETURN_NONE;
+    at::Tensor grad_x, mid;
+    {
+        const WithoutLock no_lock;
+        const at::NoGradGuard no_grad;
+        const c10::OptionalDeviceGuard guard(grad.device());
+        grad_x = in_place ? grad : at::empty({n, d}, grad.options());
+        if (with_mid) mid = at::empty({n, d}, grad.options());
+        ok(entry.checkpoint_backward(pointer(grad), pointer(held), pointer(scale), pointer(grad_x), pointer(mid), pointer(table), n, d,
+                                     dtype_code(grad), (int)activation, stream_of(grad)));
+    }
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(grad_x)), wrap_or_none(std::move(mid)));
     END_HANDLE_TH_ERRORS
 }

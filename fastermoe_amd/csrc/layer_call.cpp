@@ -109,12 +109,17 @@ PyObject *infer(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+PyCFunction fast(PyObject *(*f)(PyObject *, PyObject *const *, Py_ssize_t)) {
+    return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f));
+}
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "The addresses of fmoe_layer_sizes and fmoe_layer_forward."},
-    {"infer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(infer)), METH_FASTCALL, "A layer's output where nothing is differentiated."},
-    {"bind_block", fmoe_block_bind, METH_VARARGS, "The addresses of the library's entry points that the next two call."},
-    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fmoe_block_layer_norm)), METH_FASTCALL, "Layer norm of rows."},
-    {"balance_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fmoe_block_balance_loss)), METH_FASTCALL, "A gate's balance loss."},
+    {"infer", fast(infer), METH_FASTCALL, "A layer's output where nothing is differentiated."},
+    {"bind_block", fmoe_block_bind, METH_VARARGS, "The addresses of the library's entry points that the next ones call."},
+    {"layer_norm", fast(fmoe_block_layer_norm), METH_FASTCALL, "Layer norm of rows."},
+    {"balance_loss", fast(fmoe_block_balance_loss), METH_FASTCALL, "A gate's balance loss."},
+    {"act_checkpoint_forward", fast(fmoe_block_checkpoint_forward), METH_FASTCALL, "Rows in 8 bits, and their activation."},
+    {"act_checkpoint_backward", fast(fmoe_block_checkpoint_backward), METH_FASTCALL, "The backward from rows in 8 bits."},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_layer_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

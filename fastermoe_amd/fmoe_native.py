@@ -823,6 +823,11 @@ def act_checkpoint_forward(x, activation, with_act=True, table=None):
     """``(act(x) or None, held, scale)``: ``x [rows, features]`` in 8 bits (``held``, ``float8_e4m3fn``), 32 elements along a row under
     one power of two (``scale [rows, ceil(features / 32)]``, ``float8_e8m0fnu``), for :func:`act_checkpoint_backward`.  ``table``: a
     segment table; only the rows that its counts add up to are read and written."""
+    module = _lib.load_layer_call()
+    if module is not None:
+        kept = module.act_checkpoint_forward(x, table, activation, with_act)
+        if kept is not None:
+            return kept
     dt = _rows("x", x)
     if not act_checkpoint_supported(x.dtype):
         raise TypeError(f"act_checkpoint_forward does not take {x.dtype}")
@@ -840,6 +845,11 @@ def act_checkpoint_forward(x, activation, with_act=True, table=None):
 def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=None, in_place=False):
     """``(grad * act'(v), act(v) or None)`` with ``v`` the values that ``held`` and ``scale`` stand for.  ``in_place``: the first result
     is written over ``grad``."""
+    module = _lib.load_layer_call()
+    if module is not None:
+        made = module.act_checkpoint_backward(grad, held, scale, table, activation, with_mid, in_place)
+        if made is not None:
+            return made
     dt = _rows("grad", grad)
     if not act_checkpoint_supported(grad.dtype):
         raise TypeError(f"act_checkpoint_backward does not take {grad.dtype}")

@@ -231,3 +231,18 @@ def test_another_stream_and_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step())), k
+
+
+def test_called_from_python_the_same(device, monkeypatch):
+    """Without the extension module: the same bits."""
+    x, g = (torch.randn(40, 100, device=device, dtype=torch.float16) for _ in range(2))
+
+    def run():
+        y, held, scale = fmoe_native.act_checkpoint_forward(x, _lib.ACT_GELU)
+        return (y, held.view(torch.uint8), scale.view(torch.uint8)) + fmoe_native.act_checkpoint_backward(g, held, scale, _lib.ACT_GELU)
+
+    native = run()
+    monkeypatch.setattr(_lib, "_layer_call", None)
+    assert all(torch.equal(a, b) for a, b in zip(native, run()))
+    for act in CODES:
+        check(x, act)
