@@ -7,17 +7,21 @@
 // Statistics, sums and everything between the loads and the one rounding at a store are float32.
 //
 // A row lies in the registers of G lanes, V vectors of 16 bytes to each, between its one load and its one store: G x V is the smallest that
-// holds it (held_forward, held_backward).  Rows longer than any holds are read again for every sum (long_* kernels: 1000 bfloat16 rows of 40000 take
-// 208 us and 317).  Bound by memory (TB/s of what has to move; a large copy on the same card 5.0):
+// holds it (held_forward, held_backward), wherever it begins and whatever its length.  Rows longer than any holds, or shorter than a vector, are read again for
+// every sum (long_* kernels: 1000 bfloat16 rows of 40000 take 208 us and 317).  Bound by memory (TB/s of what has to move; a large copy on the same
+// card 5.0):
 //   rows x features             forward          backward            of it without the parameters' gradients
-//   16384 x 4096 bf16, residual   94 us  5.7        91 us  5.9         84 us  6.4
-//   32768 x 4096 bf16            101     5.3       143     5.6        136     5.9
-//   16384 x 2048 f32, residual    91     5.9        89     6.0         85     6.3
-//   32768 x 1024 bf16             27     4.9        41     4.9         36     5.6
-//   32768 x 500 bf16, any start   18     3.7        27     3.6         22     4.5
-//   509 x 4096 f16, residual      6.1               13                5.2
-//   64 x 4096 bf16, residual      3.8               8.8               4.0
-// (The first with a row read again for every sum and the parameters' gradients in a pass of their own: 358 and 431 us.)
+//   16384 x 4096 bf16, residual   92 us  5.8        91 us  5.9         84 us  6.4
+//   32768 x 4096 bf16             98     5.5       144     5.6        137     5.9
+//   16384 x 2048 f32, residual    92     5.8        88     6.1         83     6.4
+//   32768 x 1024 bf16             27     5.0        41     4.9         36     5.6
+//   65536 x 900 bf16, residual    85     5.5        86     5.5
+//   32768 x 500 bf16              15     4.4        22     4.4         17     5.8
+//   5000 x 12000 bf16, residual   92     5.2       125     3.8
+//   509 x 4096 f16, residual      6.0               13                5.1
+//   64 x 4096 bf16, residual      3.8               8.9               4.1
+// (The first with a row read again for every sum and the parameters' gradients in a pass of their own: 358 and 431 us.  Rows of 900 and 500 whose last
+// elements were loaded and stored apart: 102 and 129, 18 and 27.)
 #include "common.hpp"
 #include "lane_elems.hpp"
 
@@ -28,7 +32,7 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kWavesPerBlock = kBlock / kWave;
-constexpr int kBwdBlock = 1024;      // of the backward over rows in registers
+constexpr int bwd_threads(int v) { return v >= 4 ? 512 : 1024; }   // of the backward over rows in registers: twice the registers for long float32 rows
 constexpr int kBwdMostBlocks = 256;  // and its workgroups at most, each of which leaves sums over its rows
 constexpr int64_t kPartBytes = 4 << 20;
 constexpr int64_t kCacheBytes = 256 << 20;   // of the memory-side cache
@@ -51,7 +55,7 @@ template <int G> __device__ __forceinline__ float lanes_sum(float v) {   // G <=
     }
     return v;
 }
-// NS sums; rows of more than one wave meet in scratch [waves of the workgroup][NS], which the next call must not be handed again
+// NS sums; rows of more than one wave meet in scratch [waves of the workgroup][NS] (another scratch than the call before, whose sums may still be read)
 template <int G, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS], float (*scratch)[NS]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) v[i] = lanes_sum<(G < kWave ? G : kWave)>(v[i]);
@@ -73,58 +77,50 @@ template <int G, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS]
     }
 }
 
-// weight or bias: of the rows' type T or float32 (kind: what the pointer is to; none where it is null)
+// weight or bias: of the rows' type or float32; none where the pointer is null
 struct Param { const void *p; bool f32; };
-// N of them from column c on; `none` where there are none.  WHOLE: d is whole vectors.
-template <typename T, int N, bool WHOLE> __device__ __forceinline__ void load_params(const Param &p, int c, int d, float none, float (&f)[N]) {
+// N of them from column `from` on; `none` where there are none
+template <typename T, int N> __device__ __forceinline__ void load_params(const Param &p, int from, float none, float (&f)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = none;
-    if (!p.p || (WHOLE && c >= d)) return;
-    auto vec = [&](auto *at, int n) { return WHOLE ? (u32x4) * (const AnyVec *)at : load_vec<false>(at, n, false); };
+    if (!p.p) return;
     float t[8];
     if (sizeof(T) == 2 && !p.f32) {
-        Vec<T>::unpack(vec((const T *)p.p + c, d - c), t);
+        Vec<T>::unpack(*(const AnyVec *)((const T *)p.p + from), t);
 #pragma unroll
         for (int i = 0; i < N; ++i) f[i] = t[i];
     } else {
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
-            Vec<float>::unpack(vec((const float *)p.p + c + k, d - c - k), t);
+            Vec<float>::unpack(*(const AnyVec *)((const float *)p.p + from + k), t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) f[k + i] = t[i];
         }
     }
 }
 
-// The lane's vector of row `row` of rows that begin `stride` elements apart, zeros where it has none.  WHOLE: a row is whole vectors.
-template <typename T, bool WHOLE, bool ONCE>
-__device__ __forceinline__ u32x4 load_row(const T *p, int64_t stride, int64_t row, int64_t rows, int c, int d) {
-    constexpr int N = Vec<T>::N;
-    const bool live = row < rows;
-    if constexpr (WHOLE) {
-        u32x4 v = {0, 0, 0, 0};
-        if (live && c < d) {
-            const AnyVec *at = (const AnyVec *)(p + row * stride + c);
-            v = ONCE ? __builtin_nontemporal_load(at) : *at;
-        }
-        return v;
-    } else {
-        return load_vec<ONCE>(p + row * stride + c, live ? d - c : 0, (row - rows + 1) * stride + c + N <= d);
-    }
+// Where a lane's vector number v lies in a row of d >= N elements: it begins at `from` and its first `skip` elements are another lane's.  The last vector of
+// a row that is not whole vectors ends with the row and overlaps the one before it, whose lane does what the sums need of the elements they
+// share; what both store there is the same.  Lanes behind the row's end take its last vector and none of its elements (skip >= N).
+template <int N> struct Place {
+    int from, skip;
+    __device__ __forceinline__ Place(int vec, int d) : from(vec * N < d - N ? vec * N : d - N), skip(vec * N - from) {}
+    __device__ __forceinline__ bool own(int i) const { return i >= skip; }
+};
+
+// The lane's vector of row `row` of `rows`, of the last one where there is none.  Always a load, with neither a branch around it nor a look at what it
+// brought, either of which would have everything before its use wait for it.
+template <bool ONCE, typename T> __device__ __forceinline__ u32x4 load_row(const T *p, int64_t stride, int64_t row, int64_t rows, int from) {
+    const AnyVec *at = (const AnyVec *)(p + (row < rows ? row : rows - 1) * stride + from);
+    return ONCE ? (u32x4)__builtin_nontemporal_load(at) : (u32x4)*at;
 }
-template <typename T, bool WHOLE, bool ONCE> __device__ __forceinline__ void store_row(T *p, int c, int d, const u32x4 &v) {
-    if constexpr (WHOLE) {
-        if (c < d) {
-            if (ONCE) __builtin_nontemporal_store(v, (AnyVec *)(p + c));
-            else *(AnyVec *)(p + c) = v;
-        }
-    } else {
-        store_vec<ONCE>(p + c, d - c, v);
-    }
+template <bool ONCE, typename T> __device__ __forceinline__ void store_row(T *p, const u32x4 &v) {
+    if (ONCE) __builtin_nontemporal_store(v, (AnyVec *)p);
+    else *(AnyVec *)p = v;
 }
 
 // ---- forward over rows in registers ------------------------------------------------------
-template <typename T, int G, int V, bool WHOLE>
+template <typename T, int G, int V>
 __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const T *__restrict__ x, int64_t x_stride, const T *__restrict__ r,
                                                                            int64_t r_stride, Param w, Param b, T *__restrict__ sum,
                                                                            T *__restrict__ y, float *__restrict__ mean,
@@ -136,13 +132,14 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
     u32x4 e[V], re[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * G + lane) * N;
-        e[v] = load_row<T, WHOLE, false>(x, x_stride, row, rows, c, d);
-        if (r) re[v] = load_row<T, WHOLE, false>(r, r_stride, row, rows, c, d);
+        const Place<N> at(v * G + lane, d);
+        e[v] = load_row<false>(x, x_stride, row, rows, at.from);
+        if (r) re[v] = load_row<false>(r, r_stride, row, rows, at.from);
     }
     float f[V][8], s[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+        const Place<N> at(v * G + lane, d);
         Vec<T>::unpack(e[v], f[v]);
         if (r) {
             float t[8];
@@ -153,31 +150,34 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
             Vec<T>::unpack(e[v], f[v]);
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[0] += f[v][i];
+        for (int i = 0; i < N; ++i) s[0] += at.own(i) ? f[v][i] : 0.f;
     }
     row_sums<G>(s, scratch[0]);
     const float m = s[0] / (float)d;
     s[0] = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < V; ++v) {
+        const Place<N> at(v * G + lane, d);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             f[v][i] -= m;
-            s[0] += (v * G + lane) * N + i < d ? f[v][i] * f[v][i] : 0.f;
+            s[0] += at.own(i) ? f[v][i] * f[v][i] : 0.f;
         }
+    }
     row_sums<G>(s, scratch[1]);
     const float rs = 1.f / sqrtf(s[0] / (float)d + eps);
     if (row >= rows) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * G + lane) * N;
+        const Place<N> at(v * G + lane, d);
+        if (at.skip >= N) continue;
         float wf[N], bf[N], out[8];
-        load_params<T, N, WHOLE>(w, c, d, 1.f, wf);
-        load_params<T, N, WHOLE>(b, c, d, 0.f, bf);
+        load_params<T, N>(w, at.from, 1.f, wf);
+        load_params<T, N>(b, at.from, 0.f, bf);
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = f[v][i] * rs * wf[i] + bf[i];
-        store_row<T, WHOLE, false>(y + row * d, c, d, Vec<T>::pack(out));
-        if (sum) store_row<T, WHOLE, false>(sum + row * d, c, d, e[v]);
+        store_row<false>(y + row * d + at.from, Vec<T>::pack(out));
+        if (sum) store_row<false>(sum + row * d + at.from, e[v]);
     }
     if (mean && lane == 0) {
         mean[row] = m;
@@ -185,83 +185,60 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
     }
 }
 
-// The lane's vector of a row to come.  WHOLE: loaded whatever it is, with neither a branch around the load nor a look at what it brought, either of
-// which would have the sums of the row before wait for it; the row is one that there is, and lanes behind its end take its beginning.
-template <typename T, bool WHOLE, bool ONCE>
-__device__ __forceinline__ u32x4 load_ahead(const T *p, int64_t stride, int64_t row, int64_t rows, int c, int d) {
-    if constexpr (WHOLE) {
-        const AnyVec *at = (const AnyVec *)(p + row * stride + (c < d ? c : 0));
-        return ONCE ? (u32x4)__builtin_nontemporal_load(at) : (u32x4)*at;
-    } else {
-        return load_row<T, WHOLE, ONCE>(p, stride, row, rows, c, d);
-    }
-}
-
 // ---- backward over rows in registers -----------------------------------------------------
-// A workgroup takes kRows rows at a time and every gridDim-th such set, with the next set's loads on their way (16384 x 4096: 104 us where a branch
-// or a select made the sums wait for them).  The lanes keep the sums of grad_y h and grad_y of their columns over all of them; at the end the
+// A workgroup takes kRows rows at a time and every gridDim-th such set, with the next set's loads on their way (16384 x 4096: 104 us where a
+// branch or a select made the sums wait for them).  The lanes keep the sums of grad_y h and grad_y of their columns over all of them; at the end the
 // lanes of one column meet in LDS and part[workgroup] gets 2 d sums.  One workgroup of 1024 to a compute unit: two of 512 leave twice the parts (4096 x 8192:
-// 59 us against 68).  One vector to a lane: with two the next set's registers no longer fit beside this one's.
+// 59 us against 68).  One vector to a lane, where the next set's registers fit beside this one's; longer rows take two and no set ahead, in float32
+// four (ahead) or eight in half the lanes (2048 x 8192, residual: 60 us against 78 with two in 1024 lanes; 3600 x 16384 213 against 249 with four, and
+// 192 against 156 without a residual).
 template <int V> struct RowData {
     u32x4 g[V], x[V], gs[V];
     float mean, rstd;
 };
-template <typename T, int G, int V, bool WHOLE, bool ONCE, bool SUM>
-__global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict__ gy, int64_t gy_stride, const T *__restrict__ gs,
+template <typename T, int G, int V, bool ONCE, bool SUM>
+__global__ __launch_bounds__(bwd_threads(V)) void norm_bwd_kernel(const T *__restrict__ gy, int64_t gy_stride, const T *__restrict__ gs,
                                                              int64_t gs_stride, const T *__restrict__ x, int64_t x_stride,
                                                              const float *__restrict__ mean, const float *__restrict__ rstd, Param w,
                                                              T *__restrict__ gx, float *__restrict__ part, int64_t rows, int d) {
-    constexpr int N = Vec<T>::N, kRows = kBwdBlock / G;
-    constexpr bool kAhead = V == 1 || V * N <= 8;
-    __shared__ float scratch[2][kBwdBlock / kWave][2];
-    __shared__ float sums[kRows > 1 ? kBwdBlock * V * N : 1];
+    constexpr int N = Vec<T>::N, kThreads = bwd_threads(V), kRows = kThreads / G;
+    constexpr bool kAhead = V * N <= (kThreads == 512 ? 16 : 8);
+    __shared__ float scratch[2][kThreads / kWave][2];
+    __shared__ float sums[kRows > 1 ? kThreads * V * N : 1];
     const int lane = threadIdx.x % G, mine = threadIdx.x / G;
-    const bool has_sum = WHOLE ? SUM : gs != nullptr;
     auto load = [&](int64_t row, RowData<V> &a) {
-        if constexpr (WHOLE) row = row < rows ? row : rows - 1;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * G + lane) * N;
-            if (has_sum) a.gs[v] = load_ahead<T, WHOLE, ONCE>(gs, gs_stride, row, rows, c, d);
-            a.g[v] = load_ahead<T, WHOLE, ONCE>(gy, gy_stride, row, rows, c, d);
-            a.x[v] = load_ahead<T, WHOLE, ONCE>(x, x_stride, row, rows, c, d);
+            const Place<N> at(v * G + lane, d);
+            if (SUM) a.gs[v] = load_row<ONCE>(gs, gs_stride, row, rows, at.from);
+            a.g[v] = load_row<ONCE>(gy, gy_stride, row, rows, at.from);
+            a.x[v] = load_row<ONCE>(x, x_stride, row, rows, at.from);
         }
         const int64_t at = row < rows ? row : rows - 1;
         a.mean = mean[at];
         a.rstd = rstd[at];
     };
-    // zeros for what load_ahead was not to load
-    auto have = [&](int64_t row, RowData<V> &a) {
-        if constexpr (!WHOLE) return;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const bool in = row < rows && (v * G + lane) * N < d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                a.g[v][j] = in ? a.g[v][j] : 0;
-                a.x[v][j] = in ? a.x[v][j] : 0;
-            }
-        }
-    };
     float wf[V][N], sw[V][N], sb[V][N];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        load_params<T, N, WHOLE>(w, (v * G + lane) * N, d, 1.f, wf[v]);
+        load_params<T, N>(w, Place<N>(v * G + lane, d).from, 1.f, wf[v]);
 #pragma unroll
         for (int i = 0; i < N; ++i) sw[v][i] = sb[v][i] = 0.f;
     }
     int turn = 0;
     // one set's rows: sums, the gradient of the rows, and what they add to the parameters'
     auto use = [&](int64_t row, RowData<V> &a) {
-        have(row, a);
+        const bool live = row < rows;
         float c12[2] = {0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < V; ++v) {
+            const Place<N> at(v * G + lane, d);
             float g[8], h[8];
             Vec<T>::unpack(a.g[v], g);
             Vec<T>::unpack(a.x[v], h);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
+                g[i] = live && at.own(i) ? g[i] : 0.f;
                 h[i] = (h[i] - a.mean) * a.rstd;
                 const float t = g[i] * wf[v][i];
                 c12[0] += t;
@@ -272,22 +249,23 @@ __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict
         }
         row_sums<G>(c12, scratch[turn]);
         turn ^= 1;
-        if (gx && row < rows) {
+        if (gx && live) {
             const float c1 = c12[0] / (float)d, c2 = c12[1] / (float)d;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int c = (v * G + lane) * N;
+                const Place<N> at(v * G + lane, d);
+                if (at.skip >= N) continue;
                 float g[8], h[8], t[8];
                 Vec<T>::unpack(a.g[v], g);
                 Vec<T>::unpack(a.x[v], h);
-                    if (has_sum) Vec<T>::unpack(a.gs[v], t);
+                if (SUM) Vec<T>::unpack(a.gs[v], t);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     h[i] = (h[i] - a.mean) * a.rstd;
                     g[i] = a.rstd * (g[i] * wf[v][i] - c1 - h[i] * c2);
-                    if (has_sum) g[i] += t[i];
+                    if (SUM) g[i] += t[i];
                 }
-                store_row<T, WHOLE, ONCE>(gx + row * d, c, d, Vec<T>::pack(g));
+                store_row<ONCE>(gx + row * d + at.from, Vec<T>::pack(g));
             }
         }
     };
@@ -320,7 +298,16 @@ __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict
     for (int which = 0; which < 2; ++which, out += d) {
         if constexpr (kRows == 1) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) store_elems<false>(out + (v * G + lane) * N, d - (v * G + lane) * N, which ? sb[v] : sw[v]);
+            for (int v = 0; v < V; ++v) {
+                const Place<N> at(v * G + lane, d);
+                if (at.skip == 0) {
+                    __builtin_memcpy(out + at.from, which ? sb[v] : sw[v], N * sizeof(float));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (at.own(i)) out[at.from + i] = which ? sb[v][i] : sw[v][i];
+                }
+            }
         } else {
             __syncthreads();
 #pragma unroll
@@ -329,8 +316,8 @@ __global__ __launch_bounds__(kBwdBlock) void norm_bwd_kernel(const T *__restrict
                 for (int i = 0; i < N; ++i) sums[(mine * V + v) * G * N + i * G + lane] = which ? sb[v][i] : sw[v][i];
             __syncthreads();
             // (a column's place: its vector's number, then which of the vector's elements, then the lane)
-            for (int c = threadIdx.x; c < d; c += kBwdBlock) {
-                const int v = c / (G * N), at = c % (G * N), place = v * G * N + at % N * G + at / N;
+            for (int c = threadIdx.x; c < d; c += kThreads) {
+                const int vec = c / N, place = vec / G * G * N + (c - Place<N>(vec, d).from) * G + vec % G;
                 float s = 0.f;
 #pragma unroll
                 for (int u = 0; u < kRows; ++u) s += sums[u * V * G * N + place];
@@ -448,7 +435,7 @@ __global__ __launch_bounds__(kSumBlock) void norm_param_sum_kernel(const float *
 
 // How a row is held: f(lanes, vectors to each), integral constants; false where nothing holds it
 template <int N, int G, int V, typename F> bool held_by(int64_t d, F &&f) {
-    if (d > (int64_t)G * V * N) return false;
+    if (d < N || d > (int64_t)G * V * N) return false;
     f(std::integral_constant<int, G>{}, std::integral_constant<int, V>{});
     return true;
 }
@@ -463,10 +450,10 @@ template <int N, typename F> bool held_forward(int64_t d, bool one_each, F &&f) 
 }
 template <int N, typename F> bool held_backward(int64_t d, F &&f) {
     if (held_by<N, 8, 1>(d, f) || held_by<N, 32, 1>(d, f) || held_by<N, 64, 1>(d, f) || held_by<N, 128, 1>(d, f) || held_by<N, 256, 1>(d, f) ||
-        held_by<N, 512, 1>(d, f) || held_by<N, 1024, 1>(d, f) || held_by<N, 1024, 2>(d, f))
+        held_by<N, 512, 1>(d, f) || held_by<N, 1024, 1>(d, f))
         return true;
-    if constexpr (N == 4) return held_by<N, 1024, 4>(d, f);
-    return false;
+    if constexpr (N == 4) return held_by<N, 512, 4>(d, f) || held_by<N, 512, 8>(d, f);
+    else return held_by<N, 1024, 2>(d, f);
 }
 
 constexpr int kLongParts = 128;
@@ -506,11 +493,10 @@ extern "C" int fmoe_layer_norm_forward(const void *x, int64_t x_stride, const vo
     with_types(dtype, param_dtype, [&](auto t, auto p) {
         using T = decltype(t);
         using P = decltype(p);
-        const bool whole = row_elems % Vec<T>::N == 0, param_f32 = std::is_same<P, float>::value;
+        const bool param_f32 = std::is_same<P, float>::value;
         const bool held = held_forward<Vec<T>::N>(row_elems, residual || rows < kFewRows, [&](auto g, auto v) {
             constexpr int kThreads = g.value > kBlock ? g.value : kBlock;
-            (whole ? norm_fwd_kernel<T, g.value, v.value, true> : norm_fwd_kernel<T, g.value, v.value, false>)<<<
-                (int)ceil_div(rows, kThreads / g.value), kThreads, 0, st>>>(
+            norm_fwd_kernel<T, g.value, v.value><<<(int)ceil_div(rows, kThreads / g.value), kThreads, 0, st>>>(
                 (const T *)x, x_stride, (const T *)residual, residual_stride, Param{weight, param_f32}, Param{bias, param_f32}, (T *)sum, (T *)y,
                 mean, rstd, rows, (int)row_elems, (float)eps);
         });
@@ -551,14 +537,13 @@ extern "C" int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_strid
         const bool held = rows == 0 || held_backward<Vec<T>::N>(row_elems, [&](auto g, auto v) {
             // (one set to a workgroup, unless the workgroups' sums would be more than kPartBytes, then two: 509 x 4096 float16 16.4 us with
             // 255 workgroups, 13 with 128; 777 x 1302, whose 195 leave 2 MB, 12.1 and 14)
-            const int64_t sets = ceil_div(rows, kBwdBlock / g.value);
+            const int64_t sets = ceil_div(rows, bwd_threads(v.value) / g.value);
             const int64_t blocks = params && sets * 8 * row_elems > kPartBytes ? ceil_div(sets, 2) : sets;
             parts = (int)(blocks < kBwdMostBlocks ? blocks : kBwdMostBlocks);
-            const bool whole = row_elems % Vec<T>::N == 0, once = rows * row_elems * (int64_t)sizeof(T) * (grad_sum ? 4 : 3) > kCacheBytes;
-            auto kernel = !whole ? norm_bwd_kernel<T, g.value, v.value, false, false, false>
-                          : once ? (grad_sum ? norm_bwd_kernel<T, g.value, v.value, true, true, true> : norm_bwd_kernel<T, g.value, v.value, true, true, false>)
-                                 : (grad_sum ? norm_bwd_kernel<T, g.value, v.value, true, false, true> : norm_bwd_kernel<T, g.value, v.value, true, false, false>);
-            kernel<<<parts, kBwdBlock, 0, st>>>((const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride, (const T *)x, x_stride, mean,
+            const bool once = rows * row_elems * (int64_t)sizeof(T) * (grad_sum ? 4 : 3) > kCacheBytes;
+            auto kernel = once ? (grad_sum ? norm_bwd_kernel<T, g.value, v.value, true, true> : norm_bwd_kernel<T, g.value, v.value, true, false>)
+                               : (grad_sum ? norm_bwd_kernel<T, g.value, v.value, false, true> : norm_bwd_kernel<T, g.value, v.value, false, false>);
+            kernel<<<parts, bwd_threads(v.value), 0, st>>>((const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride, (const T *)x, x_stride, mean,
                                            rstd, Param{weight, std::is_same<P, float>::value}, (T *)grad_x,
                                            params ? (float *)workspace : nullptr, rows, (int)row_elems);
         });
