@@ -7,8 +7,14 @@
 // (The gradient does not feel a constant added to u, as the probabilities of a token add up to one: with the counts less
 // their mean, taken before anything is rounded, no two nearly equal numbers are subtracted where the experts are nearly balanced.)
 //
-// L lanes hold a token's logits, V vectors of 16 bytes to each (as many lanes and vectors as the experts need: held_logits), a wave 64 / L tokens; probabilities stay
-// in registers between the one load and the sums over the tokens, which each lane keeps for its experts over all the tokens of its workgroup's range.
+// L lanes hold a token's logits, V vectors of 16 bytes to each (as many lanes and vectors as the experts need: held_logits), a wave 64 / L tokens;
+// probabilities stay in registers between the one load and the sums over the tokens, which each lane keeps for its experts over all the tokens of its
+// workgroup's range.  The logits are read once in each direction, some tokens ahead; at these sizes the chain from the first load over the sums
+// to a second launch's results bounds the forward, the memory the larger backward passes (us, forward and backward):
+//   32768 x 256 bf16, top-8    15.8   9.7        131072 x 64 f32, top-2    17.1  12.5 (5.4 TB/s)      8192 x 1024 f32, top-2   16.8  11.4
+//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      6.8   2.9
+// (A pass for every token's largest logit and sum, one for the sums over the tokens and a workgroup for the results took 158 us of the first's forward,
+// a token to a wave 25 of its backward.)
 #include "common.hpp"
 #include "lane_elems.hpp"
 
@@ -20,7 +26,7 @@ namespace {
 constexpr int kMostExperts = 8192;
 constexpr int kMostParts = 256;      // workgroups of the forward, each of which leaves sums over its tokens
 constexpr int kBwdBlock = 256, kBwdBlocks = 512;
-constexpr int kOneRound = 4;
+constexpr int kFewRounds = 8;
 constexpr int kSumCols = 16, kSumRanges = 64, kSumBlock = kSumCols * kSumRanges;
 constexpr int waves_of(int v) { return v <= 2 ? 16 : v <= 8 ? 8 : 3; }   // of a workgroup of the forward
 constexpr int ahead_of(int v) { return v == 1 ? 4 : v == 2 ? 2 : 1; }    // tokens in flight per lane
@@ -396,9 +402,10 @@ extern "C" int fmoe_balance_loss_forward(const void *logits, const int64_t *topk
         using T = decltype(type);
         held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
             constexpr int kTokens = waves_of(v.value) * (kWave / l.value);
-            // (what one workgroup goes through in kOneRound rounds is not worth a second launch)
+            // (what one workgroup goes through in kFewRounds rounds is not worth a second launch: 1000 x 16 float32, four rounds, 6.0 us, with
+            // four workgroups and the launch that joins them 8.5; 2000 x 16, eight, 8.1 and 8.5)
             const int64_t rounds = ceil_div(n_tokens, kTokens);
-            const int parts = (int)(rounds <= kOneRound ? 1 : rounds < most ? rounds : most);
+            const int parts = (int)(rounds <= kFewRounds ? 1 : rounds < most ? rounds : most);
             balance_sum_kernel<T, l.value, v.value, whole.value><<<parts, waves_of(v.value) * kWave, 0, st>>>(
                 (const T *)logits, topk_idx, (const uint8_t *)token_mask, sums, results, n_tokens, (int)n_expert, (int)top_k);
             if (parts > 1) balance_finish_kernel<<<columns, kSumBlock, 0, st>>>(sums, results, parts, (int)n_expert);
@@ -418,7 +425,8 @@ extern "C" int fmoe_balance_loss_backward(const void *logits, const void *token_
     with_type(dtype, [&](auto type) {
         using T = decltype(type);
         held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
-            // (one token in flight per lane where more would leave compute units without a workgroup)
+            // (one token in flight per lane where more would leave compute units without a workgroup: 16384 x 64 float32 3.6 us, four ahead 4.5;
+            // 32768 x 256 bfloat16 9.7 four ahead, one 20)
             constexpr int kTokens = kBwdBlock / l.value, kAhead = ahead_of(v.value);
             const bool ahead = n_tokens >= kBwdBlocks * kTokens * kAhead;
             (ahead ? balance_bwd_kernel<T, l.value, v.value, whole.value, kAhead> : balance_bwd_kernel<T, l.value, v.value, whole.value, 1>)<<<
