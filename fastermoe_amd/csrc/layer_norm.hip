@@ -456,6 +456,14 @@ template <int N, typename F> bool held_backward(int64_t d, F &&f) {
     else return held_by<N, 1024, 2>(d, f);
 }
 
+// Ranges of the rows, as a launch counts its threads, `lanes` to a row, in 32 bits: f(first row, rows)
+constexpr int64_t kLaunchThreads = INT64_C(1) << 31;
+template <typename F> void in_launches(int64_t rows, int lanes, F &&f) {
+    const int64_t most = kLaunchThreads / lanes;
+    for (int64_t at = 0; at < rows; at += most) f(at, rows - at < most ? rows - at : most);
+}
+template <typename T> T *behind(T *p, int64_t elems) { return p ? p + elems : p; }
+
 constexpr int kLongParts = 128;
 int n_parts(int64_t rows) { return (int)(rows < 1 ? 1 : rows < kBwdMostBlocks ? rows : kBwdMostBlocks); }
 
@@ -464,7 +472,7 @@ int check(const char *who, int64_t rows, int64_t d, int dtype, int param_dtype) 
                  dtype);
     FMOE_REQUIRE(param_dtype == dtype || param_dtype == FMOE_F32, "%s: parameters must be of the rows' type or float32", who);
     FMOE_REQUIRE(rows >= 0 && d >= 1, "%s: bad sizes", who);
-    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 28)) return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
+    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 26)) return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     return FMOE_OK;
 }
 
@@ -496,14 +504,19 @@ extern "C" int fmoe_layer_norm_forward(const void *x, int64_t x_stride, const vo
         const bool param_f32 = std::is_same<P, float>::value;
         const bool held = held_forward<Vec<T>::N>(row_elems, residual || rows < kFewRows, [&](auto g, auto v) {
             constexpr int kThreads = g.value > kBlock ? g.value : kBlock;
-            norm_fwd_kernel<T, g.value, v.value><<<(int)ceil_div(rows, kThreads / g.value), kThreads, 0, st>>>(
-                (const T *)x, x_stride, (const T *)residual, residual_stride, Param{weight, param_f32}, Param{bias, param_f32}, (T *)sum, (T *)y,
-                mean, rstd, rows, (int)row_elems, (float)eps);
+            in_launches(rows, g.value, [&](int64_t at, int64_t n) {
+                norm_fwd_kernel<T, g.value, v.value><<<(int)ceil_div(n, kThreads / g.value), kThreads, 0, st>>>(
+                    (const T *)x + at * x_stride, x_stride, behind((const T *)residual, at * residual_stride), residual_stride, Param{weight, param_f32},
+                    Param{bias, param_f32}, behind((T *)sum, at * row_elems), (T *)y + at * row_elems, behind(mean, at), behind(rstd, at), n, (int)row_elems,
+                    (float)eps);
+            });
         });
         if (!held)
-            long_fwd_kernel<T, P><<<(int)rows, kBlock, 0, st>>>((const T *)x, x_stride, (const T *)residual, residual_stride,
-                                                                (const P *)weight, (const P *)bias, (T *)sum, (T *)y, mean, rstd, row_elems,
-                                                                (float)eps);
+            in_launches(rows, kBlock, [&](int64_t at, int64_t n) {
+                long_fwd_kernel<T, P><<<(int)n, kBlock, 0, st>>>((const T *)x + at * x_stride, x_stride, behind((const T *)residual, at * residual_stride),
+                                                                 residual_stride, (const P *)weight, (const P *)bias, behind((T *)sum, at * row_elems),
+                                                                 (T *)y + at * row_elems, behind(mean, at), behind(rstd, at), row_elems, (float)eps);
+            });
     });
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
@@ -550,9 +563,12 @@ extern "C" int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_strid
         if (!held) {
             parts = n_parts(rows) < kLongParts ? n_parts(rows) : kLongParts;
             if (grad_x)
-                long_bwd_kernel<T, P><<<(int)rows, kBlock, 0, st>>>((const T *)grad_y, grad_y_stride, (const T *)grad_sum, grad_sum_stride,
-                                                                    (const T *)x, x_stride, mean, rstd, (const P *)weight, (T *)grad_x,
-                                                                    row_elems);
+                in_launches(rows, kBlock, [&](int64_t at, int64_t n) {
+                    long_bwd_kernel<T, P><<<(int)n, kBlock, 0, st>>>((const T *)grad_y + at * grad_y_stride, grad_y_stride,
+                                                                     behind((const T *)grad_sum, at * grad_sum_stride), grad_sum_stride,
+                                                                     (const T *)x + at * x_stride, x_stride, mean + at, rstd + at, (const P *)weight,
+                                                                     (T *)grad_x + at * row_elems, row_elems);
+                });
             if (params)
                 long_param_kernel<T><<<dim3((int)ceil_div(row_elems, kBlock), parts), kBlock, 0, st>>>(
                     (const T *)grad_y, grad_y_stride, (const T *)x, x_stride, mean, rstd, (float *)workspace, rows, row_elems);

@@ -56,6 +56,10 @@ def test_c_entries_refuse(call, arguments, code):
     assert call.__name__.split("_")[1].encode() in lib.fmoe_last_error()
 
 
+def test_rows_longer_than_a_launch_sums():
+    assert _norm_forward(d=(1 << 26) + 1) == ELIMIT and _norm_backward(d=(1 << 26) + 1) == ELIMIT
+
+
 def test_c_entries_take_nothing_to_do():
     assert _norm_forward(rows=0) == 0 and _checkpoint(rows=0) == 0 and _checkpoint(d=0) == 0 and _checkpoint_back(rows=0) == 0
     assert _norm_backward(rows=0, gw=None, gb=None, ws=None, wsb=0) == 0

@@ -347,3 +347,24 @@ def test_saved_tensors_may_come_back_otherwise(device):
         y = functions.layer_norm(x, w)
     got = torch.autograd.grad(y, [x, w], dy)
     assert all(torch.equal(a, e) for a, e in zip(want, got))
+
+
+@pytest.mark.parametrize("shape,rows", [("shorter than a vector", (1 << 23) + 1001), ("one vector", (1 << 28) + 1001)])
+def test_more_rows_than_one_launch_counts(device, shape, rows):
+    """2^31 threads and more, 256 or 8 to a row: every row is normalised, those behind the first launch's as the same few alone."""
+    d = 4 if shape == "shorter than a vector" else 8
+    few = torch.randn(64, d, device=device).bfloat16()
+    w = torch.randn(d, device=device)
+    want = functions.layer_norm(few, w)
+    if d == 4:
+        x = few.repeat(-(-rows // 64), 1)[:rows].requires_grad_(True)
+        y = functions.layer_norm(x, w)
+        assert torch.equal(y.detach(), want.repeat(-(-rows // 64), 1)[:rows])
+        g = torch.randn(64, d, device=device).bfloat16()
+        alone = few.clone().requires_grad_(True)
+        g_alone, = torch.autograd.grad(functions.layer_norm(alone, w), alone, g)
+        g_x, = torch.autograd.grad(y, x, g.repeat(-(-rows // 64), 1)[:rows])
+        assert torch.equal(g_x, g_alone.repeat(-(-rows // 64), 1)[:rows])
+    else:
+        y = functions.layer_norm(few[:1].expand(rows, d), w)     # (4.3 GB of results, every row the same)
+        assert bool((y == want[:1]).all())
