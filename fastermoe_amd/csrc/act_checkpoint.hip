@@ -168,7 +168,7 @@ int check(const char *who, int64_t rows, int64_t d, int dtype, int activation) {
     FMOE_REQUIRE(activation == FMOE_ACT_NONE || activation == FMOE_ACT_RELU || activation == FMOE_ACT_GELU, "%s: unknown activation %d",
                  who, activation);
     FMOE_REQUIRE(rows >= 0 && d >= 0, "%s: bad sizes", who);
-    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 28) || n_blocks(rows, d) > INT32_MAX)
+    if (rows > (int64_t)INT32_MAX || d > (int64_t)(1 << 28) || n_blocks(rows, d) > kMostThreads / kBlock)
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     return FMOE_OK;
 }

@@ -422,6 +422,7 @@ extern "C" int fmoe_balance_loss_backward(const void *logits, const void *token_
     if (int rc = check(who, n_tokens, n_expert, dtype)) return rc;
     if (n_tokens == 0) return FMOE_OK;
     FMOE_REQUIRE(logits && slope && grad_logits, "%s: NULL pointer", who);
+    bool fits = true;
     with_type(dtype, [&](auto type) {
         using T = decltype(type);
         held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
@@ -429,11 +430,15 @@ extern "C" int fmoe_balance_loss_backward(const void *logits, const void *token_
             // 32768 x 256 bfloat16 9.7 four ahead, one 20)
             constexpr int kTokens = kBwdBlock / l.value, kAhead = ahead_of(v.value);
             const bool ahead = n_tokens >= kBwdBlocks * kTokens * kAhead;
+            const int64_t blocks = ceil_div(n_tokens, kTokens * (ahead ? kAhead : 1));
+            fits = blocks <= kMostThreads / kBwdBlock;
+            if (!fits) return;
             (ahead ? balance_bwd_kernel<T, l.value, v.value, whole.value, kAhead> : balance_bwd_kernel<T, l.value, v.value, whole.value, 1>)<<<
-                (int)ceil_div(n_tokens, kTokens * (ahead ? kAhead : 1)), kBwdBlock, 0, (hipStream_t)stream>>>(
+                (int)blocks, kBwdBlock, 0, (hipStream_t)stream>>>(
                 (const T *)logits, (const uint8_t *)token_mask, slope, grad_loss, grad_prob, (T *)grad_logits, n_tokens, (int)n_expert);
         });
     });
+    if (!fits) return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
 }

@@ -38,6 +38,8 @@ inline int fail(int code, const char *fmt, ...) {
 // after a kernel launch
 #define FMOE_LAUNCH_CHECK() FMOE_HIP_CHECK(hipGetLastError())
 
+constexpr int64_t kMostThreads = INT64_C(0xffffffff);   // of a launch, which counts them in 32 bits
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline int dtype_bytes(int dtype) {

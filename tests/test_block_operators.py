@@ -60,6 +60,12 @@ def test_rows_longer_than_a_launch_sums():
     assert _norm_forward(d=(1 << 26) + 1) == ELIMIT and _norm_backward(d=(1 << 26) + 1) == ELIMIT
 
 
+def test_launches_of_too_many_threads():
+    """2^32 and more: 16 of them for 128 elements kept in 8 bits, 64 for a token of more than 1024 experts."""
+    assert _checkpoint(rows=1 << 28, d=128) == ELIMIT and _checkpoint_back(rows=1 << 28, d=100) == ELIMIT
+    assert lib.fmoe_balance_loss_backward(P, None, P, P, None, P, (1 << 26) + 1, 2000, _lib.F32, None) == ELIMIT
+
+
 def test_c_entries_take_nothing_to_do():
     assert _norm_forward(rows=0) == 0 and _checkpoint(rows=0) == 0 and _checkpoint(d=0) == 0 and _checkpoint_back(rows=0) == 0
     assert _norm_backward(rows=0, gw=None, gb=None, ws=None, wsb=0) == 0
