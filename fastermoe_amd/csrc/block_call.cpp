@@ -193,7 +193,11 @@ bool number(PyObject *arg, long &n) {
     n = PyLong_AsLong(arg);
     return n != -1 || !PyErr_Occurred();
 }
-bool on_gpu(const at::Tensor &t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(); }
+// (a tensor without memory of its own, as some wrappers are, has a null pointer, which a parameter that is left out has too)
+bool on_gpu(const at::Tensor &t) {
+    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg() && t.has_storage() &&
+           (t.numel() == 0 || t.storage().data() != nullptr);
+}
 
 }  // namespace
 
@@ -262,6 +266,7 @@ PyObject *fmoe_block_balance_loss(PyObject *, PyObject *const *args, Py_ssize_t 
     if (!on_gpu(logits) || !on_gpu(idx) || logits.dim() != 2 || dtype_code(logits) < 0 || idx.device() != logits.device() || idx.scalar_type() != at::kLong)
         Py_RETURN_NONE;
     const int64_t n = logits.size(0), e = logits.size(1);
+    if (idx.dim() > 1 && idx.size(0) != n) Py_RETURN_NONE;
     if (e < 1 || e > 8192 || n > INT32_MAX / 8 || idx.numel() > INT32_MAX || idx.numel() % (n ? n : 1) != 0 || (n == 0) != (idx.numel() == 0)) Py_RETURN_NONE;
     if (mask.defined() && (!on_gpu(mask) || mask.device() != logits.device() || mask.scalar_type() != at::kBool || mask.numel() != n || !mask.is_contiguous()))
         Py_RETURN_NONE;

@@ -829,6 +829,7 @@ def act_checkpoint_forward(x, activation, with_act=True, table=None):
         if kept is not None:
             return kept
     dt = _rows("x", x)
+    _near("x", x, x.device)
     if not act_checkpoint_supported(x.dtype):
         raise TypeError(f"act_checkpoint_forward does not take {x.dtype}")
     activation = _activation_of(activation)
@@ -851,6 +852,7 @@ def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=
         if made is not None:
             return made
     dt = _rows("grad", grad)
+    _near("grad", grad, grad.device)
     if not act_checkpoint_supported(grad.dtype):
         raise TypeError(f"act_checkpoint_backward does not take {grad.dtype}")
     activation = _activation_of(activation)
@@ -872,6 +874,8 @@ def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=
 def _near(name, t, device):
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.numel() and t.data_ptr() == t.storage_offset() * t.element_size():   # (a wrapper, whose null pointer would say that there is none)
+        raise ValueError(f"{name} has no memory of its own")
     return t
 
 
@@ -883,8 +887,8 @@ def _strided_rows(name, t, like=None):
         raise ValueError(f"{name} must be a CUDA (HIP) tensor, got device {t.device}")
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D [rows, features], got shape {tuple(t.shape)}")
+    _near(name, t, t.device if like is None else like.device)
     if like is not None:
-        _near(name, t, like.device)
         if t.dtype != like.dtype:
             raise TypeError(f"{name} must have dtype {like.dtype}, got {t.dtype}")
         if t.shape != like.shape:
@@ -977,6 +981,7 @@ def balance_loss_supported(n_expert, dtype):
 
 def _balance_args(logits, mask):
     dt = _rows("logits", logits)
+    _near("logits", logits, logits.device)
     n, e = logits.shape
     if not balance_loss_supported(e, logits.dtype):
         raise ValueError(f"balance_loss does not take n_expert={e}, dtype={logits.dtype}")
@@ -993,6 +998,8 @@ def balance_loss_forward(logits, topk_idx, mask, per_slot):
     :func:`balance_loss_backward`."""
     dt, n, e = _balance_args(logits, mask)
     _near("topk_idx", _dev("topk_idx", topk_idx, torch.int64), logits.device)
+    if topk_idx.dim() > 1 and topk_idx.shape[0] != n:
+        raise ValueError(f"topk_idx is {tuple(topk_idx.shape)}, expected its first dimension to be that of {n} tokens")
     if topk_idx.numel() % max(n, 1) or (n == 0) != (topk_idx.numel() == 0):
         raise ValueError(f"topk_idx has {topk_idx.numel()} entries, expected as many for each of {n} tokens")
     k = topk_idx.numel() // n if n else 1

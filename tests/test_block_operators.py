@@ -92,6 +92,46 @@ def test_functions_refuse_what_the_kernels_do_not_take():
         functions.act_checkpoint(torch.tensor(1.0), None)
 
 
+class _Wrapper(torch.Tensor):
+    """A tensor that says where it is and has no memory of its own."""
+    @staticmethod
+    def __new__(cls, *shape, dtype=torch.float32, device="cuda:0"):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError("nothing to see here")
+
+
+def test_tensors_without_memory():
+    x = _Wrapper(4, 8)
+    held, scale = _Wrapper(4, 8, dtype=torch.float8_e4m3fn), _Wrapper(4, 1, dtype=torch.float8_e8m0fnu)
+    for call in (lambda: fmoe_native.layer_norm_forward(x, None, None, None, 1e-5), lambda: fmoe_native._norm_params(x, _Wrapper(8), None),
+                 lambda: fmoe_native.balance_loss_forward(x, x, None, False), lambda: fmoe_native._balance_args(x, _Wrapper(4, dtype=torch.bool)),
+                 lambda: fmoe_native.act_checkpoint_forward(x, 0), lambda: fmoe_native.act_checkpoint_backward(x, held, scale, 0)):
+        with pytest.raises(ValueError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_parameters_without_memory(device):
+    x, idx = torch.randn(4, 8, device=device), torch.zeros(4, 1, dtype=torch.int64, device=device)
+    for call in (lambda: functions.layer_norm(x, _Wrapper(8)), lambda: functions.layer_norm(x, None, _Wrapper(8)),
+                 lambda: fmoe_native.balance_loss_forward(x, idx, _Wrapper(4, dtype=torch.bool), False),
+                 lambda: fmoe_native.act_checkpoint_forward(x, 0, table=_Wrapper(16, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_indices_of_tokens_the_other_way_round(device):
+    x, idx = torch.randn(6, 8, device=device), torch.zeros(2, 6, dtype=torch.int64, device=device)
+    for call in (lambda: functions.balance_loss(x, idx), lambda: fmoe_native.balance_loss_forward(x, idx, None, False)):
+        with pytest.raises(ValueError, match="first dimension"):
+            call()
+    assert torch.equal(functions.balance_loss(x, idx.view(-1))[1], functions.balance_loss(x, idx.view(6, 2))[1])
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu(device):
     x = torch.randn(4, 8, device=device)
