@@ -12,7 +12,7 @@
 // workgroup's range.  The logits are read once in each direction, some tokens ahead; at these sizes the chain from the first load over the sums
 // to a second launch's results bounds the forward, the memory the larger backward passes (us, forward and backward):
 //   32768 x 256 bf16, top-8    15.8   9.7        131072 x 64 f32, top-2    17.1  12.5 (5.4 TB/s)      8192 x 1024 f32, top-2   16.8  11.4
-//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      6.8   2.9
+//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      6.6   2.8
 // (A pass for every token's largest logit and sum, one for the sums over the tokens and a workgroup for the results took 158 us of the first's forward,
 // a token to a wave 25 of its backward.)
 #include "common.hpp"
@@ -402,7 +402,7 @@ extern "C" int fmoe_balance_loss_forward(const void *logits, const int64_t *topk
         using T = decltype(type);
         held_logits<Vec<T>::N>((int)n_expert, [&](auto l, auto v, auto whole) {
             constexpr int kTokens = waves_of(v.value) * (kWave / l.value);
-            // (what one workgroup goes through in kFewRounds rounds is not worth a second launch: 1000 x 16 float32, four rounds, 6.0 us, with
+            // (what one workgroup goes through in kFewRounds rounds is not worth a second launch: 1000 x 16 float32, four rounds, 6.6 us, with
             // four workgroups and the launch that joins them 8.5; 2000 x 16, eight, 8.1 and 8.5)
             const int64_t rounds = ceil_div(n_tokens, kTokens);
             const int parts = (int)(rounds <= kFewRounds ? 1 : rounds < most ? rounds : most);
