@@ -136,7 +136,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
         ok(entry.balance_forward(pointer(logits), (int64_t *)pointer(idx), pointer(mask), n, e, n ? idx.numel() / n : 1, dtype_code(logits),
                                  (int)per_slot, floats(loss), (int64_t *)pointer(count), floats(prob), floats(slope), pointer(space), bytes,
                                  stream_of(logits)));
-        ctx->save_for_backward({logits, mask, slope});
+        ctx->save_for_backward({given, mask, slope});   // (a copy made in here has no history for a second derivative)
         ctx->set_materialize_grads(false);
         ctx->mark_non_differentiable({count});
         return {loss, count, prob};

@@ -185,8 +185,8 @@ class BalanceLoss(Function):
     @staticmethod
     def forward(ctx, logits, topk_idx, mask, per_slot):
         ctx.set_materialize_grads(False)
-        logits = logits.contiguous()
-        loss, count, prob, slope = fmoe_native.balance_loss_forward(logits, topk_idx, mask, per_slot)
+        loss, count, prob, slope = fmoe_native.balance_loss_forward(logits.contiguous(), topk_idx, mask, per_slot)
+        # (the logits as given: a copy made in here has no history for a second derivative)
         ctx.save_for_backward(logits, mask, slope)
         ctx.mark_non_differentiable(count)
         return loss, count, prob

@@ -290,3 +290,27 @@ def test_saved_tensors_may_come_back_otherwise(device):
         loss = functions.balance_loss(logits, idx)[0]
     got, = torch.autograd.grad(loss, logits)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("order", ["sliced", "expanded", "transposed"])
+def test_second_derivatives_of_logits_in_any_order(order, native, device, monkeypatch):
+    """Logits that the kernels read a copy of: the gradient's gradient reaches them all the same.  (Some fifty float32 roundings on the way, 2^-24 each of
+    magnitudes that cancel at most a hundredfold: 1e-3 of the largest.)"""
+    if not native:
+        monkeypatch.setattr(_lib, "_layer_call", None)
+    shape, view = {"sliced": ((40, 9), lambda t: t[:, 2:8]), "expanded": ((1, 6), lambda t: t.expand(40, 6)), "transposed": ((6, 40), lambda t: t.t())}[order]
+    leaf = torch.randn(shape, generator=torch.Generator().manual_seed(6)).to(device).requires_grad_(True)
+    idx = torch.randint(6, (40, 2), generator=torch.Generator().manual_seed(7)).to(device)
+    idx[::2] = 1
+    gp = torch.linspace(-1, 1, 6, device=device)
+    loss, counts, prob = functions.balance_loss(view(leaf), idx)
+    first, = torch.autograd.grad([loss, prob], leaf, [torch.tensor(0.7, device=device), gp], create_graph=True)
+    assert first.requires_grad
+    second, = torch.autograd.grad(first.square().sum(), leaf)
+    l64 = leaf.detach().double().requires_grad_(True)
+    u = 0.7 * 6 / 40 ** 2 * (counts.double() - counts.sum() / 6) + gp.double() / 40
+    h, = torch.autograd.grad((torch.softmax(view(l64), 1) * u).sum(), l64, create_graph=True)
+    want, = torch.autograd.grad(h.square().sum(), l64)
+    assert torch.allclose(first.detach().double(), h.detach(), rtol=1e-3, atol=1e-3 * float(h.abs().max()))
+    assert torch.allclose(second.double(), want, rtol=1e-3, atol=1e-3 * float(want.abs().max()))
