@@ -72,7 +72,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                               pointer(total), pointer(out), floats(stats), keep ? floats(stats) + n : nullptr, n, d, eps, dtype_code(inp),
                               param.defined() ? dtype_code(param) : dtype_code(inp), stream_of(inp)));
         if (keep) {
-            ctx->save_for_backward({total.defined() ? total : inp, stats, weight, bias});
+            ctx->save_for_backward({total.defined() ? total : given, stats, weight, bias});   // (a copy has no history for a second derivative)
             ctx->saved_data["eps"] = eps;
             ctx->set_materialize_grads(false);
         }
@@ -136,7 +136,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
         ok(entry.balance_forward(pointer(logits), (int64_t *)pointer(idx), pointer(mask), n, e, n ? idx.numel() / n : 1, dtype_code(logits),
                                  (int)per_slot, floats(loss), (int64_t *)pointer(count), floats(prob), floats(slope), pointer(space), bytes,
                                  stream_of(logits)));
-        ctx->save_for_backward({given, mask, slope});   // (a copy made in here has no history for a second derivative)
+        ctx->save_for_backward({given, mask, slope});   // (as above)
         ctx->set_materialize_grads(false);
         ctx->mark_non_differentiable({count});
         return {loss, count, prob};

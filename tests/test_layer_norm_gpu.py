@@ -368,3 +368,30 @@ def test_more_rows_than_one_launch_counts(device, shape, rows):
     else:
         y = functions.layer_norm(few[:1].expand(rows, d), w)     # (4.3 GB of results, every row the same)
         assert bool((y == want[:1]).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("order", ["transposed", "sliced", "expanded"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_second_derivatives_of_rows_in_any_order(residual, order, native, device, monkeypatch):
+    """Rows that the kernels read a copy of, or where they lie: the gradient's gradient reaches them all the same."""
+    if not native:
+        monkeypatch.setattr(_lib, "_layer_call", None)
+    torch.manual_seed(8)
+    shape, view = {"transposed": ((24, 5), lambda t: t.t()), "sliced": ((5, 30), lambda t: t[:, 3:27]), "expanded": ((1, 24), lambda t: t.expand(5, 24))}[order]
+    leaves = [torch.randn(s, device=device) for s in ([shape, shape] if residual else [shape]) + [(24,), (24,)]]
+    dy, ds = torch.randn(5, 24, device=device), torch.randn(5, 24, device=device)
+
+    def own(x, *rest):
+        return functions.add_layer_norm(view(x), view(rest[0]), *rest[1:]) if residual else functions.layer_norm(view(x), *rest)
+
+    def plain(x, *rest):
+        s = view(x) + view(rest[0]) if residual else view(x)
+        w, b = rest[-2:]
+        y = (s - s.mean(1, keepdim=True)) * (s.var(1, correction=0, keepdim=True) + 1e-5).rsqrt() * w + b
+        return (y, s) if residual else y
+
+    got = _twice(own, [t.clone().requires_grad_(True) for t in leaves], [dy, ds])
+    want = _twice(plain, [t.double().requires_grad_(True) for t in leaves], [dy.double(), ds.double()])
+    for g, e in zip(got, want):
+        assert torch.allclose(g.double(), e, rtol=1e-3, atol=1e-3 * float(e.abs().max()) + 1e-12)
