@@ -395,3 +395,22 @@ def test_second_derivatives_of_rows_in_any_order(residual, order, native, device
     want = _twice(plain, [t.double().requires_grad_(True) for t in leaves], [dy.double(), ds.double()])
     for g, e in zip(got, want):
         assert torch.allclose(g.double(), e, rtol=1e-3, atol=1e-3 * float(e.abs().max()) + 1e-12)
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 260), ("f32", 300), ("f32", 512), ("f32", 777), ("f32", 1024), ("f32", 2048), ("bf16", 1024), ("f16", 4096)])
+def test_rows_do_not_depend_on_how_many_there_are(dtype, d, device):
+    """One row, a few and thousands, alone or as a sum with a residual: the same bits, in float32 too, which shows the order of the sums, and in the
+    gradients of the rows."""
+    x, dy = (torch.randn(6000, d, device=device).to(TYPES[dtype]) for _ in range(2))
+    w, b = torch.randn(d, device=device), torch.randn(d, device=device)
+
+    def run(rows):
+        leaf = x[rows].detach().requires_grad_(True)
+        y = functions.layer_norm(leaf, w, b)
+        return y.detach(), torch.autograd.grad(y, leaf, dy[rows])[0]
+
+    every = run(slice(None))
+    for rows in (slice(0, 1), slice(17, 60), slice(1, 2048), slice(4000, 6000)):
+        assert all(torch.equal(a, e[rows]) for a, e in zip(run(rows), every)), rows
+    y, s = functions.add_layer_norm(x, torch.zeros_like(x), w, b)
+    assert torch.equal(s, x) and torch.equal(y, every[0])
