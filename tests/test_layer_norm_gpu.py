@@ -414,3 +414,24 @@ def test_rows_do_not_depend_on_how_many_there_are(dtype, d, device):
         assert all(torch.equal(a, e[rows]) for a, e in zip(run(rows), every)), rows
     y, s = functions.add_layer_norm(x, torch.zeros_like(x), w, b)
     assert torch.equal(s, x) and torch.equal(y, every[0])
+
+
+def test_parameter_gradients_over_many_short_rows(device):
+    """8 million rows shorter than a vector, whose gradients have one sign: a float32 sum of 65 thousand terms one after the other would be off by
+    hundreds of steps.  A term passes through at most 8 float32 roundings (three in the normalised element, its product, a part's sum and those that join
+    the parts' 128: at most 24 more), each of 2^-24 of it."""
+    rows, d = (1 << 23) + 3, 3
+    x = torch.randn(rows, d, device=device, generator=torch.Generator(device=device).manual_seed(3))
+    w, b = torch.ones(d, device=device, requires_grad=True), torch.zeros(d, device=device, requires_grad=True)
+    dy = torch.full((rows, d), 0.1, device=device)
+    # (the sign of every normalised element, so that grad_w's terms have one sign too)
+    mean, rstd, h = _reference(x.double(), None, None, 1e-5)[:3]
+    for g, name in ((dy, "grad_b"), (torch.where(h < 0, -dy, dy), "grad_w")):
+        gw, gb = torch.autograd.grad(functions.layer_norm(x, w, b), [w, b], g)
+        if name == "grad_b":
+            want = g.double().sum(0)
+            assert bool(((gb.double() - want).abs() <= 32 * ULP32 * want).all()), ((gb.double() - want) / want).tolist()
+        else:
+            # (an element's own error: what the mean's rounding is to it, with the magnitudes that it was taken off)
+            want, reach = (g.double() * h).sum(0), (g.double().abs() * (x.double().abs() + mean.abs()) * rstd).sum(0)
+            assert bool(((gw.double() - want).abs() <= 32 * ULP32 * (want + reach)).all()), ((gw.double() - want) / want).tolist()
