@@ -437,7 +437,7 @@ class ActCheckpoint(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        held, scale = ctx.saved_tensors
+        held, scale = map(_as_chunks, ctx.saved_tensors)
         return fmoe_native.act_checkpoint_backward(grad_out.contiguous(), held, scale, ctx.activation, with_mid=False)[0], None
 
 
@@ -511,7 +511,7 @@ class MOEExpertMLPCheckpointed(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        inp, fwd_expert_count, w1, b1, w2, b2, held, scale = ctx.saved_tensors
+        inp, fwd_expert_count, w1, b1, w2, b2, held, scale = map(_as_chunks, ctx.saved_tensors)
         n = held.shape[0]
         grad_out = grad_out.contiguous()
         g_mid = fmoe_native.linear_dact_backward(grad_out, fwd_expert_count, w2, None, _lib.ACT_NONE)

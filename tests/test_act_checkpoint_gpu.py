@@ -246,3 +246,39 @@ def test_called_from_python_the_same(device, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(native, run()))
     for act in CODES:
         check(x, act)
+
+
+def _otherwise(t):
+    """An equal tensor whose elements lie in another order."""
+    if t.dim() < 2 or t.shape[0] < 2:
+        return t
+    return t.view(torch.uint8).t().contiguous().t().view(t.dtype) if t.element_size() == 1 else t.transpose(0, 1).contiguous().transpose(0, 1)
+
+
+def test_saved_tensors_may_come_back_otherwise(device):
+    """Saved-tensor hooks hand back what is held in another order."""
+    x = torch.randn(33, 96, device=device, requires_grad=True)
+    dy = torch.randn(33, 96, device=device)
+    want, = torch.autograd.grad(functions.act_checkpoint(x, torch.nn.GELU()), x, dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _otherwise):
+        y = functions.act_checkpoint(x, torch.nn.GELU())
+    got, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(got, want)
+
+
+def test_experts_saved_tensors_may_come_back_otherwise(device):
+    """The same of the experts' node over rows that are counted on the host."""
+    from fastermoe_amd.functions import MOEExpertMLPCheckpointed
+    torch.manual_seed(2)
+    x = torch.randn(40, 64, device=device)
+    counts = torch.tensor([13, 0, 27])
+    params = [torch.randn(s, device=device) * 0.1 for s in ((3, 96, 64), (3, 96), (3, 64, 96), (3, 64))]
+    dy = torch.randn(40, 64, device=device)
+
+    def run(hook):
+        leaves = [t.detach().requires_grad_(True) for t in (x, *params)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, hook):
+            out = MOEExpertMLPCheckpointed.apply(leaves[0], counts, *leaves[1:], _lib.ACT_GELU)
+        return torch.autograd.grad(out, leaves, dy)
+
+    assert all(torch.equal(a, b) for a, b in zip(run(lambda t: t), run(lambda t: _otherwise(t) if t.is_cuda else t)))
