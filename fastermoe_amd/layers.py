@@ -69,6 +69,7 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     gather and the score-weighted sum over each token's ``top_k`` rows run as one pass
     over the experts' output where it lies, and the first result is ``[N, d]``."""
     from .fused_functions import MOEForward
+    from .transformer import _Expert
 
     topk = gate.shape[1] if gate.dim() == 2 else 1
     # On the GPU, with one gate index per (token, k) pair and this package's own expert module
@@ -83,7 +84,7 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     own = (inp.is_cuda and gate.is_cuda and inp.dim() == 2 and inp.shape[0] > 0
            and gate.numel() == inp.shape[0] * topk and fused and _own_expert_path(expert_fn, experts))
     # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way)
-    enable_fuse = enable_fuse and not (getattr(experts, "act_checkpoint", False) and experts._checkpoints(inp))
+    enable_fuse = enable_fuse and not (isinstance(experts, _Expert) and experts._checkpoints(inp))
     if own:
         _single_worker(world_size, "count_by_gate")
         enable_fuse = enable_fuse and not experts.unchunked_is_faster(inp, gate.numel())

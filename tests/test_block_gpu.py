@@ -355,3 +355,28 @@ def test_block_in_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step())), k
+
+
+class _UsersExperts(torch.nn.Module):
+    """Experts of a user's own that the fused pipeline takes, with a switch that happens to have the name of this package's."""
+    act_checkpoint = True
+
+    def __init__(self):
+        super().__init__()
+        self.htoh4, self.h4toh = fmoe.FMoELinear(4, 32, 64), fmoe.FMoELinear(4, 64, 32)
+        self.activation = torch.nn.GELU()
+
+    def forward(self, inp, fwd_expert_count):
+        return self.h4toh(self.activation(self.htoh4(inp, fwd_expert_count)), fwd_expert_count)
+
+
+def test_users_experts_with_a_switch_of_that_name(device):
+    layer = fmoe.FMoE(num_expert=4, d_model=32, top_k=2)
+    layer.experts, layer.experts_fused = _UsersExperts(), True
+    layer = layer.to(device)
+    x = torch.randn(50, 32, device=device, requires_grad=True)
+    want = layer(x)
+    layer.enable_fuse = True
+    got = layer(x)
+    assert_close(got.detach(), want.detach(), TOL[torch.float32])
+    got.sum().backward()
