@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint
     const int b = scale_byte(lanes_max(most));
     if (at.n <= 0) return;
     const float inv = __uint_as_float((uint32_t)(254 - b) << 23), limit = b == top_byte<T>() ? 240.f : 448.f;
-    if (threadIdx.x % kLanes == 0) scale[at.block] = (uint8_t)b;
+    if (held && threadIdx.x % kLanes == 0) scale[at.block] = (uint8_t)b;
     float v[kLaneElems];
 #pragma unroll
     for (int j = 0; j < kLaneElems; ++j) v[j] = fmaf(f[j], 0.f, __builtin_amdgcn_fmed3f(f[j] * inv, -limit, limit));
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kBlock) void ckpt_fwd_kernel(const T *x, T *y, uint
         q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
         q[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], q[h], true);
     }
-    store_elems<FLAT>(held + at.at, at.n, __builtin_bit_cast(Bytes8, q).byte);
+    if (held) store_elems<FLAT>(held + at.at, at.n, __builtin_bit_cast(Bytes8, q).byte);
     if (y) {
 #pragma unroll
         for (int j = 0; j < kLaneElems; ++j) e[j] = (T)act_value<ACT>(f[j]);
@@ -200,7 +200,7 @@ extern "C" int fmoe_act_checkpoint_forward(const void *x, void *y, void *held, v
     const char *who = "fmoe_act_checkpoint_forward";
     if (int rc = check(who, rows, row_elems, dtype, activation)) return rc;
     if (rows == 0 || row_elems == 0) return FMOE_OK;
-    FMOE_REQUIRE(x && held && scale, "%s: NULL pointer", who);
+    FMOE_REQUIRE(x && !held == !scale && (held || y), "%s: NULL pointer", who);
     with_kernel(dtype, activation, row_elems, [&](auto t, auto act, auto flat) {
         using T = decltype(t);
         ckpt_fwd_kernel<T, act.value, flat.value><<<(int)n_blocks(rows, row_elems), kBlock, 0, (hipStream_t)stream>>>(

@@ -296,16 +296,16 @@ PyObject *wrap_or_none(at::Tensor t) {
 
 }  // namespace
 
-// act_checkpoint_forward(x, table, activation, with_act): (y or None, held, scale); None where the call does not take these tensors
+// act_checkpoint_forward(x, table, activation, with_act, with_held): (y or None, held, scale or None, None); None where the call does not take these tensors
 PyObject *fmoe_block_checkpoint_forward(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
-    if (n_args != 4 || entry.checkpoint_forward == nullptr) {
-        PyErr_SetString(PyExc_TypeError, "act_checkpoint_forward: 4 arguments, after bind_block");
+    if (n_args != 5 || entry.checkpoint_forward == nullptr) {
+        PyErr_SetString(PyExc_TypeError, "act_checkpoint_forward: 5 arguments, after bind_block");
         return nullptr;
     }
     std::array<at::Tensor, 2> t;
-    long activation, with_act;
-    if (!tensors(args, t) || !number(args[2], activation) || !number(args[3], with_act)) return nullptr;
+    long activation, with_act, with_held;
+    if (!tensors(args, t) || !number(args[2], activation) || !number(args[3], with_act) || !number(args[4], with_held)) return nullptr;
     const auto &[x, table] = t;
     if (!keeps(x, activation) || !no_or_table(table, x)) Py_RETURN_NONE;
     at::Tensor y, held, scale;
@@ -314,13 +314,15 @@ PyObject *fmoe_block_checkpoint_forward(PyObject *, PyObject *const *args, Py_ss
         const at::NoGradGuard no_grad;
         const c10::OptionalDeviceGuard guard(x.device());
         const int64_t n = x.size(0), d = x.size(1);
-        held = at::empty({n, d}, x.options().dtype(at::kFloat8_e4m3fn));
-        scale = at::empty({n, (d + kScaleElems - 1) / kScaleElems}, x.options().dtype(at::kFloat8_e8m0fnu));
+        if (with_held) {
+            held = at::empty({n, d}, x.options().dtype(at::kFloat8_e4m3fn));
+            scale = at::empty({n, (d + kScaleElems - 1) / kScaleElems}, x.options().dtype(at::kFloat8_e8m0fnu));
+        }
         if (with_act) y = at::empty({n, d}, x.options());
         ok(entry.checkpoint_forward(pointer(x), pointer(y), pointer(held), pointer(scale), pointer(table), n, d, dtype_code(x), (int)activation,
                                     stream_of(x)));
     }
-    return Py_BuildValue("NNN", wrap_or_none(std::move(y)), THPVariable_Wrap(std::move(held)), THPVariable_Wrap(std::move(scale)));
+    return Py_BuildValue("NNN", wrap_or_none(std::move(y)), wrap_or_none(std::move(held)), wrap_or_none(std::move(scale)));
     END_HANDLE_TH_ERRORS
 }
 

@@ -819,13 +819,15 @@ def act_checkpoint_supported(dtype):
     return dtype in (torch.float32, torch.bfloat16, torch.float16)
 
 
-def act_checkpoint_forward(x, activation, with_act=True, table=None):
+def act_checkpoint_forward(x, activation, with_act=True, table=None, with_held=True):
     """``(act(x) or None, held, scale)``: ``x [rows, features]`` in 8 bits (``held``, ``float8_e4m3fn``), 32 elements along a row under
     one power of two (``scale [rows, ceil(features / 32)]``, ``float8_e8m0fnu``), for :func:`act_checkpoint_backward`.  ``table``: a
-    segment table; only the rows that its counts add up to are read and written."""
+    segment table; only the rows that its counts add up to are read and written.  ``with_held=False``: nothing is kept (``None``, ``None``)."""
+    if not with_act and not with_held:
+        raise ValueError("neither the activation nor the rows in 8 bits are wanted")
     module = _lib.load_layer_call()
     if module is not None:
-        kept = module.act_checkpoint_forward(x, table, activation, with_act)
+        kept = module.act_checkpoint_forward(x, table, activation, with_act, with_held)
         if kept is not None:
             return kept
     dt = _rows("x", x)
@@ -834,8 +836,8 @@ def act_checkpoint_forward(x, activation, with_act=True, table=None):
         raise TypeError(f"act_checkpoint_forward does not take {x.dtype}")
     activation = _activation_of(activation)
     n, d = x.shape
-    held = torch.empty(n, d, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(n, -(-d // SCALE_ELEMS), dtype=torch.float8_e8m0fnu, device=x.device)
+    held = torch.empty(n, d, dtype=torch.float8_e4m3fn, device=x.device) if with_held else None
+    scale = torch.empty(n, -(-d // SCALE_ELEMS), dtype=torch.float8_e8m0fnu, device=x.device) if with_held else None
     y = torch.empty_like(x) if with_act else None
     with _on(x.device):
         check(_lib.load().fmoe_act_checkpoint_forward(_ptr(x), _ptr(y), _ptr(held), _ptr(scale), _live_rows(table, n, x.device), n, d, dt,

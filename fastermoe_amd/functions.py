@@ -428,8 +428,8 @@ class ActCheckpoint(Function):
     r"""An activation whose argument is kept in 8 bits for the backward (see :func:`act_checkpoint`)."""
 
     @staticmethod
-    def forward(ctx, inp, activation):
-        out, held, scale = fmoe_native.act_checkpoint_forward(inp.contiguous(), activation)
+    def forward(ctx, inp, activation, keep):
+        out, held, scale = fmoe_native.act_checkpoint_forward(inp.contiguous(), activation, with_held=keep)
         ctx.save_for_backward(held, scale)
         ctx.activation = activation
         return out
@@ -438,7 +438,7 @@ class ActCheckpoint(Function):
     @once_differentiable
     def backward(ctx, grad_out):
         held, scale = map(_as_chunks, ctx.saved_tensors)
-        return fmoe_native.act_checkpoint_backward(grad_out.contiguous(), held, scale, ctx.activation, with_mid=False)[0], None
+        return fmoe_native.act_checkpoint_backward(grad_out.contiguous(), held, scale, ctx.activation, with_mid=False)[0], None, None
 
 
 def _as_rows(inp):
@@ -452,9 +452,10 @@ def act_checkpoint(inp, activation):
     r"""``activation(inp)`` (an ``ACT_*`` code, ``torch.nn.GELU()`` or ``torch.nn.ReLU()``; exact GELU, ReLU or none) over rows ``[rows, features]`` or of any
     leading shape, from ``inp`` as it is; for the backward ``inp`` is kept as e4m3 numbers with a power of two for every 32
     elements along a row, 1.03 bytes an element, and the derivative is taken where those are (off by at most 2^-4 of an element,
-    or 2^-10 of the block's scale where it is small against the block).  Float32, bfloat16 and float16."""
+    or 2^-10 of the block's scale where it is small against the block).  Nothing is kept where nothing is differentiated.  Float32,
+    bfloat16 and float16."""
     code = activation if type(activation) is int else _activation_code(activation)
-    out = ActCheckpoint.apply(_as_rows(inp), code)
+    out = ActCheckpoint.apply(_as_rows(inp), code, torch.is_grad_enabled() and inp.requires_grad)
     return out if inp.dim() == 2 else out.view(inp.shape)
 
 

@@ -712,7 +712,8 @@ int fmoe_balance_loss_backward(const void *logits, const void *token_mask,
  * max|x| <= 448 * scale over the finite ones (byte >= 1); held is x / scale
  * rounded to nearest, infinities and NaN as NaN; what would round past the
  * largest number of the type is held as the largest that it does.
- * y [rows, row_elems]: act(x) from x itself; NULL: not wanted; may be x.
+ * y [rows, row_elems]: act(x) from x itself; NULL: not wanted; may be x.  held
+ * and scale both NULL: nothing is kept.
  * segment_table (optional, of fmoe_segment_table_build): only the rows that its
  * counts add up to are read and written.  FMOE_F32 / FMOE_BF16 / FMOE_F16. */
 int fmoe_act_checkpoint_forward(const void *x, void *y, void *held, void *scale,

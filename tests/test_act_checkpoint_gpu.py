@@ -282,3 +282,28 @@ def test_experts_saved_tensors_may_come_back_otherwise(device):
         return torch.autograd.grad(out, leaves, dy)
 
     assert all(torch.equal(a, b) for a, b in zip(run(lambda t: t), run(lambda t: _otherwise(t) if t.is_cuda else t)))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("act", ["gelu", "relu", "none"])
+@pytest.mark.parametrize("d", [96, 50])
+def test_nothing_is_held_where_nothing_is_differentiated(d, act, native, device, monkeypatch):
+    """One allocation, the result's, whose bits are those of a call that is differentiated."""
+    if not native:
+        monkeypatch.setattr(_lib, "_layer_call", None)
+    x = torch.randn(70, d, device=device)
+    want = functions.act_checkpoint(x.clone().requires_grad_(True), CODES[act]).detach()
+
+    def count(call):
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        out = call()
+        return out, torch.cuda.memory_stats()["allocation.all.allocated"] - before
+
+    with torch.no_grad():
+        out, n = count(lambda: functions.act_checkpoint(x.requires_grad_(True), CODES[act]))
+    assert n == 1 and torch.equal(out, want)
+    out, n = count(lambda: functions.act_checkpoint(x.detach(), CODES[act]))
+    assert n == 1 and torch.equal(out, want) and not out.requires_grad
+    with torch.inference_mode():
+        out, n = count(lambda: functions.act_checkpoint(x, CODES[act]))
+    assert n == 1 and torch.equal(out, want)

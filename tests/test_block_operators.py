@@ -204,3 +204,10 @@ def test_calls_on_two_streams_at_once(device):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_rows_in_8_bits_or_their_activation():
+    """Held numbers and scales come together, and something has to be wanted."""
+    assert _checkpoint(y=None, held=None, scale=None) == EINVAL and _checkpoint(held=None, scale=None, rows=0) == 0
+    with pytest.raises(ValueError, match="wanted"):
+        fmoe_native.act_checkpoint_forward(torch.randn(4, 8), _lib.ACT_GELU, with_act=False, with_held=False)
