@@ -11,8 +11,8 @@
 // probabilities stay in registers between the one load and the sums over the tokens, which each lane keeps for its experts over all the tokens of its
 // workgroup's range.  The logits are read once in each direction, some tokens ahead; at these sizes the chain from the first load over the sums
 // to a second launch's results bounds the forward, the memory the larger backward passes (us, forward and backward):
-//   32768 x 256 bf16, top-8    15.8   9.7        131072 x 64 f32, top-2    17.1  12.5 (5.4 TB/s)      8192 x 1024 f32, top-2   16.8  11.4
-//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      6.6   2.8
+//   32768 x 256 bf16, top-8    16.5  10.4        131072 x 64 f32, top-2    18.0  13.1 (5.1 TB/s)      8192 x 1024 f32, top-2   17.4  11.5
+//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      7.1   2.8
 // (A pass for every token's largest logit and sum, one for the sums over the tokens and a workgroup for the results took 158 us of the first's forward,
 // a token to a wave 25 of its backward.)
 #include "common.hpp"
@@ -46,6 +46,16 @@ template <int L, typename F> __device__ __forceinline__ float over_lanes(float v
         v = op(op(lane(0), lane(16)), op(lane(32), lane(48)));
     }
     return v;
+}
+
+// exp(x) for x <= 0 (or NaN): 2^h of the rounded h = x log2(e), and e^r = 1 + r of what that rounding took away, r = x - h ln(2) <= 1e-5 (ln(2) in two parts).
+// Minus infinity leaves no difference, and r has to be a number then.  Off by two units in the last place.  (The exponential instruction of a rounded product alone is off
+// by |x| / 2 such units besides; that one takes 9.7 us of the backward of 32768 x 256 bfloat16, this 10.4, the library's function 11.5.)
+__device__ __forceinline__ float exp_down(float x) {
+    const float h = x * 1.44269504088896341f;
+    const float r = fmaf(-h, -1.90465429995776e-9f, fmaf(-h, 0.693147182464599609f, x));
+    const float e = __builtin_amdgcn_exp2f(h);
+    return fmaf(e, __builtin_amdgcn_fmed3f(r, -1.f, 1.f), e);
 }
 
 // A token's logits as its lanes hold them.
@@ -83,7 +93,7 @@ template <typename T, int L, int V, bool WHOLE> struct Logits {
         for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                p[v][i] = __expf(p[v][i] - most);
+                p[v][i] = exp_down(p[v][i] - most);
                 sum += p[v][i];
             }
         sum = over_lanes<L>(sum, [](float a, float b) { return a + b; });

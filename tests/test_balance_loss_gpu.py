@@ -314,3 +314,22 @@ def test_second_derivatives_of_logits_in_any_order(order, native, device, monkey
     want, = torch.autograd.grad(h.square().sum(), l64)
     assert torch.allclose(first.detach().double(), h.detach(), rtol=1e-3, atol=1e-3 * float(h.abs().max()))
     assert torch.allclose(second.double(), want, rtol=1e-3, atol=1e-3 * float(want.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_small_probabilities(dtype, device):
+    """Logits that lie whole numbers apart, so that no difference is rounded: an exponential is off by at most 4 steps of 2^-24, the sum of them by 12
+    (additions of a lane and over the lanes), then a reciprocal, a product and a mean, by one each.  Twenty steps of every probability and gradient."""
+    e = 81
+    logits = -torch.arange(e, device=device, dtype=torch.float32).expand(7, e).to(TYPES[dtype]).contiguous().requires_grad_(True)
+    idx = torch.zeros(7, 1, dtype=torch.int64, device=device)
+    loss, counts, prob = functions.balance_loss(logits, idx)
+    p = torch.softmax(logits.detach()[0].double(), 0)
+    assert float(((prob.detach().double() - p).abs() / p).max()) <= 20 * ULP32
+    if dtype == "f32":
+        grad, = torch.autograd.grad(loss, logits, torch.tensor(1.0, device=device))
+        u = e / 49 * (counts.double() - 7 / e)
+        want = p * (u - (p * u).sum())
+        # (u's own roundings, and those of a difference of two of its size)
+        slack = 20 * ULP32 * p * (u.abs() + (p * u.abs()).sum())
+        assert bool(((grad.double() - want).abs() <= slack + 20 * ULP32 * want.abs()).all())
