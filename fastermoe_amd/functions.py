@@ -5,6 +5,8 @@ the reference's ``fmoe.functions`` (fmoe/functions.py), on top of
 Single worker only: ``world_size > 1`` (token all-to-all, dynamic shadowing) is
 outside this package and raises ``NotImplementedError``.
 """
+import math
+
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -445,7 +447,7 @@ def _as_rows(inp):
     """``inp`` as rows of its last dimension."""
     if inp.dim() == 0:
         raise ValueError("a tensor without dimensions has no rows")
-    return inp.reshape(-1, inp.shape[-1]) if inp.dim() != 2 else inp
+    return inp if inp.dim() == 2 else inp.reshape(math.prod(inp.shape[:-1]), inp.shape[-1])   # (-1 is ambiguous where there are no features)
 
 
 def act_checkpoint(inp, activation):

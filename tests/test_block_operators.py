@@ -211,3 +211,18 @@ def test_rows_in_8_bits_or_their_activation():
     assert _checkpoint(y=None, held=None, scale=None) == EINVAL and _checkpoint(held=None, scale=None, rows=0) == 0
     with pytest.raises(ValueError, match="wanted"):
         fmoe_native.act_checkpoint_forward(torch.randn(4, 8), _lib.ACT_GELU, with_act=False, with_held=False)
+
+
+def test_rows_without_features_of_any_leading_shape():
+    """As rows of two dimensions are: the layer norm refuses them, the rows kept in 8 bits have nothing to keep."""
+    assert functions._as_rows(torch.zeros(2, 3, 0)).shape == (6, 0) and functions._as_rows(torch.zeros(0, 3, 4)).shape == (0, 4)
+    assert functions._as_rows(torch.zeros(5)).shape == (1, 5) and functions._as_rows(torch.zeros(0)).shape == (1, 0)
+
+
+@pytest.mark.gpu
+def test_rows_without_features_on_the_gpu(device):
+    x = torch.zeros(2, 3, 0, device=device, requires_grad=True)
+    y = functions.act_checkpoint(x, torch.nn.GELU())
+    assert y.shape == x.shape and torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+    with pytest.raises(ValueError, match="features"):
+        functions.layer_norm(x)
