@@ -192,9 +192,10 @@ class FMoEPositionwiseFF(FMoETransformerMLP):
         """Whether calling ``layer_norm`` is the kernel on its parameters and nothing else."""
         norm, first = self.layer_norm, tensors[0]
         return (type(norm) is nn.LayerNorm and _no_hooks(norm) and norm.normalized_shape == (self.d_model,) and first.is_cuda
-                and fmoe_native.layer_norm_supported(first.dtype) and not torch.is_autocast_enabled()
+                and first.shape[-1:] == norm.normalized_shape and fmoe_native.layer_norm_supported(first.dtype) and not torch.is_autocast_enabled()
                 and all(t.dtype == first.dtype and t.device == first.device and t.shape == first.shape for t in tensors)
-                and all(p is None or (p.device == first.device and p.dtype in (first.dtype, torch.float32)) for p in (norm.weight, norm.bias))
+                and all(p is None or (p.device == first.device and p.dtype in (first.dtype, torch.float32) and p.is_contiguous())
+                        for p in (norm.weight, norm.bias))
                 and (norm.weight is None or norm.bias is None or norm.weight.dtype == norm.bias.dtype))
 
     def forward(self, inp):

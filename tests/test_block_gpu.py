@@ -380,3 +380,22 @@ def test_users_experts_with_a_switch_of_that_name(device):
     got = layer(x)
     assert_close(got.detach(), want.detach(), TOL[torch.float32])
     got.sum().backward()
+
+
+def test_block_with_parameters_and_tokens_that_the_kernel_does_not_take(device):
+    """Parameters that lie apart go to the module, as any module's would; tokens of another length are the module's error."""
+    block = fmoe.FMoEPositionwiseFF(num_expert=4, d_model=32, d_hidden=64, pre_lnorm=True).to(device)
+    x = torch.randn(9, 32, device=device)
+    with torch.no_grad():
+        block.layer_norm.weight.normal_()
+        want = block(x)
+        wide = torch.empty(32, 2, device=device)
+        wide[:, 0] = block.layer_norm.weight
+        block.layer_norm.weight = torch.nn.Parameter(wide[:, 0])
+        assert not block.layer_norm.weight.is_contiguous()
+        assert torch.allclose(block(x), want, rtol=1e-5, atol=1e-5)
+        block.layer_norm = torch.nn.LayerNorm(32, elementwise_affine=False).to(device)
+        for pre in (True, False):
+            block.pre_lnorm = pre
+            with pytest.raises(RuntimeError, match="normalized_shape"):
+                block(torch.randn(4, 64, device=device))
