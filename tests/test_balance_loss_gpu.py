@@ -333,3 +333,14 @@ def test_small_probabilities(dtype, device):
         # (u's own roundings, and those of a difference of two of its size)
         slack = 20 * ULP32 * p * (u.abs() + (p * u.abs()).sum())
         assert bool(((grad.double() - want).abs() <= slack + 20 * ULP32 * want.abs()).all())
+
+
+@pytest.mark.parametrize("per", ["token", "slot"])
+@pytest.mark.parametrize("n,e,dtype", [(65701, 60, "bf16"), (65701, 64, "f16"), (32901, 61, "f32"), (32901, 64, "f32"), (4201, 601, "bf16"), (4201, 600, "bf16"),
+                                       (4201, 301, "f32"), (4201, 300, "f32"), (9000, 1100, "bf16"), (270001, 5, "f32")])
+def test_several_tokens_ahead_in_the_backward(n, e, per, dtype, device):
+    """Enough tokens for the backward to load several ahead, with experts in whole vectors and not, in one vector to a lane and two, one token behind a whole
+    workgroup's."""
+    logits, idx = _inputs(n, e, 2, dtype, drop=0.2 if per == "slot" else 0.0)
+    mask = (torch.arange(n, device=device) % 11 == 0) if per == "slot" else None
+    _check(logits, idx, per, mask, g_loss=300.0 if dtype == "f16" else 0.7)

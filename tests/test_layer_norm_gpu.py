@@ -435,3 +435,26 @@ def test_parameter_gradients_over_many_short_rows(device):
             # (an element's own error: what the mean's rounding is to it, with the magnitudes that it was taken off)
             want, reach = (g.double() * h).sum(0), (g.double().abs() * (x.double().abs() + mean.abs()) * rstd).sum(0)
             assert bool(((gw.double() - want).abs() <= 32 * ULP32 * (want + reach)).all()), ((gw.double() - want) / want).tolist()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n,d,dtype", [(9001, 768, "bf16"), (9001, 768, "f32"), (1001, 4096, "f16"), (1001, 4096, "f32"), (70001, 40, "bf16"), (4099, 2052, "f32")])
+def test_several_sets_of_rows_to_a_workgroup(n, d, dtype, residual, device):
+    """Backward passes whose workgroups walk over several sets of rows, the last one not full."""
+    _run(n, d, dtype, residual, "same")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n,d", [(5, 8200), (300, 8200), (7, 12000), (515, 12000), (3, 16384), (300, 16384), (3, 16381), (9, 20000), (2, 32768)])
+def test_long_rows(n, d, residual, dtype, device):
+    """Rows that take the most registers, alone and several to a workgroup."""
+    _run(n, d, dtype, residual, "same")
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("n,d,dtype", [(11003, 4096, "bf16"), (6001, 4096, "f32"), (3001, 8192, "f32"), (1501, 16384, "f32"), (4001, 12000, "bf16"), (60001, 768, "f16"),
+                                       (30001, 1500, "bf16")])
+def test_rows_past_the_caches(n, d, dtype, residual, device):
+    """More than 256 MiB to read and write in the backward, which goes past the caches then."""
+    _run(n, d, dtype, residual, "f32" if dtype == "f16" else "same")
