@@ -430,7 +430,7 @@ class ActCheckpoint(Function):
     r"""An activation whose argument is kept in 8 bits for the backward (see :func:`act_checkpoint`)."""
 
     @staticmethod
-    def forward(ctx, inp, activation, keep):
+    def forward(ctx, inp, activation, keep=True):
         out, held, scale = fmoe_native.act_checkpoint_forward(inp.contiguous(), activation, with_held=keep)
         ctx.save_for_backward(held, scale)
         ctx.activation = activation

@@ -69,7 +69,6 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     gather and the score-weighted sum over each token's ``top_k`` rows run as one pass
     over the experts' output where it lies, and the first result is ``[N, d]``."""
     from .fused_functions import MOEForward
-    from .transformer import _Expert
 
     topk = gate.shape[1] if gate.dim() == 2 else 1
     # On the GPU, with one gate index per (token, k) pair and this package's own expert module
@@ -83,8 +82,9 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     # rows and CPU counts it can read (fmoe/layers.py:117-140).
     own = (inp.is_cuda and gate.is_cuda and inp.dim() == 2 and inp.shape[0] > 0
            and gate.numel() == inp.shape[0] * topk and fused and _own_expert_path(expert_fn, experts))
-    # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way)
-    enable_fuse = enable_fuse and not (isinstance(experts, _Expert) and experts._checkpoints(inp))
+    if enable_fuse:   # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way)
+        from .transformer import _Expert
+        enable_fuse = not (isinstance(experts, _Expert) and experts._checkpoints(inp))
     if own:
         _single_worker(world_size, "count_by_gate")
         enable_fuse = enable_fuse and not experts.unchunked_is_faster(inp, gate.numel())

@@ -307,3 +307,12 @@ def test_nothing_is_held_where_nothing_is_differentiated(d, act, native, device,
     with torch.inference_mode():
         out, n = count(lambda: functions.act_checkpoint(x, CODES[act]))
     assert n == 1 and torch.equal(out, want)
+
+
+def test_the_node_by_itself(device):
+    """``ActCheckpoint.apply`` with and without the last argument."""
+    x = torch.randn(20, 64, device=device, requires_grad=True)
+    want, = torch.autograd.grad(functions.act_checkpoint(x, CODES["gelu"]).sum(), x)
+    for more in ((), (True,)):
+        got, = torch.autograd.grad(functions.ActCheckpoint.apply(x, CODES["gelu"], *more).sum(), x)
+        assert torch.equal(got, want)
