@@ -4,7 +4,8 @@
 // (b >= -126) with max|x| <= 448 2^b over the block's finite elements:  q = e4m3(x 2^-b), to nearest, ties to even; the scale is the
 // byte b + 127.  Dividing by a power of two is exact, so the numbers are off by their own rounding alone: 2^-4 of themselves, or, small
 // against the block, 2^-10 2^b.  What rounds to more than the rows' type holds is held as the largest that it does (240 2^b in the one
-// block that can); infinities and NaN are held as NaN, so that a forward that overflowed still shows in the gradients.
+// block that can); infinities and NaN are held as NaN, so that a forward that overflowed still shows in the gradients.  A ReLU's argument of at most 2^-10 2^b is
+// held as 0, where its slope is 0: positive elements that are 2 to 5 10^5 times smaller than their block's largest get no gradient.
 //
 //   forward   y = act(x), q, b          backward  x~ = q 2^b   mid = act(x~)   grad_x = grad act'(x~)
 //
@@ -28,6 +29,8 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kScaleElems = 32, kLaneElems = 8, kLanes = kScaleElems / kLaneElems;   // lanes that share a scale
 
+// (GELU by gelu_terms in float32 too: off by up to 5.3 2^-24 |x|, where the library's error function is by 1.8.  That one takes 14.4 us instead of 13.3 of the forward of
+// 8192 x 1024, 6.6 instead of 5.9 of 2048 x 1024 and nothing of 32768 x 4096, and in the backward, whose argument is off by 2^-4, 21.0 instead of 20.3 and 309 instead of 298.)
 template <int ACT> __device__ __forceinline__ float act_value(float x) {
     if (ACT == FMOE_ACT_RELU) return x < 0.f ? 0.f : x;   // (NaN stays)
     if (ACT == FMOE_ACT_GELU) return x * gemm::gelu_terms(x).cdf;

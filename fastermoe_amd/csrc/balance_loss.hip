@@ -14,7 +14,8 @@
 //   32768 x 256 bf16, top-8    16.5  10.4        131072 x 64 f32, top-2    18.0  13.1 (5.1 TB/s)      8192 x 1024 f32, top-2   17.4  11.5
 //   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      7.1   2.8
 // (A pass for every token's largest logit and sum, one for the sums over the tokens and a workgroup for the results took 158 us of the first's forward,
-// a token to a wave 25 of its backward.)
+// a token to a wave 25 of its backward.)  More than 2048 experts in float32, 32 vectors to a lane, do not fit: 528 bytes of scratch memory to a lane (1024 tokens of 8192
+// experts: 55 us and 34).
 #include "common.hpp"
 #include "lane_elems.hpp"
 

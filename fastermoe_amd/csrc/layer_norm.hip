@@ -8,20 +8,22 @@
 //
 // A row lies in the registers of G lanes, V vectors of 16 bytes to each, between its one load and its one store: G x V is the smallest that
 // holds it (held_forward, held_backward), wherever it begins and whatever its length.  Rows longer than any holds, or shorter than a vector, are read again for
-// every sum (long_* kernels: 1000 bfloat16 rows of 40000 take 208 us and 317).  Bound by memory (TB/s of what has to move; a large copy on the same
-// card 5.0):
+// every sum (long_* kernels: 1000 bfloat16 rows of 40000 take 208 us and 317).  Bound by memory (us by events, small launches eight to a graph; TB/s of what has
+// to move; a large copy on the same card 5.0):
 //   rows x features             forward          backward            of it without the parameters' gradients
 //   16384 x 4096 bf16, residual   92 us  5.8        91 us  5.9         84 us  6.4
 //   32768 x 4096 bf16             98     5.5       144     5.6        137     5.9
 //   16384 x 2048 f32, residual    92     5.8        88     6.1         83     6.4
-//   32768 x 1024 bf16             27     5.0        41     4.9         36     5.6
+//   32768 x 1024 bf16             26     5.1        41     4.9         36     5.6
 //   65536 x 900 bf16, residual    85     5.5        86     5.5
 //   32768 x 500 bf16              15     4.4        22     4.4         17     5.8
 //   5000 x 12000 bf16, residual   92     5.2       125     3.8
 //   509 x 4096 f16, residual      6.0               13                5.1
 //   64 x 4096 bf16, residual      3.8               8.9               4.1
 // (The first with a row read again for every sum and the parameters' gradients in a pass of their own: 358 and 431 us.  Rows of 900 and 500 whose last
-// elements were loaded and stored apart: 102 and 129, 18 and 27.)
+// elements were loaded and stored apart: 102 and 129, 18 and 27.)  The backward over the longest held rows does not fit its registers: 16-bit rows of 8193 to 16384
+// elements spill 10 to 19 of a lane's 128 to scratch memory (44 to 80 bytes), float32 rows of 4097 to 8192 with a residual 11 of 256 (48), and those of 8193 to 16384 keep
+// 160 bytes there, which goes with their 3.7 to 4.5 TB/s.
 #include "common.hpp"
 #include "lane_elems.hpp"
 
@@ -565,8 +567,9 @@ extern "C" int fmoe_layer_norm_backward(const void *grad_y, int64_t grad_y_strid
         // smaller launches lose by it: 4096 x 8192 53 and 55; 65536 x 512 50 and 54.  Without rows there is nothing to load from, and the parameters' gradients are sums of no parts)
         int parts = 0;
         const bool held = rows == 0 || held_backward<Vec<T>::N>(row_elems, [&](auto g, auto v) {
-            // (one set to a workgroup, unless the workgroups' sums would be more than kPartBytes, then two: 509 x 4096 float16 16.4 us with
-            // 255 workgroups, 13 with 128; 777 x 1302, whose 195 leave 2 MB, 12.1 and 14)
+            // (one set to a workgroup, unless the workgroups' sums would be more than kPartBytes, then two.  One and two, us, of sums of 1.0 MB (64 x 4096
+            // bfloat16) 8.7 and 9.6, 1.9 MB (777 x 1302) 10.4 and 11.1, (1000 x 1024 float32) 8.4 and 9.2, 3.1 MB (200 x 4096 bfloat16) 11.2 and 11.0,
+            // 6.3 MB (100 x 8192) 11.9 and 10.9, 8.0 MB (509 x 4096 float16) 14.7 and 12.1, (128 x 8192 float32) 12.3 both, 18.8 MB (300 x 8192 bfloat16) 15.6 and 14.2)
             const int64_t sets = ceil_div(rows, bwd_threads(v.value) / g.value);
             const int64_t blocks = params && sets * 8 * row_elems > kPartBytes ? ceil_div(sets, 2) : sets;
             parts = (int)(blocks < kBwdMostBlocks ? blocks : kBwdMostBlocks);

@@ -454,8 +454,8 @@ def act_checkpoint(inp, activation):
     r"""``activation(inp)`` (an ``ACT_*`` code, ``torch.nn.GELU()`` or ``torch.nn.ReLU()``; exact GELU, ReLU or none) over rows ``[rows, features]`` or of any
     leading shape, from ``inp`` as it is; for the backward ``inp`` is kept as e4m3 numbers with a power of two for every 32
     elements along a row, 1.03 bytes an element, and the derivative is taken where those are (off by at most 2^-4 of an element,
-    or 2^-10 of the block's scale where it is small against the block).  Nothing is kept where nothing is differentiated.  Float32,
-    bfloat16 and float16."""
+    or 2^-10 of the block's scale where it is small against the block; a ReLU's argument that small is kept as 0, whose slope is 0).
+    Nothing is kept where nothing is differentiated.  Float32, bfloat16 and float16."""
     code = activation if type(activation) is int else _activation_code(activation)
     out = ActCheckpoint.apply(_as_rows(inp), code, torch.is_grad_enabled() and inp.requires_grad)
     return out if inp.dim() == 2 else out.view(inp.shape)
@@ -575,9 +575,9 @@ class MOERoutedMLP(Function):
 
 class MOERoutedMLPCheckpointed(Function):
     r""":class:`MOERoutedMLP` with what the backward needs of the activation kept in 8 bits (``fmoe_native.act_checkpoint_forward``): the
-    pre-activations, or for ReLU and none the activations, whose sign says as much, instead of both in the rows' type: 1.03 bytes an element of ``[rows, d_hidden]``
+    pre-activations, or for ReLU and none the activations, instead of both in the rows' type: 1.03 bytes an element of ``[rows, d_hidden]``
     instead of 4 for a 16-bit GELU layer.  The output is the same; the derivative is taken, and the second linear's weight gradient
-    made, where the numbers kept are."""
+    made, where the numbers kept are (a ReLU's activation of at most 2^-10 of its block's scale is kept as 0, whose slope is 0)."""
 
     @staticmethod
     def forward(ctx, inp, w1, b1, w2, b2, pos_buf, slot_to_row, table, top_k, activation):
