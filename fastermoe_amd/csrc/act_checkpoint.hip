@@ -11,8 +11,8 @@
 //
 // A lane takes eight elements of a row, four lanes a block: one 16-byte load of a 16-bit type, a maximum over the lanes of a quad, eight
 // bytes out.  Rows of whole blocks are one run of such pieces (FLAT); others, of any length, are cut into pieces row by row, and a row's last one is
-// stored in parts.  Bound by memory: 32768 rows of 14336 in bfloat16 with GELU forward 381 us, without y 230, backward 543 (6.1 to 6.2 TB/s;
-// a large copy on the same card 5.0); 32768 of 4096 in float32 207 and 300 (5.8); 32768 of 1302 in bfloat16, whose rows begin anywhere, 44 and 58 (4.8
+// stored in parts.  Bound by memory: 32768 rows of 14336 in bfloat16 with GELU forward 385 us, without y 231, backward 545 (6.1 to 6.2 TB/s;
+// a large copy on the same card 5.0); 32768 of 4096 in float32 207 and 298 (5.9); 32768 of 1302 in bfloat16, whose rows begin anywhere, 44 and 58 (4.8
 // and 5.2).  One piece to a lane: two or four in flight, on a half or a quarter of the workgroups, took 383 and 572 or 413 and 586 us of the first,
 // and 4.8 and 7.0 of the 4.5 and 5.6 that 1554 rows of 1302 take.  A block to a thread, one element after the other, took 21600 for the first.
 #include "common.hpp"

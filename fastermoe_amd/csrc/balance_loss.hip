@@ -12,7 +12,7 @@
 // workgroup's range.  The logits are read once in each direction, some tokens ahead; at these sizes the chain from the first load over the sums
 // to a second launch's results bounds the forward, the memory the larger backward passes (us, forward and backward):
 //   32768 x 256 bf16, top-8    16.5  10.4        131072 x 64 f32, top-2    18.0  13.1 (5.1 TB/s)      8192 x 1024 f32, top-2   17.4  11.5
-//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   14.6   9.1                 1000 x 16 f32, top-2      7.1   2.8
+//   16384 x 64 f32, top-1      11.4   3.6        100000 x 60 bf16, top-2   15.2   9.7                 1000 x 16 f32, top-2      7.1   2.8
 // (A pass for every token's largest logit and sum, one for the sums over the tokens and a workgroup for the results took 158 us of the first's forward,
 // a token to a wave 25 of its backward.)  More than 2048 experts in float32, 32 vectors to a lane, do not fit: 528 bytes of scratch memory to a lane (1024 tokens of 8192
 // experts: 55 us and 34).

@@ -17,13 +17,14 @@
 //   32768 x 1024 bf16             26     5.1        41     4.9         36     5.6
 //   65536 x 900 bf16, residual    85     5.5        86     5.5
 //   32768 x 500 bf16              15     4.4        22     4.4         17     5.8
-//   5000 x 12000 bf16, residual   92     5.2       125     3.8
+//   5000 x 12000 bf16, residual   91     5.3       130     3.7        116     4.1
+//   3600 x 16384 f32, residual   184     5.1       212     4.5        197     4.8
 //   509 x 4096 f16, residual      6.0               13                5.1
 //   64 x 4096 bf16, residual      3.8               8.9               4.1
 // (The first with a row read again for every sum and the parameters' gradients in a pass of their own: 358 and 431 us.  Rows of 900 and 500 whose last
 // elements were loaded and stored apart: 102 and 129, 18 and 27.)  The backward over the longest held rows does not fit its registers: 16-bit rows of 8193 to 16384
-// elements spill 10 to 19 of a lane's 128 to scratch memory (44 to 80 bytes), float32 rows of 4097 to 8192 with a residual 11 of 256 (48), and those of 8193 to 16384 keep
-// 160 bytes there, which goes with their 3.7 to 4.5 TB/s.
+// elements spill 10 to 19 of a lane's 128 to scratch memory (44 to 80 bytes; 3.7 to 4.1 TB/s), float32 rows of 8193 to 16384 keep 160 bytes there (3.7 to 4.5), and those
+// of 4097 to 8192 with a residual spill 11 of 256 (48 bytes; 3001 x 8192 79 us, 5.0 TB/s).
 #include "common.hpp"
 #include "lane_elems.hpp"
 
@@ -208,8 +209,8 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void norm_fwd_kernel(const
 // branch or a select made the sums wait for them).  The lanes keep the sums of grad_y h and grad_y of their columns over all of them; at the end the
 // lanes of one column meet in LDS and part[workgroup] gets 2 d sums.  One workgroup of 1024 to a compute unit: two of 512 leave twice the parts (4096 x 8192:
 // 59 us against 68).  One vector to a lane, where the next set's registers fit beside this one's; longer rows take two and no set ahead, in float32
-// four (ahead) or eight in half the lanes (2048 x 8192, residual: 60 us against 78 with two in 1024 lanes; 3600 x 16384 213 against 249 with four, and
-// 192 against 156 without a residual).
+// four (ahead) or eight in half the lanes (2048 x 8192, residual: 60 us against 78 with two in 1024 lanes; 3600 x 16384 212 against 249 with four, and
+// 191 against 156 without a residual).
 template <int V> struct RowData {
     u32x4 g[V], x[V], gs[V];
     float mean, rstd;
