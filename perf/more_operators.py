@@ -207,8 +207,8 @@ def _plain_int8(s):
     case, x, held, scale, bias = (s[n] for n in ("case", "x", "held", "scale", "bias"))
     h, act = case["h"], case["act"]
     x32 = x.float()
-    row_scale = (x32.abs().amax(dim=1, keepdim=True) / INT8_MAX).clamp(min=LEAST_SCALE)
-    # (quotients next to a half: 64 bits)
+    # (quotients next to a border between two numbers: 64 bits)
+    row_scale = (x32.abs().amax(dim=1, keepdim=True).double() / INT8_MAX).float().clamp(min=LEAST_SCALE)
     q = torch.round(x32.double() / row_scale.double()).float()
     y = torch.zeros(x.shape[0], h, dtype=x.dtype, device=x.device)
     for e, lo, hi in _segments(s["counts"]):
