@@ -103,6 +103,12 @@ SIGNATURES = {
     "fmoe_balance_loss_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "fmoe_act_checkpoint_forward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
     "fmoe_act_checkpoint_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "fmoe_gated_mlp_forward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int, _int]),
+    "fmoe_gated_mlp_forward": (_int, [_vp] * 10 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
+    "fmoe_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int]),
+    "fmoe_gated_mlp_backward": (_int, [_vp] * 13 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
+    "fmoe_quantize_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp]),
     "fmoe_layer_sizes": (_int, [_i64, _i64, _i64, _i64, _i64, _int, _int, _int, _int, _vp]),
     "fmoe_layer_forward": (_int, [_vp] * 17 + [_i64] * 5 + [_int] * 4 + [_vp, _i64, _vp]),
     "fmoe_layer_backward": (_int, [_vp] * 21 + [_i64] * 5 + [_int] * 3 + [_vp, _i64, _vp]),
@@ -116,7 +122,7 @@ PROFILE_CLASSES = ["gemm_fwd", "gemm_dgrad", "gemm_wgrad", "bias_grad", "gather_
 
 F32, BF16, F16, F64 = 0, 1, 2, 3
 GATE_LINEAR, GATE_LOGITS, GATE_ROUTED = 0, 1, 2
-ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 4
 
 _lib = None
 

@@ -1,0 +1,23 @@
+// Interface of the experts' products in 8-bit integers.
+#pragma once
+#include "gemm_kernel.hpp"
+
+namespace fmoe {
+
+// y[r, c] = act(s_r t_c sum_k x[r, k] w[c, k] + bias[c]) of each expert's rows; gated: w has 2 n_cols rows a gate's and then its linear half's,
+// y[r, c] = act(first) second.
+struct Int8Params {
+    const int8_t *x, *w;          // rows of ldx bytes, zeros from the contraction's end to whole 16 bytes; rows of ldw bytes
+    const float *x_scale, *w_scale;
+    const void *bias;             // [E, columns] of y's type, or null
+    void *y;                      // [rows, n_cols]
+    int64_t ldx, ldw, w_expert_stride;   // bytes, multiples of 16
+    int32_t n_cols, k_extent;     // k_extent: bytes of contraction, a multiple of 16
+    int32_t gated, activation;
+    const int32_t *dev_tab;       // segtab layout
+    int64_t n_expert, rows_cap;
+    int dtype;                    // of y
+    int32_t tiles_n, map_off;     // set by the launch
+};
+
+}  // namespace fmoe

@@ -1,0 +1,169 @@
+// Rows rounded to 8-bit integers, each under a scale of its own (gfx950):
+//
+//   s = max(fl32(max|x| / 127), 2^-126)        q = x / s to the nearest integer, ties to even, of the exact quotient
+//
+// A row with an infinity or a NaN has the scale NaN and zeros, so that whatever is made of it is NaN.
+//
+// The exact quotient's rounding, without a division per element: t = x * (1 / s) is off by at most 1.5 2^-16, so rint(t) = q is the right integer or
+// the one beside it, and r = x - q s, one fused multiply-add, is exact (a multiple of ulp(s) or of x's, below 2 s).  So |r| against s / 2 says whether
+// q is off, and a tie is seen as one.
+//
+// A lane takes eight elements at a time.  A row that fits the registers of its wave, or, longer, of its workgroup's four waves, is read once; a longer one is
+// read again, from the caches.
+#include "common.hpp"
+#include "grouped_gemm.hpp"
+#include "lane_elems.hpp"
+
+#include <type_traits>
+
+namespace fmoe {
+namespace {
+
+constexpr int kBlock = 256, kWaves = kBlock / kWave, kLaneElems = 8;
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
+
+struct Params {
+    const void *x;
+    const int64_t *row_index;    // or null: row r is read from row row_index[r] / index_div of x
+    int64_t index_div, x_rows, ldx;
+    int8_t *q;                   // rows of ldq bytes, zeros from d on
+    float *scale;
+    const int32_t *table;        // or null
+    int64_t rows, ldq;
+    int d, dq;                   // features; features rounded up to whole pieces
+    uint8_t *tail;               // or null: rows of tail_bytes bytes, those behind the table's become zeros
+    int64_t tail_bytes;
+};
+
+struct Bytes8 { uint8_t byte[kLaneElems]; };
+
+template <typename T> __device__ __forceinline__ uint32_t magnitude_bits(T v) {
+    return __float_as_uint((float)v) & 0x7fffffffu;   // (ordered as the magnitudes are, infinity and then NaN above them)
+}
+
+__device__ __forceinline__ int8_t round_to(float x, float inv, float s, float half) {
+    float q = rintf(x * inv);
+    const float r = fmaf(-q, s, x), a = fabsf(r);
+    const bool odd = (int)q & 1;
+    if (a > half || (a == half && odd)) q += r > 0.f ? 1.f : -1.f;
+    return (int8_t)(int)q;
+}
+
+// ROW_WAVES: waves that share a row, 1 or all of the workgroup; NV: pieces of a lane that stay in registers (0: the row is read twice)
+template <typename T, int ROW_WAVES, int NV>
+__global__ __launch_bounds__(kBlock) void quantize_rows_kernel(const Params prm) {
+    __shared__ uint32_t most_of[kWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int64_t live = prm.table ? min((int64_t)prm.table[segtab::kRows], prm.rows) : prm.rows;
+    const int64_t row = ROW_WAVES == 1 ? (int64_t)blockIdx.x * kWaves + wave : (int64_t)blockIdx.x;
+    if (row >= live) {   // (ROW_WAVES > 1: the whole workgroup)
+        if (prm.tail && row < prm.rows) {
+            uint8_t *at = prm.tail + row * prm.tail_bytes;   // (bytes: rows of any length)
+            for (int64_t i = ROW_WAVES == 1 ? lane : (int)threadIdx.x; i < prm.tail_bytes; i += ROW_WAVES * kWave) at[i] = 0;
+        }
+        return;
+    }
+    int64_t src = row;
+    bool there = true;
+    if (prm.row_index) {
+        const int64_t idx = prm.row_index[row];
+        src = idx < 0 ? -1 : prm.index_div == 1 ? idx : idx / prm.index_div;
+        there = src >= 0 && src < prm.x_rows;
+    }
+    const T *x = (const T *)prm.x + (there ? src : 0) * prm.ldx;
+    int8_t *q = prm.q + row * prm.ldq;
+    const int first = ((ROW_WAVES == 1 ? 0 : wave * kWave) + lane) * kLaneElems;
+    constexpr int kStep = ROW_WAVES * kWave * kLaneElems;
+    const int d = there ? prm.d : 0;   // (a row from nowhere is one of zeros)
+    T e[NV ? NV : 1][kLaneElems];
+    uint32_t most = 0;
+    auto look = [&](T (&v)[kLaneElems]) {
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) most = max(most, magnitude_bits(v[j]));
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load_elems<false>(x + first + i * kStep, d - first - i * kStep, false, e[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) look(e[i]);
+    } else {
+        for (int c = first; c < d; c += kStep) {
+            load_elems<false>(x + c, d - c, false, e[0]);
+            look(e[0]);
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
+    if (ROW_WAVES > 1) {
+        if (lane == 0) most_of[wave] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = max(most, most_of[w]);
+    }
+    const bool finite = most < 0x7f800000u;
+    const float s = fmaxf(__uint_as_float(finite ? most : 0u) / 127.f, kLeastScale), inv = 1.f / s, half = 0.5f * s;
+    if (first == 0) prm.scale[row] = finite ? s : __uint_as_float(0x7fc00000u);
+    auto store = [&](int c, const T (&v)[kLaneElems]) {
+        Bytes8 b;
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) b.byte[j] = finite ? (uint8_t)round_to((float)v[j], inv, s, half) : 0;
+        if (c < prm.dq) *(uint2 *)(q + c) = __builtin_bit_cast(uint2, b);
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store(first + i * kStep, e[i]);
+    } else {
+        for (int c = first; c < prm.dq; c += kStep) {
+            load_elems<false>(x + c, d - c, false, e[0]);
+            store(c, e[0]);
+        }
+    }
+}
+
+template <typename T> int launch(const Params &prm, hipStream_t stream) {
+    auto go = [&](auto waves, auto nv) {
+        constexpr int W = decltype(waves)::value;
+        const int64_t grid = W == 1 ? ceil_div(prm.rows, kWaves) : prm.rows;
+        quantize_rows_kernel<T, W, decltype(nv)::value><<<(unsigned)grid, kBlock, 0, stream>>>(prm);
+    };
+    typedef std::integral_constant<int, 0> Again;
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
+    typedef std::integral_constant<int, 8> Eight;
+    const int pieces = (int)ceil_div(prm.dq, kWave * kLaneElems);   // of a wave
+    if (pieces <= 1) go(One{}, One{});
+    else if (pieces <= 2) go(One{}, Two{});
+    else if (pieces <= 4) go(Four{}, One{});
+    else if (pieces <= 8) go(Four{}, Two{});
+    else if (pieces <= 16) go(Four{}, Four{});
+    else if (pieces <= 32) go(Four{}, Eight{});
+    else go(Four{}, Again{});
+    FMOE_LAUNCH_CHECK();
+    return FMOE_OK;
+}
+
+}  // namespace
+}  // namespace fmoe
+
+using namespace fmoe;
+
+extern "C" int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index, int64_t index_div, int64_t x_rows, void *q, int64_t ldq,
+                                  void *scale, const void *segment_table, void *tail, int64_t tail_bytes, int64_t rows, int64_t row_elems, int dtype,
+                                  void *stream) {
+    const char *who = "fmoe_quantize_rows";
+    FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who, dtype);
+    FMOE_REQUIRE(rows >= 0 && row_elems >= 0 && x_rows >= 0, "%s: bad sizes", who);
+    FMOE_REQUIRE(row_index == nullptr || index_div >= 1, "%s: index_div=%lld", who, (long long)index_div);
+    FMOE_REQUIRE(row_index != nullptr || x_rows >= rows, "%s: %lld rows of %lld", who, (long long)rows, (long long)x_rows);
+    FMOE_REQUIRE(tail == nullptr || (segment_table != nullptr && tail_bytes >= 0), "%s: a tail goes with a segment table", who);
+    if (rows > kMostThreads / kBlock || row_elems > (int64_t)(1 << 28)) return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
+    const int64_t whole = ceil_div(row_elems, 16) * 16;
+    FMOE_REQUIRE(ldq >= whole && ldq % 16 == 0 && aligned16(q), "%s: rows of 8-bit integers begin on 16 bytes, at least %lld apart", who, (long long)whole);
+    if (rows == 0) return FMOE_OK;
+    FMOE_REQUIRE((x || row_elems == 0 || x_rows == 0) && (q || row_elems == 0) && scale, "%s: NULL pointer", who);
+    const Params prm{x, row_index, index_div, x_rows, ldx, (int8_t *)q, (float *)scale, (const int32_t *)segment_table, rows, ldq, (int)row_elems,
+                     (int)whole, (uint8_t *)tail, tail_bytes};
+    if (dtype == FMOE_F32) return launch<float>(prm, (hipStream_t)stream);
+    return dtype == FMOE_BF16 ? launch<__bf16>(prm, (hipStream_t)stream) : launch<_Float16>(prm, (hipStream_t)stream);
+}

@@ -871,6 +871,200 @@ def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=
     return grad_x, mid
 
 
+# ---- gated experts ------------------------------------------------------------------------
+
+_GATE_ACTIVATIONS = (_lib.ACT_NONE, _lib.ACT_RELU, _lib.ACT_GELU, _lib.ACT_SILU)
+
+
+def gated_mlp_supported(dtype):
+    """Whether gated experts of this type are one call."""
+    return dtype in (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _gate_activation(activation):
+    if activation not in _GATE_ACTIVATIONS:
+        raise ValueError(f"unknown activation code {activation}")
+    return activation
+
+
+def _exact_table(table, n_expert, rows, device):
+    """A segment table for just these experts and rows."""
+    _near("segment_table", _dev("segment_table", table, torch.int32), device)
+    need = _lib.load().fmoe_segment_table_bytes(int(rows), int(n_expert)) // 4
+    if table.numel() != need:
+        raise ValueError(f"segment_table has {table.numel()} entries, {need} expected for {rows} rows / {n_expert} experts")
+    return table
+
+
+def _gated_args(x, w1, b1, w2, b2):
+    """Checks of a gated block's tensors; the code of their type and ``(experts, rows, d_model, d_hidden)``."""
+    dt = _rows("x", x)
+    if not gated_mlp_supported(x.dtype):
+        raise TypeError(f"gated_mlp does not take {x.dtype}")
+    for name, t in (("w1", w1), ("b1", b1), ("w2", w2), ("b2", b2)):
+        if t is not None:
+            _near(name, _dev(name, t, x.dtype), x.device)
+    if w1.dim() != 3 or w1.shape[2] != x.shape[1] or w1.shape[1] % 2 or 0 in w1.shape:
+        raise ValueError(f"w1 must be [num_expert, 2 * d_hidden, {x.shape[1]}], got {tuple(w1.shape)}")
+    e, h, d = w1.shape[0], w1.shape[1] // 2, x.shape[1]
+    if tuple(w2.shape) != (e, d, h):
+        raise ValueError(f"w2 must be {(e, d, h)}, got {tuple(w2.shape)}")
+    if b1 is not None and tuple(b1.shape) != (e, 2 * h):
+        raise ValueError(f"b1 must be {(e, 2 * h)}, got {tuple(b1.shape)}")
+    if b2 is not None and tuple(b2.shape) != (e, d):
+        raise ValueError(f"b2 must be {(e, d)}, got {tuple(b2.shape)}")
+    return dt, e, x.shape[0], d, h
+
+
+def _gated_segments(table, counts, n_expert, rows, device):
+    """Pointers of a segment table or of the counts on the host, one of which there is."""
+    if table is not None:
+        return _ptr(_exact_table(table, n_expert, rows, device)), None, None
+    counts = _host_counts("expert_count", counts, n_expert)
+    return None, ctypes.c_void_p(counts.data_ptr()), counts
+
+
+def gated_mlp_forward(x, w1, b1, w2, b2, activation, table=None, expert_count=None, keep=True):
+    """``(y, pre, mid)`` of gated experts: ``pre = x @ w1_e^T + b1_e`` (a gate's half and a linear one), ``mid = act(gate) * linear``,
+    ``y = mid @ w2_e^T + b2_e``.  The rows' segments: ``table`` (:func:`segment_table` for as many rows as ``x`` has), or ``expert_count`` (int64, CPU).
+    ``keep=False``: ``pre`` and ``mid`` are ``None``.  Rows of ``y`` behind the experts' are zeros."""
+    dt, e, n, d, h = _gated_args(x, w1, b1, w2, b2)
+    activation = _gate_activation(activation)
+    seg, cnt, hold = _gated_segments(table, expert_count, e, n, x.device)
+    y = torch.empty(n, d, dtype=x.dtype, device=x.device)
+    pre = torch.empty(n, 2 * h, dtype=x.dtype, device=x.device) if keep else None
+    mid = torch.empty(n, h, dtype=x.dtype, device=x.device)
+    lib = _lib.load()
+    with _on(x.device):
+        ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep)), x.device)
+        check(lib.fmoe_gated_mlp_forward(_ptr(x), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(pre), _ptr(mid), _ptr(y), seg, cnt, e, n, d, h, dt,
+                                         activation, _ptr(ws), ws.numel(), _stream(x)))
+    return y, pre, mid if keep else None
+
+
+def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table=None, expert_count=None, want_x=True, want_w1=True, want_b1=True,
+                       want_w2=True, want_b2=True):
+    """``(grad_x, grad_w1, grad_b1, grad_w2, grad_b2)`` from what :func:`gated_mlp_forward` left; ``None`` where not wanted."""
+    dt, e, n, d, h = _gated_args(x, w1, None, w2, None)
+    activation = _gate_activation(activation)
+    for name, t, shape in (("grad_y", grad_y, (n, d)), ("pre", pre, (n, 2 * h)), ("mid", mid, (n, h))):
+        _near(name, _dev(name, t, x.dtype), x.device)
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    seg, cnt, hold = _gated_segments(table, expert_count, e, n, x.device)
+    new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None
+    grad_x = new(want_x, n, d)
+    grad_w1, grad_b1 = new(want_w1 or want_b1, e, 2 * h, d), new(want_b1, e, 2 * h)
+    grad_w2, grad_b2 = new(want_w2 or want_b2, e, d, h), new(want_b2, e, d)
+    lib = _lib.load()
+    with _on(x.device):
+        ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation), x.device)
+        check(lib.fmoe_gated_mlp_backward(_ptr(grad_y), _ptr(x), _ptr(w1), _ptr(w2), _ptr(pre), _ptr(mid), _ptr(grad_x), _ptr(grad_w1), _ptr(grad_b1),
+                                          _ptr(grad_w2), _ptr(grad_b2), seg, cnt, e, n, d, h, dt, activation, _ptr(ws), ws.numel(), _stream(x)))
+    return grad_x, grad_w1 if want_w1 else None, grad_b1, grad_w2 if want_w2 else None, grad_b2
+
+
+# ---- experts in 8-bit integers ------------------------------------------------------------
+
+INT8_ROW_BYTES = 16   # rows of 8-bit integers begin on these
+
+
+def _int8_rows(n, d, device):
+    """Rows of ``d`` 8-bit integers as the products read them: whole 16-byte pieces."""
+    whole = -(-d // INT8_ROW_BYTES) * INT8_ROW_BYTES
+    return torch.empty(n, whole, dtype=torch.int8, device=device)
+
+
+def quantize_rows(x, row_index=None, index_div=1, table=None, tail=None):
+    """``(q, scale)`` of rows ``x [rows, features]``: int8 and float32 ``[rows]`` with ``x ~ q * scale[:, None]``, ``scale`` a 127th of a row's largest
+    magnitude.  ``q``'s rows lie whole 16-byte pieces apart.  ``row_index`` (int64): row ``r`` is made of row ``row_index[r] // index_div`` of
+    ``x``.  ``table``: only the rows of this segment table are made, and those behind them in ``tail [rows, ..]`` become zeros."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x must be a torch.Tensor, got {type(x).__name__}")
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"quantize_rows does not take {x.dtype}")
+    x, ldx = _strided_rows("x", x)
+    n, d = x.shape
+    if row_index is not None:
+        _near("row_index", _dev("row_index", row_index, torch.int64), x.device)
+        n = row_index.numel()
+        if int(index_div) < 1:
+            raise ValueError(f"index_div is {index_div}")
+    if tail is not None and (table is None or tail.shape[0] != n or not tail.is_contiguous() or tail.device != x.device):
+        raise ValueError("tail must be as many adjacent rows, with a segment table")
+    q = _int8_rows(n, d, x.device)
+    scale = torch.empty(n, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        check(_lib.load().fmoe_quantize_rows(_ptr(x), ldx, _ptr(row_index), int(index_div), x.shape[0], _ptr(q), q.shape[1], _ptr(scale),
+                                             _live_rows(table, n, x.device), _ptr(tail), 0 if tail is None else tail.shape[1] * tail.element_size(),
+                                             n, d, _DTYPES[x.dtype], _stream(x)))
+    return q[:, :d], scale
+
+
+def int8_layout(weight):
+    """``weight`` (int8 ``[E, out, in]``) where its rows lie as :func:`linear_int8` reads them, whole 16-byte pieces apart (as :func:`quantize_rows`
+    leaves them), else a copy that does."""
+    e, out, d = weight.shape
+    whole = -(-d // INT8_ROW_BYTES) * INT8_ROW_BYTES
+    by_expert, by_row, by_elem = weight.stride()
+    last = weight.storage_offset() + (e - 1) * by_expert + (out - 1) * by_row + whole   # (what a row's last piece may read up to)
+    if ((by_elem == 1 or d == 1) and by_row % INT8_ROW_BYTES == 0 and by_row >= whole and by_expert % INT8_ROW_BYTES == 0
+            and weight.data_ptr() % 16 == 0 and last <= weight.untyped_storage().nbytes()):
+        return weight
+    held = torch.empty(e, out, whole, dtype=torch.int8, device=weight.device)[:, :, :d]
+    return held.copy_(weight)
+
+
+def _int8_weights(weight, scale, device):
+    """``weight [E, out, in]`` with rows that the kernels read where they lie; others are copied."""
+    for name, t, dtype in (("weight", weight, torch.int8), ("weight_scale", scale, torch.float32)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must have dtype {dtype}, got {t.dtype}")
+        _near(name, t, device)
+    if weight.dim() != 3 or 0 in weight.shape:
+        raise ValueError(f"weight must be [num_expert, out_feat, in_feat], got {tuple(weight.shape)}")
+    e, out, d = weight.shape
+    if tuple(scale.shape) != (e, out):
+        raise ValueError(f"weight_scale must be {(e, out)}, got {tuple(scale.shape)}")
+    weight = int8_layout(weight)
+    by_expert, by_row, _ = weight.stride()
+    return weight, by_expert, by_row, scale.contiguous()
+
+
+def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_NONE, gated=False, row_index=None, index_div=1):
+    """``act((q_x @ weight_e^T) * scale_x * weight_scale_e + bias_e)`` over the segments of ``table`` (:func:`segment_table` for as many rows as
+    ``x``, or ``row_index``, has), ``q_x, scale_x`` the rows of :func:`quantize_rows`; in ``x``'s type.  ``gated``: the first half of ``weight``'s
+    rows is a gate's, the result ``act(first) * second``.  Rows behind the experts' are zeros."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x must be a torch.Tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"x must be a CUDA (HIP) tensor, got device {x.device}")
+    if x.dim() != 2:
+        raise ValueError(f"x must be 2-D [rows, features], got shape {tuple(x.shape)}")
+    weight, by_expert, by_row, weight_scale = _int8_weights(weight, weight_scale, x.device)
+    activation = _gate_activation(activation)
+    e, out, d = weight.shape
+    if x.shape[1] != d:
+        raise ValueError(f"x has {x.shape[1]} features, weight expects {d}")
+    if gated and out % 2:
+        raise ValueError(f"a gated product's weight has an even number of rows, got {out}")
+    if bias is not None:
+        _near("bias", _dev("bias", bias, x.dtype), x.device)
+        if tuple(bias.shape) != (e, out):
+            raise ValueError(f"bias must be {(e, out)}, got {tuple(bias.shape)}")
+    n = x.shape[0] if row_index is None else row_index.numel()
+    out = out // 2 if gated else out
+    _exact_table(table, e, n, x.device)
+    y = torch.empty(n, out, dtype=x.dtype, device=x.device)
+    q, scale = quantize_rows(x, row_index, index_div, table, y)
+    with _on(x.device):
+        check(_lib.load().fmoe_linear_int8(_ptr(q), q.stride(0), _ptr(scale), _ptr(weight), by_row, by_expert, _ptr(weight_scale), _ptr(bias), _ptr(y),
+                                           _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _stream(x)))
+    return y
+
+
 # ---- layer norm of token rows -----------------------------------------------------------
 
 def _near(name, t, device):

@@ -731,6 +731,156 @@ def nothing_watches(*tensors):
             and (not _modes_watch() or saving_is_watched()))
 
 
+def _gate_activation_code(activation):
+    """The code of an activation that gated experts and products in 8 bits take; an ``ACT_*`` code stays what it is."""
+    if type(activation) is int:
+        return activation
+    if isinstance(activation, torch.nn.SiLU) or activation is torch.nn.functional.silu:
+        return _lib.ACT_SILU
+    return _activation_code(activation)
+
+
+def _segments(expert_count, table, n_expert, rows, device):
+    """The segment table of ``rows`` rows: ``table``, or one made of ``expert_count`` (int64 ``[n_expert]``, on the device or the CPU)."""
+    if table is not None:
+        return table
+    if not isinstance(expert_count, torch.Tensor):
+        raise TypeError(f"expert_count must be a torch.Tensor, got {type(expert_count).__name__}")
+    if expert_count.dtype != torch.int64:
+        raise TypeError(f"expert_count must have dtype torch.int64, got {expert_count.dtype}")
+    if expert_count.numel() != n_expert:
+        raise ValueError(f"expert_count has {expert_count.numel()} entries, expected {n_expert}")
+    if not expert_count.is_cuda:
+        expert_count = _checked_counts(expert_count, n_expert, rows).to(device)
+    elif expert_count.device != device:
+        raise ValueError(f"expert_count is on {expert_count.device}, expected {device}")
+    return fmoe_native.segment_table(expert_count.reshape(-1).contiguous(), rows)
+
+
+def _checked_counts(expert_count, n_expert, rows):
+    """Counts on the CPU that ``rows`` rows can have."""
+    counts = fmoe_native._host_counts("expert_count", expert_count, n_expert)
+    if counts.numel() and (int(counts.min()) < 0 or int(counts.sum()) > rows):
+        raise ValueError(f"expert_count sums to {int(counts.sum())} (least {int(counts.min())}) but there are {rows} rows")
+    return counts
+
+
+def _segments_on_host(expert_count, table, n_expert, rows):
+    """The counts of ``table`` or ``expert_count`` on the CPU (read from the device where they are there)."""
+    if table is not None:
+        at = table[8:8 + n_expert + 1].cpu().to(torch.int64)
+        return at[1:] - at[:-1]
+    return _checked_counts(expert_count.cpu() if isinstance(expert_count, torch.Tensor) else expert_count, n_expert, rows)
+
+
+class GatedMLP(Function):
+    r"""Gated experts over expert-sorted rows as one node (see :func:`gated_mlp`); ``counts``: on the CPU, in a table's place."""
+
+    @staticmethod
+    def forward(ctx, inp, w1, b1, w2, b2, table, counts, activation, keep):
+        inp = inp.contiguous()
+        out, pre, mid = fmoe_native.gated_mlp_forward(inp, w1, b1, w2, b2, activation, table, counts, keep)
+        if keep:
+            ctx.save_for_backward(inp, w1, w2, pre, mid, table, counts)
+            ctx.moe_args = activation, b1 is not None, b2 is not None
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        inp, w1, w2, pre, mid, table, counts = map(_as_chunks, ctx.saved_tensors)
+        activation, bias1, bias2 = ctx.moe_args
+        need = ctx.needs_input_grad
+        grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), inp, w1, w2, pre, mid, activation, table, counts, need[0], need[1],
+                                               bias1 and need[2], need[3], bias2 and need[4])
+        return (*grads, None, None, None, None)
+
+
+def _over_a_table(inp, w1, w2, *biases):
+    """Whether a gated block runs over a table on the device: 16-bit types always, float32 in sizes and from addresses of whole 16 bytes."""
+    return inp.dtype != torch.float32 or (
+        fmoe_native.linear_dev_supported(inp.shape[1], w2.shape[2] if w2.dim() == 3 else 0, inp.dtype)
+        and all(t is None or t.data_ptr() % 16 == 0 for t in (inp, w1, w2, *biases)))
+
+
+def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
+    r"""Gated feed-forward block of every expert over its rows: ``w2_e (act(g) * u) + b2_e`` with ``[g u] = w1_e x + b1_e``, in one call each way.
+    ``inp [rows, d_model]`` (bfloat16, float16, float32) sorted by expert; ``w1 [E, 2 * d_hidden, d_model]``, the gate's rows first, ``w2
+    [E, d_model, d_hidden]``, ``b1``, ``b2`` or ``None``; ``activation``: ``torch.nn.SiLU()``, exact ``GELU()``, ``ReLU()``, ``None`` or an
+    ``ACT_*`` code.  ``expert_count`` (int64 ``[E]``): rows of each expert, on the device (nothing is read back) or the CPU; or ``table``,
+    their :func:`fmoe_native.segment_table` for as many rows, which a routing call leaves.  Rows behind the counted ones come out as
+    zeros, and so do their gradients.  Differentiable once, with respect to ``inp``, the weights and the biases; the gradients are made from ``g``, ``u``
+    and ``act(g) * u`` as ``inp``'s type holds them.  (float32 in sizes or from addresses that are no multiple of 16 bytes: the counts are read on the host.)"""
+    code = _gate_activation_code(activation)
+    fmoe_native._gated_args(inp if inp.is_contiguous() else inp.contiguous(), w1, b1, w2, b2)
+    counts = None
+    if _over_a_table(inp, w1, w2, b1, b2):
+        table = _segments(expert_count, table, w1.shape[0], inp.shape[0], inp.device)
+    else:
+        counts, table = _segments_on_host(expert_count, table, w1.shape[0], inp.shape[0]), None
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (inp, w1, b1, w2, b2))
+    return GatedMLP.apply(inp, w1, b1, w2, b2, table, counts, code, keep)
+
+
+def quantize_rows(inp):
+    r"""``(q, scale)``: ``inp [.., features]`` (float32, bfloat16, float16) rounded to 8-bit integers along its last dimension, ``q`` int8 of ``inp``'s shape and
+    ``scale`` float32 of its leading one, ``inp ~ q * scale``.  ``scale`` is a 127th of the largest magnitude (at least ``2^-126``), ``q`` the integer nearest to
+    ``inp / scale``, ties to even; a row with an infinity or a NaN has the scale NaN.  What :func:`linear_int8` does with its rows, and what makes its weights:
+    ``q``'s rows lie whole 16 bytes apart, as the products read them.  Not differentiable."""
+    with torch.no_grad():
+        q, scale = fmoe_native.quantize_rows(_as_rows(inp.detach()))
+    if inp.dim() == 2:
+        return q, scale
+    lead, whole = inp.shape[:-1], q.stride(0)
+    strides = [whole]
+    for size in reversed(lead[1:]):
+        strides.insert(0, strides[0] * size)
+    return q.as_strided(inp.shape, (*strides[:len(lead)], 1)), scale.view(lead)
+
+
+def linear_int8(inp, expert_count, weight, weight_scale, bias=None, activation=None, gated=False, table=None, row_index=None, index_div=1):
+    r"""Every expert's ``act(x w_e^T + bias_e)`` over its rows in 8-bit integers, for inference: ``inp [rows, in_feat]`` (bfloat16, float16, float32), sorted
+    by expert, is rounded as :func:`quantize_rows` does, a scale to each row; ``weight`` int8 ``[E, out_feat, in_feat]`` and ``weight_scale`` float32 ``[E,
+    out_feat]`` are that function's results for an expert's weights (rows that do not begin on 16 bytes are copied in every call).  The sums are
+    exact (``in_feat`` up to 131072), the result is of ``inp``'s type.  ``gated``: ``weight`` has the rows of a gate and then as many of a linear half, the
+    result is ``act(first) * second``.  ``expert_count``, ``table``: as for :func:`gated_mlp`.  ``row_index`` (int64, one entry per sorted row): row ``r``
+    is ``inp[row_index[r] // index_div]``.  Rows behind the counted ones come out as zeros."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (inp, bias, weight_scale)):
+        raise NotImplementedError("linear_int8 has no gradients: call it under torch.no_grad(), or with tensors that require none")
+    code = _gate_activation_code(activation)
+    rows = inp.shape[0] if row_index is None else row_index.numel()
+    table = _segments(expert_count, table, weight.shape[0], rows, inp.device)
+    return fmoe_native.linear_int8(inp, table, weight, weight_scale, bias, code, gated, row_index, index_div)
+
+
+class MOERoutedGatedMLP(Function):
+    r"""``MOEScatter`` and gated experts over the rows as the routing kernels left them, as :class:`MOERoutedMLP` does for plain ones: returns their output
+    in expert-sorted order, one row per slot."""
+
+    @staticmethod
+    def forward(ctx, inp, w1, b1, w2, b2, pos_buf, slot_to_row, table, top_k, activation, save):
+        inp = inp.contiguous()
+        rows = fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)
+        out, pre, mid = fmoe_native.gated_mlp_forward(rows, w1, b1, w2, b2, activation, table, keep=save)
+        if save:
+            ctx.save_for_backward(inp, w1, w2, pre, mid, pos_buf, slot_to_row, table)
+        ctx.moe_args = top_k, activation, b1 is not None, b2 is not None
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        inp, w1, w2, pre, mid, pos_buf, slot_to_row, table = map(_as_chunks, ctx.saved_tensors)
+        top_k, activation, bias1, bias2 = ctx.moe_args
+        need = ctx.needs_input_grad
+        rows = fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)   # (made again, not kept: see MOERoutedMLP)
+        g_rows, *grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), rows, w1, w2, pre, mid, activation, table, None, need[0], need[1],
+                                                        bias1 and need[2], need[3], bias2 and need[4])
+        del rows
+        g_inp = fmoe_native.reduce_slots(g_rows, slot_to_row, inp.shape[0], top_k) if need[0] else None
+        return (g_inp, *grads, None, None, None, None, None, None)
+
+
 class MOEGather(Function):
     r"""Expert-sorted rows -> slot order, zero rows for dropped slots
     (fmoe/functions.py:278-330).  ``slot_to_row`` (optional extra) is the inverse

@@ -53,11 +53,12 @@ def mark_module_parallel_comm(module, comm):
 
 def _own_expert_path(expert_fn, experts):
     """True when ``expert_fn`` is :meth:`FMoE.expert_fn` itself (not overridden, not replaced on the
-    instance) and ``experts`` is this package's ``_Expert`` with its own ``forward``: only then may
+    instance) and ``experts`` is this package's ``_Expert`` (or its gated or 8-bit form) with its own ``forward``: only then may
     the layer skip handing rows and counts through ``expert_fn``."""
-    from .transformer import _Expert
+    from .transformer import _Expert, _GatedExpert, _Int8Expert
     return (getattr(expert_fn, "__func__", None) is FMoE.expert_fn
-            and isinstance(experts, _Expert) and type(experts).forward is _Expert.forward)
+            and isinstance(experts, (_Expert, _Int8Expert))
+            and type(experts).forward in (_Expert.forward, _GatedExpert.forward, _Int8Expert.forward))
 
 
 def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_expert, world_size,
@@ -82,9 +83,9 @@ def _fmoe_general_global_forward(inp, gate, expert_fn, policy_fn, experts, num_e
     # rows and CPU counts it can read (fmoe/layers.py:117-140).
     own = (inp.is_cuda and gate.is_cuda and inp.dim() == 2 and inp.shape[0] > 0
            and gate.numel() == inp.shape[0] * topk and fused and _own_expert_path(expert_fn, experts))
-    if enable_fuse:   # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way)
-        from .transformer import _Expert
-        enable_fuse = not (isinstance(experts, _Expert) and experts._checkpoints(inp))
+    if enable_fuse:   # (the pipeline keeps its buffers whole: experts that keep their activations in 8 bits go the other way, as do those it does not have)
+        from .transformer import _Expert, _GatedExpert, _Int8Expert
+        enable_fuse = not isinstance(experts, (_GatedExpert, _Int8Expert)) and not (isinstance(experts, _Expert) and experts._checkpoints(inp))
     if own:
         _single_worker(world_size, "count_by_gate")
         enable_fuse = enable_fuse and not experts.unchunked_is_faster(inp, gate.numel())

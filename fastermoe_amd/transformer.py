@@ -5,8 +5,9 @@ import torch
 import torch.nn as nn
 
 from . import _lib, fmoe_native
-from .functions import (MOEExpertMLP, MOEExpertMLPCheckpointed, MOERoutedMLP, MOERoutedMLPCheckpointed, _no_hooks, add_layer_norm,
-                        layer_call, layer_norm, nothing_watches)
+from .functions import (MOEExpertMLP, MOEExpertMLPCheckpointed, MOERoutedGatedMLP, MOERoutedMLP, MOERoutedMLPCheckpointed,
+                        _gate_activation_code, _no_hooks, _over_a_table, add_layer_norm, gated_mlp, layer_call, layer_norm, linear_int8,
+                        nothing_watches, quantize_rows)
 from .gates import NaiveGate
 from .layers import FMoE, FMoELinear
 
@@ -131,6 +132,128 @@ class _Expert(nn.Module):
             return None
 
 
+def _gate_code_or_none(activation):
+    """The code of an activation that the kernels of gated experts and of experts in 8 bits have."""
+    try:
+        return _gate_activation_code(activation)
+    except NotImplementedError:
+        return None
+
+
+class _GatedExpert(_Expert):
+    r"""All experts of a worker as gated blocks, ``h4toh(act(g) * u)`` with ``[g u] = htoh4(x)``: ``htoh4`` has ``2 * d_hidden`` outputs, the
+    gate's first.  With SiLU, exact GELU, ReLU or no activation one call each way (:func:`fastermoe_amd.functions.gated_mlp`), else the
+    modules one by one."""
+
+    def __init__(self, num_expert, d_model, d_hidden, activation, rank=0, bias=True):
+        super().__init__(num_expert, d_model, d_hidden, activation, rank=rank, bias=bias)
+        self.htoh4 = FMoELinear(num_expert, d_model, 2 * d_hidden, bias=bias, rank=rank)
+
+    def _checkpoints(self, inp):
+        if self.act_checkpoint and inp.is_cuda and self._saves(inp):
+            raise NotImplementedError("act_checkpoint does not take gated experts")
+        return False
+
+    def _one_call(self, inp):
+        """The activation's code where the block is one call, else ``None``."""
+        if not (inp.is_cuda and fmoe_native.gated_mlp_supported(inp.dtype) and os.environ.get("FMOE_EXPERT_EPILOGUE", "1") != "0"
+                and all(p is None or p.dtype == inp.dtype for linear in (self.htoh4, self.h4toh) for p in (linear.weight, linear.bias))):
+            return None
+        return _gate_code_or_none(self.activation)
+
+    def forward(self, inp, fwd_expert_count):
+        code = self._one_call(inp)
+        self._checkpoints(inp)
+        if code is not None:
+            return gated_mlp(inp, fwd_expert_count, self.htoh4.weight, self.htoh4.bias, self.h4toh.weight, self.h4toh.bias, code)
+        gate, linear = self.htoh4(inp, fwd_expert_count).chunk(2, dim=1)
+        x = self.activation(gate) if self.activation is not None else gate
+        return self.h4toh((x * linear).contiguous(), fwd_expert_count)
+
+    def routed_forward(self, inp, pos_buf, slot_to_row, counts_dev, top_k, table=None):
+        if not self._device_tables_apply(inp):
+            return None
+        self._checkpoints(inp)
+        if table is None:
+            table = fmoe_native.segment_table(counts_dev, pos_buf.numel())
+        return MOERoutedGatedMLP.apply(inp, self.htoh4.weight, self.htoh4.bias, self.h4toh.weight, self.h4toh.bias, pos_buf, slot_to_row, table,
+                                       top_k, self._one_call(inp), self._saves(inp))
+
+    def routed_layer(self, inp, gate_w, gate_b, score, routing, top_k):
+        return None
+
+    def unchunked_is_faster(self, inp, n_slots):
+        return True   # (the pipeline has no gated experts)
+
+    def _device_tables_apply(self, inp):
+        return (self._one_call(inp) is not None and os.environ.get("FMOE_DEVICE_TABLES", "1") != "0"
+                and _over_a_table(inp, self.htoh4.weight, self.h4toh.weight, self.htoh4.bias, self.h4toh.bias))
+
+
+class _Int8Expert(nn.Module):
+    r"""The experts of ``experts`` for inference, their weights in 8-bit integers with a scale to each output channel and their rows rounded to the same as they come (:func:`fastermoe_amd.functions.linear_int8`).
+    Biases stay as they are."""
+
+    act_checkpoint = False
+
+    def __init__(self, experts):
+        super().__init__()
+        if type(experts) not in (_Expert, _GatedExpert):
+            raise TypeError(f"only this package's own experts are held in 8 bits, got {type(experts).__name__}")
+        self.activation, self.gated = experts.activation, isinstance(experts, _GatedExpert)
+        if _gate_code_or_none(self.activation) is None:
+            raise NotImplementedError(f"experts in 8 bits take SiLU, GELU, ReLU or no activation, got {self.activation!r}")
+        for name in ("htoh4", "h4toh"):
+            linear = getattr(experts, name)
+            q, scale = quantize_rows(linear.weight)
+            self.register_buffer(name + "_weight", q)
+            self.register_buffer(name + "_scale", scale)
+            self.register_buffer(name + "_bias", None if linear.bias is None else linear.bias.detach())
+
+    def _apply(self, fn, recurse=True):
+        # (scales are float32 and rows lie whole 16 bytes apart, whatever type or device the layer moves to)
+        scales = {name: self._buffers[name] for name in ("htoh4_scale", "h4toh_scale")}
+        super()._apply(fn, recurse)
+        for name, scale in scales.items():
+            if self._buffers[name].dtype != torch.float32:
+                self._buffers[name] = scale.to(self._buffers[name].device)
+        for name in ("htoh4_weight", "h4toh_weight"):
+            self._buffers[name] = fmoe_native.int8_layout(self._buffers[name])
+        return self
+
+    def _product(self, inp, table, name, activation, gated, expert_count=None, **rows):
+        bias = getattr(self, name + "_bias")
+        return linear_int8(inp, expert_count, getattr(self, name + "_weight"), getattr(self, name + "_scale"),
+                           None if bias is None else bias.to(inp.dtype), activation, gated, table, **rows)
+
+    def _inference_only(self, inp):
+        if torch.is_grad_enabled() and inp.requires_grad:
+            raise NotImplementedError("experts in 8 bits have no gradients: call the layer under torch.no_grad()")
+
+    def forward(self, inp, fwd_expert_count):
+        self._inference_only(inp)
+        with torch.no_grad():
+            mid = self._product(inp, None, "htoh4", self.activation, self.gated, fwd_expert_count)
+            return self._product(mid, None, "h4toh", None, False, fwd_expert_count)
+
+    def routed_forward(self, inp, pos_buf, slot_to_row, counts_dev, top_k, table=None):
+        self._inference_only(inp)
+        with torch.no_grad():
+            if table is None:
+                table = fmoe_native.segment_table(counts_dev, pos_buf.numel())
+            mid = self._product(inp, table, "htoh4", self.activation, self.gated, row_index=pos_buf, index_div=top_k)
+            return self._product(mid, table, "h4toh", None, False)
+
+    def routed_layer(self, inp, gate_w, gate_b, score, routing, top_k):
+        return None
+
+    def unchunked_is_faster(self, inp, n_slots):
+        return True   # (the pipeline has no products in 8 bits)
+
+    def _checkpoints(self, inp):
+        return False
+
+
 def _gen_policy(alpha):
     r"""Shadowing policy factory (fmoe/transformer.py:33-87).  Shadowing copies
     experts between workers; with one worker the policy selects nothing."""
@@ -145,6 +268,8 @@ class FMoETransformerMLP(FMoE):
     r"""``Linear(d_model, d_hidden) -> activation -> Linear(d_hidden, d_model)`` per
     expert, any leading input shape (fmoe/transformer.py:89-139)."""
 
+    _expert_class = _Expert
+
     def __init__(self, num_expert=32, d_model=1024, d_hidden=4096, world_size=1, mp_group=None,
                  moe_group=None, activation=torch.nn.GELU(), gate=NaiveGate, top_k=2,
                  expert_dp_comm="none", gate_hook=None, bias=True, mask=None, mask_dict=None):
@@ -152,7 +277,7 @@ class FMoETransformerMLP(FMoE):
                          world_size=world_size, mp_group=mp_group, moe_group=moe_group,
                          gate_hook=gate_hook, mask=mask, policy_fn=_gen_policy(d_hidden / d_model),
                          mask_dict=mask_dict)
-        self.experts = _Expert(num_expert, d_model, d_hidden, activation, rank=self.mp_rank, bias=bias)
+        self.experts = self._expert_class(num_expert, d_model, d_hidden, activation, rank=self.mp_rank, bias=bias)
         self.mark_parallel_comm(expert_dp_comm)
 
     def forward(self, inp: torch.Tensor):
@@ -177,13 +302,38 @@ class FMoETransformerMLP(FMoE):
         self.experts.act_checkpoint = bool(on)
 
 
+    def quantize_experts(self):
+        r"""Holds the experts in 8-bit integers from here on, for inference: weights with a scale to each output channel, rows rounded with a scale of their own
+        as they come, exact sums.  Half of the memory of 16-bit weights, and half of the bytes that a decoding step reads.  The experts have no
+        parameters afterwards; calls that would need their gradients raise.  Returns the layer."""
+        self.experts = _Int8Expert(self.experts)
+        return self
+
+
+def _gated_defaults(args, kwargs):
+    """A layer's arguments, with SiLU where no activation is named (it is the seventh)."""
+    return kwargs if len(args) > 6 or "activation" in kwargs else dict(kwargs, activation=nn.SiLU())
+
+
+class FMoEGatedMLP(FMoETransformerMLP):
+    r""":class:`FMoETransformerMLP` with gated experts (not in the reference): ``h4toh(activation(g) * u)`` with ``[g u] = htoh4(x)``, ``htoh4`` with
+    ``2 * d_hidden`` outputs, the gate's first.  ``activation`` is SiLU unless given.  The pipeline of ``enable_fuse`` stands back for gated experts."""
+
+    _expert_class = _GatedExpert
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **_gated_defaults(args, kwargs))
+
+
 class FMoEPositionwiseFF(FMoETransformerMLP):
     r"""The layer in a transformer block, with the layer norm and the residual around it (``CustomizedMoEPositionwiseFF``,
     examples/transformer-xl/mem_transformer.py:379-409): ``x + layer(norm(x))`` with ``pre_lnorm``, else ``norm(x + layer(x))``, with dropout on
-    the layer's output.  Further arguments are those of :class:`FMoETransformerMLP`."""
+    the layer's output.  ``gated``: with gated experts, as :class:`FMoEGatedMLP` has them.  Further arguments are those of :class:`FMoETransformerMLP`."""
 
-    def __init__(self, *args, pre_lnorm=False, dropout=0.0, **kwargs):
-        super().__init__(*args, **kwargs)
+    def __init__(self, *args, pre_lnorm=False, dropout=0.0, gated=False, **kwargs):
+        if gated:
+            self._expert_class = _GatedExpert
+        super().__init__(*args, **(_gated_defaults(args, kwargs) if gated else kwargs))
         self.layer_norm = nn.LayerNorm(self.d_model)
         self.pre_lnorm = pre_lnorm
         self.dropout = nn.Dropout(dropout)

@@ -39,6 +39,8 @@ extern "C" {
 #define FMOE_ACT_NONE 0
 #define FMOE_ACT_RELU 1
 #define FMOE_ACT_GELU 2 /* exact erf form, torch.nn.GELU() default */
+/* x / (1 + e^-x): gated experts and products in 8 bits only */
+#define FMOE_ACT_SILU 4
 
 const char *fmoe_last_error(void);
 int fmoe_abi_version(void);
@@ -728,6 +730,81 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
                                  const void *segment_table, int64_t rows,
                                  int64_t row_elems, int dtype, int activation,
                                  void *stream);
+
+/* ---- gated experts ----------------------------------------------------------- */
+
+/* Per expert, over its rows:  [g u] = pre = x W1^T + b1,  mid = act(g) * u,
+ * y = mid W2^T + b2.  w1 [E, 2 d_hidden, d_model] (the gate's rows, then the
+ * linear half's), b1 [E, 2 d_hidden] or NULL, w2 [E, d_model, d_hidden], b2
+ * [E, d_model] or NULL; pre [rows, 2 d_hidden] (NULL: not kept), mid
+ * [rows, d_hidden] and y [rows, d_model]; behind the rows that the experts have
+ * y is zero, pre and mid are left as they are.
+ * The rows' segments come from segment_table (of fmoe_segment_table_build for
+ * `rows` rows; 16-bit types of any sizes, FMOE_F32 as fmoe_linear_dev_supported
+ * says and with tensors on 16 bytes), or else from expert_count_host (any sizes).
+ * FMOE_F32 / FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
+ * The workspace (on 16 bytes) belongs to the call until it has run. */
+int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows,
+                                               int64_t d_model, int64_t d_hidden,
+                                               int dtype, int activation, int keep);
+int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
+                           const void *w2, const void *b2, void *pre, void *mid,
+                           void *y, const void *segment_table,
+                           const int64_t *expert_count_host, int64_t n_expert,
+                           int64_t rows, int64_t d_model, int64_t d_hidden,
+                           int dtype, int activation, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/* The block's gradients from the pre and mid that its forward left; grad_x,
+ * grad_w1 (with grad_b1 or without) and grad_w2 (with grad_b2 or without) may
+ * be NULL: not wanted.  Experts without rows get zeros, and so do rows of grad_x
+ * behind the experts'. */
+int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows,
+                                                int64_t d_model, int64_t d_hidden,
+                                                int dtype, int activation);
+int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1,
+                            const void *w2, const void *pre, const void *mid,
+                            void *grad_x, void *grad_w1, void *grad_b1,
+                            void *grad_w2, void *grad_b2, const void *segment_table,
+                            const int64_t *expert_count_host, int64_t n_expert,
+                            int64_t rows, int64_t d_model, int64_t d_hidden,
+                            int dtype, int activation, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
+/* ---- experts in 8-bit integers ------------------------------------------------ */
+
+/* q[r] = x[i] / scale[r] to the nearest integer (ties to even, of the exact
+ * quotient), scale[r] = max|x[i]| / 127 rounded to float32, at least 2^-126; a
+ * row with an infinity or a NaN: scale NaN, zeros.  i = r, or
+ * row_index[r] / index_div where row_index is not NULL (outside [0, x_rows): a
+ * row of zeros).  x: rows of row_elems adjacent elements, ldx elements apart.
+ * q: rows ldq bytes apart (a multiple of 16), on 16 bytes, zeros from row_elems
+ * up to the next multiple of 16; scale [rows] float32.  segment_table
+ * (optional): only the rows that its counts add up to are made, and rows of
+ * tail_bytes bytes behind them in tail (optional: the result that a product of
+ * these rows leaves as it is there) become zeros.
+ * FMOE_F32 / FMOE_BF16 / FMOE_F16. */
+int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
+                       int64_t index_div, int64_t x_rows, void *q, int64_t ldq,
+                       void *scale, const void *segment_table, void *tail,
+                       int64_t tail_bytes, int64_t rows, int64_t row_elems,
+                       int dtype, void *stream);
+
+/* y[r, c] = act(x_scale[r] w_scale[c] sum_k x[r, k] w[c, k] + bias[c]) per
+ * expert over its rows; gated: act(that of row c) * (that of row out_feat + c).
+ * x: rows of 8-bit integers as fmoe_quantize_rows leaves them, ldx bytes apart.
+ * w: per expert out_feat (gated: 2 out_feat) rows of in_feat integers, ldw bytes
+ * apart, experts w_expert_stride bytes apart, all multiples of 16, on 16 bytes;
+ * a row can be read up to the next multiple of 16 bytes.  w_scale [E, rows of w]
+ * float32, bias the same of y's type or NULL, y [rows_cap, out_feat] of dtype
+ * (rows behind the experts' are left as they are).  The sums are exact; in_feat
+ * is at most 131072, an expert's weights less than 2 GiB. */
+int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w,
+                     int64_t ldw, int64_t w_expert_stride, const void *w_scale,
+                     const void *bias, void *y, const void *segment_table,
+                     int64_t n_expert, int64_t rows_cap, int64_t in_feat,
+                     int64_t out_feat, int gated, int activation, int dtype,
+                     void *stream);
 
 /* ---- a whole layer pass in one call ------------------------------------- */
 
