@@ -108,7 +108,8 @@ SIGNATURES = {
     "fmoe_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int]),
     "fmoe_gated_mlp_backward": (_int, [_vp] * 13 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
     "fmoe_quantize_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
-    "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp]),
+    "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp, _i64, _vp]),
+    "fmoe_linear_int8_workspace_bytes": (_i64, [_i64]),
     "fmoe_layer_sizes": (_int, [_i64, _i64, _i64, _i64, _i64, _int, _int, _int, _int, _vp]),
     "fmoe_layer_forward": (_int, [_vp] * 17 + [_i64] * 5 + [_int] * 4 + [_vp, _i64, _vp]),
     "fmoe_layer_backward": (_int, [_vp] * 21 + [_i64] * 5 + [_int] * 3 + [_vp, _i64, _vp]),

@@ -33,6 +33,7 @@ PLAIN_UNITS = ["error.cpp", "profile.cpp", "routing.hip", "segment_table.hip", "
                "layer_norm.hip", "balance_loss.hip", "act_checkpoint.hip", "gated_mlp.hip", "quantize_rows.hip", "gemm_int8.hip"]
 GEMM_TYPES = {0: "f32", 1: "bf16", 2: "f16"}
 GEMM_PRODUCTS = {0: "fwd", 1: "dgrad", 2: "wgrad"}
+RING_PRODUCTS = {**GEMM_PRODUCTS, 3: "gated", 4: "dgated", 5: "int8"}
 
 
 def _units():
@@ -44,6 +45,8 @@ def _units():
         for p, pname in GEMM_PRODUCTS.items():
             units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",
                           [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))
+    for t, tname in GEMM_TYPES.items():
+        for p, pname in RING_PRODUCTS.items():
             if tname != "f32":
                 units.append(("gemm_ring_inst.hip", f"gemm_ring_{tname}_{pname}.o",
                               [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))

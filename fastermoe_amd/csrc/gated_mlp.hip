@@ -231,6 +231,11 @@ extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void 
         return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need.total());
     char *ws = (char *)workspace;
     const Products p = products(s, segment_table, expert_count_host, ws + need.first, need.split, stream);
+    const GatedArgs fused{x, w1, b1, pre, mid, y, d_model, d_hidden, n_expert, rows, dtype, activation, p.table, p.ws, p.ws_bytes};
+    if (gated_forward_fused(fused)) {
+        if (int rc = grouped_gated_forward(fused, p.stream)) return rc;
+        return p.forward(mid, w2, b2, y, d_hidden, d_model);
+    }
     void *between = pre ? pre : ws;
     if (int rc = p.forward(x, w1, b1, between, d_model, 2 * d_hidden)) return rc;
     if (int rc = gated_act_forward(between, mid, Between{p.table, p.total, d_hidden, dtype, activation, y, rows, d_model, p.stream})) return rc;
@@ -260,7 +265,11 @@ extern "C" int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const 
     char *ws = (char *)workspace;
     const Products p = products(s, segment_table, expert_count_host, ws + need.first + need.second, need.split, stream);
     void *grad_pre = ws, *grad_mid = ws + need.first;
-    if (rows > 0 && (grad_x || grad_w1)) {
+    const GatedArgs fused{grad_y, w2, nullptr, const_cast<void *>(pre), grad_pre, grad_x, d_model, d_hidden, n_expert, rows, dtype, activation, p.table,
+                          p.ws, p.ws_bytes};
+    if (rows > 0 && (grad_x || grad_w1) && gated_dgrad_fused(fused)) {
+        if (int rc = grouped_gated_dgrad(fused, p.stream)) return rc;
+    } else if (rows > 0 && (grad_x || grad_w1)) {
         if (int rc = p.dgrad(grad_y, w2, grad_mid, d_hidden, d_model)) return rc;
         if (int rc = gated_act_backward(grad_mid, pre, grad_pre, Between{p.table, p.total, d_hidden, dtype, activation, grad_x, rows, d_model, p.stream}))
             return rc;

@@ -35,5 +35,8 @@ template <bool kNarrow> __device__ __forceinline__ ActTerms gate_terms(float x, 
     return ActTerms{x, 1.f};
 }
 template <bool kNarrow> __device__ __forceinline__ float gate_act(float x, int act) { return gate_terms<kNarrow>(x, act).value; }
+// ReLU (floor 0) or none (minus infinity), which of them known when the kernel runs
+struct ReluOrNone { float floor; };
+template <bool kNarrow> __device__ __forceinline__ float gate_act(float x, ReluOrNone act) { return x < act.floor ? act.floor : x; }
 
 }  // namespace fmoe

@@ -168,7 +168,8 @@ using namespace fmoe;
 
 extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w, int64_t ldw, int64_t w_expert_stride,
                                 const void *w_scale, const void *bias, void *y, const void *segment_table, int64_t n_expert, int64_t rows_cap,
-                                int64_t in_feat, int64_t out_feat, int gated, int activation, int dtype, void *stream) {
+                                int64_t in_feat, int64_t out_feat, int gated, int activation, int dtype, void *workspace, int64_t workspace_bytes,
+                                void *stream) {
     const char *who = "fmoe_linear_int8";
     FMOE_REQUIRE(dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who, dtype);
     FMOE_REQUIRE(is_gate_activation(activation), "%s: unknown activation %d", who, activation);
@@ -188,6 +189,11 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     prm.bias = bias; prm.y = y; prm.ldx = ldx; prm.ldw = ldw; prm.w_expert_stride = w_expert_stride;
     prm.n_cols = (int)out_feat; prm.k_extent = (int)whole; prm.gated = gated != 0; prm.activation = activation;
     prm.dev_tab = (const int32_t *)segment_table; prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.dtype = dtype;
+    if (int8_ring_takes(prm)) return launch_int8_ring(prm, workspace, workspace_bytes, (hipStream_t)stream);
     if (dtype == FMOE_F32) return launch<float>(prm, (hipStream_t)stream);
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, (hipStream_t)stream) : launch<_Float16>(prm, (hipStream_t)stream);
+}
+
+extern "C" int64_t fmoe_linear_int8_workspace_bytes(int64_t in_feat) {
+    return in_feat < 1 || in_feat > 131072 ? 0 : int8_ring_workspace_bytes(ceil_div(in_feat, 16) * 16);
 }

@@ -20,4 +20,9 @@ struct Int8Params {
     int32_t tiles_n, map_off;     // set by the launch
 };
 
+// The persistent kernel (gemm_ring.hpp): whether it takes a product, its workspace (not needed, but used to share a last round's tiles), the launch.
+bool int8_ring_takes(const Int8Params &a);
+int64_t int8_ring_workspace_bytes(int64_t k_extent);
+int launch_int8_ring(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
 }  // namespace fmoe

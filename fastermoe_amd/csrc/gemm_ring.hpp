@@ -20,10 +20,32 @@
 //     rows are filled with zeros outside the stream (ring_fill);
 //   * the bias gradient is one more column of products (a block of ones times the output gradient).
 #pragma once
+#include "gated_terms.hpp"
 #include "gemm_kernel.hpp"
 
 namespace fmoe {
 namespace gemm {
+
+// Two 8-bit integers of a row: to this kernel's loads and LDS images rows of them are rows of 16-bit elements.  OUT: the results' type.
+template <typename OUT> struct Int8Pair { uint16_t both; };
+template <typename T> struct RingElem {
+    typedef T Out;
+    static constexpr bool kInt8 = false;
+    __device__ static __forceinline__ void mma(f32x4 &acc, const u32x4 &p, const u32x4 &q) { Elem<T>::mma(acc, p, q); }
+    __device__ static __forceinline__ f32x4 add(const f32x4 &a, const f32x4 &b) { return a + b; }
+};
+template <typename OUT_T> struct RingElem<Int8Pair<OUT_T>> {   // (the accumulators are 32-bit integers in the same registers)
+    typedef OUT_T Out;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    static constexpr bool kInt8 = true;
+    __device__ static __forceinline__ void mma(f32x4 &acc, const u32x4 &p, const u32x4 &q) {
+        acc = __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, p), __builtin_bit_cast(i32x4, q),
+                                                                             __builtin_bit_cast(i32x4, acc), 0, 0, 0));
+    }
+    __device__ static __forceinline__ f32x4 add(const f32x4 &a, const f32x4 &b) {
+        return __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, a) + __builtin_bit_cast(i32x4, b));
+    }
+};
 
 struct RingParams {
     const void *P;     // column operand
@@ -41,6 +63,13 @@ struct RingParams {
     // ring_ws_tiles() tiles of floats; ws_wgs workgroups run the launch (the number the second kernel plans with).
     float *split_ws;
     int32_t ws_wgs;
+    // Gated products (kEpiGated, kEpiDGated): n_cols are a half's columns, C and aux see there.  Rows of `tail` (tail_elems 16-bit elements each) behind
+    // the table's become zeros, up to tail_rows (null: none).
+    int32_t activation;
+    void *tail;
+    int64_t tail_rows, tail_elems;
+    // 8-bit integers: scale of each row, and of each row of P
+    const float *q_scale, *p_scale;
 };
 
 // A workgroup's work item: a tile, or (partial) a range of a tile's slabs.
@@ -48,6 +77,7 @@ template <typename T> struct RingTile {
     const T *P, *Q;           // at the item's first contraction element
     int64_t c_off;
     int expert, K;            // contraction elements of the item
+    int row0;                 // ragged rows: the tile's first row
     int p_valid, q_valid, n0, m0;
     int first_slab, ws_slot;  // partial items: place in the contraction, and where the accumulators go
     bool partial;
@@ -121,6 +151,10 @@ struct RingShare {
 
 constexpr int kRingThreads = 512, kRingWaves = 8;
 constexpr int kRingTile = 256;
+// Products of two halves of P's rows: a tile has 128 columns of each, a wave 64 and 64 (rows 0 to 63 of its 128 the first half's), so that a lane has
+// both halves of its columns.
+__host__ __device__ constexpr bool ring_halves(int epi) { return epi == kEpiGated || epi == kEpiInt8Gated; }
+__host__ __device__ constexpr int ring_cols(int epi) { return ring_halves(epi) ? kRingTile / 2 : kRingTile; }
 constexpr int kRingSlab = kRingTile * kSlabBytes;   // 32 KiB
 constexpr int kRingPBufs = 3, kRingQBase = kRingPBufs * kRingSlab;
 constexpr int kRingLds = (kRingPBufs + 2) * kRingSlab;
@@ -383,6 +417,278 @@ __device__ __forceinline__ void ring_epilogue(const RingParams &prm, const RingT
 #endif
 }
 
+// f(activation) with the activation as a constant; MERGED: ReLU and none as one
+template <bool MERGED, typename F> __device__ __forceinline__ void ring_by_activation(int activation, F &&f) {
+    // (the comments keep the compiler from computing what all have in common ahead of them, in more registers than there are)
+    if (activation == FMOE_ACT_SILU) {
+        asm volatile("; silu");
+        f(std::integral_constant<int, FMOE_ACT_SILU>{});
+    } else if (activation == FMOE_ACT_GELU) {
+        asm volatile("; gelu");
+        f(std::integral_constant<int, FMOE_ACT_GELU>{});
+    } else if constexpr (MERGED) {
+        asm volatile("; relu or none");
+        f(ReluOrNone{activation == FMOE_ACT_RELU ? 0.f : -INFINITY});
+    } else if (activation == FMOE_ACT_RELU) {
+        asm volatile("; relu");
+        f(std::integral_constant<int, FMOE_ACT_RELU>{});
+    } else {
+        asm volatile("; none");
+        f(std::integral_constant<int, FMOE_ACT_NONE>{});
+    }
+}
+
+// What goes from a wave's registers to memory by way of its 4 KiB of LDS, sixteen rows of CHUNKS 16-byte pieces at a time.
+template <int CHUNKS> struct RingStage {
+    static constexpr int kStores = CHUNKS / 4, kRowsAt = 16 / kStores;   // rows of a store of the wave
+    unsigned char *stg;
+    int lb, hq, io_r, io_c;
+    __device__ __forceinline__ RingStage(unsigned char *stg, int el)
+        : stg(stg), lb(el & 15), hq(el >> 4), io_r(el / CHUNKS), io_c(el % CHUNKS) {}
+    // this lane's four columns of block column x of row lb
+    __device__ __forceinline__ unsigned char *mine(int x) const {
+        return stg + lb * (CHUNKS * 16) + (((2 * x + (hq >> 1)) ^ (lb & (CHUNKS - 1))) << 4) + (hq & 1) * 8;
+    }
+    // the piece that this lane has to do with on the way from or to memory: row row(i), piece io_c
+    __device__ __forceinline__ int row(int i) const { return i * kRowsAt + io_r; }
+    __device__ __forceinline__ u32x4 *piece(int i) const {
+        const int r = row(i);
+        return (u32x4 *)(stg + r * (CHUNKS * 16) + ((io_c ^ (r & (CHUNKS - 1))) << 4));
+    }
+    static __device__ __forceinline__ void sync() {
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+// The forward product of gated experts.  acc[x][y] with x < 4: the gate's columns 64 wn + 16 x + 4 hq + i of the tile's 128, x + 4 the linear half's.
+// aux (AUX): [rows, 2 n_cols], both halves as they are; C [rows, n_cols]: act(gate) * linear, of the sums before they are rounded.
+template <typename T, bool AUX, int NY>
+__device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
+                                                    int lane, int wm, int wn, int y0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr uint32_t kOutOfRange = 0x80000000u;
+    constexpr int kRsrcFlags = 0x00020000;
+    int el = lane;
+    asm volatile("" : "+v"(el));   // (opaque per tile: its addresses would otherwise be kept in registers across the slab loop)
+    const int row0 = 64 * wm + 16 * y0;
+    if constexpr (AUX) {
+        const RingStage<16> st(stg, el);
+        const int col = 64 * wn + (st.io_c & 7) * 8;
+        const uint32_t at = col < tl.p_valid ? (uint32_t)((col + (st.io_c >> 3) * prm.n_cols) * 2) : kOutOfRange;
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc((T *)prm.aux + 2 * tl.c_off - tl.n0, 0, (int)kOutOfRange, kRsrcFlags);
+#pragma unroll
+        for (int y = 0; y < NY; ++y) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                alignas(8) T v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (T)acc[x][y][i];
+                *(u32x2 *)st.mine(x) = *(const u32x2 *)v;
+            }
+            st.sync();
+#pragma unroll
+            for (int i = 0; i < st.kStores; ++i) {
+                const int row = row0 + 16 * y + st.row(i);
+                const uint32_t off = row < tl.q_valid ? (uint32_t)(row * (int)(prm.ldc * 4)) + at : kOutOfRange;
+                __builtin_amdgcn_raw_buffer_store_b128(*st.piece(i), rs, (int)(off | (at & kOutOfRange)), 0, 0);
+            }
+            st.sync();
+        }
+    }
+    const RingStage<8> st(stg, el);
+    const int col = 64 * wn + st.io_c * 8;
+    const uint32_t at = col < tl.p_valid ? (uint32_t)(col * 2) : kOutOfRange;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((T *)prm.C + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
+    ring_by_activation<false>(prm.activation, [&](auto act) {
+#pragma unroll
+        for (int y = 0; y < NY; ++y) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                alignas(8) T v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (T)(gate_act<true>(acc[x][y][i], act) * acc[x + 4][y][i]);
+                *(u32x2 *)st.mine(x) = *(const u32x2 *)v;
+            }
+            st.sync();
+#pragma unroll
+            for (int i = 0; i < st.kStores; ++i) {
+                const int row = row0 + 16 * y + st.row(i);
+                const uint32_t off = row < tl.q_valid ? (uint32_t)(row * (int)(prm.ldc * 2)) + at : kOutOfRange;
+                __builtin_amdgcn_raw_buffer_store_b128(*st.piece(i), rs, (int)(off | (at & kOutOfRange)), 0, 0);
+            }
+            st.sync();
+        }
+    });
+#endif
+}
+
+// The data gradient of a gated experts' second product, turned into those of the first one's two halves: with dm the sums and g, u from aux [rows, 2 n_cols]
+// C [rows, 2 n_cols] = [dm u act'(g), dm act(g)].  ldc: of both.  Sixteen rows of 64 columns at a time, both halves side by side in the wave's LDS, where the
+// results take their places; the next g and u are on their way meanwhile.
+template <typename T, int NY>
+__device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
+                                                     int lane, int wm, int wn, int y0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr uint32_t kOutOfRange = 0x80000000u;
+    constexpr int kRsrcFlags = 0x00020000;
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    const RingStage<8> sg(stg, el), su(stg + 2048, el);
+    const int row0 = 64 * wm + 16 * y0, col = 128 * wn + sg.io_c * 8;
+    const uint32_t half = (uint32_t)(prm.n_cols * 2);
+    const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc((T *)prm.aux + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
+    const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc((T *)prm.C + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
+    // piece i of step n: rows 16 (n / 2) on, columns 64 (n % 2) on (past the end outside the tile)
+    auto offset = [&](int n, int i) -> uint32_t {
+        const int row = row0 + 16 * (n >> 1) + sg.row(i), c = col + 64 * (n & 1);
+        return row < tl.q_valid && c < tl.p_valid ? (uint32_t)(row * (int)(prm.ldc * 2) + c * 2) : kOutOfRange;
+    };
+    u32x4 ahead[2][2];
+    auto request = [&](int n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t at = offset(n, i);
+            ahead[0][i] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)at, 0, 0);
+            ahead[1][i] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)(at + half), 0, 0);
+        }
+    };
+    request(0);
+    ring_by_activation<false>(prm.activation, [&](auto act) {
+#pragma unroll
+        for (int n = 0; n < 2 * NY; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                *sg.piece(i) = ahead[0][i];
+                *su.piece(i) = ahead[1][i];
+            }
+            if (n + 1 < 2 * NY) request(n + 1);
+            sg.sync();
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                alignas(8) T g[4], u[4];
+                *(u32x2 *)g = *(const u32x2 *)sg.mine(x);
+                *(u32x2 *)u = *(const u32x2 *)su.mine(x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float dm = acc[4 * (n & 1) + x][n >> 1][i];
+                    const ActTerms t = gate_terms<true>((float)g[i], act);
+                    g[i] = (T)(dm * (float)u[i] * t.slope);
+                    u[i] = (T)(dm * t.value);
+                }
+                *(u32x2 *)sg.mine(x) = *(const u32x2 *)g;
+                *(u32x2 *)su.mine(x) = *(const u32x2 *)u;
+            }
+            sg.sync();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t at = offset(n, i);
+                __builtin_amdgcn_raw_buffer_store_b128(*sg.piece(i), out, (int)at, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(*su.piece(i), out, (int)(at + half), 0, 0);
+            }
+            sg.sync();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+#endif
+}
+
+// Products in 8-bit integers: C = act(s_r t_c acc + bias), GATED: act(the first half's) * the second half's.  All rows of 32 columns at a time through the
+// wave's LDS, so that the scales and biases of no more columns than that are at hand (with all of them 250 registers were spilled).
+template <typename T, bool GATED, int NY>
+__device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
+                                                   int lane, int wm, int wn, int y0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef typename RingElem<T>::Out Out;
+    static_assert(sizeof(Out) == 2, "results of 16 bits");
+    constexpr uint32_t kOutOfRange = 0x80000000u;
+    constexpr int kRsrcFlags = 0x00020000, X = GATED ? 4 : 8, H = GATED ? 2 : 1;
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    const int lb = el & 15, hq = el >> 4, row0 = 64 * wm + 16 * y0, wave_col = 16 * X * wn;
+    const int io_r = el >> 2, io_c = el & 3;   // a store: sixteen rows of four 16-byte pieces
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((Out *)prm.C + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
+    // scales and biases: past the tile's columns or rows they read as zero
+    const int64_t p0 = (int64_t)tl.expert * prm.bias_expert_stride + tl.n0;
+    const int p_rows = (GATED ? prm.n_cols : 0) + tl.p_valid;
+    const __amdgpu_buffer_rsrc_t scale_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(prm.p_scale + p0), 0, p_rows * 4, kRsrcFlags);
+    const __amdgpu_buffer_rsrc_t bias_rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<Out *>(prm.bias ? (const Out *)prm.bias + p0 : nullptr), 0, prm.bias ? p_rows * 2 : 0, kRsrcFlags);
+    const __amdgpu_buffer_rsrc_t row_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(prm.q_scale + tl.row0), 0, tl.q_valid * 4, kRsrcFlags);
+    struct Columns { u32x4 scale[H][2]; u32x2 bias[H][2]; };
+    auto request = [&](int pair, Columns &c) {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int at = wave_col + 16 * (2 * pair + j) + 4 * hq + h * prm.n_cols;
+                c.scale[h][j] = __builtin_amdgcn_raw_buffer_load_b128(scale_rs, at * 4, 0, 0);
+                c.bias[h][j] = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, at * 2, 0, 0);
+            }
+    };
+    Columns cols[2];
+    uint32_t s[NY];
+#pragma unroll
+    for (int y = 0; y < NY; ++y) s[y] = __builtin_amdgcn_raw_buffer_load_b32(row_rs, (row0 + 16 * y + lb) * 4, 0, 0);
+    request(0, cols[0]);
+    ring_by_activation<true>(prm.activation, [&](auto act) {
+#pragma unroll
+        for (int pair = 0; pair < X / 2; ++pair) {
+            if (pair + 1 < X / 2) request(pair + 1, cols[(pair + 1) & 1]);
+            const Columns &c = cols[pair & 1];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int x = 2 * pair + j;
+                float add[H][4];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    alignas(8) Out b[4];
+                    *(u32x2 *)b = c.bias[h][j];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) add[h][i] = (float)b[i];
+                }
+#pragma unroll
+                for (int y = 0; y < NY; ++y) {
+                    alignas(8) Out v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        auto sum = [&](int h) -> float {
+                            return fmaf((float)(int)__float_as_uint(acc[x + 4 * h][y][i]), __uint_as_float(s[y]) * __uint_as_float(c.scale[h][j][i]), add[h][i]);
+                        };
+                        float r = gate_act<true>(sum(0), act);
+                        if constexpr (GATED) r *= sum(1);
+                        v[i] = (Out)r;
+                    }
+                    *(u32x2 *)(stg + (16 * y + lb) * 64 + (((2 * j + (hq >> 1)) ^ (lb & 3)) << 4) + (hq & 1) * 8) = *(const u32x2 *)v;
+                }
+            }
+            RingStage<8>::sync();
+            const int col = wave_col + 32 * pair + 8 * io_c;
+#pragma unroll
+            for (int y = 0; y < NY; ++y) {
+                const int row = row0 + 16 * y + io_r;
+                const uint32_t off = row < tl.q_valid && col < tl.p_valid ? (uint32_t)(row * (int)(prm.ldc * 2) + col * 2) : kOutOfRange;
+                const u32x4 v = *(const u32x4 *)(stg + (16 * y + io_r) * 64 + ((io_c ^ (io_r & 3)) << 4));
+                __builtin_amdgcn_raw_buffer_store_b128(v, rs, (int)off, 0, 0);
+            }
+            RingStage<8>::sync();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+#endif
+}
+
+// the epilogue of any product
+template <typename T, int EPI, int ACT, bool AUX, bool BIAS_GRAD, int NY>
+__device__ __forceinline__ void ring_finish(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], const f32x4 (&bacc)[BIAS_GRAD ? 4 : 1],
+                                            unsigned char *stg, int lane, int wm, int wn, int y0) {
+    if constexpr (EPI == kEpiGated) ring_epilogue_gated<T, AUX, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
+    else if constexpr (EPI == kEpiDGated) ring_epilogue_dgated<T, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
+    else if constexpr (RingElem<T>::kInt8) ring_epilogue_int8<T, EPI == kEpiInt8Gated, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
+    else ring_epilogue<T, EPI, ACT, AUX, BIAS_GRAD, NY>(prm, tl, acc, bacc, stg, lane, wm, wn, y0);
+}
+
 template <typename T, int PSHAPE, int QSHAPE, int RAGGED, int EPI, int ACT, bool AUX>
 __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const RingParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
@@ -394,7 +700,11 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
     constexpr int NLOAD = 8;                 // 16-byte loads per loading thread, slab and operand
     constexpr uint32_t kOutOfRange = 0x80000000u;
     constexpr int kRsrcFlags = 0x00020000;   // raw buffer, 32-bit data format
-    constexpr bool kForward = RAGGED == kRaggedRows && PSHAPE == kKC;
+    constexpr bool kInt8 = RingElem<T>::kInt8;
+    constexpr bool kForward = RAGGED == kRaggedRows && PSHAPE == kKC && !kInt8;
+    constexpr bool kHalves = ring_halves(EPI);   // two halves of P's rows, n_cols apart
+    constexpr int kCols = ring_cols(EPI);
+    static_assert(!kHalves || PSHAPE == kKC, "halves of rows of the contraction");
     // With both operands [contraction][row] a fragment is two transposing reads, and a phase issues its loads, reads and
     // products in four interleaved quarters (weight gradient, 256 rows per expert: 415 -> 370 us); otherwise a
     // phase's loads go out together ahead of its reads (forward, K = 14336: 1590 -> 1389 us).
@@ -412,6 +722,15 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
     const int lb = lane & 15, hq = lane >> 4;        // row inside an MFMA block, contraction chunk inside a step
     const int wm = wave >> 1, wn = wave & 1;
     const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)smem;
+
+    if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
+        const int live = dtab[segtab::kRows];
+        if (prm.tail != nullptr && live < prm.tail_rows) {
+            const int64_t n = (prm.tail_rows - live) * prm.tail_elems;
+            uint16_t *at = (uint16_t *)prm.tail + live * prm.tail_elems;
+            for (int64_t i = (int64_t)blockIdx.x * kRingThreads + t; i < n; i += (int64_t)gridDim.x * kRingThreads) at[i] = 0;
+        }
+    }
 
     // -- this workgroup's list of items -----------------------------------------------------
     const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, per = gridDim.x >> 3;
@@ -500,12 +819,14 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
         }
         if (RAGGED == kRaggedRows) RingShare(tm_total, prm.tiles_n).coords(xcd, rem, tm_total, prm.tiles_n, mt, nt);
         else ring_tile_coords(rem, prm.tiles_n, tm_total, mt, nt);
-        tl.n0 = nt * kRingTile;
-        tl.p_valid = min(kRingTile, prm.n_cols - tl.n0);
+        tl.n0 = nt * kCols;
+        tl.p_valid = min(kCols, prm.n_cols - tl.n0);
+        tl.row0 = 0;
         if (RAGGED == kRaggedRows) {
             entry = *(DevTab4)(dtab + prm.dev_map_off + 4 * mt);   // {expert, first row, rows}
             const int64_t k0 = (int64_t)tl.first_slab * BKE;
             tl.m0 = 0;
+            tl.row0 = entry[1];
             tl.q_valid = entry[2];
             tl.Q = (const T *)prm.Q + (int64_t)entry[1] * prm.ldq + k0;   // (the row operand is [row][contraction])
             const T *Pe = (const T *)prm.P + (int64_t)entry[0] * prm.p_expert_stride;
@@ -530,6 +851,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
     // resource and read as zero.  The resources move along the contraction from slab to slab.
     const uint32_t p_step = (uint32_t)((PSHAPE == kKC ? 32 : 16) * prm.ldp * 2);
     const uint32_t q_step = (uint32_t)((QSHAPE == kKC ? 32 : 16) * prm.ldq * 2);
+    const uint32_t p_half = kHalves ? (uint32_t)(prm.n_cols * prm.ldp * 2) : 0u;   // (less than 2 GiB: checked by the host)
     // contraction element of a KC chunk of this thread
     const int kc_elem = ((t & 7) ^ swz((t >> 3) & 31)) * CE;
     struct Operand {
@@ -566,7 +888,8 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
         const bool live = r < n_items;   // past the last tile everything reads as zero
         const Tile tl = decode(live ? r : 0);
         ld_left = live ? tl.K : 0;
-        set_operand(PTag{}, ldp_op, tl.P, prm.ldp, live ? tl.p_valid : 0, tl.first_slab * BKE);
+        // (halves: rows past the first half's end are the second half's, and belong to columns that are not stored)
+        set_operand(PTag{}, ldp_op, tl.P, prm.ldp, live ? (kHalves ? prm.n_cols : 0) + tl.p_valid : 0, tl.first_slab * BKE);
         set_operand(QTag{}, ldq_op, tl.Q, prm.ldq, live ? tl.q_valid : 0, tl.first_slab * BKE);
     };
     auto move_operand = [&](auto shape_tag, Operand &op, int64_t ld) {
@@ -588,7 +911,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
     };
     // The pass `it` of the operand's slab into the 32 KiB at lds_off.  go (scalar, only where cond says so): skipped by
     // a branch the compiler does not see, so that the products around it stay one basic block.
-    auto issue = [&](auto shape_tag, Operand &op, uint32_t step, uint32_t lds_off, auto it_tag, auto cond, bool go) {
+    auto issue = [&](auto shape_tag, auto halves_tag, Operand &op, uint32_t step, uint32_t lds_off, auto it_tag, auto cond, bool go) {
         constexpr int SHAPE = decltype(shape_tag)::value, it = decltype(it_tag)::value;
         if (it == 0) {
             // sign bit set where a KC chunk starts past the end of the contraction
@@ -616,13 +939,16 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
                          : "s"(lds_addr), "v"(voff), "s"(rs), "n"(it * 4096)
                          : "memory", "m0", "scc");
         }
-        if (odd) op.run1 += step; else op.run0 += step;
+        // (halves: two passes of one, two of the other, which begins n_cols rows further on)
+        if constexpr (decltype(halves_tag)::value && it % 2 == 1) op.run0 += it % 4 == 1 ? p_half - step : step - p_half;
+        else if (odd) op.run1 += step;
+        else op.run0 += step;
     };
     auto issue_p = [&](int buf, auto it_tag) {
-        issue(PTag{}, ldp_op, p_step, (uint32_t)(buf * kRingSlab), it_tag, std::false_type{}, true);
+        issue(PTag{}, std::integral_constant<bool, kHalves>{}, ldp_op, p_step, (uint32_t)(buf * kRingSlab), it_tag, std::false_type{}, true);
     };
     auto issue_q = [&](int buf, auto it_tag, bool go) {
-        issue(QTag{}, ldq_op, q_step, (uint32_t)(kRingQBase + buf * kRingSlab), it_tag, std::true_type{}, go);
+        issue(QTag{}, std::false_type{}, ldq_op, q_step, (uint32_t)(kRingQBase + buf * kRingSlab), it_tag, std::true_type{}, go);
     };
     auto issue_slab = [&](auto issue_one) {   // the eight passes of one operand
         issue_one(std::integral_constant<int, 0>{});
@@ -689,7 +1015,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
                 load_step(x_tag);
                 read_part(next, x, p_buf, q_buf);
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) Elem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
+                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
                 const int reads = (next & 1) ? kPReads : (x < 2 ? 2 * kQReads : 2 * kPReads);
 #pragma unroll
                 for (int i = 0; i < TJ; ++i) {
@@ -712,7 +1038,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
 #pragma unroll
             for (int x = 0; x < PF; ++x)
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) Elem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
+                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
             const int reads = PF * kPReads + ((next & 1) == 0 ? TJ * kQReads : 0);
 #pragma unroll
             for (int i = 0; i < PF * TJ; ++i) {
@@ -730,10 +1056,12 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
             const bool has = prm.bias != nullptr && tl.first_slab == 0;
             const T *bias = has ? (const T *)prm.bias + (int64_t)tl.expert * prm.bias_expert_stride + tl.n0 : nullptr;
             const __amdgpu_buffer_rsrc_t bias_rs =
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(bias), 0, has ? tl.p_valid * 2 : 0, kRsrcFlags);
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(bias), 0, has ? ((kHalves ? prm.n_cols : 0) + tl.p_valid) * 2 : 0, kRsrcFlags);
 #pragma unroll
-            for (int x = 0; x < TI; ++x)
-                bias_raw[x] = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, (wn * 128 + x * MB + hq * 4) * 2, 0, 0);
+            for (int x = 0; x < TI; ++x) {
+                const int col = kHalves ? wn * 64 + (x & 3) * MB + (x < 4 ? 0 : prm.n_cols) : wn * 128 + x * MB;
+                bias_raw[x] = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, (col + hq * 4) * 2, 0, 0);
+            }
         }
     };
     auto init_acc = [&]() {
@@ -809,7 +1137,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
                         if constexpr (kWithBiasGrad) {
                             if (want_bias) {
 #pragma unroll
-                                for (int y = 0; y < TJ; ++y) Elem<T>::mma(bacc[y], ones, qf[ks][y]);
+                                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(bacc[y], ones, qf[ks][y]);
                             }
                             __builtin_amdgcn_sched_barrier(0);
                         }
@@ -845,7 +1173,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
 #pragma unroll
                         for (int y = 0; y < TJ; ++y) __builtin_nontemporal_store(acc[x][y], dst + (x * TJ + y) * kRingThreads);
                 } else {
-                    ring_epilogue<T, EPI, ACT, AUX, kWithBiasGrad, TJ>(prm, tile, acc, bacc, smem + stage + wave * 4096, lane, wm, wn, 0);
+                    ring_finish<T, EPI, ACT, AUX, kWithBiasGrad, TJ>(prm, tile, acc, bacc, smem + stage + wave * 4096, lane, wm, wn, 0);
                 }
             } else {
                 for (int left = n_slabs; left > 0; --left) {
@@ -901,8 +1229,9 @@ __global__ __launch_bounds__(64) void ring_combine_kernel(const RingParams prm) 
     int mt, nt;
     share.coords(xcd, plan.full * per + tail_tile, tm_total, prm.tiles_n, mt, nt);
     const ring_i32x4 entry = *(DevTab4)(dtab + prm.dev_map_off + 4 * mt);
-    tl.n0 = nt * kRingTile;
-    tl.p_valid = min(kRingTile, prm.n_cols - tl.n0);
+    tl.n0 = nt * ring_cols(EPI);
+    tl.p_valid = min(ring_cols(EPI), prm.n_cols - tl.n0);
+    tl.row0 = entry[1];
     tl.q_valid = entry[2];
     tl.expert = entry[0];
     tl.c_off = (int64_t)entry[1] * prm.ldc + tl.n0;
@@ -925,12 +1254,12 @@ __global__ __launch_bounds__(64) void ring_combine_kernel(const RingParams prm) 
         for (int b = 0; b < kBatch; ++b)
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                if (b == 0) acc[x][0] = j0 == first ? v[0][x] : acc[x][0] + v[0][x];
-                else if (j0 + b <= last) acc[x][0] += v[b][x];
+                if (b == 0) acc[x][0] = j0 == first ? v[0][x] : RingElem<T>::add(acc[x][0], v[0][x]);
+                else if (j0 + b <= last) acc[x][0] = RingElem<T>::add(acc[x][0], v[b][x]);
             }
     }
     const f32x4 none[1] = {};
-    ring_epilogue<T, EPI, ACT, AUX, false, 1>(prm, tl, acc, none, stage, threadIdx.x, wave >> 1, wave & 1, y);
+    ring_finish<T, EPI, ACT, AUX, false, 1>(prm, tl, acc, none, stage, threadIdx.x, wave >> 1, wave & 1, y);
 #endif
 }
 
@@ -974,5 +1303,11 @@ FMOE_DECLARE_RING(launch_ring_bf16_wgrad);
 FMOE_DECLARE_RING(launch_ring_f16_fwd);
 FMOE_DECLARE_RING(launch_ring_f16_dgrad);
 FMOE_DECLARE_RING(launch_ring_f16_wgrad);
+FMOE_DECLARE_RING(launch_ring_bf16_gated);
+FMOE_DECLARE_RING(launch_ring_f16_gated);
+FMOE_DECLARE_RING(launch_ring_bf16_dgated);
+FMOE_DECLARE_RING(launch_ring_f16_dgated);
+FMOE_DECLARE_RING(launch_ring_bf16_int8);
+FMOE_DECLARE_RING(launch_ring_f16_int8);
 
 }  // namespace fmoe

@@ -16,6 +16,7 @@
 // kernel itself (tiling, LDS layouts, software pipeline, epilogues) is in
 // gemm_kernel.hpp and is instantiated once per element type and product by
 // gemm_inst.hip.
+#include "gemm_int8.hpp"
 #include "gemm_ring.hpp"
 #include "gemm_skinny.hpp"
 #include "profile.hpp"
@@ -761,6 +762,73 @@ int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts, int64_
     if (a.gb && !fast && !is_16bit(a.dtype))
         return grouped_bias_grad(a.gy, a.gb, a.out_feat, a.dtype, counts, n_expert, row_lo, row_hi, last_chunk, stream);
     return FMOE_OK;
+}
+
+// Where the two products together are at least as large as the persistent kernel wants them; its loads reach 2 GiB from a tile's first row of weights.
+bool gated_forward_fused(const GatedArgs &a) {
+    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
+           use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype), a.dtype) && 2 * a.h * a.d * 2 < ((int64_t)1 << 31) && a.h * 4 <= (1 << 22);
+}
+bool gated_dgrad_fused(const GatedArgs &a) {
+    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.pre, a.out}, {a.d, a.h}) &&
+           use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, a.h, a.d, a.dtype), a.dtype) && a.h * 4 <= (1 << 22);
+}
+namespace {
+int ring_of_table(RingParams &prm, const GatedArgs &a, int cols) {
+    prm.n_expert = (int32_t)a.n_expert;
+    prm.tiles_n = (int)ceil_div(prm.n_cols, cols);
+    prm.dev_tab = a.dev_tab;
+    prm.dev_map_off = (int32_t)segtab::map256_off(a.n_expert);
+    const int64_t order = segtab::order_off(a.rows_cap, a.n_expert), tiles = segtab::cap_tiles(a.rows_cap, a.n_expert, kRingTile) * prm.tiles_n;
+    if (order + 4 * a.n_expert > (int64_t)INT32_MAX || tiles > (int64_t)INT32_MAX - 65536)
+        return fail(FMOE_ELIMIT, "grouped GEMM: %lld tiles exceed the supported range", (long long)tiles);
+    prm.dev_order_off = (int32_t)order;
+    prm.split_ws = route_workspace({DevKernel::kRing, kManyTiles}, a.d, a.dtype, a.workspace, a.workspace_bytes);
+    prm.activation = a.activation;
+    prm.tail = a.tail; prm.tail_rows = a.rows_cap; prm.tail_elems = a.d;
+    return FMOE_OK;
+}
+}  // namespace
+int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
+    RingParams prm{};
+    prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.bias = a.bias; prm.aux = a.pre;
+    prm.ldp = a.d; prm.ldq = a.d; prm.ldc = a.h;
+    prm.p_expert_stride = 2 * a.h * a.d; prm.bias_expert_stride = 2 * a.h;
+    prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+    if (int rc = ring_of_table(prm, a, ring_cols(kEpiGated))) return rc;
+    ProfileScope prof(kProfGemmFwd, 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
+    return a.dtype == FMOE_BF16 ? launch_ring_bf16_gated(prm, kEpiGated, a.activation, stream) : launch_ring_f16_gated(prm, kEpiGated, a.activation, stream);
+}
+int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
+    RingParams prm{};
+    prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.aux = a.pre;
+    prm.ldp = a.h; prm.ldq = a.d; prm.ldc = 2 * a.h;
+    prm.p_expert_stride = a.h * a.d;
+    prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+    if (int rc = ring_of_table(prm, a, ring_cols(kEpiDGated))) return rc;
+    ProfileScope prof(kProfGemmDgrad, 2.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
+    return a.dtype == FMOE_BF16 ? launch_ring_bf16_dgated(prm, kEpiDGated, a.activation, stream) : launch_ring_f16_dgated(prm, kEpiDGated, a.activation, stream);
+}
+
+// The experts' product in 8-bit integers on the persistent kernel: results of 16 bits in rows of whole 16-byte pieces, where there are enough tiles for it.
+bool int8_ring_takes(const Int8Params &a) {
+    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && aligned16(a.y) && (a.bias == nullptr || aligned16(a.bias)) && aligned16(a.w_scale) &&
+           a.ldw <= (1 << 22) && use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.k_extent / 2, a.dtype), a.dtype);
+}
+int64_t int8_ring_workspace_bytes(int64_t k_extent) { return route_workspace_bytes({DevKernel::kRing, kManyTiles}, k_extent / 2, FMOE_BF16); }
+int launch_int8_ring(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    RingParams prm{};
+    prm.P = a.w; prm.Q = a.x; prm.C = a.y; prm.bias = a.bias; prm.q_scale = a.x_scale; prm.p_scale = a.w_scale;
+    prm.ldp = a.ldw / 2; prm.ldq = a.ldx / 2; prm.ldc = a.n_cols;   // (pairs of integers)
+    prm.p_expert_stride = a.w_expert_stride / 2; prm.bias_expert_stride = (a.gated ? 2 : 1) * (int64_t)a.n_cols;
+    prm.n_cols = a.n_cols; prm.k_extent = a.k_extent / 2;
+    const int epi = a.gated ? kEpiInt8Gated : kEpiInt8;
+    GatedArgs g{};
+    g.d = prm.k_extent; g.n_expert = a.n_expert; g.rows_cap = a.rows_cap; g.dtype = a.dtype; g.activation = a.activation; g.dev_tab = a.dev_tab;
+    g.workspace = workspace; g.workspace_bytes = workspace_bytes;
+    if (int rc = ring_of_table(prm, g, ring_cols(epi))) return rc;
+    ProfileScope prof(kProfGemmFwd, 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)prm.bias_expert_stride, stream);
+    return a.dtype == FMOE_BF16 ? launch_ring_bf16_int8(prm, epi, a.activation, stream) : launch_ring_f16_int8(prm, epi, a.activation, stream);
 }
 
 int grouped_bias_grad(const void *gy, void *gb, int64_t out_feat, int dtype, const int64_t *counts,

@@ -10,6 +10,11 @@ enum Epilogue {
     kEpiStore = 0,    // C = acc (+ bias[col])
     kEpiBiasAct = 1,  // pre = acc + bias[col]; aux = pre (if aux); C = act(pre)
     kEpiDAct = 2,     // C = acc * act'(aux)          (aux = saved pre-activation)
+    // persistent kernel only:
+    kEpiGated = 3,    // [g u] = acc + bias; aux = [g u] (if aux); C = act(g) u
+    kEpiDGated = 4,   // C = [acc u act'(g), acc act(g)]  (aux = saved [g u])
+    kEpiInt8 = 5,     // C = act(row scale * column scale * acc + bias)
+    kEpiInt8Gated = 6,  // [g u] = that before act; C = act(g) u
 };
 
 constexpr int kMaxGroupExperts = 256;  // experts per launch (table lives in kernel arguments)
@@ -137,6 +142,26 @@ int grouped_linear_dgrad(const LinearDgradArgs &a, const int64_t *counts_host, i
 // earlier chunk left (cuda/fused_compute.cuh:123, beta_weight).
 int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts_host, int64_t n_expert,
                          int64_t row_lo, int64_t row_hi, bool last_chunk, hipStream_t stream);
+// Gated experts' products with the work between them in their epilogues (see gated_mlp.hip), over a table in device memory.  False where the sizes or types go
+// another way (grouped_linear_forward / _dgrad and a kernel between).  `tail`: rows of d elements behind the table's that become zeros.
+struct GatedArgs {
+    const void *in;      // forward: x [rows, d]; dgrad: the gradient of the second product's results, [rows, d]
+    const void *w;       // forward: [E, 2 h, d]; dgrad: [E, d, h]
+    const void *bias;    // forward: [E, 2 h] or null
+    void *pre;           // [rows, 2 h]; forward: written (null: not kept), dgrad: read
+    void *out;           // forward: [rows, h]; dgrad: [rows, 2 h]
+    void *tail;
+    int64_t d, h, n_expert, rows_cap;
+    int dtype, activation;
+    const int32_t *dev_tab;
+    void *workspace;     // for the split of a last round of tiles, as LinearForwardArgs::dev_workspace
+    int64_t workspace_bytes;
+};
+bool gated_forward_fused(const GatedArgs &a);
+int grouped_gated_forward(const GatedArgs &a, hipStream_t stream);
+bool gated_dgrad_fused(const GatedArgs &a);
+int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream);
+
 // grad_b[e, c] = column sums of gy over the rows of expert e; same chunk rules.
 int grouped_bias_grad(const void *gy, void *gb, int64_t out_feat, int dtype, const int64_t *counts_host,
                       int64_t n_expert, int64_t row_lo, int64_t row_hi, bool last_chunk, hipStream_t stream);

@@ -1059,9 +1059,12 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
     _exact_table(table, e, n, x.device)
     y = torch.empty(n, out, dtype=x.dtype, device=x.device)
     q, scale = quantize_rows(x, row_index, index_div, table, y)
+    lib = _lib.load()
     with _on(x.device):
-        check(_lib.load().fmoe_linear_int8(_ptr(q), q.stride(0), _ptr(scale), _ptr(weight), by_row, by_expert, _ptr(weight_scale), _ptr(bias), _ptr(y),
-                                           _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _stream(x)))
+        ws = _dev_workspace(lib.fmoe_linear_int8_workspace_bytes(d), x.device)
+        check(lib.fmoe_linear_int8(_ptr(q), q.stride(0), _ptr(scale), _ptr(weight), by_row, by_expert, _ptr(weight_scale), _ptr(bias), _ptr(y),
+                                   _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel(),
+                                   _stream(x)))
     return y
 
 

@@ -798,13 +798,17 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
  * a row can be read up to the next multiple of 16 bytes.  w_scale [E, rows of w]
  * float32, bias the same of y's type or NULL, y [rows_cap, out_feat] of dtype
  * (rows behind the experts' are left as they are).  The sums are exact; in_feat
- * is at most 131072, an expert's weights less than 2 GiB. */
+ * is at most 131072, an expert's weights less than 2 GiB.  With a workspace (on
+ * 16 bytes; none: NULL) of fmoe_linear_int8_workspace_bytes a last round of tiles
+ * that fills a small part of the chip is shared along the contraction; the
+ * results are the same bits. */
+int64_t fmoe_linear_int8_workspace_bytes(int64_t in_feat);
 int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w,
                      int64_t ldw, int64_t w_expert_stride, const void *w_scale,
                      const void *bias, void *y, const void *segment_table,
                      int64_t n_expert, int64_t rows_cap, int64_t in_feat,
                      int64_t out_feat, int gated, int activation, int dtype,
-                     void *stream);
+                     void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ---- a whole layer pass in one call ------------------------------------- */
 
