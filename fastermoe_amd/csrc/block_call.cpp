@@ -5,19 +5,11 @@
 // Python, the kernels of a small batch 5.  What a call takes is decided here; None sends it the way through Python, which says what is wrong with its tensors.
 #include "block_call.hpp"
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
+#include "call_tools.hpp"
 
-#include <array>
 #include <cmath>
-#include <cstdint>
-#include <optional>
 
-#include "../../include/fmoe_hip.h"
+using namespace fmoe_call;
 
 namespace {
 
@@ -37,24 +29,10 @@ struct Entries {
     decltype(&fmoe_act_checkpoint_backward) checkpoint_backward;
 } entry = {};
 
-int dtype_code(const at::Tensor &t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return FMOE_F32;
-        case at::kBFloat16: return FMOE_BF16;
-        case at::kHalf: return FMOE_F16;
-        default: return -1;
-    }
-}
-void *pointer(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 float *floats(const at::Tensor &t) { return (float *)pointer(t); }
-void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void ok(int rc) { TORCH_CHECK(rc == FMOE_OK, "libfmoe_hip error ", rc, ": ", entry.last_error()); }
-at::Tensor same(const at::Tensor &t) { return at::empty(t.sizes(), t.options()); }
 // rows of adjacent elements, as the kernels read them
 at::Tensor as_rows(const at::Tensor &t) { return t.size(1) > 1 && t.stride(1) != 1 ? t.contiguous() : t; }
-
-using Maybe = std::optional<at::Tensor>;   // (what a node takes where there may be no tensor)
-Maybe maybe(const at::Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &given, const Maybe &of_residual, const Maybe &of_weight,
@@ -170,35 +148,6 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     }
 };
 
-// The interpreter's lock, given back while this lives: an allocation may wait for the device, a launch for a full queue
-struct WithoutLock {
-    PyThreadState *state = PyEval_SaveThread();
-    ~WithoutLock() { PyEval_RestoreThread(state); }
-};
-
-// The first N arguments as tensors (undefined for None); false, with an exception set, where one is neither
-template <size_t N> bool tensors(PyObject *const *args, std::array<at::Tensor, N> &t) {
-    for (size_t i = 0; i < N; ++i) {
-        if (args[i] == Py_None) continue;
-        if (!THPVariable_Check(args[i])) {
-            PyErr_SetString(PyExc_TypeError, "tensors or None");
-            return false;
-        }
-        t[i] = THPVariable_Unpack(args[i]);
-    }
-    return true;
-}
-// The number behind them; false, with an exception set, where it is none
-bool number(PyObject *arg, long &n) {
-    n = PyLong_AsLong(arg);
-    return n != -1 || !PyErr_Occurred();
-}
-// (a tensor without memory of its own, as some wrappers are, has a null pointer, which a parameter that is left out has too)
-bool on_gpu(const at::Tensor &t) {
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg() && t.has_storage() &&
-           (t.numel() == 0 || t.storage().data() != nullptr);
-}
-
 }  // namespace
 
 PyObject *fmoe_block_bind(PyObject *, PyObject *args) {
@@ -289,11 +238,6 @@ bool keeps(const at::Tensor &x, long activation) {
 bool no_or_table(const at::Tensor &t, const at::Tensor &x) {
     return !t.defined() || (on_gpu(t) && t.device() == x.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= 8);
 }
-PyObject *wrap_or_none(at::Tensor t) {
-    if (t.defined()) return THPVariable_Wrap(std::move(t));
-    Py_RETURN_NONE;
-}
-
 }  // namespace
 
 // act_checkpoint_forward(x, table, activation, with_act, with_held): (y or None, held, scale or None, None); None where the call does not take these tensors

@@ -194,6 +194,10 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, (hipStream_t)stream) : launch<_Float16>(prm, (hipStream_t)stream);
 }
 
-extern "C" int64_t fmoe_linear_int8_workspace_bytes(int64_t in_feat) {
-    return in_feat < 1 || in_feat > 131072 ? 0 : int8_ring_workspace_bytes(ceil_div(in_feat, 16) * 16);
+extern "C" int64_t fmoe_linear_int8_workspace_bytes(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat, int gated, int dtype) {
+    if (n_expert < 1 || rows_cap < 1 || in_feat < 1 || in_feat > 131072 || out_feat < 1 || out_feat > (1 << 28)) return 0;
+    Int8Params prm{};
+    prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.n_cols = (int)out_feat; prm.k_extent = (int)(ceil_div(in_feat, 16) * 16);
+    prm.gated = gated != 0; prm.dtype = dtype;
+    return int8_ring_takes(prm) ? int8_ring_workspace_bytes(prm.k_extent) : 0;
 }

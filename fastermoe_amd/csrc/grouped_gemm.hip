@@ -773,6 +773,7 @@ bool gated_dgrad_fused(const GatedArgs &a) {
     return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.pre, a.out}, {a.d, a.h}) &&
            use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, a.h, a.d, a.dtype), a.dtype) && a.h * 4 <= (1 << 22);
 }
+int64_t gated_workspace_bytes(int64_t contraction, int dtype) { return route_workspace_bytes({DevKernel::kRing, kManyTiles}, contraction, dtype); }
 namespace {
 int ring_of_table(RingParams &prm, const GatedArgs &a, int cols) {
     prm.n_expert = (int32_t)a.n_expert;

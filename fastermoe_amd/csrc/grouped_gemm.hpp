@@ -157,7 +157,8 @@ struct GatedArgs {
     void *workspace;     // for the split of a last round of tiles, as LinearForwardArgs::dev_workspace
     int64_t workspace_bytes;
 };
-bool gated_forward_fused(const GatedArgs &a);
+bool gated_forward_fused(const GatedArgs &a);   // (sizes alone where the tensors are null)
+int64_t gated_workspace_bytes(int64_t contraction, int dtype);
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream);
 bool gated_dgrad_fused(const GatedArgs &a);
 int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream);

@@ -120,6 +120,9 @@ PyMethodDef methods[] = {
     {"balance_loss", fast(fmoe_block_balance_loss), METH_FASTCALL, "A gate's balance loss."},
     {"act_checkpoint_forward", fast(fmoe_block_checkpoint_forward), METH_FASTCALL, "Rows in 8 bits, and their activation."},
     {"act_checkpoint_backward", fast(fmoe_block_checkpoint_backward), METH_FASTCALL, "The backward from rows in 8 bits."},
+    {"bind_expert", fmoe_expert_bind, METH_VARARGS, "The addresses of the library's entry points that the next ones call."},
+    {"gated_mlp", fast(fmoe_expert_gated_mlp), METH_FASTCALL, "Gated experts."},
+    {"linear_int8", fast(fmoe_expert_linear_int8), METH_FASTCALL, "The experts' product in 8-bit integers."},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_layer_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -896,6 +896,10 @@ def _exact_table(table, n_expert, rows, device):
     return table
 
 
+def _all_aligned(*tensors):
+    return all(t is None or t.data_ptr() % 16 == 0 for t in tensors)
+
+
 def _gated_args(x, w1, b1, w2, b2):
     """Checks of a gated block's tensors; the code of their type and ``(experts, rows, d_model, d_hidden)``."""
     dt = _rows("x", x)
@@ -936,7 +940,8 @@ def gated_mlp_forward(x, w1, b1, w2, b2, activation, table=None, expert_count=No
     mid = torch.empty(n, h, dtype=x.dtype, device=x.device)
     lib = _lib.load()
     with _on(x.device):
-        ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep)), x.device)
+        ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep),
+                                                                       int(table is not None and _all_aligned(x, w1, b1, w2, b2))), x.device)
         check(lib.fmoe_gated_mlp_forward(_ptr(x), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(pre), _ptr(mid), _ptr(y), seg, cnt, e, n, d, h, dt,
                                          activation, _ptr(ws), ws.numel(), _stream(x)))
     return y, pre, mid if keep else None
@@ -958,7 +963,8 @@ def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table=None, expe
     grad_w2, grad_b2 = new(want_w2 or want_b2, e, d, h), new(want_b2, e, d)
     lib = _lib.load()
     with _on(x.device):
-        ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation), x.device)
+        ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation,
+                                                                        int(table is not None and _all_aligned(grad_y, x, w1, w2, pre, mid))), x.device)
         check(lib.fmoe_gated_mlp_backward(_ptr(grad_y), _ptr(x), _ptr(w1), _ptr(w2), _ptr(pre), _ptr(mid), _ptr(grad_x), _ptr(grad_w1), _ptr(grad_b1),
                                           _ptr(grad_w2), _ptr(grad_b2), seg, cnt, e, n, d, h, dt, activation, _ptr(ws), ws.numel(), _stream(x)))
     return grad_x, grad_w1 if want_w1 else None, grad_b1, grad_w2 if want_w2 else None, grad_b2
@@ -1043,6 +1049,11 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
         raise ValueError(f"x must be a CUDA (HIP) tensor, got device {x.device}")
     if x.dim() != 2:
         raise ValueError(f"x must be 2-D [rows, features], got shape {tuple(x.shape)}")
+    module = _lib.load_layer_call()
+    if module is not None:
+        y = module.linear_int8(x, weight, weight_scale, bias, table, row_index, int(index_div), int(activation), int(bool(gated)))
+        if y is not None:
+            return y
     weight, by_expert, by_row, weight_scale = _int8_weights(weight, weight_scale, x.device)
     activation = _gate_activation(activation)
     e, out, d = weight.shape
@@ -1061,7 +1072,7 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
     q, scale = quantize_rows(x, row_index, index_div, table, y)
     lib = _lib.load()
     with _on(x.device):
-        ws = _dev_workspace(lib.fmoe_linear_int8_workspace_bytes(d), x.device)
+        ws = _dev_workspace(lib.fmoe_linear_int8_workspace_bytes(e, n, d, out, int(gated), _DTYPES[x.dtype]), x.device)
         check(lib.fmoe_linear_int8(_ptr(q), q.stride(0), _ptr(scale), _ptr(weight), by_row, by_expert, _ptr(weight_scale), _ptr(bias), _ptr(y),
                                    _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel(),
                                    _stream(x)))

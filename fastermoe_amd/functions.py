@@ -812,6 +812,14 @@ def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
     zeros, and so do their gradients.  Differentiable once, with respect to ``inp``, the weights and the biases; the gradients are made from ``g``, ``u``
     and ``act(g) * u`` as ``inp``'s type holds them.  (float32 in sizes or from addresses that are no multiple of 16 bytes: the counts are read on the host.)"""
     code = _gate_activation_code(activation)
+    module = _lib.load_layer_call()
+    if module is not None and nothing_watches(*(t for t in (inp, w1, b1, w2, b2, table) if t is not None)):
+        if table is None and isinstance(expert_count, torch.Tensor) and isinstance(w1, torch.Tensor) and w1.dim() == 3 and inp.dim() == 2:
+            table = _segments(expert_count, None, w1.shape[0], inp.shape[0], inp.device)
+        if table is not None:
+            out = module.gated_mlp(inp, w1, b1, w2, b2, table, code)
+            if out is not None:
+                return out
     fmoe_native._gated_args(inp if inp.is_contiguous() else inp.contiguous(), w1, b1, w2, b2)
     counts = None
     if _over_a_table(inp, w1, w2, b1, b2):

@@ -743,10 +743,12 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
  * `rows` rows; 16-bit types of any sizes, FMOE_F32 as fmoe_linear_dev_supported
  * says and with tensors on 16 bytes), or else from expert_count_host (any sizes).
  * FMOE_F32 / FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
- * The workspace (on 16 bytes) belongs to the call until it has run. */
+ * The workspace (on 16 bytes) belongs to the call until it has run.  Its size: keep
+ * not 0 where pre is given, aligned not 0 where all tensors begin on 16 bytes. */
 int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                int64_t d_model, int64_t d_hidden,
-                                               int dtype, int activation, int keep);
+                                               int dtype, int activation, int keep,
+                                               int aligned);
 int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
                            const void *w2, const void *b2, void *pre, void *mid,
                            void *y, const void *segment_table,
@@ -761,7 +763,7 @@ int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
  * behind the experts'. */
 int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                 int64_t d_model, int64_t d_hidden,
-                                                int dtype, int activation);
+                                                int dtype, int activation, int aligned);
 int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1,
                             const void *w2, const void *pre, const void *mid,
                             void *grad_x, void *grad_w1, void *grad_b1,
@@ -802,7 +804,9 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
  * 16 bytes; none: NULL) of fmoe_linear_int8_workspace_bytes a last round of tiles
  * that fills a small part of the chip is shared along the contraction; the
  * results are the same bits. */
-int64_t fmoe_linear_int8_workspace_bytes(int64_t in_feat);
+int64_t fmoe_linear_int8_workspace_bytes(int64_t n_expert, int64_t rows_cap,
+                                         int64_t in_feat, int64_t out_feat, int gated,
+                                         int dtype);
 int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w,
                      int64_t ldw, int64_t w_expert_stride, const void *w_scale,
                      const void *bias, void *y, const void *segment_table,
