@@ -29,7 +29,7 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-
 # extra -D switches for experiments, e.g. FMOE_EXTRA_FLAGS="-DFMOE_X=1"
 FLAGS += os.environ.get("FMOE_EXTRA_FLAGS", "").split()
 
-PLAIN_UNITS = ["error.cpp", "profile.cpp", "routing.hip", "segment_table.hip", "permute.hip", "combine.hip", "gate_grad.hip", "grouped_gemm.hip", "gemm_any.hip", "gemm_unaligned.hip", "gemm_skinny.hip", "pipeline.hip", "layer.hip",
+PLAIN_UNITS = ["error.cpp", "profile.cpp", "routing.hip", "segment_table.hip", "permute.hip", "combine.hip", "gate_grad.hip", "grouped_gemm.hip", "gemm_any.hip", "gemm_unaligned.hip", "pipeline.hip", "layer.hip",
                "layer_norm.hip", "balance_loss.hip", "act_checkpoint.hip", "gated_mlp.hip", "quantize_rows.hip", "gemm_int8.hip"]
 GEMM_TYPES = {0: "f32", 1: "bf16", 2: "f16"}
 GEMM_PRODUCTS = {0: "fwd", 1: "dgrad", 2: "wgrad"}
@@ -41,6 +41,8 @@ def _units():
     for src in PLAIN_UNITS:
         if os.path.exists(os.path.join(CSRC, src)):
             units.append((src, os.path.splitext(src)[0] + ".o", []))
+    for i, name in enumerate(("plain", "gated", "int8")):
+        units.append(("gemm_skinny.hip", f"gemm_skinny_{name}.o", [f"-DFMOE_SKINNY={i}"]))
     for t, tname in GEMM_TYPES.items():
         for p, pname in GEMM_PRODUCTS.items():
             units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",

@@ -192,9 +192,10 @@ struct Products {
         a.dev_rows_cap = table ? rows : 0;
         a.dev_any_grid = true;
     }
-    int forward(const void *x, const void *w, const void *bias, void *y, int64_t in, int64_t out) const {
+    int forward(const void *x, const void *w, const void *bias, void *y, int64_t in, int64_t out, bool once) const {
         LinearForwardArgs a{x, w, bias, y, nullptr, in, out, dtype, kEpiStore, FMOE_ACT_NONE};
         place(a);
+        a.dev_weights_once = once;   // (no backward that reads them again)
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;
         return grouped_linear_forward(a, counts, n_expert, 0, total, stream);
@@ -248,12 +249,12 @@ extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void 
     const GatedArgs fused{x, w1, b1, pre, mid, y, d_model, d_hidden, n_expert, rows, dtype, activation, p.table, p.ws, p.ws_bytes};
     if (gated_forward_fused(fused)) {
         if (int rc = grouped_gated_forward(fused, p.stream)) return rc;
-        return p.forward(mid, w2, b2, y, d_hidden, d_model);
+        return p.forward(mid, w2, b2, y, d_hidden, d_model, pre == nullptr);
     }
     void *between = pre ? pre : ws;
-    if (int rc = p.forward(x, w1, b1, between, d_model, 2 * d_hidden)) return rc;
+    if (int rc = p.forward(x, w1, b1, between, d_model, 2 * d_hidden, pre == nullptr)) return rc;
     if (int rc = gated_act_forward(between, mid, Between{p.table, p.total, d_hidden, dtype, activation, y, rows, d_model, p.stream})) return rc;
-    return p.forward(mid, w2, b2, y, d_hidden, d_model);
+    return p.forward(mid, w2, b2, y, d_hidden, d_model, pre == nullptr);
 }
 
 extern "C" int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,

@@ -189,6 +189,7 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     prm.bias = bias; prm.y = y; prm.ldx = ldx; prm.ldw = ldw; prm.w_expert_stride = w_expert_stride;
     prm.n_cols = (int)out_feat; prm.k_extent = (int)whole; prm.gated = gated != 0; prm.activation = activation;
     prm.dev_tab = (const int32_t *)segment_table; prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.dtype = dtype;
+    if (int8_few_takes(prm)) return launch_int8_few(prm, (hipStream_t)stream);
     if (int8_ring_takes(prm)) return launch_int8_ring(prm, workspace, workspace_bytes, (hipStream_t)stream);
     if (dtype == FMOE_F32) return launch<float>(prm, (hipStream_t)stream);
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, (hipStream_t)stream) : launch<_Float16>(prm, (hipStream_t)stream);

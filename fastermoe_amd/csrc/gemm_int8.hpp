@@ -20,6 +20,9 @@ struct Int8Params {
     int32_t tiles_n, map_off;     // set by the launch
 };
 
+// Few rows per expert (gemm_skinny.hip).
+bool int8_few_takes(const Int8Params &a);
+int launch_int8_few(const Int8Params &a, hipStream_t stream);
 // The persistent kernel (gemm_ring.hpp): whether it takes a product, its workspace (not needed, but used to share a last round's tiles), the launch.
 bool int8_ring_takes(const Int8Params &a);
 int64_t int8_ring_workspace_bytes(int64_t k_extent);

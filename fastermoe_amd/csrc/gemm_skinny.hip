@@ -16,6 +16,10 @@
 //     sum, in the order of the units from there on, does not depend on how many rows other experts have;
 //   * the compiler may not move a unit's loads behind the products of the one before, which left none in flight at their end.
 // Where it is used, and what it measured: use_skinny() in grouped_gemm.hip.
+//
+// Gated products (HALVES): half of a workgroup's blocks of columns are the gate's and the others the same columns of the linear half, so that the wave that adds up a
+// block of the one adds up the other's too.  8-bit integers: see Int8Pair; the sums are integers and exact.
+// The build compiles this file with -DFMOE_SKINNY=<0 plain products|1 gated ones|2 8-bit integers>.
 #include "gemm_skinny.hpp"
 #include "segment_table.hpp"
 
@@ -28,6 +32,10 @@ constexpr int kSkRows = 32;   // rows of a pass
 
 // one 16 x 16 block over 64 bytes of contraction; acc as for the 16 x 16 x 32 form
 template <typename T> __device__ __forceinline__ void mma_step(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<T>::mma(acc, w, x); }
+template <typename T> struct IsInt8 : std::false_type {};
+template <typename OUT> struct IsInt8<Int8Pair<OUT>> : std::true_type {};
+template <> __device__ __forceinline__ void mma_step<Int8Pair<__bf16>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { RingElem<Int8Pair<__bf16>>::mma(acc, w, x); }
+template <> __device__ __forceinline__ void mma_step<Int8Pair<_Float16>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { RingElem<Int8Pair<_Float16>>::mma(acc, w, x); }
 template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u32x4 &w, const u32x4 &x) {
     // product j takes element j of every lane's four: contraction elements j, 4 + j, 8 + j and 12 + j of the step
 #pragma unroll
@@ -47,12 +55,16 @@ __device__ __forceinline__ void pair_to_steps(u32x4 &a, u32x4 &b) {
     }
 }
 
-// COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch)
-template <typename T, int COL_BLOCKS, bool APART>
+// COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch).  HALVES: gated
+template <typename T, int COL_BLOCKS, bool APART, bool HALVES>
 __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_gemm_skinny_kernel(const SkinnyParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
     constexpr int EB = (int)sizeof(T), CE = 16 / EB, kLine = 128 / EB;    // elements per lane's load and per line
     typedef std::conditional_t<sizeof(T) == 2, u32x2, u32x4> Vec4;        // four elements
+    constexpr bool kInt8 = IsInt8<T>::value;
+    typedef typename RingElem<T>::Out Out;                                // of the results
+    constexpr int kCols = COL_BLOCKS * 16 / (HALVES ? 2 : 1);             // columns of a workgroup
+    static_assert(!HALVES || (COL_BLOCKS >= 2 && sizeof(T) == 2), "halves: two blocks of columns or more");
     constexpr uint32_t kOutOfRange = 0x80000000u;
     constexpr int kRsrcFlags = 0x00020000;   // raw buffer, 32-bit data format
     typedef const int32_t __attribute__((address_space(4))) *DevTab;    // read-only, uniform: scalar loads
@@ -62,9 +74,15 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
 
     const DevTab dtab = (DevTab)(uintptr_t)prm.dev_tab;
     int place = __builtin_amdgcn_readfirstlane(blockIdx.x / prm.tiles_n);
-    const int tile_n = blockIdx.x - place * prm.tiles_n, n0 = tile_n * (COL_BLOCKS * 16), K = prm.k_extent;
+    const int tile_n = blockIdx.x - place * prm.tiles_n, n0 = tile_n * kCols, K = prm.k_extent;
     const DevTab4 order = (DevTab4)(dtab + prm.order_off);   // {expert, first row, rows}: of an expert, or (not APART) of a tile of at most 128 rows
     const int live = dtab[APART ? segtab::kLive : segtab::kTiles128];
+    if constexpr (HALVES && !kInt8) {
+        const int64_t there = dtab[segtab::kRows];
+        if (prm.tail != nullptr && there < prm.tail_rows)
+            for (int64_t i = (int64_t)blockIdx.x * kSkThreads + threadIdx.x; i < (prm.tail_rows - there) * prm.tail_elems; i += (int64_t)gridDim.x * kSkThreads)
+                ((uint16_t *)prm.tail)[there * prm.tail_elems + i] = 0;
+    }
     int r0 = 0;   // first row
     i32x4 entry;
     if (APART && place < prm.extra_groups) {
@@ -95,10 +113,14 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     const int chunk = hq | ((lane & 8) >> 1), row8 = lane & 7;
 
     // weights: rows past the last column lie past the end of the resource and read as zero
-    const T *W = (const T *)prm.w + ((int64_t)expert * prm.n_cols + n0) * K;
-    const int w_bytes = min(COL_BLOCKS * 16, prm.n_cols - n0) * K * EB;
+    // (gated: past the last of the gate's columns lie the linear half's)
+    const int ldw = kInt8 ? (int)prm.ldw : K, ldx = kInt8 ? (int)prm.ldx : K;   // elements from row to row
+    const int64_t w_expert = kInt8 ? prm.w_expert_stride : (int64_t)(HALVES ? 2 : 1) * prm.n_cols * K;
+    const T *W = (const T *)prm.w + expert * w_expert + (int64_t)n0 * ldw;
+    const int w_bytes = (min(kCols, prm.n_cols - n0) + (HALVES ? prm.n_cols : 0)) * ldw * EB;
     const __amdgpu_buffer_rsrc_t w_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(W), 0, w_bytes, kRsrcFlags);
-    const uint32_t w_off = (uint32_t)(row8 * K * EB + chunk * 16), eight_rows = (uint32_t)(8 * K * EB);
+    const uint32_t w_off = (uint32_t)(row8 * ldw * EB + chunk * 16), eight_rows = (uint32_t)(8 * ldw * EB);
+    const uint32_t half_rows = HALVES ? (uint32_t)prm.n_cols * (uint32_t)(ldw * EB) : 0u;
     const bool gather = prm.row_index != nullptr;
 
     // NB blocks of 16 columns from column c0 of the workgroup on times RB blocks of 16 rows from the expert's row r0 on; a unit is LINES times
@@ -107,16 +129,17 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
         constexpr int NB = decltype(nb_tag)::value, RB = decltype(rb_tag)::value, LINES = decltype(lines_tag)::value;
         constexpr int POLICY = decltype(policy_tag)::value;
         static_assert(NB * RB <= 2 * COL_BLOCKS && NB <= kSkWaves, "the waves' sums");
+        constexpr int NH = HALVES ? NB / 2 : NB;   // blocks of a half
         struct Unit { u32x4 w[LINES][NB][2], x[LINES][RB][2]; };
         // The rows, in a resource that begins at the pass's first or at the tile's: all of an expert can be more than the 2 GiB that offsets reach (bit
         // 31 marks one as out of range), these are at most 32 or 128 of 4 MiB.  A gathered matrix is less than 2 GiB as a whole.
         const int base = APART ? r0 : 0, base_rows = APART ? min(rows - r0, 16 * RB) : rows;
         const int64_t base_at = (int64_t)first + base;
         const __amdgpu_buffer_rsrc_t x_rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<T *>((const T *)prm.x + (gather ? (int64_t)0 : base_at * K)), 0, (int)(gather ? prm.x_total_rows : (int64_t)base_rows) * K * EB, kRsrcFlags);
+            const_cast<T *>((const T *)prm.x + (gather ? (int64_t)0 : base_at * ldx)), 0, (int)(gather ? prm.x_total_rows : (int64_t)base_rows) * ldx * EB, kRsrcFlags);
         const __amdgpu_buffer_rsrc_t index_rs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<int64_t *>(gather ? prm.row_index + base_at : nullptr), 0, gather ? base_rows * 8 : 0, kRsrcFlags);
-        const uint32_t w_base = w_off + (uint32_t)c0 * (uint32_t)(K * EB);
+        const uint32_t w_base = w_off + (uint32_t)c0 * (uint32_t)(ldw * EB);
         const int n_units = (K + kLine * LINES - 1) / (kLine * LINES);
         const int turn = __builtin_amdgcn_readfirstlane((int)(start % (uint32_t)n_units));   // the unit it begins with
         // (offsets past the contraction, as of every unit past it, have the sign bit set)
@@ -131,8 +154,9 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                 const uint32_t at = w_base + line_offset(unit, l);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    u.w[l][n][0] = __builtin_amdgcn_raw_buffer_load_b128(w_rs, (int)(at + 2 * n * eight_rows), 0, POLICY);
-                    u.w[l][n][1] = __builtin_amdgcn_raw_buffer_load_b128(w_rs, (int)(at + (2 * n + 1) * eight_rows), 0, POLICY);
+                    const uint32_t block = at + 2 * (n % NH) * eight_rows + (n < NH ? 0u : half_rows);
+                    u.w[l][n][0] = __builtin_amdgcn_raw_buffer_load_b128(w_rs, (int)block, 0, POLICY);
+                    u.w[l][n][1] = __builtin_amdgcn_raw_buffer_load_b128(w_rs, (int)(block + eight_rows), 0, POLICY);
                 }
             }
         };
@@ -159,7 +183,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     src = prm.div_shift < 0 ? idx : __umulhi(idx, prm.div_mul) >> prm.div_shift;
                     valid = valid && index[y][h][1] == 0 && idx <= (uint32_t)INT32_MAX && (int64_t)src < prm.x_total_rows;
                 }
-                x_off[y][h] = valid ? src * (uint32_t)(K * EB) + chunk * 16 : kOutOfRange;
+                x_off[y][h] = valid ? src * (uint32_t)(ldx * EB) + chunk * 16 : kOutOfRange;
             }
         f32x4 acc[NB][RB];
 #pragma unroll
@@ -209,18 +233,71 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
             __builtin_amdgcn_sched_barrier(0);
             unit += kSkWaves;
         }
-        // the waves' sums in ascending order of the wave; wave n adds column block n's
+        // the waves' sums in ascending order of the wave; wave n adds column block n's (of both halves)
         __syncthreads();   // (the pass before has read its sums)
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            if (wave == n) continue;
+            if (wave == n % NH) continue;
 #pragma unroll
-            for (int y = 0; y < RB; ++y) part[wave - (wave > n ? 1 : 0)][n * RB + y][lane] = acc[n][y];
+            for (int y = 0; y < RB; ++y) part[wave - (wave > n % NH ? 1 : 0)][n * RB + y][lane] = acc[n][y];
         }
         __syncthreads();
+        auto summed = [&](int n, int y) -> f32x4 {
+            f32x4 v = n % NH == 0 ? acc[n][y] : part[0][n * RB + y][lane];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
+            for (int w = 1; w < kSkWaves; ++w)
+                v = RingElem<T>::add(v, w == n % NH ? acc[n][y] : part[w - (w > n % NH ? 1 : 0)][n * RB + y][lane]);
+            return v;
+        };
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
             if (wave != n) continue;
+            if constexpr (HALVES || kInt8) {
+                // the sums (in integers: under their scales) with the bias, of one half or both
+                constexpr int H = HALVES ? 2 : 1;
+                const int col = n0 + c0 + 16 * n + 4 * hq;
+                if (col >= prm.n_cols) continue;
+                const int64_t channel = (int64_t)expert * (H * prm.n_cols) + col;
+                float add[H][4] = {}, scale[H][4] = {};
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    if (prm.bias != nullptr) {
+                        alignas(8) Out b4[4];
+                        *(u32x2 *)b4 = *(const u32x2 *)((const Out *)prm.bias + channel + h * prm.n_cols);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) add[h][i] = (float)b4[i];
+                    }
+                    if constexpr (kInt8) __builtin_memcpy(scale[h], prm.w_scale + channel + h * prm.n_cols, 16);
+                }
+#pragma unroll
+                for (int y = 0; y < RB; ++y) {
+                    const int row = r0 + 16 * y + lb;
+                    const f32x4 sum[2] = {summed(n, y), HALVES ? summed(n + NH, y) : f32x4{}};
+                    if (row >= rows) continue;
+                    const float s = kInt8 ? prm.x_scale[first + row] : 1.f;
+                    alignas(8) Out pre[H][4], res[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v[H];
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            if constexpr (kInt8) v[h] = fmaf((float)(int)__float_as_uint(sum[h][i]), s * scale[h][i], add[h][i]);
+                            else v[h] = sum[h][i] + add[h][i];
+                            pre[h][i] = (Out)v[h];
+                        }
+                        float r = gate_act<true>(v[0], prm.activation);
+                        if constexpr (HALVES) r *= v[1];
+                        res[i] = (Out)r;
+                    }
+                    const int64_t at = (int64_t)(first + row) * prm.n_cols + col;
+                    if (HALVES && prm.aux != nullptr) {
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+                            *(u32x2 *)((Out *)prm.aux + 2 * at - col + h * prm.n_cols) = *(const u32x2 *)pre[h];
+                    }
+                    *(u32x2 *)((Out *)prm.y + at) = *(const u32x2 *)res;
+                }
+            } else {
             // acc[n][y][i] is C(row 16 y + lb, column 16 n + 4 hq + i)
             const int col = n0 + c0 + 16 * n + 4 * hq;
             alignas(16) T b4[4] = {};
@@ -228,9 +305,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                 *(Vec4 *)b4 = *(const Vec4 *)((const T *)prm.bias + (int64_t)expert * prm.n_cols + col);
 #pragma unroll
             for (int y = 0; y < RB; ++y) {
-                f32x4 v = n == 0 ? acc[n][y] : part[0][n * RB + y][lane];
-#pragma unroll
-                for (int w = 1; w < kSkWaves; ++w) v += w == n ? acc[n][y] : part[w - (w > n ? 1 : 0)][n * RB + y][lane];
+                const f32x4 v = summed(n, y);
                 const int row = r0 + 16 * y + lb;
                 if (row >= rows || col >= prm.n_cols) continue;
                 alignas(16) T pre[4], res[4];
@@ -243,6 +318,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                 const int64_t at = (int64_t)(first + row) * prm.n_cols + col;
                 if (prm.aux != nullptr) *(Vec4 *)((T *)prm.aux + at) = *(const Vec4 *)pre;
                 *(Vec4 *)((T *)prm.y + at) = *(const Vec4 *)res;
+            }
             }
         }
     };
@@ -270,7 +346,8 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
         }
     };
     up_to_two(0);
-    if (COL_BLOCKS > 2 && prm.n_cols - n0 > 32) up_to_two(32);
+    constexpr int kNext = HALVES ? 16 : 32;
+    if (COL_BLOCKS > 2 && prm.n_cols - n0 > kNext) up_to_two(kNext);
 #endif
 }
 
@@ -280,14 +357,14 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
 // 8 of 4096 x 14336, 64: 178 / 152 / 137, shares 1 / rank^1.2: 179 / 157 / 146; 64 of 8192 x 2048, 512, such shares: 445 / 400 / 515.  So
 // one where two would make fewer workgroups than there are compute units, and four where one expert makes half as many.
 // (float32 with 4 loses on skewed counts everywhere: 8 of 2048 x 8192, 192 rows: 183 / 144 / 161.)
-template <typename T> int skinny_blocks(const SkinnyParams &prm, int64_t experts) {
+template <typename T> int skinny_blocks(const SkinnyParams &prm, int64_t experts, int n_cols, bool gated) {
     const int64_t cus = device_compute_units();
-    if (experts * ceil_div(prm.n_cols, 32) < cus) return 1;
+    if (!gated && experts * ceil_div(n_cols, 32) < cus) return 1;
     // (a workgroup's weights in one buffer resource)
-    return sizeof(T) == 2 && ceil_div(prm.n_cols, 64) * 2 >= cus && (int64_t)prm.k_extent * 2 * 64 < ((int64_t)1 << 31) ? 4 : 2;
+    return sizeof(T) == 2 && ceil_div(n_cols, 64) * 2 >= cus && (int64_t)prm.k_extent * 2 * 64 < ((int64_t)1 << 31) ? 4 : 2;
 }
 
-template <typename T> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+template <typename T, bool HALVES = false> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     SkinnyParams prm = params;
     // An expert's groups of rows go to workgroups of their own, where the experts come in order of their rows: the further groups first,
     // which leave at once where there are none.  128 experts of 1280 x 1280, 448 rows, 144 of them one expert's: 37 us in turn, 29 apart; 64 of 1280 x
@@ -298,25 +375,41 @@ template <typename T> int launch(const SkinnyParams &params, int64_t rows_cap, i
     prm.order_off = (int32_t)(apart ? segtab::order_off(rows_cap, n_expert) : segtab::map128_off(rows_cap, n_expert));
     prm.extra_groups = apart ? (int32_t)(rows_cap / kSkRows) : 0;
     const int64_t experts = apart ? std::min(rows_cap, n_expert) : segtab::cap_tiles(rows_cap, n_expert, 128);
-    const int blocks = apart ? skinny_blocks<T>(prm, experts) : 2;
-    prm.tiles_n = (int)ceil_div(prm.n_cols, 16 * blocks);
+    const int blocks = apart ? skinny_blocks<T>(prm, experts, (HALVES ? 2 : 1) * prm.n_cols, HALVES) : 2;
+    prm.tiles_n = (int)ceil_div(prm.n_cols, 16 * blocks / (HALVES ? 2 : 1));
     const int64_t grid = (experts + prm.extra_groups) * prm.tiles_n;
     if (grid > (int64_t)INT32_MAX) return fail(FMOE_ELIMIT, "grouped GEMM: grid of %lld workgroups", (long long)grid);
-    if (!apart) grouped_gemm_skinny_kernel<T, 2, false><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
-    else if (blocks == 1) grouped_gemm_skinny_kernel<T, 1, true><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
-    else if (blocks == 2) grouped_gemm_skinny_kernel<T, 2, true><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
-    else if constexpr (sizeof(T) == 2) grouped_gemm_skinny_kernel<T, 4, true><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    if (!apart) grouped_gemm_skinny_kernel<T, 2, false, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    else if (blocks == 2) grouped_gemm_skinny_kernel<T, 2, true, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    else if (blocks == 1) { if constexpr (!HALVES) grouped_gemm_skinny_kernel<T, 1, true, false><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm); }
+    else if constexpr (sizeof(T) == 2) grouped_gemm_skinny_kernel<T, 4, true, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
 }
 
 }  // namespace
 
+#if FMOE_SKINNY == 0
 int launch_skinny(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16 || dtype == FMOE_F32, "grouped GEMM: dtype %d is not a 16- or 32-bit float type", dtype);
     if (dtype == FMOE_F32) return launch<float>(prm, rows_cap, n_expert, stream);
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, rows_cap, n_expert, stream) : launch<_Float16>(prm, rows_cap, n_expert, stream);
 }
+#elif FMOE_SKINNY == 1
+int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+    FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16, "grouped GEMM: dtype %d is not a 16-bit float type", dtype);
+    return dtype == FMOE_BF16 ? launch<__bf16, true>(prm, rows_cap, n_expert, stream) : launch<_Float16, true>(prm, rows_cap, n_expert, stream);
+}
+#elif FMOE_SKINNY == 2
+int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+    FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16, "grouped GEMM: dtype %d is not a 16-bit float type", dtype);
+    if (gated)
+        return dtype == FMOE_BF16 ? launch<Int8Pair<__bf16>, true>(prm, rows_cap, n_expert, stream) : launch<Int8Pair<_Float16>, true>(prm, rows_cap, n_expert, stream);
+    return dtype == FMOE_BF16 ? launch<Int8Pair<__bf16>>(prm, rows_cap, n_expert, stream) : launch<Int8Pair<_Float16>>(prm, rows_cap, n_expert, stream);
+}
+#else
+#error "FMOE_SKINNY must be 0, 1 or 2"
+#endif
 
 }  // namespace gemm
 }  // namespace fmoe

@@ -764,10 +764,15 @@ int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts, int64_
     return FMOE_OK;
 }
 
+// Few rows per expert: as for a plain product of as many columns.
+bool gated_forward_few(const GatedArgs &a) {
+    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
+           use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype) && (a.h + 32) * a.d * 2 < ((int64_t)1 << 31);
+}
 // Where the two products together are at least as large as the persistent kernel wants them; its loads reach 2 GiB from a tile's first row of weights.
 bool gated_forward_fused(const GatedArgs &a) {
     return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
-           use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype), a.dtype) && 2 * a.h * a.d * 2 < ((int64_t)1 << 31) && a.h * 4 <= (1 << 22);
+           (gated_forward_few(a) || use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype), a.dtype)) && 2 * a.h * a.d * 2 < ((int64_t)1 << 31) && a.h * 4 <= (1 << 22);
 }
 bool gated_dgrad_fused(const GatedArgs &a) {
     return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.pre, a.out}, {a.d, a.h}) &&
@@ -791,6 +796,17 @@ int ring_of_table(RingParams &prm, const GatedArgs &a, int cols) {
 }
 }  // namespace
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
+    if (gated_forward_few(a)) {
+        SkinnyParams sk{};
+        sk.w = a.w; sk.x = a.in; sk.bias = a.bias; sk.y = a.out; sk.aux = a.pre; sk.dev_tab = a.dev_tab;
+        sk.n_cols = (int)a.h; sk.k_extent = (int)a.d; sk.activation = a.activation;
+        LinearForwardArgs like{};
+        like.in_feat = a.d; like.out_feat = 2 * a.h; like.dtype = a.dtype; like.dev_weights_once = a.pre == nullptr;
+        sk.weights_cached = caches_few_row_weights(like, a.n_expert);
+        sk.tail = a.tail; sk.tail_rows = a.rows_cap; sk.tail_elems = a.d;
+        ProfileScope prof(kProfGemmFwd, 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
+        return launch_skinny_gated(sk, a.dtype, a.rows_cap, a.n_expert, stream);
+    }
     RingParams prm{};
     prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.bias = a.bias; prm.aux = a.pre;
     prm.ldp = a.d; prm.ldq = a.d; prm.ldc = a.h;
@@ -811,6 +827,22 @@ int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
     return a.dtype == FMOE_BF16 ? launch_ring_bf16_dgated(prm, kEpiDGated, a.activation, stream) : launch_ring_f16_dgated(prm, kEpiDGated, a.activation, stream);
 }
 
+// The experts' product in 8-bit integers with few rows per expert.
+bool int8_few_takes(const Int8Params &a) {
+    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && a.ldx <= (1 << 22) && a.ldw * 64 < ((int64_t)1 << 31) && (a.bias == nullptr || aligned16(a.bias)) &&
+           use_skinny(a.rows_cap, a.n_expert, a.k_extent / 2, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.dtype);
+}
+int launch_int8_few(const Int8Params &a, hipStream_t stream) {
+    SkinnyParams sk{};
+    sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
+    sk.n_cols = a.n_cols; sk.k_extent = a.k_extent / 2; sk.activation = a.activation;
+    sk.ldw = a.ldw / 2; sk.ldx = a.ldx / 2; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
+    LinearForwardArgs like{};
+    like.in_feat = a.k_extent / 2; like.out_feat = (a.gated ? 2 : 1) * (int64_t)a.n_cols; like.dtype = a.dtype; like.dev_weights_once = true;
+    sk.weights_cached = caches_few_row_weights(like, a.n_expert);
+    ProfileScope prof(kProfGemmFwd, 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)like.out_feat, stream);
+    return launch_skinny_int8(sk, a.dtype, a.gated != 0, a.rows_cap, a.n_expert, stream);
+}
 // The experts' product in 8-bit integers on the persistent kernel: results of 16 bits in rows of whole 16-byte pieces, where there are enough tiles for it.
 bool int8_ring_takes(const Int8Params &a) {
     return is_16bit(a.dtype) && a.n_cols % 8 == 0 && aligned16(a.y) && (a.bias == nullptr || aligned16(a.bias)) && aligned16(a.w_scale) &&
