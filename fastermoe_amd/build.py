@@ -32,8 +32,7 @@ FLAGS += os.environ.get("FMOE_EXTRA_FLAGS", "").split()
 PLAIN_UNITS = ["error.cpp", "profile.cpp", "routing.hip", "segment_table.hip", "permute.hip", "combine.hip", "gate_grad.hip", "grouped_gemm.hip", "gemm_any.hip", "gemm_unaligned.hip", "pipeline.hip", "layer.hip",
                "layer_norm.hip", "balance_loss.hip", "act_checkpoint.hip", "gated_mlp.hip", "quantize_rows.hip", "gemm_int8.hip"]
 GEMM_TYPES = {0: "f32", 1: "bf16", 2: "f16"}
-GEMM_PRODUCTS = {0: "fwd", 1: "dgrad", 2: "wgrad"}
-RING_PRODUCTS = {**GEMM_PRODUCTS, 3: "gated", 4: "dgated", 5: "int8"}
+GEMM_PRODUCTS = {0: "fwd", 1: "dgrad", 2: "wgrad", 3: "gated", 4: "dgated", 5: "int8"}
 
 
 def _units():
@@ -45,10 +44,9 @@ def _units():
         units.append(("gemm_skinny.hip", f"gemm_skinny_{name}.o", [f"-DFMOE_SKINNY={i}"]))
     for t, tname in GEMM_TYPES.items():
         for p, pname in GEMM_PRODUCTS.items():
-            units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",
-                          [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))
-    for t, tname in GEMM_TYPES.items():
-        for p, pname in RING_PRODUCTS.items():
+            if tname != "f32" or pname != "int8":
+                units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",
+                              [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))
             if tname != "f32":
                 units.append(("gemm_ring_inst.hip", f"gemm_ring_{tname}_{pname}.o",
                               [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))

@@ -164,7 +164,7 @@ GatedArgs gated_sizes(const Sizes &s) {
 Scratch forward_scratch(const Sizes &s, bool keeps_pre, bool aligned) {
     const bool fused = aligned && gated_forward_fused(gated_sizes(s));
     return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)), 0,
-                   std::max(fused ? gated_workspace_bytes(s.d, s.dtype)
+                   std::max(fused ? gated_forward_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE, 0, 0),
                             fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0))};
 }
@@ -172,7 +172,7 @@ Scratch backward_scratch(const Sizes &s, bool aligned) {
     const bool fused = aligned && gated_dgrad_fused(gated_sizes(s));
     const int64_t row = s.rows * s.h * dtype_bytes(s.dtype);
     return Scratch{round256(2 * row), fused ? 0 : round256(row),
-                   std::max(fused ? gated_workspace_bytes(s.d, s.dtype)
+                   std::max(fused ? gated_dgrad_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE),
                             fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE))};
 }

@@ -1,6 +1,6 @@
 // One translation unit per (element type, product) of the grouped GEMM; the build
-// compiles this file nine times with -DFMOE_GEMM_TYPE=<0 f32|1 bf16|2 f16> and
-// -DFMOE_GEMM_PRODUCT=<0 fwd|1 dgrad|2 wgrad>.
+// compiles this file with -DFMOE_GEMM_TYPE=<0 f32|1 bf16|2 f16> and -DFMOE_GEMM_PRODUCT=<0 fwd|1 dgrad|2 wgrad|3 gated forward|4 data gradient up to a gated
+// forward's product|5 forward in 8-bit integers, the type (1 or 2) its results'>.
 #include "gemm_kernel.hpp"
 
 #if FMOE_GEMM_TYPE == 0
@@ -34,8 +34,20 @@ int FMOE_CAT(FMOE_TNAME, dgrad)(GemmParams &prm, int epilogue, hipStream_t strea
 int FMOE_CAT(FMOE_TNAME, wgrad)(GemmParams &prm, int epilogue, hipStream_t stream) {
     return launch_by_epilogue<FMOE_T, kMC, kMC, kRaggedK, (1 << kEpiStore)>(prm, epilogue, stream);
 }
+#elif FMOE_GEMM_PRODUCT == 3
+int FMOE_CAT(FMOE_TNAME, gated)(GemmParams &prm, int epilogue, hipStream_t stream) {
+    return launch_by_epilogue<FMOE_T, kKC, kKC, kRaggedRows, 1 << kEpiGated>(prm, epilogue, stream);
+}
+#elif FMOE_GEMM_PRODUCT == 4
+int FMOE_CAT(FMOE_TNAME, dgated)(GemmParams &prm, int epilogue, hipStream_t stream) {
+    return launch_by_epilogue<FMOE_T, kMC, kKC, kRaggedRows, 1 << kEpiDGated>(prm, epilogue, stream);
+}
+#elif FMOE_GEMM_PRODUCT == 5
+int FMOE_CAT(FMOE_TNAME, int8)(GemmParams &prm, int epilogue, hipStream_t stream) {
+    return launch_by_epilogue<Int8Pair<FMOE_T>, kKC, kKC, kRaggedRows, (1 << kEpiInt8) | (1 << kEpiInt8Gated)>(prm, epilogue, stream);
+}
 #else
-#error "FMOE_GEMM_PRODUCT must be 0, 1 or 2"
+#error "FMOE_GEMM_PRODUCT must be 0 to 5"
 #endif
 
 }  // namespace fmoe

@@ -189,8 +189,7 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     prm.bias = bias; prm.y = y; prm.ldx = ldx; prm.ldw = ldw; prm.w_expert_stride = w_expert_stride;
     prm.n_cols = (int)out_feat; prm.k_extent = (int)whole; prm.gated = gated != 0; prm.activation = activation;
     prm.dev_tab = (const int32_t *)segment_table; prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.dtype = dtype;
-    if (int8_few_takes(prm)) return launch_int8_few(prm, (hipStream_t)stream);
-    if (int8_ring_takes(prm)) return launch_int8_ring(prm, workspace, workspace_bytes, (hipStream_t)stream);
+    if (int8_in_pairs(prm)) return launch_int8_pairs(prm, workspace, workspace_bytes, (hipStream_t)stream);
     if (dtype == FMOE_F32) return launch<float>(prm, (hipStream_t)stream);
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, (hipStream_t)stream) : launch<_Float16>(prm, (hipStream_t)stream);
 }
@@ -200,5 +199,5 @@ extern "C" int64_t fmoe_linear_int8_workspace_bytes(int64_t n_expert, int64_t ro
     Int8Params prm{};
     prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.n_cols = (int)out_feat; prm.k_extent = (int)(ceil_div(in_feat, 16) * 16);
     prm.gated = gated != 0; prm.dtype = dtype;
-    return int8_ring_takes(prm) ? int8_ring_workspace_bytes(prm.k_extent) : 0;
+    return int8_in_pairs(prm) ? int8_workspace_bytes(prm) : 0;
 }

@@ -20,12 +20,10 @@ struct Int8Params {
     int32_t tiles_n, map_off;     // set by the launch
 };
 
-// Few rows per expert (gemm_skinny.hip).
-bool int8_few_takes(const Int8Params &a);
-int launch_int8_few(const Int8Params &a, hipStream_t stream);
-// The persistent kernel (gemm_ring.hpp): whether it takes a product, its workspace (not needed, but used to share a last round's tiles), the launch.
-bool int8_ring_takes(const Int8Params &a);
-int64_t int8_ring_workspace_bytes(int64_t k_extent);
-int launch_int8_ring(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+// The kernels of 16-bit types with pairs of integers in their elements' places (grouped_gemm.hip): whether they take a product, their workspace (not needed, but used
+// to share a last round's tiles), the launch.
+bool int8_in_pairs(const Int8Params &a);
+int64_t int8_workspace_bytes(const Int8Params &a);
+int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
 }  // namespace fmoe

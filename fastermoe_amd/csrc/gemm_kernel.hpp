@@ -2,6 +2,7 @@
 // gemm_inst.hip (one translation unit per element type and product, so that the
 // variants build in parallel) and by grouped_gemm.hip (host dispatch).
 #pragma once
+#include "gated_terms.hpp"
 #include "gelu_terms.hpp"
 #include "grouped_gemm.hpp"
 #include "profile.hpp"
@@ -64,6 +65,7 @@ template <typename T> struct Elem;
 // flops it moves half as many accumulator registers as 32 x 32 x 16, and under the chip's
 // power limit that buys clock.  fp32 uses 32 x 32 x 2 where its bf16 parts do not do (Split8).
 template <> struct Elem<__bf16> {
+    typedef __bf16 Out;   // of the results
     static constexpr int kPerChunk = 8;
     static constexpr int kBlk = 16;  // rows and columns of one MFMA block
     typedef f32x4 Acc;
@@ -75,6 +77,7 @@ template <> struct Elem<__bf16> {
 };
 
 template <> struct Elem<_Float16> {
+    typedef _Float16 Out;
     static constexpr int kPerChunk = 8;
     static constexpr int kBlk = 16;
     typedef f32x4 Acc;
@@ -85,6 +88,7 @@ template <> struct Elem<_Float16> {
 };
 
 template <> struct Elem<float> {
+    typedef float Out;
     static constexpr int kPerChunk = 4;
     static constexpr int kBlk = 32;
     typedef f32x16 Acc;
@@ -94,6 +98,54 @@ template <> struct Elem<float> {
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(p[j]), __uint_as_float(q[j]), acc, 0, 0, 0);
     }
 };
+
+// Two 8-bit integers of a row: to the loads and the LDS images of slabs rows of them are rows of 16-bit elements, and v_mfma_i32_16x16x64_i8 takes 16 bytes of
+// a row per lane as the 16-bit forms do, at twice their rate.  The accumulators are 32-bit integers in the same registers.  OUT_T: the results' type.
+template <typename OUT_T> struct Int8Pair { uint16_t both; };
+typedef int int32x4 __attribute__((ext_vector_type(4)));
+template <typename OUT_T> struct Elem<Int8Pair<OUT_T>> {
+    typedef OUT_T Out;
+    static constexpr int kPerChunk = 8;
+    static constexpr int kBlk = 16;
+    typedef f32x4 Acc;
+    __device__ static __forceinline__ void mma(Acc &acc, const u32x4 &p, const u32x4 &q) {
+        acc = __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int32x4, p), __builtin_bit_cast(int32x4, q),
+                                                                             __builtin_bit_cast(int32x4, acc), 0, 0, 0));
+    }
+};
+template <typename T> struct IsInt8 : std::false_type {};
+template <typename OUT_T> struct IsInt8<Int8Pair<OUT_T>> : std::true_type {};
+// the sum of two parts of an accumulator
+template <typename T> __device__ __forceinline__ f32x4 add_parts(const f32x4 &a, const f32x4 &b) {
+    if constexpr (IsInt8<T>::value) return __builtin_bit_cast(f32x4, __builtin_bit_cast(int32x4, a) + __builtin_bit_cast(int32x4, b));
+    else return a + b;
+}
+// what an accumulator's element stands for
+template <typename T> __device__ __forceinline__ float acc_value(float v) { return IsInt8<T>::value ? (float)(int)__float_as_uint(v) : v; }
+
+// Products of two halves of P's rows, n_cols apart, that are one result's (a gate's and a linear half's)
+__host__ __device__ constexpr bool epi_halves(int epi) { return epi == kEpiGated || epi == kEpiInt8Gated; }
+
+// f(activation) with the activation as a constant; MERGED: ReLU and none as one
+template <bool MERGED, typename F> __device__ __forceinline__ void by_gate_activation(int activation, F &&f) {
+    // (the comments keep the compiler from computing what all have in common ahead of them, in more registers than there are)
+    if (activation == FMOE_ACT_SILU) {
+        asm volatile("; silu");
+        f(std::integral_constant<int, FMOE_ACT_SILU>{});
+    } else if (activation == FMOE_ACT_GELU) {
+        asm volatile("; gelu");
+        f(std::integral_constant<int, FMOE_ACT_GELU>{});
+    } else if constexpr (MERGED) {
+        asm volatile("; relu or none");
+        f(ReluOrNone{activation == FMOE_ACT_RELU ? 0.f : -INFINITY});
+    } else if (activation == FMOE_ACT_RELU) {
+        asm volatile("; relu");
+        f(std::integral_constant<int, FMOE_ACT_RELU>{});
+    } else {
+        asm volatile("; none");
+        f(std::integral_constant<int, FMOE_ACT_NONE>{});
+    }
+}
 
 // fp32 products on the bf16 matrix pipe.  A float is the sum of three bf16 numbers, each the rounding of what the ones before
 // it left (8 significant bits each): exactly from 2^-110 up, to 2^-134 below.  Of the nine products of two such sums the three
@@ -276,6 +328,11 @@ struct GemmParams {
     // the workspace of at least dev_cus tiles of fp32 accumulators, copied to split_ws for the launch)
     int32_t dev_cus;
     float *dev_split_ws;
+    // Gated products: rows of `tail` (tail_elems elements each) behind the table's become zeros, up to tail_rows (null: none).
+    void *tail;
+    int64_t tail_rows, tail_elems;
+    // 8-bit integers: scale of each row, and of each row of P
+    const float *q_scale, *p_scale;
     int64_t dev_rows_cap;      // host only: rows the device table was laid out for
     int32_t block_m, block_n;  // host only: tile height the segment table was built for (256, 128 or 64) and tile width
     int32_t loaders;           // host only: Loaders
@@ -391,6 +448,15 @@ struct LowTiles {
     }
 };
 
+// The staging area of a wave in the epilogues of gated products and of those in 8-bit integers: rows of kPiece bytes, kCols columns of the results, kRow bytes
+// apart; kAreas of them.
+template <typename T, int BM, int BN, int EPI> struct EpiStage {
+    static constexpr int kOutBytes = (int)sizeof(typename Elem<T>::Out), kWave = BN / kWavesN / (epi_halves(EPI) ? 2 : 1);
+    static constexpr int kCols = kWave * kOutBytes < 128 ? kWave : 128 / kOutBytes;
+    static constexpr int kPiece = kCols * kOutBytes, kRow = kPiece + 16, kAreas = EPI == kEpiDGated ? 2 : 1;
+    static constexpr int kWaveBytes = BM / waves_m_of(BN) * kRow * kAreas;
+};
+
 // ---- the kernel ---------------------------------------------------------------
 // P_POLICY: of the column operand's loads, kPolicyCached or kPolicyOnce
 template <typename T, int BM, int BN, int PSHAPE, int QSHAPE, int RAGGED, int EPI, int LOADERS, int P_POLICY>
@@ -415,6 +481,16 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
     constexpr int kAhead = ahead_of(LOADERS);        // slabs requested beyond two
     // fp32 row-ragged tiles of at most half their rows: see low_tile_loop
     constexpr bool kLowTiles = kSplit && RAGGED == kRaggedRows && TI == 2;
+    constexpr bool kHalves = epi_halves(EPI);        // see epi_halves
+    constexpr int kCols = kHalves ? BN / 2 : BN;     // C columns of a tile
+    static_assert(!kHalves || (PSHAPE == kKC && RAGGED == kRaggedRows && (sizeof(T) == 4 || TI % 2 == 0)), "halves of rows of the contraction");
+
+    if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
+        const int64_t there = ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)prm.dev_tab)[segtab::kRows];
+        if (prm.tail != nullptr && prm.fixup == 0 && there < prm.tail_rows)
+            for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (prm.tail_rows - there) * prm.tail_elems; i += (int64_t)gridDim.x * blockDim.x)
+                ((T *)prm.tail)[there * prm.tail_elems + i] = (T)0.f;
+    }
 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
@@ -538,7 +614,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
         seg_lo = prm.tab.seg[ei];
         seg_hi = prm.tab.seg[ei + 1];
     }
-    const int n0 = nt * BN;
+    const int n0 = nt * kCols;
 
     const T *Pb;
     const T *Qb;
@@ -573,7 +649,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
         Pb = (const T *)prm.P + (int64_t)seg_lo * prm.ldp + n0;
         aux_off = (int64_t)expert * prm.c_expert_stride + (int64_t)m0 * prm.ldc + n0;
     }
-    p_valid = min(BN, prm.n_cols - n0);
+    p_valid = min(kCols, prm.n_cols - n0);
     Cb = (T *)prm.C + aux_off;
 
     const int t = threadIdx.x;
@@ -636,10 +712,16 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
         const int r = lt >> 3;
         p_kc_chunk = (lt & 7) ^ swz(r);
 #pragma unroll
-        for (int it = 0; it < NP; ++it)
-            p_voff[it] = (it * kRowsPerPass + r < p_valid)
-                             ? (uint32_t)(((int64_t)(it * kRowsPerPass + r) * prm.ldp + p_kc_chunk * CE) * sizeof(T))
+        for (int it = 0; it < NP; ++it) {
+            // Halves: row `at` of the tile is of half `half`, column `col`.  16-bit types: the first half of a wave's rows, so that its blocks x and
+            // x + TI / 2 are the two halves of the same columns; fp32: the first 16 of every 32, so that a block has both.
+            const int at = it * kRowsPerPass + r;
+            constexpr int kRun = sizeof(T) == 4 ? 16 : WN / 2;
+            const int half = kHalves ? at / kRun & 1 : 0, col = kHalves ? at / (2 * kRun) * kRun + at % kRun : at;
+            p_voff[it] = (col < p_valid)
+                             ? (uint32_t)(((int64_t)(col + (half ? prm.n_cols : 0)) * prm.ldp + p_kc_chunk * CE) * sizeof(T))
                              : kOutOfRange;
+        }
     } else {
         const int kk = lt / P_CPR;
 #pragma unroll
@@ -1368,6 +1450,178 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
     if constexpr (RAGGED == kRaggedK && QSHAPE == kMC) {
         if (want_bias) __syncthreads();  // the bias reduction used the start of LDS
     }
+    if constexpr (EPI >= kEpiGated) {
+        // Epilogues of gated products and of those in 8-bit integers: a wave's sub-tile goes through its staging area kEpiCols columns at a time
+        // (rows of 64 or 128 bytes and 16 of padding); where g and u come in, they lie in two such areas and the results take their places.
+        typedef typename Elem<T>::Out Out;
+        typedef EpiStage<T, BM, BN, EPI> St;
+        constexpr bool kNarrow = sizeof(Out) == 2;
+        constexpr int kOut = 16 / (int)sizeof(Out), kChunks = St::kPiece / 16, kRows = 64 / kChunks, kSteps = WM / kRows;
+        constexpr int H = kHalves ? 2 : 1, kGroups = MB == 16 ? 1 : kHalves ? 2 : 4;                  // runs of four columns of a block, per half
+        constexpr int kBlockCols = kHalves && MB == 32 ? 16 : MB, kXs = St::kCols / kBlockCols;       // columns of a block; blocks of a pass
+        unsigned char *area = smem + (fixup ? 0 : wave) * (WM * St::kRow * St::kAreas);
+        const int col0 = kHalves ? wave_n0 / 2 : wave_n0, col_end = min(p_valid, kHalves ? wave_n_end / 2 : wave_n_end);
+        const int sr = lane / kChunks, sc = lane % kChunks;
+        typedef std::conditional_t<kNarrow, u32x2, u32x4> Vec4;
+        // half h of four columns: of block x (of the wave's columns), group g, in block row y
+        auto value = [&](int h, int x, int g, int y, int i) -> float {
+            if constexpr (MB == 16) return acc_value<T>(acc[kHalves ? x + h * (TI / 2) : x][y][i]);
+            else return acc[x][y][4 * (g + 2 * h) + i];
+        };
+        auto sync = [&]() { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); __builtin_amdgcn_wave_barrier(); };
+        auto at4 = [&](int a, int x, int g, int y) {
+            return (Vec4 *)(area + a * (WM * St::kRow) + (y * MB + lb) * St::kRow + (x * kBlockCols + g * 8 + hq * 4) * (int)sizeof(Out));
+        };
+        auto piece = [&](int a, int i) { return (u32x4 *)(area + a * (WM * St::kRow) + (i * kRows + sr) * St::kRow + sc * 16); };
+        // where this lane's 16 bytes of step i lie: row, column `col` of a matrix whose rows are ld elements
+        auto offset = [&](int i, int col, int64_t ld) -> uint32_t {
+            const int row = wave_m0 + i * kRows + sr, c = col + sc * kOut;
+            return row < q_valid && c < col_end ? (uint32_t)(((int64_t)row * ld + c) * (int64_t)sizeof(Out)) : kOutOfRange;
+        };
+        auto store = [&](int a, Out *dst, int col, int64_t ld) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(dst, 0, (int)kOutOfRange, kRsrcFlags);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) __builtin_amdgcn_raw_buffer_store_b128(*piece(a, i), rs, (int)offset(i, col, ld), 0, 0);
+        };
+        if constexpr (EPI == kEpiDGated) {
+            // acc: dm; aux, C: [rows, 2 n_cols], g and u, dg and du
+            const Out *in = (const Out *)prm.aux + aux_off;
+            Out *out = (Out *)prm.C + aux_off;
+            by_gate_activation<false>(prm.activation, [&](auto act) {
+#pragma unroll
+                for (int pass = 0; pass < WN / St::kCols; ++pass) {
+                    const int col = col0 + pass * St::kCols;
+                    // (all of both on their way at once where the registers are there)
+                    constexpr int kBatch = LOADERS == kLoadersShared ? 1 : 2;
+#pragma unroll
+                    for (int a0 = 0; a0 < 2; a0 += kBatch) {
+                        u32x4 v[kBatch][kSteps];
+#pragma unroll
+                        for (int a = 0; a < kBatch; ++a) {
+                            const __amdgpu_buffer_rsrc_t rs =
+                                __builtin_amdgcn_make_buffer_rsrc(const_cast<Out *>(in + (a0 + a) * prm.n_cols), 0, (int)kOutOfRange, kRsrcFlags);
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) v[a][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset(i, col, prm.ldc), 0, 0);
+                        }
+#pragma unroll
+                        for (int a = 0; a < kBatch; ++a)
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) *piece(a0 + a, i) = v[a][i];
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    sync();
+#pragma unroll
+                    for (int x = 0; x < kXs; ++x)
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                            for (int y = 0; y < TJ; ++y) {
+                                alignas(16) Out gate[4], lin[4];
+                                *(Vec4 *)gate = *at4(0, x, g, y);
+                                *(Vec4 *)lin = *at4(1, x, g, y);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float dm = acc[pass * kXs + x][y][MB == 16 ? i : 4 * g + i];
+                                    const ActTerms t = gate_terms<kNarrow>((float)gate[i], act);
+                                    gate[i] = (Out)(dm * (float)lin[i] * t.slope);
+                                    lin[i] = (Out)(dm * t.value);
+                                }
+                                *at4(0, x, g, y) = *(const Vec4 *)gate;
+                                *at4(1, x, g, y) = *(const Vec4 *)lin;
+                            }
+                    sync();
+                    store(0, out, col, prm.ldc);
+                    store(1, out + prm.n_cols, col, prm.ldc);
+                    sync();
+                }
+            });
+        } else {
+            // scales and biases: past the tile's columns they are another column's, or zero past the last
+            const int64_t p0 = (int64_t)expert * prm.bias_expert_stride + n0;
+            const int p_rows = (kHalves ? prm.n_cols : 0) + p_valid;
+            const __amdgpu_buffer_rsrc_t bias_rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<Out *>(prm.bias ? (const Out *)prm.bias + p0 : nullptr), 0, prm.bias ? p_rows * (int)sizeof(Out) : 0, kRsrcFlags);
+            const __amdgpu_buffer_rsrc_t scale_rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<float *>(IsInt8<T>::value ? prm.p_scale + p0 : nullptr), 0, IsInt8<T>::value ? p_rows * 4 : 0, kRsrcFlags);
+            const __amdgpu_buffer_rsrc_t row_rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<float *>(IsInt8<T>::value ? prm.q_scale + q_row0 : nullptr), 0, IsInt8<T>::value ? q_valid * 4 : 0, kRsrcFlags);
+            float row_scale[TJ];
+#pragma unroll
+            for (int y = 0; y < TJ; ++y)
+                row_scale[y] = IsInt8<T>::value ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(row_rs, (wave_m0 + y * MB + lb) * 4, 0, 0)) : 1.f;
+            // f(x, g, sums): four columns at a time, for all block rows: the products with scales and biases, of each half
+            auto each = [&](int pass, auto &&f) {
+#pragma unroll
+                for (int x = 0; x < kXs; ++x)
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        float add[H][4], scale[H][4];
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const int c = col0 + pass * St::kCols + x * kBlockCols + g * 8 + hq * 4 + (h ? prm.n_cols : 0);
+                            alignas(16) Out b[4];
+                            if constexpr (kNarrow) *(u32x2 *)b = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, c * (int)sizeof(Out), 0, 0);
+                            else *(u32x4 *)b = __builtin_amdgcn_raw_buffer_load_b128(bias_rs, c * (int)sizeof(Out), 0, 0);
+                            u32x4 s = {};
+                            if constexpr (IsInt8<T>::value) s = __builtin_amdgcn_raw_buffer_load_b128(scale_rs, c * 4, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                add[h][i] = (float)b[i];
+                                scale[h][i] = __uint_as_float(s[i]);
+                            }
+                        }
+#pragma unroll
+                        for (int y = 0; y < TJ; ++y) {
+                            float sum[H][4];
+#pragma unroll
+                            for (int h = 0; h < H; ++h)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float v = value(h, pass * kXs + x, g, y, i);
+                                    sum[h][i] = IsInt8<T>::value ? fmaf(v, row_scale[y] * scale[h][i], add[h][i]) : v + add[h][i];
+                                }
+                            f(x, g, y, sum);
+                        }
+                    }
+            };
+            if constexpr (EPI == kEpiGated) {
+                if (prm.aux != nullptr) {   // both halves as they are, [rows, 2 n_cols]
+                    Out *pre = (Out *)prm.aux + 2 * aux_off - n0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        each(0, [&](int x, int g, int y, const float (&sum)[H][4]) {
+                            alignas(16) Out v[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = (Out)sum[h][i];
+                            *at4(0, x, g, y) = *(const Vec4 *)v;
+                        });
+                        sync();
+                        store(0, pre + (h ? prm.n_cols : 0), col0, 2 * prm.ldc);
+                        sync();
+                    }
+                }
+            }
+            Out *out = (Out *)prm.C + aux_off;
+            by_gate_activation<IsInt8<T>::value>(prm.activation, [&](auto act) {
+#pragma unroll
+                for (int pass = 0; pass < WN / H / St::kCols; ++pass) {
+                    each(pass, [&](int x, int g, int y, const float (&sum)[H][4]) {
+                        alignas(16) Out v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float r = gate_act<kNarrow>(sum[0][i], act);
+                            if constexpr (kHalves) r *= sum[H - 1][i];
+                            v[i] = (Out)r;
+                        }
+                        *at4(0, x, g, y) = *(const Vec4 *)v;
+                    });
+                    sync();
+                    store(0, out, col0 + pass * St::kCols, prm.ldc);
+                    sync();
+                }
+            });
+        }
+    } else {
     constexpr int kPieceBytes = WN * (int)sizeof(T) < 256 ? WN * (int)sizeof(T) : 256;  // row piece moved per pass
     constexpr int kStgRow = kPieceBytes + 16;    // bytes; the pad spreads rows over the banks
     constexpr int CPP = kPieceBytes / (int)sizeof(T);  // C columns per pass through the staging area
@@ -1560,6 +1814,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
     } else {
         by_activation(std::false_type{});
     }
+    }
 #endif  // __HIP_DEVICE_COMPILE__
 }
 
@@ -1626,7 +1881,8 @@ int launch_tiles(GemmParams &prm, hipStream_t stream) {
     constexpr int kAhead = ahead_of(LOADERS);
     constexpr int smem_loop = ((3 + kAhead) * BN + (2 + kAhead) * BM) * kSlabBytes;
     constexpr int wave_cols_bytes = BN / kWavesN * (int)sizeof(T);
-    constexpr int smem_wave_epi = (BM / kWavesM) * ((wave_cols_bytes < 256 ? wave_cols_bytes : 256) + 16);
+    constexpr int smem_wave_epi = EPI >= kEpiGated ? EpiStage<T, BM, BN, EPI>::kWaveBytes
+                                                   : (BM / kWavesM) * ((wave_cols_bytes < 256 ? wave_cols_bytes : 256) + 16);
     constexpr int smem_epi = kWavesM * kWavesN * smem_wave_epi;
     constexpr int smem = smem_loop > smem_epi ? smem_loop : smem_epi;
     // the opt-in to more than 64 KiB of dynamic LDS is per device (and per kernel instantiation)
@@ -1719,7 +1975,7 @@ int launch_tiles(GemmParams &prm, hipStream_t stream) {
 // are built.
 template <typename T, int BM, int BN, int PS, int QS, int RG, int EPI_MASK, int LOADERS = kLoadersCompute, int P_POLICY = kPolicyCached>
 int launch_for_height(GemmParams &prm, int epi, hipStream_t stream) {
-    prm.tiles_n = (int)ceil_div(prm.n_cols, BN);
+    prm.tiles_n = (int)ceil_div(prm.n_cols, epi_halves(epi) ? BN / 2 : BN);
     int64_t total;
     if (RG == kRaggedRows) {
         prm.tiles_m = 0;
@@ -1741,6 +1997,14 @@ int launch_for_height(GemmParams &prm, int epi, hipStream_t stream) {
         if (epi == kEpiBiasAct) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiBiasAct, LOADERS, P_POLICY>(prm, stream);
     if constexpr ((EPI_MASK >> kEpiDAct) & 1)
         if (epi == kEpiDAct) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiDAct, LOADERS, P_POLICY>(prm, stream);
+    if constexpr ((EPI_MASK >> kEpiGated) & 1)
+        if (epi == kEpiGated) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiGated, LOADERS, P_POLICY>(prm, stream);
+    if constexpr ((EPI_MASK >> kEpiDGated) & 1)
+        if (epi == kEpiDGated) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiDGated, LOADERS, P_POLICY>(prm, stream);
+    if constexpr ((EPI_MASK >> kEpiInt8) & 1)
+        if (epi == kEpiInt8) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiInt8, LOADERS, P_POLICY>(prm, stream);
+    if constexpr ((EPI_MASK >> kEpiInt8Gated) & 1)
+        if (epi == kEpiInt8Gated) return launch_tiles<T, BM, BN, PS, QS, RG, kEpiInt8Gated, LOADERS, P_POLICY>(prm, stream);
     return fail(FMOE_EINVAL, "epilogue %d is not built for this product", epi);
 }
 
@@ -1793,6 +2057,14 @@ FMOE_DECLARE_MFMA(launch_mfma_f16_wgrad);
 FMOE_DECLARE_MFMA(launch_mfma_f32_fwd);
 FMOE_DECLARE_MFMA(launch_mfma_f32_dgrad);
 FMOE_DECLARE_MFMA(launch_mfma_f32_wgrad);
+FMOE_DECLARE_MFMA(launch_mfma_bf16_gated);
+FMOE_DECLARE_MFMA(launch_mfma_f16_gated);
+FMOE_DECLARE_MFMA(launch_mfma_f32_gated);
+FMOE_DECLARE_MFMA(launch_mfma_bf16_dgated);
+FMOE_DECLARE_MFMA(launch_mfma_f16_dgated);
+FMOE_DECLARE_MFMA(launch_mfma_f32_dgated);
+FMOE_DECLARE_MFMA(launch_mfma_bf16_int8);
+FMOE_DECLARE_MFMA(launch_mfma_f16_int8);
 // Feature sizes or pointers off the 16-byte grid, all three products (0 forward, 1 data gradient, 2 weight gradient):
 // 16-bit types in gemm_unaligned.hip, 32-bit ones and double precision (whatever its sizes) in gemm_any.hip
 int launch_mfma_unaligned(gemm::GemmParams &prm, int dtype, int product, int epilogue, hipStream_t stream);

@@ -20,32 +20,10 @@
 //     rows are filled with zeros outside the stream (ring_fill);
 //   * the bias gradient is one more column of products (a block of ones times the output gradient).
 #pragma once
-#include "gated_terms.hpp"
 #include "gemm_kernel.hpp"
 
 namespace fmoe {
 namespace gemm {
-
-// Two 8-bit integers of a row: to this kernel's loads and LDS images rows of them are rows of 16-bit elements.  OUT: the results' type.
-template <typename OUT> struct Int8Pair { uint16_t both; };
-template <typename T> struct RingElem {
-    typedef T Out;
-    static constexpr bool kInt8 = false;
-    __device__ static __forceinline__ void mma(f32x4 &acc, const u32x4 &p, const u32x4 &q) { Elem<T>::mma(acc, p, q); }
-    __device__ static __forceinline__ f32x4 add(const f32x4 &a, const f32x4 &b) { return a + b; }
-};
-template <typename OUT_T> struct RingElem<Int8Pair<OUT_T>> {   // (the accumulators are 32-bit integers in the same registers)
-    typedef OUT_T Out;
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    static constexpr bool kInt8 = true;
-    __device__ static __forceinline__ void mma(f32x4 &acc, const u32x4 &p, const u32x4 &q) {
-        acc = __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, p), __builtin_bit_cast(i32x4, q),
-                                                                             __builtin_bit_cast(i32x4, acc), 0, 0, 0));
-    }
-    __device__ static __forceinline__ f32x4 add(const f32x4 &a, const f32x4 &b) {
-        return __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, a) + __builtin_bit_cast(i32x4, b));
-    }
-};
 
 struct RingParams {
     const void *P;     // column operand
@@ -153,8 +131,7 @@ constexpr int kRingThreads = 512, kRingWaves = 8;
 constexpr int kRingTile = 256;
 // Products of two halves of P's rows: a tile has 128 columns of each, a wave 64 and 64 (rows 0 to 63 of its 128 the first half's), so that a lane has
 // both halves of its columns.
-__host__ __device__ constexpr bool ring_halves(int epi) { return epi == kEpiGated || epi == kEpiInt8Gated; }
-__host__ __device__ constexpr int ring_cols(int epi) { return ring_halves(epi) ? kRingTile / 2 : kRingTile; }
+__host__ __device__ constexpr int ring_cols(int epi) { return epi_halves(epi) ? kRingTile / 2 : kRingTile; }
 constexpr int kRingSlab = kRingTile * kSlabBytes;   // 32 KiB
 constexpr int kRingPBufs = 3, kRingQBase = kRingPBufs * kRingSlab;
 constexpr int kRingLds = (kRingPBufs + 2) * kRingSlab;
@@ -417,27 +394,6 @@ __device__ __forceinline__ void ring_epilogue(const RingParams &prm, const RingT
 #endif
 }
 
-// f(activation) with the activation as a constant; MERGED: ReLU and none as one
-template <bool MERGED, typename F> __device__ __forceinline__ void ring_by_activation(int activation, F &&f) {
-    // (the comments keep the compiler from computing what all have in common ahead of them, in more registers than there are)
-    if (activation == FMOE_ACT_SILU) {
-        asm volatile("; silu");
-        f(std::integral_constant<int, FMOE_ACT_SILU>{});
-    } else if (activation == FMOE_ACT_GELU) {
-        asm volatile("; gelu");
-        f(std::integral_constant<int, FMOE_ACT_GELU>{});
-    } else if constexpr (MERGED) {
-        asm volatile("; relu or none");
-        f(ReluOrNone{activation == FMOE_ACT_RELU ? 0.f : -INFINITY});
-    } else if (activation == FMOE_ACT_RELU) {
-        asm volatile("; relu");
-        f(std::integral_constant<int, FMOE_ACT_RELU>{});
-    } else {
-        asm volatile("; none");
-        f(std::integral_constant<int, FMOE_ACT_NONE>{});
-    }
-}
-
 // What goes from a wave's registers to memory by way of its 4 KiB of LDS, sixteen rows of CHUNKS 16-byte pieces at a time.
 template <int CHUNKS> struct RingStage {
     static constexpr int kStores = CHUNKS / 4, kRowsAt = 16 / kStores;   // rows of a store of the wave
@@ -501,7 +457,7 @@ __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const
     const int col = 64 * wn + st.io_c * 8;
     const uint32_t at = col < tl.p_valid ? (uint32_t)(col * 2) : kOutOfRange;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((T *)prm.C + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
-    ring_by_activation<false>(prm.activation, [&](auto act) {
+    by_gate_activation<false>(prm.activation, [&](auto act) {
 #pragma unroll
         for (int y = 0; y < NY; ++y) {
 #pragma unroll
@@ -555,7 +511,7 @@ __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, cons
         }
     };
     request(0);
-    ring_by_activation<false>(prm.activation, [&](auto act) {
+    by_gate_activation<false>(prm.activation, [&](auto act) {
 #pragma unroll
         for (int n = 0; n < 2 * NY; ++n) {
 #pragma unroll
@@ -600,7 +556,7 @@ template <typename T, bool GATED, int NY>
 __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                    int lane, int wm, int wn, int y0) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    typedef typename RingElem<T>::Out Out;
+    typedef typename Elem<T>::Out Out;
     static_assert(sizeof(Out) == 2, "results of 16 bits");
     constexpr uint32_t kOutOfRange = 0x80000000u;
     constexpr int kRsrcFlags = 0x00020000, X = GATED ? 4 : 8, H = GATED ? 2 : 1;
@@ -632,7 +588,7 @@ __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const 
 #pragma unroll
     for (int y = 0; y < NY; ++y) s[y] = __builtin_amdgcn_raw_buffer_load_b32(row_rs, (row0 + 16 * y + lb) * 4, 0, 0);
     request(0, cols[0]);
-    ring_by_activation<true>(prm.activation, [&](auto act) {
+    by_gate_activation<true>(prm.activation, [&](auto act) {
 #pragma unroll
         for (int pair = 0; pair < X / 2; ++pair) {
             if (pair + 1 < X / 2) request(pair + 1, cols[(pair + 1) & 1]);
@@ -685,7 +641,7 @@ __device__ __forceinline__ void ring_finish(const RingParams &prm, const RingTil
                                             unsigned char *stg, int lane, int wm, int wn, int y0) {
     if constexpr (EPI == kEpiGated) ring_epilogue_gated<T, AUX, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
     else if constexpr (EPI == kEpiDGated) ring_epilogue_dgated<T, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
-    else if constexpr (RingElem<T>::kInt8) ring_epilogue_int8<T, EPI == kEpiInt8Gated, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
+    else if constexpr (IsInt8<T>::value) ring_epilogue_int8<T, EPI == kEpiInt8Gated, NY>(prm, tl, acc, stg, lane, wm, wn, y0);
     else ring_epilogue<T, EPI, ACT, AUX, BIAS_GRAD, NY>(prm, tl, acc, bacc, stg, lane, wm, wn, y0);
 }
 
@@ -700,9 +656,9 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
     constexpr int NLOAD = 8;                 // 16-byte loads per loading thread, slab and operand
     constexpr uint32_t kOutOfRange = 0x80000000u;
     constexpr int kRsrcFlags = 0x00020000;   // raw buffer, 32-bit data format
-    constexpr bool kInt8 = RingElem<T>::kInt8;
+    constexpr bool kInt8 = IsInt8<T>::value;
     constexpr bool kForward = RAGGED == kRaggedRows && PSHAPE == kKC && !kInt8;
-    constexpr bool kHalves = ring_halves(EPI);   // two halves of P's rows, n_cols apart
+    constexpr bool kHalves = epi_halves(EPI);   // two halves of P's rows, n_cols apart
     constexpr int kCols = ring_cols(EPI);
     static_assert(!kHalves || PSHAPE == kKC, "halves of rows of the contraction");
     // With both operands [contraction][row] a fragment is two transposing reads, and a phase issues its loads, reads and
@@ -1015,7 +971,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
                 load_step(x_tag);
                 read_part(next, x, p_buf, q_buf);
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
+                for (int y = 0; y < TJ; ++y) Elem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
                 const int reads = (next & 1) ? kPReads : (x < 2 ? 2 * kQReads : 2 * kPReads);
 #pragma unroll
                 for (int i = 0; i < TJ; ++i) {
@@ -1038,7 +994,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
 #pragma unroll
             for (int x = 0; x < PF; ++x)
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
+                for (int y = 0; y < TJ; ++y) Elem<T>::mma(acc[(ph & 1) * PF + x][y], pf[ph & 1][x], qf[ph >> 1][y]);
             const int reads = PF * kPReads + ((next & 1) == 0 ? TJ * kQReads : 0);
 #pragma unroll
             for (int i = 0; i < PF * TJ; ++i) {
@@ -1137,7 +1093,7 @@ __global__ __launch_bounds__(kRingThreads) void grouped_gemm_ring_kernel(const R
                         if constexpr (kWithBiasGrad) {
                             if (want_bias) {
 #pragma unroll
-                                for (int y = 0; y < TJ; ++y) RingElem<T>::mma(bacc[y], ones, qf[ks][y]);
+                                for (int y = 0; y < TJ; ++y) Elem<T>::mma(bacc[y], ones, qf[ks][y]);
                             }
                             __builtin_amdgcn_sched_barrier(0);
                         }
@@ -1254,8 +1210,8 @@ __global__ __launch_bounds__(64) void ring_combine_kernel(const RingParams prm) 
         for (int b = 0; b < kBatch; ++b)
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                if (b == 0) acc[x][0] = j0 == first ? v[0][x] : RingElem<T>::add(acc[x][0], v[0][x]);
-                else if (j0 + b <= last) acc[x][0] = RingElem<T>::add(acc[x][0], v[b][x]);
+                if (b == 0) acc[x][0] = j0 == first ? v[0][x] : add_parts<T>(acc[x][0], v[0][x]);
+                else if (j0 + b <= last) acc[x][0] = add_parts<T>(acc[x][0], v[b][x]);
             }
     }
     const f32x4 none[1] = {};

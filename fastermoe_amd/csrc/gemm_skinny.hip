@@ -32,10 +32,6 @@ constexpr int kSkRows = 32;   // rows of a pass
 
 // one 16 x 16 block over 64 bytes of contraction; acc as for the 16 x 16 x 32 form
 template <typename T> __device__ __forceinline__ void mma_step(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<T>::mma(acc, w, x); }
-template <typename T> struct IsInt8 : std::false_type {};
-template <typename OUT> struct IsInt8<Int8Pair<OUT>> : std::true_type {};
-template <> __device__ __forceinline__ void mma_step<Int8Pair<__bf16>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { RingElem<Int8Pair<__bf16>>::mma(acc, w, x); }
-template <> __device__ __forceinline__ void mma_step<Int8Pair<_Float16>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { RingElem<Int8Pair<_Float16>>::mma(acc, w, x); }
 template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u32x4 &w, const u32x4 &x) {
     // product j takes element j of every lane's four: contraction elements j, 4 + j, 8 + j and 12 + j of the step
 #pragma unroll
@@ -62,7 +58,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     constexpr int EB = (int)sizeof(T), CE = 16 / EB, kLine = 128 / EB;    // elements per lane's load and per line
     typedef std::conditional_t<sizeof(T) == 2, u32x2, u32x4> Vec4;        // four elements
     constexpr bool kInt8 = IsInt8<T>::value;
-    typedef typename RingElem<T>::Out Out;                                // of the results
+    typedef typename Elem<T>::Out Out;                                // of the results
     constexpr int kCols = COL_BLOCKS * 16 / (HALVES ? 2 : 1);             // columns of a workgroup
     static_assert(!HALVES || (COL_BLOCKS >= 2 && sizeof(T) == 2), "halves: two blocks of columns or more");
     constexpr uint32_t kOutOfRange = 0x80000000u;
@@ -246,7 +242,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
             f32x4 v = n % NH == 0 ? acc[n][y] : part[0][n * RB + y][lane];
 #pragma unroll
             for (int w = 1; w < kSkWaves; ++w)
-                v = RingElem<T>::add(v, w == n % NH ? acc[n][y] : part[w - (w > n % NH ? 1 : 0)][n * RB + y][lane]);
+                v = add_parts<T>(v, w == n % NH ? acc[n][y] : part[w - (w > n % NH ? 1 : 0)][n * RB + y][lane]);
             return v;
         };
 #pragma unroll

@@ -1,6 +1,6 @@
 // Interface of gemm_skinny.hip: the grouped forward product for few rows per expert.
 #pragma once
-#include "gemm_ring.hpp"
+#include "gemm_kernel.hpp"
 
 namespace fmoe {
 namespace gemm {

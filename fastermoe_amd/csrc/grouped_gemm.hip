@@ -764,21 +764,28 @@ int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts, int64_
     return FMOE_OK;
 }
 
+namespace {
 // Few rows per expert: as for a plain product of as many columns.
-bool gated_forward_few(const GatedArgs &a) {
-    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
-           use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype) && (a.h + 32) * a.d * 2 < ((int64_t)1 << 31);
+bool gated_forward_few(const GatedArgs &a) { return is_16bit(a.dtype) && use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype); }
+TileShape gated_forward_tile(const GatedArgs &a) { return pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype); }
+TileShape gated_dgrad_tile(const GatedArgs &a) { return pick_rows_tile_estimate(a.rows_cap, a.n_expert, a.h, a.d, a.dtype); }
+DevRoute gated_route(const GatedArgs &a, const TileShape &tile) { return {use_ring(tile, a.dtype) ? DevKernel::kRing : DevKernel::kTiles, tile}; }
+// Tensors in whole 16-byte pieces; offsets from a tile's first row of weights, over both halves, and rows of both halves in 31 bits
+bool gated_sizes_fit(const GatedArgs &a) {
+    const int64_t eb = dtype_bytes(a.dtype);
+    return (is_16bit(a.dtype) || a.dtype == FMOE_F32) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
+           (2 * a.h + 256) * a.d * eb < ((int64_t)1 << 31) && 2 * a.h * eb <= (1 << 22);
 }
-// Where the two products together are at least as large as the persistent kernel wants them; its loads reach 2 GiB from a tile's first row of weights.
+}  // namespace
+// (float32 with few rows per expert: the decoding kernel's plain product and a kernel for the activation)
 bool gated_forward_fused(const GatedArgs &a) {
-    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.bias, a.pre, a.out}, {a.d, a.h}) &&
-           (gated_forward_few(a) || use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype), a.dtype)) && 2 * a.h * a.d * 2 < ((int64_t)1 << 31) && a.h * 4 <= (1 << 22);
+    return gated_sizes_fit(a) && (is_16bit(a.dtype) || !use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype));
 }
-bool gated_dgrad_fused(const GatedArgs &a) {
-    return is_16bit(a.dtype) && a.dev_tab != nullptr && is_fast(a.dtype, {a.in, a.w, a.pre, a.out}, {a.d, a.h}) &&
-           use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, a.h, a.d, a.dtype), a.dtype) && a.h * 4 <= (1 << 22);
+bool gated_dgrad_fused(const GatedArgs &a) { return gated_sizes_fit(a); }
+int64_t gated_forward_workspace_bytes(const GatedArgs &a) {
+    return gated_forward_few(a) ? 0 : route_workspace_bytes(gated_route(a, gated_forward_tile(a)), a.d, a.dtype);
 }
-int64_t gated_workspace_bytes(int64_t contraction, int dtype) { return route_workspace_bytes({DevKernel::kRing, kManyTiles}, contraction, dtype); }
+int64_t gated_dgrad_workspace_bytes(const GatedArgs &a) { return route_workspace_bytes(gated_route(a, gated_dgrad_tile(a)), a.d, a.dtype); }
 namespace {
 int ring_of_table(RingParams &prm, const GatedArgs &a, int cols) {
     prm.n_expert = (int32_t)a.n_expert;
@@ -794,6 +801,15 @@ int ring_of_table(RingParams &prm, const GatedArgs &a, int cols) {
     prm.tail = a.tail; prm.tail_rows = a.rows_cap; prm.tail_elems = a.d;
     return FMOE_OK;
 }
+int tiles_of_table(const char *who, GemmParams &prm, const GatedArgs &a, const TileShape &tile, int64_t w_rows, int64_t contraction) {
+    if (int rc = device_table_launch(who, prm, a.dev_tab, a.rows_cap, a.n_expert, true)) return rc;
+    prm.block_m = tile.bm; prm.block_n = tile.bn; prm.loaders = tile.loaders;
+    prm.weights_once = reads_weights_once(tile, a.rows_cap, a.n_expert, contraction, w_rows, a.dtype);
+    prm.activation = a.activation;
+    prm.tail = a.tail; prm.tail_rows = a.rows_cap; prm.tail_elems = a.d;
+    prm.dev_split_ws = route_workspace({DevKernel::kTiles, tile}, contraction, a.dtype, a.workspace, a.workspace_bytes);
+    return FMOE_OK;
+}
 }  // namespace
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
     if (gated_forward_few(a)) {
@@ -807,6 +823,18 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
         ProfileScope prof(kProfGemmFwd, 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
         return launch_skinny_gated(sk, a.dtype, a.rows_cap, a.n_expert, stream);
     }
+    const TileShape tile = gated_forward_tile(a);
+    if (!use_ring(tile, a.dtype)) {
+        GemmParams prm{};
+        if (int rc = tiles_of_table("gated forward", prm, a, tile, 2 * a.h, a.d)) return rc;
+        prm.profile_class = kProfGemmFwd; prm.profile_work = 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h;
+        prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.bias = a.bias; prm.aux = a.pre;
+        prm.ldp = a.d; prm.ldq = a.d; prm.ldc = a.h;
+        prm.p_expert_stride = 2 * a.h * a.d; prm.bias_expert_stride = 2 * a.h;
+        prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+        if (a.dtype == FMOE_F32) return launch_mfma_f32_gated(prm, kEpiGated, stream);
+        return a.dtype == FMOE_BF16 ? launch_mfma_bf16_gated(prm, kEpiGated, stream) : launch_mfma_f16_gated(prm, kEpiGated, stream);
+    }
     RingParams prm{};
     prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.bias = a.bias; prm.aux = a.pre;
     prm.ldp = a.d; prm.ldq = a.d; prm.ldc = a.h;
@@ -817,6 +845,18 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
     return a.dtype == FMOE_BF16 ? launch_ring_bf16_gated(prm, kEpiGated, a.activation, stream) : launch_ring_f16_gated(prm, kEpiGated, a.activation, stream);
 }
 int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
+    const TileShape tile = gated_dgrad_tile(a);
+    if (!use_ring(tile, a.dtype)) {
+        GemmParams prm{};
+        if (int rc = tiles_of_table("gated dgrad", prm, a, tile, a.h, a.d)) return rc;
+        prm.profile_class = kProfGemmDgrad; prm.profile_work = 2.0 * (double)a.rows_cap * (double)a.d * (double)a.h;
+        prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.aux = a.pre;
+        prm.ldp = a.h; prm.ldq = a.d; prm.ldc = 2 * a.h;
+        prm.p_expert_stride = a.h * a.d;
+        prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+        if (a.dtype == FMOE_F32) return launch_mfma_f32_dgated(prm, kEpiDGated, stream);
+        return a.dtype == FMOE_BF16 ? launch_mfma_bf16_dgated(prm, kEpiDGated, stream) : launch_mfma_f16_dgated(prm, kEpiDGated, stream);
+    }
     RingParams prm{};
     prm.P = a.w; prm.Q = a.in; prm.C = a.out; prm.aux = a.pre;
     prm.ldp = a.h; prm.ldq = a.d; prm.ldc = 2 * a.h;
@@ -827,41 +867,62 @@ int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
     return a.dtype == FMOE_BF16 ? launch_ring_bf16_dgated(prm, kEpiDGated, a.activation, stream) : launch_ring_f16_dgated(prm, kEpiDGated, a.activation, stream);
 }
 
-// The experts' product in 8-bit integers with few rows per expert.
-bool int8_few_takes(const Int8Params &a) {
-    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && a.ldx <= (1 << 22) && a.ldw * 64 < ((int64_t)1 << 31) && (a.bias == nullptr || aligned16(a.bias)) &&
-           use_skinny(a.rows_cap, a.n_expert, a.k_extent / 2, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.dtype);
+// The experts' product in 8-bit integers: 16-bit results in rows of whole 16-byte pieces go to the kernels of 16-bit types, pairs of integers in their elements'
+// places, by the same rules; but for few rows per expert (at most 16 on average), whose kernel carries on further than with twice the bytes.
+// us on 128 x 128 tiles and there, weights from memory, even counts / shares 1 / rank^1.2: 8 experts of 4096 -> 2 x 14336, gated, 8 rows each: 178 / 143, 187 / 156; 16: 180 /
+// 153, 207 / 189; 24: 186 / 215, 218 / 239; 8 of 14336 -> 4096, 16: 129 / 95, 135 / 113; 24: 134 / 116, 138 / 136; 32 of 1024 -> 4096, 16: 40 / 37, 63 / 44; 64 of 2048 -> 2 x 1024,
+// gated, 12: 58 / 58, 78 / 64; 16: 59 / 61, 81 / 71; 128 of 1024 -> 1024, 16: 40 / 39, 64 / 48.
+constexpr int kInt8FewRows = 16;
+namespace {
+DevRoute int8_route(const Int8Params &a) {
+    const TileShape tile = pick_rows_tile_estimate(a.rows_cap, a.n_expert, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.k_extent / 2, a.dtype);
+    if (a.rows_cap <= kInt8FewRows * a.n_expert && getenv("FMOE_GEMM_TILE") == nullptr) return {DevKernel::kSkinny, tile};
+    return {use_ring(tile, a.dtype) ? DevKernel::kRing : DevKernel::kTiles, tile};
 }
-int launch_int8_few(const Int8Params &a, hipStream_t stream) {
-    SkinnyParams sk{};
-    sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
-    sk.n_cols = a.n_cols; sk.k_extent = a.k_extent / 2; sk.activation = a.activation;
-    sk.ldw = a.ldw / 2; sk.ldx = a.ldx / 2; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
-    LinearForwardArgs like{};
-    like.in_feat = a.k_extent / 2; like.out_feat = (a.gated ? 2 : 1) * (int64_t)a.n_cols; like.dtype = a.dtype; like.dev_weights_once = true;
-    sk.weights_cached = caches_few_row_weights(like, a.n_expert);
-    ProfileScope prof(kProfGemmFwd, 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)like.out_feat, stream);
-    return launch_skinny_int8(sk, a.dtype, a.gated != 0, a.rows_cap, a.n_expert, stream);
+}  // namespace
+bool int8_in_pairs(const Int8Params &a) {
+    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && a.ldw <= (1 << 22) && a.ldx <= (1 << 22) && (a.bias == nullptr || aligned16(a.bias)) &&
+           aligned16(a.w_scale) && aligned16(a.y);
 }
-// The experts' product in 8-bit integers on the persistent kernel: results of 16 bits in rows of whole 16-byte pieces, where there are enough tiles for it.
-bool int8_ring_takes(const Int8Params &a) {
-    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && aligned16(a.y) && (a.bias == nullptr || aligned16(a.bias)) && aligned16(a.w_scale) &&
-           a.ldw <= (1 << 22) && use_ring(pick_rows_tile_estimate(a.rows_cap, a.n_expert, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.k_extent / 2, a.dtype), a.dtype);
+int64_t int8_workspace_bytes(const Int8Params &a) {
+    const DevRoute route = int8_route(a);
+    return route.kernel == DevKernel::kRing ? route_workspace_bytes(route, a.k_extent / 2, a.dtype) : 0;   // (the tiles' parts are added up as floats)
 }
-int64_t int8_ring_workspace_bytes(int64_t k_extent) { return route_workspace_bytes({DevKernel::kRing, kManyTiles}, k_extent / 2, FMOE_BF16); }
-int launch_int8_ring(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
-    RingParams prm{};
-    prm.P = a.w; prm.Q = a.x; prm.C = a.y; prm.bias = a.bias; prm.q_scale = a.x_scale; prm.p_scale = a.w_scale;
-    prm.ldp = a.ldw / 2; prm.ldq = a.ldx / 2; prm.ldc = a.n_cols;   // (pairs of integers)
-    prm.p_expert_stride = a.w_expert_stride / 2; prm.bias_expert_stride = (a.gated ? 2 : 1) * (int64_t)a.n_cols;
-    prm.n_cols = a.n_cols; prm.k_extent = a.k_extent / 2;
+int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const DevRoute route = int8_route(a);
+    const int64_t w_rows = (a.gated ? 2 : 1) * (int64_t)a.n_cols;
+    const double work = 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)w_rows;
     const int epi = a.gated ? kEpiInt8Gated : kEpiInt8;
+    if (route.kernel == DevKernel::kSkinny) {
+        SkinnyParams sk{};
+        sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
+        sk.n_cols = a.n_cols; sk.k_extent = a.k_extent / 2; sk.activation = a.activation;
+        sk.ldw = a.ldw / 2; sk.ldx = a.ldx / 2; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
+        ProfileScope prof(kProfGemmFwd, work, stream);
+        return launch_skinny_int8(sk, a.dtype, a.gated != 0, a.rows_cap, a.n_expert, stream);
+    }
     GatedArgs g{};
-    g.d = prm.k_extent; g.n_expert = a.n_expert; g.rows_cap = a.rows_cap; g.dtype = a.dtype; g.activation = a.activation; g.dev_tab = a.dev_tab;
-    g.workspace = workspace; g.workspace_bytes = workspace_bytes;
-    if (int rc = ring_of_table(prm, g, ring_cols(epi))) return rc;
-    ProfileScope prof(kProfGemmFwd, 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)prm.bias_expert_stride, stream);
-    return a.dtype == FMOE_BF16 ? launch_ring_bf16_int8(prm, epi, a.activation, stream) : launch_ring_f16_int8(prm, epi, a.activation, stream);
+    g.d = a.k_extent / 2; g.h = a.n_cols; g.n_expert = a.n_expert; g.rows_cap = a.rows_cap; g.dtype = a.dtype; g.activation = a.activation;
+    g.dev_tab = a.dev_tab; g.workspace = workspace; g.workspace_bytes = workspace_bytes;
+    auto fill = [&](auto &prm) {
+        prm.P = a.w; prm.Q = a.x; prm.C = a.y; prm.bias = a.bias; prm.q_scale = a.x_scale; prm.p_scale = a.w_scale;
+        prm.ldp = a.ldw / 2; prm.ldq = a.ldx / 2; prm.ldc = a.n_cols;   // (pairs of integers)
+        prm.p_expert_stride = a.w_expert_stride / 2; prm.bias_expert_stride = w_rows;
+        prm.n_cols = a.n_cols; prm.k_extent = a.k_extent / 2;
+    };
+    if (route.kernel == DevKernel::kRing) {
+        RingParams prm{};
+        fill(prm);
+        if (int rc = ring_of_table(prm, g, ring_cols(epi))) return rc;
+        ProfileScope prof(kProfGemmFwd, work, stream);
+        return a.dtype == FMOE_BF16 ? launch_ring_bf16_int8(prm, epi, a.activation, stream) : launch_ring_f16_int8(prm, epi, a.activation, stream);
+    }
+    GemmParams prm{};
+    g.workspace = nullptr;
+    if (int rc = tiles_of_table("int8 product", prm, g, route.tile, w_rows, g.d)) return rc;
+    fill(prm);
+    prm.profile_class = kProfGemmFwd; prm.profile_work = work;
+    return a.dtype == FMOE_BF16 ? launch_mfma_bf16_int8(prm, epi, stream) : launch_mfma_f16_int8(prm, epi, stream);
 }
 
 int grouped_bias_grad(const void *gy, void *gb, int64_t out_feat, int dtype, const int64_t *counts,

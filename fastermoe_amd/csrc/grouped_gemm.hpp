@@ -158,7 +158,8 @@ struct GatedArgs {
     int64_t workspace_bytes;
 };
 bool gated_forward_fused(const GatedArgs &a);   // (sizes alone where the tensors are null)
-int64_t gated_workspace_bytes(int64_t contraction, int dtype);
+int64_t gated_forward_workspace_bytes(const GatedArgs &a);
+int64_t gated_dgrad_workspace_bytes(const GatedArgs &a);
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream);
 bool gated_dgrad_fused(const GatedArgs &a);
 int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream);

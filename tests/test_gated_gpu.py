@@ -166,6 +166,16 @@ def test_large_enough_to_fill_the_card(dtype, act):
     _check(8200, 1032, 2072, 4, dtype, act, act in ("silu", "relu"), "tail" if act == "gelu" else "skewed")
 
 
+@pytest.mark.parametrize("dtype,tile", [(t, s) for t in (torch.bfloat16, torch.float16) for s in ("256x256", "128x256", "128x128", "128x128+", "64x128")]
+                         + [(torch.float32, s) for s in ("128x128", "128x128+", "64x64")], ids=str)
+@pytest.mark.parametrize("rows,d,h,kind", [(700, 200, 328, "skewed"), (300, 5120, 136, "tail"), (150, 72, 5128, "even")])
+def test_every_tile(monkeypatch, dtype, tile, rows, d, h, kind):
+    """Columns and contractions that end inside a tile and a slab; long contractions, whose last round of tiles is shared (forward; data gradient)."""
+    monkeypatch.setenv("FMOE_GEMM_TILE", tile)
+    for act in (ACTS if rows == 700 else ("silu",)):
+        _check(rows, d, h, 3, dtype, act, rows != 300, kind, seed=rows)
+
+
 def test_large_float32():
     _check(4100, 512, 1024, 8, torch.float32, "silu", True, "skewed")
 

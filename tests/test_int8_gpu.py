@@ -188,6 +188,16 @@ def test_large_enough_to_fill_the_card(dtype, act, gated):
     _check(8200, 1040, 4120, 4, dtype, act, gated, act in ("silu", "relu"), "tail" if act == "gelu" else "skewed")
 
 
+@pytest.mark.parametrize("tile", ["256x256", "128x256", "128x128", "128x128+", "64x128"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,d,out,kind", [(700, 400, 328, "skewed"), (300, 10250, 136, "tail"), (150, 150, 5128, "even")])
+def test_every_tile(monkeypatch, tile, gated, rows, d, out, kind):
+    monkeypatch.setenv("FMOE_GEMM_TILE", tile)
+    for act in (ACTS if rows == 700 else ("silu",)):
+        for dtype in (torch.bfloat16, torch.float16):
+            _check(rows, d, out, 3, dtype, act, gated, rows != 300, kind, seed=rows)
+
+
 def test_largest_sums():
     """Every product 127 * 127, as many as there may be."""
     d = 131072
