@@ -510,8 +510,10 @@ __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, cons
             ahead[1][i] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)(at + half), 0, 0);
         }
     };
-    request(0);
     by_gate_activation<false>(prm.activation, [&](auto act) {
+        // (asked for in here: ahead of the branches it would stay pending on a way past all of them, which the compiler believes in, and be waited for,
+        // with the slab loads, in the slab loop: 3393 us instead of 3130 for the large layer's data gradient)
+        request(0);
 #pragma unroll
         for (int n = 0; n < 2 * NY; ++n) {
 #pragma unroll
@@ -551,7 +553,8 @@ __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, cons
 }
 
 // Products in 8-bit integers: C = act(s_r t_c acc + bias), GATED: act(the first half's) * the second half's.  All rows of 32 columns at a time through the
-// wave's LDS, so that the scales and biases of no more columns than that are at hand (with all of them 250 registers were spilled).
+// wave's LDS, and the scales and biases of sixteen: with those of all columns 250 registers
+// were spilled, and waiting for them to come back drained the slab loads (65536 rows .. 2.0 us a slab instead of 1.4).
 template <typename T, bool GATED, int NY>
 __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                    int lane, int wm, int wn, int y0) {
@@ -572,35 +575,23 @@ __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const 
     const __amdgpu_buffer_rsrc_t bias_rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<Out *>(prm.bias ? (const Out *)prm.bias + p0 : nullptr), 0, prm.bias ? p_rows * 2 : 0, kRsrcFlags);
     const __amdgpu_buffer_rsrc_t row_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(prm.q_scale + tl.row0), 0, tl.q_valid * 4, kRsrcFlags);
-    struct Columns { u32x4 scale[H][2]; u32x2 bias[H][2]; };
-    auto request = [&](int pair, Columns &c) {
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int at = wave_col + 16 * (2 * pair + j) + 4 * hq + h * prm.n_cols;
-                c.scale[h][j] = __builtin_amdgcn_raw_buffer_load_b128(scale_rs, at * 4, 0, 0);
-                c.bias[h][j] = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, at * 2, 0, 0);
-            }
-    };
-    Columns cols[2];
-    uint32_t s[NY];
-#pragma unroll
-    for (int y = 0; y < NY; ++y) s[y] = __builtin_amdgcn_raw_buffer_load_b32(row_rs, (row0 + 16 * y + lb) * 4, 0, 0);
-    request(0, cols[0]);
     by_gate_activation<true>(prm.activation, [&](auto act) {
+        uint32_t s[NY];
+#pragma unroll
+        for (int y = 0; y < NY; ++y) s[y] = __builtin_amdgcn_raw_buffer_load_b32(row_rs, (row0 + 16 * y + lb) * 4, 0, 0);
 #pragma unroll
         for (int pair = 0; pair < X / 2; ++pair) {
-            if (pair + 1 < X / 2) request(pair + 1, cols[(pair + 1) & 1]);
-            const Columns &c = cols[pair & 1];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int x = 2 * pair + j;
+                u32x4 scale[H];
                 float add[H][4];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
+                    const int at = wave_col + 16 * x + 4 * hq + h * prm.n_cols;
+                    scale[h] = __builtin_amdgcn_raw_buffer_load_b128(scale_rs, at * 4, 0, 0);
                     alignas(8) Out b[4];
-                    *(u32x2 *)b = c.bias[h][j];
+                    *(u32x2 *)b = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, at * 2, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) add[h][i] = (float)b[i];
                 }
@@ -610,7 +601,7 @@ __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         auto sum = [&](int h) -> float {
-                            return fmaf((float)(int)__float_as_uint(acc[x + 4 * h][y][i]), __uint_as_float(s[y]) * __uint_as_float(c.scale[h][j][i]), add[h][i]);
+                            return fmaf((float)(int)__float_as_uint(acc[x + 4 * h][y][i]), __uint_as_float(s[y]) * __uint_as_float(scale[h][i]), add[h][i]);
                         };
                         float r = gate_act<true>(sum(0), act);
                         if constexpr (GATED) r *= sum(1);
