@@ -554,7 +554,7 @@ __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, cons
 
 // Products in 8-bit integers: C = act(s_r t_c acc + bias), GATED: act(the first half's) * the second half's.  All rows of 32 columns at a time through the
 // wave's LDS, and the scales and biases of sixteen: with those of all columns 250 registers
-// were spilled, and waiting for them to come back drained the slab loads (65536 rows .. 2.0 us a slab instead of 1.4).
+// were spilled, and waiting for them to come back drained the slab loads (32768 rows of 8 experts of 14336 -> 4096: 1866 us instead of 1400).
 template <typename T, bool GATED, int NY>
 __device__ __forceinline__ void ring_epilogue_int8(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                    int lane, int wm, int wn, int y0) {
