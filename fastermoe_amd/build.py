@@ -44,9 +44,8 @@ def _units():
         units.append(("gemm_skinny.hip", f"gemm_skinny_{name}.o", [f"-DFMOE_SKINNY={i}"]))
     for t, tname in GEMM_TYPES.items():
         for p, pname in GEMM_PRODUCTS.items():
-            if tname != "f32" or pname != "int8":
-                units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",
-                              [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))
+            units.append(("gemm_inst.hip", f"gemm_{tname}_{pname}.o",
+                          [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))
             if tname != "f32":
                 units.append(("gemm_ring_inst.hip", f"gemm_ring_{tname}_{pname}.o",
                               [f"-DFMOE_GEMM_TYPE={t}", f"-DFMOE_GEMM_PRODUCT={p}"]))

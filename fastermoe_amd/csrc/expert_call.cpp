@@ -50,10 +50,9 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
         const at::Tensor x = given.contiguous();
         const int64_t n = x.size(0), d = x.size(1), e = w1.size(0), h = w2.size(2);
         const int dtype = dtype_code(x), act = (int)activation;
-        const bool aligned = on_16_bytes(x) && on_16_bytes(w1) && on_16_bytes(b1) && on_16_bytes(w2) && on_16_bytes(b2);
         const at::Tensor y = at::empty({n, d}, x.options()), mid = at::empty({n, h}, x.options());
         const at::Tensor pre = keep ? at::empty({n, 2 * h}, x.options()) : at::Tensor();
-        const int64_t bytes = entry.gated_forward_bytes(e, n, d, h, dtype, act, keep, aligned);
+        const int64_t bytes = entry.gated_forward_bytes(e, n, d, h, dtype, act, keep, 1);
         const at::Tensor space = space_of(bytes, x);
         ok(entry.gated_forward(pointer(x), pointer(w1), pointer(b1), pointer(w2), pointer(b2), pointer(pre), pointer(mid), pointer(y), pointer(table),
                                nullptr, e, n, d, h, dtype, act, pointer(space), bytes, stream_of(x)));
@@ -186,12 +185,12 @@ PyObject *fmoe_expert_linear_int8(PyObject *, PyObject *const *args, Py_ssize_t 
     const int64_t e = weight.size(0), rows_w = weight.size(1), d = weight.size(2), whole_d = (d + 15) / 16 * 16;
     // (rows that have to be copied, and sizes that the library refuses, go through Python)
     const int64_t by_expert = weight.stride(0), by_row = weight.stride(1);
-    if (d > 131072 || by_row > (1 << 28) || (by_row > 0 && rows_w * by_row >= ((int64_t)1 << 31))) Py_RETURN_NONE;
+    if (d > 131072 || by_row > (1 << 22) || (by_row > 0 && rows_w * by_row >= ((int64_t)1 << 31))) Py_RETURN_NONE;
     if ((weight.stride(2) != 1 && d != 1) || by_row % 16 || by_row < whole_d || by_expert % 16 || by_expert < 0 || !on_16_bytes(weight) ||
         weight.storage_offset() + (e - 1) * by_expert + (rows_w - 1) * by_row + whole_d > (int64_t)weight.storage().nbytes())
         Py_RETURN_NONE;
     auto channels = [&](const at::Tensor &p, at::ScalarType type) {
-        return on_gpu(p) && p.device() == x.device() && p.scalar_type() == type && p.is_contiguous() && p.sizes() == at::IntArrayRef({e, rows_w});
+        return on_gpu(p) && p.device() == x.device() && p.scalar_type() == type && p.is_contiguous() && on_16_bytes(p) && p.sizes() == at::IntArrayRef({e, rows_w});
     };
     if (!channels(scale, at::kFloat) || (bias.defined() && !channels(bias, x.scalar_type())) || x.size(1) != d || (gated && rows_w % 2)) Py_RETURN_NONE;
     if (index.defined() && (!on_gpu(index) || index.device() != x.device() || index.scalar_type() != at::kLong || !index.is_contiguous() || index.numel() == 0))

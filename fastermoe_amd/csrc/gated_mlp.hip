@@ -161,15 +161,15 @@ GatedArgs gated_sizes(const Sizes &s) {
     a.d = s.d; a.h = s.h; a.n_expert = s.n_expert; a.rows_cap = s.rows; a.dtype = s.dtype; a.activation = s.activation; a.dev_tab = &some;
     return a;
 }
-Scratch forward_scratch(const Sizes &s, bool keeps_pre, bool aligned) {
-    const bool fused = aligned && gated_forward_fused(gated_sizes(s));
+Scratch forward_scratch(const Sizes &s, bool keeps_pre, bool table) {
+    const bool fused = table && gated_forward_fused(gated_sizes(s));
     return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)), 0,
                    std::max(fused ? gated_forward_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE, 0, 0),
                             fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0))};
 }
-Scratch backward_scratch(const Sizes &s, bool aligned) {
-    const bool fused = aligned && gated_dgrad_fused(gated_sizes(s));
+Scratch backward_scratch(const Sizes &s, bool table) {
+    const bool fused = table && gated_dgrad_fused(gated_sizes(s));
     const int64_t row = s.rows * s.h * dtype_bytes(s.dtype);
     return Scratch{round256(2 * row), fused ? 0 : round256(row),
                    std::max(fused ? gated_dgrad_workspace_bytes(gated_sizes(s))
@@ -225,11 +225,11 @@ Products products(const Sizes &s, const void *segment_table, const int64_t *coun
 using namespace fmoe;
 
 extern "C" int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,
-                                                          int activation, int keep, int aligned) {
+                                                          int activation, int keep, int table) {
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
     static const int64_t one = 0;
     if (rows < 1 || n_expert < 1 || check("fmoe_gated_mlp_forward", s, &one, nullptr) != FMOE_OK) return 0;
-    return forward_scratch(s, keep != 0, aligned != 0).total();
+    return forward_scratch(s, keep != 0, table != 0).total();
 }
 
 extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *pre, void *mid, void *y,
@@ -240,8 +240,7 @@ extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void 
     if (int rc = check(who, s, segment_table, expert_count_host)) return rc;
     if (rows == 0) return FMOE_OK;
     FMOE_REQUIRE(x && w1 && w2 && mid && y, "%s: NULL pointer", who);
-    const bool aligned = aligned16(x) && aligned16(w1) && aligned16(b1) && aligned16(w2) && aligned16(b2) && aligned16(pre) && aligned16(mid) && aligned16(y);
-    const Scratch need = forward_scratch(s, pre != nullptr, aligned && segment_table != nullptr);
+    const Scratch need = forward_scratch(s, pre != nullptr, segment_table != nullptr);
     if (need.total() > 0 && (workspace == nullptr || workspace_bytes < need.total() || !aligned16(workspace)))
         return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need.total());
     char *ws = (char *)workspace;
@@ -258,11 +257,11 @@ extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void 
 }
 
 extern "C" int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,
-                                                           int activation, int aligned) {
+                                                           int activation, int table) {
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
     static const int64_t one = 0;
     if (rows < 1 || n_expert < 1 || check("fmoe_gated_mlp_backward", s, &one, nullptr) != FMOE_OK) return 0;
-    return backward_scratch(s, aligned != 0).total();
+    return backward_scratch(s, table != 0).total();
 }
 
 extern "C" int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1, const void *w2, const void *pre, const void *mid,
@@ -272,10 +271,9 @@ extern "C" int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const 
     const char *who = "fmoe_gated_mlp_backward";
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
     if (int rc = check(who, s, segment_table, expert_count_host)) return rc;
-    const bool aligned = aligned16(grad_y) && aligned16(x) && aligned16(w1) && aligned16(w2) && aligned16(pre) && aligned16(mid);
     FMOE_REQUIRE((!grad_b1 || grad_w1) && (!grad_b2 || grad_w2), "%s: a bias gradient comes with its weight's", who);
     FMOE_REQUIRE(rows == 0 || (grad_y && x && w1 && w2 && pre && mid), "%s: NULL pointer", who);
-    const Scratch need = rows == 0 ? Scratch{0, 0, 0} : backward_scratch(s, aligned && segment_table != nullptr);
+    const Scratch need = rows == 0 ? Scratch{0, 0, 0} : backward_scratch(s, segment_table != nullptr);
     if (need.total() > 0 && (workspace == nullptr || workspace_bytes < need.total() || !aligned16(workspace)))
         return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need.total());
     char *ws = (char *)workspace;

@@ -1,6 +1,6 @@
 // One translation unit per (element type, product) of the grouped GEMM; the build
 // compiles this file with -DFMOE_GEMM_TYPE=<0 f32|1 bf16|2 f16> and -DFMOE_GEMM_PRODUCT=<0 fwd|1 dgrad|2 wgrad|3 gated forward|4 data gradient up to a gated
-// forward's product|5 forward in 8-bit integers, the type (1 or 2) its results'>.
+// forward's product|5 forward in 8-bit integers, the type its results'>.
 #include "gemm_kernel.hpp"
 
 #if FMOE_GEMM_TYPE == 0

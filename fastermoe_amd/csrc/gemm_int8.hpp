@@ -1,6 +1,6 @@
 // Interface of the experts' products in 8-bit integers.
 #pragma once
-#include "gemm_kernel.hpp"
+#include "grouped_gemm.hpp"
 
 namespace fmoe {
 
@@ -17,13 +17,11 @@ struct Int8Params {
     const int32_t *dev_tab;       // segtab layout
     int64_t n_expert, rows_cap;
     int dtype;                    // of y
-    int32_t tiles_n, map_off;     // set by the launch
 };
 
-// The kernels of 16-bit types with pairs of integers in their elements' places (grouped_gemm.hip): whether they take a product, their workspace (not needed, but used
-// to share a last round's tiles), the launch.
-bool int8_in_pairs(const Int8Params &a);
+// The kernels of 16-bit types with pairs of integers in their elements' places (grouped_gemm.hip): the workspace, which is not needed but used to share a last round's
+// tiles, and the launch.
 int64_t int8_workspace_bytes(const Int8Params &a);
-int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+int launch_int8(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
 }  // namespace fmoe

@@ -1478,7 +1478,29 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
             const int row = wave_m0 + i * kRows + sr, c = col + sc * kOut;
             return row < q_valid && c < col_end ? (uint32_t)(((int64_t)row * ld + c) * (int64_t)sizeof(Out)) : kOutOfRange;
         };
-        auto store = [&](int a, Out *dst, int col, int64_t ld) {
+        // (8-bit products have results of any number of columns, and then rows that begin anywhere)
+        const bool whole_rows = !IsInt8<T>::value || prm.n_cols * (int)sizeof(Out) % 16 == 0, fours = !IsInt8<T>::value || prm.n_cols % 4 == 0;
+        auto store = [&](int a, Out *dst, int col, int64_t ld) __attribute__((always_inline)) {
+            if (!whole_rows) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int row = wave_m0 + i * kRows + sr, c = col + sc * kOut;
+                    if (row >= q_valid || c >= col_end) continue;
+                    const u32x4 v = *piece(a, i);
+                    Out *to = dst + (int64_t)row * ld + c;
+                    if (c + kOut <= col_end) {
+                        __builtin_memcpy(to, &v, 16);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j + 1 < kOut; ++j)
+                            if (c + j < col_end) {
+                                if constexpr (kNarrow) ((uint16_t *)to)[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+                                else ((uint32_t *)to)[j] = v[j];
+                            }
+                    }
+                }
+                return;
+            }
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(dst, 0, (int)kOutOfRange, kRsrcFlags);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) __builtin_amdgcn_raw_buffer_store_b128(*piece(a, i), rs, (int)offset(i, col, ld), 0, 0);
@@ -1550,7 +1572,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
             for (int y = 0; y < TJ; ++y)
                 row_scale[y] = IsInt8<T>::value ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(row_rs, (wave_m0 + y * MB + lb) * 4, 0, 0)) : 1.f;
             // f(x, g, sums): four columns at a time, for all block rows: the products with scales and biases, of each half
-            auto each = [&](int pass, auto &&f) {
+            auto each = [&](int pass, auto &&f) __attribute__((always_inline)) {
 #pragma unroll
                 for (int x = 0; x < kXs; ++x)
 #pragma unroll
@@ -1560,7 +1582,10 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
                         for (int h = 0; h < H; ++h) {
                             const int c = col0 + pass * St::kCols + x * kBlockCols + g * 8 + hq * 4 + (h ? prm.n_cols : 0);
                             alignas(16) Out b[4];
-                            if constexpr (kNarrow) *(u32x2 *)b = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, c * (int)sizeof(Out), 0, 0);
+                            if (kNarrow && !fours) {   // (their biases may begin between two dwords)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) b[i] = prm.bias && c + i < p_rows ? ((const Out *)prm.bias)[p0 + c + i] : (Out)0.f;
+                            } else if constexpr (kNarrow) *(u32x2 *)b = __builtin_amdgcn_raw_buffer_load_b64(bias_rs, c * (int)sizeof(Out), 0, 0);
                             else *(u32x4 *)b = __builtin_amdgcn_raw_buffer_load_b128(bias_rs, c * (int)sizeof(Out), 0, 0);
                             u32x4 s = {};
                             if constexpr (IsInt8<T>::value) s = __builtin_amdgcn_raw_buffer_load_b128(scale_rs, c * 4, 0, 0);
@@ -2065,6 +2090,7 @@ FMOE_DECLARE_MFMA(launch_mfma_f16_dgated);
 FMOE_DECLARE_MFMA(launch_mfma_f32_dgated);
 FMOE_DECLARE_MFMA(launch_mfma_bf16_int8);
 FMOE_DECLARE_MFMA(launch_mfma_f16_int8);
+FMOE_DECLARE_MFMA(launch_mfma_f32_int8);
 // Feature sizes or pointers off the 16-byte grid, all three products (0 forward, 1 data gradient, 2 weight gradient):
 // 16-bit types in gemm_unaligned.hip, 32-bit ones and double precision (whatever its sizes) in gemm_any.hip
 int launch_mfma_unaligned(gemm::GemmParams &prm, int dtype, int product, int epilogue, hipStream_t stream);

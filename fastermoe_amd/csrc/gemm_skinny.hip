@@ -32,6 +32,7 @@ constexpr int kSkRows = 32;   // rows of a pass
 
 // one 16 x 16 block over 64 bytes of contraction; acc as for the 16 x 16 x 32 form
 template <typename T> __device__ __forceinline__ void mma_step(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<T>::mma(acc, w, x); }
+template <> __device__ __forceinline__ void mma_step<Int8Pair<float>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<Int8Pair<float>>::mma(acc, w, x); }
 template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u32x4 &w, const u32x4 &x) {
     // product j takes element j of every lane's four: contraction elements j, 4 + j, 8 + j and 12 + j of the step
 #pragma unroll
@@ -59,6 +60,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     typedef std::conditional_t<sizeof(T) == 2, u32x2, u32x4> Vec4;        // four elements
     constexpr bool kInt8 = IsInt8<T>::value;
     typedef typename Elem<T>::Out Out;                                // of the results
+    typedef std::conditional_t<sizeof(Out) == 2, u32x2, u32x4> OutVec4;
     constexpr int kCols = COL_BLOCKS * 16 / (HALVES ? 2 : 1);             // columns of a workgroup
     static_assert(!HALVES || (COL_BLOCKS >= 2 && sizeof(T) == 2), "halves: two blocks of columns or more");
     constexpr uint32_t kOutOfRange = 0x80000000u;
@@ -258,8 +260,8 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     if (prm.bias != nullptr) {
-                        alignas(8) Out b4[4];
-                        *(u32x2 *)b4 = *(const u32x2 *)((const Out *)prm.bias + channel + h * prm.n_cols);
+                        alignas(16) Out b4[4];
+                        *(OutVec4 *)b4 = *(const OutVec4 *)((const Out *)prm.bias + channel + h * prm.n_cols);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) add[h][i] = (float)b4[i];
                     }
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     const f32x4 sum[2] = {summed(n, y), HALVES ? summed(n + NH, y) : f32x4{}};
                     if (row >= rows) continue;
                     const float s = kInt8 ? prm.x_scale[first + row] : 1.f;
-                    alignas(8) Out pre[H][4], res[4];
+                    alignas(16) Out pre[H][4], res[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float v[H];
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                             else v[h] = sum[h][i] + add[h][i];
                             pre[h][i] = (Out)v[h];
                         }
-                        float r = gate_act<true>(v[0], prm.activation);
+                        float r = gate_act<sizeof(Out) == 2>(v[0], prm.activation);
                         if constexpr (HALVES) r *= v[1];
                         res[i] = (Out)r;
                     }
@@ -289,9 +291,9 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     if (HALVES && prm.aux != nullptr) {
 #pragma unroll
                         for (int h = 0; h < H; ++h)
-                            *(u32x2 *)((Out *)prm.aux + 2 * at - col + h * prm.n_cols) = *(const u32x2 *)pre[h];
+                            *(OutVec4 *)((Out *)prm.aux + 2 * at - col + h * prm.n_cols) = *(const OutVec4 *)pre[h];
                     }
-                    *(u32x2 *)((Out *)prm.y + at) = *(const u32x2 *)res;
+                    *(OutVec4 *)((Out *)prm.y + at) = *(const OutVec4 *)res;
                 }
             } else {
             // acc[n][y][i] is C(row 16 y + lb, column 16 n + 4 hq + i)
@@ -398,10 +400,12 @@ int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, in
 }
 #elif FMOE_SKINNY == 2
 int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
-    FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16, "grouped GEMM: dtype %d is not a 16-bit float type", dtype);
-    if (gated)
-        return dtype == FMOE_BF16 ? launch<Int8Pair<__bf16>, true>(prm, rows_cap, n_expert, stream) : launch<Int8Pair<_Float16>, true>(prm, rows_cap, n_expert, stream);
-    return dtype == FMOE_BF16 ? launch<Int8Pair<__bf16>>(prm, rows_cap, n_expert, stream) : launch<Int8Pair<_Float16>>(prm, rows_cap, n_expert, stream);
+    auto go = [&](auto pair) {
+        using Pair = decltype(pair);
+        return gated ? launch<Pair, true>(prm, rows_cap, n_expert, stream) : launch<Pair>(prm, rows_cap, n_expert, stream);
+    };
+    if (dtype == FMOE_F32) return go(Int8Pair<float>{});
+    return dtype == FMOE_BF16 ? go(Int8Pair<__bf16>{}) : go(Int8Pair<_Float16>{});
 }
 #else
 #error "FMOE_SKINNY must be 0, 1 or 2"

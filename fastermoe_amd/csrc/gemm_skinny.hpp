@@ -27,7 +27,7 @@ struct SkinnyParams {
 int launch_skinny(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 // gated forward, 16-bit types
 int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
-// rows and weights in 8-bit integers, k_extent in pairs, dtype of the results (16-bit types)
+// rows and weights in 8-bit integers, k_extent in pairs, dtype of the results, whose columns are a multiple of four
 int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 
 }  // namespace gemm

@@ -12,6 +12,7 @@
 // loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (8192 rows, 2047 x 4093:
 // 600 to 680 TFLOP/s).  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
 #include "gemm_kernel.hpp"
+#include "vec16.hpp"
 
 namespace fmoe {
 namespace {
@@ -46,8 +47,8 @@ template <typename T> __device__ __forceinline__ u32x4 load_part(const T *p, con
     return __builtin_bit_cast(u32x4, e);
 }
 
-// PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].
-template <typename T, int BM, int PSHAPE, int QSHAPE, int RAGGED>
+// PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].  EPI: kEpiGated, kEpiDGated, or 0: what the parameters say.
+template <typename T, int BM, int PSHAPE, int QSHAPE, int RAGGED, int EPI>
 __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(const GemmParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
     static_assert(QSHAPE == kKC || BM == 128, "the swizzle of a [contraction][index] slab needs rows of 256 bytes");
@@ -55,7 +56,16 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
     constexpr int NP = BN * 8 / kUaThreads, NQ = BM * 8 / kUaThreads;   // chunks per thread and slab
     constexpr int P_BYTES = BN * 128, Q_BYTES = BM * 128, STAGE = P_BYTES + Q_BYTES;
     constexpr bool kBiasGrad = RAGGED == kRaggedK;
+    constexpr bool kHalves = epi_halves(EPI);
+    constexpr int kCols = kHalves ? BN / 2 : BN;   // C columns of a tile
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+
+    if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
+        const int64_t there = ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)prm.dev_tab)[segtab::kRows];
+        if (prm.tail != nullptr && there < prm.tail_rows)
+            for (int64_t i = (int64_t)blockIdx.x * kUaThreads + threadIdx.x; i < (prm.tail_rows - there) * prm.tail_elems; i += (int64_t)gridDim.x * kUaThreads)
+                ((T *)prm.tail)[there * prm.tail_elems + i] = (T)0.f;
+    }
 
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave >> 1, wn = wave & 1, lb = lane & 15, hq = lane >> 4;
@@ -106,7 +116,7 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         seg_hi = dev ? dtab[segtab::kHeader + ei + 1] : prm.tab.seg[ei + 1];
     }
     const int expert = prm.tab.first_expert + ei;
-    const int n0 = nt * BN, p_valid = min(BN, prm.n_cols - n0);
+    const int n0 = nt * kCols, p_valid = min(kCols, prm.n_cols - n0);
     int K, q_valid, m0 = 0;
     const T *P, *Q;
     int64_t c_off;
@@ -152,6 +162,14 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         }
     };
     set_offsets(PSHAPE, p_off, NP, prm.ldp, p_valid);
+    if constexpr (kHalves) {
+        // 32 rows of the gate's weights, the same 32 of the linear half's, to each pair of waves
+#pragma unroll
+        for (int it = 0; it < NP; ++it) {
+            const int r = chunk_index(kKC, it), col = (r >> 6) * 32 + (r & 31);
+            p_off[it] = ((int64_t)min(col, p_valid - 1) + ((r >> 5) & 1 ? prm.n_cols : 0)) * prm.ldp + (t & 7) * 8;
+        }
+    }
     set_offsets(QSHAPE, q_off, NQ, prm.ldq, q_valid);
     auto fetch = [&](int shape, u32x4 *dst, int n, const T *base, const int64_t *off, int64_t ld, int valid, int extent,
                      int row_elems, int k0) {
@@ -245,6 +263,105 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
     }
     __syncthreads();
 
+    auto wave_sync = [&]() {
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (EPI != 0) {
+        // Gated products: sixteen rows at a time, 64 columns of C (dg and du, from g and u), or 32 of each half, through 2 KiB of LDS per wave and matrix
+        constexpr int kWaveCols = kHalves ? 32 : 64, kPieces = kWaveCols / 8, kSteps = kPieces / 4, kRows = 64 / kPieces;
+        unsigned char *area = smem + wave * 4096;
+        const int io_r = lane / kPieces, io_c = lane % kPieces, wave_col = kWaveCols * wn;
+        auto at4 = [&](int a, int x) { return (u32x2 *)(area + a * 2048 + lb * (kPieces * 16) + (((2 * x + (hq >> 1)) ^ (lb & (kPieces - 1))) << 4) + (hq & 1) * 8); };
+        auto piece = [&](int a, int i) {
+            const int r = i * kRows + io_r;
+            return (u32x4 *)(area + a * 2048 + r * (kPieces * 16) + ((io_c ^ (r & (kPieces - 1))) << 4));
+        };
+        // this lane's eight elements of step i of block row y: row in the tile, columns left of its eight (0 or less: none)
+        auto row_of = [&](int y, int i) { return 16 * row_block(y) + i * kRows + io_r; };
+        const int left = p_valid - (wave_col + io_c * 8);
+        auto store = [&](int a, T *to, int64_t ld, int y) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (row_of(y, i) < q_valid && left > 0) store_some(to + (int64_t)row_of(y, i) * ld + wave_col + io_c * 8, *piece(a, i), left);
+        };
+        if constexpr (kHalves) {
+            const T *bias = prm.bias ? (const T *)prm.bias + (int64_t)expert * prm.bias_expert_stride + n0 : nullptr;
+            float bias_of[TI][4];
+#pragma unroll
+            for (int x = 0; x < TI; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int col = wave_col + 16 * (x & 1) + 4 * hq + i;
+                    bias_of[x][i] = bias != nullptr && col < p_valid ? (float)bias[col + (x < 2 ? 0 : prm.n_cols)] : 0.f;
+                }
+            T *pre = prm.aux ? (T *)prm.aux + 2 * c_off - n0 : nullptr;
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) {
+                if (16 * row_block(y) >= q_valid) break;
+#pragma unroll
+                for (int kind = 0; kind < 3; ++kind) {   // the gate's half, the linear one, the result
+                    if (kind < 2 && pre == nullptr) continue;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        alignas(8) T v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float g = acc[x][y][i] + bias_of[x][i], u = acc[x + 2][y][i] + bias_of[x + 2][i];
+                            v[i] = (T)(kind == 0 ? g : kind == 1 ? u : gate_act<true>(g, prm.activation) * u);
+                        }
+                        *at4(0, x) = *(const u32x2 *)v;
+                    }
+                    wave_sync();
+                    if (kind == 2) store(0, (T *)prm.C + c_off, prm.ldc, y);
+                    else store(0, pre + (kind ? prm.n_cols : 0), 2 * prm.ldc, y);
+                    wave_sync();
+                }
+            }
+        } else {
+            const T *in = (const T *)prm.aux + c_off;
+            T *out = (T *)prm.C + c_off;
+            auto load = [&](u32x4 (&v)[2][kSteps], int y) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i)
+                        v[a][i] = row_of(y, i) < q_valid && left > 0 ? load_some(in + (int64_t)row_of(y, i) * prm.ldc + wave_col + io_c * 8 + a * prm.n_cols, left)
+                                                                    : u32x4{0u, 0u, 0u, 0u};
+            };
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) {
+                if (16 * row_block(y) >= q_valid) break;
+                u32x4 held[2][kSteps];
+                load(held, y);
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) *piece(a, i) = held[a][i];
+                wave_sync();
+#pragma unroll
+                for (int x = 0; x < TI; ++x) {
+                    alignas(8) T g[4], u[4];
+                    *(u32x2 *)g = *at4(0, x);
+                    *(u32x2 *)u = *at4(1, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const ActTerms terms = gate_terms<true>((float)g[i], prm.activation);
+                        const float dm = acc[x][y][i];
+                        g[i] = (T)(dm * (float)u[i] * terms.slope);
+                        u[i] = (T)(dm * terms.value);
+                    }
+                    *at4(0, x) = *(const u32x2 *)g;
+                    *at4(1, x) = *(const u32x2 *)u;
+                }
+                wave_sync();
+                store(0, out, prm.ldc, y);
+                store(1, out + prm.n_cols, prm.ldc, y);
+                wave_sync();
+            }
+        }
+        return;
+    }
     // -- epilogue: acc[x][y][i] is C(row 16 row_block(y) + lb, column 64 wn + 16 x + 4 hq + i); sixteen rows at a
     // time through 2 KiB of LDS per wave and out as 128-byte row pieces
     unsigned char *stg = smem + wave * 2048;
@@ -262,10 +379,6 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
             const int col = 64 * wn + 16 * x + 4 * hq + i;
             bias_of[x][i] = bias != nullptr && col < p_valid ? (float)bias[col] : 0.f;
         }
-    auto wave_sync = [&]() {
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
     auto store_rows = [&](T *to, int y) {
         wave_sync();
 #pragma unroll
@@ -319,10 +432,10 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
 #endif
 }
 
-template <typename T, int BM, int PS, int QS, int RG>
+template <typename T, int BM, int PS, int QS, int RG, int EPI = 0>
 int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     prm.epilogue = epilogue;
-    prm.tiles_n = (int)ceil_div(prm.n_cols, kUaBN);
+    prm.tiles_n = (int)ceil_div(prm.n_cols, epi_halves(EPI) ? kUaBN / 2 : kUaBN);
     prm.tiles_m = RG == kRaggedRows ? 0 : (int)ceil_div(prm.n_rows, BM);
     int64_t row_tiles = (int64_t)prm.tab.n * prm.tiles_m;
     if (RG == kRaggedRows && prm.dev_tab != nullptr) {
@@ -336,7 +449,7 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     if (total == 0) return FMOE_OK;
     prm.total_tiles = (int)total;
     ProfileScope prof(prm.profile_class, prm.profile_work, stream);
-    grouped_gemm_unaligned_kernel<T, BM, PS, QS, RG><<<(unsigned)((total + 7) / 8 * 8), kUaThreads, 0, stream>>>(prm);
+    grouped_gemm_unaligned_kernel<T, BM, PS, QS, RG, EPI><<<(unsigned)((total + 7) / 8 * 8), kUaThreads, 0, stream>>>(prm);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
 }
@@ -344,6 +457,12 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
 template <typename T> int launch_unaligned_typed(GemmParams &prm, int product, int epilogue, hipStream_t stream) {
     const bool low = prm.block_m == 64;
     switch (product) {
+        case 3:
+            return low ? launch_unaligned_tiles<T, 64, kKC, kKC, kRaggedRows, kEpiGated>(prm, epilogue, stream)
+                       : launch_unaligned_tiles<T, 128, kKC, kKC, kRaggedRows, kEpiGated>(prm, epilogue, stream);
+        case 4:
+            return low ? launch_unaligned_tiles<T, 64, kMC, kKC, kRaggedRows, kEpiDGated>(prm, epilogue, stream)
+                       : launch_unaligned_tiles<T, 128, kMC, kKC, kRaggedRows, kEpiDGated>(prm, epilogue, stream);
         case 0:
             return low ? launch_unaligned_tiles<T, 64, kKC, kKC, kRaggedRows>(prm, epilogue, stream)
                        : launch_unaligned_tiles<T, 128, kKC, kKC, kRaggedRows>(prm, epilogue, stream);
@@ -356,7 +475,7 @@ template <typename T> int launch_unaligned_typed(GemmParams &prm, int product, i
 
 }  // namespace
 
-// product: 0 forward, 1 data gradient, 2 weight gradient (with the bias gradient).  Ragged rows: prm.block_m (64 or 128)
+// product: 0 forward, 1 data gradient, 2 weight gradient (with the bias gradient), 3 gated forward, 4 data gradient up to a gated forward's product.  Ragged rows: prm.block_m (64 or 128)
 // is the tile height, for which prm.tab was filled in (a device table serves both).
 int launch_mfma_unaligned(gemm::GemmParams &prm, int dtype, int product, int epilogue, hipStream_t stream) {
     if (dtype == FMOE_BF16) return launch_unaligned_typed<__bf16>(prm, product, epilogue, stream);

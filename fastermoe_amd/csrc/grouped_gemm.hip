@@ -765,8 +765,13 @@ int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts, int64_
 }
 
 namespace {
-// Few rows per expert: as for a plain product of as many columns.
-bool gated_forward_few(const GatedArgs &a) { return is_16bit(a.dtype) && use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype); }
+// Few rows per expert: as for a plain product of as many columns, and up to sixteen rows per expert where the weights make at most two rounds of 128 x 128 tiles.
+// us on the tiles and there, weights from memory, 16 rows each, even counts / shares 1 / rank^1.2: 64 experts of 2048 -> 2 x 1024: 175 / 147, 211 / 186; 16 of
+// 2048 -> 2 x 2048: 90 / 73, 93 / 84; more weights, 8 of 4096 -> 2 x 14336: 470 / 450, 480 / 520.
+bool gated_forward_few(const GatedArgs &a) {
+    if (!is_16bit(a.dtype) || getenv("FMOE_GEMM_TILE")) return false;
+    return use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype) || (a.rows_cap <= 16 * a.n_expert && a.n_expert * ceil_div(2 * a.h, 128) <= 1024);
+}
 TileShape gated_forward_tile(const GatedArgs &a) { return pick_rows_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h, a.d, a.dtype); }
 TileShape gated_dgrad_tile(const GatedArgs &a) { return pick_rows_tile_estimate(a.rows_cap, a.n_expert, a.h, a.d, a.dtype); }
 DevRoute gated_route(const GatedArgs &a, const TileShape &tile) { return {use_ring(tile, a.dtype) ? DevKernel::kRing : DevKernel::kTiles, tile}; }
@@ -777,11 +782,13 @@ bool gated_sizes_fit(const GatedArgs &a) {
            (2 * a.h + 256) * a.d * eb < ((int64_t)1 << 31) && 2 * a.h * eb <= (1 << 22);
 }
 }  // namespace
-// (float32 with few rows per expert: the decoding kernel's plain product and a kernel for the activation)
+// (16-bit types that the aligned kernels do not take go to gemm_unaligned.hip; float32 with few rows per expert: the decoding kernel's plain product and a
+// kernel for the activation)
 bool gated_forward_fused(const GatedArgs &a) {
-    return gated_sizes_fit(a) && (is_16bit(a.dtype) || !use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype));
+    if (is_16bit(a.dtype)) return a.dev_tab != nullptr;
+    return gated_sizes_fit(a) && !use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype);
 }
-bool gated_dgrad_fused(const GatedArgs &a) { return gated_sizes_fit(a); }
+bool gated_dgrad_fused(const GatedArgs &a) { return is_16bit(a.dtype) ? a.dev_tab != nullptr : gated_sizes_fit(a); }
 int64_t gated_forward_workspace_bytes(const GatedArgs &a) {
     return gated_forward_few(a) ? 0 : route_workspace_bytes(gated_route(a, gated_forward_tile(a)), a.d, a.dtype);
 }
@@ -812,7 +819,8 @@ int tiles_of_table(const char *who, GemmParams &prm, const GatedArgs &a, const T
 }
 }  // namespace
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
-    if (gated_forward_few(a)) {
+    const bool fits = gated_sizes_fit(a);
+    if (fits && gated_forward_few(a)) {
         SkinnyParams sk{};
         sk.w = a.w; sk.x = a.in; sk.bias = a.bias; sk.y = a.out; sk.aux = a.pre; sk.dev_tab = a.dev_tab;
         sk.n_cols = (int)a.h; sk.k_extent = (int)a.d; sk.activation = a.activation;
@@ -823,8 +831,8 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
         ProfileScope prof(kProfGemmFwd, 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
         return launch_skinny_gated(sk, a.dtype, a.rows_cap, a.n_expert, stream);
     }
-    const TileShape tile = gated_forward_tile(a);
-    if (!use_ring(tile, a.dtype)) {
+    const TileShape tile = fits ? gated_forward_tile(a) : unaligned_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h);
+    if (!fits || !use_ring(tile, a.dtype)) {
         GemmParams prm{};
         if (int rc = tiles_of_table("gated forward", prm, a, tile, 2 * a.h, a.d)) return rc;
         prm.profile_class = kProfGemmFwd; prm.profile_work = 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h;
@@ -832,6 +840,7 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
         prm.ldp = a.d; prm.ldq = a.d; prm.ldc = a.h;
         prm.p_expert_stride = 2 * a.h * a.d; prm.bias_expert_stride = 2 * a.h;
         prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+        if (!fits) return launch_mfma_unaligned(prm, a.dtype, 3, kEpiGated, stream);
         if (a.dtype == FMOE_F32) return launch_mfma_f32_gated(prm, kEpiGated, stream);
         return a.dtype == FMOE_BF16 ? launch_mfma_bf16_gated(prm, kEpiGated, stream) : launch_mfma_f16_gated(prm, kEpiGated, stream);
     }
@@ -845,8 +854,9 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
     return a.dtype == FMOE_BF16 ? launch_ring_bf16_gated(prm, kEpiGated, a.activation, stream) : launch_ring_f16_gated(prm, kEpiGated, a.activation, stream);
 }
 int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
-    const TileShape tile = gated_dgrad_tile(a);
-    if (!use_ring(tile, a.dtype)) {
+    const bool fits = gated_sizes_fit(a);
+    const TileShape tile = fits ? gated_dgrad_tile(a) : unaligned_tile_estimate(a.rows_cap, a.n_expert, a.h);
+    if (!fits || !use_ring(tile, a.dtype)) {
         GemmParams prm{};
         if (int rc = tiles_of_table("gated dgrad", prm, a, tile, a.h, a.d)) return rc;
         prm.profile_class = kProfGemmDgrad; prm.profile_work = 2.0 * (double)a.rows_cap * (double)a.d * (double)a.h;
@@ -854,6 +864,7 @@ int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
         prm.ldp = a.h; prm.ldq = a.d; prm.ldc = 2 * a.h;
         prm.p_expert_stride = a.h * a.d;
         prm.n_cols = (int)a.h; prm.k_extent = (int)a.d;
+        if (!fits) return launch_mfma_unaligned(prm, a.dtype, 4, kEpiDGated, stream);
         if (a.dtype == FMOE_F32) return launch_mfma_f32_dgated(prm, kEpiDGated, stream);
         return a.dtype == FMOE_BF16 ? launch_mfma_bf16_dgated(prm, kEpiDGated, stream) : launch_mfma_f16_dgated(prm, kEpiDGated, stream);
     }
@@ -867,28 +878,24 @@ int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream) {
     return a.dtype == FMOE_BF16 ? launch_ring_bf16_dgated(prm, kEpiDGated, a.activation, stream) : launch_ring_f16_dgated(prm, kEpiDGated, a.activation, stream);
 }
 
-// The experts' product in 8-bit integers: 16-bit results in rows of whole 16-byte pieces go to the kernels of 16-bit types, pairs of integers in their elements'
-// places, by the same rules; but for few rows per expert (at most 16 on average), whose kernel carries on further than with twice the bytes.
+// The experts' product in 8-bit integers goes to the kernels of 16-bit types, pairs of integers in their elements' places, by the same rules; but for few rows per expert (at most
+// 16 on average), whose kernel carries on further than with twice the bytes.
 // us on 128 x 128 tiles and there, weights from memory, even counts / shares 1 / rank^1.2: 8 experts of 4096 -> 2 x 14336, gated, 8 rows each: 178 / 143, 187 / 156; 16: 180 /
 // 153, 207 / 189; 24: 186 / 215, 218 / 239; 8 of 14336 -> 4096, 16: 129 / 95, 135 / 113; 24: 134 / 116, 138 / 136; 32 of 1024 -> 4096, 16: 40 / 37, 63 / 44; 64 of 2048 -> 2 x 1024,
 // gated, 12: 58 / 58, 78 / 64; 16: 59 / 61, 81 / 71; 128 of 1024 -> 1024, 16: 40 / 39, 64 / 48.
 constexpr int kInt8FewRows = 16;
 namespace {
 DevRoute int8_route(const Int8Params &a) {
-    const TileShape tile = pick_rows_tile_estimate(a.rows_cap, a.n_expert, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.k_extent / 2, a.dtype);
-    if (a.rows_cap <= kInt8FewRows * a.n_expert && getenv("FMOE_GEMM_TILE") == nullptr) return {DevKernel::kSkinny, tile};
-    return {use_ring(tile, a.dtype) ? DevKernel::kRing : DevKernel::kTiles, tile};
+    const TileShape tile = pick_rows_tile_estimate(a.rows_cap, a.n_expert, (a.gated ? 2 : 1) * (int64_t)a.n_cols, a.k_extent / 2, FMOE_BF16);
+    if (a.rows_cap <= kInt8FewRows * a.n_expert && a.n_cols % 4 == 0 && getenv("FMOE_GEMM_TILE") == nullptr) return {DevKernel::kSkinny, tile};
+    return {use_ring(tile, FMOE_BF16) && is_16bit(a.dtype) && a.n_cols % 8 == 0 ? DevKernel::kRing : DevKernel::kTiles, tile};
 }
 }  // namespace
-bool int8_in_pairs(const Int8Params &a) {
-    return is_16bit(a.dtype) && a.n_cols % 8 == 0 && a.ldw <= (1 << 22) && a.ldx <= (1 << 22) && (a.bias == nullptr || aligned16(a.bias)) &&
-           aligned16(a.w_scale) && aligned16(a.y);
-}
 int64_t int8_workspace_bytes(const Int8Params &a) {
     const DevRoute route = int8_route(a);
-    return route.kernel == DevKernel::kRing ? route_workspace_bytes(route, a.k_extent / 2, a.dtype) : 0;   // (the tiles' parts are added up as floats)
+    return route.kernel == DevKernel::kRing ? route_workspace_bytes(route, a.k_extent / 2, FMOE_BF16) : 0;   // (the tiles' parts are added up as floats)
 }
-int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+int launch_int8(const Int8Params &a, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
     const DevRoute route = int8_route(a);
     const int64_t w_rows = (a.gated ? 2 : 1) * (int64_t)a.n_cols;
     const double work = 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)w_rows;
@@ -902,7 +909,7 @@ int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_by
         return launch_skinny_int8(sk, a.dtype, a.gated != 0, a.rows_cap, a.n_expert, stream);
     }
     GatedArgs g{};
-    g.d = a.k_extent / 2; g.h = a.n_cols; g.n_expert = a.n_expert; g.rows_cap = a.rows_cap; g.dtype = a.dtype; g.activation = a.activation;
+    g.d = a.k_extent / 2; g.h = a.n_cols; g.n_expert = a.n_expert; g.rows_cap = a.rows_cap; g.dtype = FMOE_BF16; g.activation = a.activation;
     g.dev_tab = a.dev_tab; g.workspace = workspace; g.workspace_bytes = workspace_bytes;
     auto fill = [&](auto &prm) {
         prm.P = a.w; prm.Q = a.x; prm.C = a.y; prm.bias = a.bias; prm.q_scale = a.x_scale; prm.p_scale = a.w_scale;
@@ -922,6 +929,7 @@ int launch_int8_pairs(const Int8Params &a, void *workspace, int64_t workspace_by
     if (int rc = tiles_of_table("int8 product", prm, g, route.tile, w_rows, g.d)) return rc;
     fill(prm);
     prm.profile_class = kProfGemmFwd; prm.profile_work = work;
+    if (a.dtype == FMOE_F32) return launch_mfma_f32_int8(prm, epi, stream);
     return a.dtype == FMOE_BF16 ? launch_mfma_bf16_int8(prm, epi, stream) : launch_mfma_f16_int8(prm, epi, stream);
 }
 

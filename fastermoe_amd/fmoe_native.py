@@ -896,10 +896,6 @@ def _exact_table(table, n_expert, rows, device):
     return table
 
 
-def _all_aligned(*tensors):
-    return all(t is None or t.data_ptr() % 16 == 0 for t in tensors)
-
-
 def _gated_args(x, w1, b1, w2, b2):
     """Checks of a gated block's tensors; the code of their type and ``(experts, rows, d_model, d_hidden)``."""
     dt = _rows("x", x)
@@ -941,7 +937,7 @@ def gated_mlp_forward(x, w1, b1, w2, b2, activation, table=None, expert_count=No
     lib = _lib.load()
     with _on(x.device):
         ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep),
-                                                                       int(table is not None and _all_aligned(x, w1, b1, w2, b2))), x.device)
+                                                                       int(table is not None)), x.device)
         check(lib.fmoe_gated_mlp_forward(_ptr(x), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(pre), _ptr(mid), _ptr(y), seg, cnt, e, n, d, h, dt,
                                          activation, _ptr(ws), ws.numel(), _stream(x)))
     return y, pre, mid if keep else None
@@ -964,7 +960,7 @@ def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table=None, expe
     lib = _lib.load()
     with _on(x.device):
         ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation,
-                                                                        int(table is not None and _all_aligned(grad_y, x, w1, w2, pre, mid))), x.device)
+                                                                        int(table is not None)), x.device)
         check(lib.fmoe_gated_mlp_backward(_ptr(grad_y), _ptr(x), _ptr(w1), _ptr(w2), _ptr(pre), _ptr(mid), _ptr(grad_x), _ptr(grad_w1), _ptr(grad_b1),
                                           _ptr(grad_w2), _ptr(grad_b2), seg, cnt, e, n, d, h, dt, activation, _ptr(ws), ws.numel(), _stream(x)))
     return grad_x, grad_w1 if want_w1 else None, grad_b1, grad_w2 if want_w2 else None, grad_b2
@@ -1014,11 +1010,16 @@ def int8_layout(weight):
     whole = -(-d // INT8_ROW_BYTES) * INT8_ROW_BYTES
     by_expert, by_row, by_elem = weight.stride()
     last = weight.storage_offset() + (e - 1) * by_expert + (out - 1) * by_row + whole   # (what a row's last piece may read up to)
-    if ((by_elem == 1 or d == 1) and by_row % INT8_ROW_BYTES == 0 and by_row >= whole and by_expert % INT8_ROW_BYTES == 0
+    if ((by_elem == 1 or d == 1) and by_row % INT8_ROW_BYTES == 0 and whole <= by_row <= 1 << 22 and by_expert % INT8_ROW_BYTES == 0
             and weight.data_ptr() % 16 == 0 and last <= weight.untyped_storage().nbytes()):
         return weight
     held = torch.empty(e, out, whole, dtype=torch.int8, device=weight.device)[:, :, :d]
     return held.copy_(weight)
+
+
+def _on_16_bytes(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _int8_weights(weight, scale, device):
@@ -1036,7 +1037,7 @@ def _int8_weights(weight, scale, device):
         raise ValueError(f"weight_scale must be {(e, out)}, got {tuple(scale.shape)}")
     weight = int8_layout(weight)
     by_expert, by_row, _ = weight.stride()
-    return weight, by_expert, by_row, scale.contiguous()
+    return weight, by_expert, by_row, _on_16_bytes(scale)
 
 
 def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_NONE, gated=False, row_index=None, index_div=1):
@@ -1065,6 +1066,7 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
         _near("bias", _dev("bias", bias, x.dtype), x.device)
         if tuple(bias.shape) != (e, out):
             raise ValueError(f"bias must be {(e, out)}, got {tuple(bias.shape)}")
+        bias = _on_16_bytes(bias)
     n = x.shape[0] if row_index is None else row_index.numel()
     out = out // 2 if gated else out
     _exact_table(table, e, n, x.device)

@@ -744,11 +744,11 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
  * says and with tensors on 16 bytes), or else from expert_count_host (any sizes).
  * FMOE_F32 / FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
  * The workspace (on 16 bytes) belongs to the call until it has run.  Its size: keep
- * not 0 where pre is given, aligned not 0 where all tensors begin on 16 bytes. */
+ * not 0 where pre is given, table not 0 where a segment table is. */
 int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                int64_t d_model, int64_t d_hidden,
                                                int dtype, int activation, int keep,
-                                               int aligned);
+                                               int table);
 int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
                            const void *w2, const void *b2, void *pre, void *mid,
                            void *y, const void *segment_table,
@@ -763,7 +763,7 @@ int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
  * behind the experts'. */
 int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                 int64_t d_model, int64_t d_hidden,
-                                                int dtype, int activation, int aligned);
+                                                int dtype, int activation, int table);
 int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1,
                             const void *w2, const void *pre, const void *mid,
                             void *grad_x, void *grad_w1, void *grad_b1,
@@ -800,7 +800,8 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
  * a row can be read up to the next multiple of 16 bytes.  w_scale [E, rows of w]
  * float32, bias the same of y's type or NULL, y [rows_cap, out_feat] of dtype
  * (rows behind the experts' are left as they are).  The sums are exact; in_feat
- * is at most 131072, an expert's weights less than 2 GiB.  With a workspace (on
+ * is at most 131072, an expert's weights less than 2 GiB.  Tensors begin on 16
+ * bytes.  With a workspace (on
  * 16 bytes; none: NULL) of fmoe_linear_int8_workspace_bytes a last round of tiles
  * that fills a small part of the chip is shared along the contraction; the
  * results are the same bits. */

@@ -176,6 +176,20 @@ def test_every_tile(monkeypatch, dtype, tile, rows, d, h, kind):
         _check(rows, d, h, 3, dtype, act, rows != 300, kind, seed=rows)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("rows,d,h,experts", [(1, 70, 63, 2), (70, 65, 64, 1), (140, 64, 65, 2), (300, 33, 130, 3), (6000, 131, 1301, 2)])
+def test_every_column_off_the_grid(dtype, rows, d, h, experts):
+    """Rows that begin anywhere, tiles of both heights, every activation."""
+    for act in ACTS:
+        _check(rows, d, h, experts, dtype, act, act != "none", "tail" if act == "relu" else "skewed", seed=rows)
+
+
+@pytest.mark.parametrize("rows", [13, 16, 47, 48, 49])
+def test_few_rows(rows):
+    _check(rows, 512, 1024, 3, torch.bfloat16, "silu", True, "skewed", seed=rows)
+    _check(rows, 512, 1024, 3, torch.float16, "gelu", False, "tail", seed=rows)
+
+
 def test_large_float32():
     _check(4100, 512, 1024, 8, torch.float32, "silu", True, "skewed")
 

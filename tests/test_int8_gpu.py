@@ -198,6 +198,23 @@ def test_every_tile(monkeypatch, tile, gated, rows, d, out, kind):
             _check(rows, d, out, 3, dtype, act, gated, rows != 300, kind, seed=rows)
 
 
+@pytest.mark.parametrize("tile", ["256x256", "128x256", "128x128", "128x128+", "64x128"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("out", [320, 331, 332, 334])
+def test_every_tile_and_columns_of_any_number(monkeypatch, tile, gated, out):
+    """Results in rows of whole 16-byte pieces, of whole groups of four columns, and of neither."""
+    monkeypatch.setenv("FMOE_GEMM_TILE", tile)
+    for dtype in DTYPES:
+        _check(430, 270, out, 3, dtype, "gelu" if out % 4 else "none", gated, out != 334, "skewed", seed=out)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_few_rows_of_float32(gated):
+    for rows in (1, 3, 16, 40, 64):
+        for out in (132, 130):
+            _check(rows, 300, out, 4, torch.float32, "silu", gated, rows != 16, "tail", seed=rows)
+
+
 def test_largest_sums():
     """Every product 127 * 127, as many as there may be."""
     d = 131072
