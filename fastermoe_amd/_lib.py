@@ -108,7 +108,8 @@ SIGNATURES = {
     "fmoe_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int, _int]),
     "fmoe_gated_mlp_backward": (_int, [_vp] * 13 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
     "fmoe_quantize_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
-    "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp, _i64, _vp]),
+    "fmoe_linear_int8_rounds_rows": (_int, [_i64, _i64, _i64, _i64, _int, _int]),
+    "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp, _i64, _vp]),
     "fmoe_linear_int8_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int]),
     "fmoe_layer_sizes": (_int, [_i64, _i64, _i64, _i64, _i64, _int, _int, _int, _int, _vp]),
     "fmoe_layer_forward": (_int, [_vp] * 17 + [_i64] * 5 + [_int] * 4 + [_vp, _i64, _vp]),
@@ -178,7 +179,8 @@ def load_layer_call():
                                          "fmoe_balance_loss_workspace_bytes", "fmoe_act_checkpoint_forward", "fmoe_act_checkpoint_backward")))
         module.bind_expert(*map(address, ("fmoe_last_error", "fmoe_segment_table_bytes", "fmoe_linear_dev_supported",
                                           "fmoe_gated_mlp_forward_workspace_bytes", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward_workspace_bytes",
-                                          "fmoe_gated_mlp_backward", "fmoe_quantize_rows", "fmoe_linear_int8_workspace_bytes", "fmoe_linear_int8")))
+                                          "fmoe_gated_mlp_backward", "fmoe_quantize_rows", "fmoe_linear_int8_workspace_bytes", "fmoe_linear_int8",
+                                          "fmoe_linear_int8_rounds_rows")))
         _layer_call = module
     return _layer_call
 

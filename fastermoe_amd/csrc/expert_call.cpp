@@ -27,8 +27,9 @@ struct Entries {
     decltype(&fmoe_quantize_rows) quantize_rows;
     decltype(&fmoe_linear_int8_workspace_bytes) int8_bytes;
     decltype(&fmoe_linear_int8) linear_int8;
+    decltype(&fmoe_linear_int8_rounds_rows) int8_rounds_rows;
 } entry = {};
-constexpr int kEntries = 10;
+constexpr int kEntries = 11;
 
 void ok(int rc) { TORCH_CHECK(rc == FMOE_OK, "libfmoe_hip error ", rc, ": ", entry.last_error()); }
 bool on_16_bytes(const at::Tensor &t) { return !t.defined() || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
@@ -118,7 +119,7 @@ bool activation_taken(long a) { return a == FMOE_ACT_NONE || a == FMOE_ACT_RELU 
 
 PyObject *fmoe_expert_bind(PyObject *, PyObject *args) {
     unsigned long long a[kEntries];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9])) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10])) return nullptr;
     auto set = [&](auto &fn, int i) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(static_cast<uintptr_t>(a[i])); };
     set(entry.last_error, 0);
     set(entry.table_bytes, 1);
@@ -130,6 +131,7 @@ PyObject *fmoe_expert_bind(PyObject *, PyObject *args) {
     set(entry.quantize_rows, 7);
     set(entry.int8_bytes, 8);
     set(entry.linear_int8, 9);
+    set(entry.int8_rounds_rows, 10);
     Py_RETURN_NONE;
 }
 
@@ -205,14 +207,19 @@ PyObject *fmoe_expert_linear_int8(PyObject *, PyObject *const *args, Py_ssize_t 
         const int dtype = dtype_code(x);
         y = at::empty({n, out}, x.options());
         // the rows' integers, their scales, and what the product wants, in one piece
-        const int64_t q_bytes = n * whole_d, s_bytes = (n * 4 + 15) / 16 * 16, ws_bytes = entry.int8_bytes(e, n, d, out, (int)gated, dtype);
+        const bool round_first = entry.int8_rounds_rows(e, n, d, out, (int)gated, dtype) == 0;
+        const int64_t q_bytes = round_first ? n * whole_d : 0, s_bytes = round_first ? (n * 4 + 15) / 16 * 16 : 0;
+        const int64_t ws_bytes = entry.int8_bytes(e, n, d, out, (int)gated, dtype);
         const at::Tensor space = at::empty({q_bytes + s_bytes + ws_bytes}, x.options().dtype(at::kByte));
         char *q = (char *)pointer(space), *s = q + q_bytes, *ws = ws_bytes ? s + s_bytes : nullptr;
+        const int64_t *row_index = (const int64_t *)pointer(index);
         void *stream = stream_of(x);
-        ok(entry.quantize_rows(pointer(x), x.stride(0), (const int64_t *)pointer(index), index_div, x.size(0), q, whole_d, s, pointer(table), pointer(y),
-                               out * x.element_size(), n, d, dtype, stream));
-        ok(entry.linear_int8(q, whole_d, s, pointer(weight), by_row, by_expert, pointer(scale), pointer(bias), pointer(y), pointer(table), e, n, d, out,
-                             (int)gated, (int)activation, dtype, ws, ws_bytes, stream));
+        if (round_first)
+            ok(entry.quantize_rows(pointer(x), x.stride(0), row_index, index_div, x.size(0), q, whole_d, s, pointer(table), pointer(y), out * x.element_size(),
+                                   n, d, dtype, stream));
+        ok(entry.linear_int8(round_first ? q : pointer(x), round_first ? whole_d : x.stride(0), round_first ? s : nullptr, round_first ? nullptr : row_index,
+                             index_div, round_first ? n : x.size(0), pointer(weight), by_row, by_expert, pointer(scale), pointer(bias), pointer(y),
+                             pointer(table), e, n, d, out, (int)gated, (int)activation, dtype, ws, ws_bytes, stream));
     }
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS

@@ -12,7 +12,19 @@
 
 using namespace fmoe;
 
-extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w, int64_t ldw, int64_t w_expert_stride,
+namespace {
+Int8Params sizes(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat, int gated, int dtype) {
+    Int8Params prm{};
+    prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.n_cols = (int)out_feat; prm.k_extent = (int)(ceil_div(in_feat, 16) * 16);
+    prm.gated = gated != 0; prm.dtype = dtype; prm.in_feat = in_feat;
+    return prm;
+}
+bool sizes_known(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat) {
+    return n_expert >= 1 && rows_cap >= 1 && in_feat >= 1 && in_feat <= 131072 && out_feat >= 1 && out_feat <= (1 << 28);
+}
+}  // namespace
+
+extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const int64_t *row_index, int64_t index_div, int64_t x_rows, const void *w, int64_t ldw, int64_t w_expert_stride,
                                 const void *w_scale, const void *bias, void *y, const void *segment_table, int64_t n_expert, int64_t rows_cap,
                                 int64_t in_feat, int64_t out_feat, int gated, int activation, int dtype, void *workspace, int64_t workspace_bytes,
                                 void *stream) {
@@ -22,27 +34,30 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     FMOE_REQUIRE(n_expert >= 1 && rows_cap >= 0 && in_feat >= 1 && out_feat >= 1, "%s: bad sizes", who);
     const int64_t whole = ceil_div(in_feat, 16) * 16, w_rows = out_feat * (gated ? 2 : 1);
     // (131072 products of numbers up to 128: below 2^31)
-    if (in_feat > 131072 || n_expert > (1 << 24) || rows_cap > (int64_t)INT32_MAX - 65536 || out_feat > (1 << 28) || ldx > (1 << 22) ||
+    if (in_feat > 131072 || n_expert > (1 << 24) || rows_cap > (int64_t)INT32_MAX - 65536 || out_feat > (1 << 28) || (x_scale != nullptr && ldx > (1 << 22)) ||
         ldw > (1 << 22) || w_rows * ldw >= ((int64_t)1 << 31))
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
-    FMOE_REQUIRE(ldx >= whole && ldw >= whole && ldx % 16 == 0 && ldw % 16 == 0 && w_expert_stride % 16 == 0 && w_expert_stride >= 0,
+    FMOE_REQUIRE((x_scale == nullptr || (ldx >= whole && ldx % 16 == 0)) && ldw >= whole && ldw % 16 == 0 && w_expert_stride % 16 == 0 && w_expert_stride >= 0,
                  "%s: rows of 8-bit integers begin on 16 bytes, at least %lld apart", who, (long long)whole);
     if (rows_cap == 0) return FMOE_OK;
-    FMOE_REQUIRE(x && x_scale && w && w_scale && y && segment_table, "%s: NULL pointer", who);
-    FMOE_REQUIRE(aligned16(x) && aligned16(w) && aligned16(segment_table) && aligned16(y) && aligned16(w_scale) && (bias == nullptr || aligned16(bias)),
+    Int8Params prm = sizes(n_expert, rows_cap, in_feat, out_feat, gated, dtype);
+    FMOE_REQUIRE(x_scale != nullptr || int8_rounds_rows(prm), "%s: rows of these sizes come in 8-bit integers with x_scale", who);
+    FMOE_REQUIRE(x_scale == nullptr || row_index == nullptr, "%s: row_index goes with rows that are not rounded yet", who);
+    FMOE_REQUIRE(x_scale != nullptr || (index_div >= 1 && x_rows >= 0 && (row_index != nullptr || x_rows >= rows_cap)), "%s: bad rows", who);
+    FMOE_REQUIRE((x || (x_scale == nullptr && x_rows == 0)) && w && w_scale && y && segment_table, "%s: NULL pointer", who);
+    FMOE_REQUIRE((x_scale == nullptr || aligned16(x)) && aligned16(w) && aligned16(segment_table) && aligned16(y) && aligned16(w_scale) && (bias == nullptr || aligned16(bias)),
                  "%s: tensors begin on 16 bytes", who);
-    Int8Params prm{};
-    prm.x = (const int8_t *)x; prm.w = (const int8_t *)w; prm.x_scale = (const float *)x_scale; prm.w_scale = (const float *)w_scale;
+    prm.x = x; prm.w = (const int8_t *)w; prm.x_scale = (const float *)x_scale; prm.w_scale = (const float *)w_scale;
     prm.bias = bias; prm.y = y; prm.ldx = ldx; prm.ldw = ldw; prm.w_expert_stride = w_expert_stride;
-    prm.n_cols = (int)out_feat; prm.k_extent = (int)whole; prm.gated = gated != 0; prm.activation = activation;
-    prm.dev_tab = (const int32_t *)segment_table; prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.dtype = dtype;
+    prm.row_index = row_index; prm.index_div = index_div; prm.x_rows = x_rows;
+    prm.activation = activation; prm.dev_tab = (const int32_t *)segment_table;
     return launch_int8(prm, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
+extern "C" int fmoe_linear_int8_rounds_rows(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat, int gated, int dtype) {
+    return sizes_known(n_expert, rows_cap, in_feat, out_feat) && int8_rounds_rows(sizes(n_expert, rows_cap, in_feat, out_feat, gated, dtype));
+}
+
 extern "C" int64_t fmoe_linear_int8_workspace_bytes(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat, int gated, int dtype) {
-    if (n_expert < 1 || rows_cap < 1 || in_feat < 1 || in_feat > 131072 || out_feat < 1 || out_feat > (1 << 28)) return 0;
-    Int8Params prm{};
-    prm.n_expert = n_expert; prm.rows_cap = rows_cap; prm.n_cols = (int)out_feat; prm.k_extent = (int)(ceil_div(in_feat, 16) * 16);
-    prm.gated = gated != 0; prm.dtype = dtype;
-    return int8_workspace_bytes(prm);
+    return sizes_known(n_expert, rows_cap, in_feat, out_feat) ? int8_workspace_bytes(sizes(n_expert, rows_cap, in_feat, out_feat, gated, dtype)) : 0;
 }

@@ -18,9 +18,11 @@
 // Where it is used, and what it measured: use_skinny() in grouped_gemm.hip.
 //
 // Gated products (HALVES): half of a workgroup's blocks of columns are the gate's and the others the same columns of the linear half, so that the wave that adds up a
-// block of the one adds up the other's too.  8-bit integers: see Int8Pair; the sums are integers and exact.
+// block of the one adds up the other's too.  8-bit integers: see Int8Pair; the sums are integers and exact.  ROUND: the rows come as they are and each workgroup rounds
+// its expert's to integers in LDS while its first weights are on their way: see kSkinnyRoundElems.
 // The build compiles this file with -DFMOE_SKINNY=<0 plain products|1 gated ones|2 8-bit integers>.
 #include "gemm_skinny.hpp"
+#include "row_rounding.hpp"
 #include "segment_table.hpp"
 
 namespace fmoe {
@@ -52,8 +54,9 @@ __device__ __forceinline__ void pair_to_steps(u32x4 &a, u32x4 &b) {
     }
 }
 
-// COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch).  HALVES: gated
-template <typename T, int COL_BLOCKS, bool APART, bool HALVES>
+// COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch).  HALVES: gated.  ROUND: at most
+// kSkinnyRoundRows rows in all, of the results' type
+template <typename T, int COL_BLOCKS, bool APART, bool HALVES, bool ROUND>
 __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_gemm_skinny_kernel(const SkinnyParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
     constexpr int EB = (int)sizeof(T), CE = 16 / EB, kLine = 128 / EB;    // elements per lane's load and per line
@@ -69,17 +72,20 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     typedef const i32x4 __attribute__((address_space(4))) *DevTab4;
     __shared__ f32x4 part[kSkWaves - 1][COL_BLOCKS * 2][64];
+    // (16 bytes more than a row: eight rows' pieces at one place of theirs lie in different banks)
+    __shared__ __attribute__((aligned(16))) unsigned char rounded[ROUND ? kSkinnyRoundElems + kSkinnyRoundRows * 16 : 16];
+    __shared__ uint32_t most_of[kSkinnyRoundRows];
 
     const DevTab dtab = (DevTab)(uintptr_t)prm.dev_tab;
     int place = __builtin_amdgcn_readfirstlane(blockIdx.x / prm.tiles_n);
     const int tile_n = blockIdx.x - place * prm.tiles_n, n0 = tile_n * kCols, K = prm.k_extent;
     const DevTab4 order = (DevTab4)(dtab + prm.order_off);   // {expert, first row, rows}: of an expert, or (not APART) of a tile of at most 128 rows
     const int live = dtab[APART ? segtab::kLive : segtab::kTiles128];
-    if constexpr (HALVES && !kInt8) {
+    if constexpr ((HALVES && !kInt8) || ROUND) {
         const int64_t there = dtab[segtab::kRows];
         if (prm.tail != nullptr && there < prm.tail_rows)
             for (int64_t i = (int64_t)blockIdx.x * kSkThreads + threadIdx.x; i < (prm.tail_rows - there) * prm.tail_elems; i += (int64_t)gridDim.x * kSkThreads)
-                ((uint16_t *)prm.tail)[there * prm.tail_elems + i] = 0;
+                ((Out *)prm.tail)[there * prm.tail_elems + i] = (Out)0.f;
     }
     int r0 = 0;   // first row
     i32x4 entry;
@@ -101,7 +107,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
         asm volatile("" : "+s"(entry));
         if (place >= live) return;
     }
-    const int expert = entry[0], first = entry[1], rows = entry[2];
+    const int expert = entry[0], first = entry[1], rows = ROUND ? min(entry[2], kSkinnyRoundRows) : entry[2];
     if (rows == 0) return;
     // where its contraction begins, by expert and columns alone: a row's sum does not depend on the rows that other experts have
     const uint32_t start = __builtin_amdgcn_readfirstlane((uint32_t)expert * (uint32_t)prm.tiles_n + (uint32_t)tile_n);
@@ -119,7 +125,48 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     const __amdgpu_buffer_rsrc_t w_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(W), 0, w_bytes, kRsrcFlags);
     const uint32_t w_off = (uint32_t)(row8 * ldw * EB + chunk * 16), eight_rows = (uint32_t)(8 * ldw * EB);
     const uint32_t half_rows = HALVES ? (uint32_t)prm.n_cols * (uint32_t)(ldw * EB) : 0u;
-    const bool gather = prm.row_index != nullptr;
+    const bool gather = !ROUND && prm.row_index != nullptr;
+
+    // Rows to be rounded: all of the expert's, eight elements at a time, asked for before the first weights.
+    constexpr int kPieces = ROUND ? kSkinnyRoundElems / (kLaneElems * kSkThreads) : 1;
+    Eight<Out> raw[kPieces];
+    const int row_bytes = K * 2 + 16, row_pieces = K * 2 / kLaneElems;   // (K: pairs)
+    auto place_of = [&](int i, int &row, int &col) {
+        const int p = t + i * kSkThreads;
+        row = (int)((uint32_t)p / (uint32_t)row_pieces);
+        col = (p - row * row_pieces) * kLaneElems;
+        return row < rows;
+    };
+    if constexpr (ROUND) {
+        if (t < kSkinnyRoundRows) most_of[t] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            int row, col;
+            bool there = place_of(i, row, col);
+            int64_t src = first + row;
+            if (prm.row_index != nullptr && there) {   // (a row from nowhere is one of zeros)
+                const int64_t idx = prm.row_index[src];
+                src = idx < 0 ? -1 : prm.index_div == 1 ? idx : idx / prm.index_div;
+                there = src >= 0 && src < prm.x_total_rows;
+            }
+            raw[i].load((const Out *)prm.x + (there ? src * prm.ldx + col : 0), there ? prm.x_elems - col : 0);
+        }
+    }
+    auto round_rows = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            int row, col;
+            if (place_of(i, row, col)) atomicMax(&most_of[row], magnitude_bits<Out>(larger<Out>(0u, raw[i])));   // (a maximum: in any order)
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            int row, col;
+            if (place_of(i, row, col)) *(uint2 *)(rounded + row * row_bytes + col) = RowScale(most_of[row]).round(raw[i]);
+        }
+        __syncthreads();
+    };
 
     // NB blocks of 16 columns from column c0 of the workgroup on times RB blocks of 16 rows from the expert's row r0 on; a unit is LINES times
     // 128 bytes of contraction.  POLICY: of the weights' loads
@@ -168,6 +215,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
             for (int h = 0; h < 2; ++h) index[y][h] = __builtin_amdgcn_raw_buffer_load_b64(index_rs, (r0 - base + 16 * y + 8 * h + row8) * 8, 0, 0);
         load_w(a, unit);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (ROUND) round_rows();
         uint32_t x_off[RB][2];
 #pragma unroll
         for (int y = 0; y < RB; ++y)
@@ -196,7 +244,10 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                 for (int y = 0; y < RB; ++y) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h)   // (both offsets may have the sign bit)
-                        u.x[l][y][h] = __builtin_amdgcn_raw_buffer_load_b128(x_rs, (int)((x_off[y][h] + (at & ~kOutOfRange)) | (at & kOutOfRange)), 0, 0);
+                        if constexpr (ROUND)
+                            u.x[l][y][h] = row8 + 8 * h < rows && !(at & kOutOfRange) ? *(const u32x4 *)(rounded + (row8 + 8 * h) * row_bytes + (int)at + chunk * 16)
+                                                                                  : u32x4{0u, 0u, 0u, 0u};
+                        else u.x[l][y][h] = __builtin_amdgcn_raw_buffer_load_b128(x_rs, (int)((x_off[y][h] + (at & ~kOutOfRange)) | (at & kOutOfRange)), 0, 0);
                 }
             }
         };
@@ -272,7 +323,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     const int row = r0 + 16 * y + lb;
                     const f32x4 sum[2] = {summed(n, y), HALVES ? summed(n + NH, y) : f32x4{}};
                     if (row >= rows) continue;
-                    const float s = kInt8 ? prm.x_scale[first + row] : 1.f;
+                    const float s = ROUND ? RowScale(most_of[row]).shown() : kInt8 ? prm.x_scale[first + row] : 1.f;
                     alignas(16) Out pre[H][4], res[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -328,12 +379,13 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     typedef std::integral_constant<int, (COL_BLOCKS < 2 ? COL_BLOCKS : 2)> UpToTwo;
     // (Two units have to fit 168 registers: scratch memory costs launches that never touch it a tenth of their time.  The weights of an
     // expert with several groups are read again, from the caches.)
-    if (rows <= 16) {
+    if (ROUND || rows <= 16) {
         const std::integral_constant<int, COL_BLOCKS == 1 ? 2 : 1> lines;
         if (prm.weights_cached) pass(All{}, One{}, lines, Cached{}, 0, 0);
         else pass(All{}, One{}, lines, Nontemporal{}, 0, 0);
         return;
     }
+    if constexpr (!ROUND) {
     auto up_to_two = [&](int c0) {
         if (rows <= kSkRows && !prm.weights_cached) {
             pass(UpToTwo{}, Two{}, One{}, Nontemporal{}, c0, 0);
@@ -346,6 +398,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
     up_to_two(0);
     constexpr int kNext = HALVES ? 16 : 32;
     if (COL_BLOCKS > 2 && prm.n_cols - n0 > kNext) up_to_two(kNext);
+    }
 #endif
 }
 
@@ -362,7 +415,7 @@ template <typename T> int skinny_blocks(const SkinnyParams &prm, int64_t experts
     return sizeof(T) == 2 && ceil_div(n_cols, 64) * 2 >= cus && (int64_t)prm.k_extent * 2 * 64 < ((int64_t)1 << 31) ? 4 : 2;
 }
 
-template <typename T, bool HALVES = false> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+template <typename T, bool HALVES = false, bool ROUND = false> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     SkinnyParams prm = params;
     // An expert's groups of rows go to workgroups of their own, where the experts come in order of their rows: the further groups first,
     // which leave at once where there are none.  128 experts of 1280 x 1280, 448 rows, 144 of them one expert's: 37 us in turn, 29 apart; 64 of 1280 x
@@ -377,10 +430,10 @@ template <typename T, bool HALVES = false> int launch(const SkinnyParams &params
     prm.tiles_n = (int)ceil_div(prm.n_cols, 16 * blocks / (HALVES ? 2 : 1));
     const int64_t grid = (experts + prm.extra_groups) * prm.tiles_n;
     if (grid > (int64_t)INT32_MAX) return fail(FMOE_ELIMIT, "grouped GEMM: grid of %lld workgroups", (long long)grid);
-    if (!apart) grouped_gemm_skinny_kernel<T, 2, false, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
-    else if (blocks == 2) grouped_gemm_skinny_kernel<T, 2, true, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
-    else if (blocks == 1) { if constexpr (!HALVES) grouped_gemm_skinny_kernel<T, 1, true, false><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm); }
-    else if constexpr (sizeof(T) == 2) grouped_gemm_skinny_kernel<T, 4, true, HALVES><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    if (!apart) grouped_gemm_skinny_kernel<T, 2, false, HALVES, ROUND><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    else if (blocks == 2) grouped_gemm_skinny_kernel<T, 2, true, HALVES, ROUND><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
+    else if (blocks == 1) { if constexpr (!HALVES) grouped_gemm_skinny_kernel<T, 1, true, false, ROUND><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm); }
+    else if constexpr (sizeof(T) == 2) grouped_gemm_skinny_kernel<T, 4, true, HALVES, ROUND><<<(unsigned)grid, kSkThreads, 0, stream>>>(prm);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
 }
@@ -402,6 +455,7 @@ int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, in
 int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     auto go = [&](auto pair) {
         using Pair = decltype(pair);
+        if (prm.x_scale == nullptr) return gated ? launch<Pair, true, true>(prm, rows_cap, n_expert, stream) : launch<Pair, false, true>(prm, rows_cap, n_expert, stream);
         return gated ? launch<Pair, true>(prm, rows_cap, n_expert, stream) : launch<Pair>(prm, rows_cap, n_expert, stream);
     };
     if (dtype == FMOE_F32) return go(Int8Pair<float>{});

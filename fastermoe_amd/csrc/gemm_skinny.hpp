@@ -17,11 +17,19 @@ struct SkinnyParams {
     int32_t weights_cached;       // not 0: the weights through the caches, see caches_few_row_weights() in grouped_gemm.hip
     // Gated products and such in 8-bit integers (w: [E, 2 n_cols or n_cols, k], a gate's rows first; aux [rows, 2 n_cols]):
     int64_t ldw, ldx, w_expert_stride;         // 8-bit integers: row strides in pairs of them (others are dense)
-    const float *w_scale, *x_scale;            // 8-bit integers: of each row of w and of x
-    void *tail;                                // gated: rows of tail_elems 16-bit elements behind the table's, up to tail_rows, become zeros (null: none)
+    const float *w_scale, *x_scale;            // 8-bit integers: of each row of w and of x; x_scale null: x in y's type, to be rounded here
+    int64_t index_div;                         // rows to be rounded: row_index's divisor, elements of a row (ldx apart)
+    int32_t x_elems;
+    void *tail;                                // gated, or rows to be rounded: rows of tail_elems elements behind the table's, up to tail_rows, become zeros (null: none)
     int64_t tail_rows, tail_elems;
     int32_t order_off, tiles_n, extra_groups;   // set by the launch: the table's list of experts (or its map of row tiles), see launch()
 };
+
+// Rows that the launch in 8-bit integers rounds itself: at most this many, of at most this many elements in all (a row's rounded up to sixteen).  Each workgroup rounds all
+// of its expert's rows, while its first weights are on their way.  us in a launch of their own and here, in a graph, weights from memory: 32 experts of 1024 -> 4096, 2
+// rows: 6.6 / 5.2, 8 rows: 11.5 / 8.7, all 8 one expert's: 6.7 / 6.8; 8 of 4096 -> 2 x 14336, gated, 2 rows: 40.0 / 37.1; 64 of 512 -> 2 x 2048, gated, 16 rows: 13.4 /
+// 10.8, all one expert's: 6.3 / 7.1; 1 row of 8192 -> 8192: 24.7 / 20.8.
+constexpr int kSkinnyRoundRows = 16, kSkinnyRoundElems = 8192;
 
 // rows_cap: the rows that the table was laid out for
 int launch_skinny(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);

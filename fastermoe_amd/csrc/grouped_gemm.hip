@@ -891,6 +891,10 @@ DevRoute int8_route(const Int8Params &a) {
     return {use_ring(tile, FMOE_BF16) && is_16bit(a.dtype) && a.n_cols % 8 == 0 ? DevKernel::kRing : DevKernel::kTiles, tile};
 }
 }  // namespace
+// Rows rounded by the product's own workgroups: where there are so few that a launch for them costs more.
+bool int8_rounds_rows(const Int8Params &a) {
+    return a.rows_cap <= kSkinnyRoundRows && a.rows_cap * a.k_extent <= kSkinnyRoundElems && int8_route(a).kernel == DevKernel::kSkinny;
+}
 int64_t int8_workspace_bytes(const Int8Params &a) {
     const DevRoute route = int8_route(a);
     return route.kernel == DevKernel::kRing ? route_workspace_bytes(route, a.k_extent / 2, FMOE_BF16) : 0;   // (the tiles' parts are added up as floats)
@@ -904,7 +908,11 @@ int launch_int8(const Int8Params &a, void *workspace, int64_t workspace_bytes, h
         SkinnyParams sk{};
         sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
         sk.n_cols = a.n_cols; sk.k_extent = a.k_extent / 2; sk.activation = a.activation;
-        sk.ldw = a.ldw / 2; sk.ldx = a.ldx / 2; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
+        sk.ldw = a.ldw / 2; sk.ldx = a.x_scale ? a.ldx / 2 : a.ldx; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
+        if (a.x_scale == nullptr) {
+            sk.row_index = a.row_index; sk.index_div = a.index_div; sk.x_total_rows = a.x_rows; sk.x_elems = (int32_t)a.in_feat;
+            sk.tail = a.y; sk.tail_rows = a.rows_cap; sk.tail_elems = a.n_cols;
+        }
         ProfileScope prof(kProfGemmFwd, work, stream);
         return launch_skinny_int8(sk, a.dtype, a.gated != 0, a.rows_cap, a.n_expert, stream);
     }

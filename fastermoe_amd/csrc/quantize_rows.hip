@@ -4,25 +4,22 @@
 //
 // A row with an infinity or a NaN has the scale NaN and zeros, so that whatever is made of it is NaN.
 //
-// The exact quotient's rounding, without a division per element: t = x * (1 / s) + 1.5 2^23, one fused multiply-add, has the integer next to x * (1 / s) in its low
-// bits; that product is off by less than 2^-16, so q = t - 1.5 2^23 is the right integer or the one beside it, and r = x - q s, another multiply-add, is
-// exact (a multiple of ulp(s) or of x's, below 2 s).  Only where |r| >= s / 2, once in some thousand elements, q may be off, or a tie: such pieces are looked at again.
+// The rounding itself: row_rounding.hpp.
 //
 // A lane takes eight elements at a time.  A row that fits the registers of its wave, or, longer (or where rows are few), of its workgroup's four waves, is read once; a
 // longer one is read again, from the caches.  Bound by memory, and next by 7 instructions an element (18 with a conversion and a correction for each: 354 us for 32768
 // rows of 14336 in bfloat16).
 #include "common.hpp"
 #include "grouped_gemm.hpp"
-#include "lane_elems.hpp"
+#include "row_rounding.hpp"
 
 #include <type_traits>
 
 namespace fmoe {
 namespace {
 
-constexpr int kBlock = 256, kWaves = kBlock / kWave, kLaneElems = 8;
+constexpr int kBlock = 256, kWaves = kBlock / kWave;
 constexpr int64_t kManyRows = 2048;
-constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
 
 struct Params {
     const void *x;
@@ -36,78 +33,6 @@ struct Params {
     uint8_t *tail;               // or null: rows of tail_bytes bytes, those behind the table's become zeros
     int64_t tail_bytes;
 };
-
-// Eight elements as they lie in memory
-template <typename T> struct Eight {
-    static constexpr int kVecs = (int)sizeof(T) / 2;
-    u32x4 v[kVecs];
-    // the first n of them at p, zeros after those
-    __device__ __forceinline__ void load(const T *p, int n) {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = load_vec<false>(p + i * Vec<T>::N, n - i * Vec<T>::N, false);
-    }
-    __device__ __forceinline__ void floats(float (&f)[kLaneElems]) const {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            float g[8];
-            Vec<T>::unpack(v[i], g);
-#pragma unroll
-            for (int j = 0; j < Vec<T>::N; ++j) f[i * Vec<T>::N + j] = g[j];
-        }
-    }
-};
-// The magnitudes' bits are in the order of the magnitudes, infinity and then NaN above them: the largest of a lane's elements, as the bits of its type (16-bit types: in
-// either half).
-template <typename T> __device__ __forceinline__ uint32_t larger(uint32_t most, const Eight<T> &e) {
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < Eight<T>::kVecs; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (sizeof(T) == 4) {
-                most = max(most, e.v[i][j] & 0x7fffffffu);
-            } else {
-                const u16x2 a = __builtin_bit_cast(u16x2, most), b = __builtin_bit_cast(u16x2, e.v[i][j] & 0x7fff7fffu);
-                most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
-            }
-        }
-    return most;
-}
-// float32 bits of the largest magnitude
-template <typename T> __device__ __forceinline__ uint32_t magnitude_bits(uint32_t most) {
-    if constexpr (sizeof(T) == 4) {
-        return most;
-    } else {
-        const uint16_t top = (uint16_t)max(most & 0xffffu, most >> 16);
-        return __float_as_uint((float)__builtin_bit_cast(T, top));
-    }
-}
-
-constexpr float kMagic = 12582912.f;   // 1.5 2^23
-// eight integers, a byte each
-__device__ __forceinline__ uint2 round_all(const float (&x)[kLaneElems], float inv, float s, float half) {
-    float t[kLaneElems], off = 0.f;
-#pragma unroll
-    for (int j = 0; j < kLaneElems; ++j) {
-        t[j] = fmaf(x[j], inv, kMagic);
-        off = fmaxf(off, fabsf(fmaf(kMagic - t[j], s, x[j])));
-    }
-    if (off >= half) {
-#pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) {
-            const float q = t[j] - kMagic, r = fmaf(-q, s, x[j]), a = fabsf(r);
-            if (a > half || (a == half && ((int)q & 1))) t[j] += r > 0.f ? 1.f : -1.f;
-        }
-    }
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * h + 1]), __float_as_uint(t[4 * h]), 0x0c0c0400u);
-        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * h + 3]), __float_as_uint(t[4 * h + 2]), 0x04000c0cu);
-        w[h] = lo | hi;
-    }
-    return make_uint2(w[0], w[1]);
-}
 
 // ROW_WAVES: waves that share a row, 1 or all of the workgroup; NV: pieces of a lane that stay in registers (0: the row is read twice)
 template <typename T, int ROW_WAVES, int NV>
@@ -157,14 +82,10 @@ __global__ __launch_bounds__(kBlock) void quantize_rows_kernel(const Params prm)
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) most = max(most, most_of[w]);
     }
-    const bool finite = most < 0x7f800000u;
-    const float s = fmaxf(__uint_as_float(finite ? most : 0u) / 127.f, kLeastScale), inv = 1.f / s, half = 0.5f * s;
-    if (first == 0) prm.scale[row] = finite ? s : __uint_as_float(0x7fc00000u);
+    const RowScale scale(most);
+    if (first == 0) prm.scale[row] = scale.shown();
     auto store = [&](int c, const Eight<T> &piece) {
-        float f[kLaneElems];
-        piece.floats(f);
-        uint2 w = round_all(f, inv, s, half);
-        if (!finite) w = make_uint2(0, 0);
+        const uint2 w = scale.round(piece);
         if (c < prm.dq) *(uint2 *)(q + c) = w;
     };
     if constexpr (NV > 0) {

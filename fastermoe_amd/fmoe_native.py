@@ -977,21 +977,28 @@ def _int8_rows(n, d, device):
     return torch.empty(n, whole, dtype=torch.int8, device=device)
 
 
-def quantize_rows(x, row_index=None, index_div=1, table=None, tail=None):
-    """``(q, scale)`` of rows ``x [rows, features]``: int8 and float32 ``[rows]`` with ``x ~ q * scale[:, None]``, ``scale`` a 127th of a row's largest
-    magnitude.  ``q``'s rows lie whole 16-byte pieces apart.  ``row_index`` (int64): row ``r`` is made of row ``row_index[r] // index_div`` of
-    ``x``.  ``table``: only the rows of this segment table are made, and those behind them in ``tail [rows, ..]`` become zeros."""
+def _rows_to_round(x, row_index, index_div):
+    """``(x, its rows' distance, rows that are made)``."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a torch.Tensor, got {type(x).__name__}")
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError(f"quantize_rows does not take {x.dtype}")
     x, ldx = _strided_rows("x", x)
-    n, d = x.shape
+    n = x.shape[0]
     if row_index is not None:
         _near("row_index", _dev("row_index", row_index, torch.int64), x.device)
         n = row_index.numel()
         if int(index_div) < 1:
             raise ValueError(f"index_div is {index_div}")
+    return x, ldx, n
+
+
+def quantize_rows(x, row_index=None, index_div=1, table=None, tail=None):
+    """``(q, scale)`` of rows ``x [rows, features]``: int8 and float32 ``[rows]`` with ``x ~ q * scale[:, None]``, ``scale`` a 127th of a row's largest
+    magnitude.  ``q``'s rows lie whole 16-byte pieces apart.  ``row_index`` (int64): row ``r`` is made of row ``row_index[r] // index_div`` of
+    ``x``.  ``table``: only the rows of this segment table are made, and those behind them in ``tail [rows, ..]`` become zeros."""
+    x, ldx, n = _rows_to_round(x, row_index, index_div)
+    d = x.shape[1]
     if tail is not None and (table is None or tail.shape[0] != n or not tail.is_contiguous() or tail.device != x.device):
         raise ValueError("tail must be as many adjacent rows, with a segment table")
     q = _int8_rows(n, d, x.device)
@@ -1067,17 +1074,23 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
         if tuple(bias.shape) != (e, out):
             raise ValueError(f"bias must be {(e, out)}, got {tuple(bias.shape)}")
         bias = _on_16_bytes(bias)
-    n = x.shape[0] if row_index is None else row_index.numel()
+    n = _rows_to_round(x, row_index, index_div)[2]
     out = out // 2 if gated else out
     _exact_table(table, e, n, x.device)
     y = torch.empty(n, out, dtype=x.dtype, device=x.device)
-    q, scale = quantize_rows(x, row_index, index_div, table, y)
     lib = _lib.load()
+    sizes = (e, n, d, out, int(gated), _DTYPES[x.dtype])
+    if n and lib.fmoe_linear_int8_rounds_rows(*sizes):
+        rows, ldx, _ = _rows_to_round(x, row_index, index_div)
+        scale, x_rows = None, x.shape[0]
+    else:
+        rows, scale = quantize_rows(x, row_index, index_div, table, y)
+        ldx, row_index, x_rows = rows.stride(0), None, n
     with _on(x.device):
-        ws = _dev_workspace(lib.fmoe_linear_int8_workspace_bytes(e, n, d, out, int(gated), _DTYPES[x.dtype]), x.device)
-        check(lib.fmoe_linear_int8(_ptr(q), q.stride(0), _ptr(scale), _ptr(weight), by_row, by_expert, _ptr(weight_scale), _ptr(bias), _ptr(y),
-                                   _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel(),
-                                   _stream(x)))
+        ws = _dev_workspace(lib.fmoe_linear_int8_workspace_bytes(*sizes), x.device)
+        check(lib.fmoe_linear_int8(_ptr(rows), ldx, _ptr(scale), _ptr(row_index), int(index_div), x_rows, _ptr(weight), by_row, by_expert, _ptr(weight_scale),
+                                   _ptr(bias), _ptr(y), _ptr(table), e, n, d, out, int(gated), activation, _DTYPES[x.dtype], _ptr(ws),
+                                   0 if ws is None else ws.numel(), _stream(x)))
     return y
 
 

@@ -794,7 +794,11 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
 
 /* y[r, c] = act(x_scale[r] w_scale[c] sum_k x[r, k] w[c, k] + bias[c]) per
  * expert over its rows; gated: act(that of row c) * (that of row out_feat + c).
- * x: rows of 8-bit integers as fmoe_quantize_rows leaves them, ldx bytes apart.
+ * x: rows of 8-bit integers as fmoe_quantize_rows leaves them, ldx bytes apart;
+ * or, few rows for which fmoe_linear_int8_rounds_rows is not 0, with x_scale NULL:
+ * rows of dtype, x_rows of them, ldx elements apart, rounded in the same launch
+ * (row_index, index_div as fmoe_quantize_rows has them; rows of y behind the
+ * experts' become zeros).
  * w: per expert out_feat (gated: 2 out_feat) rows of in_feat integers, ldw bytes
  * apart, experts w_expert_stride bytes apart, all multiples of 16, on 16 bytes;
  * a row can be read up to the next multiple of 16 bytes.  w_scale [E, rows of w]
@@ -808,8 +812,12 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
 int64_t fmoe_linear_int8_workspace_bytes(int64_t n_expert, int64_t rows_cap,
                                          int64_t in_feat, int64_t out_feat, int gated,
                                          int dtype);
-int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const void *w,
-                     int64_t ldw, int64_t w_expert_stride, const void *w_scale,
+int fmoe_linear_int8_rounds_rows(int64_t n_expert, int64_t rows_cap, int64_t in_feat,
+                                 int64_t out_feat, int gated, int dtype);
+int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
+                     const int64_t *row_index, int64_t index_div, int64_t x_rows,
+                     const void *w, int64_t ldw, int64_t w_expert_stride,
+                     const void *w_scale,
                      const void *bias, void *y, const void *segment_table,
                      int64_t n_expert, int64_t rows_cap, int64_t in_feat,
                      int64_t out_feat, int gated, int activation, int dtype,

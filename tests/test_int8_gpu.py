@@ -268,6 +268,42 @@ def test_rows_behind_the_counted_ones_are_zeros_and_never_read():
     assert not y[25:].any() and torch.isfinite(y).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,d,out,experts,kind", [(1, 1, 4, 1, "even"), (1, 8192, 64, 2, "one"), (2, 4096, 520, 2, "even"), (8, 1024, 36, 3, "skewed"), (7, 1001, 128, 20, "even"),
+                                                     (16, 512, 200, 3, "tail"), (16, 500, 132, 1, "one"), (16, 3, 8, 16, "even"), (5, 50, 2052, 600, "even"),
+                                                     (17, 16, 8, 4, "even"), (3, 2736, 64, 2, "even")])
+def test_few_rows_have_the_bits_that_they_have_among_many(rows, d, out, experts, kind, gated, dtype):
+    """Rows rounded within the product (up to 16 of up to 8192 elements in all) and in a launch of their own."""
+    x, weight, scale, b = _tensors(rows + 40, d, out * (2 if gated else 1), experts, dtype, True, seed=rows)
+    counts = _counts(kind, rows, experts, seed=rows)
+    here = sum(counts)
+    if rows > 2:
+        x[here // 2, d // 2] = float("inf")
+    few = functions.linear_int8(x[:rows], torch.tensor(counts, device="cuda"), weight, scale, b, torch.nn.SiLU(), gated=gated)
+    counts[-1] += 40
+    many = functions.linear_int8(torch.cat([x[:here], x[rows:]]), torch.tensor(counts, device="cuda"), weight, scale, b, torch.nn.SiLU(), gated=gated)
+    assert torch.equal(few[:here].nan_to_num(7.0), many[:here].nan_to_num(7.0)) and not few[here:].any()
+    if rows > 2:
+        assert torch.isnan(few[here // 2]).all()
+
+
+def test_few_rows_through_an_index_and_strides():
+    x, weight, scale, b = _tensors(20, 96, 40, 3, torch.bfloat16, True)
+    index = torch.tensor([59, 0, 7, 7, 30, 58], device="cuda")
+    counts = [2, 0, 3]
+    wide = torch.full((20, 101), 9.0, device="cuda", dtype=torch.bfloat16)
+    wide[:, 1:97] = x
+    for rows in (x, wide[:, 1:97]):
+        y = functions.linear_int8(rows, torch.tensor(counts, device="cuda"), weight, scale, b, row_index=index, index_div=3)
+        _close(y[:5], _reference(x, counts, weight, scale, b, "none", False, at=index[:5] // 3))
+        assert not y[5:].any()
+        _close(functions.linear_int8(rows[4:8], torch.tensor([1, 2, 1], device="cuda"), weight, scale, b),
+               _reference(x[4:8], [1, 2, 1], weight, scale, b, "none", False))
+    outside = functions.linear_int8(x, torch.tensor([1, 1, 1], device="cuda"), weight, scale, b, row_index=torch.tensor([-1, 60, 3], device="cuda"), index_div=3)
+    assert torch.equal(outside[0], b[0]) and torch.equal(outside[1], b[1])   # (rows from nowhere are zeros)
+
+
 def test_infinities_and_nan_show():
     x, weight, scale, b = _tensors(9, 48, 33, 1, torch.bfloat16, True)
     x[3, 5], x[7, 0] = float("inf"), float("nan")
