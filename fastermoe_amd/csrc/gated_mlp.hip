@@ -195,6 +195,7 @@ struct Products {
     int forward(const void *x, const void *w, const void *bias, void *y, int64_t in, int64_t out, bool once) const {
         LinearForwardArgs a{x, w, bias, y, nullptr, in, out, dtype, kEpiStore, FMOE_ACT_NONE};
         place(a);
+        a.dev_few_unaligned = true;
         a.dev_weights_once = once;   // (no backward that reads them again)
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;

@@ -42,18 +42,6 @@ template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u3
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[j]), acc, 0, 0, 0);
 }
 
-// Two loads of 128 bytes of rows 0 to 7 and 8 to 15 (lane: row lane % 8, bit 3: half of the line) become the operands of two
-// steps (lane: row lane % 16, chunk lane / 16 of the step's 64 bytes): the lanes with bit 3 set give the first load's second chunks
-// for the second load's first.
-__device__ __forceinline__ void pair_to_steps(u32x4 &a, u32x4 &b) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = a[i], hi = b[i];   // (row_ror 8 within 16 lanes, written to the upper or to the lower eight)
-        a[i] = __builtin_amdgcn_update_dpp(lo, hi, 0x128, 0xf, 0xc, false);
-        b[i] = __builtin_amdgcn_update_dpp(hi, lo, 0x128, 0xf, 0x3, false);
-    }
-}
-
 // COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch).  HALVES: gated.  ROUND: at most
 // kSkinnyRoundRows rows in all, of the results' type
 template <typename T, int COL_BLOCKS, bool APART, bool HALVES, bool ROUND>

@@ -38,5 +38,20 @@ int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, in
 // rows and weights in 8-bit integers, k_extent in pairs, dtype of the results, whose columns are a multiple of four
 int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 
+// Rows off the 16-byte grid, 16-bit types (gemm_few_unaligned.hip): the plain or the gated forward product
+int launch_few_unaligned(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
+
+// Two loads of 128 bytes of rows 0 to 7 and 8 to 15 (lane: row lane % 8, bit 3: half of the line) become the operands of two
+// steps (lane: row lane % 16, chunk lane / 16 of the step's 64 bytes): the lanes with bit 3 set give the first load's second chunks
+// for the second load's first.
+__device__ __forceinline__ void pair_to_steps(u32x4 &a, u32x4 &b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = a[i], hi = b[i];   // (row_ror 8 within 16 lanes, written to the upper or to the lower eight)
+        a[i] = __builtin_amdgcn_update_dpp(lo, hi, 0x128, 0xf, 0xc, false);
+        b[i] = __builtin_amdgcn_update_dpp(hi, lo, 0x128, 0xf, 0x3, false);
+    }
+}
+
 }  // namespace gemm
 }  // namespace fmoe

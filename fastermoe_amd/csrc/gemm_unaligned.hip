@@ -12,40 +12,13 @@
 // loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (8192 rows, 2047 x 4093:
 // 600 to 680 TFLOP/s).  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
 #include "gemm_kernel.hpp"
-#include "vec16.hpp"
+#include "unaligned_loads.hpp"
 
 namespace fmoe {
 namespace {
 using namespace gemm;
 
 constexpr int kUaThreads = 256, kUaBN = 128, kUaBK = 64;
-
-template <typename T> __device__ __forceinline__ u32x4 load_unaligned(const T *p) {
-    u32x4 v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
-}
-// The first n of the eight elements at p, zeros after them.  8 <= n: all of them.  0 < n < 8: with `back`, the eight
-// elements that end with them (the caller knows that as many precede them in their row), moved down; else one by one.
-// n <= 0: nothing is read at p, but with `back` eight elements at `safe`.
-template <typename T> __device__ __forceinline__ u32x4 load_part(const T *p, const T *safe, int n, bool back) {
-    if (back) {
-        const int s = 8 - max(0, min(n, 8));   // elements to move down
-        const u32x4 v = load_unaligned(n > 0 ? p - s : safe);
-        const u32x4 a = s & 4 ? u32x4{v[2], v[3], 0u, 0u} : v;
-        const u32x4 b = s & 2 ? u32x4{a[1], a[2], a[3], 0u} : a;
-        const u32x4 c = s & 1 ? u32x4{__builtin_amdgcn_alignbit(b[1], b[0], 16), __builtin_amdgcn_alignbit(b[2], b[1], 16),
-                                      __builtin_amdgcn_alignbit(b[3], b[2], 16), b[3] >> 16} : b;
-        return n > 0 ? c : u32x4{0u, 0u, 0u, 0u};
-    }
-    if (n >= 8) return load_unaligned(p);
-    alignas(16) uint16_t e[8] = {};
-    const uint16_t *src = (const uint16_t *)p;
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-        if (j < n) e[j] = src[j];
-    return __builtin_bit_cast(u32x4, e);
-}
 
 // PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].  EPI: kEpiGated, kEpiDGated, or 0: what the parameters say.
 template <typename T, int BM, int PSHAPE, int QSHAPE, int RAGGED, int EPI>

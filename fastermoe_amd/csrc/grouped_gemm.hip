@@ -444,6 +444,18 @@ bool caches_few_row_weights(const LinearForwardArgs &a, int64_t n_expert) {
     return !a.dev_weights_once && n_expert * a.in_feat * a.out_feat * dtype_bytes(a.dtype) <= kHeldWeightBytes;
 }
 
+constexpr int64_t kFewUnalignedRows = 192;
+// Whether a forward product off the 16-byte grid goes to gemm_few_unaligned.hip: few rows (a skewed gate gives its first expert several passes of sixteen, with as
+// many readings of its weights), and contractions that are long beside the number of tiles, whose slabs then come one after the other.
+// us of a gated block (both products) on the tiles and there, weights from memory, even counts / shares 1 / rank^1.2: 8 experts of 4095 -> 2 x 4097, 8 rows: 372 /
+// 184, 269 / 102; 64 rows: 390 / 213, 389 / 237; 128: 386 / 241, 387 / 309; 8 of 1000 -> 2 x 2001, 1 row: 49 / 16; 64: 75 / 36, 76 / 46; 16 of 1001 -> 2 x 703, 64: 52 / 32,
+// 51 / 35; 256: 52 / 36, 52 / 78; 33 of 443 -> 2 x 2368, the second product there, 132: 105 / 84, 83 / 78; 264: 105 / 85, 102 / 120; 64 of 513 -> 2 x 1023, the
+// second there, 64: 105 / 87, 43 / 40; 256: 104 / 89, 74 / 84; with short contractions, both there: 33 of 443 -> 2 x 2368, 33: 103 / 81, 47 / 35; 264: 105 / 89, 102 / 138;
+// 128 of 257 -> 2 x 255, 128: 43 / 48, 20 / 31; 512: 42 / 51, 24 / 72.
+bool few_unaligned(int64_t rows_cap, int64_t n_expert, int64_t in_feat, int64_t out_feat, int dtype) {
+    return is_16bit(dtype) && rows_cap <= std::min<int64_t>(16 * n_expert, kFewUnalignedRows) && std::min(rows_cap, n_expert) * ceil_div(out_feat, 64) <= in_feat;
+}
+
 // The kernel of a row-ragged launch over a device table, and the workspace it can make use of.
 enum class DevKernel { kTiles, kSkinny, kRing };
 struct DevRoute {
@@ -617,6 +629,13 @@ int grouped_linear_forward(const LinearForwardArgs &a, const int64_t *counts, in
         prm.p_expert_stride = a.in_feat * a.out_feat;
         prm.bias_expert_stride = a.out_feat;
         prm.n_cols = (int)a.out_feat; prm.k_extent = (int)a.in_feat;
+        if (any_grid && a.dev_few_unaligned && few_unaligned(a.dev_rows_cap, n_expert, a.in_feat, a.out_feat, a.dtype)) {
+            SkinnyParams sk{};
+            sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
+            sk.n_cols = prm.n_cols; sk.k_extent = prm.k_extent;
+            ProfileScope prof(prm.profile_class, prm.profile_work, stream);
+            return launch_few_unaligned(sk, a.dtype, false, a.dev_rows_cap, n_expert, stream);
+        }
         if (any_grid) return dispatch<kFwd>(prm, a.dtype, a.epilogue, false, stream);
         prm.dev_split_ws = route_workspace(route, a.in_feat, a.dtype, a.dev_workspace, a.dev_workspace_bytes);
         if (route.kernel == DevKernel::kSkinny) {
@@ -820,7 +839,8 @@ int tiles_of_table(const char *who, GemmParams &prm, const GatedArgs &a, const T
 }  // namespace
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
     const bool fits = gated_sizes_fit(a);
-    if (fits && gated_forward_few(a)) {
+    const bool few = fits ? gated_forward_few(a) : few_unaligned(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype);
+    if (few) {
         SkinnyParams sk{};
         sk.w = a.w; sk.x = a.in; sk.bias = a.bias; sk.y = a.out; sk.aux = a.pre; sk.dev_tab = a.dev_tab;
         sk.n_cols = (int)a.h; sk.k_extent = (int)a.d; sk.activation = a.activation;
@@ -829,7 +849,7 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
         sk.weights_cached = caches_few_row_weights(like, a.n_expert);
         sk.tail = a.tail; sk.tail_rows = a.rows_cap; sk.tail_elems = a.d;
         ProfileScope prof(kProfGemmFwd, 4.0 * (double)a.rows_cap * (double)a.d * (double)a.h, stream);
-        return launch_skinny_gated(sk, a.dtype, a.rows_cap, a.n_expert, stream);
+        return fits ? launch_skinny_gated(sk, a.dtype, a.rows_cap, a.n_expert, stream) : launch_few_unaligned(sk, a.dtype, true, a.rows_cap, a.n_expert, stream);
     }
     const TileShape tile = fits ? gated_forward_tile(a) : unaligned_tile_estimate(a.rows_cap, a.n_expert, 2 * a.h);
     if (!fits || !use_ring(tile, a.dtype)) {

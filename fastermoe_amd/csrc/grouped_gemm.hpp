@@ -90,6 +90,8 @@ struct LinearForwardArgs {
     int64_t dev_workspace_bytes = 0;
     // with dev_tab: 16-bit tensors and feature sizes off the 16-byte grid are taken too (gemm_unaligned.hip)
     bool dev_any_grid = false;
+    // with dev_any_grid: few rows may go to gemm_few_unaligned.hip (kEpiStore, no activation; its sums are in another order)
+    bool dev_few_unaligned = false;
     // with dev_tab: nothing will read the weights again soon, as a backward would
     bool dev_weights_once = false;
 };

@@ -184,6 +184,27 @@ def test_every_column_off_the_grid(dtype, rows, d, h, experts):
         _check(rows, d, h, experts, dtype, act, act != "none", "tail" if act == "relu" else "skewed", seed=rows)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("rows,d,h,experts,kind", [(1, 1, 3, 1, "even"), (1, 7, 9, 2, "one"), (2, 63, 65, 3, "even"), (5, 130, 333, 4, "skewed"), (16, 257, 66, 1, "even"),
+                                                   (17, 515, 129, 2, "one"), (40, 1030, 70, 3, "tail"), (47, 449, 1001, 3, "skewed"), (9, 2049, 34, 600, "even"),
+                                                   (150, 1302, 500, 12, "skewed"), (3, 8, 1, 1, "even"), (192, 2500, 11, 12, "skewed")])
+def test_few_rows_off_the_grid(dtype, rows, d, h, experts, kind):
+    for act in ("silu", "none"):
+        _check(rows, d, h, experts, dtype, act, act == "silu", kind, seed=rows)
+
+
+@pytest.mark.parametrize("off", range(1, 8))
+def test_few_rows_from_anywhere(off):
+    """Tensors of sizes on the grid that begin off it."""
+    gen = torch.Generator(device="cuda").manual_seed(off)
+    make = lambda *shape, at: torch.randn(math.prod(shape) + 8, device="cuda", generator=gen).to(torch.bfloat16)[at:at + math.prod(shape)].view(shape)
+    x, w1, w2 = make(6, 192, at=off), make(3, 256, 192, at=off // 2), make(3, 192, 128, at=0)
+    counts = [1, 3, 2]
+    y = functions.gated_mlp(x, torch.tensor(counts, device="cuda"), w1, None, w2, None, torch.nn.SiLU())
+    value, tol = _reference(x, counts, w1, None, w2, None, "silu")["y"]
+    assert ((y.double() - value).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("rows", [13, 16, 47, 48, 49])
 def test_few_rows(rows):
     _check(rows, 512, 1024, 3, torch.bfloat16, "silu", True, "skewed", seed=rows)
