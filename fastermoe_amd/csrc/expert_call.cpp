@@ -53,10 +53,10 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
         const int dtype = dtype_code(x), act = (int)activation;
         const at::Tensor y = at::empty({n, d}, x.options()), mid = at::empty({n, h}, x.options());
         const at::Tensor pre = keep ? at::empty({n, 2 * h}, x.options()) : at::Tensor();
-        const int64_t bytes = entry.gated_forward_bytes(e, n, d, h, dtype, act, keep, 1);
+        const int64_t bytes = entry.gated_forward_bytes(e, n, d, h, dtype, act, keep);
         const at::Tensor space = space_of(bytes, x);
         ok(entry.gated_forward(pointer(x), pointer(w1), pointer(b1), pointer(w2), pointer(b2), pointer(pre), pointer(mid), pointer(y), pointer(table),
-                               nullptr, e, n, d, h, dtype, act, pointer(space), bytes, stream_of(x)));
+                               e, n, d, h, dtype, act, pointer(space), bytes, stream_of(x)));
         if (keep) {
             ctx->save_for_backward({x, w1, w2, pre, mid, table});
             ctx->saved_data["activation"] = activation;
@@ -86,10 +86,10 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
             gb1 = fresh(need_b1, {e, 2 * h});
             gw2 = fresh(need_w2 || need_b2, {e, d, h});
             gb2 = fresh(need_b2, {e, d});
-            const int64_t bytes = entry.gated_backward_bytes(e, n, d, h, dtype_code(x), act, 1);
+            const int64_t bytes = entry.gated_backward_bytes(e, n, d, h, dtype_code(x), act);
             const at::Tensor space = space_of(bytes, x);
             ok(entry.gated_backward(pointer(gy), pointer(x), pointer(w1), pointer(w2), pointer(pre), pointer(mid), pointer(gx), pointer(gw1), pointer(gb1),
-                                    pointer(gw2), pointer(gb2), pointer(table), nullptr, e, n, d, h, dtype_code(x), act, pointer(space), bytes,
+                                    pointer(gw2), pointer(gb2), pointer(table), e, n, d, h, dtype_code(x), act, pointer(space), bytes,
                                     stream_of(x)));
         }
         const at::Tensor none;
@@ -155,8 +155,8 @@ PyObject *fmoe_expert_gated_mlp(PyObject *, PyObject *const *args, Py_ssize_t n_
         (b1.defined() && b1.sizes() != at::IntArrayRef({e, 2 * h})) || (b2.defined() && b2.sizes() != at::IntArrayRef({e, d})) ||
         !good_table(table, x, n, e))
         Py_RETURN_NONE;
-    if (x.scalar_type() == at::kFloat) {   // (over a table in whole 16-byte pieces only)
-        if (entry.dev_supported(d, h, FMOE_F32) != 1 || (x.is_contiguous() && !on_16_bytes(x))) Py_RETURN_NONE;
+    if (x.scalar_type() == at::kFloat) {   // (copied where they are not)
+        if (x.is_contiguous() && !on_16_bytes(x)) Py_RETURN_NONE;
         for (const at::Tensor *p : {&w1, &b1, &w2, &b2})
             if (!on_16_bytes(*p)) Py_RETURN_NONE;
     }

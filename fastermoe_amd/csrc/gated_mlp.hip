@@ -3,8 +3,9 @@
 //   g = x Wg^T + bg,  u = x Wu^T + bu,  m = act(g) u,  y = m W2^T + b2            (W1 = [Wg; Wu], its products [g u] = `pre`)
 //   dm = dy W2,  dg = dm u act'(g),  du = dm act(g),  dx = [dg du] W1,  dW1 = [dg du]^T x,  dW2 = dy^T m
 //
-// This file holds the calls of the whole block and the two kernels between its products for the shapes whose product does not do their work in
-// its epilogue.
+// The products do the activation's work in their epilogues (gemm_kernel.hpp, gemm_ring.hpp, gemm_skinny.hip; rows off the 16-byte grid, 16-bit types:
+// gemm_unaligned.hip, gemm_few_unaligned.hip).  This file holds the calls of the whole block, the activation's kernel for few rows in float32, and the kernel that moves
+// float32 tensors of sizes that are no multiple of four into rows that are, and results back: the padding is zeros, whose g, u and m are zeros too.
 #include "gated_terms.hpp"
 #include "grouped_gemm.hpp"
 #include "lane_elems.hpp"
@@ -46,107 +47,76 @@ template <typename T> struct Tail {
     }
 };
 
-// m = act(g) u.  pre [rows, 2 h], mid [rows, h].  Bound by memory.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void gated_act_fwd_kernel(const T *__restrict__ pre, T *__restrict__ mid, const int32_t *__restrict__ table,
-                                                               int64_t rows, int h, int per_row, int act, const Tail<T> tail) {
+// m = act(g) u for few rows in float32, whose products are the decoding kernel's.  pre [rows, 2 h], mid [rows, h].  Bound by its launch.
+__global__ __launch_bounds__(kBlock) void gated_act_kernel(const float *__restrict__ pre, float *__restrict__ mid, const int32_t *__restrict__ table, int64_t rows,
+                                                           int h, int per_row, int act, const Tail<float> tail) {
     const int64_t all = rows * 2 * h;
     rows = live_rows(table, rows);
     tail.clear(rows);
     const Piece p = piece_of(rows, h, per_row);
     if (p.n <= 0) return;
     const int64_t at = p.row * 2 * h + p.c;
-    T g[kLaneElems], u[kLaneElems];
+    float g[kLaneElems], u[kLaneElems];
     load_elems<false>(pre + at, p.n, at + kLaneElems <= all, g);
     load_elems<false>(pre + at + h, p.n, at + h + kLaneElems <= all, u);
 #pragma unroll
-    for (int j = 0; j < kLaneElems; ++j) g[j] = (T)(gate_act<sizeof(T) == 2>((float)g[j], act) * (float)u[j]);
+    for (int j = 0; j < kLaneElems; ++j) g[j] = gate_act<false>(g[j], act) * u[j];
     store_elems<false>(mid + p.row * h + p.c, p.n, g);
-}
-
-// grad_pre = [dm u act'(g), dm act(g)]
-template <typename T>
-__global__ __launch_bounds__(kBlock) void gated_act_bwd_kernel(const T *__restrict__ grad_mid, const T *__restrict__ pre, T *__restrict__ grad_pre,
-                                                               const int32_t *__restrict__ table, int64_t rows, int h, int per_row, int act,
-                                                               const Tail<T> tail) {
-    const int64_t all = rows * h;
-    rows = live_rows(table, rows);
-    tail.clear(rows);
-    const Piece p = piece_of(rows, h, per_row);
-    if (p.n <= 0) return;
-    const int64_t at = p.row * 2 * h + p.c, at_mid = p.row * h + p.c;
-    T g[kLaneElems], u[kLaneElems], d[kLaneElems];
-    load_elems<false>(pre + at, p.n, at + kLaneElems <= 2 * all, g);
-    load_elems<false>(pre + at + h, p.n, at + h + kLaneElems <= 2 * all, u);
-    load_elems<false>(grad_mid + at_mid, p.n, at_mid + kLaneElems <= all, d);
-#pragma unroll
-    for (int j = 0; j < kLaneElems; ++j) {
-        const ActTerms t = gate_terms<sizeof(T) == 2>((float)g[j], act);
-        const float dm = (float)d[j];
-        g[j] = (T)(dm * (float)u[j] * t.slope);
-        u[j] = (T)(dm * t.value);
-    }
-    store_elems<false>(grad_pre + at, p.n, g);
-    store_elems<false>(grad_pre + at + h, p.n, u);
 }
 
 int per_row(int64_t h) { return (int)ceil_div(h, kLaneElems); }
 
-template <typename F> void with_type(int dtype, F &&f) {
-    if (dtype == FMOE_F32) f(float{});
-    else if (dtype == FMOE_BF16) f(__bf16{});
-    else f(_Float16{});
-}
-
-// `live` rows at most (with a table: those that it has); rows of `tail` behind them become zeros
-struct Between {
+// Rows of float32 from one place into another, in blocks of rows (a matrix half, or all): what of a block or a row the source has none of becomes zeros, what the
+// destination has no room for is left out.
+struct Move {
+    const float *src;
+    float *dst;
+    int64_t rows;                              // of the destination
+    int64_t block_src, block_dst;              // rows of a block
+    int cols_src, cols_dst;
     const int32_t *table;
-    int64_t live, h;
-    int dtype, activation;
-    void *tail;
-    int64_t tail_rows, tail_elems;
-    hipStream_t stream;
+    int rows_of_row;                           // not 0: only rows r with r / rows_of_row below the table's rows
+    int blocks_of_expert;                      // not 0: only blocks of experts with rows
 };
-int gated_act_forward(const void *pre, void *mid, const Between &b) {
-    with_type(b.dtype, [&](auto t) {
-        using T = decltype(t);
-        gated_act_fwd_kernel<T><<<(unsigned)std::max<int64_t>(1, ceil_div(b.live * per_row(b.h), kBlock)), kBlock, 0, b.stream>>>(
-            (const T *)pre, (T *)mid, b.table, b.live, (int)b.h, per_row(b.h), b.activation, Tail<T>{(T *)b.tail, b.tail_rows, (int)b.tail_elems});
-    });
-    FMOE_LAUNCH_CHECK();
-    return FMOE_OK;
-}
-int gated_act_backward(const void *grad_mid, const void *pre, void *grad_pre, const Between &b) {
-    with_type(b.dtype, [&](auto t) {
-        using T = decltype(t);
-        gated_act_bwd_kernel<T><<<(unsigned)std::max<int64_t>(1, ceil_div(b.live * per_row(b.h), kBlock)), kBlock, 0, b.stream>>>(
-            (const T *)grad_mid, (const T *)pre, (T *)grad_pre, b.table, b.live, (int)b.h, per_row(b.h), b.activation,
-            Tail<T>{(T *)b.tail, b.tail_rows, (int)b.tail_elems});
-    });
-    FMOE_LAUNCH_CHECK();
-    return FMOE_OK;
+constexpr int kMoveLoads = 8;
+// A wave to a row, kMoveLoads of a lane's loads on their way at a time (one: 1001 -> 2 x 2003, 8 experts, 1 row, forward 70 us, 52 now).  Bound by memory.
+__global__ __launch_bounds__(kBlock) void move_rows_kernel(const Move m) {
+    const int lane = threadIdx.x % kWave;
+    for (int64_t row = (int64_t)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave; row < m.rows; row += (int64_t)gridDim.x * (kBlock / kWave)) {
+        if (m.rows_of_row && row / m.rows_of_row >= m.table[segtab::kRows]) return;   // (and so do the rows after)
+        const int64_t block = row / m.block_dst, in_block = row - block * m.block_dst;
+        if (m.blocks_of_expert) {
+            const int64_t e = block / m.blocks_of_expert;
+            if (m.table[segtab::kHeader + e] == m.table[segtab::kHeader + e + 1]) continue;
+        }
+        const float *src = m.src + (block * m.block_src + in_block) * m.cols_src;
+        const int n = in_block < m.block_src ? m.cols_src : 0;
+        float *dst = m.dst + row * m.cols_dst;
+        for (int c = lane; c < m.cols_dst; c += kMoveLoads * kWave) {
+            float v[kMoveLoads];
+#pragma unroll
+            for (int j = 0; j < kMoveLoads; ++j) v[j] = c + j * kWave < n ? __builtin_nontemporal_load(src + c + j * kWave) : 0.f;
+#pragma unroll
+            for (int j = 0; j < kMoveLoads; ++j)
+                if (c + j * kWave < m.cols_dst) dst[c + j * kWave] = v[j];
+        }
+    }
 }
 
 struct Sizes {
     int64_t n_expert, rows, d, h;
     int dtype, activation;
 };
-int check(const char *who, const Sizes &s, const void *segment_table, const int64_t *counts_host) {
+int check(const char *who, const Sizes &s) {
     FMOE_REQUIRE(s.dtype == FMOE_F32 || s.dtype == FMOE_BF16 || s.dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who, s.dtype);
     FMOE_REQUIRE(is_gate_activation(s.activation), "%s: unknown activation %d", who, s.activation);
     FMOE_REQUIRE(s.n_expert >= 1 && s.rows >= 0 && s.d >= 1 && s.h >= 1, "%s: bad sizes", who);
-    FMOE_REQUIRE(!segment_table != !counts_host, "%s: either a segment table or the counts on the host", who);
     if (s.n_expert > (1 << 24) || s.rows > (int64_t)INT32_MAX - 65536 || s.d > (1 << 28) || s.h > (1 << 28) ||
         ceil_div(s.rows * per_row(s.h), kBlock) > kMostThreads / kBlock)
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
-    if (counts_host) {
-        int64_t total = 0;
-        for (int64_t e = 0; e < s.n_expert; ++e) {
-            FMOE_REQUIRE(counts_host[e] >= 0 && counts_host[e] <= s.rows, "%s: expert_count[%lld]=%lld", who, (long long)e, (long long)counts_host[e]);
-            total += counts_host[e];
-        }
-        FMOE_REQUIRE(total <= s.rows, "%s: the counts add up to %lld of %lld rows", who, (long long)total, (long long)s.rows);
-    }
+    // (float32, and its rounded sizes: offsets from a tile's first row of weights, over both halves, in 31 bits)
+    if (s.dtype == FMOE_F32 && ((2 * s.h + 264) * (s.d + 3) * 4 >= ((int64_t)1 << 31) || 2 * (s.h + 3) * 4 > (1 << 22)))
+        return fail(FMOE_ELIMIT, "%s: an expert's float32 weights of 2 GiB are beyond the supported range", who);
     return FMOE_OK;
 }
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -161,27 +131,23 @@ GatedArgs gated_sizes(const Sizes &s) {
     a.d = s.d; a.h = s.h; a.n_expert = s.n_expert; a.rows_cap = s.rows; a.dtype = s.dtype; a.activation = s.activation; a.dev_tab = &some;
     return a;
 }
-Scratch forward_scratch(const Sizes &s, bool keeps_pre, bool table) {
-    const bool fused = table && gated_forward_fused(gated_sizes(s));
+Scratch forward_scratch(const Sizes &s, bool keeps_pre) {
+    const bool fused = gated_forward_fused(gated_sizes(s));
     return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)), 0,
                    std::max(fused ? gated_forward_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE, 0, 0),
                             fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0))};
 }
-Scratch backward_scratch(const Sizes &s, bool table) {
-    const bool fused = table && gated_dgrad_fused(gated_sizes(s));
-    const int64_t row = s.rows * s.h * dtype_bytes(s.dtype);
-    return Scratch{round256(2 * row), fused ? 0 : round256(row),
-                   std::max(fused ? gated_dgrad_workspace_bytes(gated_sizes(s))
-                                  : fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE),
+Scratch backward_scratch(const Sizes &s) {
+    return Scratch{round256(2 * s.rows * s.h * dtype_bytes(s.dtype)), 0,
+                   std::max(gated_dgrad_workspace_bytes(gated_sizes(s)),
                             fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE))};
 }
 
-// The products, over a table in device memory or over counts on the host.
+// The products over the table
 struct Products {
     const int32_t *table;
-    const int64_t *counts;
-    int64_t n_expert, rows, total;   // total: rows that there are, or may be
+    int64_t n_expert, rows;
     int dtype;
     void *ws;
     int64_t ws_bytes;
@@ -189,7 +155,7 @@ struct Products {
 
     template <typename Args> void place(Args &a) const {
         a.dev_tab = table;
-        a.dev_rows_cap = table ? rows : 0;
+        a.dev_rows_cap = rows;
         a.dev_any_grid = true;
     }
     int forward(const void *x, const void *w, const void *bias, void *y, int64_t in, int64_t out, bool once) const {
@@ -199,25 +165,174 @@ struct Products {
         a.dev_weights_once = once;   // (no backward that reads them again)
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;
-        return grouped_linear_forward(a, counts, n_expert, 0, total, stream);
+        return grouped_linear_forward(a, nullptr, n_expert, 0, rows, stream);
     }
     int dgrad(const void *gy, const void *w, void *gx, int64_t in, int64_t out) const {
         LinearDgradArgs a{gy, w, gx, nullptr, in, out, dtype, kEpiStore, FMOE_ACT_NONE};
         place(a);
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;
-        return grouped_linear_dgrad(a, counts, n_expert, 0, total, stream);
+        return grouped_linear_dgrad(a, nullptr, n_expert, 0, rows, stream);
     }
     int wgrad(const void *gy, const void *x, void *gw, void *gb, int64_t in, int64_t out) const {
         LinearWgradArgs a{gy, x, gw, gb, in, out, dtype};
         place(a);
-        return grouped_linear_wgrad(a, counts, n_expert, 0, total, true, stream);
+        return grouped_linear_wgrad(a, nullptr, n_expert, 0, rows, true, stream);
     }
 };
-Products products(const Sizes &s, const void *segment_table, const int64_t *counts, void *ws, int64_t ws_bytes, void *stream) {
-    int64_t total = 0;
-    for (int64_t e = 0; counts && e < s.n_expert; ++e) total += counts[e];
-    return Products{(const int32_t *)segment_table, counts, s.n_expert, s.rows, segment_table ? s.rows : total, s.dtype, ws, ws_bytes, (hipStream_t)stream};
+
+struct Forward {
+    const void *x, *w1, *b1, *w2, *b2;
+    void *pre, *mid, *y;
+};
+struct Backward {
+    const void *grad_y, *x, *w1, *w2, *pre, *mid;
+    void *grad_x, *grad_w1, *grad_b1, *grad_w2, *grad_b2;
+};
+
+int forward(const Sizes &s, const Forward &f, const int32_t *table, char *ws, hipStream_t stream) {
+    const Scratch need = forward_scratch(s, f.pre != nullptr);
+    const Products p{table, s.n_expert, s.rows, s.dtype, ws + need.first, need.split, stream};
+    const GatedArgs fused{f.x, f.w1, f.b1, f.pre, f.mid, f.y, s.d, s.h, s.n_expert, s.rows, s.dtype, s.activation, table, p.ws, p.ws_bytes};
+    const bool once = f.pre == nullptr;
+    if (gated_forward_fused(fused)) {
+        if (int rc = grouped_gated_forward(fused, stream)) return rc;
+    } else {
+        void *pre = f.pre ? f.pre : ws;
+        if (int rc = p.forward(f.x, f.w1, f.b1, pre, s.d, 2 * s.h, once)) return rc;
+        gated_act_kernel<<<(unsigned)std::max<int64_t>(1, ceil_div(s.rows * per_row(s.h), kBlock)), kBlock, 0, stream>>>(
+            (const float *)pre, (float *)f.mid, table, s.rows, (int)s.h, per_row(s.h), s.activation, Tail<float>{(float *)f.y, s.rows, (int)s.d});
+        FMOE_LAUNCH_CHECK();
+    }
+    return p.forward(f.mid, f.w2, f.b2, f.y, s.h, s.d, once);
+}
+
+int backward(const Sizes &s, const Backward &b, const int32_t *table, char *ws, hipStream_t stream) {
+    const Scratch need = s.rows == 0 ? Scratch{0, 0, 0} : backward_scratch(s);
+    const Products p{table, s.n_expert, s.rows, s.dtype, ws + need.first, need.split, stream};
+    void *grad_pre = ws;
+    if (s.rows > 0 && (b.grad_x || b.grad_w1)) {
+        const GatedArgs fused{b.grad_y, b.w2, nullptr, const_cast<void *>(b.pre), grad_pre, b.grad_x, s.d, s.h, s.n_expert, s.rows, s.dtype, s.activation, table,
+                              p.ws, p.ws_bytes};
+        if (int rc = grouped_gated_dgrad(fused, stream)) return rc;
+    }
+    if (b.grad_w2)
+        if (int rc = p.wgrad(b.grad_y, b.mid, b.grad_w2, b.grad_b2, s.h, s.d)) return rc;
+    if (b.grad_x && s.rows > 0)
+        if (int rc = p.dgrad(grad_pre, b.w1, b.grad_x, s.d, 2 * s.h)) return rc;
+    if (b.grad_w1)
+        if (int rc = p.wgrad(grad_pre, b.x, b.grad_w1, b.grad_b1, s.d, 2 * s.h)) return rc;
+    return FMOE_OK;
+}
+
+// float32 in sizes that are no multiple of four: the same with sizes that are, on copies.  (With products that check every
+// element, over counts read on the host, us forward and with the backward, and like this: 1 row, 8 experts of 1001 -> 2 x 2003: 180, 493 / 52, 286; 64 rows, 33 of 443 -> 2 x
+// 2368: 300, 801 / 199, 818; 1554 rows, 12 of 501 -> 2 x 1303: 257, 677 / 137, 425; 8192 rows, 8 of 1023 -> 2 x 2047: 2088, 5494 / 713, 2294.)
+bool padded(const Sizes &s) { return s.dtype == FMOE_F32 && (s.d % 4 != 0 || s.h % 4 != 0); }
+Sizes whole(const Sizes &s) {
+    Sizes w = s;
+    w.d = ceil_div(s.d, 4) * 4;
+    w.h = ceil_div(s.h, 4) * 4;
+    return w;
+}
+struct Copies {
+    Sizes s, w;
+    const int32_t *table;
+    char *ws;          // null: only the sizes are added up
+    hipStream_t stream;
+    int64_t used = 0;
+    int rc = FMOE_OK;
+
+    float *room(int64_t floats) {
+        float *at = ws ? (float *)(ws + used) : nullptr;
+        used += round256(floats * 4);
+        return at;
+    }
+    void move(const void *src, void *dst, int64_t blocks, int64_t block_src, int64_t block_dst, int64_t cols_src, int64_t cols_dst, int rows_of_row,
+              int blocks_of_expert) {
+        if (ws == nullptr || src == nullptr || dst == nullptr || rc != FMOE_OK) return;
+        const Move m{(const float *)src, (float *)dst, blocks * block_dst, block_src, block_dst, (int)cols_src, (int)cols_dst, table, rows_of_row, blocks_of_expert};
+        move_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(m.rows, kBlock / kWave), 1 << 20), kBlock, 0, stream>>>(m);
+        rc = launched();
+    }
+    static int launched() {
+        FMOE_LAUNCH_CHECK();
+        return FMOE_OK;
+    }
+    // [rows, halves * h or d] of a call's rows; back: all of them, or those that there are
+    float *rows_in(const void *t, int halves, bool hidden) {
+        float *at = room(s.rows * halves * (hidden ? w.h : w.d));
+        move(t, at, 1, s.rows * halves, s.rows * halves, hidden ? s.h : s.d, hidden ? w.h : w.d, halves, 0);
+        return at;
+    }
+    void rows_out(const float *at, void *t, int halves, bool hidden, bool all) {
+        move(at, t, 1, s.rows * halves, s.rows * halves, hidden ? w.h : w.d, hidden ? s.h : s.d, all ? 0 : halves, 0);
+    }
+    // W1 [E, 2 h, d] and b1 [E, 2 h], W2 [E, d, h] and b2 [E, d]
+    float *w1_in(const void *t) { float *at = room(s.n_expert * 2 * w.h * w.d); move(t, at, 2 * s.n_expert, s.h, w.h, s.d, w.d, 0, 2); return at; }
+    float *b1_in(const void *t) { float *at = room(s.n_expert * 2 * w.h); move(t, at, 1, 2 * s.n_expert, 2 * s.n_expert, s.h, w.h, 0, 0); return t ? at : nullptr; }
+    float *w2_in(const void *t) { float *at = room(s.n_expert * w.d * w.h); move(t, at, s.n_expert, s.d, w.d, s.h, w.h, 0, 1); return at; }
+    float *b2_in(const void *t) { float *at = room(s.n_expert * w.d); move(t, at, 1, s.n_expert, s.n_expert, s.d, w.d, 0, 0); return t ? at : nullptr; }
+    void w1_out(const float *at, void *t) { move(at, t, 2 * s.n_expert, w.h, s.h, w.d, s.d, 0, 0); }
+    void b1_out(const float *at, void *t) { move(at, t, 1, 2 * s.n_expert, 2 * s.n_expert, w.h, s.h, 0, 0); }
+    void w2_out(const float *at, void *t) { move(at, t, s.n_expert, w.d, s.d, w.h, s.h, 0, 0); }
+    void b2_out(const float *at, void *t) { move(at, t, 1, s.n_expert, s.n_expert, w.d, s.d, 0, 0); }
+};
+// (ws null: the workspace's bytes in *bytes)
+int padded_forward(const Sizes &s, const Forward &f, const int32_t *table, char *ws, int64_t *bytes, hipStream_t stream) {
+    const Sizes w = whole(s);
+    Copies c{s, w, table, ws, stream};
+    Forward g{};
+    g.x = c.rows_in(f.x, 1, false);
+    g.w1 = c.w1_in(f.w1); g.b1 = c.b1_in(f.b1); g.w2 = c.w2_in(f.w2); g.b2 = c.b2_in(f.b2);
+    float *mid = c.room(s.rows * w.h), *y = c.room(s.rows * w.d), *pre = f.pre ? c.room(s.rows * 2 * w.h) : nullptr;
+    g.mid = mid; g.y = y; g.pre = pre;
+    if (ws == nullptr) {
+        *bytes = c.used + forward_scratch(w, f.pre != nullptr).total();
+        return FMOE_OK;
+    }
+    if (c.rc == FMOE_OK) c.rc = forward(w, g, table, ws + c.used, stream);
+    c.rows_out(y, f.y, 1, false, true);
+    if (f.pre) {
+        c.rows_out(pre, f.pre, 2, true, false);
+        c.rows_out(mid, f.mid, 1, true, false);
+    }
+    return c.rc;
+}
+int padded_backward(const Sizes &s, const Backward &b, const int32_t *table, char *ws, int64_t *bytes, hipStream_t stream) {
+    const Sizes w = whole(s);
+    Copies c{s, w, table, ws, stream};
+    Backward g{};
+    g.grad_y = c.rows_in(b.grad_y, 1, false); g.x = c.rows_in(b.x, 1, false);
+    g.w1 = c.w1_in(b.w1); g.w2 = c.w2_in(b.w2);
+    g.pre = c.rows_in(b.pre, 2, true); g.mid = c.rows_in(b.mid, 1, true);
+    float *gx = c.room(s.rows * w.d), *gw1 = c.room(s.n_expert * 2 * w.h * w.d), *gb1 = c.room(s.n_expert * 2 * w.h);
+    float *gw2 = c.room(s.n_expert * w.d * w.h), *gb2 = c.room(s.n_expert * w.d);
+    if (ws == nullptr) {
+        *bytes = c.used + (s.rows == 0 ? 0 : backward_scratch(w).total());
+        return FMOE_OK;
+    }
+    g.grad_x = b.grad_x ? gx : nullptr; g.grad_w1 = b.grad_w1 ? gw1 : nullptr; g.grad_b1 = b.grad_b1 ? gb1 : nullptr;
+    g.grad_w2 = b.grad_w2 ? gw2 : nullptr; g.grad_b2 = b.grad_b2 ? gb2 : nullptr;
+    if (c.rc == FMOE_OK) c.rc = backward(w, g, table, ws + c.used, stream);
+    if (s.rows > 0) c.rows_out(gx, b.grad_x, 1, false, true);
+    c.w1_out(gw1, b.grad_w1); c.b1_out(gb1, b.grad_b1); c.w2_out(gw2, b.grad_w2); c.b2_out(gb2, b.grad_b2);
+    return c.rc;
+}
+int64_t forward_bytes(const Sizes &s, bool keep) {
+    if (!padded(s)) return forward_scratch(s, keep).total();
+    static char some;
+    Forward f{};
+    f.pre = keep ? &some : nullptr;
+    int64_t bytes = 0;
+    padded_forward(s, f, nullptr, nullptr, &bytes, nullptr);
+    return bytes;
+}
+int64_t backward_bytes(const Sizes &s) {
+    if (!padded(s)) return s.rows == 0 ? 0 : backward_scratch(s).total();
+    int64_t bytes = 0;
+    padded_backward(s, Backward{}, nullptr, nullptr, &bytes, nullptr);
+    return bytes;
 }
 
 }  // namespace
@@ -225,75 +340,55 @@ Products products(const Sizes &s, const void *segment_table, const int64_t *coun
 
 using namespace fmoe;
 
-extern "C" int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,
-                                                          int activation, int keep, int table) {
+extern "C" int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype, int activation,
+                                                          int keep) {
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
-    static const int64_t one = 0;
-    if (rows < 1 || n_expert < 1 || check("fmoe_gated_mlp_forward", s, &one, nullptr) != FMOE_OK) return 0;
-    return forward_scratch(s, keep != 0, table != 0).total();
+    if (rows < 1 || check("fmoe_gated_mlp_forward", s) != FMOE_OK) return 0;
+    return forward_bytes(s, keep != 0);
 }
 
 extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1, const void *w2, const void *b2, void *pre, void *mid, void *y,
-                                      const void *segment_table, const int64_t *expert_count_host, int64_t n_expert, int64_t rows, int64_t d_model,
-                                      int64_t d_hidden, int dtype, int activation, void *workspace, int64_t workspace_bytes, void *stream) {
+                                      const void *segment_table, int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,
+                                      int activation, void *workspace, int64_t workspace_bytes, void *stream) {
     const char *who = "fmoe_gated_mlp_forward";
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
-    if (int rc = check(who, s, segment_table, expert_count_host)) return rc;
+    if (int rc = check(who, s)) return rc;
     if (rows == 0) return FMOE_OK;
-    FMOE_REQUIRE(x && w1 && w2 && mid && y, "%s: NULL pointer", who);
-    const Scratch need = forward_scratch(s, pre != nullptr, segment_table != nullptr);
-    if (need.total() > 0 && (workspace == nullptr || workspace_bytes < need.total() || !aligned16(workspace)))
-        return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need.total());
-    char *ws = (char *)workspace;
-    const Products p = products(s, segment_table, expert_count_host, ws + need.first, need.split, stream);
-    const GatedArgs fused{x, w1, b1, pre, mid, y, d_model, d_hidden, n_expert, rows, dtype, activation, p.table, p.ws, p.ws_bytes};
-    if (gated_forward_fused(fused)) {
-        if (int rc = grouped_gated_forward(fused, p.stream)) return rc;
-        return p.forward(mid, w2, b2, y, d_hidden, d_model, pre == nullptr);
-    }
-    void *between = pre ? pre : ws;
-    if (int rc = p.forward(x, w1, b1, between, d_model, 2 * d_hidden, pre == nullptr)) return rc;
-    if (int rc = gated_act_forward(between, mid, Between{p.table, p.total, d_hidden, dtype, activation, y, rows, d_model, p.stream})) return rc;
-    return p.forward(mid, w2, b2, y, d_hidden, d_model, pre == nullptr);
+    FMOE_REQUIRE(x && w1 && w2 && mid && y && segment_table, "%s: NULL pointer", who);
+    FMOE_REQUIRE(aligned16(segment_table), "%s: the segment table must be 16-byte aligned", who);
+    FMOE_REQUIRE(dtype != FMOE_F32 || (aligned16(x) && aligned16(w1) && aligned16(b1) && aligned16(w2) && aligned16(b2) && aligned16(pre) && aligned16(mid) &&
+                                       aligned16(y)), "%s: float32 tensors begin on 16 bytes", who);
+    const int64_t need = forward_bytes(s, pre != nullptr);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need);
+    const Forward f{x, w1, b1, w2, b2, pre, mid, y};
+    if (padded(s)) return padded_forward(s, f, (const int32_t *)segment_table, (char *)workspace, nullptr, (hipStream_t)stream);
+    return forward(s, f, (const int32_t *)segment_table, (char *)workspace, (hipStream_t)stream);
 }
 
-extern "C" int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype,
-                                                           int activation, int table) {
+extern "C" int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype, int activation) {
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
-    static const int64_t one = 0;
-    if (rows < 1 || n_expert < 1 || check("fmoe_gated_mlp_backward", s, &one, nullptr) != FMOE_OK) return 0;
-    return backward_scratch(s, table != 0).total();
+    if (check("fmoe_gated_mlp_backward", s) != FMOE_OK) return 0;
+    return backward_bytes(s);
 }
 
 extern "C" int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1, const void *w2, const void *pre, const void *mid,
                                        void *grad_x, void *grad_w1, void *grad_b1, void *grad_w2, void *grad_b2, const void *segment_table,
-                                       const int64_t *expert_count_host, int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden,
-                                       int dtype, int activation, void *workspace, int64_t workspace_bytes, void *stream) {
+                                       int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype, int activation, void *workspace,
+                                       int64_t workspace_bytes, void *stream) {
     const char *who = "fmoe_gated_mlp_backward";
     const Sizes s{n_expert, rows, d_model, d_hidden, dtype, activation};
-    if (int rc = check(who, s, segment_table, expert_count_host)) return rc;
+    if (int rc = check(who, s)) return rc;
     FMOE_REQUIRE((!grad_b1 || grad_w1) && (!grad_b2 || grad_w2), "%s: a bias gradient comes with its weight's", who);
-    FMOE_REQUIRE(rows == 0 || (grad_y && x && w1 && w2 && pre && mid), "%s: NULL pointer", who);
-    const Scratch need = rows == 0 ? Scratch{0, 0, 0} : backward_scratch(s, segment_table != nullptr);
-    if (need.total() > 0 && (workspace == nullptr || workspace_bytes < need.total() || !aligned16(workspace)))
-        return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need.total());
-    char *ws = (char *)workspace;
-    const Products p = products(s, segment_table, expert_count_host, ws + need.first + need.second, need.split, stream);
-    void *grad_pre = ws, *grad_mid = ws + need.first;
-    const GatedArgs fused{grad_y, w2, nullptr, const_cast<void *>(pre), grad_pre, grad_x, d_model, d_hidden, n_expert, rows, dtype, activation, p.table,
-                          p.ws, p.ws_bytes};
-    if (rows > 0 && (grad_x || grad_w1) && gated_dgrad_fused(fused)) {
-        if (int rc = grouped_gated_dgrad(fused, p.stream)) return rc;
-    } else if (rows > 0 && (grad_x || grad_w1)) {
-        if (int rc = p.dgrad(grad_y, w2, grad_mid, d_hidden, d_model)) return rc;
-        if (int rc = gated_act_backward(grad_mid, pre, grad_pre, Between{p.table, p.total, d_hidden, dtype, activation, grad_x, rows, d_model, p.stream}))
-            return rc;
-    }
-    if (grad_w2)
-        if (int rc = p.wgrad(grad_y, mid, grad_w2, grad_b2, d_hidden, d_model)) return rc;
-    if (grad_x && rows > 0)
-        if (int rc = p.dgrad(grad_pre, w1, grad_x, d_model, 2 * d_hidden)) return rc;
-    if (grad_w1)
-        if (int rc = p.wgrad(grad_pre, x, grad_w1, grad_b1, d_model, 2 * d_hidden)) return rc;
-    return FMOE_OK;
+    FMOE_REQUIRE((rows == 0 || (grad_y && x && w1 && w2 && pre && mid)) && segment_table, "%s: NULL pointer", who);
+    FMOE_REQUIRE(aligned16(segment_table), "%s: the segment table must be 16-byte aligned", who);
+    FMOE_REQUIRE(dtype != FMOE_F32 || (aligned16(grad_y) && aligned16(x) && aligned16(w1) && aligned16(w2) && aligned16(pre) && aligned16(mid) &&
+                                       aligned16(grad_x) && aligned16(grad_w1) && aligned16(grad_b1) && aligned16(grad_w2) && aligned16(grad_b2)),
+                 "%s: float32 tensors begin on 16 bytes", who);
+    const int64_t need = backward_bytes(s);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need);
+    const Backward b{grad_y, x, w1, w2, pre, mid, grad_x, grad_w1, grad_b1, grad_w2, grad_b2};
+    if (padded(s)) return padded_backward(s, b, (const int32_t *)segment_table, (char *)workspace, nullptr, (hipStream_t)stream);
+    return backward(s, b, (const int32_t *)segment_table, (char *)workspace, (hipStream_t)stream);
 }

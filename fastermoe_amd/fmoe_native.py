@@ -916,34 +916,31 @@ def _gated_args(x, w1, b1, w2, b2):
     return dt, e, x.shape[0], d, h
 
 
-def _gated_segments(table, counts, n_expert, rows, device):
-    """Pointers of a segment table or of the counts on the host, one of which there is."""
-    if table is not None:
-        return _ptr(_exact_table(table, n_expert, rows, device)), None, None
-    counts = _host_counts("expert_count", counts, n_expert)
-    return None, ctypes.c_void_p(counts.data_ptr()), counts
+def _gated_float32(dtype, *tensors):
+    """``tensors`` (or ``None``) as the gated calls take them: float32 ones from addresses of whole 16 bytes."""
+    return [t if t is None or dtype != torch.float32 else _on_16_bytes(t) for t in tensors]
 
 
-def gated_mlp_forward(x, w1, b1, w2, b2, activation, table=None, expert_count=None, keep=True):
+def gated_mlp_forward(x, w1, b1, w2, b2, activation, table, keep=True):
     """``(y, pre, mid)`` of gated experts: ``pre = x @ w1_e^T + b1_e`` (a gate's half and a linear one), ``mid = act(gate) * linear``,
-    ``y = mid @ w2_e^T + b2_e``.  The rows' segments: ``table`` (:func:`segment_table` for as many rows as ``x`` has), or ``expert_count`` (int64, CPU).
+    ``y = mid @ w2_e^T + b2_e``.  ``table``: the rows' segments, :func:`segment_table` for as many rows as ``x`` has.
     ``keep=False``: ``pre`` and ``mid`` are ``None``.  Rows of ``y`` behind the experts' are zeros."""
     dt, e, n, d, h = _gated_args(x, w1, b1, w2, b2)
     activation = _gate_activation(activation)
-    seg, cnt, hold = _gated_segments(table, expert_count, e, n, x.device)
+    _exact_table(table, e, n, x.device)
+    x, w1, b1, w2, b2 = _gated_float32(x.dtype, x, w1, b1, w2, b2)
     y = torch.empty(n, d, dtype=x.dtype, device=x.device)
     pre = torch.empty(n, 2 * h, dtype=x.dtype, device=x.device) if keep else None
     mid = torch.empty(n, h, dtype=x.dtype, device=x.device)
     lib = _lib.load()
     with _on(x.device):
-        ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep),
-                                                                       int(table is not None)), x.device)
-        check(lib.fmoe_gated_mlp_forward(_ptr(x), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(pre), _ptr(mid), _ptr(y), seg, cnt, e, n, d, h, dt,
+        ws = _workspace(lib.fmoe_gated_mlp_forward_workspace_bytes(e, n, d, h, dt, activation, int(keep)), x.device)
+        check(lib.fmoe_gated_mlp_forward(_ptr(x), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(pre), _ptr(mid), _ptr(y), _ptr(table), e, n, d, h, dt,
                                          activation, _ptr(ws), ws.numel(), _stream(x)))
     return y, pre, mid if keep else None
 
 
-def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table=None, expert_count=None, want_x=True, want_w1=True, want_b1=True,
+def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table, want_x=True, want_w1=True, want_b1=True,
                        want_w2=True, want_b2=True):
     """``(grad_x, grad_w1, grad_b1, grad_w2, grad_b2)`` from what :func:`gated_mlp_forward` left; ``None`` where not wanted."""
     dt, e, n, d, h = _gated_args(x, w1, None, w2, None)
@@ -952,17 +949,17 @@ def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table=None, expe
         _near(name, _dev(name, t, x.dtype), x.device)
         if tuple(t.shape) != shape:
             raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    seg, cnt, hold = _gated_segments(table, expert_count, e, n, x.device)
+    _exact_table(table, e, n, x.device)
+    grad_y, x, w1, w2, pre, mid = _gated_float32(x.dtype, grad_y, x, w1, w2, pre, mid)
     new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None
     grad_x = new(want_x, n, d)
     grad_w1, grad_b1 = new(want_w1 or want_b1, e, 2 * h, d), new(want_b1, e, 2 * h)
     grad_w2, grad_b2 = new(want_w2 or want_b2, e, d, h), new(want_b2, e, d)
     lib = _lib.load()
     with _on(x.device):
-        ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation,
-                                                                        int(table is not None)), x.device)
+        ws = _workspace(lib.fmoe_gated_mlp_backward_workspace_bytes(e, n, d, h, dt, activation), x.device)
         check(lib.fmoe_gated_mlp_backward(_ptr(grad_y), _ptr(x), _ptr(w1), _ptr(w2), _ptr(pre), _ptr(mid), _ptr(grad_x), _ptr(grad_w1), _ptr(grad_b1),
-                                          _ptr(grad_w2), _ptr(grad_b2), seg, cnt, e, n, d, h, dt, activation, _ptr(ws), ws.numel(), _stream(x)))
+                                          _ptr(grad_w2), _ptr(grad_b2), _ptr(table), e, n, d, h, dt, activation, _ptr(ws), ws.numel(), _stream(x)))
     return grad_x, grad_w1 if want_w1 else None, grad_b1, grad_w2 if want_w2 else None, grad_b2
 
 

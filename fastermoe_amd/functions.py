@@ -765,42 +765,27 @@ def _checked_counts(expert_count, n_expert, rows):
     return counts
 
 
-def _segments_on_host(expert_count, table, n_expert, rows):
-    """The counts of ``table`` or ``expert_count`` on the CPU (read from the device where they are there)."""
-    if table is not None:
-        at = table[8:8 + n_expert + 1].cpu().to(torch.int64)
-        return at[1:] - at[:-1]
-    return _checked_counts(expert_count.cpu() if isinstance(expert_count, torch.Tensor) else expert_count, n_expert, rows)
-
-
 class GatedMLP(Function):
-    r"""Gated experts over expert-sorted rows as one node (see :func:`gated_mlp`); ``counts``: on the CPU, in a table's place."""
+    r"""Gated experts over expert-sorted rows as one node (see :func:`gated_mlp`)."""
 
     @staticmethod
-    def forward(ctx, inp, w1, b1, w2, b2, table, counts, activation, keep):
+    def forward(ctx, inp, w1, b1, w2, b2, table, activation, keep):
         inp = inp.contiguous()
-        out, pre, mid = fmoe_native.gated_mlp_forward(inp, w1, b1, w2, b2, activation, table, counts, keep)
+        out, pre, mid = fmoe_native.gated_mlp_forward(inp, w1, b1, w2, b2, activation, table, keep)
         if keep:
-            ctx.save_for_backward(inp, w1, w2, pre, mid, table, counts)
+            ctx.save_for_backward(inp, w1, w2, pre, mid, table)
             ctx.moe_args = activation, b1 is not None, b2 is not None
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        inp, w1, w2, pre, mid, table, counts = map(_as_chunks, ctx.saved_tensors)
+        inp, w1, w2, pre, mid, table = map(_as_chunks, ctx.saved_tensors)
         activation, bias1, bias2 = ctx.moe_args
         need = ctx.needs_input_grad
-        grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), inp, w1, w2, pre, mid, activation, table, counts, need[0], need[1],
+        grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), inp, w1, w2, pre, mid, activation, table, need[0], need[1],
                                                bias1 and need[2], need[3], bias2 and need[4])
-        return (*grads, None, None, None, None)
-
-
-def _over_a_table(inp, w1, w2, *biases):
-    """Whether a gated block runs over a table on the device: 16-bit types always, float32 in sizes and from addresses of whole 16 bytes."""
-    return inp.dtype != torch.float32 or (
-        fmoe_native.linear_dev_supported(inp.shape[1], w2.shape[2] if w2.dim() == 3 else 0, inp.dtype)
-        and all(t is None or t.data_ptr() % 16 == 0 for t in (inp, w1, w2, *biases)))
+        return (*grads, None, None, None)
 
 
 def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
@@ -810,7 +795,7 @@ def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
     ``ACT_*`` code.  ``expert_count`` (int64 ``[E]``): rows of each expert, on the device (nothing is read back) or the CPU; or ``table``,
     their :func:`fmoe_native.segment_table` for as many rows, which a routing call leaves.  Rows behind the counted ones come out as
     zeros, and so do their gradients.  Differentiable once, with respect to ``inp``, the weights and the biases; the gradients are made from ``g``, ``u``
-    and ``act(g) * u`` as ``inp``'s type holds them.  (float32 in sizes or from addresses that are no multiple of 16 bytes: the counts are read on the host.)"""
+    and ``act(g) * u`` as ``inp``'s type holds them."""
     code = _gate_activation_code(activation)
     module = _lib.load_layer_call()
     if module is not None and nothing_watches(*(t for t in (inp, w1, b1, w2, b2, table) if t is not None)):
@@ -821,13 +806,9 @@ def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
             if out is not None:
                 return out
     fmoe_native._gated_args(inp if inp.is_contiguous() else inp.contiguous(), w1, b1, w2, b2)
-    counts = None
-    if _over_a_table(inp, w1, w2, b1, b2):
-        table = _segments(expert_count, table, w1.shape[0], inp.shape[0], inp.device)
-    else:
-        counts, table = _segments_on_host(expert_count, table, w1.shape[0], inp.shape[0]), None
+    table = _segments(expert_count, table, w1.shape[0], inp.shape[0], inp.device)
     keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (inp, w1, b1, w2, b2))
-    return GatedMLP.apply(inp, w1, b1, w2, b2, table, counts, code, keep)
+    return GatedMLP.apply(inp, w1, b1, w2, b2, table, code, keep)
 
 
 def quantize_rows(inp):
@@ -882,7 +863,7 @@ class MOERoutedGatedMLP(Function):
         top_k, activation, bias1, bias2 = ctx.moe_args
         need = ctx.needs_input_grad
         rows = fmoe_native.gather_rows(inp, pos_buf, index_div=top_k)   # (made again, not kept: see MOERoutedMLP)
-        g_rows, *grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), rows, w1, w2, pre, mid, activation, table, None, need[0], need[1],
+        g_rows, *grads = fmoe_native.gated_mlp_backward(_as_chunks(grad_out), rows, w1, w2, pre, mid, activation, table, need[0], need[1],
                                                         bias1 and need[2], need[3], bias2 and need[4])
         del rows
         g_inp = fmoe_native.reduce_slots(g_rows, slot_to_row, inp.shape[0], top_k) if need[0] else None

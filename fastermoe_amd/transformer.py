@@ -6,7 +6,7 @@ import torch.nn as nn
 
 from . import _lib, fmoe_native
 from .functions import (MOEExpertMLP, MOEExpertMLPCheckpointed, MOERoutedGatedMLP, MOERoutedMLP, MOERoutedMLPCheckpointed,
-                        _gate_activation_code, _no_hooks, _over_a_table, add_layer_norm, gated_mlp, layer_call, layer_norm, linear_int8,
+                        _gate_activation_code, _no_hooks, add_layer_norm, gated_mlp, layer_call, layer_norm, linear_int8,
                         nothing_watches, quantize_rows)
 from .gates import NaiveGate
 from .layers import FMoE, FMoELinear
@@ -186,8 +186,7 @@ class _GatedExpert(_Expert):
         return True   # (the pipeline has no gated experts)
 
     def _device_tables_apply(self, inp):
-        return (self._one_call(inp) is not None and os.environ.get("FMOE_DEVICE_TABLES", "1") != "0"
-                and _over_a_table(inp, self.htoh4.weight, self.h4toh.weight, self.htoh4.bias, self.h4toh.bias))
+        return self._one_call(inp) is not None and os.environ.get("FMOE_DEVICE_TABLES", "1") != "0"
 
 
 class _Int8Expert(nn.Module):

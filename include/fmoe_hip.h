@@ -740,19 +740,16 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
  * [rows, d_hidden] and y [rows, d_model]; behind the rows that the experts have
  * y is zero, pre and mid are left as they are.
  * The rows' segments come from segment_table (of fmoe_segment_table_build for
- * `rows` rows; 16-bit types of any sizes, FMOE_F32 as fmoe_linear_dev_supported
- * says and with tensors on 16 bytes), or else from expert_count_host (any sizes).
- * FMOE_F32 / FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
+ * `rows` rows).  FMOE_F32 (tensors on 16 bytes, an expert's weights below 2 GiB) /
+ * FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
  * The workspace (on 16 bytes) belongs to the call until it has run.  Its size: keep
- * not 0 where pre is given, table not 0 where a segment table is. */
+ * not 0 where pre is given. */
 int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                int64_t d_model, int64_t d_hidden,
-                                               int dtype, int activation, int keep,
-                                               int table);
+                                               int dtype, int activation, int keep);
 int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
                            const void *w2, const void *b2, void *pre, void *mid,
-                           void *y, const void *segment_table,
-                           const int64_t *expert_count_host, int64_t n_expert,
+                           void *y, const void *segment_table, int64_t n_expert,
                            int64_t rows, int64_t d_model, int64_t d_hidden,
                            int dtype, int activation, void *workspace,
                            int64_t workspace_bytes, void *stream);
@@ -763,13 +760,12 @@ int fmoe_gated_mlp_forward(const void *x, const void *w1, const void *b1,
  * behind the experts'. */
 int64_t fmoe_gated_mlp_backward_workspace_bytes(int64_t n_expert, int64_t rows,
                                                 int64_t d_model, int64_t d_hidden,
-                                                int dtype, int activation, int table);
+                                                int dtype, int activation);
 int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const void *w1,
                             const void *w2, const void *pre, const void *mid,
                             void *grad_x, void *grad_w1, void *grad_b1,
                             void *grad_w2, void *grad_b2, const void *segment_table,
-                            const int64_t *expert_count_host, int64_t n_expert,
-                            int64_t rows, int64_t d_model, int64_t d_hidden,
+                            int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden,
                             int dtype, int activation, void *workspace,
                             int64_t workspace_bytes, void *stream);
 
