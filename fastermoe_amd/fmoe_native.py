@@ -1067,10 +1067,10 @@ def linear_int8(x, table, weight, weight_scale, bias=None, activation=_lib.ACT_N
     if gated and out % 2:
         raise ValueError(f"a gated product's weight has an even number of rows, got {out}")
     if bias is not None:
+        bias = _on_16_bytes(bias) if isinstance(bias, torch.Tensor) else bias
         _near("bias", _dev("bias", bias, x.dtype), x.device)
         if tuple(bias.shape) != (e, out):
             raise ValueError(f"bias must be {(e, out)}, got {tuple(bias.shape)}")
-        bias = _on_16_bytes(bias)
     n = _rows_to_round(x, row_index, index_div)[2]
     out = out // 2 if gated else out
     _exact_table(table, e, n, x.device)
