@@ -6,7 +6,9 @@
 // result.  v_mfma_i32_16x16x64_i8 takes 16 bytes of a row per lane, as the 16-bit forms do, so slabs of 128 bytes, their LDS image and its swizzle are those of
 // gemm_kernel.hpp.
 //
-// The kernels are those of 16-bit types (gemm_kernel.hpp, gemm_ring.hpp, gemm_skinny.hip); this file holds the call.
+// The kernels are those of 16-bit types (gemm_kernel.hpp, gemm_ring.hpp, gemm_skinny.hip); this file holds the call.  Few rows are bound by the weights' way from memory
+// (64 sequences of two experts each, 8 experts of 4096 -> 2 x 14336: 165 us, 5.7 TB/s), many by the matrix pipe and at last by the card's power (32768 rows there:
+// 2.93 ms, 2620 TOP/s; of zeros 3560), between them by a last round of tiles that is partly filled (8192 rows, 16 experts of 2048 -> 2048: 56 us, 1220).
 #include "gemm_int8.hpp"
 #include "gated_terms.hpp"
 

@@ -8,7 +8,7 @@
 //
 // A lane takes eight elements at a time.  A row that fits the registers of its wave, or, longer (or where rows are few), of its workgroup's four waves, is read once; a
 // longer one is read again, from the caches.  Bound by memory, and next by 7 instructions an element (18 with a conversion and a correction for each: 354 us for 32768
-// rows of 14336 in bfloat16).
+// rows of 14336 in bfloat16, 250 now, 5.6 TB/s); few rows by the chain of a load, the row's largest and a store (1018 rows of 1302: 4.3 us).
 #include "common.hpp"
 #include "grouped_gemm.hpp"
 #include "row_rounding.hpp"
@@ -19,7 +19,7 @@ namespace fmoe {
 namespace {
 
 constexpr int kBlock = 256, kWaves = kBlock / kWave;
-constexpr int64_t kManyRows = 2048;
+constexpr int64_t kManyRows = 1024;   // a row's pieces times this
 
 struct Params {
     const void *x;
@@ -111,12 +111,13 @@ template <typename T> int launch(const Params &prm, hipStream_t stream) {
     typedef std::integral_constant<int, 4> Four;
     typedef std::integral_constant<int, 8> Eight8;
     const int pieces = (int)ceil_div(prm.dq, kWave * kLaneElems);   // of a wave
-    // A wave to a row where there are rows enough for that to fill the card.
-    const bool many = prm.rows >= kManyRows;
+    // A wave to a row where there are rows enough for that to fill the card, and its pieces are few.  us with a wave / a workgroup to a row, in a graph, bfloat16: rows of
+    // 1024, 1024 of them: 3.9 / 3.6, 2048: 4.1 / 4.6, 32768: 17.8 / 30.1; of 2048, 2048: 6.0 / 5.0, 4096: 7.4 / 7.3, 32768: 32.5 / 36.4; of 4096, 2048: 9.6 / 6.8, 32768: 77 / 70;
+    // float32: of 1024, 2048: 3.4 / 4.0; of 2048, 4096: 6.9 / 7.8, 32768: 57 / 55; of 4096, 32768: 119 / 116.
+    const bool many = prm.rows >= kManyRows * pieces;
     if (pieces <= 1) go(One{}, One{});
     else if (pieces <= 2 && many) go(One{}, Two{});
     else if (pieces <= 4 && many) go(One{}, Four{});
-    else if (pieces <= 8 && many) go(One{}, Eight8{});
     else if (pieces <= 4) go(Four{}, One{});
     else if (pieces <= 8) go(Four{}, Two{});
     else if (pieces <= 16) go(Four{}, Four{});
