@@ -187,7 +187,7 @@ PyObject *fmoe_expert_linear_int8(PyObject *, PyObject *const *args, Py_ssize_t 
     const int64_t e = weight.size(0), rows_w = weight.size(1), d = weight.size(2), whole_d = (d + 15) / 16 * 16;
     // (rows that have to be copied, and sizes that the library refuses, go through Python)
     const int64_t by_expert = weight.stride(0), by_row = weight.stride(1);
-    if (d > 131072 || by_row > (1 << 22) || (by_row > 0 && rows_w * by_row >= ((int64_t)1 << 31))) Py_RETURN_NONE;
+    if (d > 131072 || by_row > (1 << 22) || (gated ? rows_w / 2 : rows_w) * x.element_size() > (1 << 22) || (by_row > 0 && rows_w * by_row >= ((int64_t)1 << 31))) Py_RETURN_NONE;
     if ((weight.stride(2) != 1 && d != 1) || by_row % 16 || by_row < whole_d || by_expert % 16 || by_expert < 0 || !on_16_bytes(weight) ||
         weight.storage_offset() + (e - 1) * by_expert + (rows_w - 1) * by_row + whole_d > (int64_t)weight.storage().nbytes())
         Py_RETURN_NONE;

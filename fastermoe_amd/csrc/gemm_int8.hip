@@ -37,7 +37,7 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     const int64_t whole = ceil_div(in_feat, 16) * 16, w_rows = out_feat * (gated ? 2 : 1);
     // (131072 products of numbers up to 128: below 2^31)
     if (in_feat > 131072 || n_expert > (1 << 24) || rows_cap > (int64_t)INT32_MAX - 65536 || out_feat > (1 << 28) || (x_scale != nullptr && ldx > (1 << 22)) ||
-        ldw > (1 << 22) || w_rows * ldw >= ((int64_t)1 << 31))
+        ldw > (1 << 22) || w_rows * ldw >= ((int64_t)1 << 31) || out_feat * dtype_bytes(dtype) > (1 << 22))   // (a tile's rows within 2 GiB of its first)
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     FMOE_REQUIRE((x_scale == nullptr || (ldx >= whole && ldx % 16 == 0)) && ldw >= whole && ldw % 16 == 0 && w_expert_stride % 16 == 0 && w_expert_stride >= 0,
                  "%s: rows of 8-bit integers begin on 16 bytes, at least %lld apart", who, (long long)whole);

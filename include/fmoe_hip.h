@@ -800,8 +800,8 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
  * a row can be read up to the next multiple of 16 bytes.  w_scale [E, rows of w]
  * float32, bias the same of y's type or NULL, y [rows_cap, out_feat] of dtype
  * (rows behind the experts' are left as they are).  The sums are exact; in_feat
- * is at most 131072, an expert's weights less than 2 GiB.  Tensors begin on 16
- * bytes.  With a workspace (on
+ * is at most 131072, an expert's weights less than 2 GiB, a row of y at most 4 MiB.
+ * Tensors begin on 16 bytes.  With a workspace (on
  * 16 bytes; none: NULL) of fmoe_linear_int8_workspace_bytes a last round of tiles
  * that fills a small part of the chip is shared along the contraction; the
  * results are the same bits. */

@@ -50,6 +50,7 @@ def _linear(x=P, ldx=32, xs=P, index=None, div=1, x_rows=4, w=P, ldw=32, wes=512
     (_linear, dict(dt=_lib.F64), EINVAL), (_linear, dict(act=3), EINVAL), (_linear, dict(e=0), EINVAL), (_linear, dict(d=0), EINVAL),
     (_linear, dict(out=0), EINVAL), (_linear, dict(d=131073, ldx=131088, ldw=131088), ELIMIT), (_linear, dict(rows=1 << 31), ELIMIT),
     (_linear, dict(ldw=1 << 23), ELIMIT), (_linear, dict(ldw=1 << 20, out=1 << 11), ELIMIT), (_linear, dict(ldx=1 << 23), ELIMIT),
+    (_linear, dict(d=16, ldw=16, wes=0, out=(1 << 21) + 8), ELIMIT), (_linear, dict(d=16, ldw=16, wes=0, out=(1 << 20) + 4, dt=_lib.F32), ELIMIT),
     (_linear, dict(ldx=16), EINVAL), (_linear, dict(ldx=40), EINVAL), (_linear, dict(ldw=16), EINVAL), (_linear, dict(ldw=40), EINVAL),
     (_linear, dict(wes=500), EINVAL), (_linear, dict(wes=-512), EINVAL), (_linear, dict(x=None), EINVAL), (_linear, dict(w=None), EINVAL),
     (_linear, dict(ws_=None), EINVAL), (_linear, dict(y=None), EINVAL), (_linear, dict(table=None), EINVAL), (_linear, dict(x=20), EINVAL),

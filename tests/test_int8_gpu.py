@@ -32,7 +32,7 @@ def _quantized(x):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows,d", [(1, 1), (3, 7), (5, 16), (2, 500), (9, 512), (4, 513), (7, 1024), (3, 1030), (2, 2048), (5, 2500), (3, 4096), (2, 8192),
-                                    (3, 16384), (2, 16390), (1, 40001), (4099, 64), (1000, 777)])
+                                    (3, 16384), (2, 16390), (1, 40001), (4099, 64), (1000, 777), (2050, 1000), (4100, 1500), (4100, 2000), (2100, 4000)])
 def test_rows(dtype, rows, d):
     gen = torch.Generator(device="cuda").manual_seed(rows * 7 + d)
     x = (torch.randn(rows, d, device="cuda", generator=gen) * torch.exp(2 * torch.randn(rows, 1, device="cuda", generator=gen))).to(dtype)
@@ -224,6 +224,22 @@ def test_largest_sums():
     y = functions.linear_int8(x, torch.tensor([3], device="cuda"), weight, scale)
     want = torch.tensor([1.0, -1.0] * 4, device="cuda").double() * 127 * 127 * d * scale[0, 0].double() ** 2
     assert ((y.double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_longest_rows_of_results(gated):
+    """4 MiB to a row; wider ones are refused."""
+    out = 1 << 21
+    for rows in (3, 200):
+        x, weight, scale, b = _tensors(rows, 16, out * (2 if gated else 1), 1, torch.bfloat16, True)
+        y = functions.linear_int8(x, torch.tensor([rows], device="cuda"), weight, scale, b, gated=gated)
+        some = weight[:, -70:] if not gated else torch.cat([weight[:, out - 70:out], weight[:, -70:]], dim=1)
+        of = scale[:, -70:] if not gated else torch.cat([scale[:, out - 70:out], scale[:, -70:]], dim=1)
+        bias = b[:, -70:] if not gated else torch.cat([b[:, out - 70:out], b[:, -70:]], dim=1)
+        _close(y[:, -70:], _reference(x, [rows], some, of, bias, "none", gated))
+        del y
+    with pytest.raises(fmoe_native._lib.FmoeHipError):
+        functions.linear_int8(x, torch.tensor([rows], device="cuda"), weight.new_zeros(1, (2 if gated else 1) * (out + 16), 16), torch.ones(1, (2 if gated else 1) * (out + 16), device="cuda"), gated=gated)
 
 
 def test_decode_rows():
