@@ -177,10 +177,9 @@ def load_layer_call():
         module.bind_block(*map(address, ("fmoe_last_error", "fmoe_layer_norm_forward", "fmoe_layer_norm_backward",
                                          "fmoe_layer_norm_backward_workspace_bytes", "fmoe_balance_loss_forward", "fmoe_balance_loss_backward",
                                          "fmoe_balance_loss_workspace_bytes", "fmoe_act_checkpoint_forward", "fmoe_act_checkpoint_backward")))
-        module.bind_expert(*map(address, ("fmoe_last_error", "fmoe_segment_table_bytes", "fmoe_linear_dev_supported",
-                                          "fmoe_gated_mlp_forward_workspace_bytes", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward_workspace_bytes",
-                                          "fmoe_gated_mlp_backward", "fmoe_quantize_rows", "fmoe_linear_int8_workspace_bytes", "fmoe_linear_int8",
-                                          "fmoe_linear_int8_rounds_rows")))
+        module.bind_expert(*map(address, ("fmoe_last_error", "fmoe_segment_table_bytes", "fmoe_gated_mlp_forward_workspace_bytes",
+                                          "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward_workspace_bytes", "fmoe_gated_mlp_backward",
+                                          "fmoe_quantize_rows", "fmoe_linear_int8_workspace_bytes", "fmoe_linear_int8", "fmoe_linear_int8_rounds_rows")))
         _layer_call = module
     return _layer_call
 

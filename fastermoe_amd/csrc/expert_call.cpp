@@ -19,7 +19,6 @@ using torch::autograd::variable_list;
 struct Entries {
     decltype(&fmoe_last_error) last_error;
     decltype(&fmoe_segment_table_bytes) table_bytes;
-    decltype(&fmoe_linear_dev_supported) dev_supported;
     decltype(&fmoe_gated_mlp_forward_workspace_bytes) gated_forward_bytes;
     decltype(&fmoe_gated_mlp_forward) gated_forward;
     decltype(&fmoe_gated_mlp_backward_workspace_bytes) gated_backward_bytes;
@@ -29,7 +28,7 @@ struct Entries {
     decltype(&fmoe_linear_int8) linear_int8;
     decltype(&fmoe_linear_int8_rounds_rows) int8_rounds_rows;
 } entry = {};
-constexpr int kEntries = 11;
+constexpr int kEntries = 10;
 
 void ok(int rc) { TORCH_CHECK(rc == FMOE_OK, "libfmoe_hip error ", rc, ": ", entry.last_error()); }
 bool on_16_bytes(const at::Tensor &t) { return !t.defined() || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
@@ -119,19 +118,18 @@ bool activation_taken(long a) { return a == FMOE_ACT_NONE || a == FMOE_ACT_RELU 
 
 PyObject *fmoe_expert_bind(PyObject *, PyObject *args) {
     unsigned long long a[kEntries];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10])) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9])) return nullptr;
     auto set = [&](auto &fn, int i) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(static_cast<uintptr_t>(a[i])); };
     set(entry.last_error, 0);
     set(entry.table_bytes, 1);
-    set(entry.dev_supported, 2);
-    set(entry.gated_forward_bytes, 3);
-    set(entry.gated_forward, 4);
-    set(entry.gated_backward_bytes, 5);
-    set(entry.gated_backward, 6);
-    set(entry.quantize_rows, 7);
-    set(entry.int8_bytes, 8);
-    set(entry.linear_int8, 9);
-    set(entry.int8_rounds_rows, 10);
+    set(entry.gated_forward_bytes, 2);
+    set(entry.gated_forward, 3);
+    set(entry.gated_backward_bytes, 4);
+    set(entry.gated_backward, 5);
+    set(entry.quantize_rows, 6);
+    set(entry.int8_bytes, 7);
+    set(entry.linear_int8, 8);
+    set(entry.int8_rounds_rows, 9);
     Py_RETURN_NONE;
 }
 

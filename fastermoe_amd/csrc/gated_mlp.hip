@@ -250,7 +250,7 @@ struct Copies {
     }
     void move(const void *src, void *dst, int64_t blocks, int64_t block_src, int64_t block_dst, int64_t cols_src, int64_t cols_dst, int rows_of_row,
               int blocks_of_expert) {
-        if (ws == nullptr || src == nullptr || dst == nullptr || rc != FMOE_OK) return;
+        if (ws == nullptr || src == nullptr || dst == nullptr || blocks * block_dst == 0 || rc != FMOE_OK) return;
         const Move m{(const float *)src, (float *)dst, blocks * block_dst, block_src, block_dst, (int)cols_src, (int)cols_dst, table, rows_of_row, blocks_of_expert};
         move_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(m.rows, kBlock / kWave), 1 << 20), kBlock, 0, stream>>>(m);
         rc = launched();

@@ -191,6 +191,25 @@ def test_the_same_row_twice_and_weights_of_one_expert_for_all(dtype):
     assert (shared_grad.float() - grad.float()).abs().max() <= 5 * torch.finfo(dtype).eps / 2 * 3 * grad.float().abs().max()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("d,h", [(64, 96), (51, 33)])
+@pytest.mark.parametrize("rows", [0, 1, 7, 300, 3000])
+def test_no_expert_has_rows(rows, dtype, d, h):
+    """All rows behind the experts': zeros, as their gradients and the weights' are, whatever the rows hold."""
+    x, w1, b1, w2, b2 = _tensors(rows, d, h, 3, dtype)
+    x.fill_(float("nan"))
+    counts = torch.zeros(3, dtype=torch.int64, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w1, b1, w2, b2)]
+    y = functions.gated_mlp(leaves[0], counts, *leaves[1:], torch.nn.SiLU())
+    assert y.shape == (rows, d) and not y.any()
+    for t, g in zip(leaves, torch.autograd.grad(y, leaves, torch.full_like(y, float("nan")))):
+        assert g.shape == t.shape and not g.any()
+    q, s = functions.quantize_rows(w1.detach())
+    with torch.no_grad():
+        y = functions.linear_int8(x, counts, q, s, b1, torch.nn.GELU(), gated=True)
+    assert y.shape == (rows, h) and not y.any()
+
+
 def test_tables_of_other_sizes_are_refused():
     x, w1, b1, w2, b2 = _tensors(10, 64, 48, 2, torch.bfloat16)
     counts = torch.tensor([4, 4], device="cuda")
