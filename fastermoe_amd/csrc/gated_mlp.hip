@@ -136,12 +136,14 @@ Scratch forward_scratch(const Sizes &s, bool keeps_pre) {
     return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)), 0,
                    std::max(fused ? gated_forward_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE, 0, 0),
-                            fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0))};
+                            std::max(fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0),
+                                     unaligned_parts_bytes(s.rows, s.n_expert, s.d, s.h, s.dtype)))};
 }
 Scratch backward_scratch(const Sizes &s) {
     return Scratch{round256(2 * s.rows * s.h * dtype_bytes(s.dtype)), 0,
                    std::max(gated_dgrad_workspace_bytes(gated_sizes(s)),
-                            fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE))};
+                            std::max(fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE),
+                                     unaligned_parts_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype)))};
 }
 
 // The products over the table
@@ -161,7 +163,7 @@ struct Products {
     int forward(const void *x, const void *w, const void *bias, void *y, int64_t in, int64_t out, bool once) const {
         LinearForwardArgs a{x, w, bias, y, nullptr, in, out, dtype, kEpiStore, FMOE_ACT_NONE};
         place(a);
-        a.dev_few_unaligned = true;
+        a.dev_any_order = true;
         a.dev_weights_once = once;   // (no backward that reads them again)
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;
@@ -170,6 +172,7 @@ struct Products {
     int dgrad(const void *gy, const void *w, void *gx, int64_t in, int64_t out) const {
         LinearDgradArgs a{gy, w, gx, nullptr, in, out, dtype, kEpiStore, FMOE_ACT_NONE};
         place(a);
+        a.dev_any_order = true;
         a.dev_workspace = ws;
         a.dev_workspace_bytes = ws_bytes;
         return grouped_linear_dgrad(a, nullptr, n_expert, 0, rows, stream);

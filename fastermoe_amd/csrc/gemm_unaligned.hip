@@ -10,7 +10,9 @@
 // 128 x 128 tiles (64 x 64 per wave), 64 x 128 where those would leave compute units without one; two slabs of
 // LDS, the next slab's chunks are requested before the products of the current one.  Bound by the latency of those
 // loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (8192 rows, 2047 x 4093:
-// 600 to 680 TFLOP/s).  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
+// 600 to 680 TFLOP/s).  Where few tiles have long contractions, a gated block's products share them between workgroups (launch_parts; see unaligned_parts() in
+// grouped_gemm.hip).  The epilogues of gated products are those of gemm_kernel.hpp: 1554 rows, 12 experts of 500 -> 2 x 1302 in float16, 25 us forward and 24 for the
+// gradient.  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
 #include "gemm_kernel.hpp"
 #include "unaligned_loads.hpp"
 
@@ -20,7 +22,11 @@ using namespace gemm;
 
 constexpr int kUaThreads = 256, kUaBN = 128, kUaBK = 64;
 
-// PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].  EPI: kEpiGated, kEpiDGated, or 0: what the parameters say.
+// the float32 sums of a part of the contraction instead of an epilogue: see launch_parts
+constexpr int kEpiParts = 100;
+__host__ __device__ __forceinline__ int parts_ld(int n_cols) { return (n_cols + 3) & ~3; }   // floats from row to row of those
+
+// PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].  EPI: kEpiGated, kEpiDGated, kEpiParts, or 0: what the parameters say.
 template <typename T, int BM, int PSHAPE, int QSHAPE, int RAGGED, int EPI>
 __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(const GemmParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
@@ -51,7 +57,7 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
     int tm_total = prm.tiles_m, total_tiles = prm.total_tiles;
     if (RAGGED == kRaggedRows) {
         tm_total = dev ? dtab[segtab::kTiles128] * (128 / BM) : prm.tab.tile[prm.tab.n];
-        total_tiles = tm_total * prm.tiles_n;
+        total_tiles = tm_total * prm.tiles_n * (EPI == kEpiParts ? prm.k_split : 1);
     }
     const int per_xcd = (total_tiles + 7) >> 3;
     const int L = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
@@ -61,6 +67,8 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         ei = L / (prm.tiles_m * prm.tiles_n);
         rem = L - ei * (prm.tiles_m * prm.tiles_n);
     }
+    const int part = EPI == kEpiParts ? rem % prm.k_split : 0;
+    if (EPI == kEpiParts) rem /= prm.k_split;
     const int grp = rem / (kGroupM * prm.tiles_n), in_grp = rem - grp * kGroupM * prm.tiles_n;
     const int gsz = min(kGroupM, tm_total - grp * kGroupM);
     const int nt = in_grp / gsz, mt = grp * kGroupM + in_grp - nt * gsz;
@@ -99,6 +107,12 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         P = (const T *)prm.P + (int64_t)expert * prm.p_expert_stride + (PSHAPE == kKC ? (int64_t)n0 * prm.ldp : (int64_t)n0);
         Q = (const T *)prm.Q + (int64_t)row0 * prm.ldq;
         c_off = (int64_t)row0 * prm.ldc + n0;
+        if (EPI == kEpiParts) {
+            const int k_lo = part * prm.split_slabs * BK;
+            P += PSHAPE == kKC ? (int64_t)k_lo : (int64_t)k_lo * prm.ldp;
+            Q += k_lo;
+            K = min(K - k_lo, prm.split_slabs * BK);   // (no part is empty)
+        }
     } else {
         m0 = mt * BM;
         q_valid = min(BM, prm.n_rows - m0);
@@ -240,7 +254,22 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    if constexpr (EPI != 0) {
+    if constexpr (EPI == kEpiParts) {
+        const int ld = parts_ld(prm.n_cols);
+        float *to = prm.split_ws + ((int64_t)part * prm.dev_rows_cap + row0) * ld + n0;
+#pragma unroll
+        for (int y = 0; y < TJ; ++y) {
+            const int row = 16 * row_block(y) + lb;
+            if (row >= q_valid) continue;
+#pragma unroll
+            for (int x = 0; x < TI; ++x) {
+                const int col = 64 * wn + 16 * x + 4 * hq;
+                if (col < p_valid) *(f32x4 *)(to + (int64_t)row * ld + col) = acc[x][y];
+            }
+        }
+        return;
+    }
+    if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
         // Gated products: sixteen rows at a time, 64 columns of C (dg and du, from g and u), or 32 of each half, through 2 KiB of LDS per wave and matrix
         constexpr int kWaveCols = kHalves ? 32 : 64, kPieces = kWaveCols / 8, kSteps = kPieces / 4, kRows = 64 / kPieces;
         unsigned char *area = smem + wave * 4096;
@@ -405,6 +434,35 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
 #endif
 }
 
+// The parts' sums in ascending order, with the bias, in the results' type: sixteen rows of a tile of the table's and 256 columns to a workgroup, four columns to a lane.
+template <typename T> __global__ __launch_bounds__(kUaThreads) void add_parts_kernel(const GemmParams prm) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int32_t *dtab = prm.dev_tab;
+    const int place = blockIdx.x >> 3;
+    if (place >= dtab[segtab::kTiles128]) return;
+    const i32x4 entry = *(const i32x4 *)(dtab + prm.dev_map_off + 4 * place);   // {expert, first row, rows}
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.y * 256 + lane * 4, ld = parts_ld(prm.n_cols);
+    if (col >= prm.n_cols) return;
+    const int n = min(4, prm.n_cols - col);
+    float b[4] = {};
+    if (prm.bias != nullptr)
+        for (int i = 0; i < n; ++i) b[i] = (float)((const T *)prm.bias)[(int64_t)entry[0] * prm.bias_expert_stride + col + i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int in_tile = (blockIdx.x & 7) * 16 + wave * 4 + j;
+        if (in_tile >= entry[2]) return;
+        const int64_t row = entry[1] + in_tile;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < prm.k_split; ++p) sum += *(const f32x4 *)(prm.split_ws + ((int64_t)p * prm.dev_rows_cap + row) * ld + col);
+        T *to = (T *)prm.C + row * prm.ldc + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) to[i] = (T)(sum[i] + b[i]);
+    }
+#endif
+}
+
 template <typename T, int BM, int PS, int QS, int RG, int EPI = 0>
 int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     prm.epilogue = epilogue;
@@ -417,7 +475,7 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     } else if (RG == kRaggedRows) {
         row_tiles = prm.tab.tile[prm.tab.n];
     }
-    const int64_t total = row_tiles * prm.tiles_n;
+    const int64_t total = row_tiles * prm.tiles_n * (EPI == kEpiParts ? prm.k_split : 1);
     if (total > (int64_t)INT32_MAX - 8) return fail(FMOE_ELIMIT, "grouped GEMM: %lld tiles exceed the grid limit", (long long)total);
     if (total == 0) return FMOE_OK;
     prm.total_tiles = (int)total;
@@ -427,9 +485,21 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     return FMOE_OK;
 }
 
+// Ragged rows over a device table, prm.k_split parts of prm.split_slabs slabs each: sums into prm.split_ws, and those added up.
+template <typename T, int PS> int launch_parts(GemmParams &prm, hipStream_t stream) {
+    if (int rc = launch_unaligned_tiles<T, 64, PS, kKC, kRaggedRows, kEpiParts>(prm, kEpiStore, stream)) return rc;
+    prm.dev_map_off = (int)segtab::map128_off(prm.dev_rows_cap, prm.tab.n);
+    const int64_t places = segtab::cap_tiles(prm.dev_rows_cap, prm.tab.n, 128);
+    add_parts_kernel<T><<<dim3((unsigned)(places * 8), (unsigned)ceil_div(prm.n_cols, 256)), kUaThreads, 0, stream>>>(prm);
+    FMOE_LAUNCH_CHECK();
+    return FMOE_OK;
+}
+
 template <typename T> int launch_unaligned_typed(GemmParams &prm, int product, int epilogue, hipStream_t stream) {
     const bool low = prm.block_m == 64;
     switch (product) {
+        case 5: return launch_parts<T, kKC>(prm, stream);
+        case 6: return launch_parts<T, kMC>(prm, stream);
         case 3:
             return low ? launch_unaligned_tiles<T, 64, kKC, kKC, kRaggedRows, kEpiGated>(prm, epilogue, stream)
                        : launch_unaligned_tiles<T, 128, kKC, kKC, kRaggedRows, kEpiGated>(prm, epilogue, stream);
@@ -448,7 +518,8 @@ template <typename T> int launch_unaligned_typed(GemmParams &prm, int product, i
 
 }  // namespace
 
-// product: 0 forward, 1 data gradient, 2 weight gradient (with the bias gradient), 3 gated forward, 4 data gradient up to a gated forward's product.  Ragged rows: prm.block_m (64 or 128)
+// product: 0 forward, 1 data gradient, 2 weight gradient (with the bias gradient), 3 gated forward, 4 data gradient up to a gated forward's product, 5 and 6 forward
+// and data gradient in parts of the contraction.  Ragged rows: prm.block_m (64 or 128)
 // is the tile height, for which prm.tab was filled in (a device table serves both).
 int launch_mfma_unaligned(gemm::GemmParams &prm, int dtype, int product, int epilogue, hipStream_t stream) {
     if (dtype == FMOE_BF16) return launch_unaligned_typed<__bf16>(prm, product, epilogue, stream);

@@ -456,6 +456,28 @@ bool few_unaligned(int64_t rows_cap, int64_t n_expert, int64_t in_feat, int64_t 
     return is_16bit(dtype) && rows_cap <= std::min<int64_t>(16 * n_expert, kFewUnalignedRows) && std::min(rows_cap, n_expert) * ceil_div(out_feat, 64) <= in_feat;
 }
 
+// Products off the 16-byte grid whose tiles leave compute units idle share their contractions between workgroups: so many parts that there are two workgroups to a unit,
+// of ten slabs or more, at most eight; a second launch adds up their float32 sums.  us of a gated block, forward and backward, bfloat16, in one part and so: 16 rows, 8 experts of
+// 1000 -> 2 x 2001: 163 / 137; 300 rows: 206 / 166; 700 rows, 12 of 500 -> 2 x 1302: 154 / 129, 1554: 165 / 151, 3000: 179 / 164; 256, 3 of 701 -> 2 x 5003: 328 / 172; 2000, 2 of
+// 333 -> 2 x 1111: 163 / 148.  (At least six slabs and four parts: 164 at 300 rows, 185 at 256; and eight: 171, 173.)
+int unaligned_parts(int64_t rows_cap, int64_t n_expert, int64_t n_cols, int64_t contraction, int dtype) {
+    if (!is_16bit(dtype)) return 1;
+    const int64_t tiles = (rows_cap / 64 + std::min(n_expert, rows_cap) / 2 + 1) * ceil_div(n_cols, 128);
+    const int64_t parts = std::min<int64_t>({8, ceil_div(contraction, 64) / 10, 2 * (int64_t)device_compute_units() / tiles});
+    return parts < 2 ? 1 : (int)parts;
+}
+bool unaligned_in_parts(GemmParams &prm, int dtype, int64_t n_expert, void *workspace, int64_t workspace_bytes) {
+    const int parts = unaligned_parts(prm.dev_rows_cap, n_expert, prm.n_cols, prm.k_extent, dtype);
+    const int64_t bytes = unaligned_parts_bytes(prm.dev_rows_cap, n_expert, prm.n_cols, prm.k_extent, dtype);
+    if (bytes == 0 || workspace == nullptr || workspace_bytes < bytes) return false;
+    const int slabs = (int)ceil_div(prm.k_extent, 64);
+    prm.split_slabs = (int)ceil_div(slabs, parts);
+    prm.k_split = (int)ceil_div(slabs, prm.split_slabs);   // no empty part
+    prm.split_ws = (float *)workspace;
+    prm.block_m = 64;
+    return true;
+}
+
 // The kernel of a row-ragged launch over a device table, and the workspace it can make use of.
 enum class DevKernel { kTiles, kSkinny, kRing };
 struct DevRoute {
@@ -594,6 +616,12 @@ int device_table_launch(const char *who, GemmParams &prm, const int32_t *dev_tab
     return FMOE_OK;
 }
 
+int64_t unaligned_parts_bytes(int64_t rows_cap, int64_t n_expert, int64_t n_cols, int64_t contraction, int dtype) {
+    if (n_cols % 8 == 0 && contraction % 8 == 0) return 0;   // (on the grid, but for tensors that begin off it)
+    const int parts = unaligned_parts(rows_cap, n_expert, n_cols, contraction, dtype);
+    return parts == 1 ? 0 : parts * rows_cap * ((n_cols + 3) / 4 * 4) * 4;
+}
+
 int64_t linear_dev_workspace_bytes(int64_t contraction, int dtype) {
     const int eb = dtype_bytes(dtype);
     if (eb == 0 || dtype == FMOE_F64 || contraction < 1) return 0;
@@ -629,13 +657,15 @@ int grouped_linear_forward(const LinearForwardArgs &a, const int64_t *counts, in
         prm.p_expert_stride = a.in_feat * a.out_feat;
         prm.bias_expert_stride = a.out_feat;
         prm.n_cols = (int)a.out_feat; prm.k_extent = (int)a.in_feat;
-        if (any_grid && a.dev_few_unaligned && few_unaligned(a.dev_rows_cap, n_expert, a.in_feat, a.out_feat, a.dtype)) {
+        if (any_grid && a.dev_any_order && few_unaligned(a.dev_rows_cap, n_expert, a.in_feat, a.out_feat, a.dtype)) {
             SkinnyParams sk{};
             sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
             sk.n_cols = prm.n_cols; sk.k_extent = prm.k_extent;
             ProfileScope prof(prm.profile_class, prm.profile_work, stream);
             return launch_few_unaligned(sk, a.dtype, false, a.dev_rows_cap, n_expert, stream);
         }
+        if (any_grid && a.dev_any_order && unaligned_in_parts(prm, a.dtype, n_expert, a.dev_workspace, a.dev_workspace_bytes))
+            return launch_mfma_unaligned(prm, a.dtype, 5, kEpiStore, stream);
         if (any_grid) return dispatch<kFwd>(prm, a.dtype, a.epilogue, false, stream);
         prm.dev_split_ws = route_workspace(route, a.in_feat, a.dtype, a.dev_workspace, a.dev_workspace_bytes);
         if (route.kernel == DevKernel::kSkinny) {
@@ -703,6 +733,8 @@ int grouped_linear_dgrad(const LinearDgradArgs &a, const int64_t *counts, int64_
         prm.ldp = a.in_feat; prm.ldq = a.out_feat; prm.ldc = a.in_feat;
         prm.p_expert_stride = a.in_feat * a.out_feat;
         prm.n_cols = (int)a.in_feat; prm.k_extent = (int)a.out_feat;
+        if (any_grid && a.dev_any_order && unaligned_in_parts(prm, a.dtype, n_expert, a.dev_workspace, a.dev_workspace_bytes))
+            return launch_mfma_unaligned(prm, a.dtype, 6, kEpiStore, stream);
         if (any_grid) return dispatch<kDgrad>(prm, a.dtype, a.epilogue, false, stream);
         prm.dev_split_ws = route_workspace(route, a.out_feat, a.dtype, a.dev_workspace, a.dev_workspace_bytes);
         if (route.kernel == DevKernel::kRing) return dispatch_ring<kDgrad>(prm, a.dtype, a.epilogue, stream);

@@ -90,8 +90,8 @@ struct LinearForwardArgs {
     int64_t dev_workspace_bytes = 0;
     // with dev_tab: 16-bit tensors and feature sizes off the 16-byte grid are taken too (gemm_unaligned.hip)
     bool dev_any_grid = false;
-    // with dev_any_grid: few rows may go to gemm_few_unaligned.hip (kEpiStore, no activation; its sums are in another order)
-    bool dev_few_unaligned = false;
+    // with dev_any_grid, kEpiStore, no activation: sums may be in another order, by gemm_few_unaligned.hip or in parts (which want unaligned_parts_bytes of workspace)
+    bool dev_any_order = false;
     // with dev_tab: nothing will read the weights again soon, as a backward would
     bool dev_weights_once = false;
 };
@@ -99,6 +99,9 @@ struct LinearForwardArgs {
 // Bytes of workspace with which a launch over a device table can split its last round of tiles along a
 // contraction of `contraction` elements; 0 when a contraction this short is never split.
 int64_t linear_dev_workspace_bytes(int64_t contraction, int dtype);
+
+// Workspace with which a product of n_cols columns off the 16-byte grid may share its contraction between workgroups; 0: it does not
+int64_t unaligned_parts_bytes(int64_t rows_cap, int64_t n_expert, int64_t n_cols, int64_t contraction, int dtype);
 
 // Whether the forward product can read its rows through an index: the MFMA path (aligned pointers,
 // feature sizes that are multiples of 16 bytes) and a token matrix of less than 2 GiB.
@@ -116,6 +119,7 @@ struct LinearDgradArgs {
     void *dev_workspace = nullptr;
     int64_t dev_workspace_bytes = 0;
     bool dev_any_grid = false;
+    bool dev_any_order = false;
 };
 
 struct LinearWgradArgs {

@@ -193,6 +193,15 @@ def test_few_rows_off_the_grid(dtype, rows, d, h, experts, kind):
         _check(rows, d, h, experts, dtype, act, act == "silu", kind, seed=rows)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("rows,d,h,experts,kind", [(300, 701, 2503, 3, "skewed"), (1100, 650, 1302, 5, "tail"), (40, 130, 2049, 2, "even"), (1, 33, 5007, 1, "even"),
+                                                   (700, 1283, 4, 40, "skewed"), (193, 1299, 643, 6, "one"), (260, 1281, 1283, 2, "tail")])
+def test_contractions_in_parts(dtype, rows, d, h, experts, kind):
+    """Off the grid, few tiles: contractions of ten slabs of 64 and more in two to eight parts, the last ones shorter."""
+    for act in ("silu", "relu"):
+        _check(rows, d, h, experts, dtype, act, act == "silu", kind, seed=rows)
+
+
 @pytest.mark.parametrize("off", range(1, 8))
 def test_few_rows_from_anywhere(off):
     """Tensors of sizes on the grid that begin off it."""
