@@ -448,17 +448,28 @@ template <typename T> __global__ __launch_bounds__(kUaThreads) void add_parts_ke
     float b[4] = {};
     if (prm.bias != nullptr)
         for (int i = 0; i < n; ++i) b[i] = (float)((const T *)prm.bias)[(int64_t)entry[0] * prm.bias_expert_stride + col + i];
+    const int in_tile = (blockIdx.x & 7) * 16 + wave * 4;
+    const int64_t row = entry[1] + in_tile;
+    // (four rows of two parts on their way at a time)
+    f32x4 sum[4] = {};
+    for (int p = 0; p < prm.k_split; p += 2) {
+        f32x4 v[2][4] = {};
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + q < prm.k_split && in_tile + j < entry[2])
+                    v[q][j] = *(const f32x4 *)(prm.split_ws + ((int64_t)(p + q) * prm.dev_rows_cap + row + j) * ld + col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = (sum[j] + v[0][j]) + v[1][j];
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int in_tile = (blockIdx.x & 7) * 16 + wave * 4 + j;
-        if (in_tile >= entry[2]) return;
-        const int64_t row = entry[1] + in_tile;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < prm.k_split; ++p) sum += *(const f32x4 *)(prm.split_ws + ((int64_t)p * prm.dev_rows_cap + row) * ld + col);
-        T *to = (T *)prm.C + row * prm.ldc + col;
+        if (in_tile + j >= entry[2]) return;
+        T *to = (T *)prm.C + (row + j) * prm.ldc + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < n) to[i] = (T)(sum[i] + b[i]);
+            if (i < n) to[i] = (T)(sum[j][i] + b[i]);
     }
 #endif
 }

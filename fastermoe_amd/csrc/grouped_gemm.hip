@@ -458,8 +458,8 @@ bool few_unaligned(int64_t rows_cap, int64_t n_expert, int64_t in_feat, int64_t 
 
 // Products off the 16-byte grid whose tiles leave compute units idle share their contractions between workgroups: so many parts that there are two workgroups to a unit,
 // of ten slabs or more, at most eight; a second launch adds up their float32 sums.  us of a gated block, forward and backward, bfloat16, in one part and so: 16 rows, 8 experts of
-// 1000 -> 2 x 2001: 163 / 137; 300 rows: 206 / 166; 700 rows, 12 of 500 -> 2 x 1302: 154 / 129, 1554: 165 / 151, 3000: 179 / 164; 256, 3 of 701 -> 2 x 5003: 328 / 172; 2000, 2 of
-// 333 -> 2 x 1111: 163 / 148.  (At least six slabs and four parts: 164 at 300 rows, 185 at 256; and eight: 171, 173.)
+// 1000 -> 2 x 2001: 163 / 135; 300 rows: 206 / 160; 700 rows, 12 of 500 -> 2 x 1302: 154 / 125, 1554: 165 / 146, 3000: 179 / 163; 256, 3 of 701 -> 2 x 5003: 328 / 160; 2000, 2 of
+// 333 -> 2 x 1111: 163 / 146.
 int unaligned_parts(int64_t rows_cap, int64_t n_expert, int64_t n_cols, int64_t contraction, int dtype) {
     if (!is_16bit(dtype)) return 1;
     const int64_t tiles = (rows_cap / 64 + std::min(n_expert, rows_cap) / 2 + 1) * ceil_div(n_cols, 128);
