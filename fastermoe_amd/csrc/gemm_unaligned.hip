@@ -7,10 +7,10 @@
 // and products are the same.  Where the contraction or the row of a [contraction][index] operand ends inside a chunk, the
 // chunk that ends with it is read and moved down; rows past a tile's end repeat its last row and are not stored.
 //
-// 128 x 128 tiles (64 x 64 per wave), 64 x 128 where those would leave compute units without one; two slabs of
-// LDS, the next slab's chunks are requested before the products of the current one.  Bound by the latency of those
-// loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (8192 rows, 2047 x 4093:
-// 600 to 680 TFLOP/s).  Where few tiles have long contractions, a gated block's products share them between workgroups (launch_parts; see unaligned_parts() in
+// 128 x 128 tiles (64 x 64 per wave), 64 x 128 where those would leave compute units without one; one slab of
+// LDS, the next slab's chunks are requested before the products of the current one: four workgroups share a unit, and one computes while others wait (with two slabs and two
+// workgroups: 8192 rows, 8 experts of 2047 -> 2 x 4093, both forward products 763 us, 690 so; 1554 rows, 12 of 500 -> 2 x 1302: 47 and 41).  Bound by the latency of those
+// loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (600 TFLOP/s there).  Where few tiles have long contractions, a gated block's products share them between workgroups (launch_parts; see unaligned_parts() in
 // grouped_gemm.hip).  The epilogues of gated products are those of gemm_kernel.hpp: 1554 rows, 12 experts of 500 -> 2 x 1302 in float16, 25 us forward and 24 for the
 // gradient.  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
 #include "gemm_kernel.hpp"
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
     constexpr bool kBiasGrad = RAGGED == kRaggedK;
     constexpr bool kHalves = epi_halves(EPI);
     constexpr int kCols = kHalves ? BN / 2 : BN;   // C columns of a tile
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[STAGE];
 
     if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
         const int64_t there = ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)prm.dev_tab)[segtab::kRows];
@@ -198,6 +198,12 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         return u32x4{l2[0], l2[1], h2[0], h2[1]};
     };
 
+    // a barrier for what lies in LDS (loads into registers go on)
+    auto lds_barrier = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
     // Block row y of a wave.  Ragged rows: every other one, so that both pairs of waves have some of an expert's few
     // rows and the epilogue ends at the last of them.
     auto row_block = [&](int y) { return RAGGED == kRaggedRows ? 2 * y + wm : TJ * wm + y; };
@@ -222,11 +228,10 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         fetch(QSHAPE, qr, NQ, Q, q_off, prm.ldq, q_valid, BM, prm.n_rows, 0);
     }
     for (int s = 0; s < n_slabs; ++s) {
-        unsigned char *buf = smem + (s & 1) * STAGE;
-        put(PSHAPE, pr, NP, buf);
-        put(QSHAPE, qr, NQ, buf + P_BYTES);
-        // (one barrier a slab: the other buffer, written next, was last read before it)
-        __syncthreads();
+        if (s > 0) lds_barrier();   // (the slab before has been read)
+        put(PSHAPE, pr, NP, smem);
+        put(QSHAPE, qr, NQ, smem + P_BYTES);
+        lds_barrier();
         if (s + 1 < n_slabs) {
             fetch(PSHAPE, pr, NP, P, p_off, prm.ldp, p_valid, BN, prm.n_cols, (s + 1) * BK);
             fetch(QSHAPE, qr, NQ, Q, q_off, prm.ldq, q_valid, BM, prm.n_rows, (s + 1) * BK);
@@ -235,9 +240,9 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         for (int ks = 0; ks < 2; ++ks) {
             u32x4 pf[TI], qf[TJ];
 #pragma unroll
-            for (int x = 0; x < TI; ++x) pf[x] = frag(PSHAPE, buf, wn * TI + x, ks);
+            for (int x = 0; x < TI; ++x) pf[x] = frag(PSHAPE, smem, wn * TI + x, ks);
 #pragma unroll
-            for (int y = 0; y < TJ; ++y) qf[y] = frag(QSHAPE, buf + P_BYTES, row_block(y), ks);
+            for (int y = 0; y < TJ; ++y) qf[y] = frag(QSHAPE, smem + P_BYTES, row_block(y), ks);
 #pragma unroll
             for (int x = 0; x < TI; ++x)
 #pragma unroll
