@@ -78,28 +78,40 @@ struct Move {
     int rows_of_row;                           // not 0: only rows r with r / rows_of_row below the table's rows
     int blocks_of_expert;                      // not 0: only blocks of experts with rows
 };
-constexpr int kMoveLoads = 8;
-// A wave to a row, kMoveLoads of a lane's loads on their way at a time (one: 1001 -> 2 x 2003, 8 experts, 1 row, forward 70 us, 52 now).  Bound by memory.
-__global__ __launch_bounds__(kBlock) void move_rows_kernel(const Move m) {
+constexpr int kMoveLoads = 8, kMoves = 6;
+// all of a direction's, one after the other
+struct Moves {
+    Move m[kMoves];
+    int n;
+};
+// A wave to a row, kMoveLoads of a lane's loads on their way at a time (one: 1001 -> 2 x 2003, 8 experts, 1 row, forward 70 us, 52 so, 40 with
+// all moves of a direction in one launch).  Bound by memory.
+__global__ __launch_bounds__(kBlock) void move_rows_kernel(const Moves all) {
     const int lane = threadIdx.x % kWave;
-    for (int64_t row = (int64_t)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave; row < m.rows; row += (int64_t)gridDim.x * (kBlock / kWave)) {
-        if (m.rows_of_row && row / m.rows_of_row >= m.table[segtab::kRows]) return;   // (and so do the rows after)
-        const int64_t block = row / m.block_dst, in_block = row - block * m.block_dst;
-        if (m.blocks_of_expert) {
-            const int64_t e = block / m.blocks_of_expert;
-            if (m.table[segtab::kHeader + e] == m.table[segtab::kHeader + e + 1]) continue;
-        }
-        const float *src = m.src + (block * m.block_src + in_block) * m.cols_src;
-        const int n = in_block < m.block_src ? m.cols_src : 0;
-        float *dst = m.dst + row * m.cols_dst;
-        for (int c = lane; c < m.cols_dst; c += kMoveLoads * kWave) {
-            float v[kMoveLoads];
+    int64_t row = (int64_t)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
+    const int64_t step = (int64_t)gridDim.x * (kBlock / kWave);
+    for (int i = 0; i < all.n; ++i) {
+        const Move &m = all.m[i];
+        for (; row < m.rows; row += step) {
+            if (m.rows_of_row && row / m.rows_of_row >= m.table[segtab::kRows]) continue;
+            const int64_t block = row / m.block_dst, in_block = row - block * m.block_dst;
+            if (m.blocks_of_expert) {
+                const int64_t e = block / m.blocks_of_expert;
+                if (m.table[segtab::kHeader + e] == m.table[segtab::kHeader + e + 1]) continue;
+            }
+            const float *src = m.src + (block * m.block_src + in_block) * m.cols_src;
+            const int n = in_block < m.block_src ? m.cols_src : 0;
+            float *dst = m.dst + row * m.cols_dst;
+            for (int c = lane; c < m.cols_dst; c += kMoveLoads * kWave) {
+                float v[kMoveLoads];
 #pragma unroll
-            for (int j = 0; j < kMoveLoads; ++j) v[j] = c + j * kWave < n ? __builtin_nontemporal_load(src + c + j * kWave) : 0.f;
+                for (int j = 0; j < kMoveLoads; ++j) v[j] = c + j * kWave < n ? __builtin_nontemporal_load(src + c + j * kWave) : 0.f;
 #pragma unroll
-            for (int j = 0; j < kMoveLoads; ++j)
-                if (c + j * kWave < m.cols_dst) dst[c + j * kWave] = v[j];
+                for (int j = 0; j < kMoveLoads; ++j)
+                    if (c + j * kWave < m.cols_dst) dst[c + j * kWave] = v[j];
+            }
         }
+        row -= m.rows;   // (the next one's rows follow)
     }
 }
 
@@ -229,8 +241,8 @@ int backward(const Sizes &s, const Backward &b, const int32_t *table, char *ws, 
 }
 
 // float32 in sizes that are no multiple of four: the same with sizes that are, on copies.  (With products that check every
-// element, over counts read on the host, us forward and with the backward, and like this: 1 row, 8 experts of 1001 -> 2 x 2003: 180, 493 / 52, 286; 64 rows, 33 of 443 -> 2 x
-// 2368: 300, 801 / 199, 818; 1554 rows, 12 of 501 -> 2 x 1303: 257, 677 / 137, 425; 8192 rows, 8 of 1023 -> 2 x 2047: 2088, 5494 / 713, 2294.)
+// element, over counts read on the host, us forward and with the backward, and like this: 1 row, 8 experts of 1001 -> 2 x 2003: 180, 493 / 40, 242; 64 rows, 33 of 443 -> 2 x
+// 2368: 300, 801 / 186, 757; 1554 rows, 12 of 501 -> 2 x 1303: 257, 677 / 128, 384; 8192 rows, 8 of 1023 -> 2 x 2047: 2088, 5494 / 694, 2240.)
 bool padded(const Sizes &s) { return s.dtype == FMOE_F32 && (s.d % 4 != 0 || s.h % 4 != 0); }
 Sizes whole(const Sizes &s) {
     Sizes w = s;
@@ -238,89 +250,107 @@ Sizes whole(const Sizes &s) {
     w.h = ceil_div(s.h, 4) * 4;
     return w;
 }
+// What lies right as it is, in rows of a size that is a multiple of four, is used where it lies.
 struct Copies {
     Sizes s, w;
     const int32_t *table;
     char *ws;          // null: only the sizes are added up
     hipStream_t stream;
     int64_t used = 0;
-    int rc = FMOE_OK;
+    Moves moves{};
 
     float *room(int64_t floats) {
         float *at = ws ? (float *)(ws + used) : nullptr;
         used += round256(floats * 4);
         return at;
     }
-    void move(const void *src, void *dst, int64_t blocks, int64_t block_src, int64_t block_dst, int64_t cols_src, int64_t cols_dst, int rows_of_row,
-              int blocks_of_expert) {
-        if (ws == nullptr || src == nullptr || dst == nullptr || blocks * block_dst == 0 || rc != FMOE_OK) return;
-        const Move m{(const float *)src, (float *)dst, blocks * block_dst, block_src, block_dst, (int)cols_src, (int)cols_dst, table, rows_of_row, blocks_of_expert};
-        move_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(m.rows, kBlock / kWave), 1 << 20), kBlock, 0, stream>>>(m);
-        rc = launched();
+    // one matrix, or per block of rows: `blocks` of `rows` rows of `cols` elements, those of the padded sizes beside them
+    struct Shape {
+        int64_t blocks, rows, rows_padded, cols, cols_padded;
+        int rows_of_row, blocks_of_expert;
+        bool as_it_is() const { return rows == rows_padded && cols == cols_padded; }
+        int64_t floats() const { return blocks * rows_padded * cols_padded; }
+    };
+    Shape rows_of(int halves, bool hidden) const { return {1, s.rows * halves, s.rows * halves, hidden ? s.h : s.d, hidden ? w.h : w.d, halves, 0}; }
+    Shape w1() const { return {2 * s.n_expert, s.h, w.h, s.d, w.d, 0, 2}; }
+    Shape b1() const { return {1, 2 * s.n_expert, 2 * s.n_expert, s.h, w.h, 0, 0}; }
+    Shape w2() const { return {s.n_expert, s.d, w.d, s.h, w.h, 0, 1}; }
+    Shape b2() const { return {1, s.n_expert, s.n_expert, s.d, w.d, 0, 0}; }
+
+    void add(const Move &m) {
+        if (m.rows > 0) moves.m[moves.n++] = m;
     }
-    static int launched() {
-        FMOE_LAUNCH_CHECK();
+    const void *in(const void *t, const Shape &at) {
+        if (at.as_it_is()) return t;
+        float *copy = room(at.floats());
+        if (ws == nullptr || t == nullptr) return nullptr;
+        add(Move{(const float *)t, copy, at.blocks * at.rows_padded, at.rows, at.rows_padded, (int)at.cols, (int)at.cols_padded, table, at.rows_of_row, at.blocks_of_expert});
+        return copy;
+    }
+    // where a result goes first: `t` itself, or room for its padded form (wanted: or nowhere)
+    void *result(void *t, const Shape &at, bool wanted = true) {
+        if (at.as_it_is()) return t;
+        float *copy = room(at.floats());
+        return wanted ? copy : nullptr;
+    }
+    // `live`: only rows that there are
+    void out(const void *from, void *t, const Shape &at, bool live) {
+        if (t == nullptr || from == nullptr || from == t) return;
+        add(Move{(const float *)from, (float *)t, at.blocks * at.rows, at.rows_padded, at.rows, (int)at.cols_padded, (int)at.cols, table, live ? at.rows_of_row : 0, 0});
+    }
+    int flush() {
+        int64_t rows = 0;
+        for (int i = 0; i < moves.n; ++i) rows += moves.m[i].rows;
+        if (rows > 0) {
+            move_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(rows, kBlock / kWave), 1 << 20), kBlock, 0, stream>>>(moves);
+            FMOE_LAUNCH_CHECK();
+        }
+        moves.n = 0;
         return FMOE_OK;
     }
-    // [rows, halves * h or d] of a call's rows; back: all of them, or those that there are
-    float *rows_in(const void *t, int halves, bool hidden) {
-        float *at = room(s.rows * halves * (hidden ? w.h : w.d));
-        move(t, at, 1, s.rows * halves, s.rows * halves, hidden ? s.h : s.d, hidden ? w.h : w.d, halves, 0);
-        return at;
-    }
-    void rows_out(const float *at, void *t, int halves, bool hidden, bool all) {
-        move(at, t, 1, s.rows * halves, s.rows * halves, hidden ? w.h : w.d, hidden ? s.h : s.d, all ? 0 : halves, 0);
-    }
-    // W1 [E, 2 h, d] and b1 [E, 2 h], W2 [E, d, h] and b2 [E, d]
-    float *w1_in(const void *t) { float *at = room(s.n_expert * 2 * w.h * w.d); move(t, at, 2 * s.n_expert, s.h, w.h, s.d, w.d, 0, 2); return at; }
-    float *b1_in(const void *t) { float *at = room(s.n_expert * 2 * w.h); move(t, at, 1, 2 * s.n_expert, 2 * s.n_expert, s.h, w.h, 0, 0); return t ? at : nullptr; }
-    float *w2_in(const void *t) { float *at = room(s.n_expert * w.d * w.h); move(t, at, s.n_expert, s.d, w.d, s.h, w.h, 0, 1); return at; }
-    float *b2_in(const void *t) { float *at = room(s.n_expert * w.d); move(t, at, 1, s.n_expert, s.n_expert, s.d, w.d, 0, 0); return t ? at : nullptr; }
-    void w1_out(const float *at, void *t) { move(at, t, 2 * s.n_expert, w.h, s.h, w.d, s.d, 0, 0); }
-    void b1_out(const float *at, void *t) { move(at, t, 1, 2 * s.n_expert, 2 * s.n_expert, w.h, s.h, 0, 0); }
-    void w2_out(const float *at, void *t) { move(at, t, s.n_expert, w.d, s.d, w.h, s.h, 0, 0); }
-    void b2_out(const float *at, void *t) { move(at, t, 1, s.n_expert, s.n_expert, w.d, s.d, 0, 0); }
 };
 // (ws null: the workspace's bytes in *bytes)
 int padded_forward(const Sizes &s, const Forward &f, const int32_t *table, char *ws, int64_t *bytes, hipStream_t stream) {
     const Sizes w = whole(s);
     Copies c{s, w, table, ws, stream};
     Forward g{};
-    g.x = c.rows_in(f.x, 1, false);
-    g.w1 = c.w1_in(f.w1); g.b1 = c.b1_in(f.b1); g.w2 = c.w2_in(f.w2); g.b2 = c.b2_in(f.b2);
-    float *mid = c.room(s.rows * w.h), *y = c.room(s.rows * w.d), *pre = f.pre ? c.room(s.rows * 2 * w.h) : nullptr;
-    g.mid = mid; g.y = y; g.pre = pre;
+    g.x = c.in(f.x, c.rows_of(1, false));
+    g.w1 = c.in(f.w1, c.w1()); g.b1 = c.in(f.b1, c.b1()); g.w2 = c.in(f.w2, c.w2()); g.b2 = c.in(f.b2, c.b2());
+    g.mid = c.result(f.mid, c.rows_of(1, true)); g.y = c.result(f.y, c.rows_of(1, false));
+    g.pre = f.pre ? c.result(f.pre, c.rows_of(2, true)) : nullptr;
     if (ws == nullptr) {
         *bytes = c.used + forward_scratch(w, f.pre != nullptr).total();
         return FMOE_OK;
     }
-    if (c.rc == FMOE_OK) c.rc = forward(w, g, table, ws + c.used, stream);
-    c.rows_out(y, f.y, 1, false, true);
+    if (int rc = c.flush()) return rc;
+    if (int rc = forward(w, g, table, ws + c.used, stream)) return rc;
+    c.out(g.y, f.y, c.rows_of(1, false), false);
     if (f.pre) {
-        c.rows_out(pre, f.pre, 2, true, false);
-        c.rows_out(mid, f.mid, 1, true, false);
+        c.out(g.pre, f.pre, c.rows_of(2, true), true);
+        c.out(g.mid, f.mid, c.rows_of(1, true), true);
     }
-    return c.rc;
+    return c.flush();
 }
 int padded_backward(const Sizes &s, const Backward &b, const int32_t *table, char *ws, int64_t *bytes, hipStream_t stream) {
     const Sizes w = whole(s);
     Copies c{s, w, table, ws, stream};
     Backward g{};
-    g.grad_y = c.rows_in(b.grad_y, 1, false); g.x = c.rows_in(b.x, 1, false);
-    g.w1 = c.w1_in(b.w1); g.w2 = c.w2_in(b.w2);
-    g.pre = c.rows_in(b.pre, 2, true); g.mid = c.rows_in(b.mid, 1, true);
-    float *gx = c.room(s.rows * w.d), *gw1 = c.room(s.n_expert * 2 * w.h * w.d), *gb1 = c.room(s.n_expert * 2 * w.h);
-    float *gw2 = c.room(s.n_expert * w.d * w.h), *gb2 = c.room(s.n_expert * w.d);
+    g.grad_y = c.in(b.grad_y, c.rows_of(1, false)); g.x = c.in(b.x, c.rows_of(1, false));
+    g.w1 = c.in(b.w1, c.w1()); g.w2 = c.in(b.w2, c.w2());
+    g.pre = c.in(b.pre, c.rows_of(2, true)); g.mid = c.in(b.mid, c.rows_of(1, true));
+    g.grad_x = c.result(b.grad_x, c.rows_of(1, false), b.grad_x != nullptr);
+    g.grad_w1 = c.result(b.grad_w1, c.w1(), b.grad_w1 != nullptr); g.grad_b1 = c.result(b.grad_b1, c.b1(), b.grad_b1 != nullptr);
+    g.grad_w2 = c.result(b.grad_w2, c.w2(), b.grad_w2 != nullptr); g.grad_b2 = c.result(b.grad_b2, c.b2(), b.grad_b2 != nullptr);
     if (ws == nullptr) {
         *bytes = c.used + (s.rows == 0 ? 0 : backward_scratch(w).total());
         return FMOE_OK;
     }
-    g.grad_x = b.grad_x ? gx : nullptr; g.grad_w1 = b.grad_w1 ? gw1 : nullptr; g.grad_b1 = b.grad_b1 ? gb1 : nullptr;
-    g.grad_w2 = b.grad_w2 ? gw2 : nullptr; g.grad_b2 = b.grad_b2 ? gb2 : nullptr;
-    if (c.rc == FMOE_OK) c.rc = backward(w, g, table, ws + c.used, stream);
-    if (s.rows > 0) c.rows_out(gx, b.grad_x, 1, false, true);
-    c.w1_out(gw1, b.grad_w1); c.b1_out(gb1, b.grad_b1); c.w2_out(gw2, b.grad_w2); c.b2_out(gb2, b.grad_b2);
-    return c.rc;
+    if (int rc = c.flush()) return rc;
+    if (int rc = backward(w, g, table, ws + c.used, stream)) return rc;
+    if (s.rows > 0) c.out(g.grad_x, b.grad_x, c.rows_of(1, false), false);
+    c.out(g.grad_w1, b.grad_w1, c.w1(), false); c.out(g.grad_b1, b.grad_b1, c.b1(), false);
+    c.out(g.grad_w2, b.grad_w2, c.w2(), false); c.out(g.grad_b2, b.grad_b2, c.b2(), false);
+    return c.flush();
 }
 int64_t forward_bytes(const Sizes &s, bool keep) {
     if (!padded(s)) return forward_scratch(s, keep).total();

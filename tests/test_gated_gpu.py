@@ -202,6 +202,12 @@ def test_contractions_in_parts(dtype, rows, d, h, experts, kind):
         _check(rows, d, h, experts, dtype, act, act == "silu", kind, seed=rows)
 
 
+@pytest.mark.parametrize("rows,d,h", [(9, 50, 64), (9, 64, 50), (300, 67, 96), (300, 96, 67), (300, 1, 8), (300, 8, 1)])
+def test_float32_with_one_size_off_the_grid(rows, d, h):
+    for act in ("silu", "gelu"):
+        _check(rows, d, h, 3, torch.float32, act, act == "gelu", "tail" if act == "gelu" else "skewed", seed=rows)
+
+
 @pytest.mark.parametrize("off", range(1, 8))
 def test_few_rows_from_anywhere(off):
     """Tensors of sizes on the grid that begin off it."""
