@@ -731,6 +731,19 @@ def nothing_watches(*tensors):
             and (not _modes_watch() or saving_is_watched()))
 
 
+def _differentiated(tensors):
+    """Whether a derivative of a call on these tensors is wanted, or a transform (``torch.func``) has to see it: a gradient, or a tangent of
+    forward mode, which ``torch.no_grad`` does not switch off and which needs no tensor that requires gradients."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        return True
+    forward = torch.autograd.forward_ad
+    if forward._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None:
+        return False
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    return (any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors)
+            or (forward._current_level >= 0 and any(forward.unpack_dual(t).tangent is not None for t in tensors)))
+
+
 def _gate_activation_code(activation):
     """The code of an activation that gated experts and products in 8 bits take; an ``ACT_*`` code stays what it is."""
     if type(activation) is int:
@@ -815,7 +828,7 @@ def quantize_rows(inp):
     r"""``(q, scale)``: ``inp [.., features]`` (float32, bfloat16, float16) rounded to 8-bit integers along its last dimension, ``q`` int8 of ``inp``'s shape and
     ``scale`` float32 of its leading one, ``inp ~ q * scale``.  ``scale`` is a 127th of the largest magnitude (at least ``2^-126``), ``q`` the integer nearest to
     ``inp / scale``, ties to even; a row with an infinity or a NaN has the scale NaN.  What :func:`linear_int8` does with its rows, and what makes its weights:
-    ``q``'s rows lie whole 16 bytes apart, as the products read them.  Not differentiable."""
+    ``q``'s rows lie whole 16 bytes apart, as the products read them.  Not differentiable: neither result has a gradient or a tangent."""
     with torch.no_grad():
         q, scale = fmoe_native.quantize_rows(_as_rows(inp.detach()))
     if inp.dim() == 2:
@@ -834,8 +847,9 @@ def linear_int8(inp, expert_count, weight, weight_scale, bias=None, activation=N
     exact (``in_feat`` up to 131072), the result is of ``inp``'s type.  ``gated``: ``weight`` has the rows of a gate and then as many of a linear half, the
     result is ``act(first) * second``.  ``expert_count``, ``table``: as for :func:`gated_mlp`.  ``row_index`` (int64, one entry per sorted row): row ``r``
     is ``inp[row_index[r] // index_div]``.  Rows behind the counted ones come out as zeros."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (inp, bias, weight_scale)):
-        raise NotImplementedError("linear_int8 has no gradients: call it under torch.no_grad(), or with tensors that require none")
+    if _differentiated((inp, weight, weight_scale, bias)):
+        raise NotImplementedError("linear_int8 has no derivatives: call it under torch.no_grad(), or with tensors that require no gradients, "
+                                  "without tangents and outside of transforms")
     code = _gate_activation_code(activation)
     rows = inp.shape[0] if row_index is None else row_index.numel()
     table = _segments(expert_count, table, weight.shape[0], rows, inp.device)

@@ -108,6 +108,32 @@ def test_gradients_of_8_bit_products_are_refused():
         functions.linear_int8(x, torch.tensor([1, 2]), torch.zeros(2, 16, 8, dtype=torch.int8), torch.ones(2, 16))
 
 
+@pytest.mark.parametrize("which", ["inp", "bias", "weight_scale"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_of_8_bit_products_are_refused(which, grad):
+    """Forward mode: a dual tensor requires no gradient, and torch.no_grad leaves its tangent."""
+    tensors = {"inp": torch.zeros(3, 8), "bias": torch.zeros(2, 16), "weight_scale": torch.ones(2, 16)}
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        tensors[which] = torch.autograd.forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        with pytest.raises(NotImplementedError, match="tangents"):
+            functions.linear_int8(tensors["inp"], torch.tensor([1, 2]), torch.zeros(2, 16, 8, dtype=torch.int8), tensors["weight_scale"], tensors["bias"])
+
+
+def test_transforms_of_8_bit_products_are_refused():
+    scale, weight = torch.ones(2, 16), torch.zeros(2, 16, 8, dtype=torch.int8)
+    call = lambda x: functions.linear_int8(x, torch.tensor([1, 2]), weight, scale)
+    for transformed in (lambda: torch.func.jvp(call, (torch.zeros(3, 8),), (torch.ones(3, 8),)), lambda: torch.func.vmap(call)(torch.zeros(4, 3, 8)),
+                        lambda: torch.func.grad(lambda x: call(x).sum())(torch.zeros(3, 8))):
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="transforms"):
+            transformed()
+
+
+def test_tangents_that_are_nobody_elses_business():
+    """A level of forward mode alone refuses nothing: what is wrong with the call is said (its tensors are the host's)."""
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA"):
+        functions.linear_int8(torch.zeros(3, 8), torch.tensor([1, 2]), torch.zeros(2, 16, 8, dtype=torch.int8), torch.ones(2, 16))
+
+
 def test_layers_have_the_parameters_of_their_kind():
     layer = FMoEGatedMLP(num_expert=3, d_model=8, d_hidden=20, top_k=2)
     assert layer.experts.htoh4.weight.shape == (3, 40, 8) and layer.experts.h4toh.weight.shape == (3, 8, 20)
