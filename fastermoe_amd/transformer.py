@@ -140,6 +140,13 @@ def _gate_code_or_none(activation):
         return None
 
 
+def _is_its_product(linear):
+    """Whether calling ``linear`` is :class:`FMoELinear`'s product of its parameters (or parametrised tensors) and nothing else: no module in its
+    place, no ``forward`` or hook of its own."""
+    return (isinstance(linear, FMoELinear) and type(linear).forward is FMoELinear.forward and "forward" not in linear.__dict__
+            and not (linear._forward_hooks or linear._forward_pre_hooks or linear._backward_hooks or linear._backward_pre_hooks))
+
+
 class _GatedExpert(_Expert):
     r"""All experts of a worker as gated blocks, ``h4toh(act(g) * u)`` with ``[g u] = htoh4(x)``: ``htoh4`` has ``2 * d_hidden`` outputs, the
     gate's first.  With SiLU, exact GELU, ReLU or no activation one call each way (:func:`fastermoe_amd.functions.gated_mlp`), else the
@@ -202,6 +209,9 @@ class _Int8Expert(nn.Module):
         self.activation, self.gated = experts.activation, isinstance(experts, _GatedExpert)
         if _gate_code_or_none(self.activation) is None:
             raise NotImplementedError(f"experts in 8 bits take SiLU, GELU, ReLU or no activation, got {self.activation!r}")
+        for name in ("htoh4", "h4toh"):
+            if not _is_its_product(getattr(experts, name)):
+                raise TypeError(f"{name} is not just its product, and only that is held in 8 bits: it was replaced, or has a forward or hooks of its own")
         for name in ("htoh4", "h4toh"):
             linear = getattr(experts, name)
             q, scale = quantize_rows(linear.weight)
@@ -304,7 +314,8 @@ class FMoETransformerMLP(FMoE):
     def quantize_experts(self):
         r"""Holds the experts in 8-bit integers from here on, for inference: weights with a scale to each output channel, rows rounded with a scale of their own
         as they come, exact sums.  Half of the memory of 16-bit weights, and half of the bytes that a decoding step reads.  The experts have no
-        parameters afterwards; calls that would need their gradients raise.  Returns the layer."""
+        parameters afterwards; calls that would need their gradients raise.  Experts of another class, or with linears that were replaced or have hooks,
+        are refused.  Returns the layer."""
         self.experts = _Int8Expert(self.experts)
         return self
 

@@ -141,3 +141,43 @@ def test_layers_have_the_parameters_of_their_kind():
     assert plain.experts.htoh4.weight.shape == (3, 20, 8)
     block = FMoEPositionwiseFF(num_expert=3, d_model=8, d_hidden=20, top_k=2, gated=True)
     assert any(p.shape == (3, 40, 8) for p in block.parameters())
+
+
+class _Adapter(torch.nn.Module):
+    """A linear with something added, and a ``weight`` of its own."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.linear = linear
+
+    weight = property(lambda self: self.linear.weight)
+    bias = property(lambda self: self.linear.bias)
+
+    def forward(self, inp, fwd_expert_count):
+        return self.linear(inp, fwd_expert_count) + 1
+
+
+@pytest.mark.parametrize("kind", [FMoETransformerMLP, FMoEGatedMLP])
+@pytest.mark.parametrize("name", ["htoh4", "h4toh"])
+def test_replaced_linears_are_not_held_in_8_bits(kind, name):
+    """What a module in a linear's place, or a hook, adds to its weight's product would be lost.  (The refusal comes before anything needs a GPU.)"""
+    def adapter(experts):
+        setattr(experts, name, _Adapter(getattr(experts, name)))
+
+    def own_forward(experts):
+        linear = getattr(experts, name)
+        linear.forward = lambda inp, count: type(linear).forward(linear, inp, count) + 1
+
+    def hook(experts):
+        getattr(experts, name).register_forward_hook(lambda module, args, out: out + 1)
+
+    def pre_hook(experts):
+        getattr(experts, name).register_forward_pre_hook(lambda module, args: None)
+
+    for change in (adapter, own_forward, hook, pre_hook):
+        layer = kind(num_expert=3, d_model=8, d_hidden=20)
+        change(layer.experts)
+        before = layer.experts
+        with pytest.raises(TypeError, match=name):
+            layer.quantize_experts()
+        assert layer.experts is before
