@@ -149,8 +149,8 @@ def _is_its_product(linear):
 
 class _GatedExpert(_Expert):
     r"""All experts of a worker as gated blocks, ``h4toh(act(g) * u)`` with ``[g u] = htoh4(x)``: ``htoh4`` has ``2 * d_hidden`` outputs, the
-    gate's first.  With SiLU, exact GELU, ReLU or no activation one call each way (:func:`fastermoe_amd.functions.gated_mlp`), else the
-    modules one by one."""
+    gate's first.  With SiLU, exact GELU, ReLU or no activation one call each way (:func:`fastermoe_amd.functions.gated_mlp`), else, or
+    where a linear was replaced or has hooks, the modules one by one."""
 
     def __init__(self, num_expert, d_model, d_hidden, activation, rank=0, bias=True):
         super().__init__(num_expert, d_model, d_hidden, activation, rank=rank, bias=bias)
@@ -164,6 +164,7 @@ class _GatedExpert(_Expert):
     def _one_call(self, inp):
         """The activation's code where the block is one call, else ``None``."""
         if not (inp.is_cuda and fmoe_native.gated_mlp_supported(inp.dtype) and os.environ.get("FMOE_EXPERT_EPILOGUE", "1") != "0"
+                and _is_its_product(self.htoh4) and _is_its_product(self.h4toh)
                 and all(p is None or p.dtype == inp.dtype for linear in (self.htoh4, self.h4toh) for p in (linear.weight, linear.bias))):
             return None
         return _gate_code_or_none(self.activation)

@@ -219,3 +219,45 @@ def test_tables_of_other_sizes_are_refused():
                  lambda: functions.linear_int8(x, None, q, s, b1, table=wrong)):
         with pytest.raises((ValueError, TypeError)):
             call()
+
+
+class _Adapter(torch.nn.Module):
+    """A linear with something added, and a ``weight`` of its own."""
+
+    def __init__(self, linear, features):
+        super().__init__()
+        self.linear, self.more = linear, torch.nn.Parameter(torch.linspace(-1, 1, features, device="cuda"))
+
+    weight = property(lambda self: self.linear.weight)
+    bias = property(lambda self: self.linear.bias)
+
+    def forward(self, inp, fwd_expert_count):
+        return self.linear(inp, fwd_expert_count) + self.more
+
+
+@pytest.mark.parametrize("name", ["htoh4", "h4toh"])
+@pytest.mark.parametrize("fuse", [False, True])
+def test_gated_experts_call_what_stands_in_a_linears_place(name, fuse):
+    """A module in a linear's place, or a hook on it, takes part: as with a bias of as much more."""
+    torch.manual_seed(5)
+    layer = FMoEGatedMLP(num_expert=4, d_model=24, d_hidden=40, top_k=2).cuda()
+    linear = getattr(layer.experts, name)
+    x = torch.randn(30, 24, device="cuda", requires_grad=True)
+    more = torch.linspace(-1, 1, linear.out_feat, device="cuda")
+    layer.enable_fuse = fuse
+    plain = layer(x).detach()
+    with torch.no_grad():
+        linear.bias += more
+        want = layer(x)
+        linear.bias -= more
+    # (float32 all through: products in another order)
+    close = lambda got: torch.allclose(got, want, rtol=1e-4, atol=1e-5) and not torch.allclose(got, plain, rtol=1e-2, atol=1e-2)
+    hook = linear.register_forward_hook(lambda module, args, out: out + more)
+    assert close(layer(x))
+    hook.remove()
+    adapter = _Adapter(linear, linear.out_feat)
+    setattr(layer.experts, name, adapter)
+    y = layer(x)
+    assert close(y)
+    y.square().sum().backward()
+    assert adapter.more.grad is not None and adapter.more.grad.abs().max() > 0 and linear.weight.grad is not None
