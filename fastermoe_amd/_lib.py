@@ -103,11 +103,13 @@ SIGNATURES = {
     "fmoe_balance_loss_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "fmoe_act_checkpoint_forward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
     "fmoe_act_checkpoint_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "fmoe_gated_mlp_supported": (_int, [_i64, _i64, _int]),
     "fmoe_gated_mlp_forward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int, _int]),
     "fmoe_gated_mlp_forward": (_int, [_vp] * 9 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
     "fmoe_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int]),
     "fmoe_gated_mlp_backward": (_int, [_vp] * 12 + [_i64] * 4 + [_int, _int, _vp, _i64, _vp]),
     "fmoe_quantize_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "fmoe_linear_int8_supported": (_int, [_i64, _i64, _int, _int]),
     "fmoe_linear_int8_rounds_rows": (_int, [_i64, _i64, _i64, _i64, _int, _int]),
     "fmoe_linear_int8": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp, _i64, _vp]),
     "fmoe_linear_int8_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _int, _int]),

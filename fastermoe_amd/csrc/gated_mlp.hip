@@ -119,16 +119,21 @@ struct Sizes {
     int64_t n_expert, rows, d, h;
     int dtype, activation;
 };
+// float32, and its rounded sizes: offsets from a tile's first row of weights, over both halves, in 31 bits; rows of at most 4 MiB
+bool features_taken(int64_t d, int64_t h, int dtype) {
+    return d <= (1 << 28) && h <= (1 << 28) &&
+           (dtype != FMOE_F32 || ((2 * h + 264) * (d + 3) * 4 < ((int64_t)1 << 31) && 2 * (h + 3) * 4 <= (1 << 22) && ceil_div(d, 4) * 16 <= (1 << 22)));
+}
 int check(const char *who, const Sizes &s) {
     FMOE_REQUIRE(s.dtype == FMOE_F32 || s.dtype == FMOE_BF16 || s.dtype == FMOE_F16, "%s: dtype %d is not float32, bfloat16 or float16", who, s.dtype);
     FMOE_REQUIRE(is_gate_activation(s.activation), "%s: unknown activation %d", who, s.activation);
     FMOE_REQUIRE(s.n_expert >= 1 && s.rows >= 0 && s.d >= 1 && s.h >= 1, "%s: bad sizes", who);
-    if (s.n_expert > (1 << 24) || s.rows > (int64_t)INT32_MAX - 65536 || s.d > (1 << 28) || s.h > (1 << 28) ||
-        ceil_div(s.rows * per_row(s.h), kBlock) > kMostThreads / kBlock)
+    if (!features_taken(s.d, s.h, s.dtype))
+        return fail(FMOE_ELIMIT, "%s: d_model=%lld d_hidden=%lld are beyond the supported range (float32: 2 GiB of an expert's weights, rows of 4 MiB)", who,
+                    (long long)s.d, (long long)s.h);
+    if (s.n_expert > (1 << 24) || s.rows > (int64_t)INT32_MAX - 65536 ||
+        (s.dtype == FMOE_F32 && ceil_div(s.rows * per_row(s.h), kBlock) > kMostThreads / kBlock))   // (the activation's kernel)
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
-    // (float32, and its rounded sizes: offsets from a tile's first row of weights, over both halves, in 31 bits)
-    if (s.dtype == FMOE_F32 && ((2 * s.h + 264) * (s.d + 3) * 4 >= ((int64_t)1 << 31) || 2 * (s.h + 3) * 4 > (1 << 22)))
-        return fail(FMOE_ELIMIT, "%s: an expert's float32 weights of 2 GiB are beyond the supported range", who);
     return FMOE_OK;
 }
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -372,6 +377,10 @@ int64_t backward_bytes(const Sizes &s) {
 }  // namespace fmoe
 
 using namespace fmoe;
+
+extern "C" int fmoe_gated_mlp_supported(int64_t d_model, int64_t d_hidden, int dtype) {
+    return (dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16) && d_model >= 1 && d_hidden >= 1 && features_taken(d_model, d_hidden, dtype);
+}
 
 extern "C" int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows, int64_t d_model, int64_t d_hidden, int dtype, int activation,
                                                           int keep) {

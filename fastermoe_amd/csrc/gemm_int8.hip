@@ -24,7 +24,16 @@ Int8Params sizes(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t ou
 bool sizes_known(int64_t n_expert, int64_t rows_cap, int64_t in_feat, int64_t out_feat) {
     return n_expert >= 1 && rows_cap >= 1 && in_feat >= 1 && in_feat <= 131072 && out_feat >= 1 && out_feat <= (1 << 28);
 }
+// (131072 products of numbers up to 128: below 2^31; a tile's rows within 2 GiB of its first)
+bool features_taken(int64_t in_feat, int64_t out_feat, int64_t w_rows, int64_t ldw, int dtype) {
+    return in_feat <= 131072 && out_feat <= (1 << 28) && ldw <= (1 << 22) && w_rows * ldw < ((int64_t)1 << 31) && out_feat * dtype_bytes(dtype) <= (1 << 22);
+}
 }  // namespace
+
+extern "C" int fmoe_linear_int8_supported(int64_t in_feat, int64_t out_feat, int gated, int dtype) {
+    return (dtype == FMOE_F32 || dtype == FMOE_BF16 || dtype == FMOE_F16) && in_feat >= 1 && out_feat >= 1 &&
+           features_taken(in_feat, out_feat, out_feat * (gated ? 2 : 1), ceil_div(in_feat, 16) * 16, dtype);
+}
 
 extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale, const int64_t *row_index, int64_t index_div, int64_t x_rows, const void *w, int64_t ldw, int64_t w_expert_stride,
                                 const void *w_scale, const void *bias, void *y, const void *segment_table, int64_t n_expert, int64_t rows_cap,
@@ -35,9 +44,7 @@ extern "C" int fmoe_linear_int8(const void *x, int64_t ldx, const void *x_scale,
     FMOE_REQUIRE(is_gate_activation(activation), "%s: unknown activation %d", who, activation);
     FMOE_REQUIRE(n_expert >= 1 && rows_cap >= 0 && in_feat >= 1 && out_feat >= 1, "%s: bad sizes", who);
     const int64_t whole = ceil_div(in_feat, 16) * 16, w_rows = out_feat * (gated ? 2 : 1);
-    // (131072 products of numbers up to 128: below 2^31)
-    if (in_feat > 131072 || n_expert > (1 << 24) || rows_cap > (int64_t)INT32_MAX - 65536 || out_feat > (1 << 28) || (x_scale != nullptr && ldx > (1 << 22)) ||
-        ldw > (1 << 22) || w_rows * ldw >= ((int64_t)1 << 31) || out_feat * dtype_bytes(dtype) > (1 << 22))   // (a tile's rows within 2 GiB of its first)
+    if (n_expert > (1 << 24) || rows_cap > (int64_t)INT32_MAX - 65536 || (x_scale != nullptr && ldx > (1 << 22)) || !features_taken(in_feat, out_feat, w_rows, ldw, dtype))
         return fail(FMOE_ELIMIT, "%s: sizes beyond the supported range", who);
     FMOE_REQUIRE((x_scale == nullptr || (ldx >= whole && ldx % 16 == 0)) && ldw >= whole && ldw % 16 == 0 && w_expert_stride % 16 == 0 && w_expert_stride >= 0,
                  "%s: rows of 8-bit integers begin on 16 bytes, at least %lld apart", who, (long long)whole);

@@ -876,9 +876,10 @@ def act_checkpoint_backward(grad, held, scale, activation, with_mid=True, table=
 _GATE_ACTIVATIONS = (_lib.ACT_NONE, _lib.ACT_RELU, _lib.ACT_GELU, _lib.ACT_SILU)
 
 
-def gated_mlp_supported(dtype):
-    """Whether gated experts of this type are one call."""
-    return dtype in (torch.float32, torch.bfloat16, torch.float16)
+def gated_mlp_supported(dtype, d_model=1, d_hidden=1):
+    """Whether gated experts of this type and these sizes are one call."""
+    return (dtype in (torch.float32, torch.bfloat16, torch.float16)
+            and _lib.load().fmoe_gated_mlp_supported(int(d_model), int(d_hidden), _DTYPES[dtype]) == 1)
 
 
 def _gate_activation(activation):
@@ -988,6 +989,12 @@ def _rows_to_round(x, row_index, index_div):
         if int(index_div) < 1:
             raise ValueError(f"index_div is {index_div}")
     return x, ldx, n
+
+
+def linear_int8_supported(in_feat, out_feat, gated, dtype):
+    """Whether :func:`linear_int8` takes these sizes for rows of this type."""
+    return (dtype in (torch.float32, torch.bfloat16, torch.float16)
+            and _lib.load().fmoe_linear_int8_supported(int(in_feat), int(out_feat), int(bool(gated)), _DTYPES[dtype]) == 1)
 
 
 def quantize_rows(x, row_index=None, index_div=1, table=None, tail=None):

@@ -150,7 +150,7 @@ def _is_its_product(linear):
 class _GatedExpert(_Expert):
     r"""All experts of a worker as gated blocks, ``h4toh(act(g) * u)`` with ``[g u] = htoh4(x)``: ``htoh4`` has ``2 * d_hidden`` outputs, the
     gate's first.  With SiLU, exact GELU, ReLU or no activation one call each way (:func:`fastermoe_amd.functions.gated_mlp`), else, or
-    where a linear was replaced or has hooks, the modules one by one."""
+    where a linear was replaced or has hooks or the call does not take the sizes, the modules one by one."""
 
     def __init__(self, num_expert, d_model, d_hidden, activation, rank=0, bias=True):
         super().__init__(num_expert, d_model, d_hidden, activation, rank=rank, bias=bias)
@@ -163,8 +163,9 @@ class _GatedExpert(_Expert):
 
     def _one_call(self, inp):
         """The activation's code where the block is one call, else ``None``."""
-        if not (inp.is_cuda and fmoe_native.gated_mlp_supported(inp.dtype) and os.environ.get("FMOE_EXPERT_EPILOGUE", "1") != "0"
+        if not (inp.is_cuda and os.environ.get("FMOE_EXPERT_EPILOGUE", "1") != "0"
                 and _is_its_product(self.htoh4) and _is_its_product(self.h4toh)
+                and fmoe_native.gated_mlp_supported(inp.dtype, *self.h4toh.weight.shape[1:])
                 and all(p is None or p.dtype == inp.dtype for linear in (self.htoh4, self.h4toh) for p in (linear.weight, linear.bias))):
             return None
         return _gate_code_or_none(self.activation)
@@ -216,6 +217,9 @@ class _Int8Expert(nn.Module):
         for name in ("htoh4", "h4toh"):
             linear = getattr(experts, name)
             q, scale = quantize_rows(linear.weight)
+            halves = 2 if self.gated and name == "htoh4" else 1
+            if not fmoe_native.linear_int8_supported(q.shape[2], q.shape[1] // halves, halves == 2, linear.weight.dtype):
+                raise NotImplementedError(f"{name} of {tuple(q.shape)} is beyond the sizes of products in 8 bits for {linear.weight.dtype} rows")
             self.register_buffer(name + "_weight", q)
             self.register_buffer(name + "_scale", scale)
             self.register_buffer(name + "_bias", None if linear.bias is None else linear.bias.detach())

@@ -733,6 +733,11 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
 
 /* ---- gated experts ----------------------------------------------------------- */
 
+/* 1 when the gated block below takes these sizes in this type (float32: an
+ * expert's w1 below 2 GiB, rows of at most 4 MiB, pre's among them), else 0.  Host
+ * only. */
+int fmoe_gated_mlp_supported(int64_t d_model, int64_t d_hidden, int dtype);
+
 /* Per expert, over its rows:  [g u] = pre = x W1^T + b1,  mid = act(g) * u,
  * y = mid W2^T + b2.  w1 [E, 2 d_hidden, d_model] (the gate's rows, then the
  * linear half's), b1 [E, 2 d_hidden] or NULL, w2 [E, d_model, d_hidden], b2
@@ -740,8 +745,8 @@ int fmoe_act_checkpoint_backward(const void *grad, const void *held,
  * [rows, d_hidden] and y [rows, d_model]; behind the rows that the experts have
  * y is zero, pre and mid are left as they are.
  * The rows' segments come from segment_table (of fmoe_segment_table_build for
- * `rows` rows).  FMOE_F32 (tensors on 16 bytes, an expert's weights below 2 GiB) /
- * FMOE_BF16 / FMOE_F16; any FMOE_ACT_*.
+ * `rows` rows).  FMOE_F32 (tensors on 16 bytes) / FMOE_BF16 / FMOE_F16, sizes of
+ * fmoe_gated_mlp_supported; any FMOE_ACT_*.
  * The workspace (on 16 bytes) belongs to the call until it has run.  Its size: keep
  * not 0 where pre is given. */
 int64_t fmoe_gated_mlp_forward_workspace_bytes(int64_t n_expert, int64_t rows,
@@ -787,6 +792,10 @@ int fmoe_quantize_rows(const void *x, int64_t ldx, const int64_t *row_index,
                        void *scale, const void *segment_table, void *tail,
                        int64_t tail_bytes, int64_t rows, int64_t row_elems,
                        int dtype, void *stream);
+
+/* 1 when fmoe_linear_int8 takes these features, with rows of w as close as they may
+ * lie and results of this type, else 0.  Host only. */
+int fmoe_linear_int8_supported(int64_t in_feat, int64_t out_feat, int gated, int dtype);
 
 /* y[r, c] = act(x_scale[r] w_scale[c] sum_k x[r, k] w[c, k] + bias[c]) per
  * expert over its rows; gated: act(that of row c) * (that of row out_feat + c).

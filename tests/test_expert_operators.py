@@ -181,3 +181,31 @@ def test_replaced_linears_are_not_held_in_8_bits(kind, name):
         with pytest.raises(TypeError, match=name):
             layer.quantize_experts()
         assert layer.experts is before
+
+
+@pytest.mark.parametrize("dt,d,h,taken", [
+    (_lib.F32, 8, 16, 1), (_lib.F32, 1 << 15, 8059, 1), (_lib.F32, 1 << 15, 8060, 0), (_lib.F32, 1 << 14, 1 << 14, 0), (_lib.F32, 16, (1 << 19) - 3, 1),
+    (_lib.F32, 16, (1 << 19) - 2, 0), (_lib.F32, 1 << 20, 4, 1), (_lib.F32, (1 << 20) + 1, 4, 0), (_lib.BF16, 1 << 14, 1 << 15, 1),
+    (_lib.F16, 1 << 28, 1 << 28, 1), (_lib.F16, (1 << 28) + 1, 4, 0), (_lib.BF16, 4, (1 << 28) + 1, 0), (_lib.BF16, 4, 1 << 60, 0)])
+def test_sizes_of_gated_experts(dt, d, h, taken):
+    """What the question says is what the call does (which says next that there is no x)."""
+    assert lib.fmoe_gated_mlp_supported(d, h, dt) == taken
+    assert _gated_forward(x=None, dt=dt, d=d, h=h) == (EINVAL if taken else ELIMIT)
+    assert _gated_backward(x=None, dt=dt, d=d, h=h) == (EINVAL if taken else ELIMIT)
+
+
+def test_sizes_that_nothing_has():
+    assert lib.fmoe_gated_mlp_supported(0, 8, _lib.BF16) == lib.fmoe_gated_mlp_supported(8, 0, _lib.BF16) == lib.fmoe_gated_mlp_supported(8, 8, _lib.F64) == 0
+    assert lib.fmoe_linear_int8_supported(0, 8, 0, _lib.BF16) == lib.fmoe_linear_int8_supported(8, 0, 0, _lib.BF16) == 0
+    assert lib.fmoe_linear_int8_supported(8, 8, 0, _lib.F64) == 0
+    assert not fmoe_native.gated_mlp_supported(torch.float64) and not fmoe_native.linear_int8_supported(8, 8, False, torch.float64)
+
+
+@pytest.mark.parametrize("dt,d,out,gated,taken", [
+    (_lib.BF16, 32, 16, 0, 1), (_lib.BF16, 131072, 16383, 0, 1), (_lib.BF16, 131072, 16384, 0, 0), (_lib.BF16, 131072, 8192, 1, 0),
+    (_lib.BF16, 131072, 8191, 1, 1), (_lib.BF16, 131073, 4, 0, 0), (_lib.F16, 16, 1 << 21, 1, 1), (_lib.F16, 16, (1 << 21) + 1, 0, 0),
+    (_lib.F32, 16, 1 << 20, 0, 1), (_lib.F32, 16, (1 << 20) + 1, 0, 0)])
+def test_sizes_of_8_bit_products(dt, d, out, gated, taken):
+    assert lib.fmoe_linear_int8_supported(d, out, gated, dt) == taken
+    whole = -(-d // 16) * 16
+    assert _linear(x=None, dt=dt, d=d, ldx=whole, ldw=whole, wes=whole, out=out, gated=gated) == (EINVAL if taken else ELIMIT)

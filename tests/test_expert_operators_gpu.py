@@ -5,7 +5,7 @@ import copy
 import pytest
 import torch
 
-from fastermoe_amd import FMoEGatedMLP, FMoEPositionwiseFF, _lib, fmoe_native, functions
+from fastermoe_amd import FMoEGatedMLP, FMoEPositionwiseFF, FMoETransformerMLP, _lib, fmoe_native, functions
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -261,3 +261,51 @@ def test_gated_experts_call_what_stands_in_a_linears_place(name, fuse):
     assert close(y)
     y.square().sum().backward()
     assert adapter.more.grad is not None and adapter.more.grad.abs().max() > 0 and linear.weight.grad is not None
+
+
+def test_gated_experts_past_one_calls_sizes():
+    """float32 weights of 2 GiB to an expert: module by module.  Errors: sums of n float32 products, 16 2^-24 sqrt(n) of their norm (see tests/test_gated_gpu.py)
+    for each of the two products, and as much again for what the first one's do to the second."""
+    d = h = 1 << 14
+    with torch.device("cuda"):
+        layer = FMoEGatedMLP(num_expert=1, d_model=d, d_hidden=h, top_k=1, bias=False)
+        with torch.no_grad():
+            layer.experts.htoh4.weight.normal_().mul_(d ** -0.5)
+            layer.experts.h4toh.weight.normal_().mul_(h ** -0.5)
+    assert not fmoe_native.gated_mlp_supported(torch.float32, d, h)
+    x = torch.randn(5, d, device="cuda", requires_grad=True)
+    y = layer(x)
+    gy = torch.randn_like(y)
+    y.backward(gy)
+    ex = layer.experts
+    with torch.no_grad():
+        score = layer.gate(x)[1].double().reshape(5, 1)
+        w1, w2 = ex.htoh4.weight[0].double(), ex.h4toh.weight[0].double()
+        g, u = (x.double() @ w1.t()).chunk(2, dim=1)
+        a = torch.nn.functional.silu(g)
+        want = (a * u) @ w2.t() * score
+        norm = lambda t: t.double().norm().item()
+        tol = 4 * 16 * 2.0 ** -24 * (d ** 0.5)
+        assert norm(y - want) <= tol * norm(want)
+        dy = gy.double() * score
+        assert norm(ex.h4toh.weight.grad[0] - dy.t() @ (a * u)) <= tol * norm(dy.t() @ (a * u))
+        dm = dy @ w2
+        s = torch.sigmoid(g)
+        dg = dm * u * s * (1 + g * (1 - s))
+        got = ex.htoh4.weight.grad[0]
+        assert norm(got[:h] - dg.t() @ x.double()) <= tol * norm(dg.t() @ x.double())
+        assert norm(got[h:] - (dm * a).t() @ x.double()) <= tol * norm((dm * a).t() @ x.double())
+    layer.zero_grad(set_to_none=True)
+
+
+@pytest.mark.parametrize("kind", [FMoETransformerMLP, FMoEGatedMLP])
+def test_experts_past_the_sizes_of_8_bit_products_stay_as_they_are(kind):
+    with torch.device("cuda"):
+        layer = kind(num_expert=1, d_model=16, d_hidden=(1 << 21) + 16, top_k=1).half()
+    before = layer.experts
+    x = torch.randn(3, 16, device="cuda").half()
+    with torch.no_grad():
+        want = layer(x)
+        with pytest.raises(NotImplementedError, match="htoh4"):
+            layer.quantize_experts()
+        assert layer.experts is before and torch.equal(layer(x), want)
