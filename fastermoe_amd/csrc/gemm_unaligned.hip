@@ -16,6 +16,8 @@
 #include "gemm_kernel.hpp"
 #include "unaligned_loads.hpp"
 
+#include <optional>
+
 namespace fmoe {
 namespace {
 using namespace gemm;
@@ -495,7 +497,8 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
     if (total > (int64_t)INT32_MAX - 8) return fail(FMOE_ELIMIT, "grouped GEMM: %lld tiles exceed the grid limit", (long long)total);
     if (total == 0) return FMOE_OK;
     prm.total_tiles = (int)total;
-    ProfileScope prof(prm.profile_class, prm.profile_work, stream);
+    std::optional<ProfileScope> prof;
+    if (EPI != kEpiParts) prof.emplace(prm.profile_class, prm.profile_work, stream);   // (parts: launch_parts, around both launches)
     grouped_gemm_unaligned_kernel<T, BM, PS, QS, RG, EPI><<<(unsigned)((total + 7) / 8 * 8), kUaThreads, 0, stream>>>(prm);
     FMOE_LAUNCH_CHECK();
     return FMOE_OK;
@@ -503,6 +506,7 @@ int launch_unaligned_tiles(GemmParams &prm, int epilogue, hipStream_t stream) {
 
 // Ragged rows over a device table, prm.k_split parts of prm.split_slabs slabs each: sums into prm.split_ws, and those added up.
 template <typename T, int PS> int launch_parts(GemmParams &prm, hipStream_t stream) {
+    ProfileScope prof(prm.profile_class, prm.profile_work, stream);
     if (int rc = launch_unaligned_tiles<T, 64, PS, kKC, kRaggedRows, kEpiParts>(prm, kEpiStore, stream)) return rc;
     prm.dev_map_off = (int)segtab::map128_off(prm.dev_rows_cap, prm.tab.n);
     const int64_t places = segtab::cap_tiles(prm.dev_rows_cap, prm.tab.n, 128);

@@ -27,3 +27,16 @@ def test_inline_asm_names_the_special_registers_it_writes():
         if any(re.match(r"s_(cmp|add|sub|and|or|lshl|lshr)\w*\s", line) for line in code):
             assert "scc" in strings, f"{name}: {body}"
     assert seen >= 3
+
+
+def test_the_profile_covers_every_launch_of_a_product():
+    """Where a file's launches open the profile's scopes themselves, none comes ahead of its function's scope: a product of two launches would be reported with
+    the time of one and the work of both."""
+    seen = 0
+    for name in ("gemm_any.hip", "gemm_kernel.hpp", "gemm_unaligned.hip"):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "fastermoe_amd", "csrc", name)).read())
+        for m in re.finditer("<<<", text):
+            start = max(f.start() for f in re.finditer(r"^[a-z][^\n;=]*\)\s*\{$", text[:m.start()], flags=re.M))   # its function's first line
+            assert re.search(r"ProfileScope", text[start:m.start()]), f"{name}: {text[start:m.start()].splitlines()[0]}"
+            seen += 1
+    assert seen >= 4
