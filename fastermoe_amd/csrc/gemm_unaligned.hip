@@ -7,9 +7,13 @@
 // and products are the same.  Where the contraction or the row of a [contraction][index] operand ends inside a chunk, the
 // chunk that ends with it is read and moved down; rows past a tile's end repeat its last row and are not stored.
 //
-// 128 x 128 tiles (64 x 64 per wave), 64 x 128 where those would leave compute units without one; one slab of
-// LDS, the next slab's chunks are requested before the products of the current one: four workgroups share a unit, and one computes while others wait (with two slabs and two
-// workgroups: 8192 rows, 8 experts of 2047 -> 2 x 4093, both forward products 763 us, 690 so; 1554 rows, 12 of 500 -> 2 x 1302: 47 and 41).  Bound by the latency of those
+// 128 x 128 tiles (64 x 64 per wave), 64 x 128 where those would leave compute units without one; the next slab's chunks are requested before the products of the current
+// one.  Forward products and data gradients have one slab of LDS, so that registers alone decide how many workgroups share a compute unit, and one computes while others
+// wait: four with 64-row forward products, three with 64-row data gradients and 128-row gated forwards, two with the other 128-row tiles.  Weight gradients, two to a
+// unit either way, have two slabs and a barrier less.  us of the kernel with one / two slabs, bfloat16: gated forward, 8192 rows, 8 experts of 1023 -> 2 x 2047: 127 / 148, of
+// 2047 -> 2 x 4093: 520 / 584, 32768 rows, 8 of 1022 -> 2 x 4090: 922 / 1006; plain, 16384 rows, 16 of 1001 x 1003: 82 / 84, with an activation 103 / 101; data gradients, 8192 rows, 8
+// of 2047 x 4093: 317 / 324 (within 1 % on average); weight gradients there 302 / 299, 8 of 1023 x 2047: 83 / 79, 1554 rows, 12 of 500 x 2604: 27.7 / 26.5.
+// Bound by the latency of those
 // loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (600 TFLOP/s there).  Where few tiles have long contractions, a gated block's products share them between workgroups (launch_parts; see unaligned_parts() in
 // grouped_gemm.hip).  The epilogues of gated products are those of gemm_kernel.hpp: 1554 rows, 12 experts of 500 -> 2 x 1302 in float16, 25 us forward and 24 for the
 // gradient.  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
@@ -28,6 +32,9 @@ constexpr int kUaThreads = 256, kUaBN = 128, kUaBK = 64;
 constexpr int kEpiParts = 100;
 __host__ __device__ __forceinline__ int parts_ld(int n_cols) { return (n_cols + 3) & ~3; }   // floats from row to row of those
 
+// Slabs of LDS: see above
+constexpr int slabs_of(int ragged) { return ragged == kRaggedK ? 2 : 1; }
+
 // PSHAPE / QSHAPE: kKC = [index][contraction] in memory, kMC = [contraction][index].  EPI: kEpiGated, kEpiDGated, kEpiParts, or 0: what the parameters say.
 template <typename T, int BM, int PSHAPE, int QSHAPE, int RAGGED, int EPI>
 __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(const GemmParams prm) {
@@ -39,7 +46,8 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
     constexpr bool kBiasGrad = RAGGED == kRaggedK;
     constexpr bool kHalves = epi_halves(EPI);
     constexpr int kCols = kHalves ? BN / 2 : BN;   // C columns of a tile
-    __shared__ __attribute__((aligned(16))) unsigned char smem[STAGE];
+    constexpr int kSlabs = slabs_of(RAGGED);
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kSlabs * STAGE];
 
     if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
         const int64_t there = ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)prm.dev_tab)[segtab::kRows];
@@ -230,9 +238,10 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         fetch(QSHAPE, qr, NQ, Q, q_off, prm.ldq, q_valid, BM, prm.n_rows, 0);
     }
     for (int s = 0; s < n_slabs; ++s) {
-        if (s > 0) lds_barrier();   // (the slab before has been read)
-        put(PSHAPE, pr, NP, smem);
-        put(QSHAPE, qr, NQ, smem + P_BYTES);
+        unsigned char *buf = smem + (kSlabs == 2 ? s & 1 : 0) * STAGE;
+        if (kSlabs == 1 && s > 0) lds_barrier();   // (the slab before has been read; with two: the one before that, ahead of the last barrier)
+        put(PSHAPE, pr, NP, buf);
+        put(QSHAPE, qr, NQ, buf + P_BYTES);
         lds_barrier();
         if (s + 1 < n_slabs) {
             fetch(PSHAPE, pr, NP, P, p_off, prm.ldp, p_valid, BN, prm.n_cols, (s + 1) * BK);
@@ -242,9 +251,9 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         for (int ks = 0; ks < 2; ++ks) {
             u32x4 pf[TI], qf[TJ];
 #pragma unroll
-            for (int x = 0; x < TI; ++x) pf[x] = frag(PSHAPE, smem, wn * TI + x, ks);
+            for (int x = 0; x < TI; ++x) pf[x] = frag(PSHAPE, buf, wn * TI + x, ks);
 #pragma unroll
-            for (int y = 0; y < TJ; ++y) qf[y] = frag(QSHAPE, smem + P_BYTES, row_block(y), ks);
+            for (int y = 0; y < TJ; ++y) qf[y] = frag(QSHAPE, buf + P_BYTES, row_block(y), ks);
 #pragma unroll
             for (int x = 0; x < TI; ++x)
 #pragma unroll
