@@ -48,7 +48,7 @@ template <typename T, bool ODD> struct Row {
 };
 
 template <typename T, bool HALVES, bool ODD>
-__global__ __launch_bounds__(kFewThreads) void grouped_gemm_few_unaligned_kernel(const SkinnyParams prm) {
+__global__ __launch_bounds__(kFewThreads) void grouped_gemm_few_unaligned_kernel(const SkinnyMoreParams prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
     constexpr int kCols = HALVES ? 16 : 32;
     typedef const int32_t __attribute__((address_space(4))) *DevTab;    // read-only, uniform: scalar loads
@@ -192,8 +192,8 @@ __global__ __launch_bounds__(kFewThreads) void grouped_gemm_few_unaligned_kernel
 #endif
 }
 
-template <typename T, bool HALVES> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
-    SkinnyParams prm = params;
+template <typename T, bool HALVES> int launch(const SkinnyMoreParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+    SkinnyMoreParams prm = params;
     prm.order_off = (int32_t)segtab::map128_off(rows_cap, n_expert);
     prm.tiles_n = (int)ceil_div(prm.n_cols, HALVES ? 16 : 32);
     const int64_t grid = segtab::cap_tiles(rows_cap, n_expert, 128) * prm.tiles_n;
@@ -207,7 +207,7 @@ template <typename T, bool HALVES> int launch(const SkinnyParams &params, int64_
 
 }  // namespace
 
-int launch_few_unaligned(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+int launch_few_unaligned(const SkinnyMoreParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16, "grouped GEMM: dtype %d is not a 16-bit float type", dtype);
     if (dtype == FMOE_BF16) return gated ? launch<__bf16, true>(prm, rows_cap, n_expert, stream) : launch<__bf16, false>(prm, rows_cap, n_expert, stream);
     return gated ? launch<_Float16, true>(prm, rows_cap, n_expert, stream) : launch<_Float16, false>(prm, rows_cap, n_expert, stream);

@@ -34,7 +34,6 @@ constexpr int kSkRows = 32;   // rows of a pass
 
 // one 16 x 16 block over 64 bytes of contraction; acc as for the 16 x 16 x 32 form
 template <typename T> __device__ __forceinline__ void mma_step(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<T>::mma(acc, w, x); }
-template <> __device__ __forceinline__ void mma_step<Int8Pair<float>>(f32x4 &acc, const u32x4 &w, const u32x4 &x) { Elem<Int8Pair<float>>::mma(acc, w, x); }
 template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u32x4 &w, const u32x4 &x) {
     // product j takes element j of every lane's four: contraction elements j, 4 + j, 8 + j and 12 + j of the step
 #pragma unroll
@@ -42,10 +41,12 @@ template <> __device__ __forceinline__ void mma_step<float>(f32x4 &acc, const u3
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[j]), acc, 0, 0, 0);
 }
 
+template <typename T, bool HALVES> using Params = std::conditional_t<HALVES || IsInt8<T>::value, SkinnyMoreParams, SkinnyParams>;
+
 // COL_BLOCKS: blocks of 16 columns of a workgroup.  APART: an expert's groups of rows have workgroups of their own (see launch).  HALVES: gated.  ROUND: at most
 // kSkinnyRoundRows rows in all, of the results' type
 template <typename T, int COL_BLOCKS, bool APART, bool HALVES, bool ROUND>
-__global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_gemm_skinny_kernel(const SkinnyParams prm) {
+__global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_gemm_skinny_kernel(const Params<T, HALVES> prm) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
     constexpr int EB = (int)sizeof(T), CE = 16 / EB, kLine = 128 / EB;    // elements per lane's load and per line
     typedef std::conditional_t<sizeof(T) == 2, u32x2, u32x4> Vec4;        // four elements
@@ -106,9 +107,14 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
 
     // weights: rows past the last column lie past the end of the resource and read as zero
     // (gated: past the last of the gate's columns lie the linear half's)
-    const int ldw = kInt8 ? (int)prm.ldw : K, ldx = kInt8 ? (int)prm.ldx : K;   // elements from row to row
-    const int64_t w_expert = kInt8 ? prm.w_expert_stride : (int64_t)(HALVES ? 2 : 1) * prm.n_cols * K;
-    const T *W = (const T *)prm.w + expert * w_expert + (int64_t)n0 * ldw;
+    int ldw = K, ldx = K;    // elements from row to row
+    int64_t w_first = ((int64_t)expert * ((HALVES ? 2 : 1) * prm.n_cols) + n0) * K;
+    if constexpr (kInt8) {
+        ldw = (int)prm.ldw;
+        ldx = (int)prm.ldx;
+        w_first = expert * prm.w_expert_stride + (int64_t)n0 * ldw;
+    }
+    const T *W = (const T *)prm.w + w_first;
     const int w_bytes = (min(kCols, prm.n_cols - n0) + (HALVES ? prm.n_cols : 0)) * ldw * EB;
     const __amdgpu_buffer_rsrc_t w_rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(W), 0, w_bytes, kRsrcFlags);
     const uint32_t w_off = (uint32_t)(row8 * ldw * EB + chunk * 16), eight_rows = (uint32_t)(8 * ldw * EB);
@@ -403,8 +409,8 @@ template <typename T> int skinny_blocks(const SkinnyParams &prm, int64_t experts
     return sizeof(T) == 2 && ceil_div(n_cols, 64) * 2 >= cus && (int64_t)prm.k_extent * 2 * 64 < ((int64_t)1 << 31) ? 4 : 2;
 }
 
-template <typename T, bool HALVES = false, bool ROUND = false> int launch(const SkinnyParams &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
-    SkinnyParams prm = params;
+template <typename T, bool HALVES = false, bool ROUND = false> int launch(const Params<T, HALVES> &params, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+    Params<T, HALVES> prm = params;
     // An expert's groups of rows go to workgroups of their own, where the experts come in order of their rows: the further groups first,
     // which leave at once where there are none.  128 experts of 1280 x 1280, 448 rows, 144 of them one expert's: 37 us in turn, 29 apart; 64 of 1280 x
     // 1280 in float32, 900 and 274: 116 and 82.
@@ -435,12 +441,12 @@ int launch_skinny(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t 
     return dtype == FMOE_BF16 ? launch<__bf16>(prm, rows_cap, n_expert, stream) : launch<_Float16>(prm, rows_cap, n_expert, stream);
 }
 #elif FMOE_SKINNY == 1
-int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+int launch_skinny_gated(const SkinnyMoreParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     FMOE_REQUIRE(dtype == FMOE_BF16 || dtype == FMOE_F16, "grouped GEMM: dtype %d is not a 16-bit float type", dtype);
     return dtype == FMOE_BF16 ? launch<__bf16, true>(prm, rows_cap, n_expert, stream) : launch<_Float16, true>(prm, rows_cap, n_expert, stream);
 }
 #elif FMOE_SKINNY == 2
-int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
+int launch_skinny_int8(const SkinnyMoreParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream) {
     auto go = [&](auto pair) {
         using Pair = decltype(pair);
         if (prm.x_scale == nullptr) return gated ? launch<Pair, true, true>(prm, rows_cap, n_expert, stream) : launch<Pair, false, true>(prm, rows_cap, n_expert, stream);

@@ -15,14 +15,17 @@ struct SkinnyParams {
     int32_t div_shift;
     int32_t n_cols, k_extent, activation;
     int32_t weights_cached;       // not 0: the weights through the caches, see caches_few_row_weights() in grouped_gemm.hip
-    // Gated products and such in 8-bit integers (w: [E, 2 n_cols or n_cols, k], a gate's rows first; aux [rows, 2 n_cols]):
+    int32_t order_off, tiles_n, extra_groups;   // set by the launch: the table's list of experts (or its map of row tiles), see launch()
+};
+// Gated products and such in 8-bit integers (w: [E, 2 n_cols or n_cols, k], a gate's rows first; aux [rows, 2 n_cols]).  A type of its own: plain
+// products of a few rows feel how long a launch's arguments are (1 row, 2048 experts of 512 x 512, in a graph: 3.72 us; with these between theirs 3.82).
+struct SkinnyMoreParams : SkinnyParams {
     int64_t ldw, ldx, w_expert_stride;         // 8-bit integers: row strides in pairs of them (others are dense)
     const float *w_scale, *x_scale;            // 8-bit integers: of each row of w and of x; x_scale null: x in y's type, to be rounded here
     int64_t index_div;                         // rows to be rounded: row_index's divisor, elements of a row (ldx apart)
     int32_t x_elems;
     void *tail;                                // gated, or rows to be rounded: rows of tail_elems elements behind the table's, up to tail_rows, become zeros (null: none)
     int64_t tail_rows, tail_elems;
-    int32_t order_off, tiles_n, extra_groups;   // set by the launch: the table's list of experts (or its map of row tiles), see launch()
 };
 
 // Rows that the launch in 8-bit integers rounds itself: at most this many, of at most this many elements in all (a row's rounded up to sixteen).  Each workgroup rounds all
@@ -34,12 +37,12 @@ constexpr int kSkinnyRoundRows = 16, kSkinnyRoundElems = 8192;
 // rows_cap: the rows that the table was laid out for
 int launch_skinny(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 // gated forward, 16-bit types
-int launch_skinny_gated(const SkinnyParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
+int launch_skinny_gated(const SkinnyMoreParams &prm, int dtype, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 // rows and weights in 8-bit integers, k_extent in pairs, dtype of the results, whose columns are a multiple of four
-int launch_skinny_int8(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
+int launch_skinny_int8(const SkinnyMoreParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 
 // Rows off the 16-byte grid, 16-bit types (gemm_few_unaligned.hip): the plain or the gated forward product
-int launch_few_unaligned(const SkinnyParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
+int launch_few_unaligned(const SkinnyMoreParams &prm, int dtype, bool gated, int64_t rows_cap, int64_t n_expert, hipStream_t stream);
 
 // Two loads of 128 bytes of rows 0 to 7 and 8 to 15 (lane: row lane % 8, bit 3: half of the line) become the operands of two
 // steps (lane: row lane % 16, chunk lane / 16 of the step's 64 bytes): the lanes with bit 3 set give the first load's second chunks

@@ -658,7 +658,7 @@ int grouped_linear_forward(const LinearForwardArgs &a, const int64_t *counts, in
         prm.bias_expert_stride = a.out_feat;
         prm.n_cols = (int)a.out_feat; prm.k_extent = (int)a.in_feat;
         if (any_grid && a.dev_any_order && few_unaligned(a.dev_rows_cap, n_expert, a.in_feat, a.out_feat, a.dtype)) {
-            SkinnyParams sk{};
+            SkinnyMoreParams sk{};
             sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
             sk.n_cols = prm.n_cols; sk.k_extent = prm.k_extent;
             ProfileScope prof(prm.profile_class, prm.profile_work, stream);
@@ -873,7 +873,7 @@ int grouped_gated_forward(const GatedArgs &a, hipStream_t stream) {
     const bool fits = gated_sizes_fit(a);
     const bool few = fits ? gated_forward_few(a) : few_unaligned(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype);
     if (few) {
-        SkinnyParams sk{};
+        SkinnyMoreParams sk{};
         sk.w = a.w; sk.x = a.in; sk.bias = a.bias; sk.y = a.out; sk.aux = a.pre; sk.dev_tab = a.dev_tab;
         sk.n_cols = (int)a.h; sk.k_extent = (int)a.d; sk.activation = a.activation;
         LinearForwardArgs like{};
@@ -957,7 +957,7 @@ int launch_int8(const Int8Params &a, void *workspace, int64_t workspace_bytes, h
     const double work = 2.0 * (double)a.rows_cap * (double)a.k_extent * (double)w_rows;
     const int epi = a.gated ? kEpiInt8Gated : kEpiInt8;
     if (route.kernel == DevKernel::kSkinny) {
-        SkinnyParams sk{};
+        SkinnyMoreParams sk{};
         sk.w = a.w; sk.x = a.x; sk.bias = a.bias; sk.y = a.y; sk.dev_tab = a.dev_tab;
         sk.n_cols = a.n_cols; sk.k_extent = a.k_extent / 2; sk.activation = a.activation;
         sk.ldw = a.ldw / 2; sk.ldx = a.x_scale ? a.ldx / 2 : a.ldx; sk.w_expert_stride = a.w_expert_stride / 2; sk.w_scale = a.w_scale; sk.x_scale = a.x_scale;
