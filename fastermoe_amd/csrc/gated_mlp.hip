@@ -139,8 +139,8 @@ int check(const char *who, const Sizes &s) {
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // where a call's scratch rows and its products' own workspace lie, one behind the other
 struct Scratch {
-    int64_t first, second, split;   // bytes
-    int64_t total() const { return first + second + split; }
+    int64_t first, split;   // bytes
+    int64_t total() const { return first + split; }
 };
 GatedArgs gated_sizes(const Sizes &s) {
     static const int32_t some = 0;
@@ -150,14 +150,14 @@ GatedArgs gated_sizes(const Sizes &s) {
 }
 Scratch forward_scratch(const Sizes &s, bool keeps_pre) {
     const bool fused = gated_forward_fused(gated_sizes(s));
-    return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)), 0,
+    return Scratch{keeps_pre || fused ? 0 : round256(s.rows * 2 * s.h * dtype_bytes(s.dtype)),
                    std::max(fused ? gated_forward_workspace_bytes(gated_sizes(s))
                                   : fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE, 0, 0),
                             std::max(fmoe_linear_forward_dev_workspace_bytes(s.rows, s.n_expert, s.h, s.d, s.dtype, FMOE_ACT_NONE, 0, 0),
                                      unaligned_parts_bytes(s.rows, s.n_expert, s.d, s.h, s.dtype)))};
 }
 Scratch backward_scratch(const Sizes &s) {
-    return Scratch{round256(2 * s.rows * s.h * dtype_bytes(s.dtype)), 0,
+    return Scratch{round256(2 * s.rows * s.h * dtype_bytes(s.dtype)),
                    std::max(gated_dgrad_workspace_bytes(gated_sizes(s)),
                             std::max(fmoe_linear_dgrad_dev_workspace_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype, FMOE_ACT_NONE),
                                      unaligned_parts_bytes(s.rows, s.n_expert, s.d, 2 * s.h, s.dtype)))};
@@ -228,7 +228,7 @@ int forward(const Sizes &s, const Forward &f, const int32_t *table, char *ws, hi
 }
 
 int backward(const Sizes &s, const Backward &b, const int32_t *table, char *ws, hipStream_t stream) {
-    const Scratch need = s.rows == 0 ? Scratch{0, 0, 0} : backward_scratch(s);
+    const Scratch need = s.rows == 0 ? Scratch{0, 0} : backward_scratch(s);
     const Products p{table, s.n_expert, s.rows, s.dtype, ws + need.first, need.split, stream};
     void *grad_pre = ws;
     if (s.rows > 0 && (b.grad_x || b.grad_w1)) {

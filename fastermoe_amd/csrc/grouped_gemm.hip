@@ -839,7 +839,6 @@ bool gated_forward_fused(const GatedArgs &a) {
     if (is_16bit(a.dtype)) return a.dev_tab != nullptr;
     return gated_sizes_fit(a) && !use_skinny(a.rows_cap, a.n_expert, a.d, 2 * a.h, a.dtype);
 }
-bool gated_dgrad_fused(const GatedArgs &a) { return is_16bit(a.dtype) ? a.dev_tab != nullptr : gated_sizes_fit(a); }
 int64_t gated_forward_workspace_bytes(const GatedArgs &a) {
     return gated_forward_few(a) ? 0 : route_workspace_bytes(gated_route(a, gated_forward_tile(a)), a.d, a.dtype);
 }

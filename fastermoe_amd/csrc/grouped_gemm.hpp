@@ -10,7 +10,7 @@ enum Epilogue {
     kEpiStore = 0,    // C = acc (+ bias[col])
     kEpiBiasAct = 1,  // pre = acc + bias[col]; aux = pre (if aux); C = act(pre)
     kEpiDAct = 2,     // C = acc * act'(aux)          (aux = saved pre-activation)
-    // persistent kernel only:
+    // over a device table only:
     kEpiGated = 3,    // [g u] = acc + bias; aux = [g u] (if aux); C = act(g) u
     kEpiDGated = 4,   // C = [acc u act'(g), acc act(g)]  (aux = saved [g u])
     kEpiInt8 = 5,     // C = act(row scale * column scale * acc + bias)
@@ -148,8 +148,8 @@ int grouped_linear_dgrad(const LinearDgradArgs &a, const int64_t *counts_host, i
 // earlier chunk left (cuda/fused_compute.cuh:123, beta_weight).
 int grouped_linear_wgrad(const LinearWgradArgs &a, const int64_t *counts_host, int64_t n_expert,
                          int64_t row_lo, int64_t row_hi, bool last_chunk, hipStream_t stream);
-// Gated experts' products with the work between them in their epilogues (see gated_mlp.hip), over a table in device memory.  False where the sizes or types go
-// another way (grouped_linear_forward / _dgrad and a kernel between).  `tail`: rows of d elements behind the table's that become zeros.
+// Gated experts' products with the work between them in their epilogues (see gated_mlp.hip), over a table in device memory.  `tail`: rows of d elements
+// behind the table's that become zeros.
 struct GatedArgs {
     const void *in;      // forward: x [rows, d]; dgrad: the gradient of the second product's results, [rows, d]
     const void *w;       // forward: [E, 2 h, d]; dgrad: [E, d, h]
@@ -163,11 +163,11 @@ struct GatedArgs {
     void *workspace;     // for the split of a last round of tiles, as LinearForwardArgs::dev_workspace
     int64_t workspace_bytes;
 };
-bool gated_forward_fused(const GatedArgs &a);   // (sizes alone where the tensors are null)
+// False where the forward goes as grouped_linear_forward and a kernel for the activation (float32, few rows).  (Sizes alone where the tensors are null)
+bool gated_forward_fused(const GatedArgs &a);
 int64_t gated_forward_workspace_bytes(const GatedArgs &a);
 int64_t gated_dgrad_workspace_bytes(const GatedArgs &a);
 int grouped_gated_forward(const GatedArgs &a, hipStream_t stream);
-bool gated_dgrad_fused(const GatedArgs &a);
 int grouped_gated_dgrad(const GatedArgs &a, hipStream_t stream);
 
 // grad_b[e, c] = column sums of gy over the rows of expert e; same chunk rules.
