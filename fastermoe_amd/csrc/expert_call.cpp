@@ -51,7 +51,7 @@ struct GatedMLP : torch::autograd::Function<GatedMLP> {
         const int64_t n = x.size(0), d = x.size(1), e = w1.size(0), h = w2.size(2);
         const int dtype = dtype_code(x), act = (int)activation;
         const at::Tensor y = at::empty({n, d}, x.options()), mid = at::empty({n, h}, x.options());
-        const at::Tensor pre = keep ? at::empty({n, 2 * h}, x.options()) : at::Tensor();
+        const at::Tensor pre = keep ? at::empty({n, 2 * h}, x.options().dtype(at::kFloat)) : at::Tensor();
         const int64_t bytes = entry.gated_forward_bytes(e, n, d, h, dtype, act, keep);
         const at::Tensor space = space_of(bytes, x);
         ok(entry.gated_forward(pointer(x), pointer(w1), pointer(b1), pointer(w2), pointer(b2), pointer(pre), pointer(mid), pointer(y), pointer(table),

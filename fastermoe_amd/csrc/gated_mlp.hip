@@ -1,6 +1,6 @@
 // Gated experts (gfx950): per expert, over its rows,
 //
-//   g = x Wg^T + bg,  u = x Wu^T + bu,  m = act(g) u,  y = m W2^T + b2            (W1 = [Wg; Wu], its products [g u] = `pre`)
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  m = act(g) u,  y = m W2^T + b2            (W1 = [Wg; Wu], its products [g u] = `pre`, float32)
 //   dm = dy W2,  dg = dm u act'(g),  du = dm act(g),  dx = [dg du] W1,  dW1 = [dg du]^T x,  dW2 = dy^T m
 //
 // The products do the activation's work in their epilogues (gemm_kernel.hpp, gemm_ring.hpp, gemm_skinny.hip; rows off the 16-byte grid, 16-bit types:
@@ -400,6 +400,7 @@ extern "C" int fmoe_gated_mlp_forward(const void *x, const void *w1, const void 
     FMOE_REQUIRE(aligned16(segment_table), "%s: the segment table must be 16-byte aligned", who);
     FMOE_REQUIRE(dtype != FMOE_F32 || (aligned16(x) && aligned16(w1) && aligned16(b1) && aligned16(w2) && aligned16(b2) && aligned16(pre) && aligned16(mid) &&
                                        aligned16(y)), "%s: float32 tensors begin on 16 bytes", who);
+    FMOE_REQUIRE(((uintptr_t)pre & 3) == 0, "%s: pre holds float32", who);
     const int64_t need = forward_bytes(s, pre != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
         return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need);
@@ -427,6 +428,7 @@ extern "C" int fmoe_gated_mlp_backward(const void *grad_y, const void *x, const 
     FMOE_REQUIRE(dtype != FMOE_F32 || (aligned16(grad_y) && aligned16(x) && aligned16(w1) && aligned16(w2) && aligned16(pre) && aligned16(mid) &&
                                        aligned16(grad_x) && aligned16(grad_w1) && aligned16(grad_b1) && aligned16(grad_w2) && aligned16(grad_b2)),
                  "%s: float32 tensors begin on 16 bytes", who);
+    FMOE_REQUIRE(((uintptr_t)pre & 3) == 0, "%s: pre holds float32", who);
     const int64_t need = backward_bytes(s);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
         return fail(FMOE_EWORKSPACE, "%s: a workspace of %lld bytes on 16 bytes is needed", who, (long long)need);

@@ -168,7 +168,8 @@ __global__ __launch_bounds__(kFewThreads) void grouped_gemm_few_unaligned_kernel
         if (r0 + lb >= rows) continue;
         const int64_t row = first + r0 + lb;
         const T *bias = prm.bias ? (const T *)prm.bias + (int64_t)expert * (HALVES ? 2 : 1) * n_cols : nullptr;
-        T *y = (T *)prm.y + row * n_cols, *pre = prm.aux ? (T *)prm.aux + row * 2 * n_cols : nullptr;
+        T *y = (T *)prm.y + row * n_cols;
+        float *pre = HALVES && prm.aux ? (float *)prm.aux + row * 2 * n_cols : nullptr;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (HALVES) {
@@ -176,8 +177,8 @@ __global__ __launch_bounds__(kFewThreads) void grouped_gemm_few_unaligned_kernel
                 if (col >= n_cols) continue;
                 const float g = acc[0][i] + (bias ? (float)bias[col] : 0.f), u = acc[1][i] + (bias ? (float)bias[n_cols + col] : 0.f);
                 if (pre != nullptr) {
-                    pre[col] = (T)g;
-                    pre[n_cols + col] = (T)u;
+                    pre[col] = g;
+                    pre[n_cols + col] = u;
                 }
                 y[col] = (T)(gate_act<true>(g, prm.activation) * u);
             } else {

@@ -1451,10 +1451,10 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
         if (want_bias) __syncthreads();  // the bias reduction used the start of LDS
     }
     if constexpr (EPI >= kEpiGated) {
-        // Epilogues of gated products and of those in 8-bit integers.  Sums, scales, biases and activations are float32; what is rounded to 16 bits is what the next
-        // product reads as its operand (m, dg, du) and g, u, which a backward reads again at half of float32's bytes.  128 rows, 8 experts of 4096 -> 2 x 14336:
-        // 292 us, 6.4 TB/s; in float32 8192 rows, 8 of 512 -> 2 x 1024: 127 us forward, 90 for the gradient, 135 and 96 TFLOP/s.  A wave's sub-tile goes through its staging area kEpiCols columns at a time
-        // (rows of 64 or 128 bytes and 16 of padding); where g and u come in, they lie in two such areas and the results take their places.
+        // Epilogues of gated products and of those in 8-bit integers.  Sums, scales, biases and activations are float32, and so are g and u as a backward reads them again; what is
+        // rounded to 16 bits is what the next product reads as its operand (m, dg, du).  128 rows, 8 experts of 4096 -> 2 x 14336:
+        // 292 us, 6.4 TB/s; in float32 8192 rows, 8 of 512 -> 2 x 1024: 127 us forward, 90 for the gradient, 135 and 96 TFLOP/s.  What is stored goes through a wave's staging
+        // area, St::kCols columns at a time (rows of 64 or 128 bytes and 16 of padding); where results of 32 bits read g and u, those lie in two such areas and the results take their places.
         typedef typename Elem<T>::Out Out;
         typedef EpiStage<T, BM, BN, EPI> St;
         constexpr bool kNarrow = sizeof(Out) == 2;
@@ -1507,7 +1507,56 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) __builtin_amdgcn_raw_buffer_store_b128(*piece(a, i), rs, (int)offset(i, col, ld), 0, 0);
         };
-        if constexpr (EPI == kEpiDGated) {
+        if constexpr (EPI == kEpiDGated && kNarrow) {
+            // acc: dm; aux [rows, 2 n_cols] float32: g and u; C of the same shape: dg and du.  g and u come straight to the lanes that hold their columns' sums, two blocks of
+            // columns (whole lines) at a time where the registers are there
+            const float *in = (const float *)prm.aux + aux_off;
+            Out *out = (Out *)prm.C + aux_off;
+            constexpr int kBatch = LOADERS == kLoadersShared ? 1 : 2;
+            by_gate_activation<false>(prm.activation, [&](auto act) {
+#pragma unroll
+                for (int pass = 0; pass < WN / St::kCols; ++pass) {
+                    const int col = col0 + pass * St::kCols;
+#pragma unroll
+                    for (int x0 = 0; x0 < kXs; x0 += kBatch) {
+                        u32x4 held[2][kBatch][TJ];
+#pragma unroll
+                        for (int a = 0; a < 2; ++a) {
+                            const __amdgpu_buffer_rsrc_t rs =
+                                __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(in + a * prm.n_cols), 0, (int)kOutOfRange, kRsrcFlags);
+#pragma unroll
+                            for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+                                for (int y = 0; y < TJ; ++y) {
+                                    const int row = wave_m0 + y * MB + lb, c = col + (x0 + x) * MB + hq * 4;
+                                    const uint32_t at = row < q_valid && c < col_end ? (uint32_t)(((int64_t)row * prm.ldc + c) * 4) : kOutOfRange;
+                                    held[a][x][y] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 0);
+                                }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+                            for (int y = 0; y < TJ; ++y) {
+                                alignas(8) Out dg[4], du[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float dm = acc[pass * kXs + x0 + x][y][i];
+                                    const ActTerms t = gate_terms<true>(__uint_as_float(held[0][x][y][i]), act);
+                                    dg[i] = (Out)(dm * __uint_as_float(held[1][x][y][i]) * t.slope);
+                                    du[i] = (Out)(dm * t.value);
+                                }
+                                *at4(0, x0 + x, 0, y) = *(const Vec4 *)dg;
+                                *at4(1, x0 + x, 0, y) = *(const Vec4 *)du;
+                            }
+                    }
+                    sync();
+                    store(0, out, col, prm.ldc);
+                    store(1, out + prm.n_cols, col, prm.ldc);
+                    sync();
+                }
+            });
+        } else if constexpr (EPI == kEpiDGated) {
             // acc: dm; aux, C: [rows, 2 n_cols], g and u, dg and du
             const Out *in = (const Out *)prm.aux + aux_off;
             Out *out = (Out *)prm.C + aux_off;
@@ -1546,9 +1595,9 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     const float dm = acc[pass * kXs + x][y][MB == 16 ? i : 4 * g + i];
-                                    const ActTerms t = gate_terms<kNarrow>((float)gate[i], act);
-                                    gate[i] = (Out)(dm * (float)lin[i] * t.slope);
-                                    lin[i] = (Out)(dm * t.value);
+                                    const ActTerms t = gate_terms<false>(gate[i], act);
+                                    gate[i] = dm * lin[i] * t.slope;
+                                    lin[i] = dm * t.value;
                                 }
                                 *at4(0, x, g, y) = *(const Vec4 *)gate;
                                 *at4(1, x, g, y) = *(const Vec4 *)lin;
@@ -1573,16 +1622,16 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
 #pragma unroll
             for (int y = 0; y < TJ; ++y)
                 row_scale[y] = IsInt8<T>::value ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(row_rs, (wave_m0 + y * MB + lb) * 4, 0, 0)) : 1.f;
-            // f(x, g, sums): four columns at a time, for all block rows: the products with scales and biases, of each half
-            auto each = [&](int pass, auto &&f) __attribute__((always_inline)) {
+            // f(x, g, sums): four columns at a time, of `count` blocks from block x0 on and all block rows: the products with scales and biases, of each half
+            auto each = [&](int x0, auto count, auto &&f) __attribute__((always_inline)) {
 #pragma unroll
-                for (int x = 0; x < kXs; ++x)
+                for (int x = 0; x < decltype(count)::value; ++x)
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
                         float add[H][4], scale[H][4];
 #pragma unroll
                         for (int h = 0; h < H; ++h) {
-                            const int c = col0 + pass * St::kCols + x * kBlockCols + g * 8 + hq * 4 + (h ? prm.n_cols : 0);
+                            const int c = col0 + (x0 + x) * kBlockCols + g * 8 + hq * 4 + (h ? prm.n_cols : 0);
                             alignas(16) Out b[4];
                             if (kNarrow && !fours) {   // (their biases may begin between two dwords)
 #pragma unroll
@@ -1604,7 +1653,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
                             for (int h = 0; h < H; ++h)
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const float v = value(h, pass * kXs + x, g, y, i);
+                                    const float v = value(h, x0 + x, g, y, i);
                                     sum[h][i] = IsInt8<T>::value ? fmaf(v, row_scale[y] * scale[h][i], add[h][i]) : v + add[h][i];
                                 }
                             f(x, g, y, sum);
@@ -1612,18 +1661,24 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
                     }
             };
             if constexpr (EPI == kEpiGated) {
-                if (prm.aux != nullptr) {   // both halves as they are, [rows, 2 n_cols]
-                    Out *pre = (Out *)prm.aux + 2 * aux_off - n0;
+                if (prm.aux != nullptr) {   // both halves as they are, [rows, 2 n_cols] float32
+                    constexpr int kPreCols = St::kPiece / 4, kPreXs = kPreCols / kBlockCols;   // columns, blocks of a pass
+                    static_assert(WN / 2 == St::kCols, "one pass of results");
+                    float *pre = (float *)prm.aux + 2 * aux_off - n0;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        each(0, [&](int x, int g, int y, const float (&sum)[H][4]) {
-                            alignas(16) Out v[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = (Out)sum[h][i];
-                            *at4(0, x, g, y) = *(const Vec4 *)v;
+                    for (int n = 0; n < 2 * (St::kCols / kPreCols); ++n) {
+                        const int h = n & 1, x0 = (n >> 1) * kPreXs, col = col0 + x0 * kBlockCols;
+                        each(x0, std::integral_constant<int, kPreXs>{}, [&](int x, int g, int y, const float (&sum)[H][4]) {
+                            *(f32x4 *)(area + (y * MB + lb) * St::kRow + (x * kBlockCols + g * 8 + hq * 4) * 4) = f32x4{sum[h][0], sum[h][1], sum[h][2], sum[h][3]};
                         });
                         sync();
-                        store(0, pre + (h ? prm.n_cols : 0), col0, 2 * prm.ldc);
+                        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(pre + (h ? prm.n_cols : 0), 0, (int)kOutOfRange, kRsrcFlags);
+#pragma unroll
+                        for (int i = 0; i < kSteps; ++i) {
+                            const int row = wave_m0 + i * kRows + sr, c = col + sc * 4;
+                            const uint32_t at = row < q_valid && c < col_end ? (uint32_t)(((int64_t)row * (2 * prm.ldc) + c) * 4) : kOutOfRange;
+                            __builtin_amdgcn_raw_buffer_store_b128(*piece(0, i), rs, (int)at, 0, 0);
+                        }
                         sync();
                     }
                 }
@@ -1632,7 +1687,7 @@ __global__ __launch_bounds__(threads_of(BN) + 64 * extra_waves(LOADERS), waves_p
             by_gate_activation<IsInt8<T>::value>(prm.activation, [&](auto act) {
 #pragma unroll
                 for (int pass = 0; pass < WN / H / St::kCols; ++pass) {
-                    each(pass, [&](int x, int g, int y, const float (&sum)[H][4]) {
+                    each(pass * kXs, std::integral_constant<int, kXs>{}, [&](int x, int g, int y, const float (&sum)[H][4]) {
                         alignas(16) Out v[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {

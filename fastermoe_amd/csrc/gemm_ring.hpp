@@ -405,6 +405,8 @@ template <int CHUNKS> struct RingStage {
     __device__ __forceinline__ unsigned char *mine(int x) const {
         return stg + lb * (CHUNKS * 16) + (((2 * x + (hq >> 1)) ^ (lb & (CHUNKS - 1))) << 4) + (hq & 1) * 8;
     }
+    // (rows of 64 floats) the same four
+    __device__ __forceinline__ f32x4 *mine_f32(int x) const { return (f32x4 *)(stg + lb * (CHUNKS * 16) + (((4 * x + hq) ^ (lb & (CHUNKS - 1))) << 4)); }
     // the piece that this lane has to do with on the way from or to memory: row row(i), piece io_c
     __device__ __forceinline__ int row(int i) const { return i * kRowsAt + io_r; }
     __device__ __forceinline__ u32x4 *piece(int i) const {
@@ -418,7 +420,7 @@ template <int CHUNKS> struct RingStage {
 };
 
 // The forward product of gated experts.  acc[x][y] with x < 4: the gate's columns 64 wn + 16 x + 4 hq + i of the tile's 128, x + 4 the linear half's.
-// aux (AUX): [rows, 2 n_cols], both halves as they are; C [rows, n_cols]: act(gate) * linear, of the sums before they are rounded.
+// aux (AUX): [rows, 2 n_cols] float32, both halves as they are; C [rows, n_cols]: act(gate) * linear, of the sums before they are rounded.
 // 32768 rows, 8 experts of 4096 -> 2 x 14336 in bfloat16, aux written: 5.4 ms, 1420 TFLOP/s, as the plain product of as many columns (5.4) without what comes after it.
 template <typename T, bool AUX, int NY>
 __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
@@ -431,27 +433,25 @@ __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const
     const int row0 = 64 * wm + 16 * y0;
     if constexpr (AUX) {
         const RingStage<16> st(stg, el);
-        const int col = 64 * wn + (st.io_c & 7) * 8;
-        const uint32_t at = col < tl.p_valid ? (uint32_t)((col + (st.io_c >> 3) * prm.n_cols) * 2) : kOutOfRange;
+        const int col = 64 * wn + st.io_c * 4;
+        const uint32_t at = col < tl.p_valid ? (uint32_t)(col * 4) : kOutOfRange;
         const __amdgpu_buffer_rsrc_t rs =
-            __builtin_amdgcn_make_buffer_rsrc((T *)prm.aux + 2 * tl.c_off - tl.n0, 0, (int)kOutOfRange, kRsrcFlags);
+            __builtin_amdgcn_make_buffer_rsrc((float *)prm.aux + 2 * tl.c_off - tl.n0, 0, (int)kOutOfRange, kRsrcFlags);
 #pragma unroll
         for (int y = 0; y < NY; ++y) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                alignas(8) T v[4];
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (T)acc[x][y][i];
-                *(u32x2 *)st.mine(x) = *(const u32x2 *)v;
-            }
-            st.sync();
+                for (int x = 0; x < 4; ++x) *st.mine_f32(x) = acc[x + 4 * h][y];
+                st.sync();
 #pragma unroll
-            for (int i = 0; i < st.kStores; ++i) {
-                const int row = row0 + 16 * y + st.row(i);
-                const uint32_t off = row < tl.q_valid ? (uint32_t)(row * (int)(prm.ldc * 4)) + at : kOutOfRange;
-                __builtin_amdgcn_raw_buffer_store_b128(*st.piece(i), rs, (int)(off | (at & kOutOfRange)), 0, 0);
+                for (int i = 0; i < st.kStores; ++i) {
+                    const int row = row0 + 16 * y + st.row(i);
+                    const uint32_t off = row < tl.q_valid ? (uint32_t)(row * (int)(prm.ldc * 8)) + (uint32_t)(h * prm.n_cols * 4) + at : kOutOfRange;
+                    __builtin_amdgcn_raw_buffer_store_b128(*st.piece(i), rs, (int)(off | (at & kOutOfRange)), 0, 0);
+                }
+                st.sync();
             }
-            st.sync();
         }
     }
     const RingStage<8> st(stg, el);
@@ -481,10 +481,10 @@ __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const
 #endif
 }
 
-// The data gradient of a gated experts' second product, turned into those of the first one's two halves: with dm the sums and g, u from aux [rows, 2 n_cols]
-// C [rows, 2 n_cols] = [dm u act'(g), dm act(g)].  ldc: of both.  Sixteen rows of 64 columns at a time, both halves side by side in the wave's LDS, where the
-// results take their places; the next g and u are on their way meanwhile, asked for inside the branch for the activation: ahead of it their loads stood between the slab
-// loop's on every path, and the loop waited for those too (8 experts of 4096 x 14336, 32768 rows: 3.39 ms; 3.08 now, 1250 TFLOP/s, of which 0.6 are 5.6 GB of g, u, dg, du).
+// The data gradient of a gated experts' second product, turned into those of the first one's two halves: with dm the sums and g, u from aux [rows, 2 n_cols], float32,
+// C [rows, 2 n_cols] = [dm u act'(g), dm act(g)].  ldc: of both.  g and u come straight to the lanes that hold their columns' sums, sixteen rows of 32 columns (whole lines) at a time with
+// the next on their way; dg and du leave through the wave's LDS, 64 columns of both halves side by side.  The first loads are asked for inside the branch for the activation: ahead of it
+// they stood between the slab loop's on every path, and the loop waited for those too (8 experts of 4096 x 14336, 32768 rows: 3.39 ms, 3.08 so, with g and u in 16 bits).
 template <typename T, int NY>
 __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                      int lane, int wm, int wn, int y0) {
@@ -494,60 +494,51 @@ __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, cons
     int el = lane;
     asm volatile("" : "+v"(el));
     const RingStage<8> sg(stg, el), su(stg + 2048, el);
-    const int row0 = 64 * wm + 16 * y0, col = 128 * wn + sg.io_c * 8;
+    const int row0 = 64 * wm + 16 * y0, col = 128 * wn;
     const uint32_t half = (uint32_t)(prm.n_cols * 2);
-    const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc((T *)prm.aux + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
+    const __amdgpu_buffer_rsrc_t in = __builtin_amdgcn_make_buffer_rsrc((float *)prm.aux + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
     const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc((T *)prm.C + tl.c_off, 0, (int)kOutOfRange, kRsrcFlags);
-    // piece i of step n: rows 16 (n / 2) on, columns 64 (n % 2) on (past the end outside the tile)
-    auto offset = [&](int n, int i) -> uint32_t {
-        const int row = row0 + 16 * (n >> 1) + sg.row(i), c = col + 64 * (n & 1);
-        return row < tl.q_valid && c < tl.p_valid ? (uint32_t)(row * (int)(prm.ldc * 2) + c * 2) : kOutOfRange;
-    };
+    // step q: rows 16 (q / 4) on, columns 32 (q % 4) on (past the end outside the tile)
     u32x4 ahead[2][2];
-    auto request = [&](int n) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t at = offset(n, i);
-            ahead[0][i] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)at, 0, 0);
-            ahead[1][i] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)(at + half), 0, 0);
-        }
+    const int first = __builtin_amdgcn_readfirstlane(row0 * (int)(prm.ldc * 4)), sixteen_rows = (int)(prm.ldc * 64);   // bytes
+    const uint32_t base = (uint32_t)(sg.lb * (int)(prm.ldc * 4) + (col + 4 * sg.hq) * 4);
+    auto request = [&](int q, int x) {
+        const int c = 32 * (q & 3) + 16 * x, from = first + (q >> 2) * sixteen_rows + c * 4;
+        const uint32_t at = row0 + 16 * (q >> 2) + sg.lb < tl.q_valid && col + c + 4 * sg.hq < tl.p_valid ? base : kOutOfRange;
+        ahead[0][x] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)at, from, 0);
+        ahead[1][x] = __builtin_amdgcn_raw_buffer_load_b128(in, (int)at, from + (int)(2 * half), 0);
     };
     by_gate_activation<false>(prm.activation, [&](auto act) {
-        // (asked for in here: ahead of the branches it would stay pending on a way past all of them, which the compiler believes in, and be waited for,
-        // with the slab loads, in the slab loop: 3393 us instead of 3130 for the large layer's data gradient)
-        request(0);
+        request(0, 0);
+        request(0, 1);
 #pragma unroll
-        for (int n = 0; n < 2 * NY; ++n) {
+        for (int q = 0; q < 4 * NY; ++q) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                *sg.piece(i) = ahead[0][i];
-                *su.piece(i) = ahead[1][i];
-            }
-            if (n + 1 < 2 * NY) request(n + 1);
-            sg.sync();
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < 2; ++x) {
+                const u32x4 gate = ahead[0][x], lin = ahead[1][x];
+                if (q + 1 < 4 * NY) request(q + 1, x);
                 alignas(8) T g[4], u[4];
-                *(u32x2 *)g = *(const u32x2 *)sg.mine(x);
-                *(u32x2 *)u = *(const u32x2 *)su.mine(x);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float dm = acc[4 * (n & 1) + x][n >> 1][i];
-                    const ActTerms t = gate_terms<true>((float)g[i], act);
-                    g[i] = (T)(dm * (float)u[i] * t.slope);
+                    const float dm = acc[2 * (q & 3) + x][q >> 2][i];
+                    const ActTerms t = gate_terms<true>(__uint_as_float(gate[i]), act);
+                    g[i] = (T)(dm * __uint_as_float(lin[i]) * t.slope);
                     u[i] = (T)(dm * t.value);
                 }
-                *(u32x2 *)sg.mine(x) = *(const u32x2 *)g;
-                *(u32x2 *)su.mine(x) = *(const u32x2 *)u;
+                *(u32x2 *)sg.mine(2 * (q & 1) + x) = *(const u32x2 *)g;
+                *(u32x2 *)su.mine(2 * (q & 1) + x) = *(const u32x2 *)u;
             }
-            sg.sync();
+            if (q & 1) {
+                sg.sync();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t at = offset(n, i);
-                __builtin_amdgcn_raw_buffer_store_b128(*sg.piece(i), out, (int)at, 0, 0);
-                __builtin_amdgcn_raw_buffer_store_b128(*su.piece(i), out, (int)(at + half), 0, 0);
+                for (int i = 0; i < 2; ++i) {
+                    const int row = row0 + 16 * (q >> 2) + sg.row(i), c = col + 64 * ((q >> 1) & 1) + sg.io_c * 8;
+                    const uint32_t at = row < tl.q_valid && c < tl.p_valid ? (uint32_t)(row * (int)(prm.ldc * 2) + c * 2) : kOutOfRange;
+                    __builtin_amdgcn_raw_buffer_store_b128(*sg.piece(i), out, (int)at, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(*su.piece(i), out, (int)(at + half), 0, 0);
+                }
+                sg.sync();
             }
-            sg.sync();
             __builtin_amdgcn_sched_barrier(0);
         }
     });

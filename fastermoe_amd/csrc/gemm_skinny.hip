@@ -318,7 +318,8 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     const f32x4 sum[2] = {summed(n, y), HALVES ? summed(n + NH, y) : f32x4{}};
                     if (row >= rows) continue;
                     const float s = ROUND ? RowScale(most_of[row]).shown() : kInt8 ? prm.x_scale[first + row] : 1.f;
-                    alignas(16) Out pre[H][4], res[4];
+                    alignas(16) Out res[4];
+                    f32x4 pre[H];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float v[H];
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                         for (int h = 0; h < H; ++h) {
                             if constexpr (kInt8) v[h] = fmaf((float)(int)__float_as_uint(sum[h][i]), s * scale[h][i], add[h][i]);
                             else v[h] = sum[h][i] + add[h][i];
-                            pre[h][i] = (Out)v[h];
+                            pre[h][i] = v[h];
                         }
                         float r = gate_act<sizeof(Out) == 2>(v[0], prm.activation);
                         if constexpr (HALVES) r *= v[1];
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(kSkThreads, COL_BLOCKS == 4 ? 3 : 4) void grouped_g
                     if (HALVES && prm.aux != nullptr) {
 #pragma unroll
                         for (int h = 0; h < H; ++h)
-                            *(OutVec4 *)((Out *)prm.aux + 2 * at - col + h * prm.n_cols) = *(const OutVec4 *)pre[h];
+                            *(f32x4 *)((float *)prm.aux + 2 * at - col + h * prm.n_cols) = pre[h];
                     }
                     *(OutVec4 *)((Out *)prm.y + at) = *(const OutVec4 *)res;
                 }

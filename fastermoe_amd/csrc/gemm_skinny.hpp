@@ -17,7 +17,7 @@ struct SkinnyParams {
     int32_t weights_cached;       // not 0: the weights through the caches, see caches_few_row_weights() in grouped_gemm.hip
     int32_t order_off, tiles_n, extra_groups;   // set by the launch: the table's list of experts (or its map of row tiles), see launch()
 };
-// Gated products and such in 8-bit integers (w: [E, 2 n_cols or n_cols, k], a gate's rows first; aux [rows, 2 n_cols]).  A type of its own: plain
+// Gated products and such in 8-bit integers (w: [E, 2 n_cols or n_cols, k], a gate's rows first; aux [rows, 2 n_cols] float32).  A type of its own: plain
 // products of a few rows feel how long a launch's arguments are (1 row, 2048 experts of 512 x 512, in a graph: 3.72 us; with these between theirs 3.82).
 struct SkinnyMoreParams : SkinnyParams {
     int64_t ldw, ldx, w_expert_stride;         // 8-bit integers: row strides in pairs of them (others are dense)

@@ -26,6 +26,28 @@ namespace fmoe {
 namespace {
 using namespace gemm;
 
+// the first n floats (4 or more: four) of four from or to wherever they begin
+__device__ __forceinline__ f32x4 load_floats(const float *p, int n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < n) v[j] = p[j];
+    }
+    return v;
+}
+__device__ __forceinline__ void store_floats(float *p, const f32x4 &v, int n) {
+    if (n >= 4) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < n) p[j] = v[j];
+    }
+}
+
 constexpr int kUaThreads = 256, kUaBN = 128, kUaBK = 64;
 
 // the float32 sums of a part of the contraction instead of an epilogue: see launch_parts
@@ -286,7 +308,7 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
         return;
     }
     if constexpr (EPI == kEpiGated || EPI == kEpiDGated) {
-        // Gated products: sixteen rows at a time, 64 columns of C (dg and du, from g and u), or 32 of each half, through 2 KiB of LDS per wave and matrix
+        // Gated products: sixteen rows at a time, 64 columns of C (dg and du), or 32 of each half, through 2 KiB of LDS per wave and matrix
         constexpr int kWaveCols = kHalves ? 32 : 64, kPieces = kWaveCols / 8, kSteps = kPieces / 4, kRows = 64 / kPieces;
         unsigned char *area = smem + wave * 4096;
         const int io_r = lane / kPieces, io_c = lane % kPieces, wave_col = kWaveCols * wn;
@@ -313,60 +335,68 @@ __global__ __launch_bounds__(kUaThreads) void grouped_gemm_unaligned_kernel(cons
                     const int col = wave_col + 16 * (x & 1) + 4 * hq + i;
                     bias_of[x][i] = bias != nullptr && col < p_valid ? (float)bias[col + (x < 2 ? 0 : prm.n_cols)] : 0.f;
                 }
-            T *pre = prm.aux ? (T *)prm.aux + 2 * c_off - n0 : nullptr;
+            float *pre = prm.aux ? (float *)prm.aux + 2 * c_off - n0 : nullptr;
 #pragma unroll
             for (int y = 0; y < TJ; ++y) {
                 if (16 * row_block(y) >= q_valid) break;
+                if (pre != nullptr) {   // float32, a half at a time: rows of 32 columns
 #pragma unroll
-                for (int kind = 0; kind < 3; ++kind) {   // the gate's half, the linear one, the result
-                    if (kind < 2 && pre == nullptr) continue;
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        alignas(8) T v[4];
+                        for (int x = 0; x < 2; ++x) {
+                            f32x4 v = acc[x + 2 * h][y];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float g = acc[x][y][i] + bias_of[x][i], u = acc[x + 2][y][i] + bias_of[x + 2][i];
-                            v[i] = (T)(kind == 0 ? g : kind == 1 ? u : gate_act<true>(g, prm.activation) * u);
+                            for (int i = 0; i < 4; ++i) v[i] += bias_of[x + 2 * h][i];
+                            *(f32x4 *)(area + lb * 128 + (((4 * x + hq) ^ (lb & 7)) << 4)) = v;
                         }
-                        *at4(0, x) = *(const u32x2 *)v;
+                        wave_sync();
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int r = i * 8 + (lane >> 3), row = 16 * row_block(y) + r, c = wave_col + (lane & 7) * 4;
+                            const f32x4 v = *(const f32x4 *)(area + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                            if (row < q_valid && c < p_valid) store_floats(pre + (int64_t)row * (2 * prm.ldc) + c + (h ? prm.n_cols : 0), v, p_valid - c);
+                        }
+                        wave_sync();
                     }
-                    wave_sync();
-                    if (kind == 2) store(0, (T *)prm.C + c_off, prm.ldc, y);
-                    else store(0, pre + (kind ? prm.n_cols : 0), 2 * prm.ldc, y);
-                    wave_sync();
                 }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    alignas(8) T v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float g = acc[x][y][i] + bias_of[x][i], u = acc[x + 2][y][i] + bias_of[x + 2][i];
+                        v[i] = (T)(gate_act<true>(g, prm.activation) * u);
+                    }
+                    *at4(0, x) = *(const u32x2 *)v;
+                }
+                wave_sync();
+                store(0, (T *)prm.C + c_off, prm.ldc, y);
+                wave_sync();
             }
         } else {
-            const T *in = (const T *)prm.aux + c_off;
+            // g and u (float32) straight to the lanes that hold their columns' sums
+            const float *in = (const float *)prm.aux + c_off;
             T *out = (T *)prm.C + c_off;
-            auto load = [&](u32x4 (&v)[2][kSteps], int y) {
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i)
-                        v[a][i] = row_of(y, i) < q_valid && left > 0 ? load_some(in + (int64_t)row_of(y, i) * prm.ldc + wave_col + io_c * 8 + a * prm.n_cols, left)
-                                                                    : u32x4{0u, 0u, 0u, 0u};
-            };
 #pragma unroll
             for (int y = 0; y < TJ; ++y) {
                 if (16 * row_block(y) >= q_valid) break;
-                u32x4 held[2][kSteps];
-                load(held, y);
+                const int row = 16 * row_block(y) + lb;
+                f32x4 held[2][TI];
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) *piece(a, i) = held[a][i];
-                wave_sync();
+                    for (int x = 0; x < TI; ++x) {
+                        const int c = wave_col + 16 * x + 4 * hq;
+                        held[a][x] = row < q_valid && c < p_valid ? load_floats(in + (int64_t)row * prm.ldc + c + a * prm.n_cols, p_valid - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+                    }
 #pragma unroll
                 for (int x = 0; x < TI; ++x) {
                     alignas(8) T g[4], u[4];
-                    *(u32x2 *)g = *at4(0, x);
-                    *(u32x2 *)u = *at4(1, x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const ActTerms terms = gate_terms<true>((float)g[i], prm.activation);
+                        const ActTerms terms = gate_terms<true>(held[0][x][i], prm.activation);
                         const float dm = acc[x][y][i];
-                        g[i] = (T)(dm * (float)u[i] * terms.slope);
+                        g[i] = (T)(dm * held[1][x][i] * terms.slope);
                         u[i] = (T)(dm * terms.value);
                     }
                     *at4(0, x) = *(const u32x2 *)g;

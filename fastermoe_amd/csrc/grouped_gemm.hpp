@@ -11,8 +11,8 @@ enum Epilogue {
     kEpiBiasAct = 1,  // pre = acc + bias[col]; aux = pre (if aux); C = act(pre)
     kEpiDAct = 2,     // C = acc * act'(aux)          (aux = saved pre-activation)
     // over a device table only:
-    kEpiGated = 3,    // [g u] = acc + bias; aux = [g u] (if aux); C = act(g) u
-    kEpiDGated = 4,   // C = [acc u act'(g), acc act(g)]  (aux = saved [g u])
+    kEpiGated = 3,    // [g u] = acc + bias; aux = [g u] in float32 (if aux); C = act(g) u
+    kEpiDGated = 4,   // C = [acc u act'(g), acc act(g)]  (aux = saved [g u], float32)
     kEpiInt8 = 5,     // C = act(row scale * column scale * acc + bias)
     kEpiInt8Gated = 6,  // [g u] = that before act; C = act(g) u
 };
@@ -154,7 +154,7 @@ struct GatedArgs {
     const void *in;      // forward: x [rows, d]; dgrad: the gradient of the second product's results, [rows, d]
     const void *w;       // forward: [E, 2 h, d]; dgrad: [E, d, h]
     const void *bias;    // forward: [E, 2 h] or null
-    void *pre;           // [rows, 2 h]; forward: written (null: not kept), dgrad: read
+    void *pre;           // [rows, 2 h] float32; forward: written (null: not kept), dgrad: read
     void *out;           // forward: [rows, h]; dgrad: [rows, 2 h]
     void *tail;
     int64_t d, h, n_expert, rows_cap;

@@ -924,14 +924,14 @@ def _gated_float32(dtype, *tensors):
 
 def gated_mlp_forward(x, w1, b1, w2, b2, activation, table, keep=True):
     """``(y, pre, mid)`` of gated experts: ``pre = x @ w1_e^T + b1_e`` (a gate's half and a linear one), ``mid = act(gate) * linear``,
-    ``y = mid @ w2_e^T + b2_e``.  ``table``: the rows' segments, :func:`segment_table` for as many rows as ``x`` has.
+    ``y = mid @ w2_e^T + b2_e``; ``pre`` is float32.  ``table``: the rows' segments, :func:`segment_table` for as many rows as ``x`` has.
     ``keep=False``: ``pre`` and ``mid`` are ``None``.  Rows of ``y`` behind the experts' are zeros."""
     dt, e, n, d, h = _gated_args(x, w1, b1, w2, b2)
     activation = _gate_activation(activation)
     _exact_table(table, e, n, x.device)
     x, w1, b1, w2, b2 = _gated_float32(x.dtype, x, w1, b1, w2, b2)
     y = torch.empty(n, d, dtype=x.dtype, device=x.device)
-    pre = torch.empty(n, 2 * h, dtype=x.dtype, device=x.device) if keep else None
+    pre = torch.empty(n, 2 * h, dtype=torch.float32, device=x.device) if keep else None
     mid = torch.empty(n, h, dtype=x.dtype, device=x.device)
     lib = _lib.load()
     with _on(x.device):
@@ -946,8 +946,8 @@ def gated_mlp_backward(grad_y, x, w1, w2, pre, mid, activation, table, want_x=Tr
     """``(grad_x, grad_w1, grad_b1, grad_w2, grad_b2)`` from what :func:`gated_mlp_forward` left; ``None`` where not wanted."""
     dt, e, n, d, h = _gated_args(x, w1, None, w2, None)
     activation = _gate_activation(activation)
-    for name, t, shape in (("grad_y", grad_y, (n, d)), ("pre", pre, (n, 2 * h)), ("mid", mid, (n, h))):
-        _near(name, _dev(name, t, x.dtype), x.device)
+    for name, t, shape, dtype in (("grad_y", grad_y, (n, d), x.dtype), ("pre", pre, (n, 2 * h), torch.float32), ("mid", mid, (n, h), x.dtype)):
+        _near(name, _dev(name, t, dtype), x.device)
         if tuple(t.shape) != shape:
             raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
     _exact_table(table, e, n, x.device)

@@ -807,8 +807,9 @@ def gated_mlp(inp, expert_count, w1, b1, w2, b2, activation, table=None):
     [E, d_model, d_hidden]``, ``b1``, ``b2`` or ``None``; ``activation``: ``torch.nn.SiLU()``, exact ``GELU()``, ``ReLU()``, ``None`` or an
     ``ACT_*`` code.  ``expert_count`` (int64 ``[E]``): rows of each expert, on the device (nothing is read back) or the CPU; or ``table``,
     their :func:`fmoe_native.segment_table` for as many rows, which a routing call leaves.  Rows behind the counted ones come out as
-    zeros, and so do their gradients.  Differentiable once, with respect to ``inp``, the weights and the biases; the gradients are made from ``g``, ``u``
-    and ``act(g) * u`` as ``inp``'s type holds them."""
+    zeros, and so do their gradients.  Differentiable once, with respect to ``inp``, the weights and the biases; the gradients are made from ``g`` and ``u`` in
+    float32 and ``act(g) * u`` as ``inp``'s type holds it, which the second product reads too: in float16 it is infinite above 65504, where 32 bits would not be,
+    and so are the gradients of ``g`` and ``u``, rounded to ``inp``'s type for the products that read them."""
     code = _gate_activation_code(activation)
     module = _lib.load_layer_call()
     if module is not None and nothing_watches(*(t for t in (inp, w1, b1, w2, b2, table) if t is not None)):

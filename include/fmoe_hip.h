@@ -741,9 +741,9 @@ int fmoe_gated_mlp_supported(int64_t d_model, int64_t d_hidden, int dtype);
 /* Per expert, over its rows:  [g u] = pre = x W1^T + b1,  mid = act(g) * u,
  * y = mid W2^T + b2.  w1 [E, 2 d_hidden, d_model] (the gate's rows, then the
  * linear half's), b1 [E, 2 d_hidden] or NULL, w2 [E, d_model, d_hidden], b2
- * [E, d_model] or NULL; pre [rows, 2 d_hidden] (NULL: not kept), mid
- * [rows, d_hidden] and y [rows, d_model]; behind the rows that the experts have
- * y is zero, pre and mid are left as they are.
+ * [E, d_model] or NULL; pre [rows, 2 d_hidden] in float32 whatever the type (NULL:
+ * not kept), mid [rows, d_hidden] and y [rows, d_model]; behind the rows that the
+ * experts have y is zero, pre and mid are left as they are.
  * The rows' segments come from segment_table (of fmoe_segment_table_build for
  * `rows` rows).  FMOE_F32 (tensors on 16 bytes) / FMOE_BF16 / FMOE_F16, sizes of
  * fmoe_gated_mlp_supported; any FMOE_ACT_*.
