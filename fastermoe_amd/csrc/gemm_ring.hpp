@@ -421,7 +421,8 @@ template <int CHUNKS> struct RingStage {
 
 // The forward product of gated experts.  acc[x][y] with x < 4: the gate's columns 64 wn + 16 x + 4 hq + i of the tile's 128, x + 4 the linear half's.
 // aux (AUX): [rows, 2 n_cols] float32, both halves as they are; C [rows, n_cols]: act(gate) * linear, of the sums before they are rounded.
-// 32768 rows, 8 experts of 4096 -> 2 x 14336 in bfloat16, aux written: 5.4 ms, 1420 TFLOP/s, as the plain product of as many columns (5.4) without what comes after it.
+// 32768 rows, 8 experts of 4096 -> 2 x 14336 in bfloat16, aux written: 5.7 ms, 1350 TFLOP/s; the plain product of as many columns takes 5.4 and writes 1.9 GB
+// less, without what comes after it.
 template <typename T, bool AUX, int NY>
 __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                     int lane, int wm, int wn, int y0) {
@@ -484,7 +485,8 @@ __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const
 // The data gradient of a gated experts' second product, turned into those of the first one's two halves: with dm the sums and g, u from aux [rows, 2 n_cols], float32,
 // C [rows, 2 n_cols] = [dm u act'(g), dm act(g)].  ldc: of both.  g and u come straight to the lanes that hold their columns' sums, sixteen rows of 32 columns (whole lines) at a time with
 // the next on their way; dg and du leave through the wave's LDS, 64 columns of both halves side by side.  The first loads are asked for inside the branch for the activation: ahead of it
-// they stood between the slab loop's on every path, and the loop waited for those too (8 experts of 4096 x 14336, 32768 rows: 3.39 ms, 3.08 so, with g and u in 16 bits).
+// they stood between the slab loop's on every path, and the loop waited for those too (8 experts of 4096 x 14336, 32768 rows: 3.39 ms, 3.08 so, with g and u
+// in 16 bits; 3.5 with theirs, 1100 TFLOP/s, of which 1.0 are 7.5 GB of g, u, dg, du).
 template <typename T, int NY>
 __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                      int lane, int wm, int wn, int y0) {

@@ -15,7 +15,7 @@
 // of 2047 x 4093: 317 / 324 (within 1 % on average); weight gradients there 302 / 299, 8 of 1023 x 2047: 83 / 79, 1554 rows, 12 of 500 x 2604: 27.7 / 26.5.
 // Bound by the latency of those
 // loads up to a few hundred rows per expert (1.2 us a slab) and by their way through registers above (600 TFLOP/s there).  Where few tiles have long contractions, a gated block's products share them between workgroups (launch_parts; see unaligned_parts() in
-// grouped_gemm.hip).  The epilogues of gated products are those of gemm_kernel.hpp: 1554 rows, 12 experts of 500 -> 2 x 1302 in float16, 25 us forward and 24 for the
+// grouped_gemm.hip).  The epilogues of gated products are those of gemm_kernel.hpp: 1554 rows, 12 experts of 500 -> 2 x 1302 in float16, 26 us forward and 22 for the
 // gradient.  Measured against the element-wise kernel it replaced: see the dispatch in grouped_gemm.hip.
 #include "gemm_kernel.hpp"
 #include "unaligned_loads.hpp"
