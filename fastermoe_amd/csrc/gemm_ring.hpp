@@ -486,7 +486,7 @@ __device__ __forceinline__ void ring_epilogue_gated(const RingParams &prm, const
 // C [rows, 2 n_cols] = [dm u act'(g), dm act(g)].  ldc: of both.  g and u come straight to the lanes that hold their columns' sums, sixteen rows of 32 columns (whole lines) at a time with
 // the next on their way; dg and du leave through the wave's LDS, 64 columns of both halves side by side.  The first loads are asked for inside the branch for the activation: ahead of it
 // they stood between the slab loop's on every path, and the loop waited for those too (8 experts of 4096 x 14336, 32768 rows: 3.39 ms, 3.08 so, with g and u
-// in 16 bits; 3.5 with theirs, 1100 TFLOP/s, of which 1.0 are 7.5 GB of g, u, dg, du).
+// in 16 bits; 3.5 with theirs, 1100 TFLOP/s, of which 0.9 are 5.6 GB of g, u, dg, du).
 template <typename T, int NY>
 __device__ __forceinline__ void ring_epilogue_dgated(const RingParams &prm, const RingTile<T> &tl, const f32x4 (&acc)[8][NY], unsigned char *stg,
                                                      int lane, int wm, int wn, int y0) {

@@ -53,9 +53,10 @@ def test_the_gradients_of_the_halves_are_rounded_once(dtype, act, rows, d, h, ex
 
 
 @pytest.mark.parametrize("rows", [3, 300])
-@pytest.mark.parametrize("d,h", [(16384, 32768), (16, (1 << 20) + 8)])
+@pytest.mark.parametrize("d,h", [(16384, 32768), (16, (1 << 20) + 8), (16, 1 << 20)])
 def test_weights_and_rows_past_31_bits(rows, d, h):
-    """An expert's W1 of 2 GiB, and rows of g and u of 4 MiB, on the 16-byte grid: the kernels for sizes off it take them."""
+    """An expert's W1 of 2 GiB, and more than 2^21 columns of g and u, on the 16-byte grid: the kernels for sizes off it take them.  With 2^21 the others do: a
+    tile's g and u just within 2 GiB."""
     assert fmoe_native.gated_mlp_supported(torch.bfloat16, d, h)
     _check(rows, d, h, 1, torch.bfloat16, "silu", True, "even")
     torch.cuda.empty_cache()
