@@ -209,3 +209,11 @@ def test_sizes_of_8_bit_products(dt, d, out, gated, taken):
     assert lib.fmoe_linear_int8_supported(d, out, gated, dt) == taken
     whole = -(-d // 16) * 16
     assert _linear(x=None, dt=dt, d=d, ldx=whole, ldw=whole, wes=whole, out=out, gated=gated) == (EINVAL if taken else ELIMIT)
+
+
+@pytest.mark.parametrize("call", [_gated_forward, _gated_backward])
+@pytest.mark.parametrize("dt", [_lib.BF16, _lib.F16])
+def test_pre_holds_float32_whatever_the_type(call, dt):
+    """An address that 16-bit elements could have and float32 cannot."""
+    assert call(pre=18, dt=dt) == EINVAL
+    assert b"float32" in lib.fmoe_last_error()
