@@ -180,22 +180,20 @@ class _GatedExpert(_Expert):
         return self.h4toh((x * linear).contiguous(), fwd_expert_count)
 
     def routed_forward(self, inp, pos_buf, slot_to_row, counts_dev, top_k, table=None):
-        if not self._device_tables_apply(inp):
+        code = self._one_call(inp)
+        if code is None or os.environ.get("FMOE_DEVICE_TABLES", "1") == "0":
             return None
         self._checkpoints(inp)
         if table is None:
             table = fmoe_native.segment_table(counts_dev, pos_buf.numel())
         return MOERoutedGatedMLP.apply(inp, self.htoh4.weight, self.htoh4.bias, self.h4toh.weight, self.h4toh.bias, pos_buf, slot_to_row, table,
-                                       top_k, self._one_call(inp), self._saves(inp))
+                                       top_k, code, self._saves(inp))
 
     def routed_layer(self, inp, gate_w, gate_b, score, routing, top_k):
         return None
 
     def unchunked_is_faster(self, inp, n_slots):
         return True   # (the pipeline has no gated experts)
-
-    def _device_tables_apply(self, inp):
-        return self._one_call(inp) is not None and os.environ.get("FMOE_DEVICE_TABLES", "1") != "0"
 
 
 class _Int8Expert(nn.Module):
